@@ -48,6 +48,7 @@ extern "C" {
 #define SNAPMIND_DTYPE_F32 0
 #define SNAPMIND_DTYPE_BF16 1
 #define SNAPMIND_DTYPE_F16 2
+#define SNAPMIND_DTYPE_E4M3 3 /* pools of the entry points that say so; rows with a power-of-two scale */
 
 /* device error word bits */
 #define SNAPMIND_DEVERR_BLOCK_ID 1      /* physical block id outside [0, num_blocks) */
@@ -504,6 +505,95 @@ SNAPMIND_API int snapmind_paged_gqa_decode_noalloc(const void *q, int64_t q_stri
                                       int32_t head_dim, int32_t block_size, int32_t num_blocks,
                                       int32_t max_seq_len, int32_t split_tokens, int32_t flags,
                                       int32_t *err_word, void *stream);
+
+/*
+ * snapmind_kv_reserve with its own number of new tokens for every sequence:
+ * n_new is a device array of `batch` counts (0 leaves a sequence as it is).
+ * A negative count sets SNAPMIND_DEVERR_TABLE and nothing changes.
+ */
+SNAPMIND_API int snapmind_kv_reserve_each(int32_t *block_tables, int64_t table_stride_seq, int32_t table_width,
+                             int32_t *seq_lens, const int32_t *n_new, int32_t batch, int32_t block_size,
+                             int32_t *free_stack, int32_t *free_top, int32_t num_blocks,
+                             int32_t *err_word, void *stream);
+
+/*
+ * Append chunks of new K/V rows, of one length for every sequence or ragged,
+ * to a pool of f32 / bf16 / f16 elements or to an 8-bit pool
+ * (pool_dtype SNAPMIND_DTYPE_E4M3).
+ *   cu_new NULL: n_tokens rows per sequence (total_new = batch * n_tokens); row
+ *     (layer, b, head, t) is read at layer*in_stride_layer + b*in_stride_seq +
+ *     head*in_stride_head + t*in_stride_tok and goes to slot
+ *     slot_starts[b] + slot_start0 + t (slot_starts NULL: 0).
+ *   cu_new (device, [batch + 1], ascending): sequence b owns rows
+ *     [cu_new[b], cu_new[b + 1]) of the packed tokens; token i is read at
+ *     layer*in_stride_layer + i*in_stride_tok + head*in_stride_head; its rows end at
+ *     slot slot_starts[b] + slot_start0 (exclusive), so slot_starts = the lengths after
+ *     the reserve stores them last.  Rows outside every sequence are not read.
+ * 8-bit pool: a row x of one token and head is stored as codes c and a byte
+ * e + 127, e the smallest integer in [-100, 120] with max |x| <= 448 * 2^e
+ * (finite values count), c = x * 2^-e rounded to e4m3, nearest even; infinities and NaN
+ * become NaN.  Codes take the pool's place ([layer][block][head][slot][dim], one byte
+ * each); `scales` is [layer][block][head][2][slot] bytes (K, then V), layers
+ * scale_layer_stride apart.  Extends PagedKVCache.store
+ * (snapmind/kv_cache/paged.py:34-54), which has no 8-bit form.
+ */
+SNAPMIND_API int snapmind_kv_append_chunk(void *k_pool, void *v_pool, void *scales, int pool_dtype,
+                             int64_t pool_layer_stride, int64_t scale_layer_stride, const void *k_new,
+                             const void *v_new, int in_dtype, int64_t in_stride_layer, int64_t in_stride_seq,
+                             int64_t in_stride_head, int64_t in_stride_tok, const int32_t *block_tables,
+                             int64_t table_stride_seq, int32_t table_width, const int32_t *slot_starts,
+                             int32_t slot_start0, const int32_t *cu_new, int32_t n_layers, int32_t batch,
+                             int32_t n_tokens, int32_t total_new, int32_t n_heads, int32_t head_dim,
+                             int32_t block_size, int32_t num_blocks, int32_t *err_word, void *stream);
+
+/*
+ * snapmind_kv_gather of an 8-bit pool: the values c * 2^e in out_dtype, in the same
+ * packed layout (per layer, the concatenation over b of (heads, seq_len, dim)).
+ * Values past out_dtype's largest are held to it; a NaN stays one.  When the lengths
+ * need more than out_layer_capacity elements nothing is written and
+ * SNAPMIND_DEVERR_TABLE is set.  batch <= 8192.
+ */
+SNAPMIND_API int snapmind_kv_gather_quant(const void *k_pool, const void *v_pool, const void *scales,
+                             int64_t pool_layer_stride, int64_t scale_layer_stride, void *k_out, void *v_out,
+                             int out_dtype, int64_t out_layer_stride, int64_t out_layer_capacity,
+                             const int32_t *block_tables, int64_t table_stride_seq, int32_t table_width,
+                             const int32_t *seq_lens, int32_t n_layers, int32_t batch, int32_t n_heads,
+                             int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t *err_word,
+                             void *stream);
+
+/*
+ * Attention of chunks of new tokens over the paged cache that already holds them, in
+ * one launch for a ragged batch: sequence b owns query rows [cu_q[b], cu_q[b + 1]) of q
+ * (device, [batch + 1], ascending, at most total_q; an empty range is allowed; rows
+ * outside every range are neither read nor written).  Query i of its n stands at
+ * position seq_lens[b] - n + i and sees the positions p up to its own; with window > 0
+ * only p > its own - window or p < sinks.  A query that sees nothing gives zeros.
+ * cu_q NULL: one query per sequence (a decode step; total_q = batch).
+ * q and out are [token][head][dim] with element strides (dim contiguous) in `dtype`;
+ * query head h reads kv head h / (n_q_heads / n_kv_heads).  pool_dtype is `dtype`, or
+ * SNAPMIND_DTYPE_E4M3 with `scales` as snapmind_kv_append_chunk writes them (of the
+ * same layer as k_pool and v_pool; NULL otherwise).  Softmax statistics and sums are
+ * f32; the tensor-core kernels round a weight 2^(s - max) to the element type (f16 for
+ * e4m3 decodes) before it multiplies V.  head_dim <= 256, batch <= 8192.
+ * A masked position never counts, with one exception: the tensor-core kernels
+ * multiply a weight of 0 with V, so an infinity or NaN in V of a token that some query
+ * of the same sequence sees can reach other queries of that sequence.
+ * `workspace` holds snapmind_paged_gqa_chunk_workspace_bytes(head_dim) bytes on a
+ * 256-byte boundary; its contents need no preparation and are not kept.  Calls
+ * that share one must not overlap on the GPU.
+ * The math of GroupedQueryAttention.forward (snapmind/layers/attention/gqa.py:62-85)
+ * under the masks of snapmind/layers/attention/sdpa.py and
+ * snapmind/models/mistral.py:14-21; sinks have no reference counterpart.
+ */
+SNAPMIND_API int64_t snapmind_paged_gqa_chunk_workspace_bytes(int32_t head_dim);
+SNAPMIND_API int snapmind_paged_gqa_chunk(const void *q, int64_t q_stride_tok, int64_t q_stride_head, int dtype,
+                             const void *k_pool, const void *v_pool, const void *scales, int pool_dtype,
+                             const int32_t *block_tables, int64_t table_stride_seq, int32_t table_width,
+                             const int32_t *seq_lens, const int32_t *cu_q, void *out, int64_t out_stride_tok,
+                             int64_t out_stride_head, float scale, int32_t batch, int32_t total_q,
+                             int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+                             int32_t num_blocks, int32_t window, int32_t sinks, int32_t flags, void *workspace,
+                             int64_t workspace_bytes, int32_t *err_word, void *stream);
 
 #ifdef __cplusplus
 }

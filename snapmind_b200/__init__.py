@@ -11,9 +11,10 @@ from snapmind_b200.attention import PagedGroupedQueryAttention
 from snapmind_b200.kv_cache import PagedKVCache, SlidingWindowKVCache, TieredPagedKVCache
 from snapmind_b200.mla import MLALatentPool, PagedLatentDict
 from snapmind_b200.paged_pool import PagedKVPool
+from snapmind_b200.quant_pool import QuantizedKVPool
 from snapmind_b200.registry import ATTENTION, INDEXER, KV_CACHE, Registry, RegistryError
 
-__all__ = ["KV_CACHE", "ATTENTION", "INDEXER", "Registry", "RegistryError", "PagedKVPool", "MLALatentPool",
+__all__ = ["KV_CACHE", "ATTENTION", "INDEXER", "Registry", "RegistryError", "PagedKVPool", "QuantizedKVPool", "MLALatentPool",
            "PagedLatentDict", "PagedGroupedQueryAttention", "PagedKVCache", "SlidingWindowKVCache",
            "TieredPagedKVCache"]
 __version__ = "0.1.0"

@@ -32,6 +32,8 @@ DEVERR_POSITION = 32
 
 DECODE_FORCE_GENERIC = 1
 
+DTYPE_E4M3 = 3  # an 8-bit pool (rows with a power-of-two scale)
+
 OUT_OF_BLOCKS_MSG = "PagedKVCache: out of blocks"
 
 _DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -132,6 +134,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _i64, _i64, _p, _p, _int, _p, _i64, _i32, _p, _p, _i64, _i64, _f32, _i32, _i32, _i32,
          _i32, _i32, _i32, _i32, _i32, _i32, _p, _p],
     ),
+    "snapmind_kv_reserve_each": (_int, [_p, _i64, _i32, _p, _p, _i32, _i32, _p, _p, _i32, _p, _p]),
+    "snapmind_kv_append_chunk": (
+        _int,
+        [_p, _p, _p, _int, _i64, _i64, _p, _p, _int, _i64, _i64, _i64, _i64, _p, _i64, _i32, _p, _i32, _p, _i32,
+         _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _p],
+    ),
+    "snapmind_kv_gather_quant": (
+        _int,
+        [_p, _p, _p, _i64, _i64, _p, _p, _int, _i64, _i64, _p, _i64, _i32, _p, _i32, _i32, _i32, _i32, _i32, _i32,
+         _p, _p],
+    ),
+    "snapmind_paged_gqa_chunk_workspace_bytes": (_i64, [_i32]),
+    "snapmind_paged_gqa_chunk": (
+        _int,
+        [_p, _i64, _i64, _int, _p, _p, _p, _int, _p, _i64, _i32, _p, _p, _p, _i64, _i64, _f32, _i32, _i32, _i32,
+         _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p],
+    ),
 }
 
 NOALLOC_DECODE_SCRATCH_BYTES = 16 << 20
@@ -205,6 +224,20 @@ def require_cuda(device: torch.device) -> None:
         raise RuntimeError(f"snapmind_b200 runs on CUDA devices only (got {device})")
     if not torch.cuda.is_available():
         raise RuntimeError("snapmind_b200: CUDA is not available")
+
+
+def require_same(what: str, like: torch.Tensor, *tensors: torch.Tensor) -> None:
+    """Raise unless every tensor is on ``like``'s device."""
+    for t in tensors:
+        if t.device != like.device:
+            raise ValueError(f"{what}: a tensor on {t.device}, the pool is on {like.device}")
+
+
+def require_offsets(what: str, cu: torch.Tensor, like: torch.Tensor) -> None:
+    """Raise unless ``cu`` is a contiguous int32 ``[B + 1]`` vector on ``like``'s device."""
+    if cu.dtype != torch.int32 or cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous():
+        raise ValueError(f"{what}: offsets must be a contiguous int32 vector of batch + 1 entries")
+    require_same(what, like, cu)
 
 
 def raise_device_error(word: int, what: str) -> None:

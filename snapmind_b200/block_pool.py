@@ -10,10 +10,14 @@ and size outputs without a device sync.
 """
 from __future__ import annotations
 
+import contextlib
+
 import numpy as np
 import torch
 
 from snapmind_b200 import _lib
+
+_NOTHING = contextlib.nullcontext()
 
 
 class BlockPool:
@@ -35,6 +39,11 @@ class BlockPool:
 
     def _stream(self) -> int:
         return _lib.stream_handle(self.device)
+
+    def _on_device(self):
+        """Context in which the pool's device is the current one (kernels launch on its stream)."""
+        index = self.block_tables.device.index
+        return _NOTHING if torch.cuda.current_device() == index else torch.cuda.device(index)
 
     @property
     def host_lens(self) -> np.ndarray:
@@ -86,6 +95,33 @@ class BlockPool:
         )  # fmt: skip
         _lib.check(status, f"{type(self).__name__}.reserve")
         self._host_lens[:batch] += n_new
+        self._host_free -= need
+
+    def reserve_each(self, n_new) -> None:
+        """Grow sequence b by ``n_new[b]`` tokens (host integers, 0 leaves it as it is;
+        sequences past the list are left alone): the ragged form of ``reserve``, in the
+        same order and all or nothing."""
+        n = np.asarray(n_new, dtype=np.int64).reshape(-1)
+        if len(n) > self.max_seqs or (n < 0).any():
+            raise ValueError("reserve_each: one count >= 0 for each of the pool's sequences at most")
+        bs = self.block_size
+        lens = self._host_lens[:len(n)]
+        want = (lens + n + bs - 1) // bs
+        need = int((want - (lens + bs - 1) // bs).sum())
+        if need > self._host_free:
+            raise RuntimeError(_lib.OUT_OF_BLOCKS_MSG)
+        if len(n) and int(want.max()) > self.max_blocks_per_seq:
+            raise ValueError("sequence would outgrow its block table row")
+        counts = torch.from_numpy(n.astype(np.int32)).to(self.device)
+        with self._on_device():
+            status = _lib.load().snapmind_kv_reserve_each(
+                self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq,
+                self.seq_lens.data_ptr(), counts.data_ptr(), len(n), bs,
+                self.free_stack.data_ptr(), self.free_top.data_ptr(), self.num_blocks,
+                self.err.data_ptr(), self._stream(),
+            )  # fmt: skip
+        _lib.check(status, f"{type(self).__name__}.reserve_each")
+        self._host_lens[:len(n)] += n
         self._host_free -= need
 
     def blocks_needed(self, n_new: int, batch: int) -> int:

@@ -1,0 +1,414 @@
+// Attention of chunks of new tokens over a paged cache: entry point, the CUDA-core
+// kernel (any head_dim up to 256, any block size, f32 / bf16 / f16 / e4m3 caches) and
+// the merge of units that more than one CTA worked on.
+//
+//   o_i = sum_p softmax_p(scale q_i . k_p) v_p over the positions p that query i sees
+//   (chunk_plan.cuh).
+//
+// The CUDA-core kernel: 64 query rows x 64 keys a step, 256 threads, thread (ty, tx)
+// holding rows ty + 16 i and keys (then dims) tx + 16 j.  All arithmetic is f32, so it
+// is the path of f32 caches.
+#include <cuda_fp8.h>
+
+#include "chunk_plan.cuh"
+
+namespace snapmind {
+namespace {
+
+constexpr int kRows = 64, kKeys = 64, kGenThreads = 256;
+constexpr int kGenMaxD = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float e4m3_to_f(uint8_t c) {
+  const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
+  return __half2float(__half(h));
+}
+// 2^(b - 127) for a scale byte in [27, 247] (a normal float's exponent field)
+__device__ __forceinline__ float scale_byte_to_f(uint8_t b) { return __uint_as_float((uint32_t)b << 23); }
+
+// D4 = head_dim / 64 rounded up; smem rows are D = 64 * D4 floats (+4: 16-byte reads of
+// 16 different rows then touch different banks), zero past head_dim.
+template <int D4>
+struct GenSmem {
+  static constexpr int D = 64 * D4, P = D + 4, PS = kKeys + 4;
+  float q[kRows * P];
+  float k[kKeys * P];
+  float v[kKeys * P];
+  float s[kRows * PS];
+  int64_t row[kKeys];  // pool row of every key of the tile, -1: seen by no row
+  int32_t pos[kKeys];
+  PlanShared plan;
+};
+
+template <typename T, typename KV, int D4>
+__global__ void __launch_bounds__(kGenThreads) chunk_generic_kernel(ChunkParams p) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  using Smem = GenSmem<D4>;
+  constexpr int P = Smem::P, PS = Smem::PS;
+  constexpr bool kQuant = std::is_same<KV, uint8_t>::value;
+  Smem& S = *reinterpret_cast<Smem*>(smem_raw);
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  plan_block(p, S.plan, reinterpret_cast<int32_t*>(S.q));
+  if (tid == 0) write_piece_info(p, S.plan);
+  const float c2 = p.scale * kLog2e;
+  const int bs = p.block_size, hd = p.head_dim;
+
+  PieceWalk w;
+  for (bool on = w.start(S.plan); on; on = w.next(p)) {
+    const Piece& c = w.c;
+    const int heads = slice_heads(p, c.slice);
+    const int i1 = min(c.n, c.i0 + p.tokens);
+    const KeyRange kr = key_range(p, c.len, c.n, c.i0, i1);
+    const int n_rows = (i1 - c.i0) * p.gw;
+    const int head0 = c.kvh * p.group + c.slice * p.gw;
+    __syncthreads();
+    for (int e = tid; e < kRows * Smem::D; e += kGenThreads) {
+      const int r = e / Smem::D, d = e - r * Smem::D;
+      const int g = r % p.gw, tok = c.q_first + c.i0 + r / p.gw;
+      float x = 0.f;
+      if (r < n_rows && g < heads && d < hd)
+        x = Conv<T>::to_f(reinterpret_cast<const T*>(p.q)[(int64_t)tok * p.q_stride_tok + (int64_t)(head0 + g) * p.q_stride_head + d]);
+      S.q[r * P + d] = x;
+    }
+    float o[4][4 * D4], m[4], l[4];
+    int qpos[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+      qpos[i] = kr.pos0 + (ty + 16 * i) / p.gw;
+#pragma unroll
+      for (int j = 0; j < 4 * D4; ++j) o[i][j] = 0.f;
+    }
+    for (int t = c.tile0; t < c.tile1; ++t) {
+      __syncthreads();
+      if (tid < kKeys) {
+        const int v = t * kKeys + tid;
+        int64_t row = -1;
+        int pos = INT32_MAX;
+        if (v < kr.v_len) {
+          pos = kr.position(v);
+          const int j = pos / bs;
+          const bool in_sink = p.window > 0 && pos < p.sinks;
+          if (pos < kr.win_lo && !in_sink) {
+            pos = INT32_MAX;  // in a block that is read, before every window
+          } else if (j >= p.table_width) {
+            flag_error(p.err, SNAPMIND_DEVERR_TABLE);
+          } else {
+            const int32_t phys = p.tables[(int64_t)c.b * p.table_stride + j];
+            if (phys < 0 || phys >= p.num_blocks)
+              flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
+            else
+              row = ((int64_t)phys * p.n_kv_heads + c.kvh) * bs + (pos - j * bs);
+          }
+        }
+        if (row < 0) pos = INT32_MAX;
+        S.row[tid] = row;
+        S.pos[tid] = pos;
+      }
+      __syncthreads();
+      bool odd = false;  // a value of V that is not finite
+      for (int e = tid; e < kKeys * Smem::D; e += kGenThreads) {
+        const int r = e / Smem::D, d = e - r * Smem::D;
+        const int64_t row = S.row[r];
+        float kx = 0.f, vx = 0.f;
+        if (row >= 0 && d < hd) {
+          if constexpr (kQuant) {
+            // scales [block][head][2][slot]: K's bytes of a (block, head), then V's
+            const int64_t tile = row / bs;
+            const uint8_t* sc = p.scales + tile * 2 * bs + (row - tile * bs);
+            kx = e4m3_to_f(reinterpret_cast<const uint8_t*>(p.k_pool)[row * hd + d]) * scale_byte_to_f(sc[0]);
+            vx = e4m3_to_f(reinterpret_cast<const uint8_t*>(p.v_pool)[row * hd + d]) * scale_byte_to_f(sc[bs]);
+          } else {
+            kx = Conv<KV>::to_f(reinterpret_cast<const KV*>(p.k_pool)[row * hd + d]);
+            vx = Conv<KV>::to_f(reinterpret_cast<const KV*>(p.v_pool)[row * hd + d]);
+          }
+        }
+        S.k[r * P + d] = kx;
+        S.v[r * P + d] = vx;
+        odd |= !isfinite(vx);
+      }
+      odd = __syncthreads_or(odd);
+      float s[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < Smem::D; d += 4) {
+        float4 a[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(&S.q[(ty + 16 * i) * P + d]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(&S.k[(tx + 16 * j) * P + d]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
+            s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
+            s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
+            s[i][j] = fmaf(a[i].w, b[j].w, s[i][j]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float mx = m[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int pos = S.pos[tx + 16 * j];
+          const bool sees = pos <= qpos[i] && (p.window <= 0 || pos > qpos[i] - p.window || pos < p.sinks);
+          s[i][j] = sees ? s[i][j] * c2 : -INFINITY;
+          mx = fmaxf(mx, s[i][j]);
+        }
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        // nothing seen so far: any finite reference gives p = 2^-inf = 0
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        const float alpha = exp2f(m[i] - ref);
+        m[i] = mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float e = exp2f(s[i][j] - ref);
+          sum += e;
+          S.s[(ty + 16 * i) * PS + tx + 16 * j] = e;
+        }
+        l[i] = l[i] * alpha + sum;  // this thread's share; summed over the row's threads at the end
+#pragma unroll
+        for (int j = 0; j < 4 * D4; ++j) o[i][j] *= alpha;
+      }
+      __syncwarp();  // a row's 16 threads share a warp
+      if (!odd) {
+#pragma unroll 2
+        for (int k = 0; k < kKeys; k += 4) {
+          float a[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float4*>(a[i]) = *reinterpret_cast<const float4*>(&S.s[(ty + 16 * i) * PS + k]);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+            for (int j = 0; j < D4; ++j) {
+              const float4 b = *reinterpret_cast<const float4*>(&S.v[(k + kk) * P + 64 * j + 4 * tx]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                o[i][4 * j] = fmaf(a[i][kk], b.x, o[i][4 * j]);
+                o[i][4 * j + 1] = fmaf(a[i][kk], b.y, o[i][4 * j + 1]);
+                o[i][4 * j + 2] = fmaf(a[i][kk], b.z, o[i][4 * j + 2]);
+                o[i][4 * j + 3] = fmaf(a[i][kk], b.w, o[i][4 * j + 3]);
+              }
+            }
+        }
+      } else {
+        // infinities or NaN in V: they reach only the rows that see their token
+        for (int k = 0; k < kKeys; ++k) {
+          const int pos = S.pos[k];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!(pos <= qpos[i] && (p.window <= 0 || pos > qpos[i] - p.window || pos < p.sinks))) continue;
+            const float a = S.s[(ty + 16 * i) * PS + k];
+#pragma unroll
+            for (int j = 0; j < 4 * D4; ++j) o[i][j] = fmaf(a, S.v[k * P + 64 * (j / 4) + 4 * tx + j % 4], o[i][j]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
+      const int r = ty + 16 * i, g = r % p.gw;
+      if (r >= n_rows || g >= heads) continue;
+      if (c.whole()) {
+        const float inv = m[i] == -INFINITY ? 0.f : 1.f / l[i];  // sees nothing: zeros
+        T* out = reinterpret_cast<T*>(p.out) + (int64_t)(c.q_first + c.i0 + r / p.gw) * p.out_stride_tok +
+                 (int64_t)(head0 + g) * p.out_stride_head;
+#pragma unroll
+        for (int j = 0; j < 4 * D4; ++j) {
+          const int d = 64 * (j / 4) + 4 * tx + j % 4;
+          if (d < hd) out[d] = Conv<T>::from_f(m[i] == -INFINITY ? 0.f : o[i][j] * inv);
+        }
+      } else {
+        const int64_t slot = part_slot(c) * p.rows + r;
+        if (tx == 0) {
+          p.part_ml[slot * 2] = m[i];
+          p.part_ml[slot * 2 + 1] = l[i];
+        }
+#pragma unroll
+        for (int j = 0; j < 4 * D4; ++j) {
+          const int d = 64 * (j / 4) + 4 * tx + j % 4;
+          if (d < hd) p.part_o[slot * hd + d] = o[i][j];
+        }
+      }
+    }
+  }
+}
+
+// Merge of the cut units: block (c, y) works when CTA c holds the first cut inside a
+// unit, on rows y, y + gridDim.y, ...; pieces are CTA c - 1's slot 1, then slot 0 of CTAs
+// c .. last.  One warp per row: M = max m_i, out = sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M).
+constexpr int kMergeWarps = 4;
+template <typename T>
+__global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkParams p) {
+  // launched as a programmatic dependent of the attention kernel: complete and visible after this
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int cta = blockIdx.x + 1;
+  const int32_t* h = p.heads + (int64_t)cta * kPieceInts;
+  if (h[0] < 0 || h[4] != cta - 1) return;
+  const int b = h[0], kvh = h[1], slice = h[2], i0 = h[3], last = h[5];
+  int first;
+  const int n = chunk_queries(p, b, &first);
+  const int heads = slice_heads(p, slice), n_rows = (min(n, i0 + p.tokens) - i0) * p.gw;
+  const int lane = threadIdx.x & 31;
+  for (int r = blockIdx.y * kMergeWarps + (threadIdx.x >> 5); r < n_rows; r += gridDim.y * kMergeWarps) {
+    const int g = r % p.gw;
+    if (g >= heads) continue;
+    const auto slot = [&](int c) { return ((int64_t)c * 2 + (c == cta - 1 ? 1 : 0)) * p.rows + r; };
+    float M = -INFINITY;
+    for (int c = cta - 1 + lane; c <= last; c += 32) M = fmaxf(M, p.part_ml[slot(c) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float ref = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    for (int c = cta - 1 + lane; c <= last; c += 32) L += p.part_ml[slot(c) * 2 + 1] * exp2f(p.part_ml[slot(c) * 2] - ref);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    const float inv = M == -INFINITY ? 0.f : 1.f / L;
+    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(first + i0 + r / p.gw) * p.out_stride_tok +
+             (int64_t)(kvh * p.group + slice * p.gw + g) * p.out_stride_head;
+    for (int d = lane; d < p.head_dim; d += 32) {
+      float a = 0.f;
+      for (int c = cta - 1; c <= last; ++c) {
+        const float mc = p.part_ml[slot(c) * 2];
+        if (mc != -INFINITY) a = fmaf(p.part_o[slot(c) * p.head_dim + d], exp2f(mc - ref), a);
+      }
+      out[d] = Conv<T>::from_f(M == -INFINITY ? 0.f : a * inv);
+    }
+  }
+}
+
+template <typename T, typename KV>
+int launch_generic(ChunkParams& p, cudaStream_t st) {
+  const auto go = [&](auto kernel, size_t smem) -> int {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
+    kernel<<<p.n_ctas, kGenThreads, smem, st>>>(p);
+    return cuda_status(cudaGetLastError(), "paged_chunk launch");
+  };
+  static_assert(sizeof(GenSmem<4>) <= 232448, "shared memory budget");
+  static_assert(sizeof(GenSmem<1>().q) + sizeof(GenSmem<1>().k) >= kMaxChunkBatch * 4, "plan scratch");
+  if (p.head_dim <= 64) return go(chunk_generic_kernel<T, KV, 1>, sizeof(GenSmem<1>));
+  if (p.head_dim <= 128) return go(chunk_generic_kernel<T, KV, 2>, sizeof(GenSmem<2>));
+  return go(chunk_generic_kernel<T, KV, 4>, sizeof(GenSmem<4>));
+}
+
+// The largest CTA count and unit rows of the kernels, for the workspace.
+int64_t max_ctas() { return (int64_t)num_sms() * 2; }
+constexpr int kMaxRows = 256;
+
+}  // namespace
+
+int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st) {
+  if (p.n_ctas < 2) return SNAPMIND_OK;
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  const int used = p.gw * p.tokens;
+  cfg.gridDim = dim3(p.n_ctas - 1, (used + kMergeWarps - 1) / kMergeWarps < 16 ? (used + kMergeWarps - 1) / kMergeWarps : 16);
+  cfg.blockDim = dim3(32 * kMergeWarps);
+  cfg.stream = st;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  switch (dtype) {
+    case SNAPMIND_DTYPE_F32: return cuda_status(cudaLaunchKernelEx(&cfg, chunk_merge_kernel<float>, p), "paged_chunk merge");
+    case SNAPMIND_DTYPE_BF16:
+      return cuda_status(cudaLaunchKernelEx(&cfg, chunk_merge_kernel<__nv_bfloat16>, p), "paged_chunk merge");
+    default: return cuda_status(cudaLaunchKernelEx(&cfg, chunk_merge_kernel<__half>, p), "paged_chunk merge");
+  }
+}
+
+}  // namespace snapmind
+
+using namespace snapmind;
+
+extern "C" {
+
+int64_t snapmind_paged_gqa_chunk_workspace_bytes(int32_t head_dim) {
+  if (head_dim <= 0 || head_dim > kGenMaxD) return 0;
+  ChunkParams p = {};
+  p.head_dim = head_dim;
+  return plan_workspace(p, nullptr, max_ctas(), kMaxRows);
+}
+
+int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stride_head, int dtype, const void* k_pool,
+                             const void* v_pool, const void* scales, int pool_dtype, const int32_t* block_tables,
+                             int64_t table_stride_seq, int32_t table_width, const int32_t* seq_lens,
+                             const int32_t* cu_q, void* out, int64_t out_stride_tok, int64_t out_stride_head,
+                             float scale, int32_t batch, int32_t total_q, int32_t n_q_heads, int32_t n_kv_heads,
+                             int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t window, int32_t sinks,
+                             int32_t flags, void* workspace, int64_t workspace_bytes, int32_t* err_word, void* stream) {
+  SNAPMIND_CHECK_ARG(dtype_size(dtype) > 0, "paged_chunk: unknown dtype");
+  SNAPMIND_CHECK_ARG(pool_dtype == dtype || pool_dtype == SNAPMIND_DTYPE_E4M3,
+                     "paged_chunk: the pool holds the query's dtype or e4m3");
+  SNAPMIND_CHECK_ARG((pool_dtype == SNAPMIND_DTYPE_E4M3) == (scales != nullptr),
+                     "paged_chunk: scales go with an e4m3 pool, and only with one");
+  SNAPMIND_CHECK_ARG(batch >= 0 && batch <= kMaxChunkBatch && total_q >= 0 && n_q_heads > 0 && n_kv_heads > 0 &&
+                         block_size > 0 && num_blocks > 0 && table_width >= 0,
+                     "paged_chunk: bad sizes (batch at most %d)", kMaxChunkBatch);
+  SNAPMIND_CHECK_ARG(n_q_heads % n_kv_heads == 0, "paged_chunk: n_q_heads (%d) must be a multiple of n_kv_heads (%d)",
+                     n_q_heads, n_kv_heads);
+  SNAPMIND_CHECK_ARG(head_dim > 0 && head_dim <= kGenMaxD, "paged_chunk: head_dim must be in [1, %d]", kGenMaxD);
+  SNAPMIND_CHECK_ARG(window >= 0 && sinks >= 0, "paged_chunk: window and sinks must not be negative");
+  SNAPMIND_CHECK_ARG(window > 0 || sinks == 0, "paged_chunk: sinks need a window");
+  SNAPMIND_CHECK_ARG(cu_q != nullptr || total_q == batch, "paged_chunk: without cu_q there is one query per sequence");
+  if (batch == 0 || total_q == 0) return SNAPMIND_OK;
+  SNAPMIND_CHECK_ARG(q && k_pool && v_pool && block_tables && seq_lens && out, "paged_chunk: null pointer");
+  ChunkParams p = {};
+  p.q = q;
+  p.q_stride_tok = q_stride_tok;
+  p.q_stride_head = q_stride_head;
+  p.k_pool = k_pool;
+  p.v_pool = v_pool;
+  p.scales = static_cast<const uint8_t*>(scales);
+  p.tables = block_tables;
+  p.table_stride = table_stride_seq;
+  p.table_width = table_width;
+  p.seq_lens = seq_lens;
+  p.cu_q = cu_q;
+  p.out = out;
+  p.out_stride_tok = out_stride_tok;
+  p.out_stride_head = out_stride_head;
+  p.scale = scale;
+  p.batch = batch;
+  p.total_q = total_q;
+  p.n_q_heads = n_q_heads;
+  p.n_kv_heads = n_kv_heads;
+  p.group = n_q_heads / n_kv_heads;
+  p.head_dim = head_dim;
+  p.block_size = block_size;
+  p.num_blocks = num_blocks;
+  p.window = window < (1 << 30) ? window : (1 << 30);  // positions stay below 2^30
+  p.sinks = sinks < (1 << 30) ? sinks : (1 << 30);
+  p.err = err_word;
+  const int64_t need = plan_workspace(p, workspace, max_ctas(), kMaxRows);
+  SNAPMIND_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
+                     "paged_chunk: workspace needs %lld bytes on a 256-byte boundary, got %lld", (long long)need,
+                     (long long)workspace_bytes);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
+  const int ctas = num_sms() * (head_dim <= 64 ? 2 : 1);
+  plan_geometry(p, kRows, kKeys, ctas);
+  int rc;
+  switch (dtype) {
+    case SNAPMIND_DTYPE_F32: rc = quant ? launch_generic<float, uint8_t>(p, st) : launch_generic<float, float>(p, st); break;
+    case SNAPMIND_DTYPE_BF16:
+      rc = quant ? launch_generic<__nv_bfloat16, uint8_t>(p, st) : launch_generic<__nv_bfloat16, __nv_bfloat16>(p, st);
+      break;
+    default: rc = quant ? launch_generic<__half, uint8_t>(p, st) : launch_generic<__half, __half>(p, st); break;
+  }
+  return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
+}
+
+}  // extern "C"

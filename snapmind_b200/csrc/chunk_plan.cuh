@@ -1,0 +1,312 @@
+// Work plan of the paged attention over chunks of new tokens (chunk_attn*.cu,
+// decode_sinks.cu).
+//
+// A unit is one (sequence b, kv head, slice of its query group, run of query tokens): at
+// most `rows` query rows that read the same keys.  Row r of a unit is token
+// i0 + r / gw, query head r % gw of the slice (gw = the slice's heads).  A unit's
+// work is the number of key tiles some row of it sees, and the tiles of all units,
+// in the order (b, kv head, slice, run), form one line that the CTAs cut into equal
+// pieces: CTA c of n takes tiles [c W / n, (c + 1) W / n) of W (n is at most W).  So every CTA streams
+// the same number of tiles whatever the lengths are, and long caches with few rows are
+// split over many CTAs by the same rule.  A unit cut by a boundary leaves one
+// partial softmax state per piece in the workspace, and a second kernel merges them.
+// The plan needs nothing from the host: lengths may come from a captured step.
+//
+// Keys of a unit.  Query position p sees keys j <= p, under a window w only
+// j > p - w or j < sinks.  The unit's keys are the sink blocks, then the blocks from
+// the first one that its first query's window reaches: a virtual axis v with one jump,
+// position(v) = v + (v >= v_sink ? shift : 0), so nothing between is read.
+#pragma once
+
+#include "common.cuh"
+
+namespace snapmind {
+
+struct ChunkParams {
+  const void* q;
+  int64_t q_stride_tok, q_stride_head;  // elements
+  const void* k_pool;
+  const void* v_pool;
+  const uint8_t* scales;  // e4m3 pools: [block][head][2][slot] exponents + 127 (else NULL)
+  const int32_t* tables;
+  int64_t table_stride;
+  int32_t table_width;
+  const int32_t* seq_lens;
+  const int32_t* cu_q;  // [batch + 1] first query row of every sequence; NULL: one each
+  void* out;
+  int64_t out_stride_tok, out_stride_head;  // elements
+  float scale;
+  int32_t batch, total_q, n_q_heads, n_kv_heads, group, head_dim, block_size, num_blocks;
+  int32_t window, sinks;   // window 0: none
+  int32_t gw, n_slices;    // query heads of a slice, slices of a group
+  int32_t tokens;          // query tokens of a unit
+  int32_t rows;            // partial rows of a unit in the workspace (>= gw * tokens)
+  int32_t key_tile;        // keys of a tile
+  int32_t n_ctas;
+  int32_t* heads;   // workspace: [n_ctas][kPieceInts], see PieceInfo
+  float* part_ml;   // workspace: [n_ctas][2][rows][2] maximum (log2 units), sum
+  float* part_o;    // workspace: [n_ctas][2][rows][head_dim]
+  int32_t* err;
+};
+
+constexpr int kPieceInts = 8;   // b, kv head, slice, first token, first piece's CTA, last piece's CTA
+constexpr int kMaxChunkBatch = 8192;
+
+// New tokens of sequence b: its first query row and their number.
+__device__ __forceinline__ int chunk_queries(const ChunkParams& p, int b, int* first) {
+  if (p.cu_q == nullptr) {
+    *first = b;
+    return 1;
+  }
+  const int lo = min(max(p.cu_q[b], 0), p.total_q);
+  *first = lo;
+  return min(max(p.cu_q[b + 1], lo), p.total_q) - lo;
+}
+
+// The keys that the query tokens [i0, i1) of n new ones see in a cache of len tokens.
+struct KeyRange {
+  int pos0;    // position of token i0
+  int end;     // positions >= end are seen by none
+  int win_lo;  // first position inside token i0's window
+  int v_sink, shift, v_len;
+  __device__ __forceinline__ int position(int v) const { return v + (v >= v_sink ? shift : 0); }
+};
+__device__ __forceinline__ KeyRange key_range(const ChunkParams& p, int len, int n, int i0, int i1) {
+  KeyRange r;
+  r.pos0 = len - n + i0;
+  r.end = max(0, min(len, len - n + i1));
+  r.win_lo = p.window > 0 ? max(0, r.pos0 - p.window + 1) : 0;
+  const int bs = p.block_size;
+  const int n_sink = p.window > 0 ? (min(p.sinks, r.end) + bs - 1) / bs : 0;
+  const int wb0 = min(r.win_lo, r.end) / bs;
+  r.v_sink = n_sink * bs;
+  r.shift = max(0, wb0 - n_sink) * bs;
+  r.v_len = r.end - r.shift;
+  return r;
+}
+// Key tiles of a unit; at least one, so that rows that see nothing are written as zeros.
+__device__ __forceinline__ int key_tiles(const ChunkParams& p, int len, int n, int i0) {
+  const KeyRange r = key_range(p, len, n, i0, min(n, i0 + p.tokens));
+  return max(1, (r.v_len + p.key_tile - 1) / p.key_tile);
+}
+
+// A piece: consecutive tiles of one unit.
+struct Piece {
+  int b, kvh, slice, i0;     // the unit
+  int n, len, q_first;       // new tokens, cached tokens, first query row of sequence b
+  int tile0, tile1, n_tiles; // tiles of the piece, tiles of the unit
+  __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == n_tiles; }
+};
+
+struct PlanShared {
+  int32_t warp_sum[32];
+  long long total, t0, t1;
+  int32_t n;            // CTAs with work: min(n_ctas, total)
+  int32_t b, rem;       // sequence of tile t0, tiles before it in the sequence
+  int32_t u;            // tiles of one (kv head, slice) of that sequence
+  Piece first;
+};
+
+__device__ __forceinline__ int clamp_len(const ChunkParams& p, int b) { return max(0, p.seq_lens[b]); }
+
+// Tiles of one (kv head, slice) of sequence b, summed by a full warp.
+__device__ __forceinline__ int seq_tiles(const ChunkParams& p, int b, int lane) {
+  int first;
+  const int n = chunk_queries(p, b, &first);
+  const int len = clamp_len(p, b);
+  int s = 0;
+  for (int i0 = lane * p.tokens; i0 < n; i0 += 32 * p.tokens) s += key_tiles(p, len, n, i0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+// The block's share of the line: fills S (total, t0, t1, first piece).  `tiles` is
+// scratch for batch ints.  Every thread of the block calls it; ends with a barrier.
+__device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* tiles) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  const int per_head = p.n_kv_heads * p.n_slices;
+  if (p.cu_q == nullptr) {
+    for (int b = tid; b < p.batch; b += blockDim.x) tiles[b] = key_tiles(p, clamp_len(p, b), 1, 0);
+  } else {
+    for (int b = warp; b < p.batch; b += nw) {
+      const int s = seq_tiles(p, b, lane);
+      if (lane == 0) tiles[b] = s;
+    }
+  }
+  __syncthreads();
+  // sums of contiguous runs of sequences, one run per thread
+  const int run = (p.batch + blockDim.x - 1) / blockDim.x;
+  const int b0 = min(p.batch, tid * run), b1 = min(p.batch, b0 + run);
+  int s = 0;
+  for (int b = b0; b < b1; ++b) s += tiles[b];
+  int incl = s;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) S.warp_sum[warp] = incl;
+  __syncthreads();
+  long long before = 0, total = 0;
+  for (int w = 0; w < nw; ++w) {
+    if (w < warp) before += S.warp_sum[w];
+    total += S.warp_sum[w];
+  }
+  before = (before + incl - s) * per_head;
+  total *= per_head;
+  const int n = (int)min((long long)p.n_ctas, total);
+  const bool works = (int)blockIdx.x < n;
+  const long long t0 = works ? (long long)blockIdx.x * total / n : total;
+  const long long t1 = works ? ((long long)blockIdx.x + 1) * total / n : total;
+  if (tid == 0) {
+    S.total = total;
+    S.n = n;
+    S.t0 = t0;
+    S.t1 = t1;
+  }
+  if (t0 < t1 && t0 >= before && t0 < before + (long long)s * per_head) {
+    long long at = before;
+    int b = b0;
+    while (t0 >= at + (long long)tiles[b] * per_head) at += (long long)tiles[b++] * per_head;
+    S.b = b;
+    S.u = tiles[b];
+    S.rem = (int)(t0 - at);
+  }
+  __syncthreads();
+  if (warp == 0 && t0 < t1) {
+    Piece f;
+    f.b = S.b;
+    const int hs = S.rem / S.u;
+    int rem = S.rem - hs * S.u;
+    f.kvh = hs / p.n_slices;
+    f.slice = hs - f.kvh * p.n_slices;
+    f.n = chunk_queries(p, f.b, &f.q_first);
+    f.len = clamp_len(p, f.b);
+    f.i0 = 0;
+    for (int base = 0;; base += 32) {  // 32 runs at a time; ends inside the sequence since rem < u
+      const int i0 = (base + lane) * p.tokens;
+      const int t = i0 < f.n ? key_tiles(p, f.len, f.n, i0) : 0;
+      int x = t;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const uint32_t m = __ballot_sync(0xffffffffu, x > rem);
+      if (m != 0 || i0 - lane * p.tokens >= f.n) {
+        const int l = m != 0 ? __ffs(m) - 1 : 0;
+        f.i0 = __shfl_sync(0xffffffffu, i0, l);
+        f.n_tiles = __shfl_sync(0xffffffffu, t, l);
+        f.tile0 = rem - (__shfl_sync(0xffffffffu, x, l) - f.n_tiles);
+        break;
+      }
+      rem -= __shfl_sync(0xffffffffu, x, 31);
+    }
+    f.tile1 = (int)min((long long)f.n_tiles, f.tile0 + (t1 - t0));
+    if (lane == 0) S.first = f;
+  }
+  __syncthreads();
+}
+
+// Walks the pieces of a CTA: `left` tiles remain after the current piece.
+struct PieceWalk {
+  Piece c;
+  long long left;
+  __device__ __forceinline__ bool start(const PlanShared& S) {
+    c = S.first;
+    left = S.t1 - S.t0;
+    if (left <= 0) return false;
+    left -= c.tile1 - c.tile0;
+    return true;
+  }
+  __device__ __forceinline__ bool next(const ChunkParams& p) {
+    if (left <= 0) return false;
+    c.i0 += p.tokens;
+    if (c.i0 >= c.n) {
+      c.i0 = 0;
+      if (++c.slice == p.n_slices) {
+        c.slice = 0;
+        if (++c.kvh == p.n_kv_heads) {
+          c.kvh = 0;
+          do {
+            if (++c.b >= p.batch) return false;
+            c.n = chunk_queries(p, c.b, &c.q_first);
+          } while (c.n == 0);
+          c.len = clamp_len(p, c.b);
+        }
+      }
+    }
+    c.n_tiles = key_tiles(p, c.len, c.n, c.i0);
+    c.tile0 = 0;
+    c.tile1 = (int)min((long long)c.n_tiles, left);
+    left -= c.tile1;
+    return true;
+  }
+};
+
+// Query heads of a slice (the last one of a group may be narrower).
+__device__ __forceinline__ int slice_heads(const ChunkParams& p, int slice) {
+  return min(p.gw, p.group - slice * p.gw);
+}
+
+// Partial slot of a piece: 0 = the unit began in an earlier CTA, 1 = it begins here.
+__device__ __forceinline__ int64_t part_slot(const Piece& c) { return (int64_t)blockIdx.x * 2 + (c.tile0 == 0 ? 1 : 0); }
+
+// What the merge kernel reads about the unit that CTA c cuts at its start: written by one
+// thread, b = -1 when the CTA starts on a unit's first tile or has no work.
+__device__ inline void write_piece_info(const ChunkParams& p, const PlanShared& S) {
+  int32_t* h = p.heads + (int64_t)blockIdx.x * kPieceInts;
+  if (S.t0 >= S.t1 || S.first.tile0 == 0) {
+    h[0] = -1;
+    return;
+  }
+  const Piece& c = S.first;
+  const long long s_u = S.t0 - c.tile0, e_u = s_u + c.n_tiles;
+  h[1] = c.kvh;
+  h[2] = c.slice;
+  h[3] = c.i0;
+  h[4] = (int32_t)(((s_u + 1) * S.n - 1) / S.total);  // the CTA that holds tile s_u
+  h[5] = (int32_t)((e_u * S.n - 1) / S.total);        // ... and tile e_u - 1
+  h[0] = c.b;
+}
+
+// 2^x by the hardware approximation (2 ulp); -inf -> 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// chunk_attn.cu: merges the cut units, after the attention kernel on the stream.
+int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st);
+
+// chunk_attn_umma.cu (tcgen05) and decode_sinks.cu (one token per sequence): whether the
+// shapes fit, the unit geometry and CTA count they want, and the launch.
+bool chunk_umma_supported(const ChunkParams& p, int dtype, int pool_dtype);
+int launch_chunk_umma(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st);
+bool decode_sinks_supported(const ChunkParams& p, int dtype, int pool_dtype);
+int launch_decode_sinks(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st);
+
+// Unit geometry for kernels of `rows` query rows, `key_tile` keys and `n_ctas` CTAs.
+inline void plan_geometry(ChunkParams& p, int rows, int key_tile, int n_ctas) {
+  p.gw = p.group < rows ? p.group : rows;
+  p.n_slices = (p.group + p.gw - 1) / p.gw;
+  p.tokens = rows / p.gw;
+  p.rows = rows;
+  p.key_tile = key_tile;
+  p.n_ctas = n_ctas;
+}
+
+// Workspace regions of n_ctas CTAs: heads, then maxima and sums, then partial outputs.
+inline int64_t plan_workspace(ChunkParams& p, void* workspace, int64_t n_ctas, int64_t rows) {
+  const int64_t ml_off = (n_ctas * kPieceInts * 4 + 255) / 256 * 256;
+  const int64_t o_off = ml_off + (n_ctas * 2 * rows * 2 * 4 + 255) / 256 * 256;
+  char* w = static_cast<char*>(workspace);
+  p.heads = reinterpret_cast<int32_t*>(w);
+  p.part_ml = reinterpret_cast<float*>(w + ml_off);
+  p.part_o = reinterpret_cast<float*>(w + o_off);
+  return o_off + n_ctas * 2 * rows * p.head_dim * 4;
+}
+
+}  // namespace snapmind

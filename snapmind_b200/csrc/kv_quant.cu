@@ -1,0 +1,517 @@
+// Rows written into a paged pool from ragged or uniform chunks, quantised to 8 bits when
+// the pool holds e4m3, and 8-bit pools read back.
+//
+// Quantisation of a row x of one token and head (head_dim values, K or V):
+//   e = the smallest integer in [-100, 120] with max |x| <= 448 2^e,
+//   c = x 2^-e rounded to e4m3 (nearest even);
+// the pool keeps the codes [block][head][slot][dim] (1 byte each) and one byte e + 127 per
+// row, [block][head][K, V][slot], so a 16-token tile's 32 scale bytes are one sector.  The
+// scale is a power of two, because then scaling is exact: no rounding but e4m3's own, codes
+// that do not hang on a division's last bit, values that bf16 holds exactly, and nothing
+// lost, since the relative step of e4m3 (2^-4 at most, half a step) is the same at
+// every scale.  Infinities and NaN are stored as NaN and do not count for the scale.
+//
+// Both kernels are byte movers: a team of lanes owns a row (16-byte vectors of the wide
+// side), several rows in flight per team.
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace snapmind {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct ChunkAppendParams {
+  uint8_t* pool[2];
+  uint8_t* scales;
+  const char* in[2];
+  int64_t pool_layer_stride, scale_layer_stride;                          // bytes
+  int64_t in_stride_layer, in_stride_seq, in_stride_head, in_stride_tok;  // bytes
+  const int32_t* tables;
+  int64_t table_stride;
+  int32_t table_width;
+  const int32_t* slot_starts;
+  int32_t slot_start0;
+  const int32_t* cu;  // [batch + 1] first row of every sequence, or NULL: n_tokens each
+  int32_t batch, n_tokens, total, n_heads, head_dim, block_size, num_blocks;
+  int32_t heads_inner;  // consecutive rows walk the heads (else the tokens)
+  int32_t* err;
+};
+
+// Exponent of a row whose largest finite magnitude is a.
+__device__ __forceinline__ int row_exponent(float a) {
+  const uint32_t u = __float_as_uint(a);
+  const int k = (int)(u >> 23) - 127;
+  const int e = (u & 0x7FFFFFu) <= 0x600000u ? k - 8 : k - 7;  // a <= 1.75 2^(e + 8)
+  return min(max(e, -100), 120);
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a < INFINITY ? a : 0.f;  // false for NaN too
+}
+__device__ __forceinline__ float scaled(float x, float inv) {
+  return fabsf(x) < INFINITY ? x * inv : __uint_as_float(0x7FC00000u);
+}
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); };
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& w, float* f) {
+  const T* t = reinterpret_cast<const T*>(&w);
+#pragma unroll
+  for (int i = 0; i < Vec<T>::N; ++i) f[i] = Conv<T>::to_f(t[i]);
+}
+
+// Row r of the (layer, K or V) plane: its source and its pool row (-1: skipped).
+__device__ __forceinline__ int64_t append_row(const ChunkAppendParams& p, int r, const char* in, const char** src) {
+  int h, i;
+  if (p.heads_inner) {
+    i = r / p.n_heads;
+    h = r - i * p.n_heads;
+  } else {  // (sequence, head, token)
+    const int bh = r / p.n_tokens, t = r - bh * p.n_tokens, b = bh / p.n_heads;
+    h = bh - b * p.n_heads;
+    i = b * p.n_tokens + t;
+  }
+  int b, t, n = 0;
+  if (p.cu != nullptr) {
+    b = upper_bound_i32(p.cu, p.batch + 1, i) - 1;  // rows outside every sequence are not stored
+    if (b < 0 || b >= p.batch) return -1;
+    t = i - p.cu[b];
+    n = p.cu[b + 1] - p.cu[b];
+    *src = in + (int64_t)i * p.in_stride_tok + (int64_t)h * p.in_stride_head;
+  } else {
+    b = i / p.n_tokens;
+    t = i - b * p.n_tokens;
+    *src = in + (int64_t)b * p.in_stride_seq + (int64_t)t * p.in_stride_tok + (int64_t)h * p.in_stride_head;
+  }
+  const int slot = (p.slot_starts ? p.slot_starts[b] : 0) + p.slot_start0 - n + t;
+  const int j = slot / p.block_size;
+  if (slot < 0 || j >= p.table_width) {
+    flag_error(p.err, SNAPMIND_DEVERR_TABLE);
+    return -1;
+  }
+  const int32_t phys = p.tables[(int64_t)b * p.table_stride + j];
+  if (phys < 0 || phys >= p.num_blocks) {
+    flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
+    return -1;
+  }
+  return ((int64_t)phys * p.n_heads + h) * p.block_size + (slot - j * p.block_size);
+}
+
+// Byte of a row's exponent: row = (block * heads + head) * block_size + slot.
+__device__ __forceinline__ int64_t scale_at(int64_t row, int bs, int kv) {
+  const int64_t tile = row / bs;
+  return (tile * 2 + kv) * bs + (row - tile * bs);
+}
+
+// Rows of TEAM lanes x one 16-byte vector each (head_dim * sizeof(T) = 16 TEAM bytes).
+// blockIdx.y = layer * 2 + (K, V).  kUnroll rows of a team are loaded before the first is
+// used.
+template <typename T, int TEAM>
+__global__ void __launch_bounds__(kThreads) quant_append_kernel(ChunkAppendParams p) {
+  constexpr int N = Vec<T>::N, kUnroll = 4;
+  const int kv = blockIdx.y & 1, layer = blockIdx.y >> 1;
+  const int lane = threadIdx.x % TEAM;
+  const int team = (blockIdx.x * kThreads + threadIdx.x) / TEAM, teams = gridDim.x * (kThreads / TEAM);
+  const int rows = p.total * p.n_heads;
+  const char* in = p.in[kv] + layer * p.in_stride_layer;
+  uint8_t* pool = p.pool[kv] + layer * p.pool_layer_stride;
+  uint8_t* scales = p.scales + layer * p.scale_layer_stride;
+  // every lane of a warp takes the same number of steps (the shuffles below are warp-wide)
+  const int steps = (rows + teams * kUnroll - 1) / (teams * kUnroll);
+  for (int s = 0; s < steps; ++s) {
+    uint4 w[kUnroll];
+    int64_t row[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t r = ((int64_t)s * kUnroll + u) * teams + team;
+      row[u] = -1;
+      w[u] = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const char* src;
+        row[u] = append_row(p, (int)r, in, &src);
+        if (row[u] >= 0) w[u] = reinterpret_cast<const uint4*>(src)[lane];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float f[N];
+      unpack<T>(w[u], f);
+      float a = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) a = fmaxf(a, finite_abs(f[i]));
+#pragma unroll
+      for (int o = TEAM / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+      if (row[u] < 0) continue;
+      const int e = row_exponent(a);
+      const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = scaled(f[i], inv);
+      uint8_t* dst = pool + row[u] * p.head_dim + lane * N;
+      if constexpr (N == 8)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(codes4(f[0], f[1], f[2], f[3]), codes4(f[4], f[5], f[6], f[7]));
+      else
+        *reinterpret_cast<uint32_t*>(dst) = codes4(f[0], f[1], f[2], f[3]);
+      if (lane == 0) scales[scale_at(row[u], p.block_size, kv)] = (uint8_t)(e + 127);
+    }
+  }
+}
+
+// Any head_dim, stride and alignment: one warp per row, one element per lane and step.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) quant_append_any_kernel(ChunkAppendParams p) {
+  const int kv = blockIdx.y & 1, layer = blockIdx.y >> 1;
+  const int lane = threadIdx.x & 31;
+  const int rows = p.total * p.n_heads;
+  const char* in = p.in[kv] + layer * p.in_stride_layer;
+  uint8_t* pool = p.pool[kv] + layer * p.pool_layer_stride;
+  const int warps = gridDim.x * (kThreads / 32);
+  for (int64_t r = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < rows; r += warps) {  // warp-uniform
+    const char* src;
+    const int64_t row = append_row(p, (int)r, in, &src);
+    if (row < 0) continue;
+    const T* x = reinterpret_cast<const T*>(src);
+    float a = 0.f;
+    for (int d = lane; d < p.head_dim; d += 32) a = fmaxf(a, finite_abs(Conv<T>::to_f(x[d])));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+    const int e = row_exponent(a);
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    for (int d = lane; d < p.head_dim; d += 32)
+      pool[row * p.head_dim + d] = __nv_cvt_float_to_fp8(scaled(Conv<T>::to_f(x[d]), inv), __NV_SATFINITE, __NV_E4M3);
+    if (lane == 0) p.scales[layer * p.scale_layer_stride + scale_at(row, p.block_size, kv)] = (uint8_t)(e + 127);
+  }
+}
+
+// A pool of plain elements: the rows are stored as they are, or converted.
+template <typename Tin, typename Tout>
+__global__ void __launch_bounds__(kThreads) chunk_append_kernel(ChunkAppendParams p) {
+  const int kv = blockIdx.y & 1, layer = blockIdx.y >> 1;
+  const int lane = threadIdx.x & 31;
+  const int rows = p.total * p.n_heads;
+  const char* in = p.in[kv] + layer * p.in_stride_layer;
+  Tout* pool = reinterpret_cast<Tout*>(p.pool[kv] + layer * p.pool_layer_stride);
+  const int warps = gridDim.x * (kThreads / 32);
+  for (int64_t r = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < rows; r += warps) {
+    const char* src;
+    const int64_t row = append_row(p, (int)r, in, &src);
+    if (row < 0) continue;
+    const Tin* x = reinterpret_cast<const Tin*>(src);
+    Tout* y = pool + row * p.head_dim;
+    if constexpr (std::is_same<Tin, Tout>::value) {
+      if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 7) == 0 && p.head_dim * sizeof(Tin) % 8 == 0) {
+        for (int d = lane; d < p.head_dim * (int)sizeof(Tin) / 8; d += 32)
+          reinterpret_cast<uint2*>(y)[d] = reinterpret_cast<const uint2*>(x)[d];
+        continue;
+      }
+    }
+    for (int d = lane; d < p.head_dim; d += 32) y[d] = Conv<Tout>::from_f(Conv<Tin>::to_f(x[d]));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// read back
+// ---------------------------------------------------------------------------
+struct QuantGatherParams {
+  const uint8_t* pool[2];
+  const uint8_t* scales;
+  char* out[2];
+  int64_t pool_layer_stride, scale_layer_stride, out_layer_stride;  // bytes
+  int64_t out_capacity;                                             // elements one layer's output holds
+  const int32_t* tables;
+  int64_t table_stride;
+  int32_t table_width;
+  const int32_t* seq_lens;
+  int32_t batch, n_heads, head_dim, block_size, num_blocks;
+  int32_t* err;
+};
+
+__device__ __forceinline__ float dequant_top(float) { return 3.402823466e38f; }
+__device__ __forceinline__ float dequant_top(__nv_bfloat16) { return 3.389531390e38f; }
+__device__ __forceinline__ float dequant_top(__half) { return 65504.f; }
+
+// c 2^e, held to T's finite range (a NaN stays one)
+template <typename T>
+__device__ __forceinline__ T dequant(float c, float scale) {
+  const float y = c * scale, top = dequant_top(T());
+  return Conv<T>::from_f(fabsf(y) > top ? copysignf(top, y) : y);
+}
+
+// Work item = one block of one sequence: all its heads, K and V of one layer
+// (blockIdx.y).  The items of a sequence start after those of the sequences before it; a
+// CTA finds its sequences by a scan of the lengths, kept in shared memory.  A thread
+// turns 16 / sizeof(T) codes into one 16-byte vector (kVec), or single elements.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kThreads) quant_gather_kernel(QuantGatherParams p) {
+  extern __shared__ int32_t cu[];  // [batch + 1] first block, then [batch + 1] first token
+  int32_t* cu_tok = cu + p.batch + 1;
+  __shared__ int32_t s_sum[2][kThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  {
+    const int run = (p.batch + kThreads - 1) / kThreads, b0 = min(p.batch, tid * run), b1 = min(p.batch, b0 + run);
+    int nb = 0, nt = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int len = max(0, p.seq_lens[b]);
+      nb += (len + p.block_size - 1) / p.block_size;
+      nt += len;
+    }
+    int xb = nb, xt = nt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int yb = __shfl_up_sync(0xffffffffu, xb, o), yt = __shfl_up_sync(0xffffffffu, xt, o);
+      if (lane >= o) {
+        xb += yb;
+        xt += yt;
+      }
+    }
+    if (lane == 31) {
+      s_sum[0][warp] = xb;
+      s_sum[1][warp] = xt;
+    }
+    __syncthreads();
+    int fb = xb - nb, ft = xt - nt;
+    for (int w = 0; w < warp; ++w) {
+      fb += s_sum[0][w];
+      ft += s_sum[1][w];
+    }
+    for (int b = b0; b < b1; ++b) {
+      const int len = max(0, p.seq_lens[b]);
+      cu[b] = fb;
+      cu_tok[b] = ft;
+      fb += (len + p.block_size - 1) / p.block_size;
+      ft += len;
+    }
+    if (b0 < p.batch && b1 == p.batch) {
+      cu[p.batch] = fb;
+      cu_tok[p.batch] = ft;
+    }
+    __syncthreads();
+  }
+  const int row_elems = p.n_heads * p.head_dim;
+  if ((int64_t)cu_tok[p.batch] * row_elems > p.out_capacity) {
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) flag_error(p.err, SNAPMIND_DEVERR_TABLE);
+    return;
+  }
+  constexpr int N = kVec ? Vec<T>::N : 1, kUnroll = 4;
+  const int layer = blockIdx.y;
+  const int per_row = p.head_dim / N;
+  for (int it = blockIdx.x; it < cu[p.batch]; it += gridDim.x) {
+    const int b = upper_bound_i32(cu, p.batch + 1, it) - 1, j = it - cu[b];
+    const int len = cu_tok[b + 1] - cu_tok[b], rows = min(p.block_size, len - j * p.block_size);
+    const int32_t phys = j < p.table_width ? p.tables[(int64_t)b * p.table_stride + j] : -1;
+    if (phys < 0 || phys >= p.num_blocks) {
+      if (tid == 0) flag_error(p.err, j < p.table_width ? SNAPMIND_DEVERR_BLOCK_ID : SNAPMIND_DEVERR_TABLE);
+      continue;
+    }
+    const uint8_t* sc = p.scales + layer * p.scale_layer_stride + (int64_t)phys * p.n_heads * 2 * p.block_size;
+    const int64_t src0 = layer * p.pool_layer_stride + (int64_t)phys * p.n_heads * p.block_size * p.head_dim;
+    const int64_t dst0 = (int64_t)cu_tok[b] * row_elems + (int64_t)j * p.block_size * p.head_dim;
+    const int per_kv = p.n_heads * rows * per_row, total = 2 * per_kv;
+    for (int v0 = tid; v0 < total; v0 += kThreads * kUnroll) {
+      uint2 codes[kUnroll];
+      uint8_t e[kUnroll];
+      int64_t dst[kUnroll];
+      int plane[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int v = v0 + u * kThreads;
+        if (v >= total) continue;
+        plane[u] = v >= per_kv;
+        const int x = v - plane[u] * per_kv;
+        const int r = x / per_row, d = (x - r * per_row) * N, h = r / rows, t = r - h * rows;
+        const uint8_t* src = p.pool[plane[u]] + src0 + ((int64_t)h * p.block_size + t) * p.head_dim + d;
+        e[u] = sc[(h * 2 + plane[u]) * p.block_size + t];
+        if constexpr (N == 8) codes[u] = *reinterpret_cast<const uint2*>(src);
+        else if constexpr (N == 4) codes[u].x = *reinterpret_cast<const uint32_t*>(src);
+        else codes[u].x = *src;
+        dst[u] = dst0 + ((int64_t)h * len + t) * p.head_dim + d;
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (v0 + u * kThreads >= total) continue;
+        const float s = __uint_as_float((uint32_t)e[u] << 23);
+        T y[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint32_t w = i < 4 ? codes[u].x : codes[u].y;
+          const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(w >> (8 * (i & 3))), __NV_E4M3);
+          y[i] = dequant<T>(__half2float(__half(hr)), s);
+        }
+        T* out = reinterpret_cast<T*>(p.out[plane[u]] + layer * p.out_layer_stride) + dst[u];
+        if constexpr (kVec) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(y);
+        else *out = y[0];
+      }
+    }
+  }
+}
+
+inline bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
+
+template <typename T>
+int launch_quant_append(const ChunkAppendParams& p, int n_layers, cudaStream_t st) {
+  const int row_bytes = p.head_dim * (int)sizeof(T);
+  const bool vec = aligned16(p.in[0]) && aligned16(p.in[1]) && aligned16(p.pool[0]) && aligned16(p.pool[1]) &&
+                   p.in_stride_layer % 16 == 0 && p.in_stride_seq % 16 == 0 && p.in_stride_head % 16 == 0 &&
+                   p.in_stride_tok % 16 == 0 && p.pool_layer_stride % 8 == 0;
+  const int64_t rows = (int64_t)p.total * p.n_heads;
+  const auto go = [&](auto kernel, int per_cta) -> int {
+    const int64_t want = (rows + per_cta - 1) / per_cta;
+    const int planes = 2 * n_layers;
+    const int64_t cap = ((int64_t)num_sms() * 8 + planes - 1) / planes;  // about one wave over all planes
+    kernel<<<dim3((unsigned)(want < cap ? want : cap), planes), kThreads, 0, st>>>(p);
+    return cuda_status(cudaGetLastError(), "kv_append_chunk launch");
+  };
+  if (vec && row_bytes == 32 * 16) return go(quant_append_kernel<T, 32>, kThreads / 32);
+  if (vec && row_bytes == 16 * 16) return go(quant_append_kernel<T, 16>, kThreads / 16);
+  if (vec && row_bytes == 8 * 16) return go(quant_append_kernel<T, 8>, kThreads / 8);
+  return go(quant_append_any_kernel<T>, kThreads / 32);
+}
+
+template <typename Tin>
+int launch_plain_append(const ChunkAppendParams& p, int pool_dtype, int n_layers, cudaStream_t st) {
+  const int64_t want = ((int64_t)p.total * p.n_heads + kThreads / 32 - 1) / (kThreads / 32);
+  const int planes = 2 * n_layers;
+  const int64_t cap = ((int64_t)num_sms() * 8 + planes - 1) / planes;
+  const dim3 grid((unsigned)(want < cap ? want : cap), planes);
+  switch (pool_dtype) {
+    case SNAPMIND_DTYPE_F32: chunk_append_kernel<Tin, float><<<grid, kThreads, 0, st>>>(p); break;
+    case SNAPMIND_DTYPE_BF16: chunk_append_kernel<Tin, __nv_bfloat16><<<grid, kThreads, 0, st>>>(p); break;
+    default: chunk_append_kernel<Tin, __half><<<grid, kThreads, 0, st>>>(p); break;
+  }
+  return cuda_status(cudaGetLastError(), "kv_append_chunk launch");
+}
+
+}  // namespace
+}  // namespace snapmind
+
+using namespace snapmind;
+
+extern "C" {
+
+int snapmind_kv_append_chunk(void* k_pool, void* v_pool, void* scales, int pool_dtype, int64_t pool_layer_stride,
+                             int64_t scale_layer_stride, const void* k_new, const void* v_new, int in_dtype,
+                             int64_t in_stride_layer, int64_t in_stride_seq, int64_t in_stride_head,
+                             int64_t in_stride_tok, const int32_t* block_tables, int64_t table_stride_seq,
+                             int32_t table_width, const int32_t* slot_starts, int32_t slot_start0,
+                             const int32_t* cu_new, int32_t n_layers, int32_t batch, int32_t n_tokens,
+                             int32_t total_new, int32_t n_heads, int32_t head_dim, int32_t block_size,
+                             int32_t num_blocks, int32_t* err_word, void* stream) {
+  const int esz_in = dtype_size(in_dtype);
+  const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
+  const int esz = quant ? 1 : dtype_size(pool_dtype);
+  SNAPMIND_CHECK_ARG(esz_in > 0 && esz > 0, "kv_append_chunk: unknown dtype");
+  SNAPMIND_CHECK_ARG(n_layers >= 0 && n_layers <= 32767 && batch >= 0 && n_tokens >= 0 && total_new >= 0 &&
+                         n_heads > 0 && head_dim > 0 && block_size > 0 && num_blocks > 0 && table_width >= 0,
+                     "kv_append_chunk: bad sizes");
+  SNAPMIND_CHECK_ARG(cu_new != nullptr || (int64_t)batch * n_tokens == total_new,
+                     "kv_append_chunk: without cu_new total_new is batch * n_tokens");
+  SNAPMIND_CHECK_ARG((int64_t)total_new * n_heads < (1LL << 31), "kv_append_chunk: too many rows");
+  SNAPMIND_CHECK_ARG(quant == (scales != nullptr), "kv_append_chunk: scales go with an e4m3 pool, and only with one");
+  if (n_layers == 0 || batch == 0 || total_new == 0) return SNAPMIND_OK;
+  SNAPMIND_CHECK_ARG(k_pool && v_pool && k_new && v_new && block_tables, "kv_append_chunk: null pointer");
+  ChunkAppendParams p;
+  p.pool[0] = static_cast<uint8_t*>(k_pool);
+  p.pool[1] = static_cast<uint8_t*>(v_pool);
+  p.scales = static_cast<uint8_t*>(scales);
+  p.in[0] = static_cast<const char*>(k_new);
+  p.in[1] = static_cast<const char*>(v_new);
+  p.pool_layer_stride = pool_layer_stride * esz;
+  p.scale_layer_stride = scale_layer_stride;
+  p.in_stride_layer = in_stride_layer * esz_in;
+  p.in_stride_seq = in_stride_seq * esz_in;
+  p.in_stride_head = in_stride_head * esz_in;
+  p.in_stride_tok = in_stride_tok * esz_in;
+  p.tables = block_tables;
+  p.table_stride = table_stride_seq;
+  p.table_width = table_width;
+  p.slot_starts = slot_starts;
+  p.slot_start0 = slot_start0;
+  p.cu = cu_new;
+  p.batch = batch;
+  p.n_tokens = n_tokens;
+  p.total = total_new;
+  p.n_heads = n_heads;
+  p.head_dim = head_dim;
+  p.block_size = block_size;
+  p.num_blocks = num_blocks;
+  // neighbouring teams walk the axis whose rows are neighbours in the input
+  p.heads_inner = cu_new != nullptr || p.in_stride_head < p.in_stride_tok;
+  p.err = err_word;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (in_dtype) {
+    case SNAPMIND_DTYPE_F32:
+      return quant ? launch_quant_append<float>(p, n_layers, st) : launch_plain_append<float>(p, pool_dtype, n_layers, st);
+    case SNAPMIND_DTYPE_BF16:
+      return quant ? launch_quant_append<__nv_bfloat16>(p, n_layers, st)
+                   : launch_plain_append<__nv_bfloat16>(p, pool_dtype, n_layers, st);
+    default:
+      return quant ? launch_quant_append<__half>(p, n_layers, st)
+                   : launch_plain_append<__half>(p, pool_dtype, n_layers, st);
+  }
+}
+
+int snapmind_kv_gather_quant(const void* k_pool, const void* v_pool, const void* scales, int64_t pool_layer_stride,
+                             int64_t scale_layer_stride, void* k_out, void* v_out, int out_dtype,
+                             int64_t out_layer_stride, int64_t out_layer_capacity, const int32_t* block_tables,
+                             int64_t table_stride_seq, int32_t table_width, const int32_t* seq_lens,
+                             int32_t n_layers, int32_t batch, int32_t n_heads, int32_t head_dim, int32_t block_size,
+                             int32_t num_blocks, int32_t* err_word, void* stream) {
+  const int esz = dtype_size(out_dtype);
+  SNAPMIND_CHECK_ARG(esz > 0, "kv_gather_quant: unknown dtype");
+  SNAPMIND_CHECK_ARG(n_layers >= 0 && n_layers <= 65535 && batch >= 0 && batch <= 8192 && n_heads > 0 && head_dim > 0 &&
+                         block_size > 0 && num_blocks > 0 && table_width >= 0 &&
+                         (int64_t)2 * n_heads * head_dim * block_size < (1LL << 31),
+                     "kv_gather_quant: bad sizes");
+  if (n_layers == 0 || batch == 0) return SNAPMIND_OK;
+  SNAPMIND_CHECK_ARG(k_pool && v_pool && scales && k_out && v_out && block_tables && seq_lens,
+                     "kv_gather_quant: null pointer");
+  QuantGatherParams p;
+  p.pool[0] = static_cast<const uint8_t*>(k_pool);
+  p.pool[1] = static_cast<const uint8_t*>(v_pool);
+  p.scales = static_cast<const uint8_t*>(scales);
+  p.out[0] = static_cast<char*>(k_out);
+  p.out[1] = static_cast<char*>(v_out);
+  p.pool_layer_stride = pool_layer_stride;
+  p.scale_layer_stride = scale_layer_stride;
+  p.out_layer_stride = out_layer_stride * esz;
+  p.out_capacity = out_layer_capacity;
+  p.tables = block_tables;
+  p.table_stride = table_stride_seq;
+  p.table_width = table_width;
+  p.seq_lens = seq_lens;
+  p.batch = batch;
+  p.n_heads = n_heads;
+  p.head_dim = head_dim;
+  p.block_size = block_size;
+  p.num_blocks = num_blocks;
+  p.err = err_word;
+  const bool vec = aligned16(k_pool) && aligned16(v_pool) && aligned16(k_out) && aligned16(v_out) &&
+                   head_dim * esz % 16 == 0 && p.out_layer_stride % 16 == 0 && pool_layer_stride % 8 == 0;
+  const size_t smem = 2 * sizeof(int32_t) * (size_t)(batch + 1);
+  const int cap = (num_sms() * 8 + n_layers - 1) / n_layers;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const auto go = [&](auto kernel) -> int {
+    if (smem > 48 * 1024) {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess) return cuda_status(e, "kv_gather_quant smem attribute");
+    }
+    kernel<<<dim3(cap, n_layers), kThreads, smem, st>>>(p);
+    return cuda_status(cudaGetLastError(), "kv_gather_quant launch");
+  };
+  switch (out_dtype) {
+    case SNAPMIND_DTYPE_F32: return vec ? go(quant_gather_kernel<float, true>) : go(quant_gather_kernel<float, false>);
+    case SNAPMIND_DTYPE_BF16:
+      return vec ? go(quant_gather_kernel<__nv_bfloat16, true>) : go(quant_gather_kernel<__nv_bfloat16, false>);
+    default: return vec ? go(quant_gather_kernel<__half, true>) : go(quant_gather_kernel<__half, false>);
+  }
+}
+
+}  // extern "C"

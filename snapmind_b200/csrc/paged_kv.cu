@@ -332,6 +332,7 @@ struct ReserveParams {
   int32_t* free_top;
   int32_t num_blocks;
   int32_t* err;
+  const int32_t* n_each = nullptr;  // reserve: new tokens of every sequence (NULL: n_new each)
 };
 
 // Exclusive block-wide scan of one int per thread; returns the prefix and
@@ -374,11 +375,12 @@ __global__ void __launch_bounds__(1024) kv_reserve_kernel(ReserveParams p) {
     int need = 0;
     if (b < p.batch) {
       const int old_len = p.seq_lens[b];
-      const int new_len = old_len + p.n_new;
+      const int n_new = p.n_each ? p.n_each[b] : p.n_new;
+      const int new_len = old_len + n_new;
       const int have = (old_len + p.block_size - 1) / p.block_size;
       const int want = (new_len + p.block_size - 1) / p.block_size;
       need = want - have;
-      if (want > p.table_width || old_len < 0) atomicOr(&s_bad, SNAPMIND_DEVERR_TABLE);
+      if (want > p.table_width || old_len < 0 || n_new < 0) atomicOr(&s_bad, SNAPMIND_DEVERR_TABLE);
     }
     int tot;
     block_exclusive_scan(need, &tot);
@@ -396,11 +398,12 @@ __global__ void __launch_bounds__(1024) kv_reserve_kernel(ReserveParams p) {
   int carry = 0;
   for (int base = 0; base < p.batch; base += blockDim.x) {
     const int b = base + threadIdx.x;
-    int need = 0, have = 0, old_len = 0;
+    int need = 0, have = 0, old_len = 0, n_new = 0;
     if (b < p.batch) {
       old_len = p.seq_lens[b];
+      n_new = p.n_each ? p.n_each[b] : p.n_new;
       have = (old_len + p.block_size - 1) / p.block_size;
-      need = (old_len + p.n_new + p.block_size - 1) / p.block_size - have;
+      need = (old_len + n_new + p.block_size - 1) / p.block_size - have;
     }
     int tot;
     const int pre = block_exclusive_scan(need, &tot) + carry;
@@ -408,7 +411,7 @@ __global__ void __launch_bounds__(1024) kv_reserve_kernel(ReserveParams p) {
       for (int k = 0; k < need; ++k) {
         p.tables[(int64_t)b * p.table_stride + have + k] = p.free_stack[top - 1 - (pre + k)];
       }
-      p.seq_lens[b] = old_len + p.n_new;
+      p.seq_lens[b] = old_len + n_new;
     }
     carry += tot;
   }
@@ -673,6 +676,19 @@ int snapmind_kv_reserve(int32_t* block_tables, int64_t table_stride_seq, int32_t
                   block_size, free_stack, free_top, num_blocks, err_word};
   kv_reserve_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(p);
   SNAPMIND_LAUNCH_CHECK("kv_reserve launch");
+}
+
+int snapmind_kv_reserve_each(int32_t* block_tables, int64_t table_stride_seq, int32_t table_width,
+                             int32_t* seq_lens, const int32_t* n_new, int32_t batch, int32_t block_size,
+                             int32_t* free_stack, int32_t* free_top, int32_t num_blocks, int32_t* err_word,
+                             void* stream) {
+  SNAPMIND_CHECK_ARG(batch >= 0 && block_size > 0 && table_width >= 0, "kv_reserve_each: bad sizes");
+  if (batch == 0) return SNAPMIND_OK;
+  SNAPMIND_CHECK_ARG(block_tables && seq_lens && n_new && free_stack && free_top, "kv_reserve_each: null pointer");
+  ReserveParams p{block_tables, table_stride_seq, table_width, seq_lens, nullptr, batch, 0,
+                  block_size, free_stack, free_top, num_blocks, err_word, n_new};
+  kv_reserve_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  SNAPMIND_LAUNCH_CHECK("kv_reserve_each launch");
 }
 
 int snapmind_kv_release(int32_t* block_tables, int64_t table_stride_seq, int32_t table_width,

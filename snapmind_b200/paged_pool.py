@@ -25,6 +25,8 @@ from snapmind_b200.block_pool import BlockPool
 
 
 class PagedKVPool(BlockPool):
+    quantised = False  # pool elements are the values themselves
+
     def __init__(
         self,
         n_layers: int,
@@ -41,11 +43,17 @@ class PagedKVPool(BlockPool):
         self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv_heads, head_dim
         self.dtype = dtype
         self._dcode = _lib.dtype_code(dtype)
-        shape = (n_layers, num_blocks, n_kv_heads, block_size, head_dim)
-        self.k = torch.empty(shape, dtype=dtype, device=self.device)
-        self.v = torch.empty(shape, dtype=dtype, device=self.device)
         self.layer_stride = num_blocks * n_kv_heads * block_size * head_dim
+        self.scale_layer_stride = 0
+        self._allocate((n_layers, num_blocks, n_kv_heads, block_size, head_dim))
         self._workspace = _lib.DecodeWorkspace(self.device)
+        with self._on_device():
+            self._chunk_ws = _lib.load().snapmind_paged_gqa_chunk_workspace_bytes(head_dim)
+
+    def _allocate(self, shape) -> None:
+        self._pool_code = self._dcode
+        self.k = torch.empty(shape, dtype=self.dtype, device=self.device)
+        self.v = torch.empty(shape, dtype=self.dtype, device=self.device)
 
     def append(self, layer: int | None, k_new: torch.Tensor, v_new: torch.Tensor, slot_starts=None,
                slot_start0: int | None = None) -> None:
@@ -83,7 +91,107 @@ class PagedKVPool(BlockPool):
         )  # fmt: skip
         _lib.check(status, "PagedKVPool.append")
 
+    def append_packed(self, layer: int | None, k_new: torch.Tensor, v_new: torch.Tensor,
+                      cu_new: torch.Tensor) -> None:
+        """Write the K/V rows of a ragged chunk, the ones that the last ``reserve_each``
+        made room for.
+
+        ``k_new``: ``[total, H, D]`` (layer ``layer``) or ``[L, total, H, D]``
+        (``layer=None``: layers 0 .. L-1); ``cu_new`` int32 ``[B + 1]`` on the device: sequence
+        b owns rows ``cu_new[b] .. cu_new[b + 1] - 1``, its newest tokens.
+        """
+        if k_new.dim() == 3:
+            if layer is None:
+                raise ValueError("layer is required for [total, H, D] inputs")
+            k_new, v_new = k_new.unsqueeze(0), v_new.unsqueeze(0)
+        n_layers, total = k_new.shape[:2]
+        self._append_chunk(0 if layer is None else layer, k_new, v_new, (0, 2, 1), None, cu_new, n_layers,
+                           cu_new.shape[0] - 1, 0, total, self.seq_lens.data_ptr(), 0)
+
+    def _append_chunk(self, base, k_new, v_new, axes, seq_axis, cu, n_layers, batch, n_tokens, total, starts, start0):
+        """``axes``: where the layer, head and token axes are; ``seq_axis``: the sequence axis or None."""
+        _lib.require_same("append", self.block_tables, k_new, v_new)
+        if k_new.shape != v_new.shape or k_new.dtype != v_new.dtype:
+            raise ValueError("append: k and v rows differ in shape or dtype")
+        if k_new.dim() < 4 or k_new.shape[axes[1]] != self.n_kv_heads or k_new.shape[-1] != self.head_dim:
+            raise ValueError(f"expected {self.n_kv_heads} heads of {self.head_dim}, got {tuple(k_new.shape)}")
+        if not 0 <= base <= self.n_layers - n_layers:
+            raise ValueError(f"append: layers {base} .. {base + n_layers - 1} of a pool of {self.n_layers}")
+        if batch > self.max_seqs or batch < 0:
+            raise ValueError(f"append: {batch} sequences, the pool holds {self.max_seqs}")
+        if cu is not None:
+            _lib.require_offsets("append", cu, self.block_tables)
+        if k_new.stride() != v_new.stride() or k_new.stride(-1) != 1:
+            k_new, v_new = k_new.contiguous(), v_new.contiguous()
+        st = k_new.stride()
+        row = self.layer_stride * self.k.element_size()
+        scales = self.scales.data_ptr() + base * self.scale_layer_stride if self.quantised else None
+        with self._on_device():
+            status = _lib.load().snapmind_kv_append_chunk(
+                self.k.data_ptr() + base * row, self.v.data_ptr() + base * row, scales, self._pool_code,
+                self.layer_stride, self.scale_layer_stride, k_new.data_ptr(), v_new.data_ptr(),
+                _lib.dtype_code(k_new.dtype), st[axes[0]], 0 if seq_axis is None else st[seq_axis], st[axes[1]],
+                st[axes[2]], self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq,
+                starts, start0, None if cu is None else cu.data_ptr(), n_layers, batch, n_tokens, total,
+                self.n_kv_heads, self.head_dim, self.block_size, self.num_blocks, self.err.data_ptr(), self._stream(),
+            )  # fmt: skip
+        _lib.check(status, f"{type(self).__name__}.append")
+
     # ----------------------------------------------------------------- reads
+    def attend_chunk(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor, out: torch.Tensor | None = None,
+                     scale: float | None = None, window: int = 0, sinks: int = 0,
+                     force_generic: bool = False) -> torch.Tensor:
+        """Causal attention of a ragged chunk of new tokens against layer ``layer``, in
+        one launch: pieces of prompts, drafted tokens and single tokens together.
+
+        ``q``/``out``: ``[total, Hq, D]``; ``cu_q`` int32 ``[B + 1]`` on the device: sequence
+        b's new tokens are rows ``cu_q[b] .. cu_q[b + 1] - 1`` (none when equal), already
+        stored in the pool as its newest.  With ``window`` > 0 a query sees the
+        ``window`` positions up to its own and the first ``sinks``.  Rows of ``out`` that
+        belong to no sequence are left as they were (whatever a new ``out`` holds)."""
+        _lib.require_offsets("attend_chunk", cu_q, self.block_tables)
+        if cu_q.shape[0] - 1 > self.max_seqs:
+            raise ValueError(f"attend_chunk: {cu_q.shape[0] - 1} sequences, the pool holds {self.max_seqs}")
+        return self._attend(layer, q, cu_q, out, scale, window, sinks,
+                            _lib.DECODE_FORCE_GENERIC if force_generic else 0)
+
+    def _attend(self, layer, q, cu, out, scale, window, sinks, flags):
+        total, n_q, d = q.shape
+        if q.dtype != self.dtype:
+            raise TypeError(f"q dtype {q.dtype} != pool dtype {self.dtype}")
+        if d != self.head_dim:
+            raise ValueError(f"q head dim {d} != the pool's {self.head_dim}")
+        if not 0 <= layer < self.n_layers:
+            raise ValueError(f"layer {layer} of a pool of {self.n_layers}")
+        if cu is None and total > self.max_seqs:
+            raise ValueError(f"decode: {total} sequences, the pool holds {self.max_seqs}")
+        if q.stride(-1) != 1:
+            q = q.contiguous()
+        if out is None:
+            out = torch.empty((total, n_q, d), dtype=self.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != self.dtype or out.stride(-1) != 1:
+            raise ValueError("out must have q's shape and dtype, head dim contiguous")
+        _lib.require_same("attend", self.block_tables, q, out)
+        lib = _lib.load()
+        # a workspace of its own for every call: calls on several streams, or in several
+        # captured graphs, never share one
+        need = self._chunk_ws
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        step = layer * self.layer_stride * self.k.element_size()
+        scales = self.scales.data_ptr() + layer * self.scale_layer_stride if self.quantised else None
+        with self._on_device():
+            status = lib.snapmind_paged_gqa_chunk(
+                q.data_ptr(), q.stride(0), q.stride(1), self._dcode, self.k.data_ptr() + step,
+                self.v.data_ptr() + step, scales, self._pool_code, self.block_tables.data_ptr(),
+                self.max_blocks_per_seq, self.max_blocks_per_seq, self.seq_lens.data_ptr(),
+                None if cu is None else cu.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+                d ** -0.5 if scale is None else scale, total if cu is None else cu.shape[0] - 1, total, n_q,
+                self.n_kv_heads, d, self.block_size, self.num_blocks, window, sinks, flags, ws.data_ptr(), need,
+                self.err.data_ptr(), self._stream(),
+            )  # fmt: skip
+        _lib.check(status, f"{type(self).__name__}.attend")
+        return out
+
     def gather(self, batch: int | None = None, layers: range | None = None, out=None):
         """Packed K/V of the first ``batch`` sequences.
 
@@ -180,8 +288,13 @@ class PagedKVPool(BlockPool):
 
     def decode(self, layer: int, q: torch.Tensor, out: torch.Tensor | None = None, scale: float | None = None,
                batch: int | None = None, split_tokens: int = 0, force_generic: bool = False,
-               max_seq_len: int | None = None, peers=None, append=None) -> torch.Tensor | None:
+               max_seq_len: int | None = None, peers=None, append=None, window: int = 0,
+               sinks: int = 0) -> torch.Tensor | None:
         """Paged GQA decode attention of ``q`` ``[B, Hq, D]`` against layer ``layer``.
+
+        With ``window`` > 0 a sequence attends to its last ``window`` tokens and its
+        first ``sinks`` tokens only, and only their blocks are read (``split_tokens``
+        and ``max_seq_len`` then have no use: the kernel plans from the device lengths).
 
         ``peers`` (a ``head_shard.PeerTargets``) sends the output rows to the
         output buffers of every rank of a head-sharded decode instead of ``out``
@@ -189,6 +302,13 @@ class PagedKVPool(BlockPool):
         dtype) stores this step's token of every sequence (the last slot the
         latest ``reserve(1)`` gave it) in the same launch, in place of an
         ``append`` call before the decode."""
+        if window or sinks:
+            if peers is not None:
+                raise ValueError("decode with a window has no peer form")
+            if append is not None:
+                self.append(layer, *append)
+            flags = _lib.DECODE_FORCE_GENERIC if force_generic else 0
+            return self._attend(layer, q if batch is None else q[:batch], None, out, scale, window, sinks, flags)
         batch = q.shape[0] if batch is None else batch
         n_q = q.shape[1]
         if peers is not None and append is not None:
