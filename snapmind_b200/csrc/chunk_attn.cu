@@ -398,6 +398,10 @@ int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stri
                      (long long)workspace_bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
+  if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && decode_sinks_supported(p, dtype, pool_dtype)) {
+    const int rc = launch_decode_sinks(p, dtype, pool_dtype, st);
+    return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
+  }
   if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && chunk_umma_supported(p, dtype, pool_dtype)) {
     const int rc = launch_chunk_umma(p, dtype, pool_dtype, st);
     return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);

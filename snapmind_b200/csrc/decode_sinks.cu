@@ -1,0 +1,558 @@
+// One token per sequence over a paged cache with a sliding window and sinks, or over an
+// 8-bit cache: head_dim 128, query groups of up to 8 heads, bf16 / f16 queries.
+//
+// HBM bound (4 flop per 16-bit byte read), so the matrix product is mma.sync with the
+// keys as M, as in paged_decode_fast.cu: S^T = K Q^T, O^T += V^T P^T, 16 keys per warp.  What
+// is different: the CTAs (two per SM) walk equal shares of the work line of chunk_plan.cuh,
+// which jumps from the sink blocks to the window's, and the pipeline runs on from
+// one unit to the next, so a batch of uneven lengths keeps every SM streaming to the end.
+//
+// e4m3 rows (c 2^e, a byte e + 127 per row): the codes become f16 in registers (exact), and
+// the scales never touch the elements: K's multiplies its key's score, V's its weight.
+// With s the score in log2 units and e_v the exponent of V's row, the reference of the running
+// softmax is M = max (s + e_v), so that the weight 2^(s + e_v - M) <= 1 that multiplies the
+// codes is a good f16 whatever the rows' scales are; the sum takes 2^(s - M).  Queries are
+// brought to [2^8, 2^9) by a power of two per head, so f16 holds a bf16 query as exactly as the
+// f32 sum needs.  Both type conversions take permuted dims (K) and pairs of dims (V), so that
+// ldmatrix can move bytes in 16-bit units:
+//   K: lane (g, t) holds dims 16 k + 4 t .. + 3 of key g as k-slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9;
+//   V: row g / g + 8 of a 16-dim step stands for dim 2 g / 2 g + 1.
+#include <cuda.h>
+#include <cuda_fp8.h>
+
+#include "chunk_plan.cuh"
+#include "sm100.cuh"
+
+namespace snapmind {
+namespace {
+
+using namespace tc;
+
+constexpr int kD = 128, kTile = 64, kConsumers = 4, kThreads = (kConsumers + 1) * 32, kHeads = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <bool kQuant> struct Stage {
+  static constexpr int kHalf = kTile * 128;                      // 64 rows of 128 bytes
+  static constexpr int kK = 0, kV = kQuant ? kHalf : 2 * kHalf;  // 16-bit rows are two halves of 64 dims
+  static constexpr int kBytes = kQuant ? 2 * kHalf : 4 * kHalf;
+  static constexpr int kCount = kQuant ? 5 : 3;
+};
+
+template <bool kQuant>
+struct Ctrl {
+  static constexpr int N = Stage<kQuant>::kCount;
+  float mo[2][kHeads][kD];
+  uint8_t scales[kQuant ? N : 1][2][kTile];  // K, V bytes of a stage's rows
+  float mm[kConsumers][kHeads], ml[kConsumers][kHeads];
+  uint64_t full[N], empty[N];
+  int32_t abort;
+  PlanShared plan;
+};
+template <bool kQuant> constexpr size_t smem_bytes() {
+  return 1024 + Stage<kQuant>::kCount * Stage<kQuant>::kBytes + sizeof(Ctrl<kQuant>);
+}
+static_assert(2 * (smem_bytes<false>() + 1024) <= 233472 && 2 * (smem_bytes<true>() + 1024) <= 233472, "two CTAs per SM");
+static_assert(Stage<true>::kCount * Stage<true>::kBytes >= kMaxChunkBatch * 4, "plan scratch in the ring");
+
+__device__ __forceinline__ void ldsm_x4(uint32_t a, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t a, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+template <bool kBf16>
+__device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (kBf16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool kBf16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (kBf16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  } else {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+}
+// two e4m3 codes in the low 16 bits -> two f16
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3);
+  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+// Byte offset of 16-byte piece `ch` (0..7) of row `row` in rows of 128 bytes, 128-byte swizzle.
+__device__ __forceinline__ uint32_t swz(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
+
+// A bulk copy of `bytes` (a multiple of 16, both addresses on 16 bytes) by the leading lane.
+__device__ __forceinline__ void bulk_load_p(uint32_t leader, uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %0, 0; @p cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%1], "
+      "[%2], %3, [%4]; }" ::"r"(leader),
+      "r"(dst), "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
+template <typename C>
+__device__ __forceinline__ bool role_wait(const C& S, uint32_t bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*reinterpret_cast<const volatile int32_t*>(&S.abort)) return false;
+    if (clock64() - t0 > kWaitTicks) return false;
+  }
+  return true;
+}
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool consumers_any(bool v) {
+  uint32_t r;
+  asm volatile("{ .reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, 1, 128, p; selp.u32 %0, 1, 0, q; }"
+               : "=r"(r)
+               : "r"((uint32_t)v)
+               : "memory");
+  return r != 0;
+}
+
+template <typename T, bool kQuant>
+__global__ void __launch_bounds__(kThreads, 2)
+    decode_sinks_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, ChunkParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  using St = Stage<kQuant>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr bool kMmaBf16 = kBf16 && !kQuant;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  auto& S = *reinterpret_cast<Ctrl<kQuant>*>(ring + St::kCount * St::kBytes);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < St::kCount; ++i) {
+      mbar_init(smem_u32(&S.full[i]), 1);
+      mbar_init(smem_u32(&S.empty[i]), kConsumers);
+    }
+    S.abort = 0;
+    mbar_init_fence();
+  }
+  plan_block(p, S.plan, reinterpret_cast<int32_t*>(ring));
+  if (tid == 0) write_piece_info(p, S.plan);
+  fence_proxy_async_smem();  // the scratch in the ring is done with before copies land there
+  __syncthreads();
+
+  PieceWalk w;
+  bool on = w.start(S.plan);
+  uint32_t tile = 0;  // running number of the CTA's tiles
+  bool ok = true;
+  if (warp == kConsumers) {
+    // ------------------------------------------------------------------ producer
+    const uint32_t leader = elect_one_sync();
+    for (; on && ok; on = w.next(p)) {
+      const Piece& c = w.c;
+      const KeyRange kr = key_range(p, c.len, c.n, c.i0, c.i0 + 1);
+      const int bs = p.block_size, box = min(bs, kTile), per_tile = kTile / box;
+      const int32_t* table = p.tables + (int64_t)c.b * p.table_stride;
+      const auto block_of = [&](int j) -> int32_t {  // block of part `lane` of tile j, or -1
+        const int v = j * kTile + lane * box;
+        if (j >= c.tile1 || lane >= per_tile || v >= kr.v_len) return -1;
+        const int lb = kr.position(v) / bs;
+        if (lb >= p.table_width) {
+          flag_error(p.err, SNAPMIND_DEVERR_TABLE);
+          return -1;
+        }
+        const int32_t phys = table[lb];
+        if (phys < 0 || phys >= p.num_blocks) {
+          flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
+          return -1;
+        }
+        return phys;
+      };
+      int32_t next = block_of(c.tile0);
+      for (int j = c.tile0; j < c.tile1; ++j, ++tile) {
+        const int32_t phys = next;
+        next = block_of(j + 1);
+        const int st = tile % St::kCount;
+        ok = __all_sync(0xffffffffu, role_wait(S, smem_u32(&S.empty[st]), ((tile / St::kCount) & 1) ^ 1));
+        if (!ok) break;
+        const int off = bs > kTile ? kr.position(j * kTile) % bs : 0;
+        const uint32_t have = __ballot_sync(0xffffffffu, phys >= 0);
+        const uint32_t bar = smem_u32(&S.full[st]);
+        const uint32_t row_bytes = kQuant ? 2 * 128 + 2 : 4 * 128;
+        mbar_arrive_expect_tx_p(leader, bar, __popc(have) * (uint32_t)box * row_bytes);
+        const uint32_t dst = smem_u32(ring + st * St::kBytes);
+        for (int x = 0; x < per_tile; ++x) {
+          if (!(have >> x & 1)) continue;
+          const int32_t tl = __shfl_sync(0xffffffffu, phys, x) * p.n_kv_heads + c.kvh;
+          const int y = tl * bs + off;
+          const uint32_t ro = x * box * 128;
+          if constexpr (kQuant) {
+            tma_load_2d_p(leader, dst + St::kK + ro, &k_map, 0, y, bar);
+            tma_load_2d_p(leader, dst + St::kV + ro, &v_map, 0, y, bar);
+            const uint8_t* sc = p.scales + (int64_t)tl * 2 * bs + off;
+            bulk_load_p(leader, smem_u32(&S.scales[st][0][x * box]), sc, box, bar);
+            bulk_load_p(leader, smem_u32(&S.scales[st][1][x * box]), sc + bs, box, bar);
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              tma_load_2d_p(leader, dst + St::kK + h * St::kHalf + ro, &k_map, 64 * h, y, bar);
+              tma_load_2d_p(leader, dst + St::kV + h * St::kHalf + ro, &v_map, 64 * h, y, bar);
+            }
+          }
+        }
+      }
+    }
+    if (!ok && lane == 0) {
+      flag_error(p.err, SNAPMIND_DEVERR_TIMEOUT);
+      atomicExch(&S.abort, 1);
+    }
+    // every copy issued lands (bounded) before the shared memory goes
+    for (uint32_t i = tile > St::kCount ? tile - St::kCount : 0; i < tile; ++i)
+      mbar_wait(smem_u32(&S.full[i % St::kCount]), (i / St::kCount) & 1);
+  } else {
+    // ------------------------------------------------------------------ consumers
+    const int g = lane >> 2, tig = lane & 3;
+    const int lrow = (lane & 7) + ((lane >> 3) & 1) * 8, lchk = lane >> 4;
+    const int vrow = (lane & 7) + ((lane >> 4) & 1) * 8, vchk = (lane >> 3) & 1;  // 16-bit V
+    const bool flip = p.scale < 0.f;  // folded into Q: the largest score has the largest weight
+    const float c2 = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
+    for (; on; on = w.next(p)) {
+      const Piece& c = w.c;
+      const KeyRange kr = key_range(p, c.len, c.n, c.i0, c.i0 + 1);
+      const int heads = slice_heads(p, c.slice), head0 = c.kvh * p.group + c.slice * p.gw;
+      // keys seen: [0, v_s) and [v_lo, v_len) of the virtual axis
+      const int v_lo = kr.win_lo - kr.shift, v_s = p.window > 0 ? min(p.sinks, kr.v_sink) : 0;
+      uint32_t qf[8][2];
+      float q0 = c2, q1 = c2;  // factors of heads 2 tig, 2 tig + 1
+      {
+        const T* qrow = reinterpret_cast<const T*>(p.q) + (int64_t)c.q_first * p.q_stride_tok +
+                        (int64_t)(head0 + min(g, heads - 1)) * p.q_stride_head;
+        if constexpr (kQuant) {
+          float x[32], a = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              x[4 * k + i] = Conv<T>::to_f(qrow[16 * k + 4 * tig + i]);
+              a = fmaxf(a, fabsf(x[4 * k + i]));
+            }
+          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+          // a 2^-e in [2^8, 2^9); 0 and what is not finite keep any e
+          const int e = min(max((int)(__float_as_uint(a) >> 23) - 127, -110), 127) - 8;
+          const float up = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) qf[k][i] = pack2<false>(x[4 * k + 2 * i] * up, x[4 * k + 2 * i + 1] * up);
+          const float f = c2 * __uint_as_float((uint32_t)(127 + e) << 23);  // of head g
+          q0 = __shfl_sync(0xffffffffu, f, 8 * tig);
+          q1 = __shfl_sync(0xffffffffu, f, 8 * tig + 4);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) qf[k][i] = *reinterpret_cast<const uint32_t*>(qrow + 16 * k + 8 * i + 2 * tig);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (g >= heads) qf[k][i] = 0u;
+            if (flip) qf[k][i] ^= 0x80008000u;
+          }
+      }
+      float o[8][4];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
+      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // log2 units
+      for (int j = c.tile0; j < c.tile1; ++j, ++tile) {
+        const int st = tile % St::kCount;
+        ok = __all_sync(0xffffffffu, role_wait(S, smem_u32(&S.full[st]), (tile / St::kCount) & 1));
+        if (!ok) break;
+        uint8_t* stage = ring + st * St::kBytes;
+        const uint32_t kb = smem_u32(stage + St::kK), vb = smem_u32(stage + St::kV);
+        const int v0 = j * kTile + 16 * warp;
+        const auto seen = [&](int i) { return v0 + i < kr.v_len && (v0 + i >= v_lo || v0 + i < v_s); };
+        const bool all = v0 + 16 <= kr.v_len && (v0 >= v_lo || v0 + 16 <= v_s);
+        if (all || __any_sync(0xffffffffu, seen(lane & 15))) {
+          if (!all) {
+            // rows of V that are not seen become zeros: 0 x (whatever lies there) must not reach O
+            for (int e = lane; e < 16 * 8; e += 32) {
+              const int i = e >> 3;
+              if (!seen(i)) {
+                const uint32_t off = swz(16 * warp + i, e & 7);
+                *reinterpret_cast<uint4*>(stage + St::kV + off) = make_uint4(0, 0, 0, 0);
+                if (!kQuant) *reinterpret_cast<uint4*>(stage + St::kV + St::kHalf + off) = make_uint4(0, 0, 0, 0);
+              }
+            }
+            __syncwarp();
+          }
+          // ---- S^T = K Q^T: 16 keys x 8 heads; keys g and g + 8, heads 2 tig, 2 tig + 1
+          float sc[4] = {0.f, 0.f, 0.f, 0.f};
+          float sv0 = 0.f, sv1 = 0.f;  // exponents of V's rows g, g + 8
+          if constexpr (kQuant) {
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) {
+              uint32_t r[4];
+              ldsm_x4(kb + swz(16 * warp + lrow, k + lchk), r);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t a[4] = {codes_f16(r[2 * i] & 0xFFFF), codes_f16(r[2 * i + 1] & 0xFFFF),
+                                       codes_f16(r[2 * i] >> 16), codes_f16(r[2 * i + 1] >> 16)};
+                mma16816<false>(sc, a, qf[k + i][0], qf[k + i][1]);
+              }
+            }
+            const uint8_t* bytes = &S.scales[st][0][16 * warp];
+            const float k0 = __uint_as_float((uint32_t)bytes[g] << 23), k1 = __uint_as_float((uint32_t)bytes[g + 8] << 23);
+            sv0 = (float)((int)bytes[kTile + g] - 127);
+            sv1 = (float)((int)bytes[kTile + g + 8] - 127);
+            sc[0] = fmaf(sc[0] * k0, q0, sv0);  // s + e_v
+            sc[1] = fmaf(sc[1] * k0, q1, sv0);
+            sc[2] = fmaf(sc[2] * k1, q0, sv1);
+            sc[3] = fmaf(sc[3] * k1, q1, sv1);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              uint32_t a[4];
+              ldsm_x4(kb + (k >> 2) * St::kHalf + swz(16 * warp + lrow, (k & 3) * 2 + lchk), a);
+              mma16816<kMmaBf16>(sc, a, qf[k][0], qf[k][1]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[i] *= c2;
+          }
+          if (!all) {
+            if (!seen(g)) {
+              sc[0] = sc[1] = -INFINITY;
+              sv0 = 0.f;
+            }
+            if (!seen(g + 8)) {
+              sc[2] = sc[3] = -INFINITY;
+              sv1 = 0.f;
+            }
+          }
+          float t0 = fmaxf(sc[0], sc[2]), t1 = fmaxf(sc[1], sc[3]);
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, off));
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
+          }
+          // some key of the 16 is seen, so the new maxima are not -inf (NaN scores aside)
+          const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+          const float a0 = ex2(m0 - n0), a1 = ex2(m1 - n1);
+          m0 = n0;
+          m1 = n1;
+          const float p0 = ex2(sc[0] - n0), p1 = ex2(sc[1] - n1), p2 = ex2(sc[2] - n0), p3 = ex2(sc[3] - n1);
+          if constexpr (kQuant) {
+            const float d0 = ex2(-sv0), d1 = ex2(-sv1);  // whole exponents: exact
+            l0 = fmaf(p0, d0, fmaf(p2, d1, l0 * a0));
+            l1 = fmaf(p1, d0, fmaf(p3, d1, l1 * a1));
+          } else {
+            l0 = l0 * a0 + p0 + p2;
+            l1 = l1 * a1 + p1 + p3;
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            o[k][0] *= a0;
+            o[k][1] *= a1;
+            o[k][2] *= a0;
+            o[k][3] *= a1;
+          }
+          // ---- P^T as the B operand: lane (g, tig) needs keys 2 tig, + 1, + 8, + 9 of head g
+          const uint32_t pr01 = pack2<kMmaBf16>(p0, p1), pr23 = pack2<kMmaBf16>(p2, p3);
+          const int src = 8 * tig + (g >> 1);
+          const uint32_t x = __shfl_sync(0xffffffffu, pr01, src), y = __shfl_sync(0xffffffffu, pr01, src + 4);
+          const uint32_t z = __shfl_sync(0xffffffffu, pr23, src), u = __shfl_sync(0xffffffffu, pr23, src + 4);
+          const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
+          const uint32_t pb0 = __byte_perm(x, y, sel), pb1 = __byte_perm(z, u, sel);
+          // ---- O^T += V^T P^T: 128 dims x 8 heads
+          if constexpr (kQuant) {
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) {
+              uint32_t r[4];
+              ldsm_x4_t(vb + swz(16 * warp + lrow, k + lchk), r);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t e0 = __byte_perm(r[2 * i], 0, 0x3120), e1 = __byte_perm(r[2 * i + 1], 0, 0x3120);
+                const uint32_t a[4] = {codes_f16(e0 & 0xFFFF), codes_f16(e0 >> 16), codes_f16(e1 & 0xFFFF),
+                                       codes_f16(e1 >> 16)};
+                mma16816<false>(o[k + i], a, pb0, pb1);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              uint32_t a[4];
+              ldsm_x4_t(vb + (k >> 2) * St::kHalf + swz(16 * warp + vrow, (k & 3) * 2 + vchk), a);
+              mma16816<kMmaBf16>(o[k], a, pb0, pb1);
+            }
+          }
+          if (!all) fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&S.empty[st]));
+      }
+      // ---- the four warps' states, merged; every consumer takes these barriers
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+      }
+      if (g == 0) {
+        S.mm[warp][2 * tig] = m0;
+        S.mm[warp][2 * tig + 1] = m1;
+        S.ml[warp][2 * tig] = l0;
+        S.ml[warp][2 * tig + 1] = l1;
+      }
+      if (consumers_any(!ok)) {
+        ok = false;
+        break;
+      }
+      float M0 = -INFINITY, M1 = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < kConsumers; ++x) {
+        M0 = fmaxf(M0, S.mm[x][2 * tig]);
+        M1 = fmaxf(M1, S.mm[x][2 * tig + 1]);
+      }
+      const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - M0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - M1);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        o[k][0] *= f0;
+        o[k][1] *= f1;
+        o[k][2] *= f0;
+        o[k][3] *= f1;
+      }
+      const int slot = warp & 1;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // warps 2 and 3 write, then 0 and 1 add theirs
+        if ((warp >= 2) == (half == 0)) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int d0 = 16 * k + (kQuant ? 2 * g : g), d1 = d0 + (kQuant ? 1 : 8);
+            float* r0 = S.mo[slot][2 * tig];
+            float* r1 = S.mo[slot][2 * tig + 1];
+            if (half == 0) {
+              r0[d0] = o[k][0];
+              r1[d0] = o[k][1];
+              r0[d1] = o[k][2];
+              r1[d1] = o[k][3];
+            } else {
+              r0[d0] += o[k][0];
+              r1[d0] += o[k][1];
+              r0[d1] += o[k][2];
+              r1[d1] += o[k][3];
+            }
+          }
+        }
+        consumers_sync();
+      }
+      const int h = tid >> 4, d = (tid & 15) * 8;  // a head's 8 dims per thread
+      if (h < heads) {
+        float M = -INFINITY, L = 0.f, x[8];
+#pragma unroll
+        for (int i = 0; i < kConsumers; ++i) M = fmaxf(M, S.mm[i][h]);
+#pragma unroll
+        for (int i = 0; i < kConsumers; ++i) L += S.mm[i][h] == -INFINITY ? 0.f : S.ml[i][h] * ex2(S.mm[i][h] - M);
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          const float4 a = *reinterpret_cast<const float4*>(&S.mo[0][h][d + i]);
+          const float4 b = *reinterpret_cast<const float4*>(&S.mo[1][h][d + i]);
+          x[i] = a.x + b.x;
+          x[i + 1] = a.y + b.y;
+          x[i + 2] = a.z + b.z;
+          x[i + 3] = a.w + b.w;
+        }
+        if (c.whole()) {
+          const float inv = M == -INFINITY ? 0.f : 1.f / L;  // nothing seen: zeros
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= inv;
+          T* out = reinterpret_cast<T*>(p.out) + (int64_t)c.q_first * p.out_stride_tok + (int64_t)(head0 + h) * p.out_stride_head + d;
+          *reinterpret_cast<uint4*>(out) = make_uint4(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]),
+                                                      pack2<kBf16>(x[4], x[5]), pack2<kBf16>(x[6], x[7]));
+        } else {
+          const int64_t row = part_slot(c) * p.rows + h;
+          if (d == 0) {
+            p.part_ml[row * 2] = M;
+            p.part_ml[row * 2 + 1] = L;
+          }
+          *reinterpret_cast<float4*>(p.part_o + row * kD + d) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4*>(p.part_o + row * kD + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        }
+      }
+      // the next piece's mm and ml are written after its own barrier-free part only once every
+      // thread has read these
+      consumers_sync();
+    }
+    if (!ok && lane == 0) {
+      flag_error(p.err, SNAPMIND_DEVERR_TIMEOUT);
+      atomicExch(&S.abort, 1);
+    }
+  }
+  __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Rows of 128 e4m3 codes, boxes of whole rows with the 128-byte swizzle.
+bool tensor_map_codes(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {kD, rows};
+  const cuuint64_t strides[1] = {kD};
+  const cuuint32_t box[2] = {kD, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, bool kQuant>
+int launch(const ChunkParams& p, cudaStream_t st) {
+  CUtensorMap k_map, v_map;
+  const uint64_t rows = (uint64_t)p.num_blocks * p.n_kv_heads * p.block_size;
+  const uint32_t box = p.block_size < kTile ? p.block_size : kTile;
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  const bool mapped = kQuant ? tensor_map_codes(&k_map, p.k_pool, rows, box) && tensor_map_codes(&v_map, p.v_pool, rows, box)
+                             : tensor_map_2d(&k_map, bf16, p.k_pool, kD, rows, kD * 2, 64, box) &&
+                                   tensor_map_2d(&v_map, bf16, p.v_pool, kD, rows, kD * 2, 64, box);
+  if (!mapped) {
+    set_last_error("paged_chunk: tensor map encoding failed");
+    return SNAPMIND_ERR_CUDA;
+  }
+  auto kernel = decode_sinks_kernel<T, kQuant>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<kQuant>());
+  if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
+  kernel<<<p.n_ctas, kThreads, smem_bytes<kQuant>(), st>>>(k_map, v_map, p);
+  return cuda_status(cudaGetLastError(), "paged_chunk launch");
+}
+
+}  // namespace
+
+// One query per sequence, groups of at most 8 heads (the N of an MMA); blocks of 16, 32 or 64
+// tokens or a multiple of 64 (a 64-key tile is whole blocks, or lies in one; 16 bytes of scales at
+// least).  Wider groups run on the tcgen05 kernel, whose 128 rows they fill better.
+bool decode_sinks_supported(const ChunkParams& p, int dtype, int pool_dtype) {
+  if (p.cu_q != nullptr || (dtype != SNAPMIND_DTYPE_BF16 && dtype != SNAPMIND_DTYPE_F16)) return false;
+  if (p.head_dim != kD || p.group > kHeads) return false;
+  const int bs = p.block_size;
+  if (bs != 16 && bs != 32 && bs % 64 != 0) return false;
+  const auto a16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+  if (!a16(p.q) || !a16(p.out) || !a16(p.k_pool) || !a16(p.v_pool)) return false;
+  if (p.q_stride_tok % 8 || p.q_stride_head % 8 || p.out_stride_tok % 8 || p.out_stride_head % 8) return false;
+  if ((int64_t)p.num_blocks * p.n_kv_heads * bs >= (int64_t)1 << 31) return false;  // TMA row coordinate
+  if (pool_dtype == SNAPMIND_DTYPE_E4M3 && !a16(p.scales)) return false;
+  return encode_tiled() != nullptr;
+}
+
+int launch_decode_sinks(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st) {
+  plan_geometry(p, kHeads, kTile, 2 * num_sms());
+  p.tokens = 1;
+  const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
+  if (dtype == SNAPMIND_DTYPE_BF16)
+    return quant ? launch<__nv_bfloat16, true>(p, st) : launch<__nv_bfloat16, false>(p, st);
+  return quant ? launch<__half, true>(p, st) : launch<__half, false>(p, st);
+}
+
+}  // namespace snapmind
