@@ -247,43 +247,94 @@ __global__ void __launch_bounds__(kGenThreads) chunk_generic_kernel(ChunkParams 
 
 // Merge of the cut units: block (c, y) works when CTA c holds the first cut inside a
 // unit, on rows y, y + gridDim.y, ...; pieces are CTA c - 1's slot 1, then slot 0 of CTAs
-// c .. last.  One warp per row: M = max m_i, out = sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M).
-constexpr int kMergeWarps = 4;
+// c .. last.  One warp per row, a lane per 4 dims (and 128 more): M = max m_i,
+// out = sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M).  32 pieces at a time: lane i holds
+// piece i's weight, and the rows of 8 pieces are in flight together (one at a time, the merge of
+// the 17 pieces of a decode took 25 us).
+constexpr int kMergeWarps = 4, kMergeBatch = 8;
 template <typename T>
 __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkParams p) {
   // launched as a programmatic dependent of the attention kernel: complete and visible after this
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int cta = blockIdx.x + 1;
-  const int32_t* h = p.heads + (int64_t)cta * kPieceInts;
-  if (h[0] < 0 || h[4] != cta - 1) return;
-  const int b = h[0], kvh = h[1], slice = h[2], i0 = h[3], last = h[5];
+  const int4 h0 = *reinterpret_cast<const int4*>(p.heads + (int64_t)cta * kPieceInts);
+  const int2 h1 = *reinterpret_cast<const int2*>(p.heads + (int64_t)cta * kPieceInts + 4);
+  if (h0.x < 0 || h1.x != cta - 1) return;
+  const int b = h0.x, kvh = h0.y, slice = h0.z, i0 = h0.w, n_pieces = h1.y - cta + 2;
   int first;
   const int n = chunk_queries(p, b, &first);
   const int heads = slice_heads(p, slice), n_rows = (min(n, i0 + p.tokens) - i0) * p.gw;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, D = p.head_dim;
   for (int r = blockIdx.y * kMergeWarps + (threadIdx.x >> 5); r < n_rows; r += gridDim.y * kMergeWarps) {
     const int g = r % p.gw;
     if (g >= heads) continue;
-    const auto slot = [&](int c) { return ((int64_t)c * 2 + (c == cta - 1 ? 1 : 0)) * p.rows + r; };
-    float M = -INFINITY;
-    for (int c = cta - 1 + lane; c <= last; c += 32) M = fmaxf(M, p.part_ml[slot(c) * 2]);
+    const auto slot = [&](int i) { return ((int64_t)(cta - 1 + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + r; };
+    float M = -INFINITY, L = 0.f;
+    float4 acc[2] = {};
+    for (int i0_ = 0; i0_ < n_pieces; i0_ += 32) {
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (i0_ + lane < n_pieces) ml = *reinterpret_cast<const float2*>(p.part_ml + slot(i0_ + lane) * 2);
+      float mb = ml.x;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    for (int c = cta - 1 + lane; c <= last; c += 32) L += p.part_ml[slot(c) * 2 + 1] * exp2f(p.part_ml[slot(c) * 2] - ref);
+      for (int o = 16; o > 0; o >>= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+      mb = fmaxf(mb, M);
+      const float ref = mb == -INFINITY ? 0.f : mb, old = ex2(M - ref);
+      M = mb;
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - ref);
+      float ls = ml.y * f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
+      L = L * old + ls;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        acc[c].x *= old;
+        acc[c].y *= old;
+        acc[c].z *= old;
+        acc[c].w *= old;
+      }
+      const int here = min(32, n_pieces - i0_);
+      for (int k = 0; k < here; k += kMergeBatch) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int d = 128 * c + 4 * lane;
+          if (128 * c >= D) break;
+          float4 v[kMergeBatch];
+#pragma unroll
+          for (int u = 0; u < kMergeBatch; ++u) {
+            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k + u >= here) continue;
+            const float* o = p.part_o + slot(i0_ + k + u) * D + d;
+            if (D % 4 == 0) {
+              if (d < D) v[u] = *reinterpret_cast<const float4*>(o);
+            } else {
+              if (d < D) v[u].x = o[0];
+              if (d + 1 < D) v[u].y = o[1];
+              if (d + 2 < D) v[u].z = o[2];
+              if (d + 3 < D) v[u].w = o[3];
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < kMergeBatch; ++u) {
+            const float fu = __shfl_sync(0xffffffffu, f, (k + u) & 31);
+            if (k + u >= here || fu == 0.f) continue;  // a piece in which the row sees nothing adds nothing
+            acc[c].x = fmaf(v[u].x, fu, acc[c].x);
+            acc[c].y = fmaf(v[u].y, fu, acc[c].y);
+            acc[c].z = fmaf(v[u].z, fu, acc[c].z);
+            acc[c].w = fmaf(v[u].w, fu, acc[c].w);
+          }
+        }
+      }
+    }
     const float inv = M == -INFINITY ? 0.f : 1.f / L;
     T* out = reinterpret_cast<T*>(p.out) + (int64_t)(first + i0 + r / p.gw) * p.out_stride_tok +
              (int64_t)(kvh * p.group + slice * p.gw + g) * p.out_stride_head;
-    for (int d = lane; d < p.head_dim; d += 32) {
-      float a = 0.f;
-      for (int c = cta - 1; c <= last; ++c) {
-        const float mc = p.part_ml[slot(c) * 2];
-        if (mc != -INFINITY) a = fmaf(p.part_o[slot(c) * p.head_dim + d], exp2f(mc - ref), a);
-      }
-      out[d] = Conv<T>::from_f(M == -INFINITY ? 0.f : a * inv);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int d = 128 * c + 4 * lane;
+      const float y[4] = {acc[c].x, acc[c].y, acc[c].z, acc[c].w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (d + u < D) out[d + u] = Conv<T>::from_f(M == -INFINITY ? 0.f : y[u] * inv);
     }
   }
 }
@@ -316,7 +367,7 @@ int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st) {
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   const int used = p.gw * p.tokens;
-  cfg.gridDim = dim3(p.n_ctas - 1, (used + kMergeWarps - 1) / kMergeWarps < 16 ? (used + kMergeWarps - 1) / kMergeWarps : 16);
+  cfg.gridDim = dim3(p.n_ctas - 1, (used + kMergeWarps - 1) / kMergeWarps);
   cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = st;
   cfg.attrs = pdl;
