@@ -528,7 +528,7 @@ SNAPMIND_API int snapmind_kv_reserve_each(int32_t *block_tables, int64_t table_s
  *     [cu_new[b], cu_new[b + 1]) of the packed tokens; token i is read at
  *     layer*in_stride_layer + i*in_stride_tok + head*in_stride_head; its rows end at
  *     slot slot_starts[b] + slot_start0 (exclusive), so slot_starts = the lengths after
- *     the reserve stores them last.  Rows outside every sequence are not read.
+ *     the reserve stores them last.  Rows outside every sequence are not stored.
  * 8-bit pool: a row x of one token and head is stored as codes c and a byte
  * e + 127, e the smallest integer in [-100, 120] with max |x| <= 448 * 2^e
  * (finite values count), c = x * 2^-e rounded to e4m3, nearest even; infinities and NaN

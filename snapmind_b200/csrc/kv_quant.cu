@@ -22,6 +22,21 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Division of 0 <= n < 2^31 by a divisor known at launch: with l = ceil(log2 d) and
+// m = floor(2^(31 + l) / d) + 1, n / d = (n m) >> (31 + l), since m d - 2^(31 + l) <= d <= 2^l.
+struct FastDiv {
+  uint32_t d = 1, m = 0, s = 0;
+  FastDiv() = default;
+  explicit FastDiv(int div) : d(div) {
+    if (d == 1) return;
+    int l = 0;
+    while ((1u << l) < d) ++l;
+    m = (uint32_t)((1ull << (31 + l)) / d) + 1;
+    s = l - 1;
+  }
+  __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> s); }
+};
+
 struct ChunkAppendParams {
   uint8_t* pool[2];
   uint8_t* scales;
@@ -36,6 +51,7 @@ struct ChunkAppendParams {
   const int32_t* cu;  // [batch + 1] first row of every sequence, or NULL: n_tokens each
   int32_t batch, n_tokens, total, n_heads, head_dim, block_size, num_blocks;
   int32_t heads_inner;  // consecutive rows walk the heads (else the tokens)
+  FastDiv by_heads, by_tokens, by_block;
   int32_t* err;
 };
 
@@ -69,31 +85,43 @@ __device__ __forceinline__ void unpack(const uint4& w, float* f) {
   for (int i = 0; i < Vec<T>::N; ++i) f[i] = Conv<T>::to_f(t[i]);
 }
 
-// Row r of the (layer, K or V) plane: its source and its pool row (-1: skipped).
-__device__ __forceinline__ int64_t append_row(const ChunkAppendParams& p, int r, const char* in, const char** src) {
-  int h, i;
+// A row of the (layer, K or V) plane.
+struct AppendRow {
+  int b, i, h;  // sequence (cu_new: unknown yet), token (packed, or within the sequence), head
+};
+__device__ __forceinline__ AppendRow append_row(const ChunkAppendParams& p, int r) {
+  AppendRow a;
   if (p.heads_inner) {
-    i = r / p.n_heads;
-    h = r - i * p.n_heads;
+    a.i = p.by_heads.div(r);
+    a.h = r - a.i * p.n_heads;
+    a.b = 0;
+    if (p.cu == nullptr) {
+      a.b = p.by_tokens.div(a.i);
+      a.i -= a.b * p.n_tokens;
+    }
   } else {  // (sequence, head, token)
-    const int bh = r / p.n_tokens, t = r - bh * p.n_tokens, b = bh / p.n_heads;
-    h = bh - b * p.n_heads;
-    i = b * p.n_tokens + t;
+    const int bh = p.by_tokens.div(r);
+    a.i = r - bh * p.n_tokens;
+    a.b = p.by_heads.div(bh);
+    a.h = bh - a.b * p.n_heads;
   }
-  int b, t, n = 0;
+  return a;
+}
+__device__ __forceinline__ const char* append_src(const ChunkAppendParams& p, const char* in, const AppendRow& a) {
+  const int64_t seq = p.cu == nullptr ? (int64_t)a.b * p.in_stride_seq : 0;
+  return in + seq + (int64_t)a.i * p.in_stride_tok + (int64_t)a.h * p.in_stride_head;
+}
+// Pool row of (block, head, slot), or -1 (skipped: outside every sequence, or flagged).
+__device__ __forceinline__ int64_t append_dst(const ChunkAppendParams& p, const AppendRow& a) {
+  int b = a.b, t = a.i, n = 0;
   if (p.cu != nullptr) {
-    b = upper_bound_i32(p.cu, p.batch + 1, i) - 1;  // rows outside every sequence are not stored
+    b = upper_bound_i32(p.cu, p.batch + 1, a.i) - 1;  // rows outside every sequence are not stored
     if (b < 0 || b >= p.batch) return -1;
-    t = i - p.cu[b];
+    t = a.i - p.cu[b];
     n = p.cu[b + 1] - p.cu[b];
-    *src = in + (int64_t)i * p.in_stride_tok + (int64_t)h * p.in_stride_head;
-  } else {
-    b = i / p.n_tokens;
-    t = i - b * p.n_tokens;
-    *src = in + (int64_t)b * p.in_stride_seq + (int64_t)t * p.in_stride_tok + (int64_t)h * p.in_stride_head;
   }
   const int slot = (p.slot_starts ? p.slot_starts[b] : 0) + p.slot_start0 - n + t;
-  const int j = slot / p.block_size;
+  const int j = slot < 0 ? 0 : p.by_block.div(slot);
   if (slot < 0 || j >= p.table_width) {
     flag_error(p.err, SNAPMIND_DEVERR_TABLE);
     return -1;
@@ -103,21 +131,48 @@ __device__ __forceinline__ int64_t append_row(const ChunkAppendParams& p, int r,
     flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
     return -1;
   }
-  return ((int64_t)phys * p.n_heads + h) * p.block_size + (slot - j * p.block_size);
+  return ((int64_t)phys * p.n_heads + a.h) * p.block_size + (slot - j * p.block_size);
 }
 
 // Byte of a row's exponent: row = (block * heads + head) * block_size + slot.
-__device__ __forceinline__ int64_t scale_at(int64_t row, int bs, int kv) {
-  const int64_t tile = row / bs;
-  return (tile * 2 + kv) * bs + (row - tile * bs);
+__device__ __forceinline__ int64_t scale_at(const ChunkAppendParams& p, int64_t row, int kv) {
+  const int tile = p.by_block.div((int)row);
+  return ((int64_t)tile * 2 + kv) * p.block_size + (row - (int64_t)tile * p.block_size);
 }
 
+// Largest magnitude of a 16-byte vector as the bits of |x| (16-bit types: both halves of
+// a word hold candidates): unsigned order is the order of magnitudes, infinities and NaN
+// above all finite values.
+template <typename T> struct Bits {
+  static constexpr uint32_t kInf = std::is_same<T, float>::value ? 0x7F800000u : std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  __device__ __forceinline__ static uint32_t max2(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) return max(a, b);
+    else return __vmaxu2(a, b);
+  }
+  __device__ __forceinline__ static uint32_t of(const uint4& w) {
+    constexpr uint32_t m = sizeof(T) == 4 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
+    return max2(max2(w.x & m, w.y & m), max2(w.z & m, w.w & m));
+  }
+  __device__ __forceinline__ static uint32_t fold(uint32_t a) {
+    if constexpr (sizeof(T) == 4) return a;
+    else return max(a & 0xFFFFu, a >> 16);
+  }
+  __device__ __forceinline__ static float value(uint32_t a) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(a);
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)a));
+    else return __uint_as_float(a << 16);
+  }
+};
+
 // Rows of TEAM lanes x one 16-byte vector each (head_dim * sizeof(T) = 16 TEAM bytes).
-// blockIdx.y = layer * 2 + (K, V).  kUnroll rows of a team are loaded before the first is
-// used.
+// blockIdx.y = layer * 2 + (K, V).  A team takes kUnroll rows at a time, all loaded before a
+// block table is read.  The magnitude is reduced on the bits, two 16-bit values a word: with
+// unpacked values and a test of every element the kernel was bound by its instructions (483 us
+// for 16 x 2049 tokens x 4 layers, 807 MB).
 template <typename T, int TEAM>
 __global__ void __launch_bounds__(kThreads) quant_append_kernel(ChunkAppendParams p) {
   constexpr int N = Vec<T>::N, kUnroll = 4;
+  using B = Bits<T>;
   const int kv = blockIdx.y & 1, layer = blockIdx.y >> 1;
   const int lane = threadIdx.x % TEAM;
   const int team = (blockIdx.x * kThreads + threadIdx.x) / TEAM, teams = gridDim.x * (kThreads / TEAM);
@@ -129,38 +184,51 @@ __global__ void __launch_bounds__(kThreads) quant_append_kernel(ChunkAppendParam
   const int steps = (rows + teams * kUnroll - 1) / (teams * kUnroll);
   for (int s = 0; s < steps; ++s) {
     uint4 w[kUnroll];
-    int64_t row[kUnroll];
+    AppendRow at[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int64_t r = ((int64_t)s * kUnroll + u) * teams + team;
-      row[u] = -1;
+      at[u].h = -1;
       w[u] = make_uint4(0, 0, 0, 0);
       if (r < rows) {
-        const char* src;
-        row[u] = append_row(p, (int)r, in, &src);
-        if (row[u] >= 0) w[u] = reinterpret_cast<const uint4*>(src)[lane];
+        at[u] = append_row(p, (int)r);
+        w[u] = reinterpret_cast<const uint4*>(append_src(p, in, at[u]))[lane];
       }
     }
+    int64_t row[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) row[u] = at[u].h < 0 ? -1 : append_dst(p, at[u]);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
+      uint32_t bits = B::of(w[u]);
+#pragma unroll
+      for (int o = TEAM / 2; o > 0; o >>= 1) bits = B::max2(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+      bits = B::fold(bits);
       float f[N];
       unpack<T>(w[u], f);
-      float a = 0.f;
+      float a = B::value(bits);
+      const bool odd = bits >= B::kInf;
+      if (__any_sync(0xffffffffu, odd)) {  // an infinity or NaN in some row of the warp
+        float fa = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) a = fmaxf(a, finite_abs(f[i]));
+        for (int i = 0; i < N; ++i) fa = fmaxf(fa, finite_abs(f[i]));
 #pragma unroll
-      for (int o = TEAM / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        for (int o = TEAM / 2; o > 0; o >>= 1) fa = fmaxf(fa, __shfl_xor_sync(0xffffffffu, fa, o));
+        a = fa;
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = scaled(f[i], 1.f);
+      }
       if (row[u] < 0) continue;
       const int e = row_exponent(a);
       const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = scaled(f[i], inv);
+      for (int i = 0; i < N; ++i) f[i] *= inv;
       uint8_t* dst = pool + row[u] * p.head_dim + lane * N;
       if constexpr (N == 8)
         *reinterpret_cast<uint2*>(dst) = make_uint2(codes4(f[0], f[1], f[2], f[3]), codes4(f[4], f[5], f[6], f[7]));
       else
         *reinterpret_cast<uint32_t*>(dst) = codes4(f[0], f[1], f[2], f[3]);
-      if (lane == 0) scales[scale_at(row[u], p.block_size, kv)] = (uint8_t)(e + 127);
+      if (lane == 0) scales[scale_at(p, row[u], kv)] = (uint8_t)(e + 127);
     }
   }
 }
@@ -175,10 +243,10 @@ __global__ void __launch_bounds__(kThreads) quant_append_any_kernel(ChunkAppendP
   uint8_t* pool = p.pool[kv] + layer * p.pool_layer_stride;
   const int warps = gridDim.x * (kThreads / 32);
   for (int64_t r = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < rows; r += warps) {  // warp-uniform
-    const char* src;
-    const int64_t row = append_row(p, (int)r, in, &src);
+    const AppendRow at = append_row(p, (int)r);
+    const int64_t row = append_dst(p, at);
     if (row < 0) continue;
-    const T* x = reinterpret_cast<const T*>(src);
+    const T* x = reinterpret_cast<const T*>(append_src(p, in, at));
     float a = 0.f;
     for (int d = lane; d < p.head_dim; d += 32) a = fmaxf(a, finite_abs(Conv<T>::to_f(x[d])));
 #pragma unroll
@@ -187,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) quant_append_any_kernel(ChunkAppendP
     const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
     for (int d = lane; d < p.head_dim; d += 32)
       pool[row * p.head_dim + d] = __nv_cvt_float_to_fp8(scaled(Conv<T>::to_f(x[d]), inv), __NV_SATFINITE, __NV_E4M3);
-    if (lane == 0) p.scales[layer * p.scale_layer_stride + scale_at(row, p.block_size, kv)] = (uint8_t)(e + 127);
+    if (lane == 0) p.scales[layer * p.scale_layer_stride + scale_at(p, row, kv)] = (uint8_t)(e + 127);
   }
 }
 
@@ -201,10 +269,10 @@ __global__ void __launch_bounds__(kThreads) chunk_append_kernel(ChunkAppendParam
   Tout* pool = reinterpret_cast<Tout*>(p.pool[kv] + layer * p.pool_layer_stride);
   const int warps = gridDim.x * (kThreads / 32);
   for (int64_t r = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < rows; r += warps) {
-    const char* src;
-    const int64_t row = append_row(p, (int)r, in, &src);
+    const AppendRow at = append_row(p, (int)r);
+    const int64_t row = append_dst(p, at);
     if (row < 0) continue;
-    const Tin* x = reinterpret_cast<const Tin*>(src);
+    const Tin* x = reinterpret_cast<const Tin*>(append_src(p, in, at));
     Tout* y = pool + row * p.head_dim;
     if constexpr (std::is_same<Tin, Tout>::value) {
       if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 7) == 0 && p.head_dim * sizeof(Tin) % 8 == 0) {
@@ -231,6 +299,7 @@ struct QuantGatherParams {
   int32_t table_width;
   const int32_t* seq_lens;
   int32_t batch, n_heads, head_dim, block_size, num_blocks;
+  FastDiv by_row, by_block;  // threads of a row, slots of a block
   int32_t* err;
 };
 
@@ -240,9 +309,41 @@ __device__ __forceinline__ float dequant_top(__half) { return 65504.f; }
 
 // c 2^e, held to T's finite range (a NaN stays one)
 template <typename T>
-__device__ __forceinline__ T dequant(float c, float scale) {
-  const float y = c * scale, top = dequant_top(T());
-  return Conv<T>::from_f(fabsf(y) > top ? copysignf(top, y) : y);
+__device__ __forceinline__ float held(float y) {
+  const float top = dequant_top(T());
+  return fabsf(y) > top ? copysignf(top, y) : y;
+}
+// Largest scale byte at which no code can pass T's range: 448 2^e <= top.
+template <typename T> constexpr int plain_bytes() { return std::is_same<T, __half>::value ? 127 + 7 : 127 + 118; }
+
+// N codes (the low bytes of w) times 2^(byte - 127).
+template <typename T, int N>
+__device__ __forceinline__ void dequant(const uint32_t* w, int byte, T* y) {
+  const float s = __uint_as_float((uint32_t)byte << 23);
+  if constexpr (N == 1) {
+    const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)w[0], __NV_E4M3);
+    y[0] = Conv<T>::from_f(held<T>(__half2float(__half(h)) * s));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 4] >> (8 * (i & 3))), __NV_E4M3);
+      float2 f = __half22float2(__half2(h));
+      f.x *= s;
+      f.y *= s;
+      if (byte > plain_bytes<T>()) {
+        f.x = held<T>(f.x);
+        f.y = held<T>(f.y);
+      }
+      if constexpr (std::is_same<T, float>::value) {
+        y[i] = f.x;
+        y[i + 1] = f.y;
+      } else if constexpr (std::is_same<T, __half>::value) {
+        *reinterpret_cast<__half2*>(y + i) = __floats2half2_rn(f.x, f.y);
+      } else {
+        *reinterpret_cast<__nv_bfloat162*>(y + i) = __floats2bfloat162_rn(f.x, f.y);
+      }
+    }
+  }
 }
 
 // Work item = one block of one sequence: all its heads, K and V of one layer
@@ -314,37 +415,34 @@ __global__ void __launch_bounds__(kThreads) quant_gather_kernel(QuantGatherParam
     const uint8_t* sc = p.scales + layer * p.scale_layer_stride + (int64_t)phys * p.n_heads * 2 * p.block_size;
     const int64_t src0 = layer * p.pool_layer_stride + (int64_t)phys * p.n_heads * p.block_size * p.head_dim;
     const int64_t dst0 = (int64_t)cu_tok[b] * row_elems + (int64_t)j * p.block_size * p.head_dim;
-    const int per_kv = p.n_heads * rows * per_row, total = 2 * per_kv;
+    // rows (K or V, head, slot) of per_row threads each; slots past the sequence's end are skipped
+    const int total = 2 * p.n_heads * p.block_size * per_row;
     for (int v0 = tid; v0 < total; v0 += kThreads * kUnroll) {
-      uint2 codes[kUnroll];
-      uint8_t e[kUnroll];
+      uint32_t codes[kUnroll][2];
+      int byte[kUnroll], plane[kUnroll];
       int64_t dst[kUnroll];
-      int plane[kUnroll];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         const int v = v0 + u * kThreads;
+        byte[u] = -1;
         if (v >= total) continue;
-        plane[u] = v >= per_kv;
-        const int x = v - plane[u] * per_kv;
-        const int r = x / per_row, d = (x - r * per_row) * N, h = r / rows, t = r - h * rows;
-        const uint8_t* src = p.pool[plane[u]] + src0 + ((int64_t)h * p.block_size + t) * p.head_dim + d;
-        e[u] = sc[(h * 2 + plane[u]) * p.block_size + t];
-        if constexpr (N == 8) codes[u] = *reinterpret_cast<const uint2*>(src);
-        else if constexpr (N == 4) codes[u].x = *reinterpret_cast<const uint32_t*>(src);
-        else codes[u].x = *src;
+        const int row = p.by_row.div(v), d = (v - row * per_row) * N;
+        const int th = p.by_block.div(row), t = row - th * p.block_size;  // th: (K or V, head)
+        if (t >= rows) continue;
+        plane[u] = th >= p.n_heads;
+        const int h = th - plane[u] * p.n_heads;
+        const uint8_t* src = p.pool[plane[u]] + src0 + (int64_t)(h * p.block_size + t) * p.head_dim + d;
+        byte[u] = sc[(h * 2 + plane[u]) * p.block_size + t];
+        if constexpr (N == 8) *reinterpret_cast<uint2*>(codes[u]) = *reinterpret_cast<const uint2*>(src);
+        else if constexpr (N == 4) codes[u][0] = *reinterpret_cast<const uint32_t*>(src);
+        else codes[u][0] = *src;
         dst[u] = dst0 + ((int64_t)h * len + t) * p.head_dim + d;
       }
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        if (v0 + u * kThreads >= total) continue;
-        const float s = __uint_as_float((uint32_t)e[u] << 23);
-        T y[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint32_t w = i < 4 ? codes[u].x : codes[u].y;
-          const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(w >> (8 * (i & 3))), __NV_E4M3);
-          y[i] = dequant<T>(__half2float(__half(hr)), s);
-        }
+        if (byte[u] < 0) continue;
+        __align__(16) T y[N];
+        dequant<T, N>(codes[u], byte[u], y);
         T* out = reinterpret_cast<T*>(p.out[plane[u]] + layer * p.out_layer_stride) + dst[u];
         if constexpr (kVec) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(y);
         else *out = y[0];
@@ -413,7 +511,8 @@ int snapmind_kv_append_chunk(void* k_pool, void* v_pool, void* scales, int pool_
                      "kv_append_chunk: bad sizes");
   SNAPMIND_CHECK_ARG(cu_new != nullptr || (int64_t)batch * n_tokens == total_new,
                      "kv_append_chunk: without cu_new total_new is batch * n_tokens");
-  SNAPMIND_CHECK_ARG((int64_t)total_new * n_heads < (1LL << 31), "kv_append_chunk: too many rows");
+  SNAPMIND_CHECK_ARG((int64_t)total_new * n_heads < (1LL << 31) && (int64_t)num_blocks * n_heads * block_size < (1LL << 31),
+                     "kv_append_chunk: too many rows");
   SNAPMIND_CHECK_ARG(quant == (scales != nullptr), "kv_append_chunk: scales go with an e4m3 pool, and only with one");
   if (n_layers == 0 || batch == 0 || total_new == 0) return SNAPMIND_OK;
   SNAPMIND_CHECK_ARG(k_pool && v_pool && k_new && v_new && block_tables, "kv_append_chunk: null pointer");
@@ -443,6 +542,9 @@ int snapmind_kv_append_chunk(void* k_pool, void* v_pool, void* scales, int pool_
   p.block_size = block_size;
   p.num_blocks = num_blocks;
   // neighbouring teams walk the axis whose rows are neighbours in the input
+  p.by_heads = FastDiv(n_heads);
+  p.by_tokens = FastDiv(n_tokens > 0 ? n_tokens : 1);
+  p.by_block = FastDiv(block_size);
   p.heads_inner = cu_new != nullptr || p.in_stride_head < p.in_stride_tok;
   p.err = err_word;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -495,6 +597,8 @@ int snapmind_kv_gather_quant(const void* k_pool, const void* v_pool, const void*
   p.err = err_word;
   const bool vec = aligned16(k_pool) && aligned16(v_pool) && aligned16(k_out) && aligned16(v_out) &&
                    head_dim * esz % 16 == 0 && p.out_layer_stride % 16 == 0 && pool_layer_stride % 8 == 0;
+  p.by_row = FastDiv(vec ? head_dim * esz / 16 : head_dim);
+  p.by_block = FastDiv(block_size);
   const size_t smem = 2 * sizeof(int32_t) * (size_t)(batch + 1);
   const int cap = (num_sms() * 8 + n_layers - 1) / n_layers;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
