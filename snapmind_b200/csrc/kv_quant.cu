@@ -165,41 +165,47 @@ template <typename T> struct Bits {
 };
 
 // Rows of TEAM lanes x one 16-byte vector each (head_dim * sizeof(T) = 16 TEAM bytes).
-// blockIdx.y = layer * 2 + (K, V).  A team takes kUnroll rows at a time, all loaded before a
-// block table is read.  The magnitude is reduced on the bits, two 16-bit values a word: with
-// unpacked values and a test of every element the kernel was bound by its instructions (483 us
-// for 16 x 2049 tokens x 4 layers, 807 MB).
+// blockIdx.y = layer * 2 + (K, V).  A warp takes kRows rows a step: lane i works out where row i
+// comes from and goes to, the teams fetch that by shuffles, and kUnroll vectors a lane are in
+// flight.  The magnitude is reduced on the bits, two 16-bit values a word.  (This kernel is bound
+// by instructions first: with every lane resolving its rows, and unpacked magnitudes, 16 x
+// 2049 tokens x 4 layers took 483 us, with the bits 296 us at 228 instructions a vector.)
 template <typename T, int TEAM>
 __global__ void __launch_bounds__(kThreads) quant_append_kernel(ChunkAppendParams p) {
-  constexpr int N = Vec<T>::N, kUnroll = 4;
+  constexpr int N = Vec<T>::N, kTeams = 32 / TEAM, kUnroll = 32 / kTeams < 8 ? 32 / kTeams : 8, kRows = kTeams * kUnroll;
   using B = Bits<T>;
   const int kv = blockIdx.y & 1, layer = blockIdx.y >> 1;
-  const int lane = threadIdx.x % TEAM;
-  const int team = (blockIdx.x * kThreads + threadIdx.x) / TEAM, teams = gridDim.x * (kThreads / TEAM);
+  const int lane = threadIdx.x & 31, piece = lane % TEAM, sub = lane / TEAM;
   const int rows = p.total * p.n_heads;
   const char* in = p.in[kv] + layer * p.in_stride_layer;
-  uint8_t* pool = p.pool[kv] + layer * p.pool_layer_stride;
+  uint8_t* pool = p.pool[kv] + layer * p.pool_layer_stride + piece * N;
   uint8_t* scales = p.scales + layer * p.scale_layer_stride;
-  // every lane of a warp takes the same number of steps (the shuffles below are warp-wide)
-  const int steps = (rows + teams * kUnroll - 1) / (teams * kUnroll);
-  for (int s = 0; s < steps; ++s) {
-    uint4 w[kUnroll];
-    AppendRow at[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t r = ((int64_t)s * kUnroll + u) * teams + team;
-      at[u].h = -1;
-      w[u] = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        at[u] = append_row(p, (int)r);
-        w[u] = reinterpret_cast<const uint4*>(append_src(p, in, at[u]))[lane];
-      }
+  const int64_t stride = (int64_t)gridDim.x * (kThreads / 32) * kRows;
+  for (int64_t r0 = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kRows; r0 < rows; r0 += stride) {
+    AppendRow at;
+    const char* src = nullptr;
+    const bool mine = lane < kRows && r0 + lane < rows;
+    if (mine) {
+      at = append_row(p, (int)(r0 + lane));
+      src = append_src(p, in, at);
     }
-    int64_t row[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) row[u] = at[u].h < 0 ? -1 : append_dst(p, at[u]);
+    uint4 w[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
+      const char* from = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), u * kTeams + sub));
+      w[u] = make_uint4(0, 0, 0, 0);
+      if (from != nullptr) w[u] = __ldcs(reinterpret_cast<const uint4*>(from) + piece);
+    }
+    int row = -1;  // num_blocks * heads * block_size < 2^31
+    uint32_t scale = 0;
+    if (mine) {
+      row = (int)append_dst(p, at);
+      if (row >= 0) scale = (uint32_t)scale_at(p, row, kv);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int to = __shfl_sync(0xffffffffu, row, u * kTeams + sub);
+      const uint32_t sc = __shfl_sync(0xffffffffu, scale, u * kTeams + sub);
       uint32_t bits = B::of(w[u]);
 #pragma unroll
       for (int o = TEAM / 2; o > 0; o >>= 1) bits = B::max2(bits, __shfl_xor_sync(0xffffffffu, bits, o));
@@ -207,8 +213,7 @@ __global__ void __launch_bounds__(kThreads) quant_append_kernel(ChunkAppendParam
       float f[N];
       unpack<T>(w[u], f);
       float a = B::value(bits);
-      const bool odd = bits >= B::kInf;
-      if (__any_sync(0xffffffffu, odd)) {  // an infinity or NaN in some row of the warp
+      if (__any_sync(0xffffffffu, bits >= B::kInf)) {  // an infinity or NaN in some row of the warp
         float fa = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) fa = fmaxf(fa, finite_abs(f[i]));
@@ -218,17 +223,17 @@ __global__ void __launch_bounds__(kThreads) quant_append_kernel(ChunkAppendParam
 #pragma unroll
         for (int i = 0; i < N; ++i) f[i] = scaled(f[i], 1.f);
       }
-      if (row[u] < 0) continue;
+      if (to < 0) continue;
       const int e = row_exponent(a);
       const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] *= inv;
-      uint8_t* dst = pool + row[u] * p.head_dim + lane * N;
+      uint8_t* dst = pool + (int64_t)to * p.head_dim;
       if constexpr (N == 8)
         *reinterpret_cast<uint2*>(dst) = make_uint2(codes4(f[0], f[1], f[2], f[3]), codes4(f[4], f[5], f[6], f[7]));
       else
         *reinterpret_cast<uint32_t*>(dst) = codes4(f[0], f[1], f[2], f[3]);
-      if (lane == 0) scales[scale_at(p, row[u], kv)] = (uint8_t)(e + 127);
+      if (piece == 0) scales[sc] = (uint8_t)(e + 127);
     }
   }
 }
@@ -299,7 +304,7 @@ struct QuantGatherParams {
   int32_t table_width;
   const int32_t* seq_lens;
   int32_t batch, n_heads, head_dim, block_size, num_blocks;
-  FastDiv by_row, by_block;  // threads of a row, slots of a block
+  FastDiv by_block;
   int32_t* err;
 };
 
@@ -348,9 +353,11 @@ __device__ __forceinline__ void dequant(const uint32_t* w, int byte, T* y) {
 
 // Work item = one block of one sequence: all its heads, K and V of one layer
 // (blockIdx.y).  The items of a sequence start after those of the sequences before it; a
-// CTA finds its sequences by a scan of the lengths, kept in shared memory.  A thread
-// turns 16 / sizeof(T) codes into one 16-byte vector (kVec), or single elements.
-template <typename T, bool kVec>
+// CTA finds its sequences by a scan of the lengths, kept in shared memory.  Rows are handled
+// as in quant_append_kernel: TEAM lanes x 16 bytes of output, a lane per row resolving it (and
+// reading its scale byte); TEAM 0 is one lane per row's element, for any head_dim and
+// alignment.
+template <typename T, int TEAM>
 __global__ void __launch_bounds__(kThreads) quant_gather_kernel(QuantGatherParams p) {
   extern __shared__ int32_t cu[];  // [batch + 1] first block, then [batch + 1] first token
   int32_t* cu_tok = cu + p.batch + 1;
@@ -401,12 +408,12 @@ __global__ void __launch_bounds__(kThreads) quant_gather_kernel(QuantGatherParam
     if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) flag_error(p.err, SNAPMIND_DEVERR_TABLE);
     return;
   }
-  constexpr int N = kVec ? Vec<T>::N : 1, kUnroll = 4;
-  const int layer = blockIdx.y;
-  const int per_row = p.head_dim / N;
+  constexpr int N = TEAM ? Vec<T>::N : 1, kTeam = TEAM ? TEAM : 32, kTeams = 32 / kTeam;
+  constexpr int kUnroll = !TEAM ? 1 : 32 / kTeams < 8 ? 32 / kTeams : 8, kRows = kTeams * kUnroll;
+  const int layer = blockIdx.y, piece = lane % kTeam, sub = lane / kTeam;
   for (int it = blockIdx.x; it < cu[p.batch]; it += gridDim.x) {
     const int b = upper_bound_i32(cu, p.batch + 1, it) - 1, j = it - cu[b];
-    const int len = cu_tok[b + 1] - cu_tok[b], rows = min(p.block_size, len - j * p.block_size);
+    const int len = cu_tok[b + 1] - cu_tok[b], valid = min(p.block_size, len - j * p.block_size);
     const int32_t phys = j < p.table_width ? p.tables[(int64_t)b * p.table_stride + j] : -1;
     if (phys < 0 || phys >= p.num_blocks) {
       if (tid == 0) flag_error(p.err, j < p.table_width ? SNAPMIND_DEVERR_BLOCK_ID : SNAPMIND_DEVERR_TABLE);
@@ -415,37 +422,53 @@ __global__ void __launch_bounds__(kThreads) quant_gather_kernel(QuantGatherParam
     const uint8_t* sc = p.scales + layer * p.scale_layer_stride + (int64_t)phys * p.n_heads * 2 * p.block_size;
     const int64_t src0 = layer * p.pool_layer_stride + (int64_t)phys * p.n_heads * p.block_size * p.head_dim;
     const int64_t dst0 = (int64_t)cu_tok[b] * row_elems + (int64_t)j * p.block_size * p.head_dim;
-    // rows (K or V, head, slot) of per_row threads each; slots past the sequence's end are skipped
-    const int total = 2 * p.n_heads * p.block_size * per_row;
-    for (int v0 = tid; v0 < total; v0 += kThreads * kUnroll) {
-      uint32_t codes[kUnroll][2];
-      int byte[kUnroll], plane[kUnroll];
-      int64_t dst[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int v = v0 + u * kThreads;
-        byte[u] = -1;
-        if (v >= total) continue;
-        const int row = p.by_row.div(v), d = (v - row * per_row) * N;
-        const int th = p.by_block.div(row), t = row - th * p.block_size;  // th: (K or V, head)
-        if (t >= rows) continue;
-        plane[u] = th >= p.n_heads;
-        const int h = th - plane[u] * p.n_heads;
-        const uint8_t* src = p.pool[plane[u]] + src0 + (int64_t)(h * p.block_size + t) * p.head_dim + d;
-        byte[u] = sc[(h * 2 + plane[u]) * p.block_size + t];
-        if constexpr (N == 8) *reinterpret_cast<uint2*>(codes[u]) = *reinterpret_cast<const uint2*>(src);
-        else if constexpr (N == 4) codes[u][0] = *reinterpret_cast<const uint32_t*>(src);
-        else codes[u][0] = *src;
-        dst[u] = dst0 + ((int64_t)h * len + t) * p.head_dim + d;
+    const int rows = 2 * p.n_heads * p.block_size;  // (K or V, head, slot)
+    for (int r0 = warp * kRows; r0 < rows; r0 += kThreads / 32 * kRows) {
+      int byte = -1, plane = 0;
+      uint32_t from = 0;  // within the block: 2 * heads * head_dim * block_size < 2^31
+      int64_t to = 0;
+      const int row = r0 + lane;
+      if (lane < kRows && row < rows) {
+        const int th = p.by_block.div(row), t = row - th * p.block_size;
+        if (t < valid) {  // slots past the sequence's end are skipped
+          plane = th >= p.n_heads;
+          const int h = th - plane * p.n_heads;
+          byte = sc[(h * 2 + plane) * p.block_size + t];
+          from = (uint32_t)(h * p.block_size + t) * p.head_dim;
+          to = dst0 + ((int64_t)h * len + t) * p.head_dim;
+        }
       }
+      byte = byte < 0 ? -1 : byte | plane << 8;
+      for (int d0 = 0; d0 < p.head_dim; d0 += kTeam * N) {  // one turn with TEAM lanes a row
+        const int d = d0 + piece * N;
+        uint32_t codes[kUnroll][2];
+        int by[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (byte[u] < 0) continue;
-        __align__(16) T y[N];
-        dequant<T, N>(codes[u], byte[u], y);
-        T* out = reinterpret_cast<T*>(p.out[plane[u]] + layer * p.out_layer_stride) + dst[u];
-        if constexpr (kVec) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(y);
-        else *out = y[0];
+        for (int u = 0; u < kUnroll; ++u) {
+          by[u] = __shfl_sync(0xffffffffu, byte, u * kTeams + sub);
+          const uint32_t f = __shfl_sync(0xffffffffu, from, u * kTeams + sub);
+          if (by[u] < 0 || d >= p.head_dim) continue;
+          const uint8_t* src = p.pool[by[u] >> 8] + src0 + f + d;
+          if constexpr (N == 8) {
+            const uint2 x = __ldcs(reinterpret_cast<const uint2*>(src));
+            codes[u][0] = x.x;
+            codes[u][1] = x.y;
+          } else if constexpr (N == 4) {
+            codes[u][0] = __ldcs(reinterpret_cast<const uint32_t*>(src));
+          } else {
+            codes[u][0] = *src;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int64_t dst = __shfl_sync(0xffffffffu, to, u * kTeams + sub) + d;
+          if (by[u] < 0 || d >= p.head_dim) continue;
+          __align__(16) T y[N];
+          dequant<T, N>(codes[u], by[u] & 255, y);
+          T* out = reinterpret_cast<T*>(p.out[by[u] >> 8] + layer * p.out_layer_stride) + dst;
+          if constexpr (TEAM != 0) __stcs(reinterpret_cast<uint4*>(out), *reinterpret_cast<const uint4*>(y));
+          else *out = y[0];
+        }
       }
     }
   }
@@ -597,7 +620,6 @@ int snapmind_kv_gather_quant(const void* k_pool, const void* v_pool, const void*
   p.err = err_word;
   const bool vec = aligned16(k_pool) && aligned16(v_pool) && aligned16(k_out) && aligned16(v_out) &&
                    head_dim * esz % 16 == 0 && p.out_layer_stride % 16 == 0 && pool_layer_stride % 8 == 0;
-  p.by_row = FastDiv(vec ? head_dim * esz / 16 : head_dim);
   p.by_block = FastDiv(block_size);
   const size_t smem = 2 * sizeof(int32_t) * (size_t)(batch + 1);
   const int cap = (num_sms() * 8 + n_layers - 1) / n_layers;
@@ -610,11 +632,20 @@ int snapmind_kv_gather_quant(const void* k_pool, const void* v_pool, const void*
     kernel<<<dim3(cap, n_layers), kThreads, smem, st>>>(p);
     return cuda_status(cudaGetLastError(), "kv_gather_quant launch");
   };
+  const int team = vec ? head_dim * esz / 16 : 0;
+  const auto by_team = [&](auto t) -> int {
+    using T = decltype(t);
+    switch (team) {
+      case 8: return go(quant_gather_kernel<T, 8>);
+      case 16: return go(quant_gather_kernel<T, 16>);
+      case 32: return go(quant_gather_kernel<T, 32>);
+      default: return go(quant_gather_kernel<T, 0>);
+    }
+  };
   switch (out_dtype) {
-    case SNAPMIND_DTYPE_F32: return vec ? go(quant_gather_kernel<float, true>) : go(quant_gather_kernel<float, false>);
-    case SNAPMIND_DTYPE_BF16:
-      return vec ? go(quant_gather_kernel<__nv_bfloat16, true>) : go(quant_gather_kernel<__nv_bfloat16, false>);
-    default: return vec ? go(quant_gather_kernel<__half, true>) : go(quant_gather_kernel<__half, false>);
+    case SNAPMIND_DTYPE_F32: return by_team(float());
+    case SNAPMIND_DTYPE_BF16: return by_team(__nv_bfloat16());
+    default: return by_team(__half());
   }
 }
 
