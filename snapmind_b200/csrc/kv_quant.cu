@@ -164,15 +164,26 @@ template <typename T> struct Bits {
   }
 };
 
-// Rows of TEAM lanes x one 16-byte vector each (head_dim * sizeof(T) = 16 TEAM bytes).
-// blockIdx.y = layer * 2 + (K, V).  A warp takes kRows rows a step: lane i works out where row i
-// comes from and goes to, the teams fetch that by shuffles, and kUnroll vectors a lane are in
-// flight.  The magnitude is reduced on the bits, two 16-bit values a word.  (This kernel is bound
-// by instructions first: with every lane resolving its rows, and unpacked magnitudes, 16 x
-// 2049 tokens x 4 layers took 483 us, with the bits 296 us at 228 instructions a vector.)
+// A pair of products by one power of two (one instruction on sm_100).
+__device__ __forceinline__ float2 mul2(float2 a, float s) {
+  float2 r;
+  asm("{ .reg .b64 a, b, c; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %4}; mul.rn.f32x2 c, a, b; mov.b64 {%0, %1}, c; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(s));
+  return r;
+}
+
+// Rows of TEAM lanes x two 16-byte vectors each (head_dim * sizeof(T) = 32 TEAM bytes; a lane's
+// vectors are TEAM apart, so a team reads whole lines).  blockIdx.y = layer * 2 + (K, V).  A warp
+// takes kRows rows a step: lane i works out where row i comes from and goes to, and the teams
+// fetch that by shuffles.  The magnitude is reduced on the bits, two 16-bit values a word.
+// This kernel is bound by instructions first.  16 x 2049 tokens x 4 layers, 807 MB: 483 us with
+// every lane resolving its rows and unpacked magnitudes, 296 us with the bits (228 instructions
+// a vector), 168 us with a lane per row (124), then two vectors a lane.
 template <typename T, int TEAM>
 __global__ void __launch_bounds__(kThreads) quant_append_kernel(ChunkAppendParams p) {
-  constexpr int N = Vec<T>::N, kTeams = 32 / TEAM, kUnroll = 32 / kTeams < 8 ? 32 / kTeams : 8, kRows = kTeams * kUnroll;
+  constexpr int N = Vec<T>::N, kTeams = 32 / TEAM, kUnroll = 4, kRows = kTeams * kUnroll;
+  static_assert(kRows <= 32, "a lane per row");
   using B = Bits<T>;
   const int kv = blockIdx.y & 1, layer = blockIdx.y >> 1;
   const int lane = threadIdx.x & 31, piece = lane % TEAM, sub = lane / TEAM;
@@ -189,12 +200,15 @@ __global__ void __launch_bounds__(kThreads) quant_append_kernel(ChunkAppendParam
       at = append_row(p, (int)(r0 + lane));
       src = append_src(p, in, at);
     }
-    uint4 w[kUnroll];
+    uint4 w[kUnroll][2];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const char* from = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), u * kTeams + sub));
-      w[u] = make_uint4(0, 0, 0, 0);
-      if (from != nullptr) w[u] = __ldcs(reinterpret_cast<const uint4*>(from) + piece);
+      w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+      if (from != nullptr) {
+        w[u][0] = reinterpret_cast<const uint4*>(from)[piece];
+        w[u][1] = reinterpret_cast<const uint4*>(from)[piece + TEAM];
+      }
     }
     int row = -1;  // num_blocks * heads * block_size < 2^31
     uint32_t scale = 0;
@@ -206,33 +220,41 @@ __global__ void __launch_bounds__(kThreads) quant_append_kernel(ChunkAppendParam
     for (int u = 0; u < kUnroll; ++u) {
       const int to = __shfl_sync(0xffffffffu, row, u * kTeams + sub);
       const uint32_t sc = __shfl_sync(0xffffffffu, scale, u * kTeams + sub);
-      uint32_t bits = B::of(w[u]);
+      uint32_t bits = B::max2(B::of(w[u][0]), B::of(w[u][1]));
 #pragma unroll
       for (int o = TEAM / 2; o > 0; o >>= 1) bits = B::max2(bits, __shfl_xor_sync(0xffffffffu, bits, o));
       bits = B::fold(bits);
-      float f[N];
-      unpack<T>(w[u], f);
+      float f[2][N];
+      unpack<T>(w[u][0], f[0]);
+      unpack<T>(w[u][1], f[1]);
       float a = B::value(bits);
       if (__any_sync(0xffffffffu, bits >= B::kInf)) {  // an infinity or NaN in some row of the warp
         float fa = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) fa = fmaxf(fa, finite_abs(f[i]));
+        for (int i = 0; i < 2 * N; ++i) {
+          float& x = f[i / N][i % N];
+          fa = fmaxf(fa, finite_abs(x));
+          x = scaled(x, 1.f);
+        }
 #pragma unroll
         for (int o = TEAM / 2; o > 0; o >>= 1) fa = fmaxf(fa, __shfl_xor_sync(0xffffffffu, fa, o));
         a = fa;
-#pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = scaled(f[i], 1.f);
       }
       if (to < 0) continue;
       const int e = row_exponent(a);
       const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] *= inv;
       uint8_t* dst = pool + (int64_t)to * p.head_dim;
-      if constexpr (N == 8)
-        *reinterpret_cast<uint2*>(dst) = make_uint2(codes4(f[0], f[1], f[2], f[3]), codes4(f[4], f[5], f[6], f[7]));
-      else
-        *reinterpret_cast<uint32_t*>(dst) = codes4(f[0], f[1], f[2], f[3]);
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        uint32_t c[N / 4];
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          const float2 lo = mul2(make_float2(f[v][i], f[v][i + 1]), inv), hi = mul2(make_float2(f[v][i + 2], f[v][i + 3]), inv);
+          c[i / 4] = codes4(lo.x, lo.y, hi.x, hi.y);
+        }
+        if constexpr (N == 8) *reinterpret_cast<uint2*>(dst + v * TEAM * N) = make_uint2(c[0], c[1]);
+        else *reinterpret_cast<uint32_t*>(dst + v * TEAM * N) = c[0];
+      }
       if (piece == 0) scales[sc] = (uint8_t)(e + 127);
     }
   }
@@ -321,8 +343,8 @@ __device__ __forceinline__ float held(float y) {
 // Largest scale byte at which no code can pass T's range: 448 2^e <= top.
 template <typename T> constexpr int plain_bytes() { return std::is_same<T, __half>::value ? 127 + 7 : 127 + 118; }
 
-// N codes (the low bytes of w) times 2^(byte - 127).
-template <typename T, int N>
+// N codes (the low bytes of w) times 2^(byte - 127); kHold: the range is looked at.
+template <typename T, int N, bool kHold>
 __device__ __forceinline__ void dequant(const uint32_t* w, int byte, T* y) {
   const float s = __uint_as_float((uint32_t)byte << 23);
   if constexpr (N == 1) {
@@ -332,10 +354,8 @@ __device__ __forceinline__ void dequant(const uint32_t* w, int byte, T* y) {
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
       const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 4] >> (8 * (i & 3))), __NV_E4M3);
-      float2 f = __half22float2(__half2(h));
-      f.x *= s;
-      f.y *= s;
-      if (byte > plain_bytes<T>()) {
+      float2 f = mul2(__half22float2(__half2(h)), s);
+      if constexpr (kHold) {
         f.x = held<T>(f.x);
         f.y = held<T>(f.y);
       }
@@ -354,11 +374,12 @@ __device__ __forceinline__ void dequant(const uint32_t* w, int byte, T* y) {
 // Work item = one block of one sequence: all its heads, K and V of one layer
 // (blockIdx.y).  The items of a sequence start after those of the sequences before it; a
 // CTA finds its sequences by a scan of the lengths, kept in shared memory.  Rows are handled
-// as in quant_append_kernel: TEAM lanes x 16 bytes of output, a lane per row resolving it (and
-// reading its scale byte); TEAM 0 is one lane per row's element, for any head_dim and
-// alignment.
+// as in quant_append_kernel: TEAM lanes x two 16-byte vectors of output, a lane per row resolving
+// it (and reading its scale byte); TEAM 0 is a warp per row, for any head_dim and alignment.
+// Bound by instructions and latency before DRAM: 16 x 2049 tokens x 4 layers, 807 MB: 249 us with
+// every lane resolving its vector, 147 us with a lane per row, then two vectors a lane.
 template <typename T, int TEAM>
-__global__ void __launch_bounds__(kThreads) quant_gather_kernel(QuantGatherParams p) {
+__global__ void __launch_bounds__(kThreads, 4) quant_gather_kernel(QuantGatherParams p) {
   extern __shared__ int32_t cu[];  // [batch + 1] first block, then [batch + 1] first token
   int32_t* cu_tok = cu + p.batch + 1;
   __shared__ int32_t s_sum[2][kThreads / 32];
@@ -408,13 +429,29 @@ __global__ void __launch_bounds__(kThreads) quant_gather_kernel(QuantGatherParam
     if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) flag_error(p.err, SNAPMIND_DEVERR_TABLE);
     return;
   }
-  constexpr int N = TEAM ? Vec<T>::N : 1, kTeam = TEAM ? TEAM : 32, kTeams = 32 / kTeam;
-  constexpr int kUnroll = !TEAM ? 1 : 32 / kTeams < 8 ? 32 / kTeams : 8, kRows = kTeams * kUnroll;
+  constexpr int N = TEAM ? Vec<T>::N : 1, kTeam = TEAM ? TEAM : 32, kTeams = 32 / kTeam, kV = TEAM ? 2 : 1;
+  constexpr int kUnroll = TEAM ? 4 : 1, kRows = kTeams * kUnroll;
+  static_assert(kRows <= 32, "a lane per row");
   const int layer = blockIdx.y, piece = lane % kTeam, sub = lane / kTeam;
+  struct Item {
+    int b, j;
+    int32_t phys;
+  };
+  const auto locate = [&](int it) {  // the item's block: read one item ahead
+    Item x{0, 0, -1};
+    if (it < cu[p.batch]) {
+      x.b = upper_bound_i32(cu, p.batch + 1, it) - 1;
+      x.j = it - cu[x.b];
+      if (x.j < p.table_width) x.phys = p.tables[(int64_t)x.b * p.table_stride + x.j];
+    }
+    return x;
+  };
+  Item next = locate(blockIdx.x);
   for (int it = blockIdx.x; it < cu[p.batch]; it += gridDim.x) {
-    const int b = upper_bound_i32(cu, p.batch + 1, it) - 1, j = it - cu[b];
+    const int b = next.b, j = next.j;
+    const int32_t phys = next.phys;
+    next = locate(it + gridDim.x);
     const int len = cu_tok[b + 1] - cu_tok[b], valid = min(p.block_size, len - j * p.block_size);
-    const int32_t phys = j < p.table_width ? p.tables[(int64_t)b * p.table_stride + j] : -1;
     if (phys < 0 || phys >= p.num_blocks) {
       if (tid == 0) flag_error(p.err, j < p.table_width ? SNAPMIND_DEVERR_BLOCK_ID : SNAPMIND_DEVERR_TABLE);
       continue;
@@ -424,7 +461,7 @@ __global__ void __launch_bounds__(kThreads) quant_gather_kernel(QuantGatherParam
     const int64_t dst0 = (int64_t)cu_tok[b] * row_elems + (int64_t)j * p.block_size * p.head_dim;
     const int rows = 2 * p.n_heads * p.block_size;  // (K or V, head, slot)
     for (int r0 = warp * kRows; r0 < rows; r0 += kThreads / 32 * kRows) {
-      int byte = -1, plane = 0;
+      int plane = -1, byte = 0;
       uint32_t from = 0;  // within the block: 2 * heads * head_dim * block_size < 2^31
       int64_t to = 0;
       const int row = r0 + lane;
@@ -433,41 +470,50 @@ __global__ void __launch_bounds__(kThreads) quant_gather_kernel(QuantGatherParam
         if (t < valid) {  // slots past the sequence's end are skipped
           plane = th >= p.n_heads;
           const int h = th - plane * p.n_heads;
-          byte = sc[(h * 2 + plane) * p.block_size + t];
+          byte = sc[(h * 2 + plane) * p.block_size + t];  // lands with the codes, not before them
           from = (uint32_t)(h * p.block_size + t) * p.head_dim;
           to = dst0 + ((int64_t)h * len + t) * p.head_dim;
         }
       }
-      byte = byte < 0 ? -1 : byte | plane << 8;
-      for (int d0 = 0; d0 < p.head_dim; d0 += kTeam * N) {  // one turn with TEAM lanes a row
+      const bool hold = __any_sync(0xffffffffu, byte > plain_bytes<T>());
+      for (int d0 = 0; d0 < p.head_dim; d0 += kTeam * N * kV) {  // one turn with TEAM lanes a row
         const int d = d0 + piece * N;
-        uint32_t codes[kUnroll][2];
-        int by[kUnroll];
+        uint32_t codes[kUnroll][kV][2];
+        int kv[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-          by[u] = __shfl_sync(0xffffffffu, byte, u * kTeams + sub);
+          kv[u] = __shfl_sync(0xffffffffu, plane, u * kTeams + sub);
           const uint32_t f = __shfl_sync(0xffffffffu, from, u * kTeams + sub);
-          if (by[u] < 0 || d >= p.head_dim) continue;
-          const uint8_t* src = p.pool[by[u] >> 8] + src0 + f + d;
-          if constexpr (N == 8) {
-            const uint2 x = __ldcs(reinterpret_cast<const uint2*>(src));
-            codes[u][0] = x.x;
-            codes[u][1] = x.y;
-          } else if constexpr (N == 4) {
-            codes[u][0] = __ldcs(reinterpret_cast<const uint32_t*>(src));
-          } else {
-            codes[u][0] = *src;
+          if (d >= p.head_dim) kv[u] = -1;
+          if (kv[u] < 0) continue;
+          const uint8_t* src = p.pool[kv[u]] + src0 + f + d;
+#pragma unroll
+          for (int v = 0; v < kV; ++v, src += kTeam * N) {
+            if constexpr (N == 8) {
+              const uint2 x = *reinterpret_cast<const uint2*>(src);
+              codes[u][v][0] = x.x;
+              codes[u][v][1] = x.y;
+            } else if constexpr (N == 4) {
+              codes[u][v][0] = *reinterpret_cast<const uint32_t*>(src);
+            } else {
+              codes[u][v][0] = *src;
+            }
           }
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
           const int64_t dst = __shfl_sync(0xffffffffu, to, u * kTeams + sub) + d;
-          if (by[u] < 0 || d >= p.head_dim) continue;
-          __align__(16) T y[N];
-          dequant<T, N>(codes[u], by[u] & 255, y);
-          T* out = reinterpret_cast<T*>(p.out[by[u] >> 8] + layer * p.out_layer_stride) + dst;
-          if constexpr (TEAM != 0) __stcs(reinterpret_cast<uint4*>(out), *reinterpret_cast<const uint4*>(y));
-          else *out = y[0];
+          const int by = __shfl_sync(0xffffffffu, byte, u * kTeams + sub);
+          if (kv[u] < 0) continue;
+          T* out = reinterpret_cast<T*>(p.out[kv[u]] + layer * p.out_layer_stride) + dst;
+#pragma unroll
+          for (int v = 0; v < kV; ++v, out += kTeam * N) {
+            __align__(16) T y[N];
+            if (hold) dequant<T, N, true>(codes[u][v], by, y);
+            else dequant<T, N, false>(codes[u][v], by, y);
+            if constexpr (TEAM != 0) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(y);
+            else *out = y[0];
+          }
         }
       }
     }
@@ -490,9 +536,9 @@ int launch_quant_append(const ChunkAppendParams& p, int n_layers, cudaStream_t s
     kernel<<<dim3((unsigned)(want < cap ? want : cap), planes), kThreads, 0, st>>>(p);
     return cuda_status(cudaGetLastError(), "kv_append_chunk launch");
   };
-  if (vec && row_bytes == 32 * 16) return go(quant_append_kernel<T, 32>, kThreads / 32);
-  if (vec && row_bytes == 16 * 16) return go(quant_append_kernel<T, 16>, kThreads / 16);
-  if (vec && row_bytes == 8 * 16) return go(quant_append_kernel<T, 8>, kThreads / 8);
+  if (vec && row_bytes == 16 * 32) return go(quant_append_kernel<T, 16>, 4 * kThreads / 16);
+  if (vec && row_bytes == 8 * 32) return go(quant_append_kernel<T, 8>, 4 * kThreads / 8);
+  if (vec && row_bytes == 4 * 32) return go(quant_append_kernel<T, 4>, 4 * kThreads / 4);
   return go(quant_append_any_kernel<T>, kThreads / 32);
 }
 
@@ -632,13 +678,13 @@ int snapmind_kv_gather_quant(const void* k_pool, const void* v_pool, const void*
     kernel<<<dim3(cap, n_layers), kThreads, smem, st>>>(p);
     return cuda_status(cudaGetLastError(), "kv_gather_quant launch");
   };
-  const int team = vec ? head_dim * esz / 16 : 0;
+  const int team = vec && head_dim * esz % 32 == 0 ? head_dim * esz / 32 : 0;
   const auto by_team = [&](auto t) -> int {
     using T = decltype(t);
     switch (team) {
+      case 4: return go(quant_gather_kernel<T, 4>);
       case 8: return go(quant_gather_kernel<T, 8>);
       case 16: return go(quant_gather_kernel<T, 16>);
-      case 32: return go(quant_gather_kernel<T, 32>);
       default: return go(quant_gather_kernel<T, 0>);
     }
   };
