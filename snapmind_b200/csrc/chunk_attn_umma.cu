@@ -12,7 +12,7 @@
 //   warps 0-3, 4-7  softmax of tile 0 / 1: thread = row = TMEM lane; they load their Q tile,
 //                   write P to shared memory, and write out the finished rows
 //   warp 8          issues the MMAs
-//   warps 9-11      stage K and V: warp 9 by TMA, or all three converting e4m3 rows
+//   warps 9-11      stage K and V: a warp per 64 columns by TMA, or all three converting e4m3 rows
 // P goes through shared memory, not through TMEM as an A operand: a kernel of this library that
 // read A from TMEM ended in a launch failure whose cause was not found.
 //   TMEM: S of tile 0 / 1 at columns 0 / 128, O at 256 / 256 + head_dim.
@@ -52,6 +52,9 @@ struct Ctrl {
   uint64_t s_full[2];   // MMA commit: scores ready
   uint64_t p_full[2];   // softmax threads: P written, scores read
   uint64_t pv_done[2];  // MMA commit: O += P V done
+  uint64_t x_ml[2];     // split: a group's maxima and sums are in its P rows, its O is final
+  uint64_t x_done[2];   // split: a group has read both groups' O and sums
+  uint64_t v_ready[2];  // MMA warp: V of an edge tile has landed (its unseen rows may be zeroed)
   uint32_t tmem_base;
   int32_t abort;
   PlanShared plan;
@@ -85,9 +88,48 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// The staged loads of a piece of n tiles, in order: K0, K1, V0, K2, V1, .., K(n-1), V(n-2), V(n-1).
-__device__ __forceinline__ int k_index(int j) { return j == 0 ? 0 : 2 * j - 1; }
-__device__ __forceinline__ int v_index(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
+// The lowest k bits (none for k <= 0, all for k >= 32).
+__device__ __forceinline__ uint32_t low_bits(int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; }
+// Pairs of f32 in one instruction: a b + c, a + b.
+__device__ __forceinline__ float2 fma2(float2 a, float b, float c) {
+  float2 r;
+  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %4}; mov.b64 z, {%5, %5}; fma.rn.f32x2 x, x, y, z; "
+      "mov.b64 {%0, %1}, x; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+// A piece whose rows all fit tile 0 runs split: both softmax groups take tile 0's rows, group t
+// the key tiles t, t + 2, ..., each with sums and an O of its own, added up at the end.
+//
+// The staged loads of a piece of n tiles are the first `ahead` K tiles (1, split 2), then for
+// every j K(j + ahead), while there is one, and V(j).
+__device__ __forceinline__ int k_index(int j, int n, int ahead) { return j < ahead ? j : 2 * j - ahead; }
+__device__ __forceinline__ int v_index(int j, int n, int ahead) {
+  const int lead = min(n, ahead);
+  return lead + j + min(j + 1, n - lead);
+}
+
+// Whether a key tile holds rows that no query of the unit sees: [u_s, u_lo) and from v_len on, on the
+// virtual axis.
+struct EdgeTiles {
+  int v_len, u_s, u_lo;
+  __device__ __forceinline__ EdgeTiles(const ChunkParams& p, const KeyRange& r)
+      : v_len(r.v_len), u_s(p.window > 0 ? min(p.sinks, r.v_sink) : 0), u_lo(r.win_lo - r.shift) {}
+  __device__ __forceinline__ bool operator()(int tile) const {
+    const int v0 = tile * kKeys;
+    return v0 + kKeys > v_len || (v0 < u_lo && v0 + kKeys > u_s);
+  }
+  __device__ __forceinline__ bool unseen(int v) const { return v >= v_len || (v < u_lo && v >= u_s); }
+};
 
 // Stage and parity of the load with running number i.
 template <int D> __device__ __forceinline__ int stage_of(uint32_t i) { return i % Shape<D>::kStages; }
@@ -120,7 +162,7 @@ __device__ __forceinline__ void dequant16(const uint4& codes, uint8_t byte, uint
 // gives up what the softmax threads, with a row of 128 scores each, need more of.
 constexpr int kThreads = 384;
 template <bool kQuant> struct Regs {
-  static constexpr int kOther = kQuant ? 120 : 56, kSoftmax = kQuant ? 192 : 224;
+  static constexpr int kOther = kQuant ? 120 : 104, kSoftmax = kQuant ? 192 : 200;
   static_assert(kOther + 2 * kSoftmax <= 3 * 168, "register split");
 };
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -145,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(smem_u32(&C.kv_full[i]), kQuant ? kConvert : 1);
+      mbar_init(smem_u32(&C.kv_full[i]), kQuant ? kConvert : D / 64);
       mbar_init(smem_u32(&C.kv_empty[i]), 1);
     }
     for (int t = 0; t < 2; ++t) {
@@ -153,6 +195,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&C.s_full[t]), 1);
       mbar_init(smem_u32(&C.p_full[t]), 128);
       mbar_init(smem_u32(&C.pv_done[t]), 1);
+      mbar_init(smem_u32(&C.x_ml[t]), 128);
+      mbar_init(smem_u32(&C.x_done[t]), 128);
+      mbar_init(smem_u32(&C.v_ready[t]), 1);
     }
     C.abort = 0;
     mbar_init_fence();
@@ -173,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= kMmaWarp) {
   regs_dec<Regs<kQuant>::kOther>();
   if (warp >= kLoadWarp) {
-    if (!kQuant && warp > kLoadWarp) on = false;
+    if (!kQuant && warp >= kLoadWarp + D / 64) on = false;
     // ------------------------------------------------------------------ K and V stages
     uint32_t issued = 0;
     bool ok = true;
@@ -188,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const auto block_of = [&](int j) -> int32_t {
         const int v = (c.tile0 + j) * kKeys + lane * box;
         if (j >= n || lane >= per_tile || v >= kr.v_len) return -1;
-        const int lb = kr.position(v) / bs;
+        const int lb = p.by_block.div(kr.position(v));
         if (lb >= p.table_width) {
           flag_error(p.err, SNAPMIND_DEVERR_TABLE);
           return -1;
@@ -200,18 +245,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         return phys;
       };
-      int32_t prev = -1, cur = block_of(0);  // blocks of the latest V's and K's tiles
+      const int ahead = (min(c.n, c.i0 + p.tokens) - c.i0) * p.gw > kTileM ? 1 : 2, lead = min(n, ahead);
+      int32_t b0 = -1, b1 = -1, b2 = -1;  // blocks of the latest K tile and the two before
+      int k_next = 0;
       for (int i = 0; i < 2 * n && ok; ++i) {
         // load i of the piece: tile j of K (0) or V (1)
-        const int kv = i == 0 ? 0 : (i == 2 * n - 1 ? 1 : (i & 1 ? 0 : 1));
-        const int j = kv == 0 ? (i + 1) / 2 : (i == 2 * n - 1 ? n - 1 : i / 2 - 1);
-        if (kv == 0 && i > 0) {
-          prev = cur;
-          cur = block_of(j);
-        } else if (i == 2 * n - 1) {
-          prev = cur;
+        const int r = i - lead;
+        const int kv = r < 0 ? 0 : (r < 2 * (n - lead) ? r & 1 : 1);
+        const int j = r < 0 ? i : (r < 2 * (n - lead) ? r / 2 + (kv ? 0 : ahead) : r - (n - lead));
+        if (kv == 0) {
+          b2 = b1;
+          b1 = b0;
+          b0 = block_of(j);
+          k_next = j;
         }
-        const int32_t phys = kv == 0 ? cur : prev;
+        const int32_t phys = kv == 0 || k_next == j ? b0 : (k_next == j + 1 ? b1 : b2);
         const int st = stage_of<D>(issued);
         const int off = bs > kKeys ? kr.position((c.tile0 + j) * kKeys) % bs : 0;  // tile inside a larger block
         uint8_t* dst = ring + st * Sh::kTileBytes;
@@ -219,16 +267,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t leader = elect_one_sync();
           ok = __all_sync(0xffffffffu, role_wait(C, smem_u32(&C.kv_empty[st]), full_parity<D>(issued) ^ 1));
           if (!ok) break;
+          // one warp per 64 columns: a copy takes a warp about 40 cycles to issue, and blocks of 16
+          // tokens are 2 KB copies
+          const int h = warp - kLoadWarp;
           const uint32_t have = __ballot_sync(0xffffffffu, phys >= 0);
           const uint32_t bar = smem_u32(&C.kv_full[st]);
-          mbar_arrive_expect_tx_p(leader, bar, __popc(have) * (uint32_t)box * 128u * (D / 64));
+          mbar_arrive_expect_tx_p(leader, bar, __popc(have) * (uint32_t)box * 128u);
           const CUtensorMap* map = kv == 0 ? &k_map : &v_map;
+          const uint32_t to = smem_u32(dst + h * kBlockBytes);
           for (int x = 0; x < per_tile; ++x) {
             if (!(have >> x & 1)) continue;
             const int y = (__shfl_sync(0xffffffffu, phys, x) * p.n_kv_heads + c.kvh) * bs + off;
-#pragma unroll
-            for (int h = 0; h < D / 64; ++h)
-              tma_load_2d_p(leader, smem_u32(dst + h * kBlockBytes + x * box * 128), map, 64 * h, y, bar);
+            tma_load_2d_p(leader, to + x * box * 128, map, 64 * h, y, bar);
           }
         } else {
           // D / 16 lanes share a row (16 codes each), kRowsPass rows a pass
@@ -286,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ MMA issuer
     const uint32_t leader = elect_one_sync();
     uint32_t load0 = 0, piece = 0;
-    uint32_t steps[2] = {0, 0}, pieces1 = 0;  // key tiles done by tile 0 / 1; pieces with a tile 1
+    uint32_t steps[2] = {0, 0}, pieces1 = 0;  // scores of group 0 / 1 issued; pieces with a tile 1
     uint32_t last_bar = 0, last_parity = 0;
     bool ok = true;
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -294,21 +344,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) tc_fence_after();
       return ok;
     };
-    // S of tile t = Q K^T, K in stage st
-    const auto scores = [&](int t, int st) {
+    // S of group t = (Q of tile qt) K^T, K in stage st
+    const auto scores = [&](int t, int qt, int st) {
 #pragma unroll
       for (int kb = 0; kb < D / 64; ++kb)
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
           umma_f16_p(leader, tmem + t * kKeys,
-                     smem_desc(smem_u32(q_s + t * Sh::kTileBytes + kb * kBlockBytes + kk * 32), 16, 1024, kSwizzle128B),
+                     smem_desc(smem_u32(q_s + qt * Sh::kTileBytes + kb * kBlockBytes + kk * 32), 16, 1024, kSwizzle128B),
                      smem_desc(smem_u32(ring + st * Sh::kTileBytes + kb * kBlockBytes + kk * 32), 16, 1024, kSwizzle128B),
                      kIdescS, (kb > 0 || kk > 0) ? 1u : 0u);
       umma_commit_p(leader, smem_u32(&C.s_full[t]));
       last_bar = smem_u32(&C.s_full[t]);
+      last_parity = steps[t]++ & 1;
     };
     // O of tile t (+)= P V, V in stage st
-    const auto values = [&](int t, int st, bool first) {
+    const auto values = [&](int t, int st, bool first, uint32_t step) {
 #pragma unroll
       for (int ks = 0; ks < kKeys / 16; ++ks)
         umma_f16_p(leader, tmem + 2 * kKeys + t * D,
@@ -317,43 +368,52 @@ __global__ void __launch_bounds__(kThreads, 1)
                    kIdescO, (!first || ks > 0) ? 1u : 0u);
       umma_commit_p(leader, smem_u32(&C.pv_done[t]));
       last_bar = smem_u32(&C.pv_done[t]);
+      last_parity = step & 1;
     };
     for (; on && ok; on = w.next(p)) {
       const Piece& c = w.c;
       const int n = c.tile1 - c.tile0;
-      const int tiles = (min(c.n, c.i0 + p.tokens) - c.i0) * p.gw > kTileM ? 2 : 1;
-      {
-        const uint32_t i = load0;
+      const int i1 = min(c.n, c.i0 + p.tokens);
+      const bool split = (i1 - c.i0) * p.gw <= kTileM;
+      const int ahead = split ? 2 : 1;
+      const EdgeTiles edge(p, key_range(p, c.len, c.n, c.i0, i1));
+      const uint32_t s0[2] = {steps[0], steps[1]};  // steps of the groups before this piece
+      // the scores of the first tile(s)
+      for (int j = 0; j < min(n, ahead) && ok; ++j) {
+        const uint32_t i = load0 + j;
         if (!wait(&C.kv_full[stage_of<D>(i)], full_parity<D>(i))) break;
-        for (int t = 0; t < tiles && ok; ++t) {
-          if (!wait(&C.q_full[t], (t == 0 ? piece : pieces1) & 1)) break;
-          scores(t, stage_of<D>(i));
-          last_parity = steps[t] & 1;
+        for (int t = 0; t < (split ? 1 : 2) && ok; ++t) {
+          if (j == 0 && !wait(&C.q_full[t], (t == 0 ? piece : pieces1) & 1)) break;
+          scores(split ? j : t, t, stage_of<D>(i));
         }
-        if (!ok) break;
-        umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(i)]));
+        if (ok) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(i)]));
       }
       for (int j = 0; j < n && ok; ++j) {
-        const uint32_t ik = load0 + k_index(j + 1), iv = load0 + v_index(j, n);
-        for (int t = 0; t < tiles; ++t) {
-          // P of tile j written, so its scores are read: the next ones may replace them
-          if (!wait(&C.p_full[t], steps[t] & 1)) break;
-          if (j + 1 < n) {
-            if (t == 0 && !wait(&C.kv_full[stage_of<D>(ik)], full_parity<D>(ik))) break;
-            scores(t, stage_of<D>(ik));
-            last_parity = (steps[t] + 1) & 1;
-            if (t == tiles - 1) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(ik)]));
+        const uint32_t ik = load0 + k_index(j + ahead, n, ahead), iv = load0 + v_index(j, n, ahead);
+        if (!kQuant && edge(c.tile0 + j)) {
+          const int t = split ? j & 1 : 0;
+          if (!wait(&C.kv_full[stage_of<D>(iv)], full_parity<D>(iv))) break;
+          mbar_arrive_p(leader, smem_u32(&C.v_ready[t]));
+        }
+        for (int x = 0; x < (split ? 1 : 2); ++x) {
+          const int t = split ? j & 1 : x;
+          const uint32_t step = s0[t] + (split ? j >> 1 : j);
+          // P of tile j written, so its scores are read: the group's next ones may replace them
+          if (!wait(&C.p_full[t], step & 1)) break;
+          const bool last = split || x == 1;
+          if (j + ahead < n) {
+            if (x == 0 && !wait(&C.kv_full[stage_of<D>(ik)], full_parity<D>(ik))) break;
+            scores(t, split ? 0 : t, stage_of<D>(ik));
+            if (last) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(ik)]));
           }
-          if (t == 0 && !wait(&C.kv_full[stage_of<D>(iv)], full_parity<D>(iv))) break;
-          values(t, stage_of<D>(iv), j == 0);
-          last_parity = steps[t] & 1;
-          ++steps[t];
-          if (t == tiles - 1) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(iv)]));
+          if (x == 0 && !wait(&C.kv_full[stage_of<D>(iv)], full_parity<D>(iv))) break;
+          values(t, stage_of<D>(iv), step == s0[t], step);
+          if (last) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(iv)]));
         }
       }
       load0 += 2 * n;
       ++piece;
-      pieces1 += tiles - 1;
+      pieces1 += split ? 0 : 1;
     }
     if (!ok && lane == 0) give_up(C, p.err);
     if (last_bar) mbar_wait(last_bar, last_parity);  // MMAs in flight end (bounded) before TMEM goes
@@ -368,23 +428,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float c2 = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
     uint8_t* prow = p_s + t * kPBytes + r * 128;
     const uint32_t sw = (uint32_t)(r & 7);
-    uint32_t step = 0, load0 = 0;
+    uint32_t step = 0, load0 = 0, edges = 0, splits = 0, other_steps = 0;
     bool ok = true;
-    for (; on && ok; on = w.next(p)) {
-      const Piece& c = w.c;
-      const int n = c.tile1 - c.tile0;
-      const int i1 = min(c.n, c.i0 + p.tokens), n_rows = (i1 - c.i0) * p.gw;
-      const uint32_t load = load0;
-      load0 += 2 * n;
-      if (t * kTileM >= n_rows) continue;
+    // Q tile t of a piece, by the group's 128 threads
+    const auto load_q = [&](const Piece& c) {
+      const int n_rows = (min(c.n, c.i0 + p.tokens) - c.i0) * p.gw;
+      if (t * kTileM >= n_rows) return;
       const int heads = slice_heads(p, c.slice), head0 = c.kvh * p.group + c.slice * p.gw;
-      // the Q tile (the scores of the piece before are all done: its last s_full was waited for)
+#pragma unroll 4
       for (int e = r; e < kTileM * (D / 8); e += 128) {
-        const int row = e / (D / 8), ch = e % (D / 8), R = t * kTileM + row, g = R % p.gw;
+        const int row = e / (D / 8), ch = e % (D / 8), R = t * kTileM + row;
+        const int tok = p.by_gw.div(R), g = R - tok * p.gw;
         uint4 x = make_uint4(0, 0, 0, 0);
         if (R < n_rows && g < heads)
           x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) +
-                                              (int64_t)(c.q_first + c.i0 + R / p.gw) * p.q_stride_tok +
+                                              (int64_t)(c.q_first + c.i0 + tok) * p.q_stride_tok +
                                               (int64_t)(head0 + g) * p.q_stride_head + ch * 8);
         if (flip) {
           x.x ^= 0x80008000u;
@@ -396,68 +454,74 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       fence_proxy_async_smem();
       mbar_arrive(smem_u32(&C.q_full[t]));
-
+    };
+    if (on) load_q(w.c);
+    while (on && ok) {
+      const Piece c = w.c;
+      const int n = c.tile1 - c.tile0;
+      const int i1 = min(c.n, c.i0 + p.tokens), n_rows = (i1 - c.i0) * p.gw;
+      const bool split = n_rows <= kTileM;
+      const int R = (split ? 0 : t * kTileM) + r, tok = p.by_gw.div(min(R, n_rows - 1));
       const KeyRange kr = key_range(p, c.len, c.n, c.i0, i1);
-      const int R = t * kTileM + r;
-      const int qpos = kr.pos0 + min(R, n_rows - 1) / p.gw;
-      // on the virtual axis the row sees [v_lo, v_hi) and [0, v_s); no row of the unit sees
-      // [u_s, u_lo) or past v_len
+      const EdgeTiles edge(p, kr);
+      const int qpos = kr.pos0 + tok;
+      // on the virtual axis the row sees [v_lo, v_hi) and [0, v_s)
       const int v_hi = max(0, qpos + 1 - kr.shift);
       const int v_lo = p.window > 0 ? max(0, qpos - p.window + 1) - kr.shift : 0;
       const int v_s = p.window > 0 ? min(p.sinks, v_hi) : 0;
-      const int u_s = p.window > 0 ? min(p.sinks, kr.v_sink) : 0, u_lo = kr.win_lo - kr.shift;
+      const uint32_t step0 = step;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < n; ++j) {
+      for (int j = split ? t : 0; j < n; j += split ? 2 : 1) {
         const int v0 = (c.tile0 + j) * kKeys;
-        ok = ok && role_wait(C, smem_u32(&C.s_full[t]), step & 1);
+        ok = role_wait(C, smem_u32(&C.s_full[t]), step & 1);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        if (!kQuant && t == 0) {
-          const int key = v0 + r;
-          if (v0 + kKeys > kr.v_len || (v0 < u_lo && v0 + kKeys > u_s)) {
-            // rows of V that nobody sees are zeroed: 0 x (whatever lies there) must not reach O.
-            // (After the scores: K of this tile has landed, so V's barrier is in the phase waited for.)
-            const uint32_t i = load + v_index(j, n);
-            ok = __all_sync(0xffffffffu, role_wait(C, smem_u32(&C.kv_full[stage_of<D>(i)]), full_parity<D>(i)));
-            if (!ok) break;
-            if (key >= kr.v_len || (key < u_lo && key >= u_s)) {
-              uint8_t* vrow = ring + stage_of<D>(i) * Sh::kTileBytes + r * 128;
+        float s[kKeys];
 #pragma unroll
-              for (int h = 0; h < D / 64; ++h)
+        for (int x = 0; x < kKeys; x += 32) tmem_ld32(t_s + x, s + x);
+        tmem_wait_ld();
+        if (!kQuant && (split || t == 0) && edge(c.tile0 + j)) {
+          // rows of V that nobody sees are zeroed: 0 x (whatever lies there) must not reach O
+          ok = __all_sync(0xffffffffu, role_wait(C, smem_u32(&C.v_ready[t]), edges++ & 1));
+          if (!ok) break;
+          if (edge.unseen(v0 + r)) {
+            uint8_t* vrow = ring + stage_of<D>(load0 + v_index(j, n, split ? 2 : 1)) * Sh::kTileBytes + r * 128;
 #pragma unroll
-                for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(vrow + h * kBlockBytes + x * 16) = make_uint4(0, 0, 0, 0);
-            }
+            for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+              for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(vrow + h * kBlockBytes + x * 16) = make_uint4(0, 0, 0, 0);
           }
         }
-        float s[kKeys];
-        const auto load_scores = [&]() {
-#pragma unroll
-          for (int x = 0; x < kKeys; x += 32) tmem_ld32(t_s + x, s + x);
-          tmem_wait_ld();
+        {
           const int lo = v_lo - v0, hi = v_hi - v0, sk = v_s - v0;
           if (!__all_sync(0xffffffffu, hi >= kKeys && (lo <= 0 || sk >= kKeys))) {
 #pragma unroll
-            for (int x = 0; x < kKeys; ++x)
-              if (!((x >= lo && x < hi) || x < sk)) s[x] = -INFINITY;
+            for (int x = 0; x < kKeys; x += 32) {  // bit i of `see`: key x + i
+              const uint32_t see = (low_bits(hi - x) & ~low_bits(lo - x)) | low_bits(sk - x);
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(see >> i & 1)) s[x + i] = -INFINITY;
+            }
           }
-        };
-        load_scores();
+        }
         float mx[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) mx[x] = s[x];
 #pragma unroll
-        for (int x = 4; x < kKeys; ++x) mx[x & 3] = fmaxf(mx[x & 3], s[x]);
+        for (int x = 4; x < kKeys; x += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = x + 4 + i < kKeys ? fmaxf(mx[i], fmaxf(s[x + i], s[x + 4 + i])) : fmaxf(mx[i], s[x + i]);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
         const bool raise = top > m + kRescale;
-        bool waited = j == 0;  // O += P V of the tile before: P and O are free
+        bool waited = step == step0;  // O += P V of the group's tile before: P and O are free
         if (__any_sync(0xffffffffu, raise)) {
           const float alpha = raise ? ex2(m - top) : 1.f;
           if (raise) m = top;
           l *= alpha;
-          if (j > 0) {
+          if (!waited) {
             ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);
             if (!__all_sync(0xffffffffu, ok)) {
               ok = false;
@@ -466,90 +530,139 @@ __global__ void __launch_bounds__(kThreads, 1)
             waited = true;
             tc_fence_after();
 #pragma unroll 1
-            for (int x = 0; x < D; x += 32) {
-              float o[32];
-              tmem_ld32(t_o + x, o);
+            for (int x = 0; x < D; x += 16) {
+              float o[16];
+              tmem_ld16(t_o + x, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] *= alpha;
-              tmem_st32(t_o + x, o);
+              for (int y = 0; y < 16; ++y) o[y] *= alpha;
+              tmem_st16(t_o + x, o);
             }
             tmem_wait_st();
-            load_scores();  // again, rather than 128 registers kept over the rescaling
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;  // nothing seen yet: 2^-inf = 0 for any reference
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t pk[kKeys / 2];
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int x = 0; x < kKeys; x += 2) {
-          const float a = ex2(fmaf(s[x], c2, -ref)), b = ex2(fmaf(s[x + 1], c2, -ref));
-          sum[x & 2] += a;
-          sum[(x & 2) + 1] += b;
-          pk[x / 2] = pack2<T>(a, b);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (!waited) {
-          ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
+        for (int x = 0; x < kKeys; x += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int y = 0; y < 32; y += 2) {
+            float2 e = fma2(make_float2(s[x + y], s[x + y + 1]), c2, -ref);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[(y >> 1) & 1] = add2(sum[(y >> 1) & 1], e);
+            pk[y / 2] = pack2<T>(e.x, e.y);
           }
-        }
+          if (x == 0 && !waited) {
+            ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+          }
 #pragma unroll
-        for (int x = 0; x < kKeys / 8; ++x)
-          *reinterpret_cast<uint4*>(prow + (x / 8) * kBlockBytes + (((uint32_t)(x % 8) ^ sw) << 4)) =
-              make_uint4(pk[4 * x], pk[4 * x + 1], pk[4 * x + 2], pk[4 * x + 3]);
+          for (int y = 0; y < 4; ++y)
+            *reinterpret_cast<uint4*>(prow + (x / 64) * kBlockBytes + (((uint32_t)((x % 64) / 8 + y) ^ sw) << 4)) =
+                make_uint4(pk[4 * y], pk[4 * y + 1], pk[4 * y + 2], pk[4 * y + 3]);
+        }
+        if (!ok) break;
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(smem_u32(&C.p_full[t]));
         ++step;
       }
       if (!ok) break;
-      ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);
+      load0 += 2 * n;
+      if (split) {
+        // the other group's scores read tile 0's Q too: all done before the next Q may land there
+        // (group 0's last scores follow all but the last of group 1's, so the phase is the one meant)
+        other_steps += (n - (t ^ 1) + 1) / 2;
+        if (t == 0 && other_steps > 0) ok = role_wait(C, smem_u32(&C.s_full[1]), (other_steps - 1) & 1);
+      } else {
+        other_steps += n;
+      }
+      // the next piece's Q goes out first (this piece's scores are all done), so that its products
+      // start under this piece's epilogue
+      on = w.next(p);
+      if (on && ok) load_q(w.c);
+      if (ok && step > step0) ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);
+      const uint32_t t_x = tmem + lanes + 2 * kKeys + (t ^ 1) * D;  // the other group's O
+      float f = 1.f, fx = 0.f;
+      int c0 = 0, c1 = D;
+      if (split) {
+        // both groups meet: maxima and sums go through the P rows, O is read where it is, each
+        // group writes half of the dims
+        if (ok) {
+          *reinterpret_cast<float2*>(prow) = make_float2(m, l);
+          tc_fence_before();
+          mbar_arrive(smem_u32(&C.x_ml[t]));
+          ok = role_wait(C, smem_u32(&C.x_ml[t ^ 1]), splits & 1);
+        }
+        const float2 ml = *reinterpret_cast<const float2*>(p_s + (t ^ 1) * kPBytes + r * 128);
+        const float M = fmaxf(m, ml.x);
+        f = m == -INFINITY ? 0.f : ex2(m - M);
+        fx = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+        m = M;
+        l = l * f + ml.y * fx;
+        c0 = t * (D / 2);
+        c1 = c0 + D / 2;
+      }
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const int g = R % p.gw;
-      const bool mine = R < n_rows && g < heads;
-      if (c.whole()) {
+      const int heads = slice_heads(p, c.slice), rt = p.by_gw.div(R), g = R - rt * p.gw;
+      const bool mine = R < n_rows && g < heads, whole = c.whole();
+      const int64_t slot = part_slot(c) * p.rows + R;
+      T* out = reinterpret_cast<T*>(p.out) + (int64_t)(c.q_first + c.i0 + rt) * p.out_stride_tok +
+               (int64_t)(c.kvh * p.group + c.slice * p.gw + g) * p.out_stride_head;
+      if (!whole && mine && (!split || t == 0)) {
+        p.part_ml[slot * 2] = m;
+        p.part_ml[slot * 2 + 1] = l;
+      }
+      if (whole) {  // sees nothing: zeros
         const float inv = m == -INFINITY ? 0.f : 1.f / l;
-        T* out = reinterpret_cast<T*>(p.out) + (int64_t)(c.q_first + c.i0 + R / p.gw) * p.out_stride_tok +
-                 (int64_t)(head0 + g) * p.out_stride_head;
+        f *= inv;
+        fx *= inv;
+      }
 #pragma unroll 1
-        for (int x = 0; x < D; x += 32) {
-          float o[32];
-          tmem_ld32(t_o + x, o);
+      for (int x = c0; x < c1; x += 16) {
+        float o[16];
+        tmem_ld16(t_o + x, o);
+        if (split) {
+          float o2[16];
+          tmem_ld16(t_x + x, o2);
           tmem_wait_ld();
-          if (mine) {
+          // a group without a tile (or without a key its row sees) may hold anything
 #pragma unroll
-            for (int y = 0; y < 32; y += 8)
-              *reinterpret_cast<uint4*>(out + x + y) =
-                  make_uint4(pack2<T>(o[y] * inv, o[y + 1] * inv), pack2<T>(o[y + 2] * inv, o[y + 3] * inv),
-                             pack2<T>(o[y + 4] * inv, o[y + 5] * inv), pack2<T>(o[y + 6] * inv, o[y + 7] * inv));
-          }
-        }
-      } else {
-        const int64_t slot = part_slot(c) * p.rows + R;
-        if (mine) {
-          p.part_ml[slot * 2] = m;
-          p.part_ml[slot * 2 + 1] = l;
-        }
-#pragma unroll 1
-        for (int x = 0; x < D; x += 32) {
-          float o[32];
-          tmem_ld32(t_o + x, o);
+          for (int y = 0; y < 16; ++y) o[y] = (f == 0.f ? 0.f : o[y] * f) + (fx == 0.f ? 0.f : o2[y] * fx);
+        } else {
           tmem_wait_ld();
-          if (mine) {
 #pragma unroll
-            for (int y = 0; y < 32; y += 4)
-              *reinterpret_cast<float4*>(p.part_o + slot * D + x + y) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
-          }
+          for (int y = 0; y < 16; ++y) o[y] = f == 0.f ? 0.f : o[y] * f;
+        }
+        if (!mine) continue;
+        if (whole) {
+#pragma unroll
+          for (int y = 0; y < 16; y += 8)
+            *reinterpret_cast<uint4*>(out + x + y) = make_uint4(pack2<T>(o[y], o[y + 1]), pack2<T>(o[y + 2], o[y + 3]),
+                                                                pack2<T>(o[y + 4], o[y + 5]), pack2<T>(o[y + 6], o[y + 7]));
+        } else {
+#pragma unroll
+          for (int y = 0; y < 16; y += 4)
+            *reinterpret_cast<float4*>(p.part_o + slot * D + x + y) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
         }
       }
       tc_fence_before();
+      if (split) {
+        mbar_arrive(smem_u32(&C.x_done[t]));
+        ok = role_wait(C, smem_u32(&C.x_done[t ^ 1]), splits++ & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
     }
     if (!ok && lane == 0) give_up(C, p.err);
   }

@@ -43,6 +43,7 @@ struct ChunkParams {
   int32_t rows;            // partial rows of a unit in the workspace (>= gw * tokens)
   int32_t key_tile;        // keys of a tile
   int32_t n_ctas;
+  FastDiv by_gw, by_block, by_tile;  // divisions by gw, block_size, key_tile
   int32_t* heads;   // workspace: [n_ctas][kPieceInts], see PieceInfo
   float* part_ml;   // workspace: [n_ctas][2][rows][2] maximum (log2 units), sum
   float* part_o;    // workspace: [n_ctas][2][rows][head_dim]
@@ -77,8 +78,8 @@ __device__ __forceinline__ KeyRange key_range(const ChunkParams& p, int len, int
   r.end = max(0, min(len, len - n + i1));
   r.win_lo = p.window > 0 ? max(0, r.pos0 - p.window + 1) : 0;
   const int bs = p.block_size;
-  const int n_sink = p.window > 0 ? (min(p.sinks, r.end) + bs - 1) / bs : 0;
-  const int wb0 = min(r.win_lo, r.end) / bs;
+  const int n_sink = p.window > 0 ? p.by_block.div(min(p.sinks, r.end) + bs - 1) : 0;
+  const int wb0 = p.window > 0 ? p.by_block.div(min(r.win_lo, r.end)) : 0;
   r.v_sink = n_sink * bs;
   r.shift = max(0, wb0 - n_sink) * bs;
   r.v_len = r.end - r.shift;
@@ -87,7 +88,7 @@ __device__ __forceinline__ KeyRange key_range(const ChunkParams& p, int len, int
 // Key tiles of a unit; at least one, so that rows that see nothing are written as zeros.
 __device__ __forceinline__ int key_tiles(const ChunkParams& p, int len, int n, int i0) {
   const KeyRange r = key_range(p, len, n, i0, min(n, i0 + p.tokens));
-  return max(1, (r.v_len + p.key_tile - 1) / p.key_tile);
+  return max(1, p.by_tile.div(r.v_len + p.key_tile - 1));
 }
 
 // A piece: consecutive tiles of one unit.
@@ -119,6 +120,19 @@ __device__ __forceinline__ int seq_tiles(const ChunkParams& p, int b, int lane) 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
+}
+
+// a b / c; in 32 bits where they suffice (a 64-bit division takes hundreds of cycles).
+__device__ __forceinline__ long long mul_div(long long a, long long b, int c) {
+  const long long x = a * b;
+  return x < (1ll << 32) ? (long long)((uint32_t)x / (uint32_t)c) : x / c;
+}
+__device__ __forceinline__ long long cut(int cta, long long total, int n) { return mul_div(cta, total, n); }
+// The CTA whose share holds tile t: the largest c with cut(c) <= t, which is
+// ((t + 1) n - 1) / total rounded down.
+__device__ __forceinline__ int cta_of(long long t, long long total, int n) {
+  const long long x = (t + 1) * n - 1;
+  return (int)(x < (1ll << 32) && total < (1ll << 32) ? (long long)((uint32_t)x / (uint32_t)total) : x / total);
 }
 
 // The block's share of the line: fills S (total, t0, t1, first piece).  `tiles` is
@@ -157,8 +171,8 @@ __device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* 
   total *= per_head;
   const int n = (int)min((long long)p.n_ctas, total);
   const bool works = (int)blockIdx.x < n;
-  const long long t0 = works ? (long long)blockIdx.x * total / n : total;
-  const long long t1 = works ? ((long long)blockIdx.x + 1) * total / n : total;
+  const long long t0 = works ? cut(blockIdx.x, total, n) : total;
+  const long long t1 = works ? cut(blockIdx.x + 1, total, n) : total;
   if (tid == 0) {
     S.total = total;
     S.n = n;
@@ -266,8 +280,8 @@ __device__ inline void write_piece_info(const ChunkParams& p, const PlanShared& 
   h[1] = c.kvh;
   h[2] = c.slice;
   h[3] = c.i0;
-  h[4] = (int32_t)(((s_u + 1) * S.n - 1) / S.total);  // the CTA that holds tile s_u
-  h[5] = (int32_t)((e_u * S.n - 1) / S.total);        // ... and tile e_u - 1
+  h[4] = cta_of(s_u, S.total, S.n);  // the CTA that holds tile s_u
+  h[5] = cta_of(e_u - 1, S.total, S.n);        // ... and tile e_u - 1
   h[0] = c.b;
 }
 
@@ -296,6 +310,9 @@ inline void plan_geometry(ChunkParams& p, int rows, int key_tile, int n_ctas) {
   p.rows = rows;
   p.key_tile = key_tile;
   p.n_ctas = n_ctas;
+  p.by_gw = FastDiv(p.gw);
+  p.by_block = FastDiv(p.block_size);
+  p.by_tile = FastDiv(key_tile);
 }
 
 // Workspace regions of n_ctas CTAs: heads, then maxima and sums, then partial outputs.

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const auto block_of = [&](int j) -> int32_t {  // block of part `lane` of tile j, or -1
         const int v = j * kTile + lane * box;
         if (j >= c.tile1 || lane >= per_tile || v >= kr.v_len) return -1;
-        const int lb = kr.position(v) / bs;
+        const int lb = p.by_block.div(kr.position(v));
         if (lb >= p.table_width) {
           flag_error(p.err, SNAPMIND_DEVERR_TABLE);
           return -1;

@@ -22,21 +22,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Division of 0 <= n < 2^31 by a divisor known at launch: with l = ceil(log2 d) and
-// m = floor(2^(31 + l) / d) + 1, n / d = (n m) >> (31 + l), since m d - 2^(31 + l) <= d <= 2^l.
-struct FastDiv {
-  uint32_t d = 1, m = 0, s = 0;
-  FastDiv() = default;
-  explicit FastDiv(int div) : d(div) {
-    if (d == 1) return;
-    int l = 0;
-    while ((1u << l) < d) ++l;
-    m = (uint32_t)((1ull << (31 + l)) / d) + 1;
-    s = l - 1;
-  }
-  __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> s); }
-};
-
 struct ChunkAppendParams {
   uint8_t* pool[2];
   uint8_t* scales;
