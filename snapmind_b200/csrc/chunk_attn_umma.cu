@@ -12,12 +12,15 @@
 //   warps 0-3, 4-7  softmax of tile 0 / 1: thread = row = TMEM lane; they load their Q tile,
 //                   write P to shared memory, and write out the finished rows
 //   warp 8          issues the MMAs
-//   warps 9-11      stage K and V: a warp per 64 columns by TMA, or all three converting e4m3 rows
+//   warps 9-11      stage K and V: two by TMA, or all three converting e4m3 rows
 // P goes through shared memory, not through TMEM as an A operand: a kernel of this library that
 // read A from TMEM ended in a launch failure whose cause was not found.
 //   TMEM: S of tile 0 / 1 at columns 0 / 128, O at 256 / 256 + head_dim.
-//   Shared memory: Q 2 x [128 x D], P 2 x [128 x 128], then a ring of [128 x D] stages that
-//   K and V tiles take in the order K0, K1, V0, K2, V1, ... (128-byte swizzle everywhere).
+//   Shared memory: Q 2 x [128 x D], P [128 x 128], then a ring of [128 x D] stages that K and V tiles
+//   take in the order K0, K1, V0, K2, V1, ... (128-byte swizzle everywhere).  The tiles share one P
+//   buffer: a tile's P is written after the other's product has read its own, which costs nothing
+//   while the tiles take turns, and the 32 KB are a fourth stage (three stages left every V on its way
+//   when it was needed: 4050 cycles a step of 2 x 128 x 128 scores).
 // Every wait is bounded and ends early once another role gave up; TMEM is released on
 // every path.
 #include <cuda.h>
@@ -41,28 +44,32 @@ constexpr float kRescale = 8.f;  // log2 headroom of the reference maximum
 
 template <int D> struct Shape {
   static constexpr uint32_t kTileBytes = D / 64 * kBlockBytes;  // a Q tile, a K or V stage
-  static constexpr int kStages = D == 64 ? 6 : 3;
-  static constexpr uint32_t kP = 2 * kTileBytes, kRing = kP + 2 * kPBytes;
+  static constexpr int kStages = D == 64 ? 8 : 4;
+  static constexpr uint32_t kP = 2 * kTileBytes, kRing = kP + kPBytes;
+  // K and V stages are [8-row group][64-column block][8 rows x 128 bytes]
+  static constexpr uint32_t kGroup = D / 64 * 1024;
   static constexpr uint32_t kCtrl = kRing + kStages * kTileBytes;
 };
 
 struct Ctrl {
-  uint64_t kv_full[6], kv_empty[6];
+  uint64_t kv_full[8], kv_empty[8];
   uint64_t q_full[2];   // softmax threads: the Q tile of a piece is in shared memory
   uint64_t s_full[2];   // MMA commit: scores ready
-  uint64_t p_full[2];   // softmax threads: P written, scores read
+  uint64_t s_free[2];   // softmax threads: scores read (the group's next ones may replace them)
+  uint64_t p_full[2];   // softmax threads: P written
   uint64_t pv_done[2];  // MMA commit: O += P V done
-  uint64_t x_ml[2];     // split: a group's maxima and sums are in its P rows, its O is final
-  uint64_t x_done[2];   // split: a group has read both groups' O and sums
+  uint64_t x_ml;        // split: group 1's maxima and sums are in `ml`, its O is final
+  uint64_t x_done;      // split: group 0 has read them
   uint64_t v_ready[2];  // MMA warp: V of an edge tile has landed (its unseen rows may be zeroed)
   uint32_t tmem_base;
   int32_t abort;
   PlanShared plan;
+  float2 ml[128];
 };
 
 template <int D> constexpr size_t smem_bytes() { return 1024 + Shape<D>::kCtrl + sizeof(Ctrl); }
 static_assert(smem_bytes<128>() <= 232448 && smem_bytes<64>() <= 232448, "shared memory budget");
-static_assert(2 * kPBytes >= kMaxChunkBatch * 4, "plan scratch in the P tiles");
+static_assert(kPBytes >= kMaxChunkBatch * 4, "plan scratch in the P tiles");
 
 __device__ __forceinline__ bool role_wait(const Ctrl& C, uint32_t bar, uint32_t parity) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -187,18 +194,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(smem_u32(&C.kv_full[i]), kQuant ? kConvert : D / 64);
+      mbar_init(smem_u32(&C.kv_full[i]), kQuant ? kConvert : 2);
       mbar_init(smem_u32(&C.kv_empty[i]), 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&C.q_full[t]), 128);
       mbar_init(smem_u32(&C.s_full[t]), 1);
+      mbar_init(smem_u32(&C.s_free[t]), 128);
       mbar_init(smem_u32(&C.p_full[t]), 128);
       mbar_init(smem_u32(&C.pv_done[t]), 1);
-      mbar_init(smem_u32(&C.x_ml[t]), 128);
-      mbar_init(smem_u32(&C.x_done[t]), 128);
       mbar_init(smem_u32(&C.v_ready[t]), 1);
     }
+    mbar_init(smem_u32(&C.x_ml), 128);
+    mbar_init(smem_u32(&C.x_done), 128);
     C.abort = 0;
     mbar_init_fence();
   }
@@ -218,67 +226,44 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= kMmaWarp) {
   regs_dec<Regs<kQuant>::kOther>();
   if (warp >= kLoadWarp) {
-    if (!kQuant && warp >= kLoadWarp + D / 64) on = false;
+    if (!kQuant && warp >= kLoadWarp + 2) on = false;
     // ------------------------------------------------------------------ K and V stages
     uint32_t issued = 0;
     bool ok = true;
     for (; on && ok; on = w.next(p)) {
       const Piece& c = w.c;
       const KeyRange kr = key_range(p, c.len, c.n, c.i0, min(c.n, c.i0 + p.tokens));
-      const int n = c.tile1 - c.tile0, bs = p.block_size;
-      const int32_t* table = p.tables + (int64_t)c.b * p.table_stride;
-      const int box = min(bs, kKeys);  // rows of a tile that share a block
-      const int per_tile = kKeys / box;
-      // the physical block of part `lane` of tile j (lanes >= per_tile: none), -1 when nothing is there
-      const auto block_of = [&](int j) -> int32_t {
-        const int v = (c.tile0 + j) * kKeys + lane * box;
-        if (j >= n || lane >= per_tile || v >= kr.v_len) return -1;
-        const int lb = p.by_block.div(kr.position(v));
-        if (lb >= p.table_width) {
-          flag_error(p.err, SNAPMIND_DEVERR_TABLE);
-          return -1;
-        }
-        const int32_t phys = table[lb];
-        if (phys < 0 || phys >= p.num_blocks) {
-          flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
-          return -1;
-        }
-        return phys;
-      };
+      const int n = c.tile1 - c.tile0;
+      TileRows at(p, kr, c, lane);
+      const int box = at.box;
       const int ahead = (min(c.n, c.i0 + p.tokens) - c.i0) * p.gw > kTileM ? 1 : 2, lead = min(n, ahead);
-      int32_t b0 = -1, b1 = -1, b2 = -1;  // blocks of the latest K tile and the two before
-      int k_next = 0;
       for (int i = 0; i < 2 * n && ok; ++i) {
         // load i of the piece: tile j of K (0) or V (1)
         const int r = i - lead;
         const int kv = r < 0 ? 0 : (r < 2 * (n - lead) ? r & 1 : 1);
         const int j = r < 0 ? i : (r < 2 * (n - lead) ? r / 2 + (kv ? 0 : ahead) : r - (n - lead));
-        if (kv == 0) {
-          b2 = b1;
-          b1 = b0;
-          b0 = block_of(j);
-          k_next = j;
-        }
-        const int32_t phys = kv == 0 || k_next == j ? b0 : (k_next == j + 1 ? b1 : b2);
+        const int tile = c.tile0 + j;  // V follows its K by one or two tiles: in the batch, or the one before
+        if (kv == 0) at.advance(tile);
         const int st = stage_of<D>(issued);
-        const int off = bs > kKeys ? kr.position((c.tile0 + j) * kKeys) % bs : 0;  // tile inside a larger block
         uint8_t* dst = ring + st * Sh::kTileBytes;
         if constexpr (!kQuant) {
           const uint32_t leader = elect_one_sync();
           ok = __all_sync(0xffffffffu, role_wait(C, smem_u32(&C.kv_empty[st]), full_parity<D>(issued) ^ 1));
           if (!ok) break;
-          // one warp per 64 columns: a copy takes a warp about 40 cycles to issue, and blocks of 16
-          // tokens are 2 KB copies
+          // the two warps take every second part: a copy takes a warp over 100 cycles to issue
           const int h = warp - kLoadWarp;
-          const uint32_t have = __ballot_sync(0xffffffffu, phys >= 0);
           const uint32_t bar = smem_u32(&C.kv_full[st]);
-          mbar_arrive_expect_tx_p(leader, bar, __popc(have) * (uint32_t)box * 128u);
+          mbar_arrive_expect_tx_p(leader, bar, __popc(at.have(tile) & (0x55555555u << h)) * (uint32_t)box * (D * 2u));
           const CUtensorMap* map = kv == 0 ? &k_map : &v_map;
-          const uint32_t to = smem_u32(dst + h * kBlockBytes);
-          for (int x = 0; x < per_tile; ++x) {
-            if (!(have >> x & 1)) continue;
-            const int y = (__shfl_sync(0xffffffffu, phys, x) * p.n_kv_heads + c.kvh) * bs + off;
-            tma_load_2d_p(leader, to + x * box * 128, map, 64 * h, y, bar);
+          const uint32_t to = smem_u32(dst);
+          for (int x0 = h; x0 < at.parts; x0 += 8) {
+            int y[4];  // all rows first: a shuffle between two copies costs more than the copies
+#pragma unroll
+            for (int x = 0; x < 4; ++x) y[x] = at.row(tile, (x0 + 2 * x) & (at.parts - 1));
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              tma_load_4d_p(x0 + 2 * x < at.parts && y[x] >= 0 ? leader : 0u, to + (x0 + 2 * x) * box * (D * 2), map, 0, 0, 0,
+                            y[x] >> 3, bar);
           }
         } else {
           // D / 16 lanes share a row (16 codes each), kRowsPass rows a pass
@@ -290,19 +275,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int x = 0; x < kPasses; ++x) {
             const int r = x * kRowsPass + r0;
-            const int32_t ph = __shfl_sync(0xffffffffu, phys, r / box);
+            const int part = min(r, 127) >> (7 - at.log_parts), y = at.row(tile, part);  // 128 keys: box = 128 >> log_parts
             const int v = (c.tile0 + j) * kKeys + r;
             // rows that no query of the unit sees are zeros: past the end, or in a block that is
             // read between the sinks and the first window
             const int pos = kr.position(v);
-            const bool seen = r < 128 && ph >= 0 && v < kr.v_len && (pos >= kr.win_lo || pos < p.sinks);
+            const bool seen = r < 128 && y >= 0 && v < kr.v_len && (pos >= kr.win_lo || pos < p.sinks);
             codes[x] = make_uint4(0, 0, 0, 0);
             sc[x] = 0;
             if (seen) {
-              const int64_t tile = (int64_t)ph * p.n_kv_heads + c.kvh;
-              const int slot = r % box + off;
-              codes[x] = *reinterpret_cast<const uint4*>(pool + (tile * bs + slot) * D + ch * 16);
-              sc[x] = p.scales[(tile * 2 + kv) * bs + slot];
+              const int row = y + (r - part * box);
+              codes[x] = *reinterpret_cast<const uint4*>(pool + (int64_t)row * D + ch * 16);
+              sc[x] = p.scales[at.scale_at(row, kv)];
             }
           }
           ok = role_wait(C, smem_u32(&C.kv_empty[st]), full_parity<D>(issued) ^ 1);
@@ -314,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (r >= 128) break;
             uint4 lo, hi;
             dequant16<T>(codes[x], sc[x], lo, hi);
-            uint8_t* row = dst + (ch / 4) * kBlockBytes + r * 128;
+            uint8_t* row = dst + (r >> 3) * Sh::kGroup + (ch / 4) * 1024 + (r & 7) * 128;
             const uint32_t sw = r & 7, c0 = (ch % 4) * 2;
             // lanes of the two 64-element halves write opposite pieces: no bank is hit twice
             const bool swap = ch >= 4;
@@ -344,28 +328,31 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) tc_fence_after();
       return ok;
     };
+    // shared-memory descriptors: offsets only change the address field (in 16-byte units)
+    const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, 1024, kSwizzle128B);
+    const uint64_t p_desc = smem_desc(smem_u32(p_s), 16, 1024, kSwizzle128B);
+    const uint64_t k_desc = smem_desc(smem_u32(ring), 16, Sh::kGroup, kSwizzle128B);
+    const uint64_t v_desc = smem_desc(smem_u32(ring), 1024, Sh::kGroup, kSwizzle128B);
     // S of group t = (Q of tile qt) K^T, K in stage st
     const auto scores = [&](int t, int qt, int st) {
+      const uint64_t qd = q_desc + qt * (Sh::kTileBytes >> 4), kd = k_desc + st * (Sh::kTileBytes >> 4);
 #pragma unroll
       for (int kb = 0; kb < D / 64; ++kb)
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_f16_p(leader, tmem + t * kKeys,
-                     smem_desc(smem_u32(q_s + qt * Sh::kTileBytes + kb * kBlockBytes + kk * 32), 16, 1024, kSwizzle128B),
-                     smem_desc(smem_u32(ring + st * Sh::kTileBytes + kb * kBlockBytes + kk * 32), 16, 1024, kSwizzle128B),
+          umma_f16_p(leader, tmem + t * kKeys, qd + ((kb * kBlockBytes + kk * 32) >> 4), kd + ((kb * 1024 + kk * 32) >> 4),
                      kIdescS, (kb > 0 || kk > 0) ? 1u : 0u);
       umma_commit_p(leader, smem_u32(&C.s_full[t]));
       last_bar = smem_u32(&C.s_full[t]);
       last_parity = steps[t]++ & 1;
     };
-    // O of tile t (+)= P V, V in stage st
+    // O of group t (+)= P V, V in stage st
     const auto values = [&](int t, int st, bool first, uint32_t step) {
+      const uint64_t vd = v_desc + st * (Sh::kTileBytes >> 4);
 #pragma unroll
       for (int ks = 0; ks < kKeys / 16; ++ks)
-        umma_f16_p(leader, tmem + 2 * kKeys + t * D,
-                   smem_desc(smem_u32(p_s + t * kPBytes + (ks / 4) * kBlockBytes + (ks % 4) * 32), 16, 1024, kSwizzle128B),
-                   smem_desc(smem_u32(ring + st * Sh::kTileBytes + ks * 16 * 128), kBlockBytes, 1024, kSwizzle128B),
-                   kIdescO, (!first || ks > 0) ? 1u : 0u);
+        umma_f16_p(leader, tmem + 2 * kKeys + t * D, p_desc + (((ks / 4) * kBlockBytes + (ks % 4) * 32) >> 4),
+                   vd + ((ks * 2 * Sh::kGroup) >> 4), kIdescO, (!first || ks > 0) ? 1u : 0u);
       umma_commit_p(leader, smem_u32(&C.pv_done[t]));
       last_bar = smem_u32(&C.pv_done[t]);
       last_parity = step & 1;
@@ -388,27 +375,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (ok) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(i)]));
       }
-      for (int j = 0; j < n && ok; ++j) {
-        const uint32_t ik = load0 + k_index(j + ahead, n, ahead), iv = load0 + v_index(j, n, ahead);
-        if (!kQuant && edge(c.tile0 + j)) {
-          const int t = split ? j & 1 : 0;
-          if (!wait(&C.kv_full[stage_of<D>(iv)], full_parity<D>(iv))) break;
-          mbar_arrive_p(leader, smem_u32(&C.v_ready[t]));
-        }
-        for (int x = 0; x < (split ? 1 : 2); ++x) {
-          const int t = split ? j & 1 : x;
-          const uint32_t step = s0[t] + (split ? j >> 1 : j);
-          // P of tile j written, so its scores are read: the group's next ones may replace them
-          if (!wait(&C.p_full[t], step & 1)) break;
-          const bool last = split || x == 1;
+      // Half steps h: group h & 1 takes its key tile.  Once it has read its scores, its next ones go
+      // out, then the product of the half step before: the groups find their next scores ready, and
+      // their products run under the other group's softmax.
+      const int halves = split ? n : 2 * n;
+      for (int h = 0; h <= halves && ok; ++h) {
+        if (h < halves) {
+          const int t = h & 1, j = split ? h : h >> 1;
+          const uint32_t step = s0[t] + (h >> 1);
           if (j + ahead < n) {
-            if (x == 0 && !wait(&C.kv_full[stage_of<D>(ik)], full_parity<D>(ik))) break;
+            const uint32_t ik = load0 + k_index(j + ahead, n, ahead);
+            if (!wait(&C.s_free[t], step & 1)) break;
+            if ((split || t == 0) && !wait(&C.kv_full[stage_of<D>(ik)], full_parity<D>(ik))) break;
             scores(t, split ? 0 : t, stage_of<D>(ik));
-            if (last) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(ik)]));
+            if (split || t == 1) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(ik)]));
           }
-          if (x == 0 && !wait(&C.kv_full[stage_of<D>(iv)], full_parity<D>(iv))) break;
+        }
+        if (h > 0) {
+          const int t = (h - 1) & 1, j = split ? h - 1 : (h - 1) >> 1;
+          const uint32_t step = s0[t] + ((h - 1) >> 1), iv = load0 + v_index(j, n, ahead);
+          if ((split || t == 0) && !wait(&C.kv_full[stage_of<D>(iv)], full_parity<D>(iv))) break;
+          if (!kQuant && (split || t == 0) && edge(c.tile0 + j)) mbar_arrive_p(leader, smem_u32(&C.v_ready[t]));
+          if (!wait(&C.p_full[t], step & 1)) break;
           values(t, stage_of<D>(iv), step == s0[t], step);
-          if (last) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(iv)]));
+          if (split || t == 1) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(iv)]));
         }
       }
       load0 += 2 * n;
@@ -426,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_s = tmem + lanes + t * kKeys, t_o = tmem + lanes + 2 * kKeys + t * D;
     const bool flip = p.scale < 0.f;  // a negative scale is folded into Q, so the largest score has the largest weight
     const float c2 = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
-    uint8_t* prow = p_s + t * kPBytes + r * 128;
+    uint8_t* prow = p_s + r * 128;
     const uint32_t sw = (uint32_t)(r & 7);
     uint32_t step = 0, load0 = 0, edges = 0, splits = 0, other_steps = 0;
     bool ok = true;
@@ -483,16 +473,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int x = 0; x < kKeys; x += 32) tmem_ld32(t_s + x, s + x);
         tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&C.s_free[t]));
         if (!kQuant && (split || t == 0) && edge(c.tile0 + j)) {
           // rows of V that nobody sees are zeroed: 0 x (whatever lies there) must not reach O
           ok = __all_sync(0xffffffffu, role_wait(C, smem_u32(&C.v_ready[t]), edges++ & 1));
           if (!ok) break;
           if (edge.unseen(v0 + r)) {
-            uint8_t* vrow = ring + stage_of<D>(load0 + v_index(j, n, split ? 2 : 1)) * Sh::kTileBytes + r * 128;
+            uint8_t* vrow = ring + stage_of<D>(load0 + v_index(j, n, split ? 2 : 1)) * Sh::kTileBytes +
+                            (r >> 3) * Sh::kGroup + (r & 7) * 128;
 #pragma unroll
             for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-              for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(vrow + h * kBlockBytes + x * 16) = make_uint4(0, 0, 0, 0);
+              for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(vrow + h * 1024 + x * 16) = make_uint4(0, 0, 0, 0);
           }
         }
         {
@@ -516,18 +509,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 4; ++i) mx[i] = x + 4 + i < kKeys ? fmaxf(mx[i], fmaxf(s[x + i], s[x + 4 + i])) : fmaxf(mx[i], s[x + i]);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
         const bool raise = top > m + kRescale;
-        bool waited = step == step0;  // O += P V of the group's tile before: P and O are free
         if (__any_sync(0xffffffffu, raise)) {
           const float alpha = raise ? ex2(m - top) : 1.f;
           if (raise) m = top;
           l *= alpha;
-          if (!waited) {
+          if (step > step0) {  // O += P V of the group's tile before is done: O may change
             ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);
             if (!__all_sync(0xffffffffu, ok)) {
               ok = false;
               break;
             }
-            waited = true;
             tc_fence_after();
 #pragma unroll 1
             for (int x = 0; x < D; x += 16) {
@@ -542,31 +533,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;  // nothing seen yet: 2^-inf = 0 for any reference
+        // products of the other group that come before this one's: they take turns, group 0 first
+        const uint32_t before = other_steps + (step - step0) + t;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t pk[kKeys / 2];
 #pragma unroll
-        for (int x = 0; x < kKeys; x += 32) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int y = 0; y < 32; y += 2) {
-            float2 e = fma2(make_float2(s[x + y], s[x + y + 1]), c2, -ref);
-            e.x = ex2(e.x);
-            e.y = ex2(e.y);
-            sum[(y >> 1) & 1] = add2(sum[(y >> 1) & 1], e);
-            pk[y / 2] = pack2<T>(e.x, e.y);
-          }
-          if (x == 0 && !waited) {
-            ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);
-            if (!__all_sync(0xffffffffu, ok)) {
-              ok = false;
-              break;
-            }
-          }
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            *reinterpret_cast<uint4*>(prow + (x / 64) * kBlockBytes + (((uint32_t)((x % 64) / 8 + y) ^ sw) << 4)) =
-                make_uint4(pk[4 * y], pk[4 * y + 1], pk[4 * y + 2], pk[4 * y + 3]);
+        for (int x = 0; x < kKeys; x += 2) {
+          float2 e = fma2(make_float2(s[x], s[x + 1]), c2, -ref);
+          e.x = ex2(e.x);
+          e.y = ex2(e.y);
+          sum[(x >> 1) & 1] = add2(sum[(x >> 1) & 1], e);
+          pk[x / 2] = pack2<T>(e.x, e.y);
         }
-        if (!ok) break;
+        if (before > 0) {  // the other group's product has read the P buffer
+          ok = role_wait(C, smem_u32(&C.pv_done[t ^ 1]), (before - 1) & 1);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < kKeys / 8; ++x)
+          *reinterpret_cast<uint4*>(prow + (x / 8) * kBlockBytes + (((uint32_t)(x % 8) ^ sw) << 4)) =
+              make_uint4(pk[4 * x], pk[4 * x + 1], pk[4 * x + 2], pk[4 * x + 3]);
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         fence_proxy_async_smem();
         tc_fence_before();
@@ -590,24 +579,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && step > step0) ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);
       const uint32_t t_x = tmem + lanes + 2 * kKeys + (t ^ 1) * D;  // the other group's O
       float f = 1.f, fx = 0.f;
-      int c0 = 0, c1 = D;
       if (split) {
-        // both groups meet: maxima and sums go through the P rows, O is read where it is, each
-        // group writes half of the dims
-        if (ok) {
-          *reinterpret_cast<float2*>(prow) = make_float2(m, l);
+        // group 1 hands its maxima and sums to group 0, which reads both O where they are and writes
+        // the rows out
+        if (t == 1) {
+          C.ml[r] = make_float2(m, l);
           tc_fence_before();
-          mbar_arrive(smem_u32(&C.x_ml[t]));
-          ok = role_wait(C, smem_u32(&C.x_ml[t ^ 1]), splits & 1);
+          if (ok) mbar_arrive(smem_u32(&C.x_ml));
+          ok = ok && role_wait(C, smem_u32(&C.x_done), splits++ & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_after();
+          continue;
         }
-        const float2 ml = *reinterpret_cast<const float2*>(p_s + (t ^ 1) * kPBytes + r * 128);
+        ok = ok && role_wait(C, smem_u32(&C.x_ml), splits++ & 1);
+        if (ok && other_steps > 0) ok = role_wait(C, smem_u32(&C.pv_done[1]), (other_steps - 1) & 1);
+        const float2 ml = C.ml[r];
         const float M = fmaxf(m, ml.x);
         f = m == -INFINITY ? 0.f : ex2(m - M);
         fx = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
         m = M;
         l = l * f + ml.y * fx;
-        c0 = t * (D / 2);
-        c1 = c0 + D / 2;
       }
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
@@ -619,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t slot = part_slot(c) * p.rows + R;
       T* out = reinterpret_cast<T*>(p.out) + (int64_t)(c.q_first + c.i0 + rt) * p.out_stride_tok +
                (int64_t)(c.kvh * p.group + c.slice * p.gw + g) * p.out_stride_head;
-      if (!whole && mine && (!split || t == 0)) {
+      if (!whole && mine) {
         p.part_ml[slot * 2] = m;
         p.part_ml[slot * 2 + 1] = l;
       }
@@ -629,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fx *= inv;
       }
 #pragma unroll 1
-      for (int x = c0; x < c1; x += 16) {
+      for (int x = 0; x < D; x += 16) {
         float o[16];
         tmem_ld16(t_o + x, o);
         if (split) {
@@ -657,12 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       tc_fence_before();
-      if (split) {
-        mbar_arrive(smem_u32(&C.x_done[t]));
-        ok = role_wait(C, smem_u32(&C.x_done[t ^ 1]), splits++ & 1);
-        ok = __all_sync(0xffffffffu, ok);
-        tc_fence_after();
-      }
+      if (split) mbar_arrive(smem_u32(&C.x_done));
     }
     if (!ok && lane == 0) give_up(C, p.err);
   }
@@ -680,10 +666,10 @@ int launch(const ChunkParams& p, cudaStream_t st) {
   CUtensorMap k_map = {}, v_map = {};
   if (!kQuant) {
     const uint64_t rows = (uint64_t)p.num_blocks * p.n_kv_heads * p.block_size;
-    const uint32_t box = p.block_size < kKeys ? p.block_size : kKeys;
+    const uint32_t groups = (p.block_size < kKeys ? p.block_size : kKeys) / 8;
     const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    if (!tensor_map_2d(&k_map, bf16, p.k_pool, D, rows, D * 2, 64, box) ||
-        !tensor_map_2d(&v_map, bf16, p.v_pool, D, rows, D * 2, 64, box)) {
+    if (!tensor_map_row_groups(&k_map, bf16, p.k_pool, rows, D, groups) ||
+        !tensor_map_row_groups(&v_map, bf16, p.v_pool, rows, D, groups)) {
       set_last_error("paged_chunk: tensor map encoding failed");
       return SNAPMIND_ERR_CUDA;
     }

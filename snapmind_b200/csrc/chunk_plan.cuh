@@ -259,6 +259,77 @@ struct PieceWalk {
   }
 };
 
+// Where the key tiles of a unit lie in the pool, 32 / parts tiles at a time: lane i holds part
+// i % parts (a block, or the tile's piece of a larger block) of tile first + i / parts as its pool
+// row (block * kv heads + kv head) * block_size + slot, or -1.  The entries of the next batch are
+// read while the current one is staged, so that no tile waits for the table.  (A read, a check and a
+// division per tile made the staging warp the bound of 8-bit decodes: 306 us for what takes 200 us
+// of copies.)
+struct TileRows {
+  const ChunkParams& p;
+  const KeyRange& kr;
+  const int32_t* table;
+  int kvh, end, lane;
+  int box, parts, log_parts;  // keys of a part, parts of a tile
+  int first, rows;            // the current batch
+  int prev_first, prev_rows;  // the batch before it
+  int32_t next;               // table entry of the batch after it
+
+  __device__ __forceinline__ TileRows(const ChunkParams& p_, const KeyRange& kr_, const Piece& c, int lane_)
+      : p(p_), kr(kr_), table(p_.tables + (int64_t)c.b * p_.table_stride), kvh(c.kvh), end(c.tile1), lane(lane_) {
+    box = min(p.block_size, p.key_tile);
+    parts = p.block_size >= p.key_tile ? 1 : p.by_block.div(p.key_tile);
+    log_parts = 31 - __clz(parts);  // a power of two: blocks of 8 .. 64 keys
+    first = c.tile0 - (32 >> log_parts);
+    rows = prev_rows = -1;
+    prev_first = first;
+    next = entry(c.tile0);
+  }
+  __device__ __forceinline__ int position(int first_tile) const {
+    const int v = (first_tile + (lane >> log_parts)) * p.key_tile + (lane & (parts - 1)) * box;
+    return v < kr.v_len ? kr.position(v) : -1;
+  }
+  // Table entry of the lane's part; INT32_MIN: no key there.
+  __device__ __forceinline__ int32_t entry(int first_tile) const {
+    const int pos = position(first_tile);
+    if (pos < 0 || first_tile + (lane >> log_parts) >= end) return INT32_MIN;
+    const int lb = p.by_block.div(pos);
+    return lb < p.table_width ? table[lb] : -1;
+  }
+  // Makes `tile` part of the current batch (tiles are asked for in ascending order).
+  __device__ __forceinline__ void advance(int tile) {
+    if (tile < first + (32 >> log_parts)) return;
+    prev_first = first;
+    prev_rows = rows;
+    first = tile;
+    const int32_t e = next;
+    rows = -1;
+    if (e >= 0 && e < p.num_blocks) {
+      const int pos = position(first);
+      rows = (e * p.n_kv_heads + kvh) * p.block_size + (pos - p.by_block.div(pos) * p.block_size);
+    } else if (e != INT32_MIN) {
+      flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
+    }
+    next = entry(first + (32 >> log_parts));
+  }
+  // Pool row of part x of a tile of the current batch or the one before (all lanes take part).
+  __device__ __forceinline__ int row(int tile, int x) const {
+    const bool cur = tile >= first;
+    return __shfl_sync(0xffffffffu, cur ? rows : prev_rows, ((tile - (cur ? first : prev_first)) << log_parts) + x);
+  }
+  // Parts of the tile that hold keys.
+  __device__ __forceinline__ uint32_t have(int tile) const {
+    const bool cur = tile >= first;
+    const uint32_t m = __ballot_sync(0xffffffffu, (cur ? rows : prev_rows) >= 0);
+    return m >> ((tile - (cur ? first : prev_first)) << log_parts) & (parts == 32 ? ~0u : (1u << parts) - 1u);
+  }
+  // The byte of a pool row's K (0) or V (1) scale: [block][head][2][slot].
+  __device__ __forceinline__ int64_t scale_at(int row, int kv) const {
+    const int slot = row - p.by_block.div(row) * p.block_size;
+    return 2 * (int64_t)row - slot + kv * p.block_size;
+  }
+};
+
 // Query heads of a slice (the last one of a group may be narrower).
 __device__ __forceinline__ int slice_heads(const ChunkParams& p, int slice) {
   return min(p.gw, p.group - slice * p.gw);

@@ -29,6 +29,7 @@ namespace {
 using namespace tc;
 
 constexpr int kD = 128, kTile = 64, kConsumers = 4, kThreads = (kConsumers + 1) * 32, kHeads = 8;
+constexpr int kScaleLanes = 2 * kTile / 16;  // lanes that fetch a tile's scale bytes, 16 each
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <bool kQuant> struct Stage {
@@ -92,13 +93,12 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
 // Byte offset of 16-byte piece `ch` (0..7) of row `row` in rows of 128 bytes, 128-byte swizzle.
 __device__ __forceinline__ uint32_t swz(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
 
-// A bulk copy of `bytes` (a multiple of 16, both addresses on 16 bytes) by the leading lane.
-__device__ __forceinline__ void bulk_load_p(uint32_t leader, uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %0, 0; @p cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%1], "
-      "[%2], %3, [%4]; }" ::"r"(leader),
-      "r"(dst), "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
+// 16 bytes global -> shared by the calling thread, then its arrival on `bar` once they landed.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 template <typename C>
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < St::kCount; ++i) {
-      mbar_init(smem_u32(&S.full[i]), 1);
+      mbar_init(smem_u32(&S.full[i]), kQuant ? 1 + kScaleLanes : 1);
       mbar_init(smem_u32(&S.empty[i]), kConsumers);
     }
     S.abort = 0;
@@ -151,55 +151,49 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == kConsumers) {
     // ------------------------------------------------------------------ producer
     const uint32_t leader = elect_one_sync();
+    // the scale bytes that a lane fetches: keys scale_key .. + 15 of K or V, from part scale_part
+    const int scale_kv = (lane >> 2) & 1, scale_key = (lane & 3) * 16;
+    const int scale_part = p.block_size < kTile ? p.by_block.div(scale_key) : 0;
+    const int scale_in = scale_key - scale_part * min(p.block_size, kTile);
     for (; on && ok; on = w.next(p)) {
       const Piece& c = w.c;
       const KeyRange kr = key_range(p, c.len, c.n, c.i0, c.i0 + 1);
-      const int bs = p.block_size, box = min(bs, kTile), per_tile = kTile / box;
-      const int32_t* table = p.tables + (int64_t)c.b * p.table_stride;
-      const auto block_of = [&](int j) -> int32_t {  // block of part `lane` of tile j, or -1
-        const int v = j * kTile + lane * box;
-        if (j >= c.tile1 || lane >= per_tile || v >= kr.v_len) return -1;
-        const int lb = p.by_block.div(kr.position(v));
-        if (lb >= p.table_width) {
-          flag_error(p.err, SNAPMIND_DEVERR_TABLE);
-          return -1;
-        }
-        const int32_t phys = table[lb];
-        if (phys < 0 || phys >= p.num_blocks) {
-          flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
-          return -1;
-        }
-        return phys;
-      };
-      int32_t next = block_of(c.tile0);
+      TileRows at(p, kr, c, lane);
+      const int box = at.box;
       for (int j = c.tile0; j < c.tile1; ++j, ++tile) {
-        const int32_t phys = next;
-        next = block_of(j + 1);
+        at.advance(j);
+        const uint32_t have = at.have(j);
         const int st = tile % St::kCount;
         ok = __all_sync(0xffffffffu, role_wait(S, smem_u32(&S.empty[st]), ((tile / St::kCount) & 1) ^ 1));
         if (!ok) break;
-        const int off = bs > kTile ? kr.position(j * kTile) % bs : 0;
-        const uint32_t have = __ballot_sync(0xffffffffu, phys >= 0);
         const uint32_t bar = smem_u32(&S.full[st]);
-        const uint32_t row_bytes = kQuant ? 2 * 128 + 2 : 4 * 128;
+        const uint32_t row_bytes = kQuant ? 2 * 128 : 4 * 128;
         mbar_arrive_expect_tx_p(leader, bar, __popc(have) * (uint32_t)box * row_bytes);
         const uint32_t dst = smem_u32(ring + st * St::kBytes);
-        for (int x = 0; x < per_tile; ++x) {
-          if (!(have >> x & 1)) continue;
-          const int32_t tl = __shfl_sync(0xffffffffu, phys, x) * p.n_kv_heads + c.kvh;
-          const int y = tl * bs + off;
+        if constexpr (kQuant) {
+          // the scales go by plain 16-byte copies, not as small bulk copies beside the boxes
+          const int sr = at.row(j, scale_part);
+          if (lane < kScaleLanes) {
+            if (sr >= 0) copy16(smem_u32(&S.scales[st][scale_kv][scale_key]), p.scales + at.scale_at(sr + scale_in, scale_kv));
+            copies_arrive(bar);
+          }
+        }
+        int ys[kTile / 16];  // all rows first: a shuffle between two copies costs more than the copies
+#pragma unroll
+        for (int x = 0; x < kTile / 16; ++x) ys[x] = at.row(j, x & (at.parts - 1));
+#pragma unroll
+        for (int x = 0; x < kTile / 16; ++x) {  // parts that are not there are predicated off
+          const int y = ys[x];
+          const uint32_t go = x < at.parts && y >= 0 ? leader : 0u;
           const uint32_t ro = x * box * 128;
           if constexpr (kQuant) {
-            tma_load_2d_p(leader, dst + St::kK + ro, &k_map, 0, y, bar);
-            tma_load_2d_p(leader, dst + St::kV + ro, &v_map, 0, y, bar);
-            const uint8_t* sc = p.scales + (int64_t)tl * 2 * bs + off;
-            bulk_load_p(leader, smem_u32(&S.scales[st][0][x * box]), sc, box, bar);
-            bulk_load_p(leader, smem_u32(&S.scales[st][1][x * box]), sc + bs, box, bar);
+            tma_load_2d_p(go, dst + St::kK + ro, &k_map, 0, y, bar);
+            tma_load_2d_p(go, dst + St::kV + ro, &v_map, 0, y, bar);
           } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              tma_load_2d_p(leader, dst + St::kK + h * St::kHalf + ro, &k_map, 64 * h, y, bar);
-              tma_load_2d_p(leader, dst + St::kV + h * St::kHalf + ro, &v_map, 64 * h, y, bar);
+              tma_load_2d_p(go, dst + St::kK + h * St::kHalf + ro, &k_map, 64 * h, y, bar);
+              tma_load_2d_p(go, dst + St::kV + h * St::kHalf + ro, &v_map, 64 * h, y, bar);
             }
           }
         }

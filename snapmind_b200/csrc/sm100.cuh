@@ -139,6 +139,14 @@ __device__ __forceinline__ void tma_load_2d_p(uint32_t leader, uint32_t dst, con
       "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_4d_p(uint32_t leader, uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                              int w, uint32_t bar) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %0, 0; @p cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::"
+      "bytes [%1], [%2, {%3, %4, %5, %6}], [%7]; }" ::"r"(leader),
+      "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
 __device__ __forceinline__ void tma_prefetch_3d_p(uint32_t leader, const CUtensorMap* map, int x, int y, int z) {
   asm volatile(
       "{ .reg .pred p; setp.ne.b32 p, %0, 0; @p cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%1, {%2, %3, %4}]; "
@@ -329,6 +337,22 @@ inline bool tensor_map_col_blocks(CUtensorMap* map, bool bf16, const void* base,
   const cuuint32_t box[3] = {64, box_rows, box_blocks ? box_blocks : blocks};
   const cuuint32_t estr[3] = {1, 1, 1};
   return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rows of `inner` 16-bit elements (a multiple of 64) as groups of 8 rows: a box of box_groups groups
+// lands as [group][64-element column block][8 rows][64 elements] (128-byte swizzle), so that whole
+// rows move in one copy and every 8-row atom stands a fixed distance from the next.
+inline bool tensor_map_row_groups(CUtensorMap* map, bool bf16, const void* base, uint64_t rows, uint32_t inner,
+                                  uint32_t box_groups) {
+  EncodeTiledFn fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t dims[4] = {64, 8, inner / 64, rows / 8};
+  const cuuint64_t strides[3] = {inner * 2ull, 128, inner * 16ull};
+  const cuuint32_t box[4] = {64, 8, inner / 64, box_groups};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
             dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
