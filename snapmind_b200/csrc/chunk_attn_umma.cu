@@ -11,8 +11,10 @@
 // then O is rescaled in TMEM, else O is never touched between the products.
 //   warps 0-3, 4-7  softmax of tile 0 / 1: thread = row = TMEM lane; they load their Q tile,
 //                   write P to shared memory, and write out the finished rows
-//   warp 8          issues the MMAs
-//   warps 9-11      stage K and V: two by TMA, or all three converting e4m3 rows
+//   warp 8          issues the MMAs; over 16-bit caches those of the scores only, and warp 11 those of
+//                   P V: a wait takes some 200 cycles next to operand reads that fill shared memory's
+//                   bandwidth, and the two streams cover each other's
+//   warps 9, 10     stage K and V by TMA; over 8-bit caches warps 9-11 convert e4m3 rows
 // P goes through shared memory, not through TMEM as an A operand: a kernel of this library that
 // read A from TMEM ended in a launch failure whose cause was not found.
 //   TMEM: S of tile 0 / 1 at columns 0 / 128, O at 256 / 256 + head_dim.
@@ -35,7 +37,7 @@ namespace {
 using namespace tc;
 
 constexpr int kTileM = 128, kKeys = 128;
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kValuesWarp = 11;
 constexpr int kConvert = 96;  // threads that convert e4m3 rows: warps 9-11
 constexpr uint32_t kBlockBytes = 128 * 128;  // 128 rows of 64 16-bit elements
 constexpr uint32_t kPBytes = 2 * kBlockBytes;
@@ -225,8 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool on = w.start(C.plan);
   if (warp >= kMmaWarp) {
   regs_dec<Regs<kQuant>::kOther>();
-  if (warp >= kLoadWarp) {
-    if (!kQuant && warp >= kLoadWarp + 2) on = false;
+  if (kQuant ? warp >= kLoadWarp : warp == kLoadWarp || warp == kLoadWarp + 1) {
     // ------------------------------------------------------------------ K and V stages
     uint32_t issued = 0;
     bool ok = true;
@@ -317,10 +318,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(smem_u32(&C.kv_full[stage_of<D>(i)]), full_parity<D>(i));
     }
   } else {
-    // ------------------------------------------------------------------ MMA issuer
+    // ------------------------------------------------------------------ MMA issuers
+    const bool do_s = warp == kMmaWarp, do_o = kQuant || warp == kValuesWarp;
     const uint32_t leader = elect_one_sync();
     uint32_t load0 = 0, piece = 0;
-    uint32_t steps[2] = {0, 0}, pieces1 = 0;  // scores of group 0 / 1 issued; pieces with a tile 1
+    uint32_t s0[2] = {0, 0}, pieces1 = 0;  // steps of group 0 / 1 before this piece; pieces with a tile 1
     uint32_t last_bar = 0, last_parity = 0;
     bool ok = true;
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t k_desc = smem_desc(smem_u32(ring), 16, Sh::kGroup, kSwizzle128B);
     const uint64_t v_desc = smem_desc(smem_u32(ring), 1024, Sh::kGroup, kSwizzle128B);
     // S of group t = (Q of tile qt) K^T, K in stage st
-    const auto scores = [&](int t, int qt, int st) {
+    const auto scores = [&](int t, int qt, int st, uint32_t step) {
       const uint64_t qd = q_desc + qt * (Sh::kTileBytes >> 4), kd = k_desc + st * (Sh::kTileBytes >> 4);
 #pragma unroll
       for (int kb = 0; kb < D / 64; ++kb)
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                      kIdescS, (kb > 0 || kk > 0) ? 1u : 0u);
       umma_commit_p(leader, smem_u32(&C.s_full[t]));
       last_bar = smem_u32(&C.s_full[t]);
-      last_parity = steps[t]++ & 1;
+      last_parity = step & 1;
     };
     // O of group t (+)= P V, V in stage st
     const auto values = [&](int t, int st, bool first, uint32_t step) {
@@ -364,14 +366,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool split = (i1 - c.i0) * p.gw <= kTileM;
       const int ahead = split ? 2 : 1;
       const EdgeTiles edge(p, key_range(p, c.len, c.n, c.i0, i1));
-      const uint32_t s0[2] = {steps[0], steps[1]};  // steps of the groups before this piece
       // the scores of the first tile(s)
-      for (int j = 0; j < min(n, ahead) && ok; ++j) {
+      for (int j = 0; j < min(n, ahead) && ok && do_s; ++j) {
         const uint32_t i = load0 + j;
         if (!wait(&C.kv_full[stage_of<D>(i)], full_parity<D>(i))) break;
         for (int t = 0; t < (split ? 1 : 2) && ok; ++t) {
           if (j == 0 && !wait(&C.q_full[t], (t == 0 ? piece : pieces1) & 1)) break;
-          scores(split ? j : t, t, stage_of<D>(i));
+          scores(split ? j : t, t, stage_of<D>(i), split && j == 1 ? s0[1] : s0[t]);
         }
         if (ok) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(i)]));
       }
@@ -380,18 +381,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       // their products run under the other group's softmax.
       const int halves = split ? n : 2 * n;
       for (int h = 0; h <= halves && ok; ++h) {
-        if (h < halves) {
+        if (do_s && h < halves) {
           const int t = h & 1, j = split ? h : h >> 1;
           const uint32_t step = s0[t] + (h >> 1);
           if (j + ahead < n) {
             const uint32_t ik = load0 + k_index(j + ahead, n, ahead);
             if (!wait(&C.s_free[t], step & 1)) break;
             if ((split || t == 0) && !wait(&C.kv_full[stage_of<D>(ik)], full_parity<D>(ik))) break;
-            scores(t, split ? 0 : t, stage_of<D>(ik));
+            scores(t, split ? 0 : t, stage_of<D>(ik), step + 1);
             if (split || t == 1) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(ik)]));
           }
         }
-        if (h > 0) {
+        if (do_o && h > 0) {
           const int t = (h - 1) & 1, j = split ? h - 1 : (h - 1) >> 1;
           const uint32_t step = s0[t] + ((h - 1) >> 1), iv = load0 + v_index(j, n, ahead);
           if ((split || t == 0) && !wait(&C.kv_full[stage_of<D>(iv)], full_parity<D>(iv))) break;
@@ -404,6 +405,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       load0 += 2 * n;
       ++piece;
       pieces1 += split ? 0 : 1;
+      s0[0] += split ? (n + 1) / 2 : n;
+      s0[1] += split ? n / 2 : n;
     }
     if (!ok && lane == 0) give_up(C, p.err);
     if (last_bar) mbar_wait(last_bar, last_parity);  // MMAs in flight end (bounded) before TMEM goes
