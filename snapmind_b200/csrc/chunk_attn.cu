@@ -246,34 +246,137 @@ __global__ void __launch_bounds__(kGenThreads) chunk_generic_kernel(ChunkParams 
 }
 
 // Merge of the cut units: block (c, y) works when CTA c holds the first cut inside a
-// unit, on rows y, y + gridDim.y, ...; pieces are CTA c - 1's slot 1, then slot 0 of CTAs
-// c .. last.  One warp per row, a lane per 4 dims (and 128 more): M = max m_i,
-// out = sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M).  32 pieces at a time: lane i holds
-// piece i's weight, and the rows of 8 pieces are in flight together (one at a time, the merge of
-// the 17 pieces of a decode took 25 us).
-constexpr int kMergeWarps = 4, kMergeBatch = 8;
+// unit, on rows y, y + gridDim.y, ... (in groups of kMergeRows); pieces are CTA c - 1's slot 1, then
+// slot 0 of CTAs c .. last.  M = max m_i, out = sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M).
+// The work is a few loads that wait for one another, so what counts is how many are in flight: a
+// warp takes kMergeRows rows of a unit cut into up to 8 pieces at once (one row at a time, the 256-row
+// units of a long chunk took 30 us), or one row of more pieces, 8 of them in flight (one at a
+// time, the 17 pieces of a decode took 25 us).  A lane holds 4 dims (and 128 more).
+constexpr int kMergeWarps = 4, kMergeBatch = 8, kMergeRows = 4;
+
+template <typename T>
+__device__ __forceinline__ void store4(T* out, int d, int D, const float4& v, bool vec) {
+  if (vec && d + 3 < D) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(out + d) = v;
+    } else {
+      T y[4] = {Conv<T>::from_f(v.x), Conv<T>::from_f(v.y), Conv<T>::from_f(v.z), Conv<T>::from_f(v.w)};
+      *reinterpret_cast<uint2*>(out + d) = *reinterpret_cast<const uint2*>(y);
+    }
+    return;
+  }
+  const float y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (d + u < D) out[d + u] = Conv<T>::from_f(y[u]);
+}
+__device__ __forceinline__ float4 load4(const float* o, int d, int D) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (D % 4 == 0) {
+    if (d < D) v = *reinterpret_cast<const float4*>(o + d);
+  } else {
+    if (d < D) v.x = o[d];
+    if (d + 1 < D) v.y = o[d + 1];
+    if (d + 2 < D) v.z = o[d + 2];
+    if (d + 3 < D) v.w = o[d + 3];
+  }
+  return v;
+}
+__device__ __forceinline__ void add4(float4& a, const float4& v, float f) {
+  a.x = fmaf(v.x, f, a.x);
+  a.y = fmaf(v.y, f, a.y);
+  a.z = fmaf(v.z, f, a.z);
+  a.w = fmaf(v.w, f, a.w);
+}
+__device__ __forceinline__ void mul4(float4& a, float f) {
+  a.x *= f;
+  a.y *= f;
+  a.z *= f;
+  a.w *= f;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkParams p) {
   // launched as a programmatic dependent of the attention kernel: complete and visible after this
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int cta = blockIdx.x + 1;
   const int4 h0 = *reinterpret_cast<const int4*>(p.heads + (int64_t)cta * kPieceInts);
-  const int2 h1 = *reinterpret_cast<const int2*>(p.heads + (int64_t)cta * kPieceInts + 4);
+  const int4 h1 = *reinterpret_cast<const int4*>(p.heads + (int64_t)cta * kPieceInts + 4);
   if (h0.x < 0 || h1.x != cta - 1) return;
-  const int b = h0.x, kvh = h0.y, slice = h0.z, i0 = h0.w, n_pieces = h1.y - cta + 2;
-  int first;
-  const int n = chunk_queries(p, b, &first);
+  const int kvh = h0.y, slice = h0.z, i0 = h0.w, n_pieces = h1.y - cta + 2, first = h1.z, n = h1.w;
   const int heads = slice_heads(p, slice), n_rows = (min(n, i0 + p.tokens) - i0) * p.gw;
   const int lane = threadIdx.x & 31, D = p.head_dim;
-  for (int r = blockIdx.y * kMergeWarps + (threadIdx.x >> 5); r < n_rows; r += gridDim.y * kMergeWarps) {
-    const int g = r % p.gw;
+  const bool vec = p.out_stride_tok % 4 == 0 && p.out_stride_head % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+  const auto slot = [&](int i, int r) { return ((int64_t)(cta - 1 + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + r; };
+  const auto out_row = [&](int r, int g) {
+    return reinterpret_cast<T*>(p.out) + (int64_t)(first + i0 + p.by_gw.div(r)) * p.out_stride_tok +
+           (int64_t)(kvh * p.group + slice * p.gw + g) * p.out_stride_head;
+  };
+  const int warp = blockIdx.y * kMergeWarps + (threadIdx.x >> 5), warps = gridDim.y * kMergeWarps;
+
+  if (n_pieces <= 8) {
+    for (int r0 = warp * kMergeRows; r0 < n_rows; r0 += warps * kMergeRows) {
+      // lane 8 x + i: piece i of row r0 + x
+      const int rl = r0 + (lane >> 3), il = lane & 7;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (rl < n_rows && il < n_pieces) ml = *reinterpret_cast<const float2*>(p.part_ml + slot(il, rl) * 2);
+      float4 acc[kMergeRows][2] = {};
+      float4 v[2][kMergeRows];  // the rows of two pieces at a time (each row's first 128 dims)
+      const auto fetch = [&](int i, int c) {
+#pragma unroll
+        for (int x = 0; x < kMergeRows; ++x) {
+          v[i & 1][x] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i < n_pieces && r0 + x < n_rows) v[i & 1][x] = load4(p.part_o + slot(i, r0 + x) * D, 128 * c + 4 * lane, D);
+        }
+      };
+      fetch(0, 0);
+      fetch(1, 0);
+      float M = ml.x;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      const float ref = M == -INFINITY ? 0.f : M;
+      float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - ref), L = ml.y * f;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      f *= M == -INFINITY ? 0.f : 1.f / L;  // a row that sees nothing: zeros
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (128 * c >= D) break;
+        if (c > 0) {
+          fetch(0, c);
+          fetch(1, c);
+        }
+        for (int i = 0; i < n_pieces; i += 2) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int x = 0; x < kMergeRows; ++x) {
+              const float fx = __shfl_sync(0xffffffffu, f, 8 * x + i + u);
+              if (i + u < n_pieces && fx != 0.f) add4(acc[x][c], v[u][x], fx);  // weight 0: the piece may hold anything
+            }
+            if (i + u + 2 < n_pieces) fetch(i + u + 2, c);
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kMergeRows; ++x) {
+        const int r = r0 + x, g = r - p.by_gw.div(r) * p.gw;
+        if (r >= n_rows || g >= heads) continue;
+        T* out = out_row(r, g);
+        store4(out, 4 * lane, D, acc[x][0], vec);
+        if (D > 128) store4(out, 128 + 4 * lane, D, acc[x][1], vec);
+      }
+    }
+    return;
+  }
+  for (int r = warp; r < n_rows; r += warps) {
+    const int g = r - p.by_gw.div(r) * p.gw;
     if (g >= heads) continue;
-    const auto slot = [&](int i) { return ((int64_t)(cta - 1 + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + r; };
     float M = -INFINITY, L = 0.f;
     float4 acc[2] = {};
-    for (int i0_ = 0; i0_ < n_pieces; i0_ += 32) {
+    for (int k0 = 0; k0 < n_pieces; k0 += 32) {  // lane i holds the weight of piece k0 + i
       float2 ml = make_float2(-INFINITY, 0.f);
-      if (i0_ + lane < n_pieces) ml = *reinterpret_cast<const float2*>(p.part_ml + slot(i0_ + lane) * 2);
+      if (k0 + lane < n_pieces) ml = *reinterpret_cast<const float2*>(p.part_ml + slot(k0 + lane, r) * 2);
       float mb = ml.x;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
@@ -285,57 +388,31 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
       L = L * old + ls;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        acc[c].x *= old;
-        acc[c].y *= old;
-        acc[c].z *= old;
-        acc[c].w *= old;
-      }
-      const int here = min(32, n_pieces - i0_);
+      mul4(acc[0], old);
+      mul4(acc[1], old);
+      const int here = min(32, n_pieces - k0);
       for (int k = 0; k < here; k += kMergeBatch) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int d = 128 * c + 4 * lane;
           if (128 * c >= D) break;
           float4 v[kMergeBatch];
 #pragma unroll
-          for (int u = 0; u < kMergeBatch; ++u) {
-            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (k + u >= here) continue;
-            const float* o = p.part_o + slot(i0_ + k + u) * D + d;
-            if (D % 4 == 0) {
-              if (d < D) v[u] = *reinterpret_cast<const float4*>(o);
-            } else {
-              if (d < D) v[u].x = o[0];
-              if (d + 1 < D) v[u].y = o[1];
-              if (d + 2 < D) v[u].z = o[2];
-              if (d + 3 < D) v[u].w = o[3];
-            }
-          }
+          for (int u = 0; u < kMergeBatch; ++u)
+            v[u] = k + u < here ? load4(p.part_o + slot(k0 + k + u, r) * D, 128 * c + 4 * lane, D) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int u = 0; u < kMergeBatch; ++u) {
             const float fu = __shfl_sync(0xffffffffu, f, (k + u) & 31);
-            if (k + u >= here || fu == 0.f) continue;  // a piece in which the row sees nothing adds nothing
-            acc[c].x = fmaf(v[u].x, fu, acc[c].x);
-            acc[c].y = fmaf(v[u].y, fu, acc[c].y);
-            acc[c].z = fmaf(v[u].z, fu, acc[c].z);
-            acc[c].w = fmaf(v[u].w, fu, acc[c].w);
+            if (k + u < here && fu != 0.f) add4(acc[c], v[u], fu);
           }
         }
       }
     }
     const float inv = M == -INFINITY ? 0.f : 1.f / L;
-    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(first + i0 + r / p.gw) * p.out_stride_tok +
-             (int64_t)(kvh * p.group + slice * p.gw + g) * p.out_stride_head;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int d = 128 * c + 4 * lane;
-      const float y[4] = {acc[c].x, acc[c].y, acc[c].z, acc[c].w};
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (d + u < D) out[d + u] = Conv<T>::from_f(M == -INFINITY ? 0.f : y[u] * inv);
-    }
+    mul4(acc[0], inv);
+    mul4(acc[1], inv);
+    T* out = out_row(r, g);
+    store4(out, 4 * lane, D, acc[0], vec);
+    if (D > 128) store4(out, 128 + 4 * lane, D, acc[1], vec);
   }
 }
 
@@ -367,7 +444,7 @@ int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st) {
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   const int used = p.gw * p.tokens;
-  cfg.gridDim = dim3(p.n_ctas - 1, (used + kMergeWarps - 1) / kMergeWarps);
+  cfg.gridDim = dim3(p.n_ctas - 1, (used + kMergeWarps * kMergeRows - 1) / (kMergeWarps * kMergeRows));
   cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = st;
   cfg.attrs = pdl;

@@ -50,7 +50,7 @@ struct ChunkParams {
   int32_t* err;
 };
 
-constexpr int kPieceInts = 8;   // b, kv head, slice, first token, first piece's CTA, last piece's CTA
+constexpr int kPieceInts = 8;   // b, kv head, slice, first token, first and last piece's CTA, first query row, new tokens
 constexpr int kMaxChunkBatch = 8192;
 
 // New tokens of sequence b: its first query row and their number.
@@ -353,6 +353,8 @@ __device__ inline void write_piece_info(const ChunkParams& p, const PlanShared& 
   h[3] = c.i0;
   h[4] = cta_of(s_u, S.total, S.n);  // the CTA that holds tile s_u
   h[5] = cta_of(e_u - 1, S.total, S.n);        // ... and tile e_u - 1
+  h[6] = c.q_first;
+  h[7] = c.n;
   h[0] = c.b;
 }
 
