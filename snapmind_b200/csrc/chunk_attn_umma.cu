@@ -11,18 +11,19 @@
 // then O is rescaled in TMEM, else O is never touched between the products.
 //   warps 0-3, 4-7  softmax of tile 0 / 1: thread = row = TMEM lane; they load their Q tile,
 //                   write P to shared memory, and write out the finished rows
-//   warp 8          issues the MMAs; over 16-bit caches those of the scores only, and warp 11 those of
-//                   P V: a wait takes some 200 cycles next to operand reads that fill shared memory's
-//                   bandwidth, and the two streams cover each other's
-//   warps 9, 10     stage K and V by TMA; over 8-bit caches warps 9-11 convert e4m3 rows
+//   warp 8          issues the MMAs of the scores, and another warp those of P V: a wait takes some
+//                   200 cycles next to operand reads that fill shared memory's bandwidth, and the two
+//                   streams cover each other's
+//   the others      stage K and V: two warps by TMA, or three and three converting e4m3 rows
 // P goes through shared memory, not through TMEM as an A operand: a kernel of this library that
 // read A from TMEM ended in a launch failure whose cause was not found.
 //   TMEM: S of tile 0 / 1 at columns 0 / 128, O at 256 / 256 + head_dim.
-//   Shared memory: Q 2 x [128 x D], P [128 x 128], then a ring of [128 x D] stages that K and V tiles
-//   take in the order K0, K1, V0, K2, V1, ... (128-byte swizzle everywhere).  The tiles share one P
-//   buffer: a tile's P is written after the other's product has read its own, which costs nothing
-//   while the tiles take turns, and the 32 KB are a fourth stage (three stages left every V on its way
-//   when it was needed: 4050 cycles a step of 2 x 128 x 128 scores).
+//   Shared memory: Q 2 x [128 x D], P [128 x 128], a ring of [128 x D] stages of K and one of V (128-byte
+//   swizzle everywhere).  The tiles share one P buffer: a tile's P is written after the other's
+//   product has read its own, which costs nothing while the tiles take turns, and the 32 KB are a
+//   fourth stage (with three, every V was still on its way when it was needed: 4050 cycles a step of
+//   2 x 128 x 128 scores).  Every ring has one producer and one consumer that go through it in
+//   order, so a barrier's parity always tells the phase that is meant.
 // Every wait is bounded and ends early once another role gave up; TMEM is released on
 // every path.
 #include <cuda.h>
@@ -37,8 +38,7 @@ namespace {
 using namespace tc;
 
 constexpr int kTileM = 128, kKeys = 128;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kValuesWarp = 11;
-constexpr int kConvert = 96;  // threads that convert e4m3 rows: warps 9-11
+constexpr int kConvert = 96;  // threads that convert the rows of an e4m3 stage (K and V: three warps each)
 constexpr uint32_t kBlockBytes = 128 * 128;  // 128 rows of 64 16-bit elements
 constexpr uint32_t kPBytes = 2 * kBlockBytes;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -46,15 +46,15 @@ constexpr float kRescale = 8.f;  // log2 headroom of the reference maximum
 
 template <int D> struct Shape {
   static constexpr uint32_t kTileBytes = D / 64 * kBlockBytes;  // a Q tile, a K or V stage
-  static constexpr int kStages = D == 64 ? 8 : 4;
-  static constexpr uint32_t kP = 2 * kTileBytes, kRing = kP + kPBytes;
+  static constexpr int kStages = D == 64 ? 4 : 2;  // of K, and of V
+  static constexpr uint32_t kP = 2 * kTileBytes, kRing = kP + kPBytes;  // K's stages, then V's
   // K and V stages are [8-row group][64-column block][8 rows x 128 bytes]
   static constexpr uint32_t kGroup = D / 64 * 1024;
-  static constexpr uint32_t kCtrl = kRing + kStages * kTileBytes;
+  static constexpr uint32_t kCtrl = kRing + 2 * kStages * kTileBytes;
 };
 
 struct Ctrl {
-  uint64_t kv_full[8], kv_empty[8];
+  uint64_t full[2][4], empty[2][4];  // K's and V's stages
   uint64_t q_full[2];   // softmax threads: the Q tile of a piece is in shared memory
   uint64_t s_full[2];   // MMA commit: scores ready
   uint64_t s_free[2];   // softmax threads: scores read (the group's next ones may replace them)
@@ -118,14 +118,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 
 // A piece whose rows all fit tile 0 runs split: both softmax groups take tile 0's rows, group t
 // the key tiles t, t + 2, ..., each with sums and an O of its own, added up at the end.
-//
-// The staged loads of a piece of n tiles are the first `ahead` K tiles (1, split 2), then for
-// every j K(j + ahead), while there is one, and V(j).
-__device__ __forceinline__ int k_index(int j, int n, int ahead) { return j < ahead ? j : 2 * j - ahead; }
-__device__ __forceinline__ int v_index(int j, int n, int ahead) {
-  const int lead = min(n, ahead);
-  return lead + j + min(j + 1, n - lead);
-}
 
 // Whether a key tile holds rows that no query of the unit sees: [u_s, u_lo) and from v_len on, on the
 // virtual axis.
@@ -140,9 +132,18 @@ struct EdgeTiles {
   __device__ __forceinline__ bool unseen(int v) const { return v >= v_len || (v < u_lo && v >= u_s); }
 };
 
-// Stage and parity of the load with running number i.
+// Stage and parity of the K or V tile with running number i.
 template <int D> __device__ __forceinline__ int stage_of(uint32_t i) { return i % Shape<D>::kStages; }
 template <int D> __device__ __forceinline__ uint32_t full_parity(uint32_t i) { return (i / Shape<D>::kStages) & 1; }
+
+// A pair of f32 times one factor, in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float b) {
+  float2 r;
+  asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %4}; mul.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b));
+  return r;
+}
 
 // 16 e4m3 codes of one row times 2^(byte - 127), as 16 elements of T.  The scale is a power
 // of two: exact in bf16, and in f16 as long as the value is a normal f16.
@@ -154,36 +155,36 @@ __device__ __forceinline__ void dequant16(const uint4& codes, uint8_t byte, uint
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 2] >> (16 * (i & 1))), __NV_E4M3);
-    float2 f = __half22float2(__half2(h));
-    f.x *= s;
-    f.y *= s;
+    const float2 f = mul2(__half22float2(__half2(h)), s);
     if constexpr (std::is_same<T, __half>::value) {  // hold to f16's range, keep NaN
-      if (fabsf(f.x) > 65504.f) f.x = copysignf(65504.f, f.x);
-      if (fabsf(f.y) > 65504.f) f.y = copysignf(65504.f, f.y);
+      o[i] = pack2<T>(fabsf(f.x) > 65504.f ? copysignf(65504.f, f.x) : f.x, fabsf(f.y) > 65504.f ? copysignf(65504.f, f.y) : f.y);
+    } else {
+      o[i] = pack2<T>(f.x, f.y);
     }
-    o[i] = pack2<T>(f.x, f.y);
   }
   lo = make_uint4(o[0], o[1], o[2], o[3]);
   hi = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
-// Three warpgroups.  They are launched with 168 registers a thread (3 x 128 x 168 = 64512); the third
-// gives up what the softmax threads, with a row of 128 scores each, need more of.
-constexpr int kThreads = 384;
-template <bool kQuant> struct Regs {
-  static constexpr int kOther = kQuant ? 120 : 104, kSoftmax = kQuant ? 192 : 200;
-  static_assert(kOther + 2 * kSoftmax <= 3 * 168, "register split");
+// The third warpgroup (e4m3: and the fourth) gives up registers that the softmax threads, with a row
+// of 128 scores each, need: 3 x 128 threads are launched with 168 each, 4 x 128 with 128.
+template <bool kQuant> struct Roles {
+  static constexpr int kThreads = kQuant ? 512 : 384, kLaunchRegs = kQuant ? 128 : 168;
+  static constexpr int kScores = 8, kValues = kQuant ? 9 : 11, kLoad = kQuant ? 10 : 9, kLoadWarps = kQuant ? 6 : 2;
+  static constexpr int kOther = kQuant ? 72 : 104, kSoftmax = kQuant ? 184 : 200;
+  static_assert((kThreads - 256) * kOther + 256 * kSoftmax <= kThreads * kLaunchRegs, "register split");
 };
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <typename T, int D, bool kQuant>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     chunk_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                       ChunkParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using Sh = Shape<D>;
+  using Ro = Roles<kQuant>;
   constexpr int kStages = Sh::kStages;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdescS = idesc_f16(kBf16, kTileM, kKeys, false, false);
@@ -195,9 +196,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(smem_u32(&C.kv_full[i]), kQuant ? kConvert : 2);
-      mbar_init(smem_u32(&C.kv_empty[i]), 1);
+    for (int i = 0; i < 2 * kStages; ++i) {
+      mbar_init(smem_u32(&C.full[i & 1][i >> 1]), kQuant ? kConvert : 1);
+      mbar_init(smem_u32(&C.empty[i & 1][i >> 1]), 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&C.q_full[t]), 128);
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     C.abort = 0;
     mbar_init_fence();
   }
-  if (warp == kMmaWarp) {
+  if (warp == Ro::kScores) {
     tmem_alloc(smem_u32(&C.tmem_base), 512);
     tmem_relinquish();
   }
@@ -225,89 +226,93 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   PieceWalk w;
   bool on = w.start(C.plan);
-  if (warp >= kMmaWarp) {
-  regs_dec<Regs<kQuant>::kOther>();
-  if (kQuant ? warp >= kLoadWarp : warp == kLoadWarp || warp == kLoadWarp + 1) {
+  if (warp >= Ro::kScores) {
+  regs_dec<Ro::kOther>();
+  if (warp >= Ro::kLoad && warp < Ro::kLoad + Ro::kLoadWarps) {
     // ------------------------------------------------------------------ K and V stages
+    const int kv = (warp - Ro::kLoad) / (Ro::kLoadWarps / 2);  // K or V
+    uint64_t* const full = C.full[kv];
+    uint64_t* const empty = C.empty[kv];
     uint32_t issued = 0;
     bool ok = true;
     for (; on && ok; on = w.next(p)) {
       const Piece& c = w.c;
       const KeyRange kr = key_range(p, c.len, c.n, c.i0, min(c.n, c.i0 + p.tokens));
-      const int n = c.tile1 - c.tile0;
       TileRows at(p, kr, c, lane);
       const int box = at.box;
-      const int ahead = (min(c.n, c.i0 + p.tokens) - c.i0) * p.gw > kTileM ? 1 : 2, lead = min(n, ahead);
-      for (int i = 0; i < 2 * n && ok; ++i) {
-        // load i of the piece: tile j of K (0) or V (1)
-        const int r = i - lead;
-        const int kv = r < 0 ? 0 : (r < 2 * (n - lead) ? r & 1 : 1);
-        const int j = r < 0 ? i : (r < 2 * (n - lead) ? r / 2 + (kv ? 0 : ahead) : r - (n - lead));
-        const int tile = c.tile0 + j;  // V follows its K by one or two tiles: in the batch, or the one before
-        if (kv == 0) at.advance(tile);
+      for (int tile = c.tile0; tile < c.tile1 && ok; ++tile) {
+        at.advance(tile);
         const int st = stage_of<D>(issued);
-        uint8_t* dst = ring + st * Sh::kTileBytes;
+        uint8_t* dst = ring + (kv * kStages + st) * Sh::kTileBytes;
         if constexpr (!kQuant) {
           const uint32_t leader = elect_one_sync();
-          ok = __all_sync(0xffffffffu, role_wait(C, smem_u32(&C.kv_empty[st]), full_parity<D>(issued) ^ 1));
+          ok = __all_sync(0xffffffffu, role_wait(C, smem_u32(&empty[st]), full_parity<D>(issued) ^ 1));
           if (!ok) break;
-          // the two warps take every second part: a copy takes a warp over 100 cycles to issue
-          const int h = warp - kLoadWarp;
-          const uint32_t bar = smem_u32(&C.kv_full[st]);
-          mbar_arrive_expect_tx_p(leader, bar, __popc(at.have(tile) & (0x55555555u << h)) * (uint32_t)box * (D * 2u));
+          const uint32_t bar = smem_u32(&full[st]);
+          mbar_arrive_expect_tx_p(leader, bar, __popc(at.have(tile)) * (uint32_t)box * (D * 2u));
           const CUtensorMap* map = kv == 0 ? &k_map : &v_map;
           const uint32_t to = smem_u32(dst);
-          for (int x0 = h; x0 < at.parts; x0 += 8) {
-            int y[4];  // all rows first: a shuffle between two copies costs more than the copies
+          for (int x0 = 0; x0 < at.parts; x0 += 8) {
+            int y[8];  // all rows first: a shuffle between two copies costs more than the copies
 #pragma unroll
-            for (int x = 0; x < 4; ++x) y[x] = at.row(tile, (x0 + 2 * x) & (at.parts - 1));
+            for (int x = 0; x < 8; ++x) y[x] = at.row(tile, (x0 + x) & (at.parts - 1));
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              tma_load_4d_p(x0 + 2 * x < at.parts && y[x] >= 0 ? leader : 0u, to + (x0 + 2 * x) * box * (D * 2), map, 0, 0, 0,
+            for (int x = 0; x < 8; ++x)
+              tma_load_4d_p(x0 + x < at.parts && y[x] >= 0 ? leader : 0u, to + (x0 + x) * box * (D * 2), map, 0, 0, 0,
                             y[x] >> 3, bar);
           }
         } else {
-          // D / 16 lanes share a row (16 codes each), kRowsPass rows a pass
+          // D / 16 lanes share a row (16 codes each), kRowsPass rows a pass; the passes go in batches of
+          // kBatch, one batch's rows on their way while another is converted
           constexpr int kLanes = D / 16, kRowsPass = kConvert / kLanes, kPasses = (128 + kRowsPass - 1) / kRowsPass;
-          const int ct = tid - kLoadWarp * 32, ch = ct % kLanes, r0 = ct / kLanes;
-          const uint8_t* pool = static_cast<const uint8_t*>(kv == 0 ? p.k_pool : p.v_pool);
-          uint4 codes[kPasses];
-          uint8_t sc[kPasses];
+          constexpr int kBatch = 3, kBatches = (kPasses + kBatch - 1) / kBatch;
+          const int ct = tid - (Ro::kLoad + 3 * kv) * 32, ch = ct % kLanes, r0 = ct / kLanes;
+          const uint8_t* pool = static_cast<const uint8_t*>(kv == 0 ? p.k_pool : p.v_pool) + ch * 16;
+          uint4 codes[2][kBatch];
+          uint8_t sc[2][kBatch];
+          const auto fetch = [&](int b) {
 #pragma unroll
-          for (int x = 0; x < kPasses; ++x) {
-            const int r = x * kRowsPass + r0;
-            const int part = min(r, 127) >> (7 - at.log_parts), y = at.row(tile, part);  // 128 keys: box = 128 >> log_parts
-            const int v = (c.tile0 + j) * kKeys + r;
-            // rows that no query of the unit sees are zeros: past the end, or in a block that is
-            // read between the sinks and the first window
-            const int pos = kr.position(v);
-            const bool seen = r < 128 && y >= 0 && v < kr.v_len && (pos >= kr.win_lo || pos < p.sinks);
-            codes[x] = make_uint4(0, 0, 0, 0);
-            sc[x] = 0;
-            if (seen) {
-              const int row = y + (r - part * box);
-              codes[x] = *reinterpret_cast<const uint4*>(pool + (int64_t)row * D + ch * 16);
-              sc[x] = p.scales[at.scale_at(row, kv)];
+            for (int x = 0; x < kBatch; ++x) {
+              const int r = (b * kBatch + x) * kRowsPass + r0;
+              const int part = min(r, 127) >> (7 - at.log_parts), y = at.row(tile, part);  // 128 keys: box = 128 >> log_parts
+              const int v = tile * kKeys + r;
+              // rows that no query of the unit sees are zeros: past the end, or in a block that is
+              // read between the sinks and the first window
+              const int pos = kr.position(v);
+              const bool seen = r < 128 && y >= 0 && v < kr.v_len && (pos >= kr.win_lo || pos < p.sinks);
+              codes[b & 1][x] = make_uint4(0, 0, 0, 0);
+              sc[b & 1][x] = 0;
+              if (seen) {
+                const int row = y + (r - part * box);
+                codes[b & 1][x] = *reinterpret_cast<const uint4*>(pool + (int64_t)row * D);
+                sc[b & 1][x] = p.scales[at.scale_at(row, kv)];
+              }
             }
-          }
-          ok = role_wait(C, smem_u32(&C.kv_empty[st]), full_parity<D>(issued) ^ 1);
+          };
+          fetch(0);
+          fetch(1);
+          ok = role_wait(C, smem_u32(&empty[st]), full_parity<D>(issued) ^ 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
 #pragma unroll
-          for (int x = 0; x < kPasses; ++x) {
-            const int r = x * kRowsPass + r0;
-            if (r >= 128) break;
-            uint4 lo, hi;
-            dequant16<T>(codes[x], sc[x], lo, hi);
-            uint8_t* row = dst + (r >> 3) * Sh::kGroup + (ch / 4) * 1024 + (r & 7) * 128;
-            const uint32_t sw = r & 7, c0 = (ch % 4) * 2;
-            // lanes of the two 64-element halves write opposite pieces: no bank is hit twice
-            const bool swap = ch >= 4;
-            *reinterpret_cast<uint4*>(row + ((c0 + swap) ^ sw) * 16) = swap ? hi : lo;
-            *reinterpret_cast<uint4*>(row + ((c0 + !swap) ^ sw) * 16) = swap ? lo : hi;
+          for (int b = 0; b < kBatches; ++b) {
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x) {
+              const int r = (b * kBatch + x) * kRowsPass + r0;
+              if (r >= 128) break;
+              uint4 lo, hi;
+              dequant16<T>(codes[b & 1][x], sc[b & 1][x], lo, hi);
+              uint8_t* row = dst + (r >> 3) * Sh::kGroup + (ch / 4) * 1024 + (r & 7) * 128;
+              const uint32_t sw = r & 7, c0 = (ch % 4) * 2;
+              // lanes of the two 64-element halves write opposite pieces: no bank is hit twice
+              const bool swap = ch >= 4;
+              *reinterpret_cast<uint4*>(row + ((c0 + swap) ^ sw) * 16) = swap ? hi : lo;
+              *reinterpret_cast<uint4*>(row + ((c0 + !swap) ^ sw) * 16) = swap ? lo : hi;
+            }
+            if (b + 2 < kBatches) fetch(b + 2);
           }
           fence_proxy_async_smem();
-          mbar_arrive(smem_u32(&C.kv_full[st]));
+          mbar_arrive(smem_u32(&full[st]));
         }
         ++issued;
       }
@@ -315,13 +320,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0) give_up(C, p.err);
     if constexpr (!kQuant) {  // before the shared memory goes: every copy issued has landed (bounded)
       for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
-        mbar_wait(smem_u32(&C.kv_full[stage_of<D>(i)]), full_parity<D>(i));
+        mbar_wait(smem_u32(&full[stage_of<D>(i)]), full_parity<D>(i));
     }
   } else {
     // ------------------------------------------------------------------ MMA issuers
-    const bool do_s = warp == kMmaWarp, do_o = kQuant || warp == kValuesWarp;
+    const bool do_s = warp == Ro::kScores, do_o = warp == Ro::kValues;
     const uint32_t leader = elect_one_sync();
-    uint32_t load0 = 0, piece = 0;
+    uint32_t tiles = 0, piece = 0;  // key tiles, pieces before this one
     uint32_t s0[2] = {0, 0}, pieces1 = 0;  // steps of group 0 / 1 before this piece; pieces with a tile 1
     uint32_t last_bar = 0, last_parity = 0;
     bool ok = true;
@@ -334,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, 1024, kSwizzle128B);
     const uint64_t p_desc = smem_desc(smem_u32(p_s), 16, 1024, kSwizzle128B);
     const uint64_t k_desc = smem_desc(smem_u32(ring), 16, Sh::kGroup, kSwizzle128B);
-    const uint64_t v_desc = smem_desc(smem_u32(ring), 1024, Sh::kGroup, kSwizzle128B);
+    const uint64_t v_desc = smem_desc(smem_u32(ring + kStages * Sh::kTileBytes), 1024, Sh::kGroup, kSwizzle128B);
     // S of group t = (Q of tile qt) K^T, K in stage st
     const auto scores = [&](int t, int qt, int st, uint32_t step) {
       const uint64_t qd = q_desc + qt * (Sh::kTileBytes >> 4), kd = k_desc + st * (Sh::kTileBytes >> 4);
@@ -367,14 +372,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int ahead = split ? 2 : 1;
       const EdgeTiles edge(p, key_range(p, c.len, c.n, c.i0, i1));
       // the scores of the first tile(s)
+      if (do_s && wait(&C.q_full[0], piece & 1) && !split) wait(&C.q_full[1], pieces1 & 1);
+      for (int t = 0; t < 2 && ok && do_s; ++t)  // and the groups have read the last scores of the piece before
+        if (s0[t] > 0) wait(&C.s_free[t], (s0[t] - 1) & 1);
       for (int j = 0; j < min(n, ahead) && ok && do_s; ++j) {
-        const uint32_t i = load0 + j;
-        if (!wait(&C.kv_full[stage_of<D>(i)], full_parity<D>(i))) break;
+        const uint32_t i = tiles + j;
+        if (!wait(&C.full[0][stage_of<D>(i)], full_parity<D>(i))) break;
         for (int t = 0; t < (split ? 1 : 2) && ok; ++t) {
-          if (j == 0 && !wait(&C.q_full[t], (t == 0 ? piece : pieces1) & 1)) break;
           scores(split ? j : t, t, stage_of<D>(i), split && j == 1 ? s0[1] : s0[t]);
         }
-        if (ok) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(i)]));
+        if (ok) umma_commit_p(leader, smem_u32(&C.empty[0][stage_of<D>(i)]));
       }
       // Half steps h: group h & 1 takes its key tile.  Once it has read its scores, its next ones go
       // out, then the product of the half step before: the groups find their next scores ready, and
@@ -385,24 +392,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int t = h & 1, j = split ? h : h >> 1;
           const uint32_t step = s0[t] + (h >> 1);
           if (j + ahead < n) {
-            const uint32_t ik = load0 + k_index(j + ahead, n, ahead);
+            const uint32_t ik = tiles + j + ahead;
             if (!wait(&C.s_free[t], step & 1)) break;
-            if ((split || t == 0) && !wait(&C.kv_full[stage_of<D>(ik)], full_parity<D>(ik))) break;
+            if ((split || t == 0) && !wait(&C.full[0][stage_of<D>(ik)], full_parity<D>(ik))) break;
             scores(t, split ? 0 : t, stage_of<D>(ik), step + 1);
-            if (split || t == 1) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(ik)]));
+            if (split || t == 1) umma_commit_p(leader, smem_u32(&C.empty[0][stage_of<D>(ik)]));
           }
         }
         if (do_o && h > 0) {
           const int t = (h - 1) & 1, j = split ? h - 1 : (h - 1) >> 1;
-          const uint32_t step = s0[t] + ((h - 1) >> 1), iv = load0 + v_index(j, n, ahead);
-          if ((split || t == 0) && !wait(&C.kv_full[stage_of<D>(iv)], full_parity<D>(iv))) break;
+          const uint32_t step = s0[t] + ((h - 1) >> 1), iv = tiles + j;
+          if ((split || t == 0) && !wait(&C.full[1][stage_of<D>(iv)], full_parity<D>(iv))) break;
           if (!kQuant && (split || t == 0) && edge(c.tile0 + j)) mbar_arrive_p(leader, smem_u32(&C.v_ready[t]));
           if (!wait(&C.p_full[t], step & 1)) break;
           values(t, stage_of<D>(iv), step == s0[t], step);
-          if (split || t == 1) umma_commit_p(leader, smem_u32(&C.kv_empty[stage_of<D>(iv)]));
+          if (split || t == 1) umma_commit_p(leader, smem_u32(&C.empty[1][stage_of<D>(iv)]));
         }
       }
-      load0 += 2 * n;
+      tiles += n;
       ++piece;
       pieces1 += split ? 0 : 1;
       s0[0] += split ? (n + 1) / 2 : n;
@@ -413,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   } else {
     // ------------------------------------------------------------------ softmax: thread = row
-    regs_inc<Regs<kQuant>::kSoftmax>();
+    regs_inc<Ro::kSoftmax>();
     const int t = warp >> 2, r = tid & 127;
     const uint32_t lanes = ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t t_s = tmem + lanes + t * kKeys, t_o = tmem + lanes + 2 * kKeys + t * D;
@@ -421,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float c2 = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
     uint8_t* prow = p_s + r * 128;
     const uint32_t sw = (uint32_t)(r & 7);
-    uint32_t step = 0, load0 = 0, edges = 0, splits = 0, other_steps = 0;
+    uint32_t step = 0, tiles = 0, edges = 0, splits = 0, other_steps = 0;
     bool ok = true;
     // Q tile t of a piece, by the group's 128 threads
     const auto load_q = [&](const Piece& c) {
@@ -483,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = __all_sync(0xffffffffu, role_wait(C, smem_u32(&C.v_ready[t]), edges++ & 1));
           if (!ok) break;
           if (edge.unseen(v0 + r)) {
-            uint8_t* vrow = ring + stage_of<D>(load0 + v_index(j, n, split ? 2 : 1)) * Sh::kTileBytes +
+            uint8_t* vrow = ring + (kStages + stage_of<D>(tiles + j)) * Sh::kTileBytes +
                             (r >> 3) * Sh::kGroup + (r & 7) * 128;
 #pragma unroll
             for (int h = 0; h < D / 64; ++h)
@@ -566,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++step;
       }
       if (!ok) break;
-      load0 += 2 * n;
+      tiles += n;
       if (split) {
         // the other group's scores read tile 0's Q too: all done before the next Q may land there
         // (group 0's last scores follow all but the last of group 1's, so the phase is the one meant)
@@ -658,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (warp == kMmaWarp) {
+  if (warp == Ro::kScores) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -680,7 +687,7 @@ int launch(const ChunkParams& p, cudaStream_t st) {
   auto kernel = chunk_umma_kernel<T, D, kQuant>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>());
   if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
-  kernel<<<p.n_ctas, kThreads, smem_bytes<D>(), st>>>(k_map, v_map, p);
+  kernel<<<p.n_ctas, Roles<kQuant>::kThreads, smem_bytes<D>(), st>>>(k_map, v_map, p);
   return cuda_status(cudaGetLastError(), "paged_chunk launch");
 }
 

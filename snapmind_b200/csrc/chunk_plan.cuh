@@ -272,7 +272,6 @@ struct TileRows {
   int kvh, end, lane;
   int box, parts, log_parts;  // keys of a part, parts of a tile
   int first, rows;            // the current batch
-  int prev_first, prev_rows;  // the batch before it
   int32_t next;               // table entry of the batch after it
 
   __device__ __forceinline__ TileRows(const ChunkParams& p_, const KeyRange& kr_, const Piece& c, int lane_)
@@ -281,8 +280,7 @@ struct TileRows {
     parts = p.block_size >= p.key_tile ? 1 : p.by_block.div(p.key_tile);
     log_parts = 31 - __clz(parts);  // a power of two: blocks of 8 .. 64 keys
     first = c.tile0 - (32 >> log_parts);
-    rows = prev_rows = -1;
-    prev_first = first;
+    rows = -1;
     next = entry(c.tile0);
   }
   __device__ __forceinline__ int position(int first_tile) const {
@@ -299,8 +297,6 @@ struct TileRows {
   // Makes `tile` part of the current batch (tiles are asked for in ascending order).
   __device__ __forceinline__ void advance(int tile) {
     if (tile < first + (32 >> log_parts)) return;
-    prev_first = first;
-    prev_rows = rows;
     first = tile;
     const int32_t e = next;
     rows = -1;
@@ -312,16 +308,13 @@ struct TileRows {
     }
     next = entry(first + (32 >> log_parts));
   }
-  // Pool row of part x of a tile of the current batch or the one before (all lanes take part).
+  // Pool row of part x of a tile of the current batch (all lanes take part).
   __device__ __forceinline__ int row(int tile, int x) const {
-    const bool cur = tile >= first;
-    return __shfl_sync(0xffffffffu, cur ? rows : prev_rows, ((tile - (cur ? first : prev_first)) << log_parts) + x);
+    return __shfl_sync(0xffffffffu, rows, ((tile - first) << log_parts) + x);
   }
   // Parts of the tile that hold keys.
   __device__ __forceinline__ uint32_t have(int tile) const {
-    const bool cur = tile >= first;
-    const uint32_t m = __ballot_sync(0xffffffffu, (cur ? rows : prev_rows) >= 0);
-    return m >> ((tile - (cur ? first : prev_first)) << log_parts) & (parts == 32 ? ~0u : (1u << parts) - 1u);
+    return __ballot_sync(0xffffffffu, rows >= 0) >> ((tile - first) << log_parts) & ((1u << parts) - 1u);
   }
   // The byte of a pool row's K (0) or V (1) scale: [block][head][2][slot].
   __device__ __forceinline__ int64_t scale_at(int row, int kv) const {
