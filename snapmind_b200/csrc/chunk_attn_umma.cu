@@ -14,7 +14,8 @@
 //   warp 8          issues the MMAs of the scores, and another warp those of P V: a wait takes some
 //                   200 cycles next to operand reads that fill shared memory's bandwidth, and the two
 //                   streams cover each other's
-//   the others      stage K and V: two warps by TMA, or three and three converting e4m3 rows
+//   two more        stage K and V by TMA; over 8-bit caches as they are, and four warps more turn
+//                   the rows into 16-bit stages
 // P goes through shared memory, not through TMEM as an A operand: a kernel of this library that
 // read A from TMEM ended in a launch failure whose cause was not found.
 //   TMEM: S of tile 0 / 1 at columns 0 / 128, O at 256 / 256 + head_dim.
@@ -38,19 +39,24 @@ namespace {
 using namespace tc;
 
 constexpr int kTileM = 128, kKeys = 128;
-constexpr int kConvert = 96;  // threads that convert the rows of an e4m3 stage (K and V: three warps each)
+constexpr int kConvert = 128;  // threads that convert e4m3 rows
 constexpr uint32_t kBlockBytes = 128 * 128;  // 128 rows of 64 16-bit elements
 constexpr uint32_t kPBytes = 2 * kBlockBytes;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // log2 headroom of the reference maximum
 
-template <int D> struct Shape {
+template <int D, bool kQuant> struct Shape {
   static constexpr uint32_t kTileBytes = D / 64 * kBlockBytes;  // a Q tile, a K or V stage
-  static constexpr int kStages = D == 64 ? 4 : 2;  // of K, and of V
-  static constexpr uint32_t kP = 2 * kTileBytes, kRing = kP + kPBytes;  // K's stages, then V's
+  static constexpr int kK = D == 64 ? 4 : 2, kV = kK - (kQuant ? 1 : 0);  // stages
+  static constexpr uint32_t kRawBytes = kQuant ? 128 * D : 0;             // codes of a K or V tile
+  static constexpr uint32_t kP = 2 * kTileBytes, kRing = kP + kPBytes;    // K's stages, then V's
+  static constexpr uint32_t kRaw = kRing + (kK + kV) * kTileBytes, kCtrl = kRaw + 2 * kRawBytes;
   // K and V stages are [8-row group][64-column block][8 rows x 128 bytes]
   static constexpr uint32_t kGroup = D / 64 * 1024;
-  static constexpr uint32_t kCtrl = kRing + 2 * kStages * kTileBytes;
+  // Stage and parity of the K (0) or V (1) tile with running number i.
+  __device__ __forceinline__ static int stage(int kv, uint32_t i) { return kv == 0 ? i % kK : i % kV; }
+  __device__ __forceinline__ static uint32_t parity(int kv, uint32_t i) { return (kv == 0 ? i / kK : i / kV) & 1; }
+  __device__ __forceinline__ static uint32_t at(int kv, uint32_t i) { return kRing + (kv * kK + stage(kv, i)) * kTileBytes; }
 };
 
 struct Ctrl {
@@ -62,15 +68,20 @@ struct Ctrl {
   uint64_t pv_done[2];  // MMA commit: O += P V done
   uint64_t x_ml;        // split: group 1's maxima and sums are in `ml`, its O is final
   uint64_t x_done;      // split: group 0 has read them
+  uint64_t raw_full[2], raw_empty[2];  // e4m3: codes and scales of a K / V tile
   uint64_t v_ready[2];  // MMA warp: V of an edge tile has landed (its unseen rows may be zeroed)
   uint32_t tmem_base;
   int32_t abort;
   PlanShared plan;
+  alignas(16) uint8_t scales[2][128];
   float2 ml[128];
 };
 
-template <int D> constexpr size_t smem_bytes() { return 1024 + Shape<D>::kCtrl + sizeof(Ctrl); }
-static_assert(smem_bytes<128>() <= 232448 && smem_bytes<64>() <= 232448, "shared memory budget");
+static_assert(offsetof(Ctrl, scales) % 16 == 0, "16-byte copies land there");
+
+template <int D, bool kQuant> constexpr size_t smem_bytes() { return 1024 + Shape<D, kQuant>::kCtrl + sizeof(Ctrl); }
+static_assert(smem_bytes<128, false>() <= 232448 && smem_bytes<128, true>() <= 232448, "shared memory budget");
+static_assert(smem_bytes<64, false>() <= 232448 && smem_bytes<64, true>() <= 232448, "shared memory budget");
 static_assert(kPBytes >= kMaxChunkBatch * 4, "plan scratch in the P tiles");
 
 __device__ __forceinline__ bool role_wait(const Ctrl& C, uint32_t bar, uint32_t parity) {
@@ -132,10 +143,6 @@ struct EdgeTiles {
   __device__ __forceinline__ bool unseen(int v) const { return v >= v_len || (v < u_lo && v >= u_s); }
 };
 
-// Stage and parity of the K or V tile with running number i.
-template <int D> __device__ __forceinline__ int stage_of(uint32_t i) { return i % Shape<D>::kStages; }
-template <int D> __device__ __forceinline__ uint32_t full_parity(uint32_t i) { return (i / Shape<D>::kStages) & 1; }
-
 // A pair of f32 times one factor, in one instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float b) {
   float2 r;
@@ -170,7 +177,7 @@ __device__ __forceinline__ void dequant16(const uint4& codes, uint8_t byte, uint
 // of 128 scores each, need: 3 x 128 threads are launched with 168 each, 4 x 128 with 128.
 template <bool kQuant> struct Roles {
   static constexpr int kThreads = kQuant ? 512 : 384, kLaunchRegs = kQuant ? 128 : 168;
-  static constexpr int kScores = 8, kValues = kQuant ? 9 : 11, kLoad = kQuant ? 10 : 9, kLoadWarps = kQuant ? 6 : 2;
+  static constexpr int kScores = 8, kValues = 11, kLoad = 9, kConvertWarp = 12;
   static constexpr int kOther = kQuant ? 72 : 104, kSoftmax = kQuant ? 184 : 200;
   static_assert((kThreads - 256) * kOther + 256 * kSoftmax <= kThreads * kLaunchRegs, "register split");
 };
@@ -183,22 +190,24 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
                       ChunkParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  using Sh = Shape<D>;
+  using Sh = Shape<D, kQuant>;
   using Ro = Roles<kQuant>;
-  constexpr int kStages = Sh::kStages;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdescS = idesc_f16(kBf16, kTileM, kKeys, false, false);
   constexpr uint32_t kIdescO = idesc_f16(kBf16, kTileM, D, false, true);
   uint8_t* q_s = base;
   uint8_t* p_s = base + Sh::kP;
-  uint8_t* ring = base + Sh::kRing;
   Ctrl& C = *reinterpret_cast<Ctrl*>(base + Sh::kCtrl);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
-    for (int i = 0; i < 2 * kStages; ++i) {
+    for (int i = 0; i < 2 * Sh::kK; ++i) {
       mbar_init(smem_u32(&C.full[i & 1][i >> 1]), kQuant ? kConvert : 1);
       mbar_init(smem_u32(&C.empty[i & 1][i >> 1]), 1);
+    }
+    for (int kv = 0; kv < 2; ++kv) {
+      mbar_init(smem_u32(&C.raw_full[kv]), 1 + 32);
+      mbar_init(smem_u32(&C.raw_empty[kv]), kConvert);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&C.q_full[t]), 128);
@@ -228,11 +237,65 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
   bool on = w.start(C.plan);
   if (warp >= Ro::kScores) {
   regs_dec<Ro::kOther>();
-  if (warp >= Ro::kLoad && warp < Ro::kLoad + Ro::kLoadWarps) {
-    // ------------------------------------------------------------------ K and V stages
-    const int kv = (warp - Ro::kLoad) / (Ro::kLoadWarps / 2);  // K or V
-    uint64_t* const full = C.full[kv];
-    uint64_t* const empty = C.empty[kv];
+  if (kQuant && warp >= Ro::kConvertWarp) {
+    // ------------------------------------------------------------------ e4m3 rows -> 16-bit stages
+    // In the order in which the products need them: the first K tiles (1, split 2), then K(j + ahead),
+    // while there is one, and V(j).  D / 16 threads share a row, 16 codes each.
+    constexpr int kLanes = D / 16, kRowsPass = kConvert / kLanes;
+    const int ct = tid - Ro::kConvertWarp * 32, ch = ct % kLanes, r0 = ct / kLanes;
+    const uint32_t c0 = (ch % 4) * 2;
+    const bool swap = ch >= 4;
+    uint32_t tiles = 0;
+    bool ok = true;
+    for (; on && ok; on = w.next(p)) {
+      const Piece& c = w.c;
+      const int i1 = min(c.n, c.i0 + p.tokens), n = c.tile1 - c.tile0;
+      const EdgeTiles edge(p, key_range(p, c.len, c.n, c.i0, i1));
+      const int ahead = (i1 - c.i0) * p.gw <= kTileM ? 2 : 1, lead = min(n, ahead);
+      for (int i = 0; i < 2 * n; ++i) {
+        const int x = i - lead;
+        const int kv = x < 0 ? 0 : (x < 2 * (n - lead) ? x & 1 : 1);
+        const int j = x < 0 ? i : (x < 2 * (n - lead) ? x / 2 + (kv ? 0 : ahead) : x - (n - lead));
+        const uint32_t num = tiles + j;
+        const int st = Sh::stage(kv, num);
+        ok = role_wait(C, smem_u32(&C.raw_full[kv]), num & 1) &&
+             role_wait(C, smem_u32(&C.empty[kv][st]), Sh::parity(kv, num) ^ 1);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        const uint8_t* raw = base + Sh::kRaw + kv * Sh::kRawBytes + ch * 16;
+        uint8_t* dst = base + Sh::at(kv, num) + (ch / 4) * 1024;
+        const int v0 = (c.tile0 + j) * kKeys;
+        const bool edges = edge(c.tile0 + j);
+#pragma unroll 2
+        for (int r = r0; r < 128; r += kRowsPass) {
+          uint4 codes = *reinterpret_cast<const uint4*>(raw + r * D);
+          uint8_t byte = C.scales[kv][r];
+          if (edges && edge.unseen(v0 + r)) {  // seen by no query of the unit: zeros, whatever lies there
+            codes = make_uint4(0, 0, 0, 0);
+            byte = 127;
+          }
+          uint4 lo, hi;
+          dequant16<T>(codes, byte, lo, hi);
+          uint8_t* row = dst + (r >> 3) * Sh::kGroup + (r & 7) * 128;
+          const uint32_t sw = r & 7;
+          // lanes of the two 64-element halves write opposite pieces: no bank is hit twice
+          *reinterpret_cast<uint4*>(row + ((c0 + swap) ^ sw) * 16) = swap ? hi : lo;
+          *reinterpret_cast<uint4*>(row + ((c0 + !swap) ^ sw) * 16) = swap ? lo : hi;
+        }
+        mbar_arrive(smem_u32(&C.raw_empty[kv]));
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(&C.full[kv][st]));
+      }
+      tiles += n;
+    }
+    if (!ok && lane == 0) give_up(C, p.err);
+  } else if (warp == Ro::kLoad || warp == Ro::kLoad + 1) {
+    // ------------------------------------------------------------------ K and V copies
+    const int kv = warp - Ro::kLoad;
+    const uint32_t leader = elect_one_sync();
+    const CUtensorMap* map = kv == 0 ? &k_map : &v_map;
     uint32_t issued = 0;
     bool ok = true;
     for (; on && ok; on = w.next(p)) {
@@ -240,89 +303,51 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       const KeyRange kr = key_range(p, c.len, c.n, c.i0, min(c.n, c.i0 + p.tokens));
       TileRows at(p, kr, c, lane);
       const int box = at.box;
-      for (int tile = c.tile0; tile < c.tile1 && ok; ++tile) {
+      for (int tile = c.tile0; tile < c.tile1; ++tile, ++issued) {
         at.advance(tile);
-        const int st = stage_of<D>(issued);
-        uint8_t* dst = ring + (kv * kStages + st) * Sh::kTileBytes;
-        if constexpr (!kQuant) {
-          const uint32_t leader = elect_one_sync();
-          ok = __all_sync(0xffffffffu, role_wait(C, smem_u32(&empty[st]), full_parity<D>(issued) ^ 1));
-          if (!ok) break;
-          const uint32_t bar = smem_u32(&full[st]);
-          mbar_arrive_expect_tx_p(leader, bar, __popc(at.have(tile)) * (uint32_t)box * (D * 2u));
-          const CUtensorMap* map = kv == 0 ? &k_map : &v_map;
-          const uint32_t to = smem_u32(dst);
-          for (int x0 = 0; x0 < at.parts; x0 += 8) {
-            int y[8];  // all rows first: a shuffle between two copies costs more than the copies
-#pragma unroll
-            for (int x = 0; x < 8; ++x) y[x] = at.row(tile, (x0 + x) & (at.parts - 1));
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-              tma_load_4d_p(x0 + x < at.parts && y[x] >= 0 ? leader : 0u, to + (x0 + x) * box * (D * 2), map, 0, 0, 0,
-                            y[x] >> 3, bar);
+        const int st = Sh::stage(kv, issued);
+        const uint32_t freed = smem_u32(kQuant ? &C.raw_empty[kv] : &C.empty[kv][st]);
+        ok = __all_sync(0xffffffffu, role_wait(C, freed, (kQuant ? issued & 1 : Sh::parity(kv, issued)) ^ 1));
+        if (!ok) break;
+        const uint32_t bar = smem_u32(kQuant ? &C.raw_full[kv] : &C.full[kv][st]);
+        constexpr uint32_t kRowBytes = kQuant ? D : 2 * D;
+        mbar_arrive_expect_tx_p(leader, bar, __popc(at.have(tile)) * (uint32_t)box * kRowBytes);
+        const uint32_t to = smem_u32(base + (kQuant ? Sh::kRaw + kv * Sh::kRawBytes : Sh::at(kv, issued)));
+        if constexpr (kQuant) {  // the scale bytes: 16 (blocks of 8 keys: 8) a lane
+          const int width = min(box, 16), key = lane * width, part = min(key, 127) >> (7 - at.log_parts);
+          const int y = at.row(tile, part);
+          if (key < 128 && y >= 0) {
+            const uint8_t* src = p.scales + at.scale_at(y + (key - part * box), kv);
+            const uint32_t sd = smem_u32(&C.scales[kv][key]);
+            if (width == 16)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sd), "l"(src) : "memory");
+            else
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(sd), "l"(src) : "memory");
           }
-        } else {
-          // D / 16 lanes share a row (16 codes each), kRowsPass rows a pass; the passes go in batches of
-          // kBatch, one batch's rows on their way while another is converted
-          constexpr int kLanes = D / 16, kRowsPass = kConvert / kLanes, kPasses = (128 + kRowsPass - 1) / kRowsPass;
-          constexpr int kBatch = 3, kBatches = (kPasses + kBatch - 1) / kBatch;
-          const int ct = tid - (Ro::kLoad + 3 * kv) * 32, ch = ct % kLanes, r0 = ct / kLanes;
-          const uint8_t* pool = static_cast<const uint8_t*>(kv == 0 ? p.k_pool : p.v_pool) + ch * 16;
-          uint4 codes[2][kBatch];
-          uint8_t sc[2][kBatch];
-          const auto fetch = [&](int b) {
-#pragma unroll
-            for (int x = 0; x < kBatch; ++x) {
-              const int r = (b * kBatch + x) * kRowsPass + r0;
-              const int part = min(r, 127) >> (7 - at.log_parts), y = at.row(tile, part);  // 128 keys: box = 128 >> log_parts
-              const int v = tile * kKeys + r;
-              // rows that no query of the unit sees are zeros: past the end, or in a block that is
-              // read between the sinks and the first window
-              const int pos = kr.position(v);
-              const bool seen = r < 128 && y >= 0 && v < kr.v_len && (pos >= kr.win_lo || pos < p.sinks);
-              codes[b & 1][x] = make_uint4(0, 0, 0, 0);
-              sc[b & 1][x] = 0;
-              if (seen) {
-                const int row = y + (r - part * box);
-                codes[b & 1][x] = *reinterpret_cast<const uint4*>(pool + (int64_t)row * D);
-                sc[b & 1][x] = p.scales[at.scale_at(row, kv)];
-              }
-            }
-          };
-          fetch(0);
-          fetch(1);
-          ok = role_wait(C, smem_u32(&empty[st]), full_parity<D>(issued) ^ 1);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-#pragma unroll
-          for (int b = 0; b < kBatches; ++b) {
-#pragma unroll
-            for (int x = 0; x < kBatch; ++x) {
-              const int r = (b * kBatch + x) * kRowsPass + r0;
-              if (r >= 128) break;
-              uint4 lo, hi;
-              dequant16<T>(codes[b & 1][x], sc[b & 1][x], lo, hi);
-              uint8_t* row = dst + (r >> 3) * Sh::kGroup + (ch / 4) * 1024 + (r & 7) * 128;
-              const uint32_t sw = r & 7, c0 = (ch % 4) * 2;
-              // lanes of the two 64-element halves write opposite pieces: no bank is hit twice
-              const bool swap = ch >= 4;
-              *reinterpret_cast<uint4*>(row + ((c0 + swap) ^ sw) * 16) = swap ? hi : lo;
-              *reinterpret_cast<uint4*>(row + ((c0 + !swap) ^ sw) * 16) = swap ? lo : hi;
-            }
-            if (b + 2 < kBatches) fetch(b + 2);
-          }
-          fence_proxy_async_smem();
-          mbar_arrive(smem_u32(&full[st]));
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
         }
-        ++issued;
+        for (int x0 = 0; x0 < at.parts; x0 += 8) {
+          int y[8];  // all rows first: a shuffle between two copies costs more than the copies
+#pragma unroll
+          for (int x = 0; x < 8; ++x) y[x] = at.row(tile, (x0 + x) & (at.parts - 1));
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const uint32_t go = x0 + x < at.parts && y[x] >= 0 ? leader : 0u;
+            if constexpr (kQuant) tma_load_2d_p(go, to + (x0 + x) * box * D, map, 0, y[x], bar);
+            else tma_load_4d_p(go, to + (x0 + x) * box * (D * 2), map, 0, 0, 0, y[x] >> 3, bar);
+          }
+        }
       }
     }
     if (!ok && lane == 0) give_up(C, p.err);
-    if constexpr (!kQuant) {  // before the shared memory goes: every copy issued has landed (bounded)
-      for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
-        mbar_wait(smem_u32(&full[stage_of<D>(i)]), full_parity<D>(i));
+    // before the shared memory goes: every copy issued has landed (bounded)
+    if constexpr (kQuant) {
+      if (issued > 0) mbar_wait(smem_u32(&C.raw_full[kv]), (issued - 1) & 1);
+    } else {
+      for (uint32_t i = issued > Sh::kK ? issued - Sh::kK : 0; i < issued; ++i)
+        mbar_wait(smem_u32(&C.full[kv][Sh::stage(kv, i)]), Sh::parity(kv, i));
     }
-  } else {
+  } else if (warp == Ro::kScores || warp == Ro::kValues) {
     // ------------------------------------------------------------------ MMA issuers
     const bool do_s = warp == Ro::kScores, do_o = warp == Ro::kValues;
     const uint32_t leader = elect_one_sync();
@@ -338,8 +363,8 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     // shared-memory descriptors: offsets only change the address field (in 16-byte units)
     const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, 1024, kSwizzle128B);
     const uint64_t p_desc = smem_desc(smem_u32(p_s), 16, 1024, kSwizzle128B);
-    const uint64_t k_desc = smem_desc(smem_u32(ring), 16, Sh::kGroup, kSwizzle128B);
-    const uint64_t v_desc = smem_desc(smem_u32(ring + kStages * Sh::kTileBytes), 1024, Sh::kGroup, kSwizzle128B);
+    const uint64_t k_desc = smem_desc(smem_u32(base + Sh::kRing), 16, Sh::kGroup, kSwizzle128B);
+    const uint64_t v_desc = smem_desc(smem_u32(base + Sh::kRing + Sh::kK * Sh::kTileBytes), 1024, Sh::kGroup, kSwizzle128B);
     // S of group t = (Q of tile qt) K^T, K in stage st
     const auto scores = [&](int t, int qt, int st, uint32_t step) {
       const uint64_t qd = q_desc + qt * (Sh::kTileBytes >> 4), kd = k_desc + st * (Sh::kTileBytes >> 4);
@@ -377,11 +402,11 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         if (s0[t] > 0) wait(&C.s_free[t], (s0[t] - 1) & 1);
       for (int j = 0; j < min(n, ahead) && ok && do_s; ++j) {
         const uint32_t i = tiles + j;
-        if (!wait(&C.full[0][stage_of<D>(i)], full_parity<D>(i))) break;
+        if (!wait(&C.full[0][Sh::stage(0, i)], Sh::parity(0, i))) break;
         for (int t = 0; t < (split ? 1 : 2) && ok; ++t) {
-          scores(split ? j : t, t, stage_of<D>(i), split && j == 1 ? s0[1] : s0[t]);
+          scores(split ? j : t, t, Sh::stage(0, i), split && j == 1 ? s0[1] : s0[t]);
         }
-        if (ok) umma_commit_p(leader, smem_u32(&C.empty[0][stage_of<D>(i)]));
+        if (ok) umma_commit_p(leader, smem_u32(&C.empty[0][Sh::stage(0, i)]));
       }
       // Half steps h: group h & 1 takes its key tile.  Once it has read its scores, its next ones go
       // out, then the product of the half step before: the groups find their next scores ready, and
@@ -394,19 +419,19 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
           if (j + ahead < n) {
             const uint32_t ik = tiles + j + ahead;
             if (!wait(&C.s_free[t], step & 1)) break;
-            if ((split || t == 0) && !wait(&C.full[0][stage_of<D>(ik)], full_parity<D>(ik))) break;
-            scores(t, split ? 0 : t, stage_of<D>(ik), step + 1);
-            if (split || t == 1) umma_commit_p(leader, smem_u32(&C.empty[0][stage_of<D>(ik)]));
+            if ((split || t == 0) && !wait(&C.full[0][Sh::stage(0, ik)], Sh::parity(0, ik))) break;
+            scores(t, split ? 0 : t, Sh::stage(0, ik), step + 1);
+            if (split || t == 1) umma_commit_p(leader, smem_u32(&C.empty[0][Sh::stage(0, ik)]));
           }
         }
         if (do_o && h > 0) {
           const int t = (h - 1) & 1, j = split ? h - 1 : (h - 1) >> 1;
           const uint32_t step = s0[t] + ((h - 1) >> 1), iv = tiles + j;
-          if ((split || t == 0) && !wait(&C.full[1][stage_of<D>(iv)], full_parity<D>(iv))) break;
+          if ((split || t == 0) && !wait(&C.full[1][Sh::stage(1, iv)], Sh::parity(1, iv))) break;
           if (!kQuant && (split || t == 0) && edge(c.tile0 + j)) mbar_arrive_p(leader, smem_u32(&C.v_ready[t]));
           if (!wait(&C.p_full[t], step & 1)) break;
-          values(t, stage_of<D>(iv), step == s0[t], step);
-          if (split || t == 1) umma_commit_p(leader, smem_u32(&C.empty[1][stage_of<D>(iv)]));
+          values(t, Sh::stage(1, iv), step == s0[t], step);
+          if (split || t == 1) umma_commit_p(leader, smem_u32(&C.empty[1][Sh::stage(1, iv)]));
         }
       }
       tiles += n;
@@ -490,8 +515,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
           ok = __all_sync(0xffffffffu, role_wait(C, smem_u32(&C.v_ready[t]), edges++ & 1));
           if (!ok) break;
           if (edge.unseen(v0 + r)) {
-            uint8_t* vrow = ring + (kStages + stage_of<D>(tiles + j)) * Sh::kTileBytes +
-                            (r >> 3) * Sh::kGroup + (r & 7) * 128;
+            uint8_t* vrow = base + Sh::at(1, tiles + j) + (r >> 3) * Sh::kGroup + (r & 7) * 128;
 #pragma unroll
             for (int h = 0; h < D / 64; ++h)
 #pragma unroll
@@ -674,20 +698,20 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
 template <typename T, int D, bool kQuant>
 int launch(const ChunkParams& p, cudaStream_t st) {
   CUtensorMap k_map = {}, v_map = {};
-  if (!kQuant) {
-    const uint64_t rows = (uint64_t)p.num_blocks * p.n_kv_heads * p.block_size;
-    const uint32_t groups = (p.block_size < kKeys ? p.block_size : kKeys) / 8;
-    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    if (!tensor_map_row_groups(&k_map, bf16, p.k_pool, rows, D, groups) ||
-        !tensor_map_row_groups(&v_map, bf16, p.v_pool, rows, D, groups)) {
-      set_last_error("paged_chunk: tensor map encoding failed");
-      return SNAPMIND_ERR_CUDA;
-    }
+  const uint64_t rows = (uint64_t)p.num_blocks * p.n_kv_heads * p.block_size;
+  const uint32_t box = p.block_size < kKeys ? p.block_size : kKeys;
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  const bool mapped = kQuant ? tensor_map_bytes(&k_map, p.k_pool, D, rows, box, false) && tensor_map_bytes(&v_map, p.v_pool, D, rows, box, false)
+                             : tensor_map_row_groups(&k_map, bf16, p.k_pool, rows, D, box / 8) &&
+                                   tensor_map_row_groups(&v_map, bf16, p.v_pool, rows, D, box / 8);
+  if (!mapped) {
+    set_last_error("paged_chunk: tensor map encoding failed");
+    return SNAPMIND_ERR_CUDA;
   }
   auto kernel = chunk_umma_kernel<T, D, kQuant>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>());
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D, kQuant>());
   if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
-  kernel<<<p.n_ctas, Roles<kQuant>::kThreads, smem_bytes<D>(), st>>>(k_map, v_map, p);
+  kernel<<<p.n_ctas, Roles<kQuant>::kThreads, smem_bytes<D, kQuant>(), st>>>(k_map, v_map, p);
   return cuda_status(cudaGetLastError(), "paged_chunk launch");
 }
 
@@ -705,7 +729,8 @@ bool chunk_umma_supported(const ChunkParams& p, int dtype, int pool_dtype) {
   if (!a16(p.q) || !a16(p.out) || !a16(p.k_pool) || !a16(p.v_pool)) return false;
   if (p.q_stride_tok % 8 || p.q_stride_head % 8 || p.out_stride_tok % 8 || p.out_stride_head % 8) return false;
   if ((int64_t)p.num_blocks * p.n_kv_heads * bs >= (int64_t)1 << 31) return false;  // TMA row coordinate
-  return pool_dtype == SNAPMIND_DTYPE_E4M3 || encode_tiled() != nullptr;
+  if (pool_dtype == SNAPMIND_DTYPE_E4M3 && !a16(p.scales)) return false;
+  return encode_tiled() != nullptr;
 }
 
 int launch_chunk_umma(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st) {

@@ -43,7 +43,7 @@ template <bool kQuant>
 struct Ctrl {
   static constexpr int N = Stage<kQuant>::kCount;
   float mo[2][kHeads][kD];
-  uint8_t scales[kQuant ? N : 1][2][kTile];  // K, V bytes of a stage's rows
+  alignas(16) uint8_t scales[kQuant ? N : 1][2][kTile];  // K, V bytes of a stage's rows (16-byte copies)
   float mm[kConsumers][kHeads], ml[kConsumers][kHeads];
   uint64_t full[N], empty[N];
   int32_t abort;
@@ -489,26 +489,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Rows of 128 e4m3 codes, boxes of whole rows with the 128-byte swizzle.
-bool tensor_map_codes(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows) {
-  EncodeTiledFn fn = encode_tiled();
-  if (!fn) return false;
-  const cuuint64_t dims[2] = {kD, rows};
-  const cuuint64_t strides[1] = {kD};
-  const cuuint32_t box[2] = {kD, box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, bool kQuant>
 int launch(const ChunkParams& p, cudaStream_t st) {
   CUtensorMap k_map, v_map;
   const uint64_t rows = (uint64_t)p.num_blocks * p.n_kv_heads * p.block_size;
   const uint32_t box = p.block_size < kTile ? p.block_size : kTile;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  const bool mapped = kQuant ? tensor_map_codes(&k_map, p.k_pool, rows, box) && tensor_map_codes(&v_map, p.v_pool, rows, box)
+  const bool mapped = kQuant ? tensor_map_bytes(&k_map, p.k_pool, kD, rows, box, true) && tensor_map_bytes(&v_map, p.v_pool, kD, rows, box, true)
                              : tensor_map_2d(&k_map, bf16, p.k_pool, kD, rows, kD * 2, 64, box) &&
                                    tensor_map_2d(&v_map, bf16, p.v_pool, kD, rows, kD * 2, 64, box);
   if (!mapped) {
