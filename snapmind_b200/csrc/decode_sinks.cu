@@ -28,8 +28,8 @@ namespace {
 
 using namespace tc;
 
-constexpr int kD = 128, kTile = 64, kConsumers = 4, kThreads = (kConsumers + 1) * 32, kHeads = 8;
-constexpr int kScaleLanes = 2 * kTile / 16;  // lanes that fetch a tile's scale bytes, 16 each
+constexpr int kD = 128, kTile = 64, kConsumers = 4, kThreads = (kConsumers + 2) * 32, kHeads = 8;
+constexpr int kScaleLanes = kTile / 16;  // lanes that fetch a tile's scale bytes of K, or of V, 16 each
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <bool kQuant> struct Stage {
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < St::kCount; ++i) {
-      mbar_init(smem_u32(&S.full[i]), kQuant ? 1 + kScaleLanes : 1);
+      mbar_init(smem_u32(&S.full[i]), kQuant ? 2 * (1 + kScaleLanes) : 2);
       mbar_init(smem_u32(&S.empty[i]), kConsumers);
     }
     S.abort = 0;
@@ -148,11 +148,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   bool on = w.start(S.plan);
   uint32_t tile = 0;  // running number of the CTA's tiles
   bool ok = true;
-  if (warp == kConsumers) {
-    // ------------------------------------------------------------------ producer
+  if (warp >= kConsumers) {
+    // ------------------------------------------------------------------ producers: K, V
+    const int kv = warp - kConsumers;
+    const CUtensorMap* map = kv == 0 ? &k_map : &v_map;
     const uint32_t leader = elect_one_sync();
-    // the scale bytes that a lane fetches: keys scale_key .. + 15 of K or V, from part scale_part
-    const int scale_kv = (lane >> 2) & 1, scale_key = (lane & 3) * 16;
+    // the scale bytes that a lane fetches: keys scale_key .. + 15, from part scale_part
+    const int scale_key = (lane & (kScaleLanes - 1)) * 16;
     const int scale_part = p.block_size < kTile ? p.by_block.div(scale_key) : 0;
     const int scale_in = scale_key - scale_part * min(p.block_size, kTile);
     for (; on && ok; on = w.next(p)) {
@@ -167,14 +169,14 @@ __global__ void __launch_bounds__(kThreads, 2)
         ok = __all_sync(0xffffffffu, role_wait(S, smem_u32(&S.empty[st]), ((tile / St::kCount) & 1) ^ 1));
         if (!ok) break;
         const uint32_t bar = smem_u32(&S.full[st]);
-        const uint32_t row_bytes = kQuant ? 2 * 128 : 4 * 128;
+        const uint32_t row_bytes = kQuant ? 128 : 2 * 128;
         mbar_arrive_expect_tx_p(leader, bar, __popc(have) * (uint32_t)box * row_bytes);
-        const uint32_t dst = smem_u32(ring + st * St::kBytes);
+        const uint32_t dst = smem_u32(ring + st * St::kBytes + (kv == 0 ? St::kK : St::kV));
         if constexpr (kQuant) {
           // the scales go by plain 16-byte copies, not as small bulk copies beside the boxes
           const int sr = at.row(j, scale_part);
           if (lane < kScaleLanes) {
-            if (sr >= 0) copy16(smem_u32(&S.scales[st][scale_kv][scale_key]), p.scales + at.scale_at(sr + scale_in, scale_kv));
+            if (sr >= 0) copy16(smem_u32(&S.scales[st][kv][scale_key]), p.scales + at.scale_at(sr + scale_in, kv));
             copies_arrive(bar);
           }
         }
@@ -186,16 +188,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int y = ys[x];
           const uint32_t go = x < at.parts && y >= 0 ? leader : 0u;
           const uint32_t ro = x * box * 128;
-          if constexpr (kQuant) {
-            tma_load_2d_p(go, dst + St::kK + ro, &k_map, 0, y, bar);
-            tma_load_2d_p(go, dst + St::kV + ro, &v_map, 0, y, bar);
-          } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              tma_load_2d_p(go, dst + St::kK + h * St::kHalf + ro, &k_map, 64 * h, y, bar);
-              tma_load_2d_p(go, dst + St::kV + h * St::kHalf + ro, &v_map, 64 * h, y, bar);
-            }
-          }
+          tma_load_2d_p(go, dst + ro, map, 0, y, bar);
+          if constexpr (!kQuant) tma_load_2d_p(go, dst + St::kHalf + ro, map, 64, y, bar);
         }
       }
     }
