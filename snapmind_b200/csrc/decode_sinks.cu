@@ -31,6 +31,7 @@ using namespace tc;
 constexpr int kD = 128, kTile = 64, kConsumers = 4, kThreads = (kConsumers + 2) * 32, kHeads = 8;
 constexpr int kScaleLanes = kTile / 16;  // lanes that fetch a tile's scale bytes of K, or of V, 16 each
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRaise = 8.f;  // log2 headroom of the reference maxima
 
 template <bool kQuant> struct Stage {
   static constexpr int kHalf = kTile * 128;                      // 64 rows of 128 bytes
@@ -85,10 +86,11 @@ template <bool kBf16> __device__ __forceinline__ uint32_t pack2(float lo, float 
     return *reinterpret_cast<uint32_t*>(&v);
   }
 }
-// two e4m3 codes in the low 16 bits -> two f16
-__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// four e4m3 codes -> two pairs of f16 (the low two codes, the high two)
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
 // Byte offset of 16-byte piece `ch` (0..7) of row `row` in rows of 128 bytes, 128-byte swizzle.
 __device__ __forceinline__ uint32_t swz(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
@@ -205,6 +207,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int g = lane >> 2, tig = lane & 3;
     const int lrow = (lane & 7) + ((lane >> 3) & 1) * 8, lchk = lane >> 4;
     const int vrow = (lane & 7) + ((lane >> 4) & 1) * 8, vchk = (lane >> 3) & 1;  // 16-bit V
+    // offsets of the lane's rows in a stage: e4m3 pieces k + lchk of K and of V, 16-bit pieces 2 k + ..
+    uint32_t k_off[4], v_off[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      k_off[k] = swz(16 * warp + lrow, 2 * k + lchk);
+      v_off[k] = kQuant ? k_off[k] : swz(16 * warp + vrow, 2 * k + vchk);
+    }
     const bool flip = p.scale < 0.f;  // folded into Q: the largest score has the largest weight
     const float c2 = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
     for (; on; on = w.next(p)) {
@@ -281,23 +290,26 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           // ---- S^T = K Q^T: 16 keys x 8 heads; keys g and g + 8, heads 2 tig, 2 tig + 1
           float sc[4] = {0.f, 0.f, 0.f, 0.f};
-          float sv0 = 0.f, sv1 = 0.f;  // exponents of V's rows g, g + 8
+          float d0 = 1.f, d1 = 1.f;  // 2^-e_v of V's rows g, g + 8
           if constexpr (kQuant) {
 #pragma unroll
             for (int k = 0; k < 8; k += 2) {
               uint32_t r[4];
-              ldsm_x4(kb + swz(16 * warp + lrow, k + lchk), r);
+              ldsm_x4(kb + k_off[k / 2], r);
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const uint32_t a[4] = {codes_f16(r[2 * i] & 0xFFFF), codes_f16(r[2 * i + 1] & 0xFFFF),
-                                       codes_f16(r[2 * i] >> 16), codes_f16(r[2 * i + 1] >> 16)};
+                uint32_t a[4];
+                codes_f16(r[2 * i], a[0], a[2]);
+                codes_f16(r[2 * i + 1], a[1], a[3]);
                 mma16816<false>(sc, a, qf[k + i][0], qf[k + i][1]);
               }
             }
             const uint8_t* bytes = &S.scales[st][0][16 * warp];
             const float k0 = __uint_as_float((uint32_t)bytes[g] << 23), k1 = __uint_as_float((uint32_t)bytes[g + 8] << 23);
-            sv0 = (float)((int)bytes[kTile + g] - 127);
-            sv1 = (float)((int)bytes[kTile + g + 8] - 127);
+            const int e0 = bytes[kTile + g], e1 = bytes[kTile + g + 8];
+            const float sv0 = (float)(e0 - 127), sv1 = (float)(e1 - 127);
+            d0 = __uint_as_float((uint32_t)(254 - e0) << 23);
+            d1 = __uint_as_float((uint32_t)(254 - e1) << 23);
             sc[0] = fmaf(sc[0] * k0, q0, sv0);  // s + e_v
             sc[1] = fmaf(sc[1] * k0, q1, sv0);
             sc[2] = fmaf(sc[2] * k1, q0, sv1);
@@ -306,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               uint32_t a[4];
-              ldsm_x4(kb + (k >> 2) * St::kHalf + swz(16 * warp + lrow, (k & 3) * 2 + lchk), a);
+              ldsm_x4(kb + (k >> 2) * St::kHalf + k_off[k & 3], a);
               mma16816<kMmaBf16>(sc, a, qf[k][0], qf[k][1]);
             }
 #pragma unroll
@@ -315,39 +327,44 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (!all) {
             if (!seen(g)) {
               sc[0] = sc[1] = -INFINITY;
-              sv0 = 0.f;
+              d0 = 0.f;
             }
             if (!seen(g + 8)) {
               sc[2] = sc[3] = -INFINITY;
-              sv1 = 0.f;
+              d1 = 0.f;
             }
           }
+          // The references are raised only when a score passes them by 2^8 (weights up to 2^8 are as
+          // good as those up to 1): then to the exact maxima, and the sums and O are rescaled.
           float t0 = fmaxf(sc[0], sc[2]), t1 = fmaxf(sc[1], sc[3]);
+          if (__any_sync(0xffffffffu, t0 > m0 + kRaise || t1 > m1 + kRaise)) {
 #pragma unroll
-          for (int off = 4; off < 32; off <<= 1) {
-            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, off));
-            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
+            for (int off = 4; off < 32; off <<= 1) {
+              t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, off));
+              t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
+            }
+            const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+            const float a0 = n0 == -INFINITY ? 1.f : ex2(m0 - n0), a1 = n1 == -INFINITY ? 1.f : ex2(m1 - n1);
+            m0 = n0;
+            m1 = n1;
+            l0 *= a0;
+            l1 *= a1;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              o[k][0] *= a0;
+              o[k][1] *= a1;
+              o[k][2] *= a0;
+              o[k][3] *= a1;
+            }
           }
-          // some key of the 16 is seen, so the new maxima are not -inf (NaN scores aside)
-          const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-          const float a0 = ex2(m0 - n0), a1 = ex2(m1 - n1);
-          m0 = n0;
-          m1 = n1;
-          const float p0 = ex2(sc[0] - n0), p1 = ex2(sc[1] - n1), p2 = ex2(sc[2] - n0), p3 = ex2(sc[3] - n1);
+          const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+          const float p0 = ex2(sc[0] - r0), p1 = ex2(sc[1] - r1), p2 = ex2(sc[2] - r0), p3 = ex2(sc[3] - r1);
           if constexpr (kQuant) {
-            const float d0 = ex2(-sv0), d1 = ex2(-sv1);  // whole exponents: exact
-            l0 = fmaf(p0, d0, fmaf(p2, d1, l0 * a0));
-            l1 = fmaf(p1, d0, fmaf(p3, d1, l1 * a1));
+            l0 = fmaf(p0, d0, fmaf(p2, d1, l0));
+            l1 = fmaf(p1, d0, fmaf(p3, d1, l1));
           } else {
-            l0 = l0 * a0 + p0 + p2;
-            l1 = l1 * a1 + p1 + p3;
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            o[k][0] *= a0;
-            o[k][1] *= a1;
-            o[k][2] *= a0;
-            o[k][3] *= a1;
+            l0 += p0 + p2;
+            l1 += p1 + p3;
           }
           // ---- P^T as the B operand: lane (g, tig) needs keys 2 tig, + 1, + 8, + 9 of head g
           const uint32_t pr01 = pack2<kMmaBf16>(p0, p1), pr23 = pack2<kMmaBf16>(p2, p3);
@@ -361,12 +378,12 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int k = 0; k < 8; k += 2) {
               uint32_t r[4];
-              ldsm_x4_t(vb + swz(16 * warp + lrow, k + lchk), r);
+              ldsm_x4_t(vb + v_off[k / 2], r);
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const uint32_t e0 = __byte_perm(r[2 * i], 0, 0x3120), e1 = __byte_perm(r[2 * i + 1], 0, 0x3120);
-                const uint32_t a[4] = {codes_f16(e0 & 0xFFFF), codes_f16(e0 >> 16), codes_f16(e1 & 0xFFFF),
-                                       codes_f16(e1 >> 16)};
+                uint32_t a[4];
+                codes_f16(__byte_perm(r[2 * i], 0, 0x3120), a[0], a[1]);
+                codes_f16(__byte_perm(r[2 * i + 1], 0, 0x3120), a[2], a[3]);
                 mma16816<false>(o[k + i], a, pb0, pb1);
               }
             }
@@ -374,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               uint32_t a[4];
-              ldsm_x4_t(vb + (k >> 2) * St::kHalf + swz(16 * warp + vrow, (k & 3) * 2 + vchk), a);
+              ldsm_x4_t(vb + (k >> 2) * St::kHalf + v_off[k & 3], a);
               mma16816<kMmaBf16>(o[k], a, pb0, pb1);
             }
           }
