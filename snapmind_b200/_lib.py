@@ -219,6 +219,11 @@ def stream_handle(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(index: int) -> int:
+    """The current stream of device ``index`` (without the stream object that ``stream_handle`` makes)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def require_cuda(device: torch.device) -> None:
     if device.type != "cuda":
         raise RuntimeError(f"snapmind_b200 runs on CUDA devices only (got {device})")

@@ -7,7 +7,9 @@
 //
 // The CUDA-core kernel: 64 query rows x 64 keys a step, 256 threads, thread (ty, tx)
 // holding rows ty + 16 i and keys (then dims) tx + 16 j.  All arithmetic is f32, so it
-// is the path of f32 caches.
+// is the path of f32 caches.  What bounds it is FMA issue (two products an instruction), once the
+// next step's K and V are on their way while a step is computed: with every step loaded element by
+// element as it came, 4 prompts of 256 tokens (32 heads over 4 of 64) took 80 us.
 #include <cuda_fp8.h>
 
 #include "chunk_plan.cuh"
@@ -35,23 +37,81 @@ struct GenSmem {
   float k[kKeys * P];
   float v[kKeys * P];
   float s[kRows * PS];
-  int64_t row[kKeys];  // pool row of every key of the tile, -1: seen by no row
-  int32_t pos[kKeys];
+  int64_t row[2][kKeys];  // pool row of every key of a step, -1: seen by no row
+  int32_t pos[2][kKeys];
   PlanShared plan;
 };
 
+// Pairs of f32 in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 x, x, y, z; "
+      "mov.b64 {%0, %1}, x; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
+// 16 bytes of pool elements as floats, stored to 16-byte-aligned shared memory; whether all are finite.
+template <typename KV>
+__device__ __forceinline__ bool spread(float* dst, const uint4& w, float scale) {
+  constexpr int V = 16 / sizeof(KV);
+  const KV* e = reinterpret_cast<const KV*>(&w);
+  float f[V];
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if constexpr (std::is_same<KV, uint8_t>::value) f[i] = e4m3_to_f(e[i]) * scale;
+    else f[i] = Conv<KV>::to_f(e[i]);
+    finite &= fabsf(f[i]) < INFINITY;
+  }
+#pragma unroll
+  for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+  return finite;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* out, int d, int D, const float4& v, bool vec) {
+  if (vec && d + 3 < D) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(out + d) = v;
+    } else {
+      __align__(8) T y[4] = {Conv<T>::from_f(v.x), Conv<T>::from_f(v.y), Conv<T>::from_f(v.z), Conv<T>::from_f(v.w)};
+      *reinterpret_cast<uint2*>(out + d) = *reinterpret_cast<const uint2*>(y);
+    }
+    return;
+  }
+  const float y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (d + u < D) out[d + u] = Conv<T>::from_f(y[u]);
+}
+// Whether 4 elements of an output row may be stored as one vector.
+template <typename T>
+__device__ __forceinline__ bool out_vec(const ChunkParams& p) {
+  return p.out_stride_tok % 4 == 0 && p.out_stride_head % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+}
+
 template <typename T, typename KV, int D4>
-__global__ void __launch_bounds__(kGenThreads) chunk_generic_kernel(ChunkParams p) {
+__global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_kernel(ChunkParams p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   using Smem = GenSmem<D4>;
-  constexpr int P = Smem::P, PS = Smem::PS;
+  constexpr int P = Smem::P, PS = Smem::PS, D = Smem::D;
   constexpr bool kQuant = std::is_same<KV, uint8_t>::value;
+  // whole 16-byte vectors of the pool: a row's, a thread's of K (and of V) a step
+  constexpr int V = 16 / sizeof(KV), kRowVecs = D / V, kVecs = kKeys * kRowVecs / kGenThreads;
+  constexpr bool kCanFetch = kVecs <= 8;  // registers for a step of K and V
+  constexpr int kHeld = kCanFetch ? kVecs : 1;
   Smem& S = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   plan_block(p, S.plan, reinterpret_cast<int32_t*>(S.q));
   if (tid == 0) write_piece_info(p, S.plan);
   const float c2 = p.scale * kLog2e;
   const int bs = p.block_size, hd = p.head_dim;
+  const bool fetches = kCanFetch && hd == D && ((reinterpret_cast<uintptr_t>(p.k_pool) | reinterpret_cast<uintptr_t>(p.v_pool)) & 15) == 0;
+  const bool vec = out_vec<T>(p);
+  constexpr int VQ = 16 / sizeof(T);
+  const bool q_vec = hd == D && p.q_stride_tok % VQ == 0 && p.q_stride_head % VQ == 0 && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0;
 
   PieceWalk w;
   for (bool on = w.start(S.plan); on; on = w.next(p)) {
@@ -61,81 +121,130 @@ __global__ void __launch_bounds__(kGenThreads) chunk_generic_kernel(ChunkParams 
     const KeyRange kr = key_range(p, c.len, c.n, c.i0, i1);
     const int n_rows = (i1 - c.i0) * p.gw;
     const int head0 = c.kvh * p.group + c.slice * p.gw;
+    // pool rows and positions of the keys of a step, by the first 64 threads
+    const auto find = [&](int t) {
+      if (tid >= kKeys) return;
+      const int v = t * kKeys + tid;
+      int64_t row = -1;
+      int pos = INT32_MAX;
+      if (t < c.tile1 && v < kr.v_len) {
+        pos = kr.position(v);
+        const int j = p.by_block.div(pos);
+        const bool in_sink = p.window > 0 && pos < p.sinks;
+        if (pos < kr.win_lo && !in_sink) {
+          pos = INT32_MAX;  // in a block that is read, before every window
+        } else {
+          const int32_t phys = j < p.table_width ? p.tables[(int64_t)c.b * p.table_stride + j] : -1;
+          if (phys < 0 || phys >= p.num_blocks)
+            flag_error(p.err, j < p.table_width ? SNAPMIND_DEVERR_BLOCK_ID : SNAPMIND_DEVERR_TABLE);
+          else
+            row = ((int64_t)phys * p.n_kv_heads + c.kvh) * bs + (pos - j * bs);
+        }
+      }
+      S.row[t & 1][tid] = row;
+      S.pos[t & 1][tid] = row < 0 ? INT32_MAX : pos;
+    };
+    // scales [block][head][2][slot]: K's byte of a pool row; V's is block_size further
+    const auto scale_of = [&](int64_t row) {
+      const int64_t tile = row / bs;
+      return p.scales + tile * 2 * bs + (row - tile * bs);
+    };
+    uint4 held[2][kHeld];
+    const auto fetch = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const int e = tid + i * kGenThreads, r = e / kRowVecs, x = e % kRowVecs;
+        const int64_t row = S.row[t & 1][r];
+        held[0][i] = held[1][i] = make_uint4(0, 0, 0, 0);
+        if (row >= 0) {
+          held[0][i] = reinterpret_cast<const uint4*>(p.k_pool)[row * kRowVecs + x];
+          held[1][i] = reinterpret_cast<const uint4*>(p.v_pool)[row * kRowVecs + x];
+        }
+      }
+    };
     __syncthreads();
-    for (int e = tid; e < kRows * Smem::D; e += kGenThreads) {
-      const int r = e / Smem::D, d = e - r * Smem::D;
-      const int g = r % p.gw, tok = c.q_first + c.i0 + r / p.gw;
+    find(c.tile0);
+    if (q_vec) {
+#pragma unroll
+      for (int i = 0; i < kRows * D / VQ / kGenThreads; ++i) {
+        const int e = tid + i * kGenThreads, r = e / (D / VQ), x = e % (D / VQ);
+        const int tok = p.by_gw.div(r), g = r - tok * p.gw;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < n_rows && g < heads)
+          v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (int64_t)(c.q_first + c.i0 + tok) * p.q_stride_tok +
+                                              (int64_t)(head0 + g) * p.q_stride_head + x * VQ);
+        spread<T>(&S.q[r * P + x * VQ], v, 1.f);
+      }
+    } else for (int e = tid; e < kRows * D; e += kGenThreads) {
+      const int r = e / D, d = e - r * D;
+      const int tok = p.by_gw.div(r), g = r - tok * p.gw;
       float x = 0.f;
       if (r < n_rows && g < heads && d < hd)
-        x = Conv<T>::to_f(reinterpret_cast<const T*>(p.q)[(int64_t)tok * p.q_stride_tok + (int64_t)(head0 + g) * p.q_stride_head + d]);
+        x = Conv<T>::to_f(reinterpret_cast<const T*>(p.q)[(int64_t)(c.q_first + c.i0 + tok) * p.q_stride_tok + (int64_t)(head0 + g) * p.q_stride_head + d]);
       S.q[r * P + d] = x;
     }
-    float o[4][4 * D4], m[4], l[4];
+    __syncthreads();
+    if (fetches) fetch(c.tile0);
+    float2 o[4][2 * D4];
+    float m[4], l[4];
     int qpos[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       m[i] = -INFINITY;
       l[i] = 0.f;
-      qpos[i] = kr.pos0 + (ty + 16 * i) / p.gw;
+      qpos[i] = kr.pos0 + p.by_gw.div(ty + 16 * i);
 #pragma unroll
-      for (int j = 0; j < 4 * D4; ++j) o[i][j] = 0.f;
+      for (int j = 0; j < 2 * D4; ++j) o[i][j] = make_float2(0.f, 0.f);
     }
     for (int t = c.tile0; t < c.tile1; ++t) {
-      __syncthreads();
-      if (tid < kKeys) {
-        const int v = t * kKeys + tid;
-        int64_t row = -1;
-        int pos = INT32_MAX;
-        if (v < kr.v_len) {
-          pos = kr.position(v);
-          const int j = pos / bs;
-          const bool in_sink = p.window > 0 && pos < p.sinks;
-          if (pos < kr.win_lo && !in_sink) {
-            pos = INT32_MAX;  // in a block that is read, before every window
-          } else if (j >= p.table_width) {
-            flag_error(p.err, SNAPMIND_DEVERR_TABLE);
-          } else {
-            const int32_t phys = p.tables[(int64_t)c.b * p.table_stride + j];
-            if (phys < 0 || phys >= p.num_blocks)
-              flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
-            else
-              row = ((int64_t)phys * p.n_kv_heads + c.kvh) * bs + (pos - j * bs);
-          }
-        }
-        if (row < 0) pos = INT32_MAX;
-        S.row[tid] = row;
-        S.pos[tid] = pos;
-      }
-      __syncthreads();
+      __syncthreads();  // the step before has been computed
       bool odd = false;  // a value of V that is not finite
-      for (int e = tid; e < kKeys * Smem::D; e += kGenThreads) {
-        const int r = e / Smem::D, d = e - r * Smem::D;
-        const int64_t row = S.row[r];
-        float kx = 0.f, vx = 0.f;
-        if (row >= 0 && d < hd) {
+      if (fetches) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+          const int e = tid + i * kGenThreads, r = e / kRowVecs, x = e % kRowVecs;
+          float ks = 1.f, vs = 1.f;
           if constexpr (kQuant) {
-            // scales [block][head][2][slot]: K's bytes of a (block, head), then V's
-            const int64_t tile = row / bs;
-            const uint8_t* sc = p.scales + tile * 2 * bs + (row - tile * bs);
-            kx = e4m3_to_f(reinterpret_cast<const uint8_t*>(p.k_pool)[row * hd + d]) * scale_byte_to_f(sc[0]);
-            vx = e4m3_to_f(reinterpret_cast<const uint8_t*>(p.v_pool)[row * hd + d]) * scale_byte_to_f(sc[bs]);
-          } else {
-            kx = Conv<KV>::to_f(reinterpret_cast<const KV*>(p.k_pool)[row * hd + d]);
-            vx = Conv<KV>::to_f(reinterpret_cast<const KV*>(p.v_pool)[row * hd + d]);
+            const int64_t row = S.row[t & 1][r];
+            if (row >= 0) {
+              const uint8_t* sc = scale_of(row);
+              ks = scale_byte_to_f(sc[0]);
+              vs = scale_byte_to_f(sc[bs]);
+            }
           }
+          spread<KV>(&S.k[r * P + x * V], held[0][i], ks);
+          odd |= !spread<KV>(&S.v[r * P + x * V], held[1][i], vs);
         }
-        S.k[r * P + d] = kx;
-        S.v[r * P + d] = vx;
-        odd |= !isfinite(vx);
+      } else {
+        for (int e = tid; e < kKeys * D; e += kGenThreads) {
+          const int r = e / D, d = e - r * D;
+          const int64_t row = S.row[t & 1][r];
+          float kx = 0.f, vx = 0.f;
+          if (row >= 0 && d < hd) {
+            if constexpr (kQuant) {
+              const uint8_t* sc = scale_of(row);
+              kx = e4m3_to_f(reinterpret_cast<const uint8_t*>(p.k_pool)[row * hd + d]) * scale_byte_to_f(sc[0]);
+              vx = e4m3_to_f(reinterpret_cast<const uint8_t*>(p.v_pool)[row * hd + d]) * scale_byte_to_f(sc[bs]);
+            } else {
+              kx = Conv<KV>::to_f(reinterpret_cast<const KV*>(p.k_pool)[row * hd + d]);
+              vx = Conv<KV>::to_f(reinterpret_cast<const KV*>(p.v_pool)[row * hd + d]);
+            }
+          }
+          S.k[r * P + d] = kx;
+          S.v[r * P + d] = vx;
+          odd |= !(fabsf(vx) < INFINITY);
+        }
       }
+      find(t + 1);
       odd = __syncthreads_or(odd);
-      float s[4][4];
+      if (fetches && t + 1 < c.tile1) fetch(t + 1);  // lands while this step is computed
+      float2 s2[4][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+        for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 4
-      for (int d = 0; d < Smem::D; d += 4) {
+      for (int d = 0; d < D; d += 4) {
         float4 a[4], b[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(&S.q[(ty + 16 * i) * P + d]);
@@ -145,38 +254,40 @@ __global__ void __launch_bounds__(kGenThreads) chunk_generic_kernel(ChunkParams 
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
-            s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
-            s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
-            s[i][j] = fmaf(a[i].w, b[j].w, s[i][j]);
+            s2[i][j] = fma2(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y), s2[i][j]);
+            s2[i][j] = fma2(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w), s2[i][j]);
           }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        float s[4];
         float mx = m[i];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int pos = S.pos[tx + 16 * j];
+          const int pos = S.pos[t & 1][tx + 16 * j];
           const bool sees = pos <= qpos[i] && (p.window <= 0 || pos > qpos[i] - p.window || pos < p.sinks);
-          s[i][j] = sees ? s[i][j] * c2 : -INFINITY;
-          mx = fmaxf(mx, s[i][j]);
+          s[j] = sees ? (s2[i][j].x + s2[i][j].y) * c2 : -INFINITY;
+          mx = fmaxf(mx, s[j]);
         }
 #pragma unroll
         for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
         // nothing seen so far: any finite reference gives p = 2^-inf = 0
         const float ref = mx == -INFINITY ? 0.f : mx;
-        const float alpha = exp2f(m[i] - ref);
+        const float alpha = ex2(m[i] - ref);
         m[i] = mx;
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float e = exp2f(s[i][j] - ref);
+          const float e = ex2(s[j] - ref);
           sum += e;
           S.s[(ty + 16 * i) * PS + tx + 16 * j] = e;
         }
         l[i] = l[i] * alpha + sum;  // this thread's share; summed over the row's threads at the end
 #pragma unroll
-        for (int j = 0; j < 4 * D4; ++j) o[i][j] *= alpha;
+        for (int j = 0; j < 2 * D4; ++j) {
+          o[i][j].x *= alpha;
+          o[i][j].y *= alpha;
+        }
       }
       __syncwarp();  // a row's 16 threads share a warp
       if (!odd) {
@@ -193,23 +304,26 @@ __global__ void __launch_bounds__(kGenThreads) chunk_generic_kernel(ChunkParams 
               const float4 b = *reinterpret_cast<const float4*>(&S.v[(k + kk) * P + 64 * j + 4 * tx]);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                o[i][4 * j] = fmaf(a[i][kk], b.x, o[i][4 * j]);
-                o[i][4 * j + 1] = fmaf(a[i][kk], b.y, o[i][4 * j + 1]);
-                o[i][4 * j + 2] = fmaf(a[i][kk], b.z, o[i][4 * j + 2]);
-                o[i][4 * j + 3] = fmaf(a[i][kk], b.w, o[i][4 * j + 3]);
+                const float2 x = make_float2(a[i][kk], a[i][kk]);
+                o[i][2 * j] = fma2(x, make_float2(b.x, b.y), o[i][2 * j]);
+                o[i][2 * j + 1] = fma2(x, make_float2(b.z, b.w), o[i][2 * j + 1]);
               }
             }
         }
       } else {
         // infinities or NaN in V: they reach only the rows that see their token
         for (int k = 0; k < kKeys; ++k) {
-          const int pos = S.pos[k];
+          const int pos = S.pos[t & 1][k];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (!(pos <= qpos[i] && (p.window <= 0 || pos > qpos[i] - p.window || pos < p.sinks))) continue;
             const float a = S.s[(ty + 16 * i) * PS + k];
 #pragma unroll
-            for (int j = 0; j < 4 * D4; ++j) o[i][j] = fmaf(a, S.v[k * P + 64 * (j / 4) + 4 * tx + j % 4], o[i][j]);
+            for (int j = 0; j < 2 * D4; ++j) {
+              const float* v = &S.v[k * P + 64 * (j / 2) + 4 * tx + 2 * (j % 2)];
+              o[i][j].x = fmaf(a, v[0], o[i][j].x);
+              o[i][j].y = fmaf(a, v[1], o[i][j].y);
+            }
           }
         }
       }
@@ -218,28 +332,21 @@ __global__ void __launch_bounds__(kGenThreads) chunk_generic_kernel(ChunkParams 
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
       for (int off = 8; off > 0; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
-      const int r = ty + 16 * i, g = r % p.gw;
+      const int r = ty + 16 * i, tok = p.by_gw.div(r), g = r - tok * p.gw;
       if (r >= n_rows || g >= heads) continue;
-      if (c.whole()) {
-        const float inv = m[i] == -INFINITY ? 0.f : 1.f / l[i];  // sees nothing: zeros
-        T* out = reinterpret_cast<T*>(p.out) + (int64_t)(c.q_first + c.i0 + r / p.gw) * p.out_stride_tok +
-                 (int64_t)(head0 + g) * p.out_stride_head;
+      const bool whole = c.whole();
+      const float f = !whole ? 1.f : m[i] == -INFINITY ? 0.f : 1.f / l[i];  // sees nothing: zeros
+      const int64_t slot = part_slot(c) * p.rows + r;
+      T* out = reinterpret_cast<T*>(p.out) + (int64_t)(c.q_first + c.i0 + tok) * p.out_stride_tok + (int64_t)(head0 + g) * p.out_stride_head;
+      if (!whole && tx == 0) {
+        p.part_ml[slot * 2] = m[i];
+        p.part_ml[slot * 2 + 1] = l[i];
+      }
 #pragma unroll
-        for (int j = 0; j < 4 * D4; ++j) {
-          const int d = 64 * (j / 4) + 4 * tx + j % 4;
-          if (d < hd) out[d] = Conv<T>::from_f(m[i] == -INFINITY ? 0.f : o[i][j] * inv);
-        }
-      } else {
-        const int64_t slot = part_slot(c) * p.rows + r;
-        if (tx == 0) {
-          p.part_ml[slot * 2] = m[i];
-          p.part_ml[slot * 2 + 1] = l[i];
-        }
-#pragma unroll
-        for (int j = 0; j < 4 * D4; ++j) {
-          const int d = 64 * (j / 4) + 4 * tx + j % 4;
-          if (d < hd) p.part_o[slot * hd + d] = o[i][j];
-        }
+      for (int j = 0; j < D4; ++j) {
+        const float4 y = make_float4(o[i][2 * j].x * f, o[i][2 * j].y * f, o[i][2 * j + 1].x * f, o[i][2 * j + 1].y * f);
+        if (whole) store4(out, 64 * j + 4 * tx, hd, y, vec);
+        else store4(p.part_o + slot * hd, 64 * j + 4 * tx, hd, y, hd % 4 == 0);
       }
     }
   }
@@ -254,22 +361,6 @@ __global__ void __launch_bounds__(kGenThreads) chunk_generic_kernel(ChunkParams 
 // time, the 17 pieces of a decode took 25 us).  A lane holds 4 dims (and 128 more).
 constexpr int kMergeWarps = 4, kMergeBatch = 8, kMergeRows = 4;
 
-template <typename T>
-__device__ __forceinline__ void store4(T* out, int d, int D, const float4& v, bool vec) {
-  if (vec && d + 3 < D) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(out + d) = v;
-    } else {
-      T y[4] = {Conv<T>::from_f(v.x), Conv<T>::from_f(v.y), Conv<T>::from_f(v.z), Conv<T>::from_f(v.w)};
-      *reinterpret_cast<uint2*>(out + d) = *reinterpret_cast<const uint2*>(y);
-    }
-    return;
-  }
-  const float y[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (d + u < D) out[d + u] = Conv<T>::from_f(y[u]);
-}
 __device__ __forceinline__ float4 load4(const float* o, int d, int D) {
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (D % 4 == 0) {
@@ -306,7 +397,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
   const int kvh = h0.y, slice = h0.z, i0 = h0.w, n_pieces = h1.y - cta + 2, first = h1.z, n = h1.w;
   const int heads = slice_heads(p, slice), n_rows = (min(n, i0 + p.tokens) - i0) * p.gw;
   const int lane = threadIdx.x & 31, D = p.head_dim;
-  const bool vec = p.out_stride_tok % 4 == 0 && p.out_stride_head % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+  const bool vec = out_vec<T>(p);
   const auto slot = [&](int i, int r) { return ((int64_t)(cta - 1 + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + r; };
   const auto out_row = [&](int r, int g) {
     return reinterpret_cast<T*>(p.out) + (int64_t)(first + i0 + p.by_gw.div(r)) * p.out_stride_tok +
@@ -418,22 +509,24 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
 
 template <typename T, typename KV>
 int launch_generic(ChunkParams& p, cudaStream_t st) {
-  const auto go = [&](auto kernel, size_t smem) -> int {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const auto go = [&](auto kernel, size_t smem, bool (&done)[kMaxDevices]) -> int {
+    const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem, done);
     if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
     kernel<<<p.n_ctas, kGenThreads, smem, st>>>(p);
     return cuda_status(cudaGetLastError(), "paged_chunk launch");
   };
+  static bool done[3][kMaxDevices] = {};
   static_assert(sizeof(GenSmem<4>) <= 232448, "shared memory budget");
   static_assert(sizeof(GenSmem<1>().q) + sizeof(GenSmem<1>().k) >= kMaxChunkBatch * 4, "plan scratch");
-  if (p.head_dim <= 64) return go(chunk_generic_kernel<T, KV, 1>, sizeof(GenSmem<1>));
-  if (p.head_dim <= 128) return go(chunk_generic_kernel<T, KV, 2>, sizeof(GenSmem<2>));
-  return go(chunk_generic_kernel<T, KV, 4>, sizeof(GenSmem<4>));
+  if (p.head_dim <= 64) return go(chunk_generic_kernel<T, KV, 1>, sizeof(GenSmem<1>), done[0]);
+  if (p.head_dim <= 128) return go(chunk_generic_kernel<T, KV, 2>, sizeof(GenSmem<2>), done[1]);
+  return go(chunk_generic_kernel<T, KV, 4>, sizeof(GenSmem<4>), done[2]);
 }
 
-// The largest CTA count and unit rows of the kernels, for the workspace.
-int64_t max_ctas() { return (int64_t)num_sms() * 2; }
+// The largest workspace of the kernels: one CTA per SM with units of 256 rows, or two with 64.
+int64_t max_ctas() { return num_sms(); }
 constexpr int kMaxRows = 256;
+static_assert(2 * kRows <= kMaxRows, "two CTAs per SM");
 
 }  // namespace
 
@@ -467,7 +560,7 @@ int64_t snapmind_paged_gqa_chunk_workspace_bytes(int32_t head_dim) {
   if (head_dim <= 0 || head_dim > kGenMaxD) return 0;
   ChunkParams p = {};
   p.head_dim = head_dim;
-  return plan_workspace(p, nullptr, max_ctas(), kMaxRows);
+  return plan_workspace(p, nullptr, 2 * max_ctas(), kMaxRows / 2);
 }
 
 int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stride_head, int dtype, const void* k_pool,
@@ -520,10 +613,11 @@ int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stri
   p.window = window < (1 << 30) ? window : (1 << 30);  // positions stay below 2^30
   p.sinks = sinks < (1 << 30) ? sinks : (1 << 30);
   p.err = err_word;
-  const int64_t need = plan_workspace(p, workspace, max_ctas(), kMaxRows);
+  const int64_t need = snapmind_paged_gqa_chunk_workspace_bytes(head_dim);
   SNAPMIND_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                      "paged_chunk: workspace needs %lld bytes on a 256-byte boundary, got %lld", (long long)need,
                      (long long)workspace_bytes);
+  p.workspace = workspace;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
   if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && decode_sinks_supported(p, dtype, pool_dtype)) {

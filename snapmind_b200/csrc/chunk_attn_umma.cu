@@ -709,7 +709,8 @@ int launch(const ChunkParams& p, cudaStream_t st) {
     return SNAPMIND_ERR_CUDA;
   }
   auto kernel = chunk_umma_kernel<T, D, kQuant>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D, kQuant>());
+  static bool done[kMaxDevices] = {};
+  const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem_bytes<D, kQuant>(), done);
   if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
   kernel<<<p.n_ctas, Roles<kQuant>::kThreads, smem_bytes<D, kQuant>(), st>>>(k_map, v_map, p);
   return cuda_status(cudaGetLastError(), "paged_chunk launch");

@@ -44,6 +44,7 @@ struct ChunkParams {
   int32_t key_tile;        // keys of a tile
   int32_t n_ctas;
   FastDiv by_gw, by_block, by_tile;  // divisions by gw, block_size, key_tile
+  void* workspace;
   int32_t* heads;   // workspace: [n_ctas][kPieceInts], see PieceInfo
   float* part_ml;   // workspace: [n_ctas][2][rows][2] maximum (log2 units), sum
   float* part_o;    // workspace: [n_ctas][2][rows][head_dim]
@@ -368,17 +369,17 @@ int launch_chunk_umma(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st
 bool decode_sinks_supported(const ChunkParams& p, int dtype, int pool_dtype);
 int launch_decode_sinks(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st);
 
-// Unit geometry for kernels of `rows` query rows, `key_tile` keys and `n_ctas` CTAs.
-inline void plan_geometry(ChunkParams& p, int rows, int key_tile, int n_ctas) {
-  p.gw = p.group < rows ? p.group : rows;
-  p.n_slices = (p.group + p.gw - 1) / p.gw;
-  p.tokens = rows / p.gw;
-  p.rows = rows;
-  p.key_tile = key_tile;
-  p.n_ctas = n_ctas;
-  p.by_gw = FastDiv(p.gw);
-  p.by_block = FastDiv(p.block_size);
-  p.by_tile = FastDiv(key_tile);
+// Sets a kernel's shared-memory attributes once per device (`done` is the instantiation's own).
+constexpr int kMaxDevices = 64;
+inline cudaError_t kernel_attributes(const void* kernel, size_t smem, bool (&done)[kMaxDevices]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < kMaxDevices && done[dev])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess)  // room for two CTAs where two are meant to share an SM
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess && dev < kMaxDevices) done[dev] = true;
+  return e;
 }
 
 // Workspace regions of n_ctas CTAs: heads, then maxima and sums, then partial outputs.
@@ -390,6 +391,20 @@ inline int64_t plan_workspace(ChunkParams& p, void* workspace, int64_t n_ctas, i
   p.part_ml = reinterpret_cast<float*>(w + ml_off);
   p.part_o = reinterpret_cast<float*>(w + o_off);
   return o_off + n_ctas * 2 * rows * p.head_dim * 4;
+}
+
+// Unit geometry for kernels of `rows` query rows, `key_tile` keys and `n_ctas` CTAs.
+inline void plan_geometry(ChunkParams& p, int rows, int key_tile, int n_ctas) {
+  p.gw = p.group < rows ? p.group : rows;
+  p.n_slices = (p.group + p.gw - 1) / p.gw;
+  p.tokens = rows / p.gw;
+  p.rows = rows;
+  p.key_tile = key_tile;
+  p.n_ctas = n_ctas;
+  p.by_gw = FastDiv(p.gw);
+  p.by_block = FastDiv(p.block_size);
+  p.by_tile = FastDiv(key_tile);
+  plan_workspace(p, p.workspace, n_ctas, rows);
 }
 
 }  // namespace snapmind

@@ -514,7 +514,8 @@ int launch(const ChunkParams& p, cudaStream_t st) {
     return SNAPMIND_ERR_CUDA;
   }
   auto kernel = decode_sinks_kernel<T, kQuant>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<kQuant>());
+  static bool done[kMaxDevices] = {};
+  const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem_bytes<kQuant>(), done);
   if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
   kernel<<<p.n_ctas, kThreads, smem_bytes<kQuant>(), st>>>(k_map, v_map, p);
   return cuda_status(cudaGetLastError(), "paged_chunk launch");

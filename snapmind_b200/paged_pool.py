@@ -133,7 +133,7 @@ class PagedKVPool(BlockPool):
                 _lib.dtype_code(k_new.dtype), st[axes[0]], 0 if seq_axis is None else st[seq_axis], st[axes[1]],
                 st[axes[2]], self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq,
                 starts, start0, None if cu is None else cu.data_ptr(), n_layers, batch, n_tokens, total,
-                self.n_kv_heads, self.head_dim, self.block_size, self.num_blocks, self.err.data_ptr(), self._stream(),
+                self.n_kv_heads, self.head_dim, self.block_size, self.num_blocks, self.err.data_ptr(), _lib.raw_stream(self._index),
             )  # fmt: skip
         _lib.check(status, f"{type(self).__name__}.append")
 
@@ -187,7 +187,7 @@ class PagedKVPool(BlockPool):
                 None if cu is None else cu.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
                 d ** -0.5 if scale is None else scale, total if cu is None else cu.shape[0] - 1, total, n_q,
                 self.n_kv_heads, d, self.block_size, self.num_blocks, window, sinks, flags, ws.data_ptr(), need,
-                self.err.data_ptr(), self._stream(),
+                self.err.data_ptr(), _lib.raw_stream(self._index),
             )  # fmt: skip
         _lib.check(status, f"{type(self).__name__}.attend")
         return out

@@ -54,8 +54,7 @@ class QuantizedKVPool(PagedKVPool):
         total = int(self._host_lens[:batch].sum())
         per_layer = total * self.n_kv_heads * self.head_dim
         if out is None:
-            k_out = torch.empty((len(layers), per_layer), dtype=self.dtype, device=self.device)
-            v_out = torch.empty_like(k_out)
+            k_out, v_out = torch.empty((2, len(layers), per_layer), dtype=self.dtype, device=self.device).unbind(0)
         else:
             k_out, v_out = out
             for t in (k_out, v_out):
@@ -75,7 +74,7 @@ class QuantizedKVPool(PagedKVPool):
                 self.scale_layer_stride, k_out.data_ptr(), v_out.data_ptr(), self._dcode, k_out.shape[1],
                 k_out.shape[1], self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq,
                 self.seq_lens.data_ptr(), len(layers), batch, self.n_kv_heads, self.head_dim, self.block_size,
-                self.num_blocks, self.err.data_ptr(), self._stream(),
+                self.num_blocks, self.err.data_ptr(), _lib.raw_stream(self._index),
             )  # fmt: skip
         _lib.check(status, "QuantizedKVPool.gather")
         return k_out, v_out
