@@ -587,6 +587,9 @@ int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stri
   if (batch == 0 || total_q == 0) return SNAPMIND_OK;
   SNAPMIND_CHECK_ARG(q && k_pool && v_pool && block_tables && seq_lens && out, "paged_chunk: null pointer");
   ChunkParams p = {};
+  // the stride of an axis of one is never used: give it the dense value, whatever the caller's is
+  if (total_q == 1) q_stride_tok = out_stride_tok = (int64_t)n_q_heads * head_dim;
+  if (n_q_heads == 1) q_stride_head = out_stride_head = head_dim;
   p.q = q;
   p.q_stride_tok = q_stride_tok;
   p.q_stride_head = q_stride_head;
@@ -626,7 +629,7 @@ int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stri
   }
   if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && chunk_umma_supported(p, dtype, pool_dtype)) {
     const int rc = launch_chunk_umma(p, dtype, pool_dtype, st);
-    return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
+    if (rc != SNAPMIND_ERR_UNSUPPORTED) return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
   }
   const int ctas = num_sms() * (head_dim <= 64 ? 2 : 1);
   plan_geometry(p, kRows, kKeys, ctas);

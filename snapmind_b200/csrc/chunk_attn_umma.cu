@@ -9,9 +9,10 @@
 // products, the other tile's 128 threads (one row each) take its scores.
 // A row keeps a reference maximum that is raised only when a score exceeds it by 2^8:
 // then O is rescaled in TMEM, else O is never touched between the products.
-//   warps 0-3, 4-7  softmax of tile 0 / 1: thread = row = TMEM lane; they load their Q tile,
-//                   write P to shared memory, and write out the finished rows
-//   warp 8          issues the MMAs of the scores, and another warp those of P V: a wait takes some
+//   warps 0-3, 4-7  softmax of tile 0 / 1: thread = row = TMEM lane; they write P to shared memory,
+//                   and write out the finished rows
+//   warp 8          loads Q (one copy per tile and 64 columns: 128 threads fetching rows took 14000
+//                   cycles a unit), issues the MMAs of the scores, and another warp those of P V: a wait takes some
 //                   200 cycles next to operand reads that fill shared memory's bandwidth, and the two
 //                   streams cover each other's
 //   two more        stage K and V by TMA; over 8-bit caches as they are, and four warps more turn
@@ -61,7 +62,7 @@ template <int D, bool kQuant> struct Shape {
 
 struct Ctrl {
   uint64_t full[2][4], empty[2][4];  // K's and V's stages
-  uint64_t q_full[2];   // softmax threads: the Q tile of a piece is in shared memory
+  uint64_t q_full;      // the Q tiles of a piece have landed
   uint64_t s_full[2];   // MMA commit: scores ready
   uint64_t s_free[2];   // softmax threads: scores read (the group's next ones may replace them)
   uint64_t p_full[2];   // softmax threads: P written
@@ -186,8 +187,8 @@ template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setm
 
 template <typename T, int D, bool kQuant>
 __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
-    chunk_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                      ChunkParams p) {
+    chunk_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                      const __grid_constant__ CUtensorMap v_map, ChunkParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using Sh = Shape<D, kQuant>;
@@ -210,13 +211,13 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       mbar_init(smem_u32(&C.raw_empty[kv]), kConvert);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(smem_u32(&C.q_full[t]), 128);
       mbar_init(smem_u32(&C.s_full[t]), 1);
       mbar_init(smem_u32(&C.s_free[t]), 128);
       mbar_init(smem_u32(&C.p_full[t]), 128);
       mbar_init(smem_u32(&C.pv_done[t]), 1);
       mbar_init(smem_u32(&C.v_ready[t]), 1);
     }
+    mbar_init(smem_u32(&C.q_full), 1);
     mbar_init(smem_u32(&C.x_ml), 128);
     mbar_init(smem_u32(&C.x_done), 128);
     C.abort = 0;
@@ -228,6 +229,9 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
   }
   plan_block(p, C.plan, reinterpret_cast<int32_t*>(p_s));
   if (tid == 0) write_piece_info(p, C.plan);
+  // rows of Q that no copy fills (128 / gw has a remainder) are zeros, not whatever lay there
+  for (uint32_t i = tid; i < 2 * Sh::kTileBytes / 16; i += Ro::kThreads) reinterpret_cast<uint4*>(q_s)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -251,7 +255,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       const Piece& c = w.c;
       const int i1 = min(c.n, c.i0 + p.tokens), n = c.tile1 - c.tile0;
       const EdgeTiles edge(p, key_range(p, c.len, c.n, c.i0, i1));
-      const int ahead = (i1 - c.i0) * p.gw <= kTileM ? 2 : 1, lead = min(n, ahead);
+      const int ahead = i1 - c.i0 <= p.tokens / 2 ? 2 : 1, lead = min(n, ahead);
       for (int i = 0; i < 2 * n; ++i) {
         const int x = i - lead;
         const int kv = x < 0 ? 0 : (x < 2 * (n - lead) ? x & 1 : 1);
@@ -352,8 +356,8 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     const bool do_s = warp == Ro::kScores, do_o = warp == Ro::kValues;
     const uint32_t leader = elect_one_sync();
     uint32_t tiles = 0, piece = 0;  // key tiles, pieces before this one
-    uint32_t s0[2] = {0, 0}, pieces1 = 0;  // steps of group 0 / 1 before this piece; pieces with a tile 1
-    uint32_t last_bar = 0, last_parity = 0;
+    uint32_t s0[2] = {0, 0};  // steps of group 0 / 1 before this piece
+    uint32_t last_bar = 0, last_parity = 0, q_pending = 0;
     bool ok = true;
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
       ok = ok && __all_sync(0xffffffffu, role_wait(C, smem_u32(bar), parity));
@@ -393,13 +397,26 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       const Piece& c = w.c;
       const int n = c.tile1 - c.tile0;
       const int i1 = min(c.n, c.i0 + p.tokens);
-      const bool split = (i1 - c.i0) * p.gw <= kTileM;
+      const bool split = i1 - c.i0 <= p.tokens / 2;
       const int ahead = split ? 2 : 1;
       const EdgeTiles edge(p, key_range(p, c.len, c.n, c.i0, i1));
+      if (do_s) {
+        // the groups have read the last scores of the piece before: its products are done with Q
+        for (int t = 0; t < 2 && ok; ++t)
+          if (s0[t] > 0) wait(&C.s_free[t], (s0[t] - 1) & 1);
+        if (!ok) break;
+        const int qt = split ? 1 : 2, tpt = p.tokens / 2, head0 = c.kvh * p.group + c.slice * p.gw;
+        const uint32_t bar = smem_u32(&C.q_full);
+        mbar_arrive_expect_tx_p(leader, bar, qt * (D / 64) * tpt * p.gw * 128u);
+        for (int t = 0; t < qt; ++t)
+#pragma unroll
+          for (int kb = 0; kb < D / 64; ++kb)
+            tma_load_3d_p(leader, smem_u32(q_s + t * Sh::kTileBytes + kb * kBlockBytes), &q_map, 64 * kb, head0,
+                          c.q_first + c.i0 + t * tpt, bar);
+        q_pending = piece + 1;
+        if (!wait(&C.q_full, piece & 1)) break;
+      }
       // the scores of the first tile(s)
-      if (do_s && wait(&C.q_full[0], piece & 1) && !split) wait(&C.q_full[1], pieces1 & 1);
-      for (int t = 0; t < 2 && ok && do_s; ++t)  // and the groups have read the last scores of the piece before
-        if (s0[t] > 0) wait(&C.s_free[t], (s0[t] - 1) & 1);
       for (int j = 0; j < min(n, ahead) && ok && do_s; ++j) {
         const uint32_t i = tiles + j;
         if (!wait(&C.full[0][Sh::stage(0, i)], Sh::parity(0, i))) break;
@@ -436,11 +453,11 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       }
       tiles += n;
       ++piece;
-      pieces1 += split ? 0 : 1;
       s0[0] += split ? (n + 1) / 2 : n;
       s0[1] += split ? n / 2 : n;
     }
     if (!ok && lane == 0) give_up(C, p.err);
+    if (q_pending) mbar_wait(smem_u32(&C.q_full), (q_pending - 1) & 1);  // Q has landed (bounded)
     if (last_bar) mbar_wait(last_bar, last_parity);  // MMAs in flight end (bounded) before TMEM goes
   }
   } else {
@@ -449,47 +466,22 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     const int t = warp >> 2, r = tid & 127;
     const uint32_t lanes = ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t t_s = tmem + lanes + t * kKeys, t_o = tmem + lanes + 2 * kKeys + t * D;
-    const bool flip = p.scale < 0.f;  // a negative scale is folded into Q, so the largest score has the largest weight
+    const bool flip = p.scale < 0.f;  // then the scores change sign: the largest has the largest weight
     const float c2 = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
     uint8_t* prow = p_s + r * 128;
     const uint32_t sw = (uint32_t)(r & 7);
     uint32_t step = 0, tiles = 0, edges = 0, splits = 0, other_steps = 0;
     bool ok = true;
-    // Q tile t of a piece, by the group's 128 threads
-    const auto load_q = [&](const Piece& c) {
-      const int n_rows = (min(c.n, c.i0 + p.tokens) - c.i0) * p.gw;
-      if (t * kTileM >= n_rows) return;
-      const int heads = slice_heads(p, c.slice), head0 = c.kvh * p.group + c.slice * p.gw;
-#pragma unroll 4
-      for (int e = r; e < kTileM * (D / 8); e += 128) {
-        const int row = e / (D / 8), ch = e % (D / 8), R = t * kTileM + row;
-        const int tok = p.by_gw.div(R), g = R - tok * p.gw;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (R < n_rows && g < heads)
-          x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) +
-                                              (int64_t)(c.q_first + c.i0 + tok) * p.q_stride_tok +
-                                              (int64_t)(head0 + g) * p.q_stride_head + ch * 8);
-        if (flip) {
-          x.x ^= 0x80008000u;
-          x.y ^= 0x80008000u;
-          x.z ^= 0x80008000u;
-          x.w ^= 0x80008000u;
-        }
-        *reinterpret_cast<uint4*>(q_s + t * Sh::kTileBytes + (ch / 8) * kBlockBytes + row * 128 + (((uint32_t)(ch % 8) ^ (row & 7)) << 4)) = x;
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(smem_u32(&C.q_full[t]));
-    };
-    if (on) load_q(w.c);
     while (on && ok) {
       const Piece c = w.c;
       const int n = c.tile1 - c.tile0;
-      const int i1 = min(c.n, c.i0 + p.tokens), n_rows = (i1 - c.i0) * p.gw;
-      const bool split = n_rows <= kTileM;
-      const int R = (split ? 0 : t * kTileM) + r, tok = p.by_gw.div(min(R, n_rows - 1));
+      const int i1 = min(c.n, c.i0 + p.tokens), tpt = p.tokens / 2;
+      const bool split = i1 - c.i0 <= tpt;
+      // the row's token of the unit and head of the slice
+      const int rt = p.by_gw.div(r), g = r - rt * p.gw, tok = (split ? 0 : t * tpt) + rt;
       const KeyRange kr = key_range(p, c.len, c.n, c.i0, i1);
       const EdgeTiles edge(p, kr);
-      const int qpos = kr.pos0 + tok;
+      const int qpos = kr.pos0 + min(tok, i1 - c.i0 - 1);
       // on the virtual axis the row sees [v_lo, v_hi) and [0, v_s)
       const int v_hi = max(0, qpos + 1 - kr.shift);
       const int v_lo = p.window > 0 ? max(0, qpos - p.window + 1) - kr.shift : 0;
@@ -521,6 +513,10 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
 #pragma unroll
               for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(vrow + h * 1024 + x * 16) = make_uint4(0, 0, 0, 0);
           }
+        }
+        if (flip) {
+#pragma unroll
+          for (int x = 0; x < kKeys; ++x) s[x] = -s[x];
         }
         {
           const int lo = v_lo - v0, hi = v_hi - v0, sk = v_s - v0;
@@ -599,17 +595,11 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       if (!ok) break;
       tiles += n;
       if (split) {
-        // the other group's scores read tile 0's Q too: all done before the next Q may land there
-        // (group 0's last scores follow all but the last of group 1's, so the phase is the one meant)
         other_steps += (n - (t ^ 1) + 1) / 2;
-        if (t == 0 && other_steps > 0) ok = role_wait(C, smem_u32(&C.s_full[1]), (other_steps - 1) & 1);
       } else {
         other_steps += n;
       }
-      // the next piece's Q goes out first (this piece's scores are all done), so that its products
-      // start under this piece's epilogue
       on = w.next(p);
-      if (on && ok) load_q(w.c);
       if (ok && step > step0) ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);
       const uint32_t t_x = tmem + lanes + 2 * kKeys + (t ^ 1) * D;  // the other group's O
       float f = 1.f, fx = 0.f;
@@ -639,10 +629,9 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         break;
       }
       tc_fence_after();
-      const int heads = slice_heads(p, c.slice), rt = p.by_gw.div(R), g = R - rt * p.gw;
-      const bool mine = R < n_rows && g < heads, whole = c.whole();
-      const int64_t slot = part_slot(c) * p.rows + R;
-      T* out = reinterpret_cast<T*>(p.out) + (int64_t)(c.q_first + c.i0 + rt) * p.out_stride_tok +
+      const bool mine = rt < tpt && tok < i1 - c.i0 && g < slice_heads(p, c.slice), whole = c.whole();
+      const int64_t slot = part_slot(c) * p.rows + tok * p.gw + g;
+      T* out = reinterpret_cast<T*>(p.out) + (int64_t)(c.q_first + c.i0 + tok) * p.out_stride_tok +
                (int64_t)(c.kvh * p.group + c.slice * p.gw + g) * p.out_stride_head;
       if (!whole && mine) {
         p.part_ml[slot * 2] = m;
@@ -695,24 +684,34 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
   }
 }
 
+// Q as [token][head][dim]: a box is the gw heads of a slice of 128 / gw tokens, 64 columns.
+bool q_tiles_map(CUtensorMap* map, bool bf16, const ChunkParams& p, int D) {
+  EncodeTiledFn fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.n_q_heads, (cuuint64_t)p.total_q};
+  const cuuint64_t strides[2] = {(cuuint64_t)p.q_stride_head * 2, (cuuint64_t)p.q_stride_tok * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)p.gw, (cuuint32_t)p.tokens / 2};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(p.q), dims,
+            strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D, bool kQuant>
 int launch(const ChunkParams& p, cudaStream_t st) {
-  CUtensorMap k_map = {}, v_map = {};
+  CUtensorMap q_map, k_map, v_map;
   const uint64_t rows = (uint64_t)p.num_blocks * p.n_kv_heads * p.block_size;
   const uint32_t box = p.block_size < kKeys ? p.block_size : kKeys;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   const bool mapped = kQuant ? tensor_map_bytes(&k_map, p.k_pool, D, rows, box, false) && tensor_map_bytes(&v_map, p.v_pool, D, rows, box, false)
                              : tensor_map_row_groups(&k_map, bf16, p.k_pool, rows, D, box / 8) &&
                                    tensor_map_row_groups(&v_map, bf16, p.v_pool, rows, D, box / 8);
-  if (!mapped) {
-    set_last_error("paged_chunk: tensor map encoding failed");
-    return SNAPMIND_ERR_CUDA;
-  }
+  if (!mapped || !q_tiles_map(&q_map, bf16, p, D)) return SNAPMIND_ERR_UNSUPPORTED;  // the caller takes the CUDA-core kernel
   auto kernel = chunk_umma_kernel<T, D, kQuant>;
   static bool done[kMaxDevices] = {};
   const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem_bytes<D, kQuant>(), done);
   if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
-  kernel<<<p.n_ctas, Roles<kQuant>::kThreads, smem_bytes<D, kQuant>(), st>>>(k_map, v_map, p);
+  kernel<<<p.n_ctas, Roles<kQuant>::kThreads, smem_bytes<D, kQuant>(), st>>>(q_map, k_map, v_map, p);
   return cuda_status(cudaGetLastError(), "paged_chunk launch");
 }
 
@@ -728,7 +727,7 @@ bool chunk_umma_supported(const ChunkParams& p, int dtype, int pool_dtype) {
   if (bs != 8 && bs != 16 && bs != 32 && bs != 64 && bs % 128 != 0) return false;
   const auto a16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
   if (!a16(p.q) || !a16(p.out) || !a16(p.k_pool) || !a16(p.v_pool)) return false;
-  if (p.q_stride_tok % 8 || p.q_stride_head % 8 || p.out_stride_tok % 8 || p.out_stride_head % 8) return false;
+  if (p.q_stride_tok <= 0 || p.q_stride_head <= 0 || p.q_stride_tok % 8 || p.q_stride_head % 8 || p.out_stride_tok % 8 || p.out_stride_head % 8) return false;
   if ((int64_t)p.num_blocks * p.n_kv_heads * bs >= (int64_t)1 << 31) return false;  // TMA row coordinate
   if (pool_dtype == SNAPMIND_DTYPE_E4M3 && !a16(p.scales)) return false;
   return encode_tiled() != nullptr;
@@ -736,6 +735,11 @@ bool chunk_umma_supported(const ChunkParams& p, int dtype, int pool_dtype) {
 
 int launch_chunk_umma(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st) {
   plan_geometry(p, 2 * kTileM, kKeys, num_sms());
+  // two tiles of whole tokens: a slice has at most 128 heads
+  p.gw = p.group < kTileM ? p.group : kTileM;
+  p.n_slices = (p.group + p.gw - 1) / p.gw;
+  p.tokens = 2 * (kTileM / p.gw);
+  p.by_gw = FastDiv(p.gw);
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
   const auto go = [&](auto t) -> int {
     using T = decltype(t);

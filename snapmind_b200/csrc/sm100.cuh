@@ -139,6 +139,14 @@ __device__ __forceinline__ void tma_load_2d_p(uint32_t leader, uint32_t dst, con
       "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_p(uint32_t leader, uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                              uint32_t bar) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %0, 0; @p cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::"
+      "bytes [%1], [%2, {%3, %4, %5}], [%6]; }" ::"r"(leader),
+      "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_4d_p(uint32_t leader, uint32_t dst, const CUtensorMap* map, int x, int y, int z,
                                               int w, uint32_t bar) {
   asm volatile(
