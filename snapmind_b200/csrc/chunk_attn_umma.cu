@@ -161,13 +161,18 @@ __device__ __forceinline__ void dequant16(const uint4& codes, uint8_t byte, uint
   const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
   uint32_t o[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 2] >> (16 * (i & 1))), __NV_E4M3);
-    const float2 f = mul2(__half22float2(__half2(h)), s);
-    if constexpr (std::is_same<T, __half>::value) {  // hold to f16's range, keep NaN
-      o[i] = pack2<T>(fabsf(f.x) > 65504.f ? copysignf(65504.f, f.x) : f.x, fabsf(f.y) > 65504.f ? copysignf(65504.f, f.y) : f.y);
-    } else {
-      o[i] = pack2<T>(f.x, f.y);
+  for (int i = 0; i < 8; i += 2) {
+    uint32_t h[2];
+    asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }"
+        : "=r"(h[0]), "=r"(h[1])
+        : "r"(w[i / 2]));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float2 f = mul2(__half22float2(*reinterpret_cast<const __half2*>(&h[j])), s);
+      if constexpr (std::is_same<T, __half>::value)  // hold to f16's range, keep NaN
+        o[i + j] = pack2<T>(fabsf(f.x) > 65504.f ? copysignf(65504.f, f.x) : f.x, fabsf(f.y) > 65504.f ? copysignf(65504.f, f.y) : f.y);
+      else
+        o[i + j] = pack2<T>(f.x, f.y);
     }
   }
   lo = make_uint4(o[0], o[1], o[2], o[3]);
@@ -272,7 +277,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         uint8_t* dst = base + Sh::at(kv, num) + (ch / 4) * 1024;
         const int v0 = (c.tile0 + j) * kKeys;
         const bool edges = edge(c.tile0 + j);
-#pragma unroll 2
+#pragma unroll 1
         for (int r = r0; r < 128; r += kRowsPass) {
           uint4 codes = *reinterpret_cast<const uint4*>(raw + r * D);
           uint8_t byte = C.scales[kv][r];
