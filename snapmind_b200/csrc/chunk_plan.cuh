@@ -288,12 +288,13 @@ struct TileRows {
     const int v = (first_tile + (lane >> log_parts)) * p.key_tile + (lane & (parts - 1)) * box;
     return v < kr.v_len ? kr.position(v) : -1;
   }
-  // Table entry of the lane's part; INT32_MIN: no key there.
+  // Table entry of the lane's part; kNoKey: no key there, kNoEntry: past the table's row.
+  static constexpr int32_t kNoKey = INT32_MIN, kNoEntry = INT32_MIN + 1;
   __device__ __forceinline__ int32_t entry(int first_tile) const {
     const int pos = position(first_tile);
-    if (pos < 0 || first_tile + (lane >> log_parts) >= end) return INT32_MIN;
+    if (pos < 0 || first_tile + (lane >> log_parts) >= end) return kNoKey;
     const int lb = p.by_block.div(pos);
-    return lb < p.table_width ? table[lb] : -1;
+    return lb < p.table_width ? table[lb] : kNoEntry;
   }
   // Makes `tile` part of the current batch (tiles are asked for in ascending order).
   __device__ __forceinline__ void advance(int tile) {
@@ -304,8 +305,8 @@ struct TileRows {
     if (e >= 0 && e < p.num_blocks) {
       const int pos = position(first);
       rows = (e * p.n_kv_heads + kvh) * p.block_size + (pos - p.by_block.div(pos) * p.block_size);
-    } else if (e != INT32_MIN) {
-      flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
+    } else if (e != kNoKey) {
+      flag_error(p.err, e == kNoEntry ? SNAPMIND_DEVERR_TABLE : SNAPMIND_DEVERR_BLOCK_ID);
     }
     next = entry(first + (32 >> log_parts));
   }

@@ -526,3 +526,140 @@ def test_generator_on_a_quantised_pool(cuda_device):
             # of the row's size per rounding, twice, and the weights' own
             assert (got - want).abs().max() <= 4 * 2.0**-8 * want.abs().max()
     pool.check()
+
+
+KERNELS = [  # (cache, head dim, one token per sequence, force_generic): every attention kernel
+    ("same", 128, False, False), ("same", 64, False, False), ("e4m3", 128, False, False), ("same", 128, True, False),
+    ("e4m3", 128, True, False), ("same", 128, False, True), ("e4m3", 64, True, True),
+]
+
+
+@pytest.mark.parametrize("scale", [-0.07, 0.0, 1e-3, 0.9])
+@pytest.mark.parametrize("cache,d,single,generic", KERNELS)
+def test_scales(cuda_device, cache, d, single, generic, scale):
+    """Any softmax scale: a negative one turns the scores round, zero gives the mean of V."""
+    lens = [300, 77]
+    pool, ks, vs = make_pool(torch.bfloat16, lens, 2, d, 16, 40, cache)
+    cu = [0, 1, 2] if single else [0, 40, 45]
+    q = torch.randn((cu[-1], 8, d), device="cuda").bfloat16()
+    if single:
+        out = pool.decode(0, q, scale=scale, window=90, sinks=2, force_generic=generic)
+    else:
+        out = pool.attend_chunk(0, q, torch.tensor(cu, dtype=torch.int32, device="cuda"), scale=scale, window=90, sinks=2,
+                                force_generic=generic)
+    pool.check()
+    check_scaled(out, q, cu, ks, vs, 90, 2, scale)
+
+
+def check_scaled(out, q, cu, ks, vs, window, sinks, scale):
+    # a negative scale is the positive one of -q: the tolerance's sum of magnitudes is the same
+    s = -1 if scale < 0 else 1
+    check(out, q * s, cu, ks, vs, window, sinks, 2.0**-8, abs(scale))
+
+
+@pytest.mark.parametrize("single", [False, True])
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_rows_off_every_boundary(cuda_device, cache, single):
+    """q and out one element off a 16-byte boundary, offsets that do not start at 0, odd strides."""
+    lens = [130, 64]
+    pool, ks, vs = make_pool(torch.bfloat16, lens, 2, 128, 16, 41, cache)
+    cu = [0, 1, 2] if single else [3, 60, 71]
+    flat = torch.randn(75 * 9 * 129 + 1, device="cuda").bfloat16()
+    q = flat[1:].view(75, 9, 129)[:cu[-1], :8, :128]
+    out = torch.full_like(flat, 5.0)[1:].view(75, 9, 129)[:cu[-1], :8, :128]
+    if single:
+        pool.decode(0, q, out=out, window=100, sinks=4)
+    else:
+        pool.attend_chunk(0, q, torch.tensor(cu, dtype=torch.int32, device="cuda"), out=out, window=100, sinks=4)
+    pool.check()
+    if not single:
+        assert (out[:3] == 5.0).all()
+    check(out[cu[0]:], q[cu[0]:], [c - cu[0] for c in cu], ks, vs, 100, 4, 2.0**-8)
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_offsets_past_32_bits(cuda_device, cache):
+    """Blocks at the end of a pool of more than 2^32 bytes (and rows whose elements pass 2^32): written,
+    read back, attended."""
+    from snapmind_b200 import PagedKVPool, QuantizedKVPool
+
+    hkv, d, bs, n = 8, 128, 16, 200
+    quant = cache == "e4m3"
+    nb = 290_000 if quant else 270_000  # x 16 KB of elements
+    pool = (QuantizedKVPool if quant else PagedKVPool)(1, hkv, d, nb, 1, 16, block_size=bs, dtype=torch.bfloat16)
+    assert (nb - 20) * hkv * bs * d > 2**32
+    pool.set_state(np.arange(nb - 13, nb)[::-1][None].copy(), np.array([0]), np.arange(4))
+    pool.block_tables[0, :13] = torch.arange(nb - 1, nb - 14, -1, device="cuda", dtype=torch.int32)
+    pool.seq_lens[0] = n
+    pool._host_lens[0] = n
+    k, v = (torch.randn((1, n, hkv, d), device="cuda").bfloat16() for _ in range(2))
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    pool.append_packed(None, k, v, cu)
+    ks, vs = ([(quantise64(x[0])[0] if quant else x[0].double()).transpose(0, 1)] for x in (k, v))
+    kg, vg = pool.gather()
+    assert torch.equal(kg.view(hkv, n, d).double(), ks[0]) and torch.equal(vg.view(hkv, n, d).double(), vs[0])
+    q = torch.randn((n, 32, d), device="cuda").bfloat16()
+    check(pool.attend_chunk(0, q, cu), q, [0, n], ks, vs, 0, 0, 2.0**-8)
+    check(pool.decode(0, q[:1], window=150, sinks=3), q[:1], [0, 1], ks, vs, 150, 3, 2.0**-8)
+    check(pool.attend_chunk(0, q, cu, force_generic=True), q, [0, n], ks, vs, 0, 0, 2.0**-8)
+    pool.check()
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_decode_that_stores_its_token(cuda_device, cache):
+    """decode(append=) with a window, and over an 8-bit pool; only the first sequences of the pool."""
+    pool, ks, vs = make_pool(torch.bfloat16, [70, 31, 50], 2, 128, 16, 42, cache, spare=4)
+    pool.reserve(1, batch=2)
+    kn, vn = (torch.randn((2, 2, 128), device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn((3, 8, 128), device="cuda").bfloat16()
+    out = pool.decode(0, q, append=(kn, vn), window=40, sinks=1, batch=2)
+    pool.check()
+    assert out.shape == (2, 8, 128)
+    for b in range(2):
+        for hist, x in ((ks, kn), (vs, vn)):
+            val = quantise64(x[b])[0] if cache == "e4m3" else x[b].double()
+            hist[b] = torch.cat([hist[b], val.unsqueeze(1)], 1)
+    check(out, q[:2], [0, 1, 2], ks[:2], vs[:2], 40, 1, 2.0**-8)
+
+
+@pytest.mark.parametrize("single,generic", [(False, False), (True, False), (False, True)])
+def test_a_length_past_the_table(cuda_device, single, generic):
+    pool, _, _ = make_pool(torch.bfloat16, [40], 2, 128, 16, 43)
+    pool.seq_lens[0] = 16 * pool.max_blocks_per_seq + 9
+    q = torch.randn((1, 8, 128), device="cuda").bfloat16()
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    pool.block_tables.fill_(0)
+    if single:
+        pool.decode(0, q, window=30)
+    else:
+        pool.attend_chunk(0, q, cu, force_generic=generic)
+    with pytest.raises(RuntimeError, match="table"):
+        pool.check()
+
+
+def test_generator_graph_on_a_quantised_pool(cuda_device):
+    """BatchedGraphDecoder over a QuantizedKVPool: the captured steps give the ids of eager steps."""
+    import torch.nn as nn
+
+    from snapmind_b200 import PagedGroupedQueryAttention, QuantizedKVPool
+    from snapmind_b200.engine import BatchedGraphDecoder
+
+    class Tiny(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.emb = nn.Embedding(50, 64)
+            self.attn = PagedGroupedQueryAttention(64, 4, 2, head_dim=64)
+            self.head = nn.Linear(64, 50)
+
+        def forward(self, ids, kv_cache, position_ids=None):
+            x = self.emb(ids)
+            return self.head(x + self.attn(x, kv_cache=kv_cache[0], position_ids=position_ids)[0])
+
+    torch.manual_seed(3)
+    model = Tiny().cuda()
+    prompts = torch.randint(0, 50, (3, 19), generator=torch.Generator().manual_seed(0)).cuda()
+    ids = []
+    for use_graph in (False, True):
+        pool = QuantizedKVPool(1, 2, 64, 24, 3, 8, dtype=torch.float32)
+        ids.append(BatchedGraphDecoder(model, pool, 3, use_graph=use_graph).generate(prompts, 12))
+    assert ids[0] == ids[1]
