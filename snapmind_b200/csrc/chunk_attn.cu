@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
   constexpr int kHeld = kCanFetch ? kVecs : 1;
   Smem& S = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  prior_grid_wait();
   plan_block(p, S.plan, reinterpret_cast<int32_t*>(S.q));
-  if (tid == 0) write_piece_info(p, S.plan);
   const float c2 = p.scale * kLog2e;
   const int bs = p.block_size, hd = p.head_dim;
   const bool fetches = kCanFetch && hd == D && ((reinterpret_cast<uintptr_t>(p.k_pool) | reinterpret_cast<uintptr_t>(p.v_pool)) & 15) == 0;
@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
       }
     }
   }
+  if (tid == 0) write_piece_info(p, S.plan);
 }
 
 // Merge of the cut units: block (c, y) works when CTA c holds the first cut inside a
@@ -388,8 +389,8 @@ __device__ __forceinline__ void mul4(float4& a, float f) {
 
 template <typename T>
 __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkParams p) {
-  // launched as a programmatic dependent of the attention kernel: complete and visible after this
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  next_grid_may_launch();  // every block of this grid has started by then
+  prior_grid_wait();
   const int cta = blockIdx.x + 1;
   const int4 h0 = *reinterpret_cast<const int4*>(p.heads + (int64_t)cta * kPieceInts);
   const int4 h1 = *reinterpret_cast<const int4*>(p.heads + (int64_t)cta * kPieceInts + 4);
@@ -512,8 +513,7 @@ int launch_generic(ChunkParams& p, cudaStream_t st) {
   const auto go = [&](auto kernel, size_t smem, bool (&done)[kMaxDevices]) -> int {
     const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem, done);
     if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
-    kernel<<<p.n_ctas, kGenThreads, smem, st>>>(p);
-    return cuda_status(cudaGetLastError(), "paged_chunk launch");
+    return cuda_status(launch_dependent(kernel, dim3(p.n_ctas), kGenThreads, smem, st, p), "paged_chunk launch");
   };
   static bool done[3][kMaxDevices] = {};
   static_assert(sizeof(GenSmem<4>) <= 232448, "shared memory budget");
@@ -532,21 +532,15 @@ static_assert(2 * kRows <= kMaxRows, "two CTAs per SM");
 
 int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st) {
   if (p.n_ctas < 2) return SNAPMIND_OK;
-  cudaLaunchAttribute pdl[1];
-  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  pdl[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
   const int used = p.gw * p.tokens;
-  cfg.gridDim = dim3(p.n_ctas - 1, (used + kMergeWarps * kMergeRows - 1) / (kMergeWarps * kMergeRows));
-  cfg.blockDim = dim3(32 * kMergeWarps);
-  cfg.stream = st;
-  cfg.attrs = pdl;
-  cfg.numAttrs = 1;
+  const dim3 grid(p.n_ctas - 1, (used + kMergeWarps * kMergeRows - 1) / (kMergeWarps * kMergeRows));
+  const auto go = [&](auto kernel) {
+    return cuda_status(launch_dependent(kernel, grid, 32 * kMergeWarps, 0, st, p), "paged_chunk merge");
+  };
   switch (dtype) {
-    case SNAPMIND_DTYPE_F32: return cuda_status(cudaLaunchKernelEx(&cfg, chunk_merge_kernel<float>, p), "paged_chunk merge");
-    case SNAPMIND_DTYPE_BF16:
-      return cuda_status(cudaLaunchKernelEx(&cfg, chunk_merge_kernel<__nv_bfloat16>, p), "paged_chunk merge");
-    default: return cuda_status(cudaLaunchKernelEx(&cfg, chunk_merge_kernel<__half>, p), "paged_chunk merge");
+    case SNAPMIND_DTYPE_F32: return go(chunk_merge_kernel<float>);
+    case SNAPMIND_DTYPE_BF16: return go(chunk_merge_kernel<__nv_bfloat16>);
+    default: return go(chunk_merge_kernel<__half>);
   }
 }
 

@@ -232,8 +232,8 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     tmem_alloc(smem_u32(&C.tmem_base), 512);
     tmem_relinquish();
   }
+  prior_grid_wait();
   plan_block(p, C.plan, reinterpret_cast<int32_t*>(p_s));
-  if (tid == 0) write_piece_info(p, C.plan);
   // rows of Q that no copy fills (128 / gw has a remainder) are zeros, not whatever lay there
   for (uint32_t i = tid; i < 2 * Sh::kTileBytes / 16; i += Ro::kThreads) reinterpret_cast<uint4*>(q_s)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
@@ -682,7 +682,8 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) write_piece_info(p, C.plan);
+  next_grid_may_launch();
   if (warp == Ro::kScores) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -716,8 +717,9 @@ int launch(const ChunkParams& p, cudaStream_t st) {
   static bool done[kMaxDevices] = {};
   const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem_bytes<D, kQuant>(), done);
   if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
-  kernel<<<p.n_ctas, Roles<kQuant>::kThreads, smem_bytes<D, kQuant>(), st>>>(q_map, k_map, v_map, p);
-  return cuda_status(cudaGetLastError(), "paged_chunk launch");
+  return cuda_status(launch_dependent(kernel, dim3(p.n_ctas), Roles<kQuant>::kThreads, smem_bytes<D, kQuant>(), st, q_map,
+                                      k_map, v_map, p),
+                     "paged_chunk launch");
 }
 
 }  // namespace

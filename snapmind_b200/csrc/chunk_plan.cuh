@@ -43,7 +43,7 @@ struct ChunkParams {
   int32_t rows;            // partial rows of a unit in the workspace (>= gw * tokens)
   int32_t key_tile;        // keys of a tile
   int32_t n_ctas;
-  FastDiv by_gw, by_block, by_tile;  // divisions by gw, block_size, key_tile
+  FastDiv by_gw, by_block, by_tile, by_ctas;  // divisions by gw, block_size, key_tile, n_ctas
   void* workspace;
   int32_t* heads;   // workspace: [n_ctas][kPieceInts], see PieceInfo
   float* part_ml;   // workspace: [n_ctas][2][rows][2] maximum (log2 units), sum
@@ -123,12 +123,12 @@ __device__ __forceinline__ int seq_tiles(const ChunkParams& p, int b, int lane) 
   return s;
 }
 
-// a b / c; in 32 bits where they suffice (a 64-bit division takes hundreds of cycles).
-__device__ __forceinline__ long long mul_div(long long a, long long b, int c) {
-  const long long x = a * b;
-  return x < (1ll << 32) ? (long long)((uint32_t)x / (uint32_t)c) : x / c;
+// First tile of a CTA's share, cta total / n; n is n_ctas, or total when that is less.
+__device__ __forceinline__ long long cut(const ChunkParams& p, int cta, long long total) {
+  if (total <= p.n_ctas) return cta;
+  const long long x = cta * total;
+  return x < (1ll << 31) ? p.by_ctas.div((int)x) : x / p.n_ctas;
 }
-__device__ __forceinline__ long long cut(int cta, long long total, int n) { return mul_div(cta, total, n); }
 // The CTA whose share holds tile t: the largest c with cut(c) <= t, which is
 // ((t + 1) n - 1) / total rounded down.
 __device__ __forceinline__ int cta_of(long long t, long long total, int n) {
@@ -150,56 +150,104 @@ __device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* 
     }
   }
   __syncthreads();
-  // sums of contiguous runs of sequences, one run per thread
-  const int run = (p.batch + blockDim.x - 1) / blockDim.x;
-  const int b0 = min(p.batch, tid * run), b1 = min(p.batch, b0 + run);
-  int s = 0;
-  for (int b = b0; b < b1; ++b) s += tiles[b];
-  int incl = s;
+  // The tile line's length, and where this CTA's share begins.  Up to kWarpBatch sequences: every
+  // warp goes over them, 32 a step (no barrier, the last step finds the place); more: one run of
+  // sequences per thread and a scan over the block.
+  constexpr int kWarpBatch = 256;
+  long long t0, t1;
+  if (p.batch <= kWarpBatch) {
+    int sum = 0;
+    for (int b = lane; b < p.batch; b += 32) sum += tiles[b];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const long long total = (long long)sum * per_head;
+    const int n = (int)min((long long)p.n_ctas, total);
+    const bool works = (int)blockIdx.x < n;
+    t0 = works ? cut(p, blockIdx.x, total) : total;
+    t1 = works ? cut(p, blockIdx.x + 1, total) : total;
+    if (warp == 0) {
+      long long before = 0;
+      for (int base = 0; base < p.batch && t0 < t1; base += 32) {
+        const int b = base + lane, u = b < p.batch ? tiles[b] : 0;
+        int x = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        const long long end = before + (long long)x * per_head, at = end - (long long)u * per_head;
+        if (t0 >= at && t0 < end) {
+          S.b = b;
+          S.u = u;
+          S.rem = (int)(t0 - at);
+        }
+        before += (long long)__shfl_sync(0xffffffffu, x, 31) * per_head;
+        if (t0 < before) break;
+      }
+      if (lane == 0) {
+        S.total = total;
+        S.n = n;
+        S.t0 = t0;
+        S.t1 = t1;
+      }
+      __syncwarp();
+    }
+  } else {
+    const int run = (p.batch + blockDim.x - 1) / blockDim.x;
+    const int b0 = min(p.batch, tid * run), b1 = min(p.batch, b0 + run);
+    int s = 0;
+    for (int b = b0; b < b1; ++b) s += tiles[b];
+    int incl = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) S.warp_sum[warp] = incl;
+    __syncthreads();
+    long long before = 0, total = 0;
+    for (int w = 0; w < nw; ++w) {
+      if (w < warp) before += S.warp_sum[w];
+      total += S.warp_sum[w];
+    }
+    before = (before + incl - s) * per_head;
+    total *= per_head;
+    const int n = (int)min((long long)p.n_ctas, total);
+    const bool works = (int)blockIdx.x < n;
+    t0 = works ? cut(p, blockIdx.x, total) : total;
+    t1 = works ? cut(p, blockIdx.x + 1, total) : total;
+    if (tid == 0) {
+      S.total = total;
+      S.n = n;
+      S.t0 = t0;
+      S.t1 = t1;
+    }
+    if (t0 < t1 && t0 >= before && t0 < before + (long long)s * per_head) {
+      long long at = before;
+      int b = b0;
+      while (t0 >= at + (long long)tiles[b] * per_head) at += (long long)tiles[b++] * per_head;
+      S.b = b;
+      S.u = tiles[b];
+      S.rem = (int)(t0 - at);
+    }
+    __syncthreads();
   }
-  if (lane == 31) S.warp_sum[warp] = incl;
-  __syncthreads();
-  long long before = 0, total = 0;
-  for (int w = 0; w < nw; ++w) {
-    if (w < warp) before += S.warp_sum[w];
-    total += S.warp_sum[w];
-  }
-  before = (before + incl - s) * per_head;
-  total *= per_head;
-  const int n = (int)min((long long)p.n_ctas, total);
-  const bool works = (int)blockIdx.x < n;
-  const long long t0 = works ? cut(blockIdx.x, total, n) : total;
-  const long long t1 = works ? cut(blockIdx.x + 1, total, n) : total;
-  if (tid == 0) {
-    S.total = total;
-    S.n = n;
-    S.t0 = t0;
-    S.t1 = t1;
-  }
-  if (t0 < t1 && t0 >= before && t0 < before + (long long)s * per_head) {
-    long long at = before;
-    int b = b0;
-    while (t0 >= at + (long long)tiles[b] * per_head) at += (long long)tiles[b++] * per_head;
-    S.b = b;
-    S.u = tiles[b];
-    S.rem = (int)(t0 - at);
-  }
-  __syncthreads();
   if (warp == 0 && t0 < t1) {
     Piece f;
     f.b = S.b;
-    const int hs = S.rem / S.u;
+    int hs = (int)__fdividef((float)S.rem, (float)S.u);  // off by one at most: S.rem < 2^31, hs small
+    hs -= hs * (long long)S.u > S.rem;
+    hs += (hs + 1) * (long long)S.u <= S.rem;
     int rem = S.rem - hs * S.u;
     f.kvh = hs / p.n_slices;
     f.slice = hs - f.kvh * p.n_slices;
     f.n = chunk_queries(p, f.b, &f.q_first);
     f.len = clamp_len(p, f.b);
     f.i0 = 0;
-    for (int base = 0;; base += 32) {  // 32 runs at a time; ends inside the sequence since rem < u
+    f.n_tiles = S.u;
+    f.tile0 = rem;
+    // 32 runs at a time; ends inside the sequence since rem < u (one query per sequence: one run)
+    for (int base = 0; p.cu_q != nullptr; base += 32) {
       const int i0 = (base + lane) * p.tokens;
       const int t = i0 < f.n ? key_tiles(p, f.len, f.n, i0) : 0;
       int x = t;
@@ -383,6 +431,26 @@ inline cudaError_t kernel_attributes(const void* kernel, size_t smem, bool (&don
   return e;
 }
 
+// The kernels of a call, and calls in a row, are programmatic dependents: a kernel's launch and its
+// set-up overlap the tail of the one before, and it waits for that one to be complete and visible
+// (prior_grid_wait) before it reads or writes anything in global memory.
+__device__ __forceinline__ void prior_grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void next_grid_may_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... A>
+inline cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Workspace regions of n_ctas CTAs: heads, then maxima and sums, then partial outputs.
 inline int64_t plan_workspace(ChunkParams& p, void* workspace, int64_t n_ctas, int64_t rows) {
   const int64_t ml_off = (n_ctas * kPieceInts * 4 + 255) / 256 * 256;
@@ -405,6 +473,7 @@ inline void plan_geometry(ChunkParams& p, int rows, int key_tile, int n_ctas) {
   p.by_gw = FastDiv(p.gw);
   p.by_block = FastDiv(p.block_size);
   p.by_tile = FastDiv(key_tile);
+  p.by_ctas = FastDiv(n_ctas);
   plan_workspace(p, p.workspace, n_ctas, rows);
 }
 

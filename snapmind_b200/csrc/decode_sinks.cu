@@ -141,8 +141,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     S.abort = 0;
     mbar_init_fence();
   }
+  prior_grid_wait();
   plan_block(p, S.plan, reinterpret_cast<int32_t*>(ring));
-  if (tid == 0) write_piece_info(p, S.plan);
   fence_proxy_async_smem();  // the scratch in the ring is done with before copies land there
   __syncthreads();
 
@@ -497,7 +497,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   }
   __syncthreads();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) write_piece_info(p, S.plan);
+  next_grid_may_launch();
 }
 
 template <typename T, bool kQuant>
@@ -517,8 +518,8 @@ int launch(const ChunkParams& p, cudaStream_t st) {
   static bool done[kMaxDevices] = {};
   const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem_bytes<kQuant>(), done);
   if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
-  kernel<<<p.n_ctas, kThreads, smem_bytes<kQuant>(), st>>>(k_map, v_map, p);
-  return cuda_status(cudaGetLastError(), "paged_chunk launch");
+  return cuda_status(launch_dependent(kernel, dim3(p.n_ctas), kThreads, smem_bytes<kQuant>(), st, k_map, v_map, p),
+                     "paged_chunk launch");
 }
 
 }  // namespace
