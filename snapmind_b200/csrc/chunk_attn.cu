@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
       const int r = ty + 16 * i, tok = p.by_gw.div(r), g = r - tok * p.gw;
       if (r >= n_rows || g >= heads) continue;
       const bool whole = c.whole();
-      const float f = !whole ? 1.f : m[i] == -INFINITY ? 0.f : 1.f / l[i];  // sees nothing: zeros
+      const float f = !whole ? 1.f : l[i] == 0.f ? 0.f : 1.f / l[i];  // sees nothing: zeros (a NaN stays one)
       const int64_t slot = part_slot(c) * p.rows + r;
       T* out = reinterpret_cast<T*>(p.out) + (int64_t)(c.q_first + c.i0 + tok) * p.out_stride_tok + (int64_t)(head0 + g) * p.out_stride_head;
       if (!whole && tx == 0) {
@@ -355,7 +355,8 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
 
 // Merge of the cut units: block (c, y) works when CTA c holds the first cut inside a
 // unit, on rows y, y + gridDim.y, ... (in groups of kMergeRows); pieces are CTA c - 1's slot 1, then
-// slot 0 of CTAs c .. last.  M = max m_i, out = sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M).
+// slot 0 of CTAs c .. last.  M = max m_i, out = sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M).  A piece with
+// m = -infinity saw nothing (l = 0, and o may hold anything) or only NaN (l is one, and so is out).
 // The work is a few loads that wait for one another, so what counts is how many are in flight: a
 // warp takes kMergeRows rows of a unit cut into up to 8 pieces at once (one row at a time, the 256-row
 // units of a long chunk took 30 us), or one row of more pieces, 8 of them in flight (one at a
@@ -427,10 +428,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
       const float ref = M == -INFINITY ? 0.f : M;
-      float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - ref), L = ml.y * f;
+      float f = ml.x == -INFINITY ? ml.y : ex2(ml.x - ref), L = ml.y * f;
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-      f *= M == -INFINITY ? 0.f : 1.f / L;  // a row that sees nothing: zeros
+      f *= L == 0.f ? 0.f : 1.f / L;  // a row that sees nothing: zeros
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if (128 * c >= D) break;
@@ -475,7 +476,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
       mb = fmaxf(mb, M);
       const float ref = mb == -INFINITY ? 0.f : mb, old = ex2(M - ref);
       M = mb;
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - ref);
+      const float f = ml.x == -INFINITY ? ml.y : ex2(ml.x - ref);
       float ls = ml.y * f;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
         }
       }
     }
-    const float inv = M == -INFINITY ? 0.f : 1.f / L;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
     mul4(acc[0], inv);
     mul4(acc[1], inv);
     T* out = out_row(r, g);

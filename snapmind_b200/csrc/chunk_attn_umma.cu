@@ -624,8 +624,8 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         if (ok && other_steps > 0) ok = role_wait(C, smem_u32(&C.pv_done[1]), (other_steps - 1) & 1);
         const float2 ml = C.ml[r];
         const float M = fmaxf(m, ml.x);
-        f = m == -INFINITY ? 0.f : ex2(m - M);
-        fx = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+        f = m == -INFINITY ? l : ex2(m - M);  // sees nothing: 0; only NaN: NaN
+        fx = ml.x == -INFINITY ? ml.y : ex2(ml.x - M);
         m = M;
         l = l * f + ml.y * fx;
       }
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         p.part_ml[slot * 2 + 1] = l;
       }
       if (whole) {  // sees nothing: zeros
-        const float inv = m == -INFINITY ? 0.f : 1.f / l;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         f *= inv;
         fx *= inv;
       }

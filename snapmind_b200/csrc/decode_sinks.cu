@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int i = 0; i < kConsumers; ++i) M = fmaxf(M, S.mm[i][h]);
 #pragma unroll
-        for (int i = 0; i < kConsumers; ++i) L += S.mm[i][h] == -INFINITY ? 0.f : S.ml[i][h] * ex2(S.mm[i][h] - M);
+        for (int i = 0; i < kConsumers; ++i) L += S.mm[i][h] == -INFINITY ? S.ml[i][h] : S.ml[i][h] * ex2(S.mm[i][h] - M);  // 0, or NaN
 #pragma unroll
         for (int i = 0; i < 8; i += 4) {
           const float4 a = *reinterpret_cast<const float4*>(&S.mo[0][h][d + i]);
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           x[i + 3] = a.w + b.w;
         }
         if (c.whole()) {
-          const float inv = M == -INFINITY ? 0.f : 1.f / L;  // nothing seen: zeros
+          const float inv = L == 0.f ? 0.f : 1.f / L;  // nothing seen: zeros
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] *= inv;
           T* out = reinterpret_cast<T*>(p.out) + (int64_t)c.q_first * p.out_stride_tok + (int64_t)(head0 + h) * p.out_stride_head + d;

@@ -663,3 +663,45 @@ def test_generator_graph_on_a_quantised_pool(cuda_device):
         pool = QuantizedKVPool(1, 2, 64, 24, 3, 8, dtype=torch.float32)
         ids.append(BatchedGraphDecoder(model, pool, 3, use_graph=use_graph).generate(prompts, 12))
     assert ids[0] == ids[1]
+
+
+@pytest.mark.parametrize("cache,d,single,generic", KERNELS)
+def test_nan_is_not_hidden(cuda_device, cache, d, single, generic):
+    """A NaN in a query makes that (row, head) NaN, one in a key every row and head that sees it, on
+    one CTA or on many; the others keep their values."""
+    lens, new = ([5000, 40, 0], [1, 1, 1]) if single else ([5000, 40, 0], [3, 20, 0])
+    pool, ks, vs = make_pool(torch.bfloat16, lens, 2, d, 16, 44, cache)
+    cu = [0, *itertools.accumulate(new)]
+    cud = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    q = torch.randn((cu[-1], 8, d), device="cuda").bfloat16()
+
+    def run(x, window):
+        if single:
+            return pool.decode(0, x, window=window, sinks=min(window, 2), force_generic=generic)
+        return pool.attend_chunk(0, x, cud, window=window, sinks=min(window, 2), force_generic=generic)
+
+    # one (row, head) whose every score is NaN
+    for window in (64, 4096) if single and cache == "same" else (0, 64):
+        clean = run(q, window)
+        bad = q.clone()
+        bad[0, 3] = float("nan")
+        bad[cu[1], 6, 5] = float("nan")
+        out = run(bad, window)
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        hit[0, 3] = hit[cu[1], 6] = True
+        assert torch.isnan(out[hit]).all()
+        # each within half a step of the output's type and of the weights' of sums of at most max |v|
+        assert (out - clean)[~hit].abs().max() <= 4 * 2.0**-8 * float(max(v.abs().max() for v in vs[:2]))
+    # the newest key of sequence 0, kv head 1: only its last query sees it
+    slot = lens[0] - 1
+    block = int(pool.block_tables[0, slot // 16])
+    if cache == "e4m3":
+        pool.k.view(torch.uint8)[0, block, 1, slot % 16, 7] = 0x7F
+    else:
+        pool.k[0, block, 1, slot % 16, 7] = float("nan")
+    out = run(q, 64)
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[cu[1] - 1, 4:] = True
+    assert torch.isnan(out[hit]).all()
+    assert torch.isfinite(out[~hit]).all()
+    pool.check()
