@@ -570,6 +570,8 @@ SNAPMIND_API int snapmind_kv_gather_quant(const void *k_pool, const void *v_pool
  * only p > its own - window or p < sinks.  A query that sees nothing gives zeros.
  * cu_q NULL: one query per sequence (a decode step; total_q = batch).
  * q and out are [token][head][dim] with element strides (dim contiguous) in `dtype`;
+ * A length past the table row sets SNAPMIND_DEVERR_TABLE; the positions that the row has no
+ * entry for do not count.
  * query head h reads kv head h / (n_q_heads / n_kv_heads).  pool_dtype is `dtype`, or
  * SNAPMIND_DTYPE_E4M3 with `scales` as snapmind_kv_append_chunk writes them (of the
  * same layer as k_pool and v_pool; NULL otherwise).  Softmax statistics and sums are

@@ -134,9 +134,9 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
         if (pos < kr.win_lo && !in_sink) {
           pos = INT32_MAX;  // in a block that is read, before every window
         } else {
-          const int32_t phys = j < p.table_width ? p.tables[(int64_t)c.b * p.table_stride + j] : -1;
+          const int32_t phys = p.tables[(int64_t)c.b * p.table_stride + j];
           if (phys < 0 || phys >= p.num_blocks)
-            flag_error(p.err, j < p.table_width ? SNAPMIND_DEVERR_BLOCK_ID : SNAPMIND_DEVERR_TABLE);
+            flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
           else
             row = ((int64_t)phys * p.n_kv_heads + c.kvh) * bs + (pos - j * bs);
         }
@@ -593,7 +593,6 @@ int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stri
   p.scales = static_cast<const uint8_t*>(scales);
   p.tables = block_tables;
   p.table_stride = table_stride_seq;
-  p.table_width = table_width;
   p.seq_lens = seq_lens;
   p.cu_q = cu_q;
   p.out = out;
@@ -610,6 +609,8 @@ int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stri
   p.num_blocks = num_blocks;
   p.window = window < (1 << 30) ? window : (1 << 30);  // positions stay below 2^30
   p.sinks = sinks < (1 << 30) ? sinks : (1 << 30);
+  const int64_t room = (int64_t)table_width * block_size;
+  p.max_len = room < (1 << 30) ? (int32_t)room : (1 << 30);
   p.err = err_word;
   const int64_t need = snapmind_paged_gqa_chunk_workspace_bytes(head_dim);
   SNAPMIND_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
@@ -627,8 +628,8 @@ int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stri
     if (rc != SNAPMIND_ERR_UNSUPPORTED) return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
   }
   const int ctas = num_sms() * (head_dim <= 64 ? 2 : 1);
-  plan_geometry(p, kRows, kKeys, ctas);
-  int rc;
+  int rc = plan_geometry(p, kRows, kRows, kKeys, ctas);
+  if (rc != SNAPMIND_OK) return rc;
   switch (dtype) {
     case SNAPMIND_DTYPE_F32: rc = quant ? launch_generic<float, uint8_t>(p, st) : launch_generic<float, float>(p, st); break;
     case SNAPMIND_DTYPE_BF16:

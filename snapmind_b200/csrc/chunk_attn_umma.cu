@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       const EdgeTiles edge(p, kr);
       const int qpos = kr.pos0 + min(tok, i1 - c.i0 - 1);
       // on the virtual axis the row sees [v_lo, v_hi) and [0, v_s)
-      const int v_hi = max(0, qpos + 1 - kr.shift);
+      const int v_hi = min(max(0, qpos + 1 - kr.shift), kr.v_len);
       const int v_lo = p.window > 0 ? max(0, qpos - p.window + 1) - kr.shift : 0;
       const int v_s = p.window > 0 ? min(p.sinks, v_hi) : 0;
       const uint32_t step0 = step;
@@ -741,12 +741,8 @@ bool chunk_umma_supported(const ChunkParams& p, int dtype, int pool_dtype) {
 }
 
 int launch_chunk_umma(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st) {
-  plan_geometry(p, 2 * kTileM, kKeys, num_sms());
-  // two tiles of whole tokens: a slice has at most 128 heads
-  p.gw = p.group < kTileM ? p.group : kTileM;
-  p.n_slices = (p.group + p.gw - 1) / p.gw;
-  p.tokens = 2 * (kTileM / p.gw);
-  p.by_gw = FastDiv(p.gw);
+  const int rc = plan_geometry(p, 2 * kTileM, kTileM, kKeys, num_sms());
+  if (rc != SNAPMIND_OK) return rc;
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
   const auto go = [&](auto t) -> int {
     using T = decltype(t);

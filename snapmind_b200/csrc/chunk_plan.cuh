@@ -30,7 +30,6 @@ struct ChunkParams {
   const uint8_t* scales;  // e4m3 pools: [block][head][2][slot] exponents + 127 (else NULL)
   const int32_t* tables;
   int64_t table_stride;
-  int32_t table_width;
   const int32_t* seq_lens;
   const int32_t* cu_q;  // [batch + 1] first query row of every sequence; NULL: one each
   void* out;
@@ -38,6 +37,7 @@ struct ChunkParams {
   float scale;
   int32_t batch, total_q, n_q_heads, n_kv_heads, group, head_dim, block_size, num_blocks;
   int32_t window, sinks;   // window 0: none
+  int32_t max_len;         // positions that a table row has room for
   int32_t gw, n_slices;    // query heads of a slice, slices of a group
   int32_t tokens;          // query tokens of a unit
   int32_t rows;            // partial rows of a unit in the workspace (>= gw * tokens)
@@ -68,7 +68,7 @@ __device__ __forceinline__ int chunk_queries(const ChunkParams& p, int b, int* f
 // The keys that the query tokens [i0, i1) of n new ones see in a cache of len tokens.
 struct KeyRange {
   int pos0;    // position of token i0
-  int end;     // positions >= end are seen by none
+  int end;     // positions >= end are seen by none (or have no entry in the table row)
   int win_lo;  // first position inside token i0's window
   int v_sink, shift, v_len;
   __device__ __forceinline__ int position(int v) const { return v + (v >= v_sink ? shift : 0); }
@@ -76,7 +76,7 @@ struct KeyRange {
 __device__ __forceinline__ KeyRange key_range(const ChunkParams& p, int len, int n, int i0, int i1) {
   KeyRange r;
   r.pos0 = len - n + i0;
-  r.end = max(0, min(len, len - n + i1));
+  r.end = max(0, min(min(len, p.max_len), len - n + i1));
   r.win_lo = p.window > 0 ? max(0, r.pos0 - p.window + 1) : 0;
   const int bs = p.block_size;
   const int n_sink = p.window > 0 ? p.by_block.div(min(p.sinks, r.end) + bs - 1) : 0;
@@ -104,18 +104,25 @@ struct PlanShared {
   int32_t warp_sum[32];
   long long total, t0, t1;
   int32_t n;            // CTAs with work: min(n_ctas, total)
-  int32_t b, rem;       // sequence of tile t0, tiles before it in the sequence
+  long long rem;        // tiles of the sequence of tile t0 that come before it
+  int32_t b;            // that sequence
   int32_t u;            // tiles of one (kv head, slice) of that sequence
   Piece first;
 };
 
 __device__ __forceinline__ int clamp_len(const ChunkParams& p, int b) { return max(0, p.seq_lens[b]); }
 
+// A length past the table row: its positions there are left out, and flagged (once, by CTA 0).
+__device__ __forceinline__ void check_len(const ChunkParams& p, int len) {
+  if (len > p.max_len && blockIdx.x == 0) flag_error(p.err, SNAPMIND_DEVERR_TABLE);
+}
+
 // Tiles of one (kv head, slice) of sequence b, summed by a full warp.
 __device__ __forceinline__ int seq_tiles(const ChunkParams& p, int b, int lane) {
   int first;
   const int n = chunk_queries(p, b, &first);
   const int len = clamp_len(p, b);
+  if (n > 0 && lane == 0) check_len(p, len);
   int s = 0;
   for (int i0 = lane * p.tokens; i0 < n; i0 += 32 * p.tokens) s += key_tiles(p, len, n, i0);
 #pragma unroll
@@ -142,7 +149,11 @@ __device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
   const int per_head = p.n_kv_heads * p.n_slices;
   if (p.cu_q == nullptr) {
-    for (int b = tid; b < p.batch; b += blockDim.x) tiles[b] = key_tiles(p, clamp_len(p, b), 1, 0);
+    for (int b = tid; b < p.batch; b += blockDim.x) {
+      const int len = clamp_len(p, b);
+      check_len(p, len);
+      tiles[b] = key_tiles(p, len, 1, 0);
+    }
   } else {
     for (int b = warp; b < p.batch; b += nw) {
       const int s = seq_tiles(p, b, lane);
@@ -179,7 +190,7 @@ __device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* 
         if (t0 >= at && t0 < end) {
           S.b = b;
           S.u = u;
-          S.rem = (int)(t0 - at);
+          S.rem = t0 - at;
         }
         before += (long long)__shfl_sync(0xffffffffu, x, 31) * per_head;
         if (t0 < before) break;
@@ -228,17 +239,17 @@ __device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* 
       while (t0 >= at + (long long)tiles[b] * per_head) at += (long long)tiles[b++] * per_head;
       S.b = b;
       S.u = tiles[b];
-      S.rem = (int)(t0 - at);
+      S.rem = t0 - at;
     }
     __syncthreads();
   }
   if (warp == 0 && t0 < t1) {
     Piece f;
     f.b = S.b;
-    int hs = (int)__fdividef((float)S.rem, (float)S.u);  // off by one at most: S.rem < 2^31, hs small
+    int hs = (int)__fdividef((float)S.rem, (float)S.u);  // off by one at most: hs is small
     hs -= hs * (long long)S.u > S.rem;
     hs += (hs + 1) * (long long)S.u <= S.rem;
-    int rem = S.rem - hs * S.u;
+    int rem = (int)(S.rem - hs * (long long)S.u);
     f.kvh = hs / p.n_slices;
     f.slice = hs - f.kvh * p.n_slices;
     f.n = chunk_queries(p, f.b, &f.q_first);
@@ -336,13 +347,12 @@ struct TileRows {
     const int v = (first_tile + (lane >> log_parts)) * p.key_tile + (lane & (parts - 1)) * box;
     return v < kr.v_len ? kr.position(v) : -1;
   }
-  // Table entry of the lane's part; kNoKey: no key there, kNoEntry: past the table's row.
-  static constexpr int32_t kNoKey = INT32_MIN, kNoEntry = INT32_MIN + 1;
+  // Table entry of the lane's part; kNoKey: no key there.
+  static constexpr int32_t kNoKey = INT32_MIN;
   __device__ __forceinline__ int32_t entry(int first_tile) const {
     const int pos = position(first_tile);
     if (pos < 0 || first_tile + (lane >> log_parts) >= end) return kNoKey;
-    const int lb = p.by_block.div(pos);
-    return lb < p.table_width ? table[lb] : kNoEntry;
+    return table[p.by_block.div(pos)];
   }
   // Makes `tile` part of the current batch (tiles are asked for in ascending order).
   __device__ __forceinline__ void advance(int tile) {
@@ -354,7 +364,7 @@ struct TileRows {
       const int pos = position(first);
       rows = (e * p.n_kv_heads + kvh) * p.block_size + (pos - p.by_block.div(pos) * p.block_size);
     } else if (e != kNoKey) {
-      flag_error(p.err, e == kNoEntry ? SNAPMIND_DEVERR_TABLE : SNAPMIND_DEVERR_BLOCK_ID);
+      flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
     }
     next = entry(first + (32 >> log_parts));
   }
@@ -462,12 +472,17 @@ inline int64_t plan_workspace(ChunkParams& p, void* workspace, int64_t n_ctas, i
   return o_off + n_ctas * 2 * rows * p.head_dim * 4;
 }
 
-// Unit geometry for kernels of `rows` query rows, `key_tile` keys and `n_ctas` CTAs.
-inline void plan_geometry(ChunkParams& p, int rows, int key_tile, int n_ctas) {
-  p.gw = p.group < rows ? p.group : rows;
+// Unit geometry for kernels of `rows` query rows in tiles of `tile_rows` (whole tokens each),
+// `key_tile` keys and `n_ctas` CTAs.
+inline int plan_geometry(ChunkParams& p, int rows, int tile_rows, int key_tile, int n_ctas) {
+  p.gw = p.group < tile_rows ? p.group : tile_rows;
   p.n_slices = (p.group + p.gw - 1) / p.gw;
-  p.tokens = rows / p.gw;
+  p.tokens = rows / tile_rows * (tile_rows / p.gw);
   p.rows = rows;
+  // the plan counts the tiles of one kv head in 32 bits
+  const int64_t units = p.cu_q == nullptr ? p.batch : (int64_t)p.total_q / p.tokens + p.batch;
+  SNAPMIND_CHECK_ARG(units * (p.max_len / key_tile + 2) < (int64_t)1 << 31,
+                     "paged_chunk: %d new tokens over tables of %d positions are too many for one call", p.total_q, p.max_len);
   p.key_tile = key_tile;
   p.n_ctas = n_ctas;
   p.by_gw = FastDiv(p.gw);
@@ -475,6 +490,7 @@ inline void plan_geometry(ChunkParams& p, int rows, int key_tile, int n_ctas) {
   p.by_tile = FastDiv(key_tile);
   p.by_ctas = FastDiv(n_ctas);
   plan_workspace(p, p.workspace, n_ctas, rows);
+  return SNAPMIND_OK;
 }
 
 }  // namespace snapmind

@@ -541,7 +541,8 @@ bool decode_sinks_supported(const ChunkParams& p, int dtype, int pool_dtype) {
 }
 
 int launch_decode_sinks(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st) {
-  plan_geometry(p, kHeads, kTile, 2 * num_sms());
+  const int rc = plan_geometry(p, kHeads, kHeads, kTile, 2 * num_sms());
+  if (rc != SNAPMIND_OK) return rc;
   p.tokens = 1;
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
   if (dtype == SNAPMIND_DTYPE_BF16)

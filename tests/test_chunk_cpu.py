@@ -36,6 +36,16 @@ def test_chunk_refusals(kw, word):
     assert word in lib.last_error()
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up pointers")
+@pytest.mark.parametrize("total,width", [(1 << 30, 1 << 16), (1 << 22, 1 << 22)])
+def test_chunk_of_too_much(total, width):
+    """The tiles of one kv head are counted in 32 bits: more than that is refused."""
+    x = ctypes.c_void_p(256)
+    rc = lib.load().snapmind_paged_gqa_chunk(x, 512, 64, 0, x, x, None, 0, x, width, width, x, x, x, 512, 64, 1.0, 1,
+                                             total, 8, 1, 64, 16, 4, 0, 0, 0, x, 1 << 60, None, None)
+    assert rc == lib.ERR_BAD_ARGUMENT and "too many" in lib.last_error()
+
+
 def test_chunk_of_nothing():
     assert chunk(batch=0, total=0) == lib.OK
     assert chunk(total=0, cu=ctypes.c_void_p(16)) == lib.OK

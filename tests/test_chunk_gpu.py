@@ -705,3 +705,26 @@ def test_nan_is_not_hidden(cuda_device, cache, d, single, generic):
     assert torch.isnan(out[hit]).all()
     assert torch.isfinite(out[~hit]).all()
     pool.check()
+
+
+@pytest.mark.parametrize("cache,d,single,generic", KERNELS)
+def test_positions_past_the_table_do_not_count(cuda_device, cache, d, single, generic):
+    """A length of 89 over a table row of 80 positions: the newest tokens see those 80 (under a
+    window of 30, the ones of them within it), and the pool's error word tells."""
+    pool, ks, vs = make_pool(torch.bfloat16, [80], 2, d, 16, 45, cache)
+    row = pool.block_tables[:, :5].contiguous()
+    pool.block_tables, pool.max_blocks_per_seq = row, 5
+    pool.seq_lens[0] = 89
+    t = 1 if single else 3
+    q = torch.randn((t, 8, d), device="cuda").bfloat16()
+    cu = torch.tensor([0, t], dtype=torch.int32, device="cuda")
+    for window in (30,) if single and cache == "same" else (0, 30):
+        if single:
+            out = pool.decode(0, q, window=window, force_generic=generic)
+        else:
+            out = pool.attend_chunk(0, q, cu, window=window, force_generic=generic)
+        for i in range(t):
+            lo = max(0, 89 - t + i - window + 1) if window else 0
+            check(out[i:i + 1], q[i:i + 1], [0, 1], [ks[0][:, lo:]], [vs[0][:, lo:]], 0, 0, 2.0**-8)
+        with pytest.raises(RuntimeError, match="table"):
+            pool.check()
