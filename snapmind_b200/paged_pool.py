@@ -111,19 +111,21 @@ class PagedKVPool(BlockPool):
     def _append_chunk(self, base, k_new, v_new, axes, seq_axis, cu, n_layers, batch, n_tokens, total, starts, start0):
         """``axes``: where the layer, head and token axes are; ``seq_axis``: the sequence axis or None."""
         _lib.require_same("append", self.block_tables, k_new, v_new)
-        if k_new.shape != v_new.shape or k_new.dtype != v_new.dtype:
+        shape = k_new.shape
+        if shape != v_new.shape or k_new.dtype != v_new.dtype:
             raise ValueError("append: k and v rows differ in shape or dtype")
-        if k_new.dim() < 4 or k_new.shape[axes[1]] != self.n_kv_heads or k_new.shape[-1] != self.head_dim:
-            raise ValueError(f"expected {self.n_kv_heads} heads of {self.head_dim}, got {tuple(k_new.shape)}")
+        if len(shape) < 4 or shape[axes[1]] != self.n_kv_heads or shape[-1] != self.head_dim:
+            raise ValueError(f"expected {self.n_kv_heads} heads of {self.head_dim}, got {tuple(shape)}")
         if not 0 <= base <= self.n_layers - n_layers:
             raise ValueError(f"append: layers {base} .. {base + n_layers - 1} of a pool of {self.n_layers}")
         if batch > self.max_seqs or batch < 0:
             raise ValueError(f"append: {batch} sequences, the pool holds {self.max_seqs}")
         if cu is not None:
             _lib.require_offsets("append", cu, self.block_tables)
-        if k_new.stride() != v_new.stride() or k_new.stride(-1) != 1:
-            k_new, v_new = k_new.contiguous(), v_new.contiguous()
         st = k_new.stride()
+        if st != v_new.stride() or st[-1] != 1:
+            k_new, v_new = k_new.contiguous(), v_new.contiguous()
+            st = k_new.stride()
         row = self.layer_stride * self.k.element_size()
         scales = self.scales.data_ptr() + base * self.scale_layer_stride if self.quantised else None
         with self._on_device():
@@ -135,7 +137,8 @@ class PagedKVPool(BlockPool):
                 starts, start0, None if cu is None else cu.data_ptr(), n_layers, batch, n_tokens, total,
                 self.n_kv_heads, self.head_dim, self.block_size, self.num_blocks, self.err.data_ptr(), _lib.raw_stream(self._index),
             )  # fmt: skip
-        _lib.check(status, f"{type(self).__name__}.append")
+        if status:
+            _lib.check(status, f"{type(self).__name__}.append")
 
     # ----------------------------------------------------------------- reads
     def attend_chunk(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor, out: torch.Tensor | None = None,
@@ -165,12 +168,17 @@ class PagedKVPool(BlockPool):
             raise ValueError(f"layer {layer} of a pool of {self.n_layers}")
         if cu is None and total > self.max_seqs:
             raise ValueError(f"decode: {total} sequences, the pool holds {self.max_seqs}")
-        if q.stride(-1) != 1:
+        q_st = q.stride()
+        if q_st[2] != 1:
             q = q.contiguous()
+            q_st = q.stride()
         if out is None:
-            out = torch.empty((total, n_q, d), dtype=self.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != self.dtype or out.stride(-1) != 1:
-            raise ValueError("out must have q's shape and dtype, head dim contiguous")
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            o_st = out.stride()
+        else:
+            o_st = out.stride()
+            if out.shape != q.shape or out.dtype != self.dtype or o_st[2] != 1:
+                raise ValueError("out must have q's shape and dtype, head dim contiguous")
         _lib.require_same("attend", self.block_tables, q, out)
         lib = _lib.load()
         # a workspace of its own for every call: calls on several streams, or in several
@@ -181,15 +189,16 @@ class PagedKVPool(BlockPool):
         scales = self.scales.data_ptr() + layer * self.scale_layer_stride if self.quantised else None
         with self._on_device():
             status = lib.snapmind_paged_gqa_chunk(
-                q.data_ptr(), q.stride(0), q.stride(1), self._dcode, self.k.data_ptr() + step,
+                q.data_ptr(), q_st[0], q_st[1], self._dcode, self.k.data_ptr() + step,
                 self.v.data_ptr() + step, scales, self._pool_code, self.block_tables.data_ptr(),
                 self.max_blocks_per_seq, self.max_blocks_per_seq, self.seq_lens.data_ptr(),
-                None if cu is None else cu.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+                None if cu is None else cu.data_ptr(), out.data_ptr(), o_st[0], o_st[1],
                 d ** -0.5 if scale is None else scale, total if cu is None else cu.shape[0] - 1, total, n_q,
                 self.n_kv_heads, d, self.block_size, self.num_blocks, window, sinks, flags, ws.data_ptr(), need,
                 self.err.data_ptr(), _lib.raw_stream(self._index),
             )  # fmt: skip
-        _lib.check(status, f"{type(self).__name__}.attend")
+        if status:
+            _lib.check(status, f"{type(self).__name__}.attend")
         return out
 
     def gather(self, batch: int | None = None, layers: range | None = None, out=None):

@@ -31,6 +31,7 @@ class QuantizedKVPool(PagedKVPool):
         self.v = torch.empty(shape, dtype=torch.float8_e4m3fn, device=self.device)
         self.scales = torch.empty((n_layers, num_blocks, heads, 2, bs), dtype=torch.uint8, device=self.device)
         self.scale_layer_stride = num_blocks * heads * 2 * bs
+        self._values = torch.empty(0, dtype=self.dtype, device=self.device)  # of the type that is read back
 
     def append(self, layer: int | None, k_new: torch.Tensor, v_new: torch.Tensor, slot_starts=None,
                slot_start0: int | None = None) -> None:
@@ -54,7 +55,7 @@ class QuantizedKVPool(PagedKVPool):
         total = int(self._host_lens[:batch].sum())
         per_layer = total * self.n_kv_heads * self.head_dim
         if out is None:
-            k_out, v_out = torch.empty((2, len(layers), per_layer), dtype=self.dtype, device=self.device).unbind(0)
+            k_out, v_out = self._values.new_empty((len(layers), per_layer)), self._values.new_empty((len(layers), per_layer))
         else:
             k_out, v_out = out
             for t in (k_out, v_out):
@@ -76,7 +77,8 @@ class QuantizedKVPool(PagedKVPool):
                 self.seq_lens.data_ptr(), len(layers), batch, self.n_kv_heads, self.head_dim, self.block_size,
                 self.num_blocks, self.err.data_ptr(), _lib.raw_stream(self._index),
             )  # fmt: skip
-        _lib.check(status, "QuantizedKVPool.gather")
+        if status:
+            _lib.check(status, "QuantizedKVPool.gather")
         return k_out, v_out
 
     def decode(self, layer: int, q: torch.Tensor, out: torch.Tensor | None = None, scale: float | None = None,
