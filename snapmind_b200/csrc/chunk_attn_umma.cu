@@ -12,11 +12,11 @@
 //   warps 0-3, 4-7  softmax of tile 0 / 1: thread = row = TMEM lane; they write P to shared memory,
 //                   and write out the finished rows
 //   warp 8          loads Q (one copy per tile and 64 columns: 128 threads fetching rows took 14000
-//                   cycles a unit), issues the MMAs of the scores, and another warp those of P V: a wait takes some
-//                   200 cycles next to operand reads that fill shared memory's bandwidth, and the two
-//                   streams cover each other's
-//   two more        stage K and V by TMA; over 8-bit caches as they are, and four warps more turn
-//                   the rows into 16-bit stages
+//                   cycles a unit), issues the MMAs of the scores
+//   warps 9, 10     stage K and V by TMA
+//   warp 11         issues the MMAs of P V: a wait takes some 200 cycles next to operand reads that fill
+//                   shared memory's bandwidth, and the two streams cover each other's
+//   warps 12-15     8-bit caches only: turn the staged rows into 16-bit stages
 // P goes through shared memory, not through TMEM as an A operand: a kernel of this library that
 // read A from TMEM ended in a launch failure whose cause was not found.
 //   TMEM: S of tile 0 / 1 at columns 0 / 128, O at 256 / 256 + head_dim.
@@ -28,6 +28,12 @@
 //   order, so a barrier's parity always tells the phase that is meant.
 // Every wait is bounded and ends early once another role gave up; TMEM is released on
 // every path.
+// What bounds it: both operands of every product come from shared memory, 4 x 64 KB for a step of
+// 2 x 128 x 128 scores (3072 cycles; measured 3200 to 3300).  2048 new tokens behind
+// 30720 cached ones, 32 heads over 8 of 128: 920 us, 1160 TFLOP/s.  Short units add 20000 cycles at the start of a CTA and 12000 a piece
+// (a mixed step 172 us, 772 TFLOP/s).  Over 8-bit rows the converting warps add 48 KB a tile to the same
+// traffic: 2700 cycles a tile, 2000 of them without any conversion, 484 TFLOP/s; fewer
+// instructions, rows fetched ahead and conversions by bit operations did not help.
 #include <cuda.h>
 #include <cuda_fp8.h>
 
@@ -245,226 +251,226 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
   PieceWalk w;
   bool on = w.start(C.plan);
   if (warp >= Ro::kScores) {
-  regs_dec<Ro::kOther>();
-  if (kQuant && warp >= Ro::kConvertWarp) {
-    // ------------------------------------------------------------------ e4m3 rows -> 16-bit stages
-    // In the order in which the products need them: the first K tiles (1, split 2), then K(j + ahead),
-    // while there is one, and V(j).  D / 16 threads share a row, 16 codes each.
-    constexpr int kLanes = D / 16, kRowsPass = kConvert / kLanes;
-    const int ct = tid - Ro::kConvertWarp * 32, ch = ct % kLanes, r0 = ct / kLanes;
-    const uint32_t c0 = (ch % 4) * 2;
-    const bool swap = ch >= 4;
-    uint32_t tiles = 0;
-    bool ok = true;
-    for (; on && ok; on = w.next(p)) {
-      const Piece& c = w.c;
-      const int i1 = min(c.n, c.i0 + p.tokens), n = c.tile1 - c.tile0;
-      const EdgeTiles edge(p, key_range(p, c.len, c.n, c.i0, i1));
-      const int ahead = i1 - c.i0 <= p.tokens / 2 ? 2 : 1, lead = min(n, ahead);
-      for (int i = 0; i < 2 * n; ++i) {
-        const int x = i - lead;
-        const int kv = x < 0 ? 0 : (x < 2 * (n - lead) ? x & 1 : 1);
-        const int j = x < 0 ? i : (x < 2 * (n - lead) ? x / 2 + (kv ? 0 : ahead) : x - (n - lead));
-        const uint32_t num = tiles + j;
-        const int st = Sh::stage(kv, num);
-        ok = role_wait(C, smem_u32(&C.raw_full[kv]), num & 1) &&
-             role_wait(C, smem_u32(&C.empty[kv][st]), Sh::parity(kv, num) ^ 1);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        const uint8_t* raw = base + Sh::kRaw + kv * Sh::kRawBytes + ch * 16;
-        uint8_t* dst = base + Sh::at(kv, num) + (ch / 4) * 1024;
-        const int v0 = (c.tile0 + j) * kKeys;
-        const bool edges = edge(c.tile0 + j);
+    regs_dec<Ro::kOther>();
+    if (kQuant && warp >= Ro::kConvertWarp) {
+      // ------------------------------------------------------------------ e4m3 rows -> 16-bit stages
+      // In the order in which the products need them: the first K tiles (1, split 2), then K(j + ahead),
+      // while there is one, and V(j).  D / 16 threads share a row, 16 codes each.
+      constexpr int kLanes = D / 16, kRowsPass = kConvert / kLanes;
+      const int ct = tid - Ro::kConvertWarp * 32, ch = ct % kLanes, r0 = ct / kLanes;
+      const uint32_t c0 = (ch % 4) * 2;
+      const bool swap = ch >= 4;
+      uint32_t tiles = 0;
+      bool ok = true;
+      for (; on && ok; on = w.next(p)) {
+        const Piece& c = w.c;
+        const int i1 = min(c.n, c.i0 + p.tokens), n = c.tile1 - c.tile0;
+        const EdgeTiles edge(p, key_range(p, c.len, c.n, c.i0, i1));
+        const int ahead = i1 - c.i0 <= p.tokens / 2 ? 2 : 1, lead = min(n, ahead);
+        for (int i = 0; i < 2 * n; ++i) {
+          const int x = i - lead;
+          const int kv = x < 0 ? 0 : (x < 2 * (n - lead) ? x & 1 : 1);
+          const int j = x < 0 ? i : (x < 2 * (n - lead) ? x / 2 + (kv ? 0 : ahead) : x - (n - lead));
+          const uint32_t num = tiles + j;
+          const int st = Sh::stage(kv, num);
+          ok = role_wait(C, smem_u32(&C.raw_full[kv]), num & 1) &&
+               role_wait(C, smem_u32(&C.empty[kv][st]), Sh::parity(kv, num) ^ 1);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          const uint8_t* raw = base + Sh::kRaw + kv * Sh::kRawBytes + ch * 16;
+          uint8_t* dst = base + Sh::at(kv, num) + (ch / 4) * 1024;
+          const int v0 = (c.tile0 + j) * kKeys;
+          const bool edges = edge(c.tile0 + j);
 #pragma unroll 1
-        for (int r = r0; r < 128; r += kRowsPass) {
-          uint4 codes = *reinterpret_cast<const uint4*>(raw + r * D);
-          uint8_t byte = C.scales[kv][r];
-          if (edges && edge.unseen(v0 + r)) {  // seen by no query of the unit: zeros, whatever lies there
-            codes = make_uint4(0, 0, 0, 0);
-            byte = 127;
+          for (int r = r0; r < 128; r += kRowsPass) {
+            uint4 codes = *reinterpret_cast<const uint4*>(raw + r * D);
+            uint8_t byte = C.scales[kv][r];
+            if (edges && edge.unseen(v0 + r)) {  // seen by no query of the unit: zeros, whatever lies there
+              codes = make_uint4(0, 0, 0, 0);
+              byte = 127;
+            }
+            uint4 lo, hi;
+            dequant16<T>(codes, byte, lo, hi);
+            uint8_t* row = dst + (r >> 3) * Sh::kGroup + (r & 7) * 128;
+            const uint32_t sw = r & 7;
+            // lanes of the two 64-element halves write opposite pieces: no bank is hit twice
+            *reinterpret_cast<uint4*>(row + ((c0 + swap) ^ sw) * 16) = swap ? hi : lo;
+            *reinterpret_cast<uint4*>(row + ((c0 + !swap) ^ sw) * 16) = swap ? lo : hi;
           }
-          uint4 lo, hi;
-          dequant16<T>(codes, byte, lo, hi);
-          uint8_t* row = dst + (r >> 3) * Sh::kGroup + (r & 7) * 128;
-          const uint32_t sw = r & 7;
-          // lanes of the two 64-element halves write opposite pieces: no bank is hit twice
-          *reinterpret_cast<uint4*>(row + ((c0 + swap) ^ sw) * 16) = swap ? hi : lo;
-          *reinterpret_cast<uint4*>(row + ((c0 + !swap) ^ sw) * 16) = swap ? lo : hi;
+          mbar_arrive(smem_u32(&C.raw_empty[kv]));
+          fence_proxy_async_smem();
+          mbar_arrive(smem_u32(&C.full[kv][st]));
         }
-        mbar_arrive(smem_u32(&C.raw_empty[kv]));
-        fence_proxy_async_smem();
-        mbar_arrive(smem_u32(&C.full[kv][st]));
+        tiles += n;
       }
-      tiles += n;
-    }
-    if (!ok && lane == 0) give_up(C, p.err);
-  } else if (warp == Ro::kLoad || warp == Ro::kLoad + 1) {
-    // ------------------------------------------------------------------ K and V copies
-    const int kv = warp - Ro::kLoad;
-    const uint32_t leader = elect_one_sync();
-    const CUtensorMap* map = kv == 0 ? &k_map : &v_map;
-    uint32_t issued = 0;
-    bool ok = true;
-    for (; on && ok; on = w.next(p)) {
-      const Piece& c = w.c;
-      const KeyRange kr = key_range(p, c.len, c.n, c.i0, min(c.n, c.i0 + p.tokens));
-      TileRows at(p, kr, c, lane);
-      const int box = at.box;
-      for (int tile = c.tile0; tile < c.tile1; ++tile, ++issued) {
-        at.advance(tile);
-        const int st = Sh::stage(kv, issued);
-        const uint32_t freed = smem_u32(kQuant ? &C.raw_empty[kv] : &C.empty[kv][st]);
-        ok = __all_sync(0xffffffffu, role_wait(C, freed, (kQuant ? issued & 1 : Sh::parity(kv, issued)) ^ 1));
-        if (!ok) break;
-        const uint32_t bar = smem_u32(kQuant ? &C.raw_full[kv] : &C.full[kv][st]);
-        constexpr uint32_t kRowBytes = kQuant ? D : 2 * D;
-        mbar_arrive_expect_tx_p(leader, bar, __popc(at.have(tile)) * (uint32_t)box * kRowBytes);
-        const uint32_t to = smem_u32(base + (kQuant ? Sh::kRaw + kv * Sh::kRawBytes : Sh::at(kv, issued)));
-        if constexpr (kQuant) {  // the scale bytes: 16 (blocks of 8 keys: 8) a lane
-          const int width = min(box, 16), key = lane * width, part = min(key, 127) >> (7 - at.log_parts);
-          const int y = at.row(tile, part);
-          if (key < 128 && y >= 0) {
-            const uint8_t* src = p.scales + at.scale_at(y + (key - part * box), kv);
-            const uint32_t sd = smem_u32(&C.scales[kv][key]);
-            if (width == 16)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sd), "l"(src) : "memory");
-            else
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(sd), "l"(src) : "memory");
+      if (!ok && lane == 0) give_up(C, p.err);
+    } else if (warp == Ro::kLoad || warp == Ro::kLoad + 1) {
+      // ------------------------------------------------------------------ K and V copies
+      const int kv = warp - Ro::kLoad;
+      const uint32_t leader = elect_one_sync();
+      const CUtensorMap* map = kv == 0 ? &k_map : &v_map;
+      uint32_t issued = 0;
+      bool ok = true;
+      for (; on && ok; on = w.next(p)) {
+        const Piece& c = w.c;
+        const KeyRange kr = key_range(p, c.len, c.n, c.i0, min(c.n, c.i0 + p.tokens));
+        TileRows at(p, kr, c, lane);
+        const int box = at.box;
+        for (int tile = c.tile0; tile < c.tile1; ++tile, ++issued) {
+          at.advance(tile);
+          const int st = Sh::stage(kv, issued);
+          const uint32_t freed = smem_u32(kQuant ? &C.raw_empty[kv] : &C.empty[kv][st]);
+          ok = __all_sync(0xffffffffu, role_wait(C, freed, (kQuant ? issued & 1 : Sh::parity(kv, issued)) ^ 1));
+          if (!ok) break;
+          const uint32_t bar = smem_u32(kQuant ? &C.raw_full[kv] : &C.full[kv][st]);
+          constexpr uint32_t kRowBytes = kQuant ? D : 2 * D;
+          mbar_arrive_expect_tx_p(leader, bar, __popc(at.have(tile)) * (uint32_t)box * kRowBytes);
+          const uint32_t to = smem_u32(base + (kQuant ? Sh::kRaw + kv * Sh::kRawBytes : Sh::at(kv, issued)));
+          if constexpr (kQuant) {  // the scale bytes: 16 (blocks of 8 keys: 8) a lane
+            const int width = min(box, 16), key = lane * width, part = min(key, 127) >> (7 - at.log_parts);
+            const int y = at.row(tile, part);
+            if (key < 128 && y >= 0) {
+              const uint8_t* src = p.scales + at.scale_at(y + (key - part * box), kv);
+              const uint32_t sd = smem_u32(&C.scales[kv][key]);
+              if (width == 16)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sd), "l"(src) : "memory");
+              else
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(sd), "l"(src) : "memory");
+            }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
           }
-          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-        }
-        for (int x0 = 0; x0 < at.parts; x0 += 8) {
-          int y[8];  // all rows first: a shuffle between two copies costs more than the copies
+          for (int x0 = 0; x0 < at.parts; x0 += 8) {
+            int y[8];  // all rows first: a shuffle between two copies costs more than the copies
 #pragma unroll
-          for (int x = 0; x < 8; ++x) y[x] = at.row(tile, (x0 + x) & (at.parts - 1));
+            for (int x = 0; x < 8; ++x) y[x] = at.row(tile, (x0 + x) & (at.parts - 1));
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const uint32_t go = x0 + x < at.parts && y[x] >= 0 ? leader : 0u;
-            if constexpr (kQuant) tma_load_2d_p(go, to + (x0 + x) * box * D, map, 0, y[x], bar);
-            else tma_load_4d_p(go, to + (x0 + x) * box * (D * 2), map, 0, 0, 0, y[x] >> 3, bar);
-          }
-        }
-      }
-    }
-    if (!ok && lane == 0) give_up(C, p.err);
-    // before the shared memory goes: every copy issued has landed (bounded)
-    if constexpr (kQuant) {
-      if (issued > 0) mbar_wait(smem_u32(&C.raw_full[kv]), (issued - 1) & 1);
-    } else {
-      for (uint32_t i = issued > Sh::kK ? issued - Sh::kK : 0; i < issued; ++i)
-        mbar_wait(smem_u32(&C.full[kv][Sh::stage(kv, i)]), Sh::parity(kv, i));
-    }
-  } else if (warp == Ro::kScores || warp == Ro::kValues) {
-    // ------------------------------------------------------------------ MMA issuers
-    const bool do_s = warp == Ro::kScores, do_o = warp == Ro::kValues;
-    const uint32_t leader = elect_one_sync();
-    uint32_t tiles = 0, piece = 0;  // key tiles, pieces before this one
-    uint32_t s0[2] = {0, 0};  // steps of group 0 / 1 before this piece
-    uint32_t last_bar = 0, last_parity = 0, q_pending = 0;
-    bool ok = true;
-    const auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = ok && __all_sync(0xffffffffu, role_wait(C, smem_u32(bar), parity));
-      if (ok) tc_fence_after();
-      return ok;
-    };
-    // shared-memory descriptors: offsets only change the address field (in 16-byte units)
-    const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, 1024, kSwizzle128B);
-    const uint64_t p_desc = smem_desc(smem_u32(p_s), 16, 1024, kSwizzle128B);
-    const uint64_t k_desc = smem_desc(smem_u32(base + Sh::kRing), 16, Sh::kGroup, kSwizzle128B);
-    const uint64_t v_desc = smem_desc(smem_u32(base + Sh::kRing + Sh::kK * Sh::kTileBytes), 1024, Sh::kGroup, kSwizzle128B);
-    // S of group t = (Q of tile qt) K^T, K in stage st
-    const auto scores = [&](int t, int qt, int st, uint32_t step) {
-      const uint64_t qd = q_desc + qt * (Sh::kTileBytes >> 4), kd = k_desc + st * (Sh::kTileBytes >> 4);
-#pragma unroll
-      for (int kb = 0; kb < D / 64; ++kb)
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          umma_f16_p(leader, tmem + t * kKeys, qd + ((kb * kBlockBytes + kk * 32) >> 4), kd + ((kb * 1024 + kk * 32) >> 4),
-                     kIdescS, (kb > 0 || kk > 0) ? 1u : 0u);
-      umma_commit_p(leader, smem_u32(&C.s_full[t]));
-      last_bar = smem_u32(&C.s_full[t]);
-      last_parity = step & 1;
-    };
-    // O of group t (+)= P V, V in stage st
-    const auto values = [&](int t, int st, bool first, uint32_t step) {
-      const uint64_t vd = v_desc + st * (Sh::kTileBytes >> 4);
-#pragma unroll
-      for (int ks = 0; ks < kKeys / 16; ++ks)
-        umma_f16_p(leader, tmem + 2 * kKeys + t * D, p_desc + (((ks / 4) * kBlockBytes + (ks % 4) * 32) >> 4),
-                   vd + ((ks * 2 * Sh::kGroup) >> 4), kIdescO, (!first || ks > 0) ? 1u : 0u);
-      umma_commit_p(leader, smem_u32(&C.pv_done[t]));
-      last_bar = smem_u32(&C.pv_done[t]);
-      last_parity = step & 1;
-    };
-    for (; on && ok; on = w.next(p)) {
-      const Piece& c = w.c;
-      const int n = c.tile1 - c.tile0;
-      const int i1 = min(c.n, c.i0 + p.tokens);
-      const bool split = i1 - c.i0 <= p.tokens / 2;
-      const int ahead = split ? 2 : 1;
-      const EdgeTiles edge(p, key_range(p, c.len, c.n, c.i0, i1));
-      if (do_s) {
-        // the groups have read the last scores of the piece before: its products are done with Q
-        for (int t = 0; t < 2 && ok; ++t)
-          if (s0[t] > 0) wait(&C.s_free[t], (s0[t] - 1) & 1);
-        if (!ok) break;
-        const int qt = split ? 1 : 2, tpt = p.tokens / 2, head0 = c.kvh * p.group + c.slice * p.gw;
-        const uint32_t bar = smem_u32(&C.q_full);
-        mbar_arrive_expect_tx_p(leader, bar, qt * (D / 64) * tpt * p.gw * 128u);
-        for (int t = 0; t < qt; ++t)
-#pragma unroll
-          for (int kb = 0; kb < D / 64; ++kb)
-            tma_load_3d_p(leader, smem_u32(q_s + t * Sh::kTileBytes + kb * kBlockBytes), &q_map, 64 * kb, head0,
-                          c.q_first + c.i0 + t * tpt, bar);
-        q_pending = piece + 1;
-        if (!wait(&C.q_full, piece & 1)) break;
-      }
-      // the scores of the first tile(s)
-      for (int j = 0; j < min(n, ahead) && ok && do_s; ++j) {
-        const uint32_t i = tiles + j;
-        if (!wait(&C.full[0][Sh::stage(0, i)], Sh::parity(0, i))) break;
-        for (int t = 0; t < (split ? 1 : 2) && ok; ++t) {
-          scores(split ? j : t, t, Sh::stage(0, i), split && j == 1 ? s0[1] : s0[t]);
-        }
-        if (ok) umma_commit_p(leader, smem_u32(&C.empty[0][Sh::stage(0, i)]));
-      }
-      // Half steps h: group h & 1 takes its key tile.  Once it has read its scores, its next ones go
-      // out, then the product of the half step before: the groups find their next scores ready, and
-      // their products run under the other group's softmax.
-      const int halves = split ? n : 2 * n;
-      for (int h = 0; h <= halves && ok; ++h) {
-        if (do_s && h < halves) {
-          const int t = h & 1, j = split ? h : h >> 1;
-          const uint32_t step = s0[t] + (h >> 1);
-          if (j + ahead < n) {
-            const uint32_t ik = tiles + j + ahead;
-            if (!wait(&C.s_free[t], step & 1)) break;
-            if ((split || t == 0) && !wait(&C.full[0][Sh::stage(0, ik)], Sh::parity(0, ik))) break;
-            scores(t, split ? 0 : t, Sh::stage(0, ik), step + 1);
-            if (split || t == 1) umma_commit_p(leader, smem_u32(&C.empty[0][Sh::stage(0, ik)]));
+            for (int x = 0; x < 8; ++x) {
+              const uint32_t go = x0 + x < at.parts && y[x] >= 0 ? leader : 0u;
+              if constexpr (kQuant) tma_load_2d_p(go, to + (x0 + x) * box * D, map, 0, y[x], bar);
+              else tma_load_4d_p(go, to + (x0 + x) * box * (D * 2), map, 0, 0, 0, y[x] >> 3, bar);
+            }
           }
         }
-        if (do_o && h > 0) {
-          const int t = (h - 1) & 1, j = split ? h - 1 : (h - 1) >> 1;
-          const uint32_t step = s0[t] + ((h - 1) >> 1), iv = tiles + j;
-          if ((split || t == 0) && !wait(&C.full[1][Sh::stage(1, iv)], Sh::parity(1, iv))) break;
-          if (!kQuant && (split || t == 0) && edge(c.tile0 + j)) mbar_arrive_p(leader, smem_u32(&C.v_ready[t]));
-          if (!wait(&C.p_full[t], step & 1)) break;
-          values(t, Sh::stage(1, iv), step == s0[t], step);
-          if (split || t == 1) umma_commit_p(leader, smem_u32(&C.empty[1][Sh::stage(1, iv)]));
-        }
       }
-      tiles += n;
-      ++piece;
-      s0[0] += split ? (n + 1) / 2 : n;
-      s0[1] += split ? n / 2 : n;
+      if (!ok && lane == 0) give_up(C, p.err);
+      // before the shared memory goes: every copy issued has landed (bounded)
+      if constexpr (kQuant) {
+        if (issued > 0) mbar_wait(smem_u32(&C.raw_full[kv]), (issued - 1) & 1);
+      } else {
+        for (uint32_t i = issued > Sh::kK ? issued - Sh::kK : 0; i < issued; ++i)
+          mbar_wait(smem_u32(&C.full[kv][Sh::stage(kv, i)]), Sh::parity(kv, i));
+      }
+    } else if (warp == Ro::kScores || warp == Ro::kValues) {
+      // ------------------------------------------------------------------ MMA issuers
+      const bool do_s = warp == Ro::kScores, do_o = warp == Ro::kValues;
+      const uint32_t leader = elect_one_sync();
+      uint32_t tiles = 0, piece = 0;  // key tiles, pieces before this one
+      uint32_t s0[2] = {0, 0};  // steps of group 0 / 1 before this piece
+      uint32_t last_bar = 0, last_parity = 0, q_pending = 0;
+      bool ok = true;
+      const auto wait = [&](uint64_t* bar, uint32_t parity) {
+        ok = ok && __all_sync(0xffffffffu, role_wait(C, smem_u32(bar), parity));
+        if (ok) tc_fence_after();
+        return ok;
+      };
+      // shared-memory descriptors: offsets only change the address field (in 16-byte units)
+      const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, 1024, kSwizzle128B);
+      const uint64_t p_desc = smem_desc(smem_u32(p_s), 16, 1024, kSwizzle128B);
+      const uint64_t k_desc = smem_desc(smem_u32(base + Sh::kRing), 16, Sh::kGroup, kSwizzle128B);
+      const uint64_t v_desc = smem_desc(smem_u32(base + Sh::kRing + Sh::kK * Sh::kTileBytes), 1024, Sh::kGroup, kSwizzle128B);
+      // S of group t = (Q of tile qt) K^T, K in stage st
+      const auto scores = [&](int t, int qt, int st, uint32_t step) {
+        const uint64_t qd = q_desc + qt * (Sh::kTileBytes >> 4), kd = k_desc + st * (Sh::kTileBytes >> 4);
+#pragma unroll
+        for (int kb = 0; kb < D / 64; ++kb)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f16_p(leader, tmem + t * kKeys, qd + ((kb * kBlockBytes + kk * 32) >> 4), kd + ((kb * 1024 + kk * 32) >> 4),
+                       kIdescS, (kb > 0 || kk > 0) ? 1u : 0u);
+        umma_commit_p(leader, smem_u32(&C.s_full[t]));
+        last_bar = smem_u32(&C.s_full[t]);
+        last_parity = step & 1;
+      };
+      // O of group t (+)= P V, V in stage st
+      const auto values = [&](int t, int st, bool first, uint32_t step) {
+        const uint64_t vd = v_desc + st * (Sh::kTileBytes >> 4);
+#pragma unroll
+        for (int ks = 0; ks < kKeys / 16; ++ks)
+          umma_f16_p(leader, tmem + 2 * kKeys + t * D, p_desc + (((ks / 4) * kBlockBytes + (ks % 4) * 32) >> 4),
+                     vd + ((ks * 2 * Sh::kGroup) >> 4), kIdescO, (!first || ks > 0) ? 1u : 0u);
+        umma_commit_p(leader, smem_u32(&C.pv_done[t]));
+        last_bar = smem_u32(&C.pv_done[t]);
+        last_parity = step & 1;
+      };
+      for (; on && ok; on = w.next(p)) {
+        const Piece& c = w.c;
+        const int n = c.tile1 - c.tile0;
+        const int i1 = min(c.n, c.i0 + p.tokens);
+        const bool split = i1 - c.i0 <= p.tokens / 2;
+        const int ahead = split ? 2 : 1;
+        const EdgeTiles edge(p, key_range(p, c.len, c.n, c.i0, i1));
+        if (do_s) {
+          // the groups have read the last scores of the piece before: its products are done with Q
+          for (int t = 0; t < 2 && ok; ++t)
+            if (s0[t] > 0) wait(&C.s_free[t], (s0[t] - 1) & 1);
+          if (!ok) break;
+          const int qt = split ? 1 : 2, tpt = p.tokens / 2, head0 = c.kvh * p.group + c.slice * p.gw;
+          const uint32_t bar = smem_u32(&C.q_full);
+          mbar_arrive_expect_tx_p(leader, bar, qt * (D / 64) * tpt * p.gw * 128u);
+          for (int t = 0; t < qt; ++t)
+#pragma unroll
+            for (int kb = 0; kb < D / 64; ++kb)
+              tma_load_3d_p(leader, smem_u32(q_s + t * Sh::kTileBytes + kb * kBlockBytes), &q_map, 64 * kb, head0,
+                            c.q_first + c.i0 + t * tpt, bar);
+          q_pending = piece + 1;
+          if (!wait(&C.q_full, piece & 1)) break;
+        }
+        // the scores of the first tile(s)
+        for (int j = 0; j < min(n, ahead) && ok && do_s; ++j) {
+          const uint32_t i = tiles + j;
+          if (!wait(&C.full[0][Sh::stage(0, i)], Sh::parity(0, i))) break;
+          for (int t = 0; t < (split ? 1 : 2) && ok; ++t) {
+            scores(split ? j : t, t, Sh::stage(0, i), split && j == 1 ? s0[1] : s0[t]);
+          }
+          if (ok) umma_commit_p(leader, smem_u32(&C.empty[0][Sh::stage(0, i)]));
+        }
+        // Half steps h: group h & 1 takes its key tile.  Once it has read its scores, its next ones go
+        // out, then the product of the half step before: the groups find their next scores ready, and
+        // their products run under the other group's softmax.
+        const int halves = split ? n : 2 * n;
+        for (int h = 0; h <= halves && ok; ++h) {
+          if (do_s && h < halves) {
+            const int t = h & 1, j = split ? h : h >> 1;
+            const uint32_t step = s0[t] + (h >> 1);
+            if (j + ahead < n) {
+              const uint32_t ik = tiles + j + ahead;
+              if (!wait(&C.s_free[t], step & 1)) break;
+              if ((split || t == 0) && !wait(&C.full[0][Sh::stage(0, ik)], Sh::parity(0, ik))) break;
+              scores(t, split ? 0 : t, Sh::stage(0, ik), step + 1);
+              if (split || t == 1) umma_commit_p(leader, smem_u32(&C.empty[0][Sh::stage(0, ik)]));
+            }
+          }
+          if (do_o && h > 0) {
+            const int t = (h - 1) & 1, j = split ? h - 1 : (h - 1) >> 1;
+            const uint32_t step = s0[t] + ((h - 1) >> 1), iv = tiles + j;
+            if ((split || t == 0) && !wait(&C.full[1][Sh::stage(1, iv)], Sh::parity(1, iv))) break;
+            if (!kQuant && (split || t == 0) && edge(c.tile0 + j)) mbar_arrive_p(leader, smem_u32(&C.v_ready[t]));
+            if (!wait(&C.p_full[t], step & 1)) break;
+            values(t, Sh::stage(1, iv), step == s0[t], step);
+            if (split || t == 1) umma_commit_p(leader, smem_u32(&C.empty[1][Sh::stage(1, iv)]));
+          }
+        }
+        tiles += n;
+        ++piece;
+        s0[0] += split ? (n + 1) / 2 : n;
+        s0[1] += split ? n / 2 : n;
+      }
+      if (!ok && lane == 0) give_up(C, p.err);
+      if (q_pending) mbar_wait(smem_u32(&C.q_full), (q_pending - 1) & 1);  // Q has landed (bounded)
+      if (last_bar) mbar_wait(last_bar, last_parity);  // MMAs in flight end (bounded) before TMEM goes
     }
-    if (!ok && lane == 0) give_up(C, p.err);
-    if (q_pending) mbar_wait(smem_u32(&C.q_full), (q_pending - 1) & 1);  // Q has landed (bounded)
-    if (last_bar) mbar_wait(last_bar, last_parity);  // MMAs in flight end (bounded) before TMEM goes
-  }
   } else {
     // ------------------------------------------------------------------ softmax: thread = row
     regs_inc<Ro::kSoftmax>();
