@@ -5,11 +5,13 @@
 //   o_i = sum_p softmax_p(scale q_i . k_p) v_p over the positions p that query i sees
 //   (chunk_plan.cuh).
 //
-// The CUDA-core kernel: 64 query rows x 64 keys a step, 256 threads, thread (ty, tx)
-// holding rows ty + 16 i and keys (then dims) tx + 16 j.  All arithmetic is f32, so it
-// is the path of f32 caches.  What bounds it is FMA issue (two products an instruction), once the
-// next step's K and V are on their way while a step is computed: 4 prompts of 256 tokens (32 heads over 4 of 64)
-// take 61 us (17 TFLOP/s of what is seen); they took 92 with every step loaded element by element as it came.
+// The CUDA-core kernel: 64 query rows x 64 keys a step, thread (ty, tx) holding rows ty + 16 i and keys
+// (then 4-dim pieces) tx + kTx j.  All arithmetic is f32, so it is the path of f32 caches.  What bounds
+// it is shared memory and FMA issue together: with head_dim up to 64 a thread takes 4 x 8 products from
+// 12 16-byte reads, three CTAs of 128 threads to an SM, which hide one another's loads: 4 prompts of 256
+// tokens (32 heads over 4 of 64) take 55 us, 20 TFLOP/s of what is seen.  4 x 4 products from 8 reads, two CTAs of
+// 256 threads and loads a step ahead took 60 us (63000 wavefronts of shared memory in 92000 cycles), loads
+// element by element 92.  Larger rows need the threads: one CTA of 256, 4 x 4 products.
 #include <cuda_fp8.h>
 
 #include "chunk_plan.cuh"
@@ -17,7 +19,7 @@
 namespace snapmind {
 namespace {
 
-constexpr int kRows = 64, kKeys = 64, kGenThreads = 256;
+constexpr int kRows = 64, kKeys = 64;
 constexpr int kGenMaxD = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -32,7 +34,11 @@ __device__ __forceinline__ float scale_byte_to_f(uint8_t b) { return __uint_as_f
 // 16 different rows then touch different banks), zero past head_dim.
 template <int D4>
 struct GenSmem {
-  static constexpr int D = 64 * D4, P = D + 4, PS = kKeys + 4;
+  static constexpr int D = 64 * D4, P = D + 4;
+  // threads that share a row, keys and 16-byte pieces of V of a thread; CTAs per SM
+  static constexpr int kTx = D4 == 1 ? 8 : 16, kJ = kKeys / kTx, kX = D / (4 * kTx), kThreads = 16 * kTx;
+  static constexpr int kCtas = D4 == 1 ? 3 : 1;
+  static constexpr int PS = kKeys + (D4 == 1 ? 8 : 4);
   float q[kRows * P];
   float k[kKeys * P];
   float v[kKeys * P];
@@ -93,17 +99,20 @@ __device__ __forceinline__ bool out_vec(const ChunkParams& p) {
 }
 
 template <typename T, typename KV, int D4>
-__global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_kernel(ChunkParams p) {
+__global__ void __launch_bounds__(GenSmem<D4>::kThreads, GenSmem<D4>::kCtas) chunk_generic_kernel(ChunkParams p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   using Smem = GenSmem<D4>;
-  constexpr int P = Smem::P, PS = Smem::PS, D = Smem::D;
+  constexpr int P = Smem::P, PS = Smem::PS, D = Smem::D, kTx = Smem::kTx, kJ = Smem::kJ, kX = Smem::kX;
+  constexpr int kGenThreads = Smem::kThreads;
   constexpr bool kQuant = std::is_same<KV, uint8_t>::value;
   // whole 16-byte vectors of the pool: a row's, a thread's of K (and of V) a step
   constexpr int V = 16 / sizeof(KV), kRowVecs = D / V, kVecs = kKeys * kRowVecs / kGenThreads;
-  constexpr bool kCanFetch = kVecs <= 8;  // registers for a step of K and V
+  constexpr bool kCanFetch = kVecs <= 8;                    // registers for a step of K and V
+  constexpr bool kAhead = D4 > 1 && kCanFetch;              // ... while the step before is computed
+  constexpr int kUnroll = D4 == 1 ? 2 : 4;                  // 4 spills with 168 registers
   constexpr int kHeld = kCanFetch ? kVecs : 1;
   Smem& S = *reinterpret_cast<Smem*>(smem_raw);
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int tid = threadIdx.x, tx = tid % kTx, ty = tid / kTx;
   prior_grid_wait();
   plan_block(p, S.plan, reinterpret_cast<int32_t*>(S.q));
   const float c2 = p.scale * kLog2e;
@@ -184,8 +193,8 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
       S.q[r * P + d] = x;
     }
     __syncthreads();
-    if (fetches) fetch(c.tile0);
-    float2 o[4][2 * D4];
+    if (kAhead && fetches) fetch(c.tile0);
+    float2 o[4][2 * kX];
     float m[4], l[4];
     int qpos[4];
 #pragma unroll
@@ -194,12 +203,13 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
       l[i] = 0.f;
       qpos[i] = kr.pos0 + p.by_gw.div(ty + 16 * i);
 #pragma unroll
-      for (int j = 0; j < 2 * D4; ++j) o[i][j] = make_float2(0.f, 0.f);
+      for (int j = 0; j < 2 * kX; ++j) o[i][j] = make_float2(0.f, 0.f);
     }
     for (int t = c.tile0; t < c.tile1; ++t) {
       __syncthreads();  // the step before has been computed
       bool odd = false;  // a value of V that is not finite
       if (fetches) {
+        if (!kAhead) fetch(t);
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
           const int e = tid + i * kGenThreads, r = e / kRowVecs, x = e % kRowVecs;
@@ -237,59 +247,59 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
       }
       find(t + 1);
       odd = __syncthreads_or(odd);
-      if (fetches && t + 1 < c.tile1) fetch(t + 1);  // lands while this step is computed
-      float2 s2[4][4];
+      if (kAhead && fetches && t + 1 < c.tile1) fetch(t + 1);  // lands while this step is computed
+      float2 s2[4][kJ];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0.f, 0.f);
-#pragma unroll 4
+        for (int j = 0; j < kJ; ++j) s2[i][j] = make_float2(0.f, 0.f);
+#pragma unroll kUnroll
       for (int d = 0; d < D; d += 4) {
-        float4 a[4], b[4];
+        float4 a[4], b[kJ];
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(&S.q[(ty + 16 * i) * P + d]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(&S.k[(tx + 16 * j) * P + d]);
+        for (int j = 0; j < kJ; ++j) b[j] = *reinterpret_cast<const float4*>(&S.k[(tx + kTx * j) * P + d]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < kJ; ++j) {
             s2[i][j] = fma2(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y), s2[i][j]);
             s2[i][j] = fma2(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w), s2[i][j]);
           }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float s[4];
+        float s[kJ];
         float mx = m[i];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int pos = S.pos[t & 1][tx + 16 * j];
+        for (int j = 0; j < kJ; ++j) {
+          const int pos = S.pos[t & 1][tx + kTx * j];
           const bool sees = pos <= qpos[i] && (p.window <= 0 || pos > qpos[i] - p.window || pos < p.sinks);
           s[j] = sees ? (s2[i][j].x + s2[i][j].y) * c2 : -INFINITY;
           mx = fmaxf(mx, s[j]);
         }
 #pragma unroll
-        for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        for (int off = kTx / 2; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
         // nothing seen so far: any finite reference gives p = 2^-inf = 0
         const float ref = mx == -INFINITY ? 0.f : mx;
         const float alpha = ex2(m[i] - ref);
         m[i] = mx;
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kJ; ++j) {
           const float e = ex2(s[j] - ref);
           sum += e;
-          S.s[(ty + 16 * i) * PS + tx + 16 * j] = e;
+          S.s[(ty + 16 * i) * PS + tx + kTx * j] = e;
         }
         l[i] = l[i] * alpha + sum;  // this thread's share; summed over the row's threads at the end
 #pragma unroll
-        for (int j = 0; j < 2 * D4; ++j) {
+        for (int j = 0; j < 2 * kX; ++j) {
           o[i][j].x *= alpha;
           o[i][j].y *= alpha;
         }
       }
-      __syncwarp();  // a row's 16 threads share a warp
+      __syncwarp();  // a row's threads share a warp
       if (!odd) {
 #pragma unroll 2
         for (int k = 0; k < kKeys; k += 4) {
@@ -300,8 +310,8 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-            for (int j = 0; j < D4; ++j) {
-              const float4 b = *reinterpret_cast<const float4*>(&S.v[(k + kk) * P + 64 * j + 4 * tx]);
+            for (int j = 0; j < kX; ++j) {
+              const float4 b = *reinterpret_cast<const float4*>(&S.v[(k + kk) * P + 4 * (kTx * j + tx)]);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const float2 x = make_float2(a[i][kk], a[i][kk]);
@@ -319,8 +329,8 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
             if (!(pos <= qpos[i] && (p.window <= 0 || pos > qpos[i] - p.window || pos < p.sinks))) continue;
             const float a = S.s[(ty + 16 * i) * PS + k];
 #pragma unroll
-            for (int j = 0; j < 2 * D4; ++j) {
-              const float* v = &S.v[k * P + 64 * (j / 2) + 4 * tx + 2 * (j % 2)];
+            for (int j = 0; j < 2 * kX; ++j) {
+              const float* v = &S.v[k * P + 4 * (kTx * (j / 2) + tx) + 2 * (j % 2)];
               o[i][j].x = fmaf(a, v[0], o[i][j].x);
               o[i][j].y = fmaf(a, v[1], o[i][j].y);
             }
@@ -331,7 +341,7 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int off = 8; off > 0; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
+      for (int off = kTx / 2; off > 0; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
       const int r = ty + 16 * i, tok = p.by_gw.div(r), g = r - tok * p.gw;
       if (r >= n_rows || g >= heads) continue;
       const bool whole = c.whole();
@@ -343,10 +353,10 @@ __global__ void __launch_bounds__(kGenThreads, D4 == 1 ? 2 : 1) chunk_generic_ke
         p.part_ml[slot * 2 + 1] = l[i];
       }
 #pragma unroll
-      for (int j = 0; j < D4; ++j) {
+      for (int j = 0; j < kX; ++j) {
         const float4 y = make_float4(o[i][2 * j].x * f, o[i][2 * j].y * f, o[i][2 * j + 1].x * f, o[i][2 * j + 1].y * f);
-        if (whole) store4(out, 64 * j + 4 * tx, hd, y, vec);
-        else store4(p.part_o + slot * hd, 64 * j + 4 * tx, hd, y, hd % 4 == 0);
+        if (whole) store4(out, 4 * (kTx * j + tx), hd, y, vec);
+        else store4(p.part_o + slot * hd, 4 * (kTx * j + tx), hd, y, hd % 4 == 0);
       }
     }
   }
@@ -511,23 +521,23 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
 
 template <typename T, typename KV>
 int launch_generic(ChunkParams& p, cudaStream_t st) {
-  const auto go = [&](auto kernel, size_t smem, bool (&done)[kMaxDevices]) -> int {
+  const auto go = [&](auto kernel, int threads, size_t smem, bool (&done)[kMaxDevices]) -> int {
     const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem, done);
     if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
-    return cuda_status(launch_dependent(kernel, dim3(p.n_ctas), kGenThreads, smem, st, p), "paged_chunk launch");
+    return cuda_status(launch_dependent(kernel, dim3(p.n_ctas), threads, smem, st, p), "paged_chunk launch");
   };
   static bool done[3][kMaxDevices] = {};
   static_assert(sizeof(GenSmem<4>) <= 232448, "shared memory budget");
   static_assert(sizeof(GenSmem<1>().q) + sizeof(GenSmem<1>().k) >= kMaxChunkBatch * 4, "plan scratch");
-  if (p.head_dim <= 64) return go(chunk_generic_kernel<T, KV, 1>, sizeof(GenSmem<1>), done[0]);
-  if (p.head_dim <= 128) return go(chunk_generic_kernel<T, KV, 2>, sizeof(GenSmem<2>), done[1]);
-  return go(chunk_generic_kernel<T, KV, 4>, sizeof(GenSmem<4>), done[2]);
+  if (p.head_dim <= 64) return go(chunk_generic_kernel<T, KV, 1>, GenSmem<1>::kThreads, sizeof(GenSmem<1>), done[0]);
+  if (p.head_dim <= 128) return go(chunk_generic_kernel<T, KV, 2>, GenSmem<2>::kThreads, sizeof(GenSmem<2>), done[1]);
+  return go(chunk_generic_kernel<T, KV, 4>, GenSmem<4>::kThreads, sizeof(GenSmem<4>), done[2]);
 }
 
-// The largest workspace of the kernels: one CTA per SM with units of 256 rows, or two with 64.
+// The largest workspace of the kernels: one CTA per SM with units of 256 rows, or three with 64.
 int64_t max_ctas() { return num_sms(); }
 constexpr int kMaxRows = 256;
-static_assert(2 * kRows <= kMaxRows, "two CTAs per SM");
+static_assert(3 * kRows <= kMaxRows, "three CTAs per SM");
 
 }  // namespace
 
@@ -627,7 +637,7 @@ int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stri
     const int rc = launch_chunk_umma(p, dtype, pool_dtype, st);
     if (rc != SNAPMIND_ERR_UNSUPPORTED) return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
   }
-  const int ctas = num_sms() * (head_dim <= 64 ? 2 : 1);
+  const int ctas = num_sms() * (head_dim <= 64 ? GenSmem<1>::kCtas : 1);
   int rc = plan_geometry(p, kRows, kRows, kKeys, ctas);
   if (rc != SNAPMIND_OK) return rc;
   switch (dtype) {
