@@ -101,9 +101,10 @@ class BlockPool:
         """Grow sequence b by ``n_new[b]`` tokens (host integers, 0 leaves it as it is;
         sequences past the list are left alone): the ragged form of ``reserve``, in the
         same order and all or nothing."""
-        n = np.asarray(n_new, dtype=np.int64).reshape(-1)
-        if len(n) > self.max_seqs or (n < 0).any():
-            raise ValueError("reserve_each: one count >= 0 for each of the pool's sequences at most")
+        n = np.asarray(n_new).reshape(-1)
+        if len(n) > self.max_seqs or (n.size and (n.dtype.kind not in "iu" or (n < 0).any())):
+            raise ValueError("reserve_each: one integer >= 0 for each of the pool's sequences at most")
+        n = n.astype(np.int64)
         bs = self.block_size
         lens = self._host_lens[:len(n)]
         want = (lens + n + bs - 1) // bs

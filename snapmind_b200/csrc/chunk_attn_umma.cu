@@ -28,8 +28,9 @@
 //   order, so a barrier's parity always tells the phase that is meant.
 // Every wait is bounded and ends early once another role gave up; TMEM is released on
 // every path.
-// What bounds it: both operands of every product come from shared memory, 4 x 64 KB for a step of
-// 2 x 128 x 128 scores (3072 cycles; measured 3200 to 3300).  2048 new tokens behind
+// What bounds it is shared memory: a step of 2 x 128 x 128 scores reads 4 x 64 KB of operands, writes 64 KB of P
+// and receives 64 KB of K and V, 3072 cycles at 128 bytes each (measured 3200 to 3300; the products
+// themselves take 2048).  2048 new tokens behind
 // 30720 cached ones, 32 heads over 8 of 128: 920 us, 1160 TFLOP/s.  Short units add 20000 cycles at the start of a CTA and 12000 a piece
 // (a mixed step 172 us, 772 TFLOP/s).  Over 8-bit rows the converting warps add 48 KB a tile to the same
 // traffic: 2700 cycles a tile, 2000 of them without any conversion, 484 TFLOP/s; fewer

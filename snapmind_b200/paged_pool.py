@@ -100,6 +100,7 @@ class PagedKVPool(BlockPool):
         (``layer=None``: layers 0 .. L-1); ``cu_new`` int32 ``[B + 1]`` on the device: sequence
         b owns rows ``cu_new[b] .. cu_new[b + 1] - 1``, its newest tokens.
         """
+        _lib.require_offsets("append", cu_new, self.block_tables)
         if k_new.dim() == 3:
             if layer is None:
                 raise ValueError("layer is required for [total, H, D] inputs")
@@ -120,8 +121,6 @@ class PagedKVPool(BlockPool):
             raise ValueError(f"append: layers {base} .. {base + n_layers - 1} of a pool of {self.n_layers}")
         if batch > self.max_seqs or batch < 0:
             raise ValueError(f"append: {batch} sequences, the pool holds {self.max_seqs}")
-        if cu is not None:
-            _lib.require_offsets("append", cu, self.block_tables)
         st = k_new.stride()
         if st != v_new.stride() or st[-1] != 1:
             k_new, v_new = k_new.contiguous(), v_new.contiguous()

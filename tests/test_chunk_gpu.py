@@ -728,3 +728,21 @@ def test_positions_past_the_table_do_not_count(cuda_device, cache, d, single, ge
             check(out[i:i + 1], q[i:i + 1], [0, 1], [ks[0][:, lo:]], [vs[0][:, lo:]], 0, 0, 2.0**-8)
         with pytest.raises(RuntimeError, match="table"):
             pool.check()
+
+
+def test_counts_and_offsets_of_other_types(cuda_device):
+    pool, _, _ = make_pool(torch.bfloat16, [40, 30], 2, 128, 16, 4, spare=4)
+    kv = torch.randn((2, 2, 128), device="cuda").bfloat16()
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    for bad in ([1.5, 1.0], ["1", "1"]):
+        with pytest.raises(ValueError):
+            pool.reserve_each(bad)
+    for bad in (cu[0], cu.long(), cu.cpu(), cu[:0]):
+        with pytest.raises(ValueError):
+            pool.append_packed(0, kv, kv, bad)
+    assert pool.host_lens.tolist() == [40, 30]
+    pool.reserve_each([])
+    pool.reserve_each(np.array([1, 0], dtype=np.uint8))
+    pool.reserve_each(torch.tensor([0, 1]))
+    assert pool.host_lens.tolist() == pool.seq_lens.tolist() == [41, 31]
+    pool.check()
