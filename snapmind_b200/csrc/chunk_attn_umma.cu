@@ -160,6 +160,13 @@ __device__ __forceinline__ float2 mul2(float2 a, float b) {
   return r;
 }
 
+// 32 bytes, one sector, in one store.
+__device__ __forceinline__ void store32(void* p, const uint32_t* x) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(x[0]), "r"(x[1]), "r"(x[2]),
+               "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+               : "memory");
+}
+
 // 16 e4m3 codes of one row times 2^(byte - 127), as 16 elements of T.  The scale is a power
 // of two: exact in bf16, and in f16 as long as the value is a normal f16.
 template <typename T>
@@ -678,8 +685,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
                                                                 pack2<T>(o[y + 4], o[y + 5]), pack2<T>(o[y + 6], o[y + 7]));
         } else {
 #pragma unroll
-          for (int y = 0; y < 16; y += 4)
-            *reinterpret_cast<float4*>(p.part_o + slot * D + x + y) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+          for (int y = 0; y < 16; y += 8) store32(p.part_o + slot * D + x + y, reinterpret_cast<const uint32_t*>(o + y));
         }
       }
       tc_fence_before();
