@@ -32,8 +32,8 @@
 // and receives 64 KB of K and V, 3072 cycles at 128 bytes each (measured 3200 to 3300; the products
 // themselves take 2048).  2048 new tokens behind
 // 30720 cached ones, 32 heads over 8 of 128: 920 us, 1160 TFLOP/s.  Short units add 20000 cycles at the start of a CTA and 12000 a piece
-// (a mixed step 172 us, 772 TFLOP/s).  Over 8-bit rows the converting warps add 48 KB a tile to the same
-// traffic: 2700 cycles a tile, 2000 of them without any conversion, 484 TFLOP/s; fewer
+// (a mixed step 167 us, 800 TFLOP/s).  Over 8-bit rows the converting warps add 48 KB a tile to the same
+// traffic: 2700 cycles a tile, 2000 of them without any conversion, 505 TFLOP/s; fewer
 // instructions, rows fetched ahead and conversions by bit operations did not help.
 #include <cuda.h>
 #include <cuda_fp8.h>
@@ -160,7 +160,8 @@ __device__ __forceinline__ float2 mul2(float2 a, float b) {
   return r;
 }
 
-// 32 bytes, one sector, in one store.
+// 32 bytes, one sector, in one store (a lane stores a row of its own: with 16 bytes a store, a mixed
+// step took 172 us, not 167).
 __device__ __forceinline__ void store32(void* p, const uint32_t* x) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(x[0]), "r"(x[1]), "r"(x[2]),
                "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
