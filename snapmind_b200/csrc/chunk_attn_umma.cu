@@ -29,7 +29,7 @@
 // Every wait is bounded and ends early once another role gave up; TMEM is released on
 // every path.
 // What bounds it is shared memory: a step of 2 x 128 x 128 scores reads 4 x 64 KB of operands, writes 64 KB of P
-// and receives 64 KB of K and V, 3072 cycles at 128 bytes each (measured 3200 to 3300; the products
+// and receives 64 KB of K and V, 3070 cycles at 128 bytes each (measured 3200 to 3300; the products
 // themselves take 2048).  2048 new tokens behind
 // 30720 cached ones, 32 heads over 8 of 128: 920 us, 1160 TFLOP/s.  Short units add 20000 cycles at the start of a CTA and 12000 a piece
 // (a mixed step 167 us, 800 TFLOP/s).  Over 8-bit rows the converting warps add 48 KB a tile to the same
