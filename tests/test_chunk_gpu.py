@@ -746,3 +746,33 @@ def test_counts_and_offsets_of_other_types(cuda_device):
     pool.reserve_each(torch.tensor([0, 1]))
     assert pool.host_lens.tolist() == pool.seq_lens.tolist() == [41, 31]
     pool.check()
+
+
+@pytest.mark.parametrize("d", [64, 128, 40, 256])
+@pytest.mark.parametrize("src,dst", [("bf16", "bf16"), ("f32", "f32"), ("f16", "f16"), ("f32", "bf16"), ("bf16", "f32")])
+def test_packed_rows_are_stored(cuda_device, src, dst, d):
+    """append_packed puts every row where it belongs and nothing elsewhere: aligned rows, rows off
+    every boundary, rows outside every sequence, an empty sequence, one layer of several."""
+    from snapmind_b200 import PagedKVPool
+
+    pool = PagedKVPool(3, 2, d, 40, 4, 20, block_size=8, dtype=DT[dst])
+    new = [37, 0, 1, 90]
+    pool.reserve_each([5, 3, 0, 2])
+    pool.reserve_each(new)
+    pool.k.fill_(7)
+    pool.v.fill_(7)
+    total = sum(new) + 3
+    cu = torch.tensor([2, 39, 39, 40, 130], dtype=torch.int32, device="cuda")  # rows 0, 1 and 130 are no one's
+    for off in (0, 1):
+        k, v = (torch.randn((2, total, 2, d + 1), device="cuda").to(DT[src])[..., off:off + d] for _ in range(2))
+        if not off:
+            k, v = k.contiguous(), v.contiguous()
+        pool.append_packed(None, k, v, cu)  # layers 0 and 1
+        pool.check()
+        for x, p in ((k, pool.k), (v, pool.v)):
+            want = torch.full_like(p, 7)
+            for b, n in enumerate(new):
+                for i in range(n):
+                    slot = int(pool.host_lens[b]) - n + i
+                    want[:2, int(pool.block_tables[b, slot // 8]), :, slot % 8] = x[:, int(cu[b]) + i].to(DT[dst])
+            assert torch.equal(p, want)
