@@ -509,7 +509,9 @@ SNAPMIND_API int snapmind_paged_gqa_decode_noalloc(const void *q, int64_t q_stri
 /*
  * snapmind_kv_reserve with its own number of new tokens for every sequence:
  * n_new is a device array of `batch` counts (0 leaves a sequence as it is).
- * A negative count sets SNAPMIND_DEVERR_TABLE and nothing changes.
+ * A count that is negative or that a sequence's table row has no room for sets
+ * SNAPMIND_DEVERR_TABLE, a demand past the free blocks SNAPMIND_DEVERR_OUT_OF_BLOCKS;
+ * either way nothing changes.
  */
 SNAPMIND_API int snapmind_kv_reserve_each(int32_t *block_tables, int64_t table_stride_seq, int32_t table_width,
                              int32_t *seq_lens, const int32_t *n_new, int32_t batch, int32_t block_size,

@@ -102,8 +102,8 @@ class BlockPool:
         sequences past the list are left alone): the ragged form of ``reserve``, in the
         same order and all or nothing."""
         n = np.asarray(n_new).reshape(-1)
-        if len(n) > self.max_seqs or (n.size and (n.dtype.kind not in "iu" or (n < 0).any())):
-            raise ValueError("reserve_each: one integer >= 0 for each of the pool's sequences at most")
+        if len(n) > self.max_seqs or (n.size and (n.dtype.kind not in "iu" or (n < 0).any() or (n >= 1 << 31).any())):
+            raise ValueError("reserve_each: one integer in [0, 2^31) for each of the pool's sequences at most")
         n = n.astype(np.int64)
         bs = self.block_size
         lens = self._host_lens[:len(n)]

@@ -366,34 +366,37 @@ __device__ int block_exclusive_scan(int x, int* total) {
 
 __global__ void __launch_bounds__(1024) kv_reserve_kernel(ReserveParams p) {
   __shared__ int s_bad;
-  if (threadIdx.x == 0) s_bad = 0;
-  __syncthreads();
-  // pass 1: total demand and table-width check
-  int need_total = 0;
-  for (int base = 0; base < p.batch; base += blockDim.x) {
-    const int b = base + threadIdx.x;
-    int need = 0;
-    if (b < p.batch) {
-      const int old_len = p.seq_lens[b];
-      const int n_new = p.n_each ? p.n_each[b] : p.n_new;
-      const int new_len = old_len + n_new;
-      const int have = (old_len + p.block_size - 1) / p.block_size;
-      const int want = (new_len + p.block_size - 1) / p.block_size;
-      need = want - have;
-      if (want > p.table_width || old_len < 0 || n_new < 0) atomicOr(&s_bad, SNAPMIND_DEVERR_TABLE);
-    }
-    int tot;
-    block_exclusive_scan(need, &tot);
-    need_total += tot;
+  __shared__ unsigned long long s_need;
+  if (threadIdx.x == 0) {
+    s_bad = 0;
+    s_need = 0;
   }
   __syncthreads();
+  // pass 1: total demand and table-width check, in 64 bits: counts may come from device memory and hold
+  // anything, and a wrapped length or demand would pass for a small one
+  const int64_t room = min((int64_t)p.table_width * p.block_size, (int64_t)INT32_MAX - p.block_size);
+  unsigned long long mine = 0;
+  for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
+    const int64_t old_len = p.seq_lens[b], n_new = p.n_each ? p.n_each[b] : p.n_new;
+    if (old_len < 0 || n_new < 0 || old_len + n_new > room) {
+      atomicOr(&s_bad, SNAPMIND_DEVERR_TABLE);
+      continue;
+    }
+    const int64_t have = (old_len + p.block_size - 1) / p.block_size;
+    mine += (old_len + n_new + p.block_size - 1) / p.block_size - have;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if ((threadIdx.x & 31) == 0 && mine > 0) atomicAdd(&s_need, mine);
+  __syncthreads();
   const int top = *p.free_top;
-  if (threadIdx.x == 0 && need_total > top) s_bad |= SNAPMIND_DEVERR_OUT_OF_BLOCKS;
+  if (threadIdx.x == 0 && s_need > (unsigned long long)max(top, 0)) s_bad |= SNAPMIND_DEVERR_OUT_OF_BLOCKS;
   __syncthreads();
   if (s_bad) {
     if (threadIdx.x == 0) flag_error(p.err, s_bad);
     return;
   }
+  const int need_total = (int)s_need;
   // pass 2: deterministic assignment, ascending sequence order
   int carry = 0;
   for (int base = 0; base < p.batch; base += blockDim.x) {
