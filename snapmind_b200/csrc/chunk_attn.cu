@@ -365,7 +365,8 @@ __global__ void __launch_bounds__(GenSmem<D4>::kThreads, GenSmem<D4>::kCtas) chu
 
 // Merge of the cut units: block (c, y) works when CTA c holds the first cut inside a
 // unit, on rows y, y + gridDim.y, ... (in groups of kMergeRows); pieces are CTA c - 1's slot 1, then
-// slot 0 of CTAs c .. last.  M = max m_i, out = sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M).  A piece with
+// slot 0 of CTAs c .. last.  M = max m_i, out = sum o_i 2^(m_i - M) / sum l_i 2^(m_i - M); pieces that left
+// means (8-bit decodes: sums relative to M could pass f32's range) have l_i o_i for o_i.  A piece with
 // m = -infinity saw nothing (l = 0, and o may hold anything) or only NaN (l is one, and so is out).
 // The work is a few loads that wait for one another, so what counts is how many are in flight: a
 // warp takes kMergeRows rows of a unit cut into up to 8 pieces at once (one row at a time, the 256-row
@@ -442,6 +443,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
       f *= L == 0.f ? 0.f : 1.f / L;  // a row that sees nothing: zeros
+      if (p.means) f *= ml.y;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if (128 * c >= D) break;
@@ -487,12 +489,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
       const float ref = mb == -INFINITY ? 0.f : mb, old = ex2(M - ref);
       M = mb;
       const float f = ml.x == -INFINITY ? ml.y : ex2(ml.x - ref);
-      float ls = ml.y * f;
+      const float ls_mine = ml.y * f;
+      float ls = ls_mine;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
       L = L * old + ls;
       mul4(acc[0], old);
       mul4(acc[1], old);
+      const float fo = p.means ? ls_mine : f;
       const int here = min(32, n_pieces - k0);
       for (int k = 0; k < here; k += kMergeBatch) {
 #pragma unroll
@@ -504,7 +508,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
             v[u] = k + u < here ? load4(p.part_o + slot(k0 + k + u, r) * D, 128 * c + 4 * lane, D) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int u = 0; u < kMergeBatch; ++u) {
-            const float fu = __shfl_sync(0xffffffffu, f, (k + u) & 31);
+            const float fu = __shfl_sync(0xffffffffu, fo, (k + u) & 31);
             if (k + u < here && fu != 0.f) add4(acc[c], v[u], fu);
           }
         }

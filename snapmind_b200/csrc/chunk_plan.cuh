@@ -48,6 +48,7 @@ struct ChunkParams {
   int32_t* heads;   // workspace: [n_ctas][kPieceInts], see PieceInfo
   float* part_ml;   // workspace: [n_ctas][2][rows][2] maximum (log2 units), sum
   float* part_o;    // workspace: [n_ctas][2][rows][head_dim]
+  int32_t means;    // part_o holds a piece's weighted means of V (else its weighted sums)
   int32_t* err;
 };
 

@@ -12,9 +12,11 @@
 //
 // e4m3 rows (c 2^e, a byte e + 127 per row): the codes become f16 in registers (exact), and
 // the scales never touch the elements: K's multiplies its key's score, V's its weight.
-// With s the score in log2 units and e_v the exponent of V's row, the reference of the running
-// softmax is M = max (s + e_v), so that the weight 2^(s + e_v - M) <= 1 that multiplies the
-// codes is a good f16 whatever the rows' scales are; the sum takes 2^(s - M).  Queries are
+// With s the score in log2 units and e_v the exponent of V's row, the weight that multiplies the
+// codes is 2^(s + e_v - R), R = max (s + e_v), a good f16 whatever the rows' scales are.  The sum
+// has a reference of its own, 2^(s - M), M = max s: R - M may be anything in [-100, 120] and s + e_v
+// differ by more than f32's exponents between rows that count alike (a row of zeros has e = -100), so
+// neither can be had from the other.  A piece's result is O 2^(R - M) / sum, a mean of V.  Queries are
 // brought to [2^8, 2^9) by a power of two per head, so f16 holds a bf16 query as exactly as the
 // f32 sum needs.  Both type conversions take permuted dims (K) and pairs of dims (V), so that
 // ldmatrix can move bytes in 16-bit units:
@@ -35,6 +37,7 @@ constexpr int kD = 128, kTile = 64, kConsumers = 4, kThreads = (kConsumers + 2) 
 constexpr int kScaleLanes = kTile / 16;  // lanes that fetch a tile's scale bytes of K, or of V, 16 each
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.f;  // log2 headroom of the reference maxima
+constexpr float kNone = -3e38f;  // a reference before any score: finite, so that -infinity less it stays one
 
 template <bool kQuant> struct Stage {
   static constexpr int kHalf = kTile * 128;                      // 64 rows of 128 bytes
@@ -48,7 +51,8 @@ struct Ctrl {
   static constexpr int N = Stage<kQuant>::kCount;
   float mo[2][kHeads][kD];
   alignas(16) uint8_t scales[kQuant ? N : 1][2][kTile];  // K, V bytes of a stage's rows (16-byte copies)
-  float mm[kConsumers][kHeads], ml[kConsumers][kHeads];
+  float mm[kConsumers][kHeads], ml[kConsumers][kHeads];  // M, sum
+  float mr[kConsumers][kHeads];                          // R (16-bit caches: M)
   uint64_t full[N], empty[N];
   int32_t abort;
   PlanShared plan;
@@ -268,7 +272,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       float o[8][4];
 #pragma unroll
       for (int k = 0; k < 8; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
-      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // log2 units
+      float m0 = kNone, m1 = kNone, l0 = 0.f, l1 = 0.f;  // M (log2 units), sum
+      float R0 = kNone, R1 = kNone;                      // R
       for (int j = c.tile0; j < c.tile1; ++j, ++tile) {
         const int st = tile % St::kCount;
         ok = __all_sync(0xffffffffu, role_wait(S, smem_u32(&S.full[st]), (tile / St::kCount) & 1));
@@ -293,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           // ---- S^T = K Q^T: 16 keys x 8 heads; keys g and g + 8, heads 2 tig, 2 tig + 1
           float sc[4] = {0.f, 0.f, 0.f, 0.f};
-          float d0 = 1.f, d1 = 1.f;  // 2^-e_v of V's rows g, g + 8
+          float sv0 = 0.f, sv1 = 0.f;  // e_v of V's rows g, g + 8
           if constexpr (kQuant) {
 #pragma unroll
             for (int k = 0; k < 8; k += 2) {
@@ -309,14 +314,12 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
             const uint8_t* bytes = &S.scales[st][0][16 * warp];
             const float k0 = __uint_as_float((uint32_t)bytes[g] << 23), k1 = __uint_as_float((uint32_t)bytes[g + 8] << 23);
-            const int e0 = bytes[kTile + g], e1 = bytes[kTile + g + 8];
-            const float sv0 = (float)(e0 - 127), sv1 = (float)(e1 - 127);
-            d0 = __uint_as_float((uint32_t)(254 - e0) << 23);
-            d1 = __uint_as_float((uint32_t)(254 - e1) << 23);
-            sc[0] = fmaf(sc[0] * k0, q0, sv0);  // s + e_v
-            sc[1] = fmaf(sc[1] * k0, q1, sv0);
-            sc[2] = fmaf(sc[2] * k1, q0, sv1);
-            sc[3] = fmaf(sc[3] * k1, q1, sv1);
+            sv0 = (float)((int)bytes[kTile + g] - 127);
+            sv1 = (float)((int)bytes[kTile + g + 8] - 127);
+            sc[0] *= k0;
+            sc[1] *= k0;
+            sc[2] *= k1;
+            sc[3] *= k1;
           } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -324,51 +327,56 @@ __global__ void __launch_bounds__(kThreads, 2)
               ldsm_x4(kb + (k >> 2) * St::kHalf + k_off[k & 3], a);
               mma16816<kMmaBf16>(sc, a, qf[k][0], qf[k][1]);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[i] *= c2;
           }
-          if (!all) {
-            if (!seen(g)) {
-              sc[0] = sc[1] = -INFINITY;
-              d0 = 0.f;
-            }
-            if (!seen(g + 8)) {
-              sc[2] = sc[3] = -INFINITY;
-              d1 = 0.f;
-            }
-          }
-          // The references are raised only when a score passes them by 2^8 (weights up to 2^8 are as
-          // good as those up to 1): then to the exact maxima, and the sums and O are rescaled.
-          float t0 = fmaxf(sc[0], sc[2]), t1 = fmaxf(sc[1], sc[3]);
-          if (__any_sync(0xffffffffu, t0 > m0 + kRaise || t1 > m1 + kRaise)) {
+          // Scores less their references: xs for the sum, ys for the weights (16-bit caches: xs).  A
+          // reference is raised only when a score passes it by 2^8 (weights up to 2^8 are as good as
+          // those up to 1): then to the exact maximum, and what was summed is rescaled.
+          float xs[4], ys[4];
+          const auto refer = [&](float M0, float M1, float r0, float r1) {
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) {
-              t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, off));
-              t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
+            for (int i = 0; i < 4; ++i) {
+              const float f = i & 1 ? q1 : q0, sv = i & 2 ? sv1 : sv0;
+              xs[i] = fmaf(sc[i], f, i & 1 ? -M1 : -M0);
+              ys[i] = kQuant ? fmaf(sc[i], f, sv - (i & 1 ? r1 : r0)) : xs[i];
             }
-            const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-            const float a0 = n0 == -INFINITY ? 1.f : ex2(m0 - n0), a1 = n1 == -INFINITY ? 1.f : ex2(m1 - n1);
-            m0 = n0;
-            m1 = n1;
-            l0 *= a0;
-            l1 *= a1;
+            if (!all) {
+              if (!seen(g)) xs[0] = xs[1] = ys[0] = ys[1] = -INFINITY;
+              if (!seen(g + 8)) xs[2] = xs[3] = ys[2] = ys[3] = -INFINITY;
+            }
+          };
+          refer(m0, m1, R0, R1);
+          float top = fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3]));
+          if constexpr (kQuant) top = fmaxf(top, fmaxf(fmaxf(ys[0], ys[1]), fmaxf(ys[2], ys[3])));
+          if (__any_sync(0xffffffffu, top > kRaise)) {
+            refer(0.f, 0.f, 0.f, 0.f);
+            const auto raised = [](float& ref, float a, float b) {  // the factor of what was summed before
+              float n = fmaxf(a, b);
+#pragma unroll
+              for (int off = 4; off < 32; off <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, off));
+              n = fmaxf(n, ref);
+              const float f = ex2(ref - n);
+              ref = n;
+              return f;
+            };
+            float b0 = raised(m0, xs[0], xs[2]), b1 = raised(m1, xs[1], xs[3]);
+            l0 *= b0;
+            l1 *= b1;
+            if constexpr (kQuant) {
+              b0 = raised(R0, ys[0], ys[2]);
+              b1 = raised(R1, ys[1], ys[3]);
+            }
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              o[k][0] *= a0;
-              o[k][1] *= a1;
-              o[k][2] *= a0;
-              o[k][3] *= a1;
+              o[k][0] *= b0;
+              o[k][1] *= b1;
+              o[k][2] *= b0;
+              o[k][3] *= b1;
             }
+            refer(m0, m1, R0, R1);
           }
-          const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
-          const float p0 = ex2(sc[0] - r0), p1 = ex2(sc[1] - r1), p2 = ex2(sc[2] - r0), p3 = ex2(sc[3] - r1);
-          if constexpr (kQuant) {
-            l0 = fmaf(p0, d0, fmaf(p2, d1, l0));
-            l1 = fmaf(p1, d0, fmaf(p3, d1, l1));
-          } else {
-            l0 += p0 + p2;
-            l1 += p1 + p3;
-          }
+          const float p0 = ex2(ys[0]), p1 = ex2(ys[1]), p2 = ex2(ys[2]), p3 = ex2(ys[3]);
+          l0 += kQuant ? ex2(xs[0]) + ex2(xs[2]) : p0 + p2;
+          l1 += kQuant ? ex2(xs[1]) + ex2(xs[3]) : p1 + p3;
           // ---- P^T as the B operand: lane (g, tig) needs keys 2 tig, + 1, + 8, + 9 of head g
           const uint32_t pr01 = pack2<kMmaBf16>(p0, p1), pr23 = pack2<kMmaBf16>(p2, p3);
           const int src = 8 * tig + (g >> 1);
@@ -404,6 +412,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (lane == 0) mbar_arrive(smem_u32(&S.empty[st]));
       }
       // ---- the four warps' states, merged; every consumer takes these barriers
+      if (!kQuant) R0 = m0, R1 = m1;
+      const auto known = [](float& ref) { ref = ref == kNone ? -INFINITY : ref; };  // nothing seen, or only NaN
+      known(m0), known(m1), known(R0), known(R1);
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, off);
@@ -414,18 +425,20 @@ __global__ void __launch_bounds__(kThreads, 2)
         S.mm[warp][2 * tig + 1] = m1;
         S.ml[warp][2 * tig] = l0;
         S.ml[warp][2 * tig + 1] = l1;
+        S.mr[warp][2 * tig] = R0;
+        S.mr[warp][2 * tig + 1] = R1;
       }
       if (consumers_any(!ok)) {
         ok = false;
         break;
       }
-      float M0 = -INFINITY, M1 = -INFINITY;
+      float M0 = -INFINITY, M1 = -INFINITY;  // of R
 #pragma unroll
       for (int x = 0; x < kConsumers; ++x) {
-        M0 = fmaxf(M0, S.mm[x][2 * tig]);
-        M1 = fmaxf(M1, S.mm[x][2 * tig + 1]);
+        M0 = fmaxf(M0, S.mr[x][2 * tig]);
+        M1 = fmaxf(M1, S.mr[x][2 * tig + 1]);
       }
-      const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - M0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - M1);
+      const float f0 = R0 == -INFINITY ? 0.f : ex2(R0 - M0), f1 = R1 == -INFINITY ? 0.f : ex2(R1 - M1);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         o[k][0] *= f0;
@@ -473,10 +486,20 @@ __global__ void __launch_bounds__(kThreads, 2)
           x[i + 2] = a.z + b.z;
           x[i + 3] = a.w + b.w;
         }
-        if (c.whole()) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;  // nothing seen: zeros
+        const float inv = L == 0.f ? 0.f : 1.f / L;  // nothing seen: zeros
+        if constexpr (kQuant) {
+          // the mean of V, of a piece too: 2^(R - M) in two halves, since R - M can pass f32's exponents
+          float R = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= inv;
+          for (int i = 0; i < kConsumers; ++i) R = fmaxf(R, S.mr[i][h]);
+          const float half = R == -INFINITY ? 0.f : ex2(0.5f * (R - M));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * half * half;
+        }
+        if (c.whole()) {
+          if constexpr (!kQuant)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= inv;
           T* out = reinterpret_cast<T*>(p.out) + (int64_t)c.q_first * p.out_stride_tok + (int64_t)(head0 + h) * p.out_stride_head + d;
           *reinterpret_cast<uint4*>(out) = make_uint4(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]),
                                                       pack2<kBf16>(x[4], x[5]), pack2<kBf16>(x[6], x[7]));
@@ -547,6 +570,7 @@ int launch_decode_sinks(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t 
   const int rc = plan_geometry(p, kHeads, kHeads, kTile, 2 * num_sms());
   if (rc != SNAPMIND_OK) return rc;
   p.tokens = 1;
+  p.means = pool_dtype == SNAPMIND_DTYPE_E4M3;
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
   if (dtype == SNAPMIND_DTYPE_BF16)
     return quant ? launch<__nv_bfloat16, true>(p, st) : launch<__nv_bfloat16, false>(p, st);

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import snapmind_b200._lib as lib
+from test_chunk_gpu import HALF, check, make_pool
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +42,54 @@ def test_device_counts_that_do_not_fit(cuda_device, counts, word):
     pool.err.zero_()
     assert reserve([24, 47, 14]) == 0  # up to the rows' ends and the last block
     assert pool.seq_lens.tolist() == [64, 48, 64] and int(pool.free_top.item()) == 0
+
+
+def set_exponents(pool, lens, k_exp, v_exp):
+    """Gives the rows of an 8-bit pool these exponents ([blocks, heads, slots]); the sequences' K and V in f64."""
+    _, _, heads, bs, d = pool.k.shape
+    kv = []
+    for i, (codes, e) in enumerate(((pool.k, k_exp), (pool.v, v_exp))):
+        keep = pool.scales[0, :, :, i] == 255  # slots without a token
+        pool.scales[0, :, :, i] = torch.where(keep, pool.scales[0, :, :, i], (e + 127).to(torch.uint8))
+        val = codes[0].double() * torch.exp2(e.double()).unsqueeze(-1)
+        kv.append([val[pool.block_tables[b, :(n + bs - 1) // bs].long()].permute(1, 0, 2, 3).reshape(heads, -1, d)[:, :n]
+                   for b, n in enumerate(lens)])
+    return kv
+
+
+def pick(g, values, shape):
+    return torch.tensor(values, device="cuda")[torch.randint(0, len(values), shape, generator=g, device="cuda")]
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 5)])
+@pytest.mark.parametrize("exps", [(-100, 40), (-99, 40), (-100, -60, -20, 20, 60, 100), tuple(range(-100, 101, 7))],
+                         ids=lambda e: f"{e[0]}..{e[-1]}x{len(e)}")
+@pytest.mark.parametrize("lens", [[2], [5000, 33, 1], [40000]], ids=str)
+def test_values_of_far_apart_scales(cuda_device, lens, exps, window, sinks):
+    """8-bit decode: every seen row counts in the softmax sum by its score alone, whatever the scale of its
+    values; in one tile, over a CTA's warps, and over many CTAs."""
+    pool, _, _ = make_pool(torch.bfloat16, lens, 2, 128, 16, 50, "e4m3")
+    g = torch.Generator(device="cuda").manual_seed(4)
+    shape = pool.scales.shape[1:3] + (16,)
+    v_exp = pick(g, exps, shape)
+    pool.v.view(torch.uint8)[0].masked_fill_((v_exp == -100).unsqueeze(-1) & (pool.scales[0, :, :, 1] != 255).unsqueeze(-1), 0)
+    ks, vs = set_exponents(pool, lens, pick(g, (-9, -8, -7), shape), v_exp)
+    q = torch.randn((len(lens), 8, 128), generator=g, device="cuda").bfloat16()
+    out = pool.decode(0, q, window=window, sinks=sinks)
+    pool.check()
+    check(out, q, list(range(len(lens) + 1)), ks, vs, window, sinks, HALF[torch.float16])
+
+
+def test_a_row_of_zeros_counts(cuda_device):
+    """Two keys of equal score, one with V = 0 (stored with the smallest exponent), one with V = 2^40: 2^39."""
+    from snapmind_b200 import QuantizedKVPool
+
+    pool = QuantizedKVPool(1, 1, 128, 4, 1, 2, dtype=torch.bfloat16)
+    pool.reserve(2, batch=1)
+    k = torch.zeros((1, 1, 2, 128), device="cuda").bfloat16()
+    v = k.clone()
+    v[0, 0, 1] = 2.0**40
+    pool.append(0, k, v)
+    out = pool.decode(0, torch.ones((1, 4, 128), device="cuda").bfloat16())
+    pool.check()
+    assert (out == 2.0**39).all()
