@@ -230,7 +230,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       // keys seen: [0, v_s) and [v_lo, v_len) of the virtual axis
       const int v_lo = kr.win_lo - kr.shift, v_s = p.window > 0 ? min(p.sinks, kr.v_sink) : 0;
       uint32_t qf[8][2];
-      float q0 = c2, q1 = c2;  // factors of heads 2 tig, 2 tig + 1
+      float q0 = c2, q1 = c2;            // factors of heads 2 tig, 2 tig + 1
+      uint32_t down0 = 0, down1 = 0;     // e4m3: powers of two (in exponent bits) that K's scales leave to them
       {
         const T* qrow = reinterpret_cast<const T*>(p.q) + (int64_t)c.q_first * p.q_stride_tok +
                         (int64_t)(head0 + min(g, heads - 1)) * p.q_stride_head;
@@ -252,9 +253,15 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int k = 0; k < 8; ++k)
 #pragma unroll
             for (int i = 0; i < 2; ++i) qf[k][i] = pack2<false>(x[4 * k + 2 * i] * up, x[4 * k + 2 * i + 1] * up);
-          const float f = c2 * __uint_as_float((uint32_t)(127 + e) << 23);  // of head g
+          // A sum of products is below 2^25 (128 x 448 x 2^9), K's scale at most 2^120: 2^17 of it goes
+          // to the head's factor, so that what overflows is a score, not a step towards one.  (A query above
+          // 2^110 has no room for it and needs none.)
+          const int down = e < 100 ? 17 : 0;
+          const float f = c2 * __uint_as_float((uint32_t)(127 + down + e) << 23);  // of head g
           q0 = __shfl_sync(0xffffffffu, f, 8 * tig);
           q1 = __shfl_sync(0xffffffffu, f, 8 * tig + 4);
+          down0 = __shfl_sync(0xffffffffu, (uint32_t)down << 23, 8 * tig);
+          down1 = __shfl_sync(0xffffffffu, (uint32_t)down << 23, 8 * tig + 4);
         } else {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
@@ -313,13 +320,13 @@ __global__ void __launch_bounds__(kThreads, 2)
               }
             }
             const uint8_t* bytes = &S.scales[st][0][16 * warp];
-            const float k0 = __uint_as_float((uint32_t)bytes[g] << 23), k1 = __uint_as_float((uint32_t)bytes[g + 8] << 23);
+            const uint32_t e0 = (uint32_t)bytes[g] << 23, e1 = (uint32_t)bytes[g + 8] << 23;
             sv0 = (float)((int)bytes[kTile + g] - 127);
             sv1 = (float)((int)bytes[kTile + g + 8] - 127);
-            sc[0] *= k0;
-            sc[1] *= k0;
-            sc[2] *= k1;
-            sc[3] *= k1;
+            sc[0] *= __uint_as_float(e0 - down0);
+            sc[1] *= __uint_as_float(e0 - down1);
+            sc[2] *= __uint_as_float(e1 - down0);
+            sc[3] *= __uint_as_float(e1 - down1);
           } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {

@@ -93,3 +93,21 @@ def test_a_row_of_zeros_counts(cuda_device):
     out = pool.decode(0, torch.ones((1, 4, 128), device="cuda").bfloat16())
     pool.check()
     assert (out == 2.0**39).all()
+
+
+@pytest.mark.parametrize("k_exp,size,scale", [
+    (126, 2.0**-109, 2.0**-20), (126, 2.0**-90, 2.0**-39), (112, 2.0**-109, None), (100, 2.0**-99, 40.0),
+    (-92, 2.0**97, None), (-92, 2.0**115, 2.0**-22), (90, 2.0**-92, 2.0**-10),
+])
+@pytest.mark.parametrize("generic", [False, True])
+def test_keys_of_far_scales(cuda_device, k_exp, size, scale, generic):
+    """8-bit decode of keys near the ends of the range and queries near the other end: scores of ordinary size."""
+    lens = [300, 65]
+    pool, _, _ = make_pool(torch.bfloat16, lens, 2, 128, 16, 51, "e4m3")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    shape = pool.scales.shape[1:3] + (16,)
+    ks, vs = set_exponents(pool, lens, pick(g, (k_exp - 8, k_exp - 7), shape), pick(g, (-9, -8), shape))
+    q = (size * torch.randn((2, 8, 128), generator=g, device="cuda")).bfloat16()
+    out = pool.decode(0, q, scale=scale, force_generic=generic)
+    pool.check()
+    check(out, q, [0, 1, 2], ks, vs, 0, 0, 0.0 if generic else HALF[torch.float16], scale)
