@@ -7,8 +7,8 @@
 //   S = Q K^T [128 x 128] (Q and K K-major), P = 2^(S c - m), O += P V (V MN-major).
 // Softmax and MMA of the two tiles alternate: while the tensor core works on one tile's
 // products, the other tile's 128 threads (one row each) take its scores.
-// A row keeps a reference maximum that is raised only when a score exceeds it by 2^8:
-// then O is rescaled in TMEM, else O is never touched between the products.
+// A row keeps a reference that is raised only when a score exceeds it by 2^8 (f16: 2^15): then O is
+// rescaled in TMEM, else O is never touched between the products.
 //   warps 0-3, 4-7  softmax of tile 0 / 1: thread = row = TMEM lane; they write P to shared memory,
 //                   and write out the finished rows
 //   warp 8          loads Q (one copy per tile and 64 columns: 128 threads fetching rows took 14000
@@ -51,7 +51,12 @@ constexpr int kConvert = 128;  // threads that convert e4m3 rows
 constexpr uint32_t kBlockBytes = 128 * 128;  // 128 rows of 64 16-bit elements
 constexpr uint32_t kPBytes = 2 * kBlockBytes;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescale = 8.f;  // log2 headroom of the reference maximum
+// A raised reference stands 2^kLow below the maximum, and stays until a score exceeds it by 2^kRescale.
+// f16 weights go up to 2^15: a weight 2^25 below a largest one of 1 would vanish, and the weights of
+// thousands of keys behind a strong sink lie there; 2^7 further up, a weight is off by 2^-32 of the
+// largest at most.
+template <typename T> constexpr float kLow = std::is_same<T, __half>::value ? 7.f : 0.f;
+template <typename T> constexpr float kRescale = kLow<T> + 8.f;
 
 template <int D, bool kQuant> struct Shape {
   static constexpr uint32_t kTileBytes = D / 64 * kBlockBytes;  // a Q tile, a K or V stage
@@ -558,10 +563,10 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) mx[i] = x + 4 + i < kKeys ? fmaxf(mx[i], fmaxf(s[x + i], s[x + 4 + i])) : fmaxf(mx[i], s[x + i]);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
-        const bool raise = top > m + kRescale;
+        const bool raise = top > m + kRescale<T>;
         if (__any_sync(0xffffffffu, raise)) {
-          const float alpha = raise ? ex2(m - top) : 1.f;
-          if (raise) m = top;
+          const float alpha = raise ? ex2(m - (top - kLow<T>)) : 1.f;
+          if (raise) m = top - kLow<T>;
           l *= alpha;
           if (step > step0) {  // O += P V of the group's tile before is done: O may change
             ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);

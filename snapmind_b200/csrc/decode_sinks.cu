@@ -36,7 +36,12 @@ using namespace tc;
 constexpr int kD = 128, kTile = 64, kConsumers = 4, kThreads = (kConsumers + 2) * 32, kHeads = 8;
 constexpr int kScaleLanes = kTile / 16;  // lanes that fetch a tile's scale bytes of K, or of V, 16 each
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRaise = 8.f;  // log2 headroom of the reference maxima
+// A raised reference stands 2^kLow below the maximum, and stays until a score passes it by 2^kRaise
+// (weights up to 2^kRaise are as good as those up to 1).  f16 weights go up to 2^15: what is 2^25
+// below the largest weight would vanish if that were 1, although thousands of such keys behind a
+// strong sink may be all that shows; 2^7 further up, a weight is off by 2^-32 of the largest at most.
+template <bool kBf16> constexpr float kLow = kBf16 ? 0.f : 7.f;
+template <bool kBf16> constexpr float kRaise = kLow<kBf16> + 8.f;
 constexpr float kNone = -3e38f;  // a reference before any score: finite, so that -infinity less it stays one
 
 template <bool kQuant> struct Stage {
@@ -335,9 +340,8 @@ __global__ void __launch_bounds__(kThreads, 2)
               mma16816<kMmaBf16>(sc, a, qf[k][0], qf[k][1]);
             }
           }
-          // Scores less their references: xs for the sum, ys for the weights (16-bit caches: xs).  A
-          // reference is raised only when a score passes it by 2^8 (weights up to 2^8 are as good as
-          // those up to 1): then to the exact maximum, and what was summed is rescaled.
+          // Scores less their references: xs for the sum, ys for the weights (16-bit caches: xs).  When a
+          // reference is raised, what was summed is rescaled.
           float xs[4], ys[4];
           const auto refer = [&](float M0, float M1, float r0, float r1) {
 #pragma unroll
@@ -354,13 +358,13 @@ __global__ void __launch_bounds__(kThreads, 2)
           refer(m0, m1, R0, R1);
           float top = fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3]));
           if constexpr (kQuant) top = fmaxf(top, fmaxf(fmaxf(ys[0], ys[1]), fmaxf(ys[2], ys[3])));
-          if (__any_sync(0xffffffffu, top > kRaise)) {
+          if (__any_sync(0xffffffffu, top > kRaise<kMmaBf16>)) {
             refer(0.f, 0.f, 0.f, 0.f);
             const auto raised = [](float& ref, float a, float b) {  // the factor of what was summed before
               float n = fmaxf(a, b);
 #pragma unroll
               for (int off = 4; off < 32; off <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, off));
-              n = fmaxf(n, ref);
+              n = fmaxf(n - kLow<kMmaBf16>, ref);
               const float f = ex2(ref - n);
               ref = n;
               return f;

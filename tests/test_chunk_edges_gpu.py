@@ -1,10 +1,13 @@
 """The chunk operators and the 8-bit cache at the ends of their ranges: counts from device memory,
 exponents far apart, masked infinities, bad block ids."""
+import math
+
+import numpy as np
 import pytest
 import torch
 
 import snapmind_b200._lib as lib
-from test_chunk_gpu import HALF, check, make_pool
+from test_chunk_gpu import DT, HALF, check, make_pool
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +114,43 @@ def test_keys_of_far_scales(cuda_device, k_exp, size, scale, generic):
     out = pool.decode(0, q, scale=scale, force_generic=generic)
     pool.check()
     check(out, q, [0, 1, 2], ks, vs, 0, 0, 0.0 if generic else HALF[torch.float16], scale)
+
+
+@pytest.mark.parametrize("dtype,cache,single,generic", [
+    ("f16", "same", True, False), ("f16", "same", False, False), ("bf16", "same", True, False), ("bf16", "same", False, False),
+    ("f16", "e4m3", True, False), ("f16", "e4m3", False, False), ("bf16", "e4m3", True, False), ("bf16", "e4m3", False, False),
+    ("f16", "same", False, True),
+])
+@pytest.mark.parametrize("n,drop", [(16384, 26), (5000, 24), (60000, 28)])
+def test_many_small_weights_behind_a_sink(cuda_device, dtype, cache, single, generic, n, drop):
+    """The first key has 2^drop times the weight of each other one, and V = 0: the others' sum is all there is.
+
+    want = (n - 1) 2^-drop / (1 + (n - 1) 2^-drop).  A weight is off by half a step of its type (2^-11 of it, bf16
+    2^-8) or, below f16's normal range, by 2^-32 of the largest weight; the score 2^8 scale by two roundings of
+    24 bits, 2^-18 of the result with 2^x; the output by half a step."""
+    from snapmind_b200 import PagedKVPool, QuantizedKVPool
+
+    dtype = DT[dtype]
+    t, nseq, hkv, blocks = 1 if single else 3, 40, 8, (n + 15) // 16
+    # 320 (sequence, kv head) pairs over one set of blocks: nearly every CTA goes through whole sequences
+    pool = (QuantizedKVPool if cache == "e4m3" else PagedKVPool)(1, hkv, 128, blocks, nseq, blocks, dtype=dtype)
+    pool.set_state(np.arange(blocks)[None].repeat(nseq, 0), np.full(nseq, n), np.arange(0))
+    k = torch.zeros((1, hkv, n, 128), device="cuda", dtype=dtype)
+    v = torch.ones_like(k)
+    k[:, :, 0, 3], v[:, :, 0] = 16.0, 0.0
+    pool.append(0, k, v)
+    q = torch.zeros((nseq * t, 2 * hkv, 128), device="cuda", dtype=dtype)
+    q[:, :, 3] = 16.0
+    scale = drop * math.log(2) / 256
+    if single:
+        out = pool.decode(0, q, scale=scale, window=1 << 20, force_generic=generic)
+    else:
+        cu = torch.arange(nseq + 1, dtype=torch.int32, device="cuda") * t
+        out = pool.attend_chunk(0, q, cu, scale=scale, force_generic=generic)
+    pool.check()
+    for i in range(t):
+        others = (n - t + i) * 2.0**-drop
+        want = others / (1 + others)
+        weights = HALF[torch.float16] if cache == "e4m3" and single else 0.0 if generic else HALF[dtype]
+        tol = want * (weights + HALF[dtype] * 1.01 + 2.0**-18) + (0 if generic else n * 2.0**-32)
+        assert (out[i::t].double() - want).abs().max() <= tol
