@@ -98,6 +98,7 @@ __device__ __forceinline__ bool out_vec(const ChunkParams& p) {
   return p.out_stride_tok % 4 == 0 && p.out_stride_head % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
 }
 
+// p.odd: a second go at a call of the tcgen05 kernel, which only some CTA's odd rows make necessary.
 template <typename T, typename KV, int D4>
 __global__ void __launch_bounds__(GenSmem<D4>::kThreads, GenSmem<D4>::kCtas) chunk_generic_kernel(ChunkParams p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -114,6 +115,7 @@ __global__ void __launch_bounds__(GenSmem<D4>::kThreads, GenSmem<D4>::kCtas) chu
   Smem& S = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, tx = tid % kTx, ty = tid / kTx;
   prior_grid_wait();
+  if (p.odd != nullptr && !any_odd(p)) return;
   plan_block(p, S.plan, reinterpret_cast<int32_t*>(S.q));
   const float c2 = p.scale * kLog2e;
   const int bs = p.block_size, hd = p.head_dim;
@@ -400,10 +402,9 @@ __device__ __forceinline__ void mul4(float4& a, float f) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkParams p) {
-  next_grid_may_launch();  // every block of this grid has started by then
-  prior_grid_wait();
+__device__ __forceinline__ void merge_units(const ChunkParams& p) {
   const int cta = blockIdx.x + 1;
+  if (cta >= p.n_ctas) return;
   const int4 h0 = *reinterpret_cast<const int4*>(p.heads + (int64_t)cta * kPieceInts);
   const int4 h1 = *reinterpret_cast<const int4*>(p.heads + (int64_t)cta * kPieceInts + 4);
   if (h0.x < 0 || h1.x != cta - 1) return;
@@ -523,8 +524,29 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
   }
 }
 
+template <typename T>
+__global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkParams p) {
+  next_grid_may_launch();  // every block of this grid has started by then
+  prior_grid_wait();
+  merge_units<T>(p);
+}
+// After a call that may have been done over: `again` merges the units of that.
+template <typename T>
+__global__ void __launch_bounds__(32 * kMergeWarps)
+    chunk_merge_either_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ ChunkParams again) {
+  next_grid_may_launch();
+  prior_grid_wait();
+  if (any_odd(again)) merge_units<T>(again);
+  else merge_units<T>(p);
+}
+
+dim3 merge_grid(const ChunkParams& p) {
+  const int used = p.gw * p.tokens;
+  return dim3(p.n_ctas - 1, (used + kMergeWarps * kMergeRows - 1) / (kMergeWarps * kMergeRows));
+}
+
 template <typename T, typename KV>
-int launch_generic(ChunkParams& p, cudaStream_t st) {
+int launch_generic(const ChunkParams& p, cudaStream_t st) {
   const auto go = [&](auto kernel, int threads, size_t smem, bool (&done)[kMaxDevices]) -> int {
     const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem, done);
     if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
@@ -538,19 +560,42 @@ int launch_generic(ChunkParams& p, cudaStream_t st) {
   return go(chunk_generic_kernel<T, KV, 4>, GenSmem<4>::kThreads, sizeof(GenSmem<4>), done[2]);
 }
 
+int plan_generic(ChunkParams& p) {
+  return plan_geometry(p, kRows, kRows, kKeys, num_sms() * (p.head_dim <= 64 ? GenSmem<1>::kCtas : 1));
+}
+
+// The tcgen05 kernel, then the CUDA-core kernel over the same call, which returns at once unless a
+// CTA of the first met rows that f16 does not hold, then one merge for both.
+int launch_f16_over_e4m3(ChunkParams& p, cudaStream_t st) {
+  ChunkParams again = p;
+  int rc = plan_generic(again);
+  if (rc == SNAPMIND_OK) rc = launch_chunk_umma(p, SNAPMIND_DTYPE_F16, SNAPMIND_DTYPE_E4M3, st);
+  if (rc != SNAPMIND_OK) return rc;
+  again.n_odd = p.n_ctas;
+  rc = launch_generic<__half, uint8_t>(again, st);
+  if (rc != SNAPMIND_OK) return rc;
+  const dim3 a = merge_grid(p), b = merge_grid(again);
+  return cuda_status(launch_dependent(chunk_merge_either_kernel<__half>, dim3(a.x > b.x ? a.x : b.x, a.y > b.y ? a.y : b.y),
+                                      32 * kMergeWarps, 0, st, p, again),
+                     "paged_chunk merge");
+}
+
 // The largest workspace of the kernels: one CTA per SM with units of 256 rows, or three with 64.
 int64_t max_ctas() { return num_sms(); }
 constexpr int kMaxRows = 256;
 static_assert(3 * kRows <= kMaxRows, "three CTAs per SM");
+int64_t partials_bytes(int head_dim) {
+  ChunkParams p = {};
+  p.head_dim = head_dim;
+  return plan_workspace(p, nullptr, 2 * max_ctas(), kMaxRows / 2);
+}
 
 }  // namespace
 
 int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st) {
   if (p.n_ctas < 2) return SNAPMIND_OK;
-  const int used = p.gw * p.tokens;
-  const dim3 grid(p.n_ctas - 1, (used + kMergeWarps * kMergeRows - 1) / (kMergeWarps * kMergeRows));
   const auto go = [&](auto kernel) {
-    return cuda_status(launch_dependent(kernel, grid, 32 * kMergeWarps, 0, st, p), "paged_chunk merge");
+    return cuda_status(launch_dependent(kernel, merge_grid(p), 32 * kMergeWarps, 0, st, p), "paged_chunk merge");
   };
   switch (dtype) {
     case SNAPMIND_DTYPE_F32: return go(chunk_merge_kernel<float>);
@@ -567,9 +612,7 @@ extern "C" {
 
 int64_t snapmind_paged_gqa_chunk_workspace_bytes(int32_t head_dim) {
   if (head_dim <= 0 || head_dim > kGenMaxD) return 0;
-  ChunkParams p = {};
-  p.head_dim = head_dim;
-  return plan_workspace(p, nullptr, 2 * max_ctas(), kMaxRows / 2);
+  return partials_bytes(head_dim) + (max_ctas() * 4 + 255) / 256 * 256;
 }
 
 int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stride_head, int dtype, const void* k_pool,
@@ -631,6 +674,7 @@ int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stri
                      "paged_chunk: workspace needs %lld bytes on a 256-byte boundary, got %lld", (long long)need,
                      (long long)workspace_bytes);
   p.workspace = workspace;
+  p.odd = nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
   if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && decode_sinks_supported(p, dtype, pool_dtype)) {
@@ -638,11 +682,16 @@ int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stri
     return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
   }
   if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && chunk_umma_supported(p, dtype, pool_dtype)) {
+    if (quant && dtype == SNAPMIND_DTYPE_F16) {
+      p.odd = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + partials_bytes(head_dim));
+      const int rc = launch_f16_over_e4m3(p, st);
+      if (rc != SNAPMIND_ERR_UNSUPPORTED) return rc;
+      p.odd = nullptr;
+    }
     const int rc = launch_chunk_umma(p, dtype, pool_dtype, st);
     if (rc != SNAPMIND_ERR_UNSUPPORTED) return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
   }
-  const int ctas = num_sms() * (head_dim <= 64 ? GenSmem<1>::kCtas : 1);
-  int rc = plan_geometry(p, kRows, kRows, kKeys, ctas);
+  int rc = plan_generic(p);
   if (rc != SNAPMIND_OK) return rc;
   switch (dtype) {
     case SNAPMIND_DTYPE_F32: rc = quant ? launch_generic<float, uint8_t>(p, st) : launch_generic<float, float>(p, st); break;

@@ -85,6 +85,7 @@ struct Ctrl {
   uint64_t v_ready[2];  // MMA warp: V of an edge tile has landed (its unseen rows may be zeroed)
   uint32_t tmem_base;
   int32_t abort;
+  int32_t odd;  // f16 over e4m3: a row that f16 does not hold was met
   PlanShared plan;
   alignas(16) uint8_t scales[2][128];
   float2 ml[128];
@@ -173,11 +174,11 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* x) {
                : "memory");
 }
 
-// 16 e4m3 codes of one row times 2^(byte - 127), as 16 elements of T.  The scale is a power
-// of two: exact in bf16, and in f16 as long as the value is a normal f16.
+// 16 e4m3 codes of one row times 2^(byte - 127), as 16 elements of T.  The scale is a power of two:
+// exact in bf16, and in f16 unless odd_row says otherwise.
 template <typename T>
-__device__ __forceinline__ void dequant16(const uint4& codes, uint8_t byte, uint4& lo, uint4& hi) {
-  const float s = __uint_as_float((uint32_t)byte << 23);
+__device__ __forceinline__ void dequant16(const uint4& codes, uint32_t byte, uint4& lo, uint4& hi) {
+  const float s = __uint_as_float(byte << 23);
   const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
   uint32_t o[8];
 #pragma unroll
@@ -189,14 +190,28 @@ __device__ __forceinline__ void dequant16(const uint4& codes, uint8_t byte, uint
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const float2 f = mul2(__half22float2(*reinterpret_cast<const __half2*>(&h[j])), s);
-      if constexpr (std::is_same<T, __half>::value)  // hold to f16's range, keep NaN
-        o[i + j] = pack2<T>(fabsf(f.x) > 65504.f ? copysignf(65504.f, f.x) : f.x, fabsf(f.y) > 65504.f ? copysignf(65504.f, f.y) : f.y);
-      else
-        o[i + j] = pack2<T>(f.x, f.y);
+      o[i + j] = pack2<T>(f.x, f.y);
     }
   }
   lo = make_uint4(o[0], o[1], o[2], o[3]);
   hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// f16 over e4m3 rows.  K is staged times 2^5, which the scores' factor takes back, so that f16 holds
+// it exactly for exponents from -20 (its smallest code is 2^-9 and f16's smallest number 2^-24) to 2
+// (largest values of a row from 2e-4 to 1800); V as it is, for exponents up to 7, and up to 8 unless
+// its values pass f16's largest.  (Smaller V lose at most 2^-25, half a step of the smallest f16 output.)
+// A row outside that, zeros aside, makes the call odd: its results are of no use, and the CUDA-core
+// kernel, which takes any exponent, does the call over.
+template <typename T, bool kQuant> constexpr int kKeyUp = kQuant && std::is_same<T, __half>::value ? 5 : 0;
+__device__ __forceinline__ bool odd_byte(int kv, uint32_t byte) { return kv == 0 ? byte - 107u > 22u : byte > 134u; }
+__device__ __forceinline__ bool odd_row(int kv, const uint4& codes, const uint4& lo, const uint4& hi) {
+  if (kv == 0) return ((codes.x | codes.y | codes.z | codes.w) & 0x7F7F7F7Fu) != 0;
+  const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  uint32_t top = 0;  // an exponent of all ones carries into the sign's place
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top |= (w[i] & 0x7C007C00u) + 0x04000400u;
+  return (top & 0x80008000u) != 0;
 }
 
 // The third warpgroup (e4m3: and the fourth) gives up registers that the softmax threads, with a row
@@ -245,7 +260,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     mbar_init(smem_u32(&C.q_full), 1);
     mbar_init(smem_u32(&C.x_ml), 128);
     mbar_init(smem_u32(&C.x_done), 128);
-    C.abort = 0;
+    C.abort = C.odd = 0;
     mbar_init_fence();
   }
   if (warp == Ro::kScores) {
@@ -300,13 +315,16 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
 #pragma unroll 1
           for (int r = r0; r < 128; r += kRowsPass) {
             uint4 codes = *reinterpret_cast<const uint4*>(raw + r * D);
-            uint8_t byte = C.scales[kv][r];
+            uint32_t byte = C.scales[kv][r];
             if (edges && edge.unseen(v0 + r)) {  // seen by no query of the unit: zeros, whatever lies there
               codes = make_uint4(0, 0, 0, 0);
               byte = 127;
             }
             uint4 lo, hi;
-            dequant16<T>(codes, byte, lo, hi);
+            dequant16<T>(codes, byte + (kv == 0 ? kKeyUp<T, kQuant> : 0), lo, hi);
+            if constexpr (std::is_same<T, __half>::value) {
+              if (odd_byte(kv, byte) && odd_row(kv, codes, lo, hi)) C.odd = 1;
+            }
             uint8_t* row = dst + (r >> 3) * Sh::kGroup + (r & 7) * 128;
             const uint32_t sw = r & 7;
             // lanes of the two 64-element halves write opposite pieces: no bank is hit twice
@@ -492,7 +510,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     const uint32_t lanes = ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t t_s = tmem + lanes + t * kKeys, t_o = tmem + lanes + 2 * kKeys + t * D;
     const bool flip = p.scale < 0.f;  // then the scores change sign: the largest has the largest weight
-    const float c2 = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
+    const float c2 = fmaxf(fabsf(p.scale) * (kLog2e / (1 << kKeyUp<T, kQuant>)), 1e-37f);
     uint8_t* prow = p_s + r * 128;
     const uint32_t sw = (uint32_t)(r & 7);
     uint32_t step = 0, tiles = 0, edges = 0, splits = 0, other_steps = 0;
@@ -701,7 +719,10 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (tid == 0) write_piece_info(p, C.plan);
+  if (tid == 0) {
+    write_piece_info(p, C.plan);
+    if (p.odd != nullptr) p.odd[blockIdx.x] = C.odd;
+  }
   next_grid_may_launch();
   if (warp == Ro::kScores) {
     tc_fence_after();

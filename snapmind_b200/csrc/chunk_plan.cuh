@@ -48,6 +48,8 @@ struct ChunkParams {
   int32_t* heads;   // workspace: [n_ctas][kPieceInts], see PieceInfo
   float* part_ml;   // workspace: [n_ctas][2][rows][2] maximum (log2 units), sum
   float* part_o;    // workspace: [n_ctas][2][rows][head_dim]
+  int32_t* odd;     // workspace: [n_odd] whether a CTA met rows that its kernel's types do not hold, or NULL
+  int32_t n_odd;
   int32_t means;    // part_o holds a piece's weighted means of V (else its weighted sums)
   int32_t* err;
 };
@@ -419,6 +421,14 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Whether some CTA of the tcgen05 kernel before met such rows (then the CUDA-core kernel does the call
+// over); every thread of the block calls it.
+__device__ __forceinline__ bool any_odd(const ChunkParams& p) {
+  int x = 0;
+  for (int i = threadIdx.x; i < p.n_odd; i += blockDim.x) x |= p.odd[i];
+  return __syncthreads_or(x) != 0;
+}
+
 // chunk_attn.cu: merges the cut units, after the attention kernel on the stream.
 int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st);
 
@@ -470,7 +480,7 @@ inline int64_t plan_workspace(ChunkParams& p, void* workspace, int64_t n_ctas, i
   p.heads = reinterpret_cast<int32_t*>(w);
   p.part_ml = reinterpret_cast<float*>(w + ml_off);
   p.part_o = reinterpret_cast<float*>(w + o_off);
-  return o_off + n_ctas * 2 * rows * p.head_dim * 4;
+  return (o_off + n_ctas * 2 * rows * p.head_dim * 4 + 255) / 256 * 256;
 }
 
 // Unit geometry for kernels of `rows` query rows in tiles of `tile_rows` (whole tokens each),

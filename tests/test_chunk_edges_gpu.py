@@ -154,3 +154,41 @@ def test_many_small_weights_behind_a_sink(cuda_device, dtype, cache, single, gen
         weights = HALF[torch.float16] if cache == "e4m3" and single else 0.0 if generic else HALF[dtype]
         tol = want * (weights + HALF[dtype] * 1.01 + 2.0**-18) + (0 if generic else n * 2.0**-32)
         assert (out[i::t].double() - want).abs().max() <= tol
+
+
+@pytest.mark.parametrize("generic", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("k_exps,v_exps,size", [
+    ((-20, -8, 2), (-15, -3, 7), 1.0),            # what f16 holds
+    ((-9, -8, -21), (-9,), 2.0**13),              # K below it, queries that bring it back
+    ((-40, -39), (-9,), 2.0**13),
+    ((-100, 3, 8), (-9, -100), 2.0**-14),         # K above it
+    ((-9, -8), (-60, -24, -9), 1.0),              # V below it: lost in an f16 output too
+    ((-9, -8), (-9, 8), 1.0),                     # V above it in one row, outputs that f16 holds
+    ((-9, -8), (-9, 15), 1.0),
+], ids=str)
+def test_f16_queries_over_any_exponent(cuda_device, d, k_exps, v_exps, size, generic):
+    """Chunks of f16 queries over 8-bit rows that f16 does not hold, one such row among a thousand too: the rows'
+    values count as they are stored."""
+    lens, new = [900, 130, 40], [70, 130, 0]
+    pool, _, _ = make_pool(torch.float16, lens, 2, d, 16, 52, "e4m3")
+    g = torch.Generator(device="cuda").manual_seed(7)
+    shape = pool.scales.shape[1:3] + (16,)
+    cu = [0, 70, 200, 200]
+    cud = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    for rare in (False, True) if max(v_exps) < 8 else (True,):
+        k_exp, v_exp = pick(g, k_exps, shape), pick(g, v_exps, shape)
+        if rare:  # ordinary rows, but for one
+            one = torch.zeros(shape, dtype=torch.bool, device="cuda")
+            one[int(pool.block_tables[0, 20]), 1, 7] = True
+            k_exp, v_exp = torch.where(one, k_exps[-1], -9), torch.where(one, v_exps[-1], -9)
+        ks, vs = set_exponents(pool, lens, k_exp, v_exp)
+        q = (size * torch.randn((200, 8, d), generator=g, device="cuda")).half()
+        scale = 0.1 / (size * float(max(k.abs().max() for k in ks)))
+        out = pool.attend_chunk(0, q, cud, scale=scale, force_generic=generic)
+        pool.check()
+        check(out, q, cu, ks, vs, 0, 0, 0.0 if generic else HALF[torch.float16], scale)
+        # a token each, as a decode step
+        out = pool.decode(0, q[:3], scale=scale, force_generic=generic)
+        check(out, q[:3], [0, 1, 2, 3], ks, vs, 0, 0, HALF[torch.float16], scale)
+    pool.check()
