@@ -162,7 +162,18 @@ class PagedKVPool(BlockPool):
         return self._attend(layer, q, cu_q, out, scale, window, sinks,
                             _lib.DECODE_FORCE_GENERIC if force_generic else 0)
 
-    def _attend(self, layer, q, cu, out, scale, window, sinks, flags):
+    def _attend_tokens(self, layer, q, out, scale, batch, window, sinks, force_generic, append):
+        """One query per sequence for the first ``batch`` sequences, their newest token stored first if given."""
+        if batch is not None:
+            q = q[:batch]
+        if append is not None:
+            want = (q.shape[0], self.n_kv_heads, self.head_dim)
+            if append[0].shape != want or append[1].shape != want:
+                raise ValueError(f"append rows must be {list(want)}, got {tuple(append[0].shape)} and {tuple(append[1].shape)}")
+        return self._attend(layer, q, None, out, scale, window, sinks,
+                            _lib.DECODE_FORCE_GENERIC if force_generic else 0, append)
+
+    def _attend(self, layer, q, cu, out, scale, window, sinks, flags, append=None):
         total, n_q, d = q.shape
         if q.dtype != self.dtype:
             raise TypeError(f"q dtype {q.dtype} != pool dtype {self.dtype}")
@@ -184,6 +195,8 @@ class PagedKVPool(BlockPool):
             if out.shape != q.shape or out.dtype != self.dtype or o_st[2] != 1:
                 raise ValueError("out must have q's shape and dtype, head dim contiguous")
         _lib.require_same("attend", self.block_tables, q, out)
+        if append is not None:
+            self.append(layer, *append)
         lib = _lib.load()
         # a workspace of its own for every call: calls on several streams, or in several
         # captured graphs, never share one
@@ -318,10 +331,7 @@ class PagedKVPool(BlockPool):
         if window or sinks:
             if peers is not None:
                 raise ValueError("decode with a window has no peer form")
-            if append is not None:
-                self.append(layer, *append)
-            flags = _lib.DECODE_FORCE_GENERIC if force_generic else 0
-            return self._attend(layer, q if batch is None else q[:batch], None, out, scale, window, sinks, flags)
+            return self._attend_tokens(layer, q, out, scale, batch, window, sinks, force_generic, append)
         batch = q.shape[0] if batch is None else batch
         n_q = q.shape[1]
         if peers is not None and append is not None:

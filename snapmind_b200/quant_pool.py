@@ -89,10 +89,7 @@ class QuantizedKVPool(PagedKVPool):
         have no use: the kernel plans from the device lengths)."""
         if peers is not None:
             raise ValueError("QuantizedKVPool: decode has no peer form")
-        if append is not None:
-            self.append(layer, *append)
-        flags = _lib.DECODE_FORCE_GENERIC if force_generic else 0
-        return self._attend(layer, q if batch is None else q[:batch], None, out, scale, window, sinks, flags)
+        return self._attend_tokens(layer, q, out, scale, batch, window, sinks, force_generic, append)
 
     def decode_layers(self, *args, **kwargs):
         raise NotImplementedError("QuantizedKVPool: decode one layer at a time")

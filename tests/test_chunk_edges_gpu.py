@@ -192,3 +192,23 @@ def test_f16_queries_over_any_exponent(cuda_device, d, k_exps, v_exps, size, gen
         out = pool.decode(0, q[:3], scale=scale, force_generic=generic)
         check(out, q[:3], [0, 1, 2, 3], ks, vs, 0, 0, HALF[torch.float16], scale)
     pool.check()
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_decode_stores_tokens_of_its_own_batch_only(cuda_device, cache):
+    """decode(append=, window=): rows of another number of sequences or another shape are refused, as without a
+    window, and so is the whole call when its queries are; nothing is stored then."""
+    pool, _, _ = make_pool(torch.bfloat16, [70, 31, 50], 2, 128, 16, 42, cache, spare=4)
+    pool.reserve(1, batch=2)
+    kept = [pool.k.view(torch.uint8).clone(), pool.v.view(torch.uint8).clone()]
+    kv = torch.randn((3, 2, 128), device="cuda").bfloat16()
+    q = torch.randn((3, 8, 128), device="cuda").bfloat16()
+    for bad in ((kv, kv), (kv[:2], kv), (kv[:2], kv[:1]), (kv[:2, :1], kv[:2, :1])):
+        with pytest.raises(ValueError):
+            pool.decode(0, q, append=bad, window=40, batch=2)
+    with pytest.raises(ValueError):
+        pool.decode(0, q[:2], append=(kv, kv), window=40)
+    with pytest.raises(TypeError):
+        pool.decode(0, q.half(), append=(kv[:2], kv[:2]), window=40, batch=2)
+    pool.check()
+    assert torch.equal(kept[0], pool.k.view(torch.uint8)) and torch.equal(kept[1], pool.v.view(torch.uint8))
