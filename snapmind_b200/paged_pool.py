@@ -164,14 +164,18 @@ class PagedKVPool(BlockPool):
 
     def _attend_tokens(self, layer, q, out, scale, batch, window, sinks, force_generic, append):
         """One query per sequence for the first ``batch`` sequences, their newest token stored first if given."""
+        rows = out
         if batch is not None:
-            q = q[:batch]
+            if not 0 <= batch <= q.shape[0]:
+                raise ValueError(f"decode: batch {batch} of {q.shape[0]} queries")
+            q, rows = q[:batch], None if out is None else out[:batch]
         if append is not None:
             want = (q.shape[0], self.n_kv_heads, self.head_dim)
             if append[0].shape != want or append[1].shape != want:
                 raise ValueError(f"append rows must be {list(want)}, got {tuple(append[0].shape)} and {tuple(append[1].shape)}")
-        return self._attend(layer, q, None, out, scale, window, sinks,
-                            _lib.DECODE_FORCE_GENERIC if force_generic else 0, append)
+        got = self._attend(layer, q, None, rows, scale, window, sinks,
+                           _lib.DECODE_FORCE_GENERIC if force_generic else 0, append)
+        return got if out is None else out
 
     def _attend(self, layer, q, cu, out, scale, window, sinks, flags, append=None):
         total, n_q, d = q.shape

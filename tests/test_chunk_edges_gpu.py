@@ -212,3 +212,22 @@ def test_decode_stores_tokens_of_its_own_batch_only(cuda_device, cache):
         pool.decode(0, q.half(), append=(kv[:2], kv[:2]), window=40, batch=2)
     pool.check()
     assert torch.equal(kept[0], pool.k.view(torch.uint8)) and torch.equal(kept[1], pool.v.view(torch.uint8))
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_decode_of_the_first_sequences(cuda_device, cache):
+    """batch= with queries and an output buffer for the whole pool, as without a window: the rows behind stay."""
+    lens = [70, 31, 50]
+    pool, ks, vs = make_pool(torch.bfloat16, lens, 2, 128, 16, 42, cache)
+    q = torch.randn((3, 8, 128), device="cuda").bfloat16()
+    out = torch.full_like(q, 7.0)
+    assert pool.decode(0, q, out=out, window=40, sinks=1, batch=2) is out
+    pool.check()
+    check(out[:2], q[:2], [0, 1, 2], ks[:2], vs[:2], 40, 1, 2.0**-8)
+    assert (out[2] == 7.0).all()
+    assert pool.decode(0, q, window=40, batch=0).shape == (0, 8, 128)
+    for batch in (4, -1):
+        with pytest.raises(ValueError):
+            pool.decode(0, q, window=40, batch=batch)
+    with pytest.raises(ValueError):
+        pool.decode(0, q, out=out[:1], window=40, batch=2)
