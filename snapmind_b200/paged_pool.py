@@ -24,6 +24,9 @@ from snapmind_b200 import _lib
 from snapmind_b200.block_pool import BlockPool
 
 
+_FAR = 1 << 30  # no position is as far
+
+
 class PagedKVPool(BlockPool):
     quantised = False  # pool elements are the values themselves
 
@@ -201,6 +204,8 @@ class PagedKVPool(BlockPool):
         _lib.require_same("attend", self.block_tables, q, out)
         if append is not None:
             self.append(layer, *append)
+        if not (-1 <= window <= _FAR and -1 <= sinks <= _FAR):  # the C entry takes 32 bits
+            window, sinks = (max(-1, min(x, _FAR)) for x in (window, sinks))
         lib = _lib.load()
         # a workspace of its own for every call: calls on several streams, or in several
         # captured graphs, never share one

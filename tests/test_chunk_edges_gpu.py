@@ -231,3 +231,21 @@ def test_decode_of_the_first_sequences(cuda_device, cache):
             pool.decode(0, q, window=40, batch=batch)
     with pytest.raises(ValueError):
         pool.decode(0, q, out=out[:1], window=40, batch=2)
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_windows_past_32_bits(cuda_device, cache):
+    """Windows and sinks of 2^31 and more are what they say, not their lowest bits; negative ones are refused."""
+    lens = [70, 31]
+    pool, ks, vs = make_pool(torch.bfloat16, lens, 2, 128, 16, 42, cache)
+    q = torch.randn((2, 8, 128), device="cuda").bfloat16()
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    for window, sinks in ((2**31, 0), (2**32 + 5, 2), (2**64 + 5, 2**40), (5, 2**32 + 1)):
+        for out in (pool.decode(0, q, window=window, sinks=sinks), pool.attend_chunk(0, q, cu, window=window, sinks=sinks)):
+            check(out, q, [0, 1, 2], ks, vs, 0, 0, 2.0**-8)
+    for window, sinks in ((-(2**32) + 5, 0), (5, -(2**32) + 1), (-(2**31), 0)):
+        with pytest.raises(ValueError, match="negative"):
+            pool.attend_chunk(0, q, cu, window=window, sinks=sinks)
+        with pytest.raises(ValueError, match="negative"):
+            pool.decode(0, q, window=window, sinks=sinks)
+    pool.check()
