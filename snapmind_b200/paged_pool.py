@@ -180,7 +180,8 @@ class PagedKVPool(BlockPool):
                            _lib.DECODE_FORCE_GENERIC if force_generic else 0, append)
         return got if out is None else out
 
-    def _attend(self, layer, q, cu, out, scale, window, sinks, flags, append=None):
+    def _attend(self, layer, q, cu, out, scale, window, sinks, flags, append=None, row=None):
+        """``row``: ``(table, length)`` pointers of the one sequence, in place of the pool's own tables and lengths."""
         total, n_q, d = q.shape
         if q.dtype != self.dtype:
             raise TypeError(f"q dtype {q.dtype} != pool dtype {self.dtype}")
@@ -216,8 +217,9 @@ class PagedKVPool(BlockPool):
         with self._on_device():
             status = lib.snapmind_paged_gqa_chunk(
                 q.data_ptr(), q_st[0], q_st[1], self._dcode, self.k.data_ptr() + step,
-                self.v.data_ptr() + step, scales, self._pool_code, self.block_tables.data_ptr(),
-                self.max_blocks_per_seq, self.max_blocks_per_seq, self.seq_lens.data_ptr(),
+                self.v.data_ptr() + step, scales, self._pool_code,
+                self.block_tables.data_ptr() if row is None else row[0],
+                self.max_blocks_per_seq, self.max_blocks_per_seq, self.seq_lens.data_ptr() if row is None else row[1],
                 None if cu is None else cu.data_ptr(), out.data_ptr(), o_st[0], o_st[1],
                 d ** -0.5 if scale is None else scale, total if cu is None else cu.shape[0] - 1, total, n_q,
                 self.n_kv_heads, d, self.block_size, self.num_blocks, window, sinks, flags, ws.data_ptr(), need,

@@ -96,12 +96,13 @@ class QuantizedKVPool(PagedKVPool):
 
     def attend_causal(self, layer: int, b: int, q: torch.Tensor, out: torch.Tensor, n_b: int,
                       scale: float | None = None) -> torch.Tensor:
-        """``PagedKVPool.attend_causal`` (``q``/``out`` ``[Hq, T, D]``) through ``attend_chunk``;
-        ``n_b`` has to be the sequence's length."""
+        """``PagedKVPool.attend_causal`` (``q``/``out`` ``[Hq, T, D]``, the sequence's first ``n_b`` tokens, the
+        newest T of them the queries') as a chunk of one sequence."""
         n_t = q.shape[1]
         if n_t == 0:
             return out
-        cu = torch.zeros(b + 2, dtype=torch.int32, device=self.device)
-        cu[b + 1] = n_t
-        self.attend_chunk(layer, q.transpose(0, 1), cu, out=out.transpose(0, 1), scale=scale)
+        cu = torch.zeros(2, dtype=torch.int32, device=self.device)
+        cu[1] = n_t
+        row = self.block_tables[b].data_ptr(), self._lens_ladder(n_b).data_ptr() + 4 * (n_b - 1)
+        self._attend(layer, q.transpose(0, 1), cu, out.transpose(0, 1), scale, 0, 0, 0, row=row)
         return out

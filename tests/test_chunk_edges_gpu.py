@@ -249,3 +249,27 @@ def test_windows_past_32_bits(cuda_device, cache):
         with pytest.raises(ValueError, match="negative"):
             pool.decode(0, q, window=window, sinks=sinks)
     pool.check()
+
+
+def test_attend_causal_of_any_sequence_and_length(cuda_device):
+    """QuantizedKVPool.attend_causal: a sequence past the 8192nd, and n_b below the length."""
+    from snapmind_b200 import QuantizedKVPool
+
+    pool = QuantizedKVPool(1, 2, 128, 8, 8200, 6, dtype=torch.bfloat16)
+    tables = np.zeros((8200, 6), np.int64)
+    tables[8197], tables[3] = [5, 1, 0, 7, 2, 4], [3, 6, 0, 0, 0, 0]
+    lens = np.zeros(8200, np.int64)
+    lens[8197], lens[3] = 77, 20
+    pool.set_state(tables, lens, np.arange(0))
+    codes = (64 * torch.randn((2, 77, 128), device="cuda")).clamp(-448, 448).to(torch.float8_e4m3fn)
+    pool.scales.fill_(127 - 6)
+    for t in range(77):
+        for p in (pool.k, pool.v):
+            p.view(torch.uint8)[0, tables[8197, t // 16], :, t % 16] = codes.view(torch.uint8)[:, t]
+    held = codes.double() / 64
+    q = torch.randn((8, 9, 128), device="cuda").bfloat16()
+    for n_b in (77, 41, 9):
+        out = torch.empty_like(q)
+        assert pool.attend_causal(0, 8197, q, out, n_b) is out
+        pool.check()
+        check(out.transpose(0, 1), q.transpose(0, 1), [0, 9], [held[:, :n_b]], [held[:, :n_b]], 0, 0, 2.0**-8)
