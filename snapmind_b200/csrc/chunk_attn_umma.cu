@@ -85,6 +85,11 @@ struct Ctrl {
   uint64_t v_ready[2];  // MMA warp: V of an edge tile has landed (its unseen rows may be zeroed)
   uint32_t tmem_base;
   int32_t abort;
+  // A K tile i with parts whose table entry is no block: its number and a bit per lost key, at i % 8.  (Its
+  // scores are read before the loading warp is 8 tiles on: it waits for the products of 4 tiles ago, which
+  // wait for the softmax threads to have read scores.)
+  uint32_t lost_tile[8], lost[8][4];
+  int32_t any_lost;  // there was one
   int32_t odd;  // f16 over e4m3: a row that f16 does not hold was met
   PlanShared plan;
   alignas(16) uint8_t scales[2][128];
@@ -106,6 +111,20 @@ __device__ __forceinline__ bool role_wait(const Ctrl& C, uint32_t bar, uint32_t 
     if (clock64() - t0 > kWaitTicks) return false;
   }
   return true;
+}
+// Rare, so not inlined: one bit per key of the parts `missing` (2^log_box keys each) of tile `tile`.
+__device__ __noinline__ void mark_lost(Ctrl& C, uint32_t tile, uint32_t missing, int log_box) {
+  if (!C.any_lost)
+    for (int i = 0; i < 8; ++i) C.lost_tile[i] = ~0u;
+  uint32_t* lost = C.lost[tile % 8];
+#pragma unroll 1
+  for (int key = 0; key < kKeys; key += 8) {
+    if (key % 32 == 0) lost[key / 32] = 0;
+    if (missing >> (key >> log_box) & 1) lost[key / 32] |= 0xFFu << (key % 32);
+  }
+  C.lost_tile[tile % 8] = tile;
+  __threadfence_block();
+  C.any_lost = 1;
 }
 __device__ __forceinline__ void give_up(Ctrl& C, int32_t* err) {
   atomicExch(&C.abort, 1);
@@ -261,6 +280,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     mbar_init(smem_u32(&C.x_ml), 128);
     mbar_init(smem_u32(&C.x_done), 128);
     C.abort = C.odd = 0;
+    C.any_lost = 0;
     mbar_init_fence();
   }
   if (warp == Ro::kScores) {
@@ -348,7 +368,8 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       for (; on && ok; on = w.next(p)) {
         const Piece& c = w.c;
         const KeyRange kr = key_range(p, c.len, c.n, c.i0, min(c.n, c.i0 + p.tokens));
-        TileRows at(p, kr, c, lane);
+        // a part whose entry is no block is a copy from past the pool: zeros, not what the stage held
+        TileRows at(p, kr, c, lane, p.num_blocks * p.n_kv_heads * p.block_size);
         const int box = at.box;
         for (int tile = c.tile0; tile < c.tile1; ++tile, ++issued) {
           at.advance(tile);
@@ -358,12 +379,18 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
           if (!ok) break;
           const uint32_t bar = smem_u32(kQuant ? &C.raw_full[kv] : &C.full[kv][st]);
           constexpr uint32_t kRowBytes = kQuant ? D : 2 * D;
+          const uint32_t missing = at.missing(tile);
+          if (kv == 0 && missing != 0 && leader) mark_lost(C, issued, missing, 7 - at.log_parts);
           mbar_arrive_expect_tx_p(leader, bar, __popc(at.have(tile)) * (uint32_t)box * kRowBytes);
           const uint32_t to = smem_u32(base + (kQuant ? Sh::kRaw + kv * Sh::kRawBytes : Sh::at(kv, issued)));
           if constexpr (kQuant) {  // the scale bytes: 16 (blocks of 8 keys: 8) a lane
             const int width = min(box, 16), key = lane * width, part = min(key, 127) >> (7 - at.log_parts);
             const int y = at.row(tile, part);
-            if (key < 128 && y >= 0) {
+            if (missing >> part & 1) {  // its codes are zeros: any factor but the infinity that may lie there
+              if (key < 128) *reinterpret_cast<uint2*>(&C.scales[kv][key]) = make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu);
+              if (key < 128 && width == 16) *reinterpret_cast<uint2*>(&C.scales[kv][key + 8]) = make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu);
+              __threadfence_block();
+            } else if (key < 128 && y >= 0) {
               const uint8_t* src = p.scales + at.scale_at(y + (key - part * box), kv);
               const uint32_t sd = smem_u32(&C.scales[kv][key]);
               if (width == 16)
@@ -571,6 +598,15 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
               for (int i = 0; i < 32; ++i)
                 if (!(see >> i & 1)) s[x + i] = -INFINITY;
             }
+          }
+        }
+        if (C.any_lost && C.lost_tile[(tiles + j) % 8] == tiles + j) {
+#pragma unroll
+          for (int x = 0; x < kKeys; x += 32) {
+            const uint32_t lost = C.lost[(tiles + j) % 8][x / 32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (lost >> i & 1) s[x + i] = -INFINITY;
           }
         }
         float mx[4];

@@ -324,7 +324,8 @@ struct PieceWalk {
 
 // Where the key tiles of a unit lie in the pool, 32 / parts tiles at a time: lane i holds part
 // i % parts (a block, or the tile's piece of a larger block) of tile first + i / parts as its pool
-// row (block * kv heads + kv head) * block_size + slot, or -1.  The entries of the next batch are
+// row (block * kv heads + kv head) * block_size + slot, -1 (no keys there), or `bad` where the table's entry
+// is no block of the pool: such keys are seen by nobody.  The entries of the next batch are
 // read while the current one is staged, so that no tile waits for the table.  (A read, a check and a
 // division per tile made the staging warp the bound of 8-bit decodes: 306 us for what takes 200 us
 // of copies.)
@@ -334,16 +335,19 @@ struct TileRows {
   const int32_t* table;
   int kvh, end, lane;
   int box, parts, log_parts;  // keys of a part, parts of a tile
+  int bad;                    // row of a part whose entry is no block: -1, or the first row past the pool
   int first, rows;            // the current batch
+  bool none;                  // it has an entry that is no block (`bad` >= 0)
   int32_t next;               // table entry of the batch after it
 
-  __device__ __forceinline__ TileRows(const ChunkParams& p_, const KeyRange& kr_, const Piece& c, int lane_)
-      : p(p_), kr(kr_), table(p_.tables + (int64_t)c.b * p_.table_stride), kvh(c.kvh), end(c.tile1), lane(lane_) {
+  __device__ __forceinline__ TileRows(const ChunkParams& p_, const KeyRange& kr_, const Piece& c, int lane_, int bad_ = -1)
+      : p(p_), kr(kr_), table(p_.tables + (int64_t)c.b * p_.table_stride), kvh(c.kvh), end(c.tile1), lane(lane_), bad(bad_) {
     box = min(p.block_size, p.key_tile);
     parts = p.block_size >= p.key_tile ? 1 : p.by_block.div(p.key_tile);
     log_parts = 31 - __clz(parts);  // a power of two: blocks of 8 .. 64 keys
     first = c.tile0 - (32 >> log_parts);
     rows = -1;
+    none = false;
     next = entry(c.tile0);
   }
   __device__ __forceinline__ int position(int first_tile) const {
@@ -368,16 +372,21 @@ struct TileRows {
       rows = (e * p.n_kv_heads + kvh) * p.block_size + (pos - p.by_block.div(pos) * p.block_size);
     } else if (e != kNoKey) {
       flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
+      rows = bad;
     }
+    if (bad >= 0) none = __any_sync(0xffffffffu, rows == bad);
     next = entry(first + (32 >> log_parts));
   }
   // Pool row of part x of a tile of the current batch (all lanes take part).
   __device__ __forceinline__ int row(int tile, int x) const {
     return __shfl_sync(0xffffffffu, rows, ((tile - first) << log_parts) + x);
   }
-  // Parts of the tile that hold keys.
-  __device__ __forceinline__ uint32_t have(int tile) const {
-    return __ballot_sync(0xffffffffu, rows >= 0) >> ((tile - first) << log_parts) & ((1u << parts) - 1u);
+  // Parts of the tile that hold keys; those whose entry is no block (with a `bad` of 0 or more they
+  // count among the first, too).
+  __device__ __forceinline__ uint32_t have(int tile) const { return of_tile(rows >= 0, tile); }
+  __device__ __forceinline__ uint32_t missing(int tile) const { return none ? of_tile(rows == bad, tile) : 0u; }
+  __device__ __forceinline__ uint32_t of_tile(bool mine, int tile) const {
+    return __ballot_sync(0xffffffffu, mine) >> ((tile - first) << log_parts) & ((1u << parts) - 1u);
   }
   // The byte of a pool row's K (0) or V (1) scale: [block][head][2][slot].
   __device__ __forceinline__ int64_t scale_at(int row, int kv) const {

@@ -59,6 +59,7 @@ struct Ctrl {
   float mm[kConsumers][kHeads], ml[kConsumers][kHeads];  // M, sum
   float mr[kConsumers][kHeads];                          // R (16-bit caches: M)
   uint64_t full[N], empty[N];
+  uint32_t have[N];  // parts of a stage's tile that were there to be copied
   int32_t abort;
   PlanShared plan;
 };
@@ -184,6 +185,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (!ok) break;
         const uint32_t bar = smem_u32(&S.full[st]);
         const uint32_t row_bytes = kQuant ? 128 : 2 * 128;
+        if (kv == 0 && leader) S.have[st] = have;
         mbar_arrive_expect_tx_p(leader, bar, __popc(have) * (uint32_t)box * row_bytes);
         const uint32_t dst = smem_u32(ring + st * St::kBytes + (kv == 0 ? St::kK : St::kV));
         if constexpr (kQuant) {
@@ -226,6 +228,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       k_off[k] = swz(16 * warp + lrow, 2 * k + lchk);
       v_off[k] = kQuant ? k_off[k] : swz(16 * warp + vrow, 2 * k + vchk);
     }
+    const int part = p.block_size < kTile ? p.by_block.div(16 * warp) : 0;  // the warp's keys in a tile
     const bool flip = p.scale < 0.f;  // folded into Q: the largest score has the largest weight
     const float c2 = fmaxf(fabsf(p.scale) * kLog2e, 1e-37f);
     for (; on; on = w.next(p)) {
@@ -293,8 +296,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         uint8_t* stage = ring + st * St::kBytes;
         const uint32_t kb = smem_u32(stage + St::kK), vb = smem_u32(stage + St::kV);
         const int v0 = j * kTile + 16 * warp;
-        const auto seen = [&](int i) { return v0 + i < kr.v_len && (v0 + i >= v_lo || v0 + i < v_s); };
-        const bool all = v0 + 16 <= kr.v_len && (v0 >= v_lo || v0 + 16 <= v_s);
+        const bool there = S.have[st] >> part & 1;
+        const auto seen = [&](int i) { return there && v0 + i < kr.v_len && (v0 + i >= v_lo || v0 + i < v_s); };
+        const bool all = there && v0 + 16 <= kr.v_len && (v0 >= v_lo || v0 + 16 <= v_s);
         if (all || __any_sync(0xffffffffu, seen(lane & 15))) {
           if (!all) {
             // rows of V that are not seen become zeros: 0 x (whatever lies there) must not reach O

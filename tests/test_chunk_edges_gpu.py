@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import snapmind_b200._lib as lib
-from test_chunk_gpu import DT, HALF, check, make_pool
+from test_chunk_gpu import DT, HALF, KERNELS, check, make_pool, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -273,3 +273,61 @@ def test_attend_causal_of_any_sequence_and_length(cuda_device):
         assert pool.attend_causal(0, 8197, q, out, n_b) is out
         pool.check()
         check(out.transpose(0, 1), q.transpose(0, 1), [0, 9], [held[:, :n_b]], [held[:, :n_b]], 0, 0, 2.0**-8)
+
+
+def attention64(q, k, v, see, weight_half, scale=None):
+    """(o, tolerance) of one sequence in f64 under any mask see [t, n]: test_chunk_gpu's reference and its bounds."""
+    t, hq, d = q.shape
+    hkv, n, _ = k.shape
+    scale = d ** -0.5 if scale is None else scale
+    o = torch.zeros((t, hq, d), dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(o)
+    for h in range(hq):
+        kh, vh = (x[h * hkv // hq] for x in (k, v))
+        s = (q[:, h].double() @ kh.T * scale).masked_fill(~see, -torch.inf)
+        sa = (q[:, h].double().abs() @ kh.abs().T).masked_fill(~see, 0).amax(-1, keepdim=True) * scale
+        m = s.amax(-1, keepdim=True)
+        p = torch.exp(s - torch.where(torch.isfinite(m), m, 0.0))
+        z = p.sum(-1, keepdim=True)
+        p = torch.where(z > 0, p / z, 0.0)
+        u = 2.0**-24
+        w = 2.0**-21 + 2 * (d + 4) * u * sa
+        o[:, h] = p @ vh
+        top = torch.where(z > 0, 1 / z, 0.0) * (see.double() @ vh.abs())
+        tol[:, h] = p @ vh.abs() * (2 * w + 2 * n * u + weight_half) + 2.0**-25 * top * (weight_half > 0)
+    return o, tol
+
+
+def check_seen(out, q, k, v, see, weight_half):
+    o, tol = attention64(q, k, v, see, weight_half)
+    tol = tol + HALF[out.dtype] * o.abs() * (1 + 2.0**-6) + 1e-30
+    err = (out.double() - o).abs()
+    assert torch.isfinite(out).all()
+    assert not (err > tol).any(), f"worst {float((err / tol).max()):.2f} x the tolerance"
+
+
+@pytest.mark.parametrize("bs", [8, 16, 32, 64, 256])
+@pytest.mark.parametrize("cache,d,single,generic", KERNELS)
+def test_blocks_that_are_none(cuda_device, cache, d, single, generic, bs):
+    """A table entry outside the pool: its keys are seen by nobody, whatever lay where they would have been
+    staged, and the error word tells."""
+    lens, new = ([3000, 700], [1, 1]) if single else ([3000, 700], [40, 300])
+    pool, ks, vs = make_pool(torch.bfloat16, lens, 2, d, bs, 53, cache)
+    q = torch.randn((sum(new), 8, d), device="cuda").bfloat16()
+    cu = torch.tensor([0, new[0], sum(new)], dtype=torch.int32, device="cuda")
+    bad = [{0, 1, 900 // bs, 2900 // bs}, {300 // bs, 699 // bs}]  # 699: the newest tokens' own block
+    lost = [torch.zeros(n, dtype=torch.bool, device="cuda") for n in lens]
+    for b in range(2):
+        for i in bad[b]:
+            pool.block_tables[b, i] = -1 if i % 2 else 10**6
+            lost[b][i * bs:(i + 1) * bs] = True
+    window = 2900 if single and cache == "same" else 0
+    if single:
+        out = pool.decode(0, q, window=window, force_generic=generic)
+    else:
+        out = pool.attend_chunk(0, q, cu, window=window, force_generic=generic)
+    with pytest.raises(RuntimeError, match="block id"):
+        pool.check()
+    for b in range(2):
+        see = visible(lens[b], new[b], window, 0) & ~lost[b]
+        check_seen(out[cu[b]:cu[b + 1]], q[cu[b]:cu[b + 1]], ks[b], vs[b], see, HALF[torch.bfloat16])
