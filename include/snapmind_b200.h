@@ -579,9 +579,7 @@ SNAPMIND_API int snapmind_kv_gather_quant(const void *k_pool, const void *v_pool
  * same layer as k_pool and v_pool; NULL otherwise).  Softmax statistics and sums are
  * f32; the tensor-core kernels round a weight 2^(s - max) to the element type (f16 for
  * e4m3 decodes) before it multiplies V.  head_dim <= 256, batch <= 8192.
- * A masked position never counts, with one exception: the tensor-core kernels
- * multiply a weight of 0 with V, so an infinity or NaN in V of a token that some query
- * of the same sequence sees can reach other queries of that sequence.
+ * A masked position never counts, whatever K and V hold there.
  * `workspace` holds snapmind_paged_gqa_chunk_workspace_bytes(head_dim) bytes on a
  * 256-byte boundary; its contents need no preparation and are not kept.  Calls
  * that share one must not overlap on the GPU.

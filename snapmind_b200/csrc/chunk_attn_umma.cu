@@ -90,6 +90,7 @@ struct Ctrl {
   // wait for the softmax threads to have read scores.)
   uint32_t lost_tile[8], lost[8][4];
   int32_t any_lost;  // there was one
+  int32_t any_odd;  // values of V were taken out (in this piece, or one before)
   int32_t odd;  // f16 over e4m3: a row that f16 does not hold was met
   PlanShared plan;
   alignas(16) uint8_t scales[2][128];
@@ -164,7 +165,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 // the key tiles t, t + 2, ..., each with sums and an O of its own, added up at the end.
 
 // Whether a key tile holds rows that no query of the unit sees: [u_s, u_lo) and from v_len on, on the
-// virtual axis.
+// virtual axis.  Their V is zeroed: a weight of 0 times an infinity or NaN would reach O.
 struct EdgeTiles {
   int v_len, u_s, u_lo;
   __device__ __forceinline__ EdgeTiles(const ChunkParams& p, const KeyRange& r)
@@ -174,6 +175,26 @@ struct EdgeTiles {
     return v0 + kKeys > v_len || (v0 < u_lo && v0 + kKeys > u_s);
   }
   __device__ __forceinline__ bool unseen(int v) const { return v >= v_len || (v < u_lo && v >= u_s); }
+};
+// Rows that some queries of the unit see and others do not, from hi0 on and in [lo0, lo1): of their V
+// the values that are not finite are taken out for the same reason, and the rows that see them get
+// them at the end (add_odd).
+struct MixedKeys {
+  int hi0, hi1, lo0, lo1;
+  __device__ __forceinline__ MixedKeys(const ChunkParams& p, const KeyRange& r, int tokens)
+      : hi0(min(max(0, r.pos0 + 1 - r.shift), r.v_len)), hi1(r.v_len),
+        lo0(p.window > 0 ? max(r.win_lo - r.shift, min(p.sinks, r.v_sink)) : 0),
+        lo1(p.window > 0 ? max(0, r.pos0 + tokens - p.window) - r.shift : 0) {}
+  __device__ __forceinline__ bool operator()(int v) const { return (v >= hi0 && v < hi1) || (v >= lo0 && v < lo1); }
+  // Rows [first, last) of the tile at v0 hold all of its mixed keys.
+  __device__ __forceinline__ int first(int v0) const {
+    const int a = max(v0, hi0), b = max(v0, lo0);
+    return min(a < hi1 ? a : INT32_MAX, b < lo1 ? b : INT32_MAX) - v0;
+  }
+  __device__ __forceinline__ int last(int v0) const {
+    const int end = v0 + kKeys, a = min(end, hi1), b = min(end, lo1);
+    return max(a > hi0 ? a : 0, b > lo0 ? b : 0) - v0;
+  }
 };
 
 // A pair of f32 times one factor, in one instruction.
@@ -192,6 +213,14 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* x) {
                "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
                : "memory");
 }
+
+// The tiles that hold such rows (and, below the last of a window's, others).
+struct MixedTiles {
+  int from, below;
+  __device__ __forceinline__ explicit MixedTiles(const MixedKeys& m)
+      : from(m.hi0 < m.hi1 ? m.hi0 / kKeys : INT32_MAX), below(m.lo0 < m.lo1 ? (m.lo1 + kKeys - 1) / kKeys : 0) {}
+  __device__ __forceinline__ bool has(int tile) const { return tile >= from || tile < below; }
+};
 
 // 16 e4m3 codes of one row times 2^(byte - 127), as 16 elements of T.  The scale is a power of two:
 // exact in bf16, and in f16 unless odd_row says otherwise.
@@ -214,6 +243,67 @@ __device__ __forceinline__ void dequant16(const uint4& codes, uint32_t byte, uin
   }
   lo = make_uint4(o[0], o[1], o[2], o[3]);
   hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// Takes the infinities and NaN out of the mixed rows of the V stage of the tile whose first key is v0, by one
+// warp; whether the lane met one.  Short code on purpose: it runs once or twice a unit, and instructions that
+// come from L2 cost more than rounds of a loop (unrolled by 4 it took 4% of a step of chunks).
+template <typename T, int D>
+__device__ __forceinline__ bool take_odd(const MixedKeys& mixed, int v0, int lane, uint8_t* stage) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;  // an exponent of all ones
+  constexpr uint32_t carry = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;  // carries into the sign's place
+  const int last = mixed.last(v0) * (D / 8);
+  bool odd = false;
+#pragma unroll 1
+  for (int i = max(0, mixed.first(v0)) * (D / 8) + lane; i < last; i += 32) {  // 16 bytes of row r
+    const int r = i / (D / 8), x = i % (D / 8);
+    uint4* at = reinterpret_cast<uint4*>(stage + (r >> 3) * Shape<D, false>::kGroup + x / 8 * 1024 + (r & 7) * 128 + x % 8 * 16);
+    const uint4 y = *at;
+    if (((((y.x & e) + carry) | ((y.y & e) + carry) | ((y.z & e) + carry) | ((y.w & e) + carry)) & 0x80008000u) && mixed(v0 + r)) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(at);
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k) w[k] &= ~((((w[k] & e) + carry) >> 15 & 0x00010001u) * 0xFFFFu);
+      odd = true;
+    }
+  }
+  return odd;
+}
+
+// Adds to an output row (`out`, or a piece's partial row) the infinities and NaN that were taken out of V: those of
+// the piece's keys that token `tok` of the unit sees and another does not.  The rows of V come from
+// the pool once more; nothing of this runs unless there is such a value.
+template <typename T, int D, bool kQuant>
+__device__ __noinline__ void add_odd(const ChunkParams& p, const Piece c, int tok, T* out, float* part) {
+  const int tokens = min(p.tokens, c.n - c.i0);
+  const KeyRange kr = key_range(p, c.len, c.n, c.i0, c.i0 + tokens);
+  const MixedKeys mixed(p, kr, tokens);
+  const int qpos = kr.pos0 + tok;
+  const int32_t* table = p.tables + (int64_t)c.b * p.table_stride;
+  for (int v = c.tile0 * kKeys; v < min(kr.v_len, c.tile1 * kKeys); ++v) {
+    if (!mixed(v)) {
+      if (v >= mixed.lo1 && v < mixed.hi0) v = mixed.hi0 - 1;
+      continue;
+    }
+    const int pos = kr.position(v), j = p.by_block.div(pos);
+    if (pos > qpos || (p.window > 0 && pos <= qpos - p.window && pos >= p.sinks)) continue;
+    const int32_t phys = table[j];
+    if (phys < 0 || phys >= p.num_blocks) continue;
+    const int64_t tile = (int64_t)phys * p.n_kv_heads + c.kvh;
+    const int64_t row = tile * p.block_size + (pos - j * p.block_size);
+    const float scale = kQuant ? __uint_as_float((uint32_t)p.scales[row + tile * p.block_size + p.block_size] << 23) : 1.f;
+    for (int d = 0; d < D; ++d) {
+      float x;
+      if constexpr (kQuant) {
+        const __half_raw h = __nv_cvt_fp8_to_halfraw(reinterpret_cast<const __nv_fp8_storage_t*>(p.v_pool)[row * D + d], __NV_E4M3);
+        x = Conv<T>::to_f(Conv<T>::from_f(__half2float(__half(h)) * scale));
+      } else {
+        x = Conv<T>::to_f(reinterpret_cast<const T*>(p.v_pool)[row * D + d]);
+      }
+      if (fabsf(x) < INFINITY) continue;
+      if (part != nullptr) part[d] += x;
+      else out[d] = Conv<T>::from_f(Conv<T>::to_f(out[d]) + x);
+    }
+  }
 }
 
 // f16 over e4m3 rows.  K is staged times 2^5, which the scores' factor takes back, so that f16 holds
@@ -247,7 +337,7 @@ template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setm
 template <typename T, int D, bool kQuant>
 __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     chunk_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                      const __grid_constant__ CUtensorMap v_map, ChunkParams p) {
+                      const __grid_constant__ CUtensorMap v_map, const __grid_constant__ ChunkParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using Sh = Shape<D, kQuant>;
@@ -280,7 +370,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     mbar_init(smem_u32(&C.x_ml), 128);
     mbar_init(smem_u32(&C.x_done), 128);
     C.abort = C.odd = 0;
-    C.any_lost = 0;
+    C.any_lost = C.any_odd = 0;
     mbar_init_fence();
   }
   if (warp == Ro::kScores) {
@@ -469,7 +559,9 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         const int i1 = min(c.n, c.i0 + p.tokens);
         const bool split = i1 - c.i0 <= p.tokens / 2;
         const int ahead = split ? 2 : 1;
-        const EdgeTiles edge(p, key_range(p, c.len, c.n, c.i0, i1));
+        const KeyRange kr = key_range(p, c.len, c.n, c.i0, i1);
+        const EdgeTiles edge(p, kr);
+        const MixedTiles mixed(MixedKeys(p, kr, i1 - c.i0));
         if (do_s) {
           // the groups have read the last scores of the piece before: its products are done with Q
           for (int t = 0; t < 2 && ok; ++t)
@@ -516,6 +608,13 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
             const uint32_t step = s0[t] + ((h - 1) >> 1), iv = tiles + j;
             if ((split || t == 0) && !wait(&C.full[1][Sh::stage(1, iv)], Sh::parity(1, iv))) break;
             if (!kQuant && (split || t == 0) && edge(c.tile0 + j)) mbar_arrive_p(leader, smem_u32(&C.v_ready[t]));
+            // under the group's softmax
+            if ((split || t == 0) && mixed.has(c.tile0 + j)) {  // under the group's softmax
+              const MixedKeys keys(p, key_range(p, c.len, c.n, c.i0, i1), i1 - c.i0);
+              if (take_odd<T, D>(keys, (c.tile0 + j) * kKeys, lane, base + Sh::at(1, iv))) C.any_odd = 1;
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
             if (!wait(&C.p_full[t], step & 1)) break;
             values(t, Sh::stage(1, iv), step == s0[t], step);
             if (split || t == 1) umma_commit_p(leader, smem_u32(&C.empty[1][Sh::stage(1, iv)]));
@@ -747,6 +846,10 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
 #pragma unroll
           for (int y = 0; y < 16; y += 8) store32(p.part_o + slot * D + x + y, reinterpret_cast<const uint32_t*>(o + y));
         }
+      }
+      if (C.any_odd) {
+        if (mine) add_odd<T, D, kQuant>(p, c, tok, out, whole ? nullptr : p.part_o + slot * D);
+        __syncwarp();
       }
       tc_fence_before();
       if (split) mbar_arrive(smem_u32(&C.x_done));

@@ -155,10 +155,9 @@ class PagedKVPool(BlockPool):
         ``window`` positions up to its own and the first ``sinks``.  Rows of ``out`` that
         belong to no sequence are left as they were (whatever a new ``out`` holds).
 
-        A position that a query does not see never counts, except that on the tensor-core
-        kernels (16-bit queries, head dim 64 or 128) an infinity or NaN in V of a token that
-        another query of the sequence's chunk sees can reach it; ``force_generic`` takes the
-        CUDA-core kernel, which keeps them apart."""
+        A position that a query does not see never counts, whatever K and V hold there (a NaN in V
+        of one of the chunk's tokens reaches the queries from it on).  ``force_generic`` takes the
+        CUDA-core kernel, all in f32."""
         _lib.require_offsets("attend_chunk", cu_q, self.block_tables)
         if cu_q.shape[0] - 1 > self.max_seqs:
             raise ValueError(f"attend_chunk: {cu_q.shape[0] - 1} sequences, the pool holds {self.max_seqs}")

@@ -298,8 +298,10 @@ def attention64(q, k, v, see, weight_half, scale=None):
     return o, tol
 
 
-def check_seen(out, q, k, v, see, weight_half):
+def check_seen(out, q, k, v, see, weight_half, but=None):
     o, tol = attention64(q, k, v, see, weight_half)
+    if but is not None:
+        o = o.masked_fill(but, 0)
     tol = tol + HALF[out.dtype] * o.abs() * (1 + 2.0**-6) + 1e-30
     err = (out.double() - o).abs()
     assert torch.isfinite(out).all()
@@ -331,3 +333,47 @@ def test_blocks_that_are_none(cuda_device, cache, d, single, generic, bs):
     for b in range(2):
         see = visible(lens[b], new[b], window, 0) & ~lost[b]
         check_seen(out[cu[b]:cu[b + 1]], q[cu[b]:cu[b + 1]], ks[b], vs[b], see, HALF[torch.bfloat16])
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3), (16, 100)])
+@pytest.mark.parametrize("hq", [8, 1])
+@pytest.mark.parametrize("cache,dtype,d,generic", [
+    ("same", "bf16", 128, False), ("same", "f16", 64, False), ("e4m3", "bf16", 128, False), ("e4m3", "bf16", 64, False),
+    ("e4m3", "f16", 128, False), ("same", "bf16", 64, True), ("same", "f32", 128, True), ("same", "bf16", 256, True),
+    ("e4m3", "bf16", 128, True),
+])
+def test_odd_values_reach_those_that_see_them(cuda_device, cache, dtype, d, generic, hq, window, sinks):
+    """Infinities and NaN in V of tokens that some queries of a chunk see and others do not: an output is not finite
+    exactly where its query sees one in that dim, and the others have their values.  Whole units, units cut
+    into pieces, and chunks that start the sequence."""
+    dtype = DT[dtype]
+    lens, new = [9000, 300, 200, 40], [150, 300, 9, 0]
+    hkv = min(hq, 2)
+    pool, ks, vs = make_pool(dtype, lens, hkv, d, 16, 54, cache)
+    cu = [0, 150, 450, 459, 459]
+    odd = [[8999, 8900, 8851, 8840, 8803, 5000], [0, 17, 130, 299], [199, 192, 150], []]
+    hit = []
+    for b, n in enumerate(lens):
+        h = torch.zeros((hkv, n, d), dtype=torch.bool, device="cuda")
+        for i, pos in enumerate(odd[b]):
+            head, dims, blk = i % hkv, [(7 * i) % d, (7 * i + 33) % d], int(pool.block_tables[b, pos // 16])
+            for dim in dims:
+                if cache == "e4m3":
+                    pool.v.view(torch.uint8)[0, blk, head, pos % 16, dim] = 0xFF if i % 2 else 0x7F
+                else:
+                    pool.v[0, blk, head, pos % 16, dim] = float(("inf", "-inf", "nan")[i % 3])
+            h[head, pos, dims] = True
+            vs[b][head, pos, dims] = 0
+        hit.append(h)
+    q = torch.randn((cu[-1], hq, d), device="cuda").to(dtype)
+    cud = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    out = pool.attend_chunk(0, q, cud, window=window, sinks=sinks, force_generic=generic)
+    pool.check()
+    for b, (n, t) in enumerate(zip(lens, new)):
+        if t == 0:
+            continue
+        see = visible(n, t, window, sinks)
+        want = torch.stack([see.double() @ hit[b][h * hkv // hq].double() for h in range(hq)], 1) > 0
+        rows = out[cu[b]:cu[b + 1]]
+        assert torch.equal(~torch.isfinite(rows), want)
+        check_seen(rows.masked_fill(want, 0), q[cu[b]:cu[b + 1]], ks[b], vs[b], see, 0.0 if generic else HALF[dtype], want)
