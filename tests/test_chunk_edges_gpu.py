@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import snapmind_b200._lib as lib
-from test_chunk_gpu import DT, HALF, KERNELS, check, make_pool, visible
+from test_chunk_gpu import CASES, DECODE, DT, HALF, KERNELS, check, make_pool, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -377,3 +377,32 @@ def test_odd_values_reach_those_that_see_them(cuda_device, cache, dtype, d, gene
         rows = out[cu[b]:cu[b + 1]]
         assert torch.equal(~torch.isfinite(rows), want)
         check_seen(rows.masked_fill(want, 0), q[cu[b]:cu[b + 1]], ks[b], vs[b], see, 0.0 if generic else HALF[dtype], want)
+
+
+def weight_rounding(dtype, cache, hq, hkv, d, bs, single, generic):
+    """Half a step of the type that the kernel which takes the call rounds a weight to; 0 for the CUDA-core kernel."""
+    if generic or dtype == torch.float32 or d not in (64, 128) or (bs not in (8, 16, 32, 64) and bs % 128):
+        return 0.0
+    narrow = single and d == 128 and hq // hkv <= 8 and (bs in (16, 32) or bs % 64 == 0)
+    return HALF[torch.float16] if narrow and cache == "e4m3" else HALF[dtype]
+
+
+@pytest.mark.parametrize("generic", [False, True])
+@pytest.mark.parametrize("case", CASES + [(*c[:7], None, *c[7:]) for c in DECODE], ids=lambda c: "-".join(str(x) for x in c[:8]))
+def test_weights_are_rounded_once(cuda_device, case, generic):
+    """Every kernel within the bound of the one rounding of a weight that it makes: none on the CUDA cores, f16's
+    in 8-bit decodes of head dim 128, whatever the query's type."""
+    dtype, cache, hq, hkv, d, bs, lens, new, window, sinks = case
+    dtype, single = DT[dtype], new is None
+    new = [1] * len(lens) if single else new
+    pool, ks, vs = make_pool(dtype, lens, hkv, d, bs, 61, cache)
+    cu = [0, *np.cumsum(new).tolist()]
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q = (1.5 * torch.randn((cu[-1], hq, d), generator=g, device="cuda")).to(dtype)
+    if single and (window or cache == "e4m3"):
+        out = pool.decode(0, q, window=window, sinks=sinks, force_generic=generic)
+    else:
+        out = pool.attend_chunk(0, q, torch.tensor(cu, dtype=torch.int32, device="cuda"), window=window, sinks=sinks,
+                                force_generic=generic)
+    pool.check()
+    check(out, q, cu, ks, vs, window, sinks, weight_rounding(dtype, cache, hq, hkv, d, bs, single, generic))
