@@ -51,6 +51,8 @@ class QuantizedKVPool(PagedKVPool):
     def gather(self, batch: int | None = None, layers: range | None = None, out=None):
         """``PagedKVPool.gather``, read back to ``dtype`` (values past its largest are held to it)."""
         batch = self.max_seqs if batch is None else batch
+        if not 0 <= batch <= self.max_seqs:
+            raise ValueError(f"gather: {batch} sequences, the pool holds {self.max_seqs}")
         layers = range(self.n_layers) if layers is None else layers
         total = int(self._host_lens[:batch].sum())
         per_layer = total * self.n_kv_heads * self.head_dim
@@ -101,6 +103,8 @@ class QuantizedKVPool(PagedKVPool):
         n_t = q.shape[1]
         if n_t == 0:
             return out
+        if n_b < n_t:
+            raise ValueError(f"attend_causal: {n_t} queries of {n_b} tokens")
         cu = torch.zeros(2, dtype=torch.int32, device=self.device)
         cu[1] = n_t
         row = self.block_tables[b].data_ptr(), self._lens_ladder(n_b).data_ptr() + 4 * (n_b - 1)

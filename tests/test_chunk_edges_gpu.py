@@ -406,3 +406,17 @@ def test_weights_are_rounded_once(cuda_device, case, generic):
                                 force_generic=generic)
     pool.check()
     check(out, q, cu, ks, vs, window, sinks, weight_rounding(dtype, cache, hq, hkv, d, bs, single, generic))
+
+
+def test_quantised_pool_refuses_what_it_does_not_hold(cuda_device):
+    """Sequences past the pool's (their tables and lengths would be read from whatever lies behind), a length shorter
+    than its queries."""
+    pool, _, _ = make_pool(torch.bfloat16, [40, 30], 2, 128, 16, 4, "e4m3")
+    for batch in (3, 10**6, -1):
+        with pytest.raises(ValueError, match="sequences"):
+            pool.gather(batch=batch)
+    q = torch.randn((8, 5, 128), device="cuda").bfloat16()
+    for n_b in (4, 0, -3):
+        with pytest.raises(ValueError, match="queries"):
+            pool.attend_causal(0, 1, q, torch.empty_like(q), n_b)
+    pool.check()
