@@ -76,7 +76,10 @@ class PagedKVPool(BlockPool):
             n_layers, base = 1, layer
         else:
             n_layers, base = k_new.shape[0], (0 if layer is None else layer)
-        if k_new.stride() != v_new.stride():
+        if k_new.shape != v_new.shape or k_new.dtype != v_new.dtype:
+            raise ValueError("append: k and v rows differ in shape or dtype")
+        _lib.require_same("append", self.block_tables, k_new, v_new)
+        if k_new.stride() != v_new.stride() or k_new.stride(-1) != 1:
             k_new, v_new = k_new.contiguous(), v_new.contiguous()
         _, batch, n_heads, n_tokens, head_dim = k_new.shape
         if n_heads != self.n_kv_heads or head_dim != self.head_dim:

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import snapmind_b200._lib as lib
-from test_chunk_gpu import CASES, DECODE, DT, HALF, KERNELS, check, make_pool, visible
+from test_chunk_gpu import CASES, DECODE, DT, HALF, KERNELS, check, make_pool, quantise64, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -420,3 +420,24 @@ def test_quantised_pool_refuses_what_it_does_not_hold(cuda_device):
         with pytest.raises(ValueError, match="queries"):
             pool.attend_causal(0, 1, q, torch.empty_like(q), n_b)
     pool.check()
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_decode_stores_rows_of_any_layout(cuda_device, cache):
+    """decode(append=, window=): rows whose head dim is not contiguous are stored as they are; K and V of two types,
+    or from another device, are refused."""
+    lens = [70, 31]
+    pool, ks, vs = make_pool(torch.bfloat16, lens, 2, 128, 16, 42, cache, spare=4)
+    pool.reserve(1, batch=2)
+    kn, vn = (torch.randn((2, 128, 2), device="cuda").bfloat16().transpose(1, 2) for _ in range(2))
+    q = torch.randn((2, 8, 128), device="cuda").bfloat16()
+    for bad in ((kn, vn.float()), (kn.cpu(), vn.cpu()), (kn, vn.cpu())):
+        with pytest.raises(ValueError):
+            pool.decode(0, q, append=bad, window=40)
+    out = pool.decode(0, q, append=(kn, vn), window=40)
+    pool.check()
+    for b in range(2):
+        for hist, x in ((ks, kn), (vs, vn)):
+            val = quantise64(x[b])[0] if cache == "e4m3" else x[b].double()
+            hist[b] = torch.cat([hist[b], val.unsqueeze(1)], 1)
+    check(out, q, [0, 1, 2], ks, vs, 40, 0, 2.0**-8)
