@@ -12,23 +12,14 @@
 // tokens (32 heads over 4 of 64) take 55 us, 20 TFLOP/s of what is seen.  4 x 4 products from 8 reads, two CTAs of
 // 256 threads and loads a step ahead took 60 us (63000 wavefronts of shared memory in 92000 cycles), loads
 // element by element 92.  Larger rows need the threads: one CTA of 256, 4 x 4 products.
-#include <cuda_fp8.h>
-
 #include "chunk_plan.cuh"
+#include "pairs.cuh"
 
 namespace snapmind {
 namespace {
 
 constexpr int kRows = 64, kKeys = 64;
 constexpr int kGenMaxD = 256;
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float e4m3_to_f(uint8_t c) {
-  const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
-  return __half2float(__half(h));
-}
-// 2^(b - 127) for a scale byte in [27, 247] (a normal float's exponent field)
-__device__ __forceinline__ float scale_byte_to_f(uint8_t b) { return __uint_as_float((uint32_t)b << 23); }
 
 // D4 = head_dim / 64 rounded up; smem rows are D = 64 * D4 floats (+4: 16-byte reads of
 // 16 different rows then touch different banks), zero past head_dim.
@@ -47,16 +38,6 @@ struct GenSmem {
   int32_t pos[2][kKeys];
   PlanShared plan;
 };
-
-// Pairs of f32 in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 x, x, y, z; "
-      "mov.b64 {%0, %1}, x; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
 
 // 16 bytes of pool elements as floats, stored to 16-byte-aligned shared memory; whether all are finite.
 template <typename KV>

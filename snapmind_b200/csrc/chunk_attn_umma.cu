@@ -36,9 +36,9 @@
 // traffic: 2700 cycles a tile, 2000 of them without any conversion, 505 TFLOP/s; fewer
 // instructions, rows fetched ahead and conversions by bit operations did not help.
 #include <cuda.h>
-#include <cuda_fp8.h>
 
 #include "chunk_plan.cuh"
+#include "pairs.cuh"
 #include "sm100.cuh"
 
 namespace snapmind {
@@ -50,7 +50,6 @@ constexpr int kTileM = 128, kKeys = 128;
 constexpr int kConvert = 128;  // threads that convert e4m3 rows
 constexpr uint32_t kBlockBytes = 128 * 128;  // 128 rows of 64 16-bit elements
 constexpr uint32_t kPBytes = 2 * kBlockBytes;
-constexpr float kLog2e = 1.4426950408889634f;
 // A raised reference stands 2^kLow below the maximum, and stays until a score exceeds it by 2^kRescale.
 // f16 weights go up to 2^15: a weight 2^25 below a largest one of 1 would vanish, and the weights of
 // thousands of keys behind a strong sink lie there; 2^7 further up, a weight is off by 2^-32 of the
@@ -104,15 +103,6 @@ static_assert(smem_bytes<128, false>() <= 232448 && smem_bytes<128, true>() <= 2
 static_assert(smem_bytes<64, false>() <= 232448 && smem_bytes<64, true>() <= 232448, "shared memory budget");
 static_assert(kPBytes >= kMaxChunkBatch * 4, "plan scratch in the P tiles");
 
-__device__ __forceinline__ bool role_wait(const Ctrl& C, uint32_t bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity)) {
-    if (*reinterpret_cast<const volatile int32_t*>(&C.abort)) return false;
-    if (clock64() - t0 > kWaitTicks) return false;
-  }
-  return true;
-}
 // Rare, so not inlined: one bit per key of the parts `missing` (2^log_box keys each) of tile `tile`.
 __device__ __noinline__ void mark_lost(Ctrl& C, uint32_t tile, uint32_t missing, int log_box) {
   if (!C.any_lost)
@@ -132,35 +122,8 @@ __device__ __forceinline__ void give_up(Ctrl& C, int32_t* err) {
   flag_error(err, SNAPMIND_DEVERR_TIMEOUT);
 }
 
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-
 // The lowest k bits (none for k <= 0, all for k >= 32).
 __device__ __forceinline__ uint32_t low_bits(int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; }
-// Pairs of f32 in one instruction: a b + c, a + b.
-__device__ __forceinline__ float2 fma2(float2 a, float b, float c) {
-  float2 r;
-  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %4}; mov.b64 z, {%5, %5}; fma.rn.f32x2 x, x, y, z; "
-      "mov.b64 {%0, %1}, x; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-
 // A piece whose rows all fit tile 0 runs split: both softmax groups take tile 0's rows, group t
 // the key tiles t, t + 2, ..., each with sums and an O of its own, added up at the end.
 
@@ -197,15 +160,6 @@ struct MixedKeys {
   }
 };
 
-// A pair of f32 times one factor, in one instruction.
-__device__ __forceinline__ float2 mul2(float2 a, float b) {
-  float2 r;
-  asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %4}; mul.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b));
-  return r;
-}
-
 // 32 bytes, one sector, in one store (a lane stores a row of its own: with 16 bytes a store, a mixed
 // step took 172 us, not 167).
 __device__ __forceinline__ void store32(void* p, const uint32_t* x) {
@@ -226,15 +180,13 @@ struct MixedTiles {
 // exact in bf16, and in f16 unless odd_row says otherwise.
 template <typename T>
 __device__ __forceinline__ void dequant16(const uint4& codes, uint32_t byte, uint4& lo, uint4& hi) {
-  const float s = __uint_as_float(byte << 23);
+  const float s = scale_byte_to_f(byte);
   const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
   uint32_t o[8];
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     uint32_t h[2];
-    asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }"
-        : "=r"(h[0]), "=r"(h[1])
-        : "r"(w[i / 2]));
+    codes_f16(w[i / 2], h[0], h[1]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const float2 f = mul2(__half22float2(*reinterpret_cast<const __half2*>(&h[j])), s);
@@ -290,12 +242,11 @@ __device__ __noinline__ void add_odd(const ChunkParams& p, const Piece c, int to
     if (phys < 0 || phys >= p.num_blocks) continue;
     const int64_t tile = (int64_t)phys * p.n_kv_heads + c.kvh;
     const int64_t row = tile * p.block_size + (pos - j * p.block_size);
-    const float scale = kQuant ? __uint_as_float((uint32_t)p.scales[row + tile * p.block_size + p.block_size] << 23) : 1.f;
+    const float scale = kQuant ? scale_byte_to_f(p.scales[row + tile * p.block_size + p.block_size]) : 1.f;
     for (int d = 0; d < D; ++d) {
       float x;
       if constexpr (kQuant) {
-        const __half_raw h = __nv_cvt_fp8_to_halfraw(reinterpret_cast<const __nv_fp8_storage_t*>(p.v_pool)[row * D + d], __NV_E4M3);
-        x = Conv<T>::to_f(Conv<T>::from_f(__half2float(__half(h)) * scale));
+        x = Conv<T>::to_f(Conv<T>::from_f(e4m3_to_f(reinterpret_cast<const uint8_t*>(p.v_pool)[row * D + d]) * scale));
       } else {
         x = Conv<T>::to_f(reinterpret_cast<const T*>(p.v_pool)[row * D + d]);
       }
@@ -412,8 +363,8 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
           const int j = x < 0 ? i : (x < 2 * (n - lead) ? x / 2 + (kv ? 0 : ahead) : x - (n - lead));
           const uint32_t num = tiles + j;
           const int st = Sh::stage(kv, num);
-          ok = role_wait(C, smem_u32(&C.raw_full[kv]), num & 1) &&
-               role_wait(C, smem_u32(&C.empty[kv][st]), Sh::parity(kv, num) ^ 1);
+          ok = role_wait(C.abort, smem_u32(&C.raw_full[kv]), num & 1) &&
+               role_wait(C.abort, smem_u32(&C.empty[kv][st]), Sh::parity(kv, num) ^ 1);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
@@ -465,7 +416,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
           at.advance(tile);
           const int st = Sh::stage(kv, issued);
           const uint32_t freed = smem_u32(kQuant ? &C.raw_empty[kv] : &C.empty[kv][st]);
-          ok = __all_sync(0xffffffffu, role_wait(C, freed, (kQuant ? issued & 1 : Sh::parity(kv, issued)) ^ 1));
+          ok = __all_sync(0xffffffffu, role_wait(C.abort, freed, (kQuant ? issued & 1 : Sh::parity(kv, issued)) ^ 1));
           if (!ok) break;
           const uint32_t bar = smem_u32(kQuant ? &C.raw_full[kv] : &C.full[kv][st]);
           constexpr uint32_t kRowBytes = kQuant ? D : 2 * D;
@@ -520,7 +471,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       uint32_t last_bar = 0, last_parity = 0, q_pending = 0;
       bool ok = true;
       const auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && __all_sync(0xffffffffu, role_wait(C, smem_u32(bar), parity));
+        ok = ok && __all_sync(0xffffffffu, role_wait(C.abort, smem_u32(bar), parity));
         if (ok) tc_fence_after();
         return ok;
       };
@@ -659,7 +610,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (int j = split ? t : 0; j < n; j += split ? 2 : 1) {
         const int v0 = (c.tile0 + j) * kKeys;
-        ok = role_wait(C, smem_u32(&C.s_full[t]), step & 1);
+        ok = role_wait(C.abort, smem_u32(&C.s_full[t]), step & 1);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
@@ -673,7 +624,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         mbar_arrive(smem_u32(&C.s_free[t]));
         if (!kQuant && (split || t == 0) && edge(c.tile0 + j)) {
           // rows of V that nobody sees are zeroed: 0 x (whatever lies there) must not reach O
-          ok = __all_sync(0xffffffffu, role_wait(C, smem_u32(&C.v_ready[t]), edges++ & 1));
+          ok = __all_sync(0xffffffffu, role_wait(C.abort, smem_u32(&C.v_ready[t]), edges++ & 1));
           if (!ok) break;
           if (edge.unseen(v0 + r)) {
             uint8_t* vrow = base + Sh::at(1, tiles + j) + (r >> 3) * Sh::kGroup + (r & 7) * 128;
@@ -722,7 +673,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
           if (raise) m = top - kLow<T>;
           l *= alpha;
           if (step > step0) {  // O += P V of the group's tile before is done: O may change
-            ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);
+            ok = role_wait(C.abort, smem_u32(&C.pv_done[t]), (step - 1) & 1);
             if (!__all_sync(0xffffffffu, ok)) {
               ok = false;
               break;
@@ -747,14 +698,14 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         uint32_t pk[kKeys / 2];
 #pragma unroll
         for (int x = 0; x < kKeys; x += 2) {
-          float2 e = fma2(make_float2(s[x], s[x + 1]), c2, -ref);
+          float2 e = fma2(make_float2(s[x], s[x + 1]), make_float2(c2, c2), make_float2(-ref, -ref));
           e.x = ex2(e.x);
           e.y = ex2(e.y);
           sum[(x >> 1) & 1] = add2(sum[(x >> 1) & 1], e);
           pk[x / 2] = pack2<T>(e.x, e.y);
         }
         if (before > 0) {  // the other group's product has read the P buffer
-          ok = role_wait(C, smem_u32(&C.pv_done[t ^ 1]), (before - 1) & 1);
+          ok = role_wait(C.abort, smem_u32(&C.pv_done[t ^ 1]), (before - 1) & 1);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
@@ -778,7 +729,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         other_steps += n;
       }
       on = w.next(p);
-      if (ok && step > step0) ok = role_wait(C, smem_u32(&C.pv_done[t]), (step - 1) & 1);
+      if (ok && step > step0) ok = role_wait(C.abort, smem_u32(&C.pv_done[t]), (step - 1) & 1);
       const uint32_t t_x = tmem + lanes + 2 * kKeys + (t ^ 1) * D;  // the other group's O
       float f = 1.f, fx = 0.f;
       if (split) {
@@ -788,13 +739,13 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
           C.ml[r] = make_float2(m, l);
           tc_fence_before();
           if (ok) mbar_arrive(smem_u32(&C.x_ml));
-          ok = ok && role_wait(C, smem_u32(&C.x_done), splits++ & 1);
+          ok = ok && role_wait(C.abort, smem_u32(&C.x_done), splits++ & 1);
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
           continue;
         }
-        ok = ok && role_wait(C, smem_u32(&C.x_ml), splits++ & 1);
-        if (ok && other_steps > 0) ok = role_wait(C, smem_u32(&C.pv_done[1]), (other_steps - 1) & 1);
+        ok = ok && role_wait(C.abort, smem_u32(&C.x_ml), splits++ & 1);
+        if (ok && other_steps > 0) ok = role_wait(C.abort, smem_u32(&C.pv_done[1]), (other_steps - 1) & 1);
         const float2 ml = C.ml[r];
         const float M = fmaxf(m, ml.x);
         f = m == -INFINITY ? l : ex2(m - M);  // sees nothing: 0; only NaN: NaN

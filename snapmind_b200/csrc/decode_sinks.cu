@@ -23,9 +23,9 @@
 //   K: lane (g, t) holds dims 16 k + 4 t .. + 3 of key g as k-slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9;
 //   V: row g / g + 8 of a 16-dim step stands for dim 2 g / 2 g + 1.
 #include <cuda.h>
-#include <cuda_fp8.h>
 
 #include "chunk_plan.cuh"
+#include "pairs.cuh"
 #include "sm100.cuh"
 
 namespace snapmind {
@@ -35,7 +35,6 @@ using namespace tc;
 
 constexpr int kD = 128, kTile = 64, kConsumers = 4, kThreads = (kConsumers + 2) * 32, kHeads = 8;
 constexpr int kScaleLanes = kTile / 16;  // lanes that fetch a tile's scale bytes of K, or of V, 16 each
-constexpr float kLog2e = 1.4426950408889634f;
 // A raised reference stands 2^kLow below the maximum, and stays until a score passes it by 2^kRaise
 // (weights up to 2^kRaise are as good as those up to 1).  f16 weights go up to 2^15: what is 2^25
 // below the largest weight would vanish if that were 1, although thousands of such keys behind a
@@ -90,21 +89,6 @@ __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <bool kBf16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (kBf16) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
-  } else {
-    __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
-  }
-}
-// four e4m3 codes -> two pairs of f16 (the low two codes, the high two)
-__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }"
-      : "=r"(lo), "=r"(hi)
-      : "r"(w));
-}
 // Byte offset of 16-byte piece `ch` (0..7) of row `row` in rows of 128 bytes, 128-byte swizzle.
 __device__ __forceinline__ uint32_t swz(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
 
@@ -116,16 +100,6 @@ __device__ __forceinline__ void copies_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-template <typename C>
-__device__ __forceinline__ bool role_wait(const C& S, uint32_t bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity)) {
-    if (*reinterpret_cast<const volatile int32_t*>(&S.abort)) return false;
-    if (clock64() - t0 > kWaitTicks) return false;
-  }
-  return true;
-}
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ bool consumers_any(bool v) {
   uint32_t r;
@@ -143,6 +117,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   using St = Stage<kQuant>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr bool kMmaBf16 = kBf16 && !kQuant;
+  using Weight = typename std::conditional<kMmaBf16, __nv_bfloat16, __half>::type;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   auto& S = *reinterpret_cast<Ctrl<kQuant>*>(ring + St::kCount * St::kBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -181,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         at.advance(j);
         const uint32_t have = at.have(j);
         const int st = tile % St::kCount;
-        ok = __all_sync(0xffffffffu, role_wait(S, smem_u32(&S.empty[st]), ((tile / St::kCount) & 1) ^ 1));
+        ok = __all_sync(0xffffffffu, role_wait(S.abort, smem_u32(&S.empty[st]), ((tile / St::kCount) & 1) ^ 1));
         if (!ok) break;
         const uint32_t bar = smem_u32(&S.full[st]);
         const uint32_t row_bytes = kQuant ? 128 : 2 * 128;
@@ -260,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int k = 0; k < 8; ++k)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) qf[k][i] = pack2<false>(x[4 * k + 2 * i] * up, x[4 * k + 2 * i + 1] * up);
+            for (int i = 0; i < 2; ++i) qf[k][i] = pack2<__half>(x[4 * k + 2 * i] * up, x[4 * k + 2 * i + 1] * up);
           // A sum of products is below 2^25 (128 x 448 x 2^9), K's scale at most 2^120: 2^17 of it goes
           // to the head's factor, so that what overflows is a score, not a step towards one.  (A query above
           // 2^110 has no room for it and needs none.)
@@ -291,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       float R0 = kNone, R1 = kNone;                      // R
       for (int j = c.tile0; j < c.tile1; ++j, ++tile) {
         const int st = tile % St::kCount;
-        ok = __all_sync(0xffffffffu, role_wait(S, smem_u32(&S.full[st]), (tile / St::kCount) & 1));
+        ok = __all_sync(0xffffffffu, role_wait(S.abort, smem_u32(&S.full[st]), (tile / St::kCount) & 1));
         if (!ok) break;
         uint8_t* stage = ring + st * St::kBytes;
         const uint32_t kb = smem_u32(stage + St::kK), vb = smem_u32(stage + St::kV);
@@ -393,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           l0 += kQuant ? ex2(xs[0]) + ex2(xs[2]) : p0 + p2;
           l1 += kQuant ? ex2(xs[1]) + ex2(xs[3]) : p1 + p3;
           // ---- P^T as the B operand: lane (g, tig) needs keys 2 tig, + 1, + 8, + 9 of head g
-          const uint32_t pr01 = pack2<kMmaBf16>(p0, p1), pr23 = pack2<kMmaBf16>(p2, p3);
+          const uint32_t pr01 = pack2<Weight>(p0, p1), pr23 = pack2<Weight>(p2, p3);
           const int src = 8 * tig + (g >> 1);
           const uint32_t x = __shfl_sync(0xffffffffu, pr01, src), y = __shfl_sync(0xffffffffu, pr01, src + 4);
           const uint32_t z = __shfl_sync(0xffffffffu, pr23, src), u = __shfl_sync(0xffffffffu, pr23, src + 4);
@@ -516,8 +491,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] *= inv;
           T* out = reinterpret_cast<T*>(p.out) + (int64_t)c.q_first * p.out_stride_tok + (int64_t)(head0 + h) * p.out_stride_head + d;
-          *reinterpret_cast<uint4*>(out) = make_uint4(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]),
-                                                      pack2<kBf16>(x[4], x[5]), pack2<kBf16>(x[6], x[7]));
+          *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]),
+                                                      pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
         } else {
           const int64_t row = part_slot(c) * p.rows + h;
           if (d == 0) {

@@ -13,9 +13,7 @@
 //
 // Both kernels are byte movers: a team of lanes owns a row (16-byte vectors of the wide
 // side), several rows in flight per team.
-#include <cuda_fp8.h>
-
-#include "common.cuh"
+#include "pairs.cuh"
 
 namespace snapmind {
 namespace {
@@ -148,15 +146,6 @@ template <typename T> struct Bits {
     else return __uint_as_float(a << 16);
   }
 };
-
-// A pair of products by one power of two (one instruction on sm_100).
-__device__ __forceinline__ float2 mul2(float2 a, float s) {
-  float2 r;
-  asm("{ .reg .b64 a, b, c; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %4}; mul.rn.f32x2 c, a, b; mov.b64 {%0, %1}, c; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(s));
-  return r;
-}
 
 // Rows of TEAM lanes x two 16-byte vectors each (head_dim * sizeof(T) = 32 TEAM bytes; a lane's
 // vectors are TEAM apart, so a team reads whole lines).  blockIdx.y = layer * 2 + (K, V).  A warp
@@ -372,10 +361,9 @@ template <typename T> constexpr int plain_bytes() { return std::is_same<T, __hal
 // N codes (the low bytes of w) times 2^(byte - 127); kHold: the range is looked at.
 template <typename T, int N, bool kHold>
 __device__ __forceinline__ void dequant(const uint32_t* w, int byte, T* y) {
-  const float s = __uint_as_float((uint32_t)byte << 23);
+  const float s = scale_byte_to_f(byte);
   if constexpr (N == 1) {
-    const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)w[0], __NV_E4M3);
-    y[0] = Conv<T>::from_f(held<T>(__half2float(__half(h)) * s));
+    y[0] = Conv<T>::from_f(held<T>(e4m3_to_f((uint8_t)w[0]) * s));
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 2) {

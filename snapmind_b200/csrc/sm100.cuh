@@ -71,6 +71,17 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
   return true;
 }
 
+// The same for a role of a kernel: also false once another role has given up (`abort`, in shared memory).
+__device__ __forceinline__ bool role_wait(const int32_t& abort, uint32_t bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*reinterpret_cast<const volatile int32_t*>(&abort)) return false;
+    if (clock64() - t0 > kWaitTicks) return false;
+  }
+  return true;
+}
+
 // ---- TMA --------------------------------------------------------------------
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
                                             uint32_t bar) {
