@@ -616,6 +616,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
           break;
         }
         tc_fence_after();
+        const bool any_lost = *reinterpret_cast<const volatile int32_t*>(&C.any_lost);  // lands with the scores
         float s[kKeys];
 #pragma unroll
         for (int x = 0; x < kKeys; x += 32) tmem_ld32(t_s + x, s + x);
@@ -650,7 +651,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
             }
           }
         }
-        if (C.any_lost && C.lost_tile[(tiles + j) % 8] == tiles + j) {
+        if (any_lost && C.lost_tile[(tiles + j) % 8] == tiles + j) {
 #pragma unroll
           for (int x = 0; x < kKeys; x += 32) {
             const uint32_t lost = C.lost[(tiles + j) % 8][x / 32];
