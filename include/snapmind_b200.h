@@ -577,9 +577,14 @@ SNAPMIND_API int snapmind_kv_gather_quant(const void *k_pool, const void *v_pool
  * query head h reads kv head h / (n_q_heads / n_kv_heads).  pool_dtype is `dtype`, or
  * SNAPMIND_DTYPE_E4M3 with `scales` as snapmind_kv_append_chunk writes them (of the
  * same layer as k_pool and v_pool; NULL otherwise).  Softmax statistics and sums are
- * f32; the tensor-core kernels round a weight 2^(s - max) to the element type (f16 for
+ * f32; the tensor-core kernels round a weight 2^(s - ref) to the element type (f16 for
  * e4m3 decodes) before it multiplies V.  head_dim <= 256, batch <= 8192.
- * A masked position never counts, whatever K and V hold there.
+ * A masked position never counts, whatever K and V hold there; neither does one whose
+ * table entry is no block (SNAPMIND_DEVERR_BLOCK_ID is set).  Rows of an e4m3 pool count as the
+ * values c * 2^e that they stand for, of any exponent, in every kernel: those that an f16 call's
+ * tensor-core kernel cannot hold make the CUDA-core kernel, launched behind it, do the
+ * call over.  A sum of weights times V is f32 before it is divided: with n keys V should
+ * stay below 2^119 / n (8-bit decodes have no such bound).
  * `workspace` holds snapmind_paged_gqa_chunk_workspace_bytes(head_dim) bytes on a
  * 256-byte boundary; its contents need no preparation and are not kept.  Calls
  * that share one must not overlap on the GPU.

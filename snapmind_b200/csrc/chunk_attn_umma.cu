@@ -15,7 +15,8 @@
 //                   cycles a unit), issues the MMAs of the scores
 //   warps 9, 10     stage K and V by TMA
 //   warp 11         issues the MMAs of P V: a wait takes some 200 cycles next to operand reads that fill
-//                   shared memory's bandwidth, and the two streams cover each other's
+//                   shared memory's bandwidth, and the two streams cover each other's; in tiles that
+//                   only some of a unit's queries see it takes infinities and NaN out of V before
 //   warps 12-15     8-bit caches only: turn the staged rows into 16-bit stages
 // P goes through shared memory, not through TMEM as an A operand: a kernel of this library that
 // read A from TMEM ended in a launch failure whose cause was not found.
@@ -30,11 +31,15 @@
 // every path.
 // What bounds it is shared memory: a step of 2 x 128 x 128 scores reads 4 x 64 KB of operands, writes 64 KB of P
 // and receives 64 KB of K and V, 3070 cycles at 128 bytes each (measured 3200 to 3300; the products
-// themselves take 2048).  2048 new tokens behind
-// 30720 cached ones, 32 heads over 8 of 128: 920 us, 1160 TFLOP/s.  Short units add 20000 cycles at the start of a CTA and 12000 a piece
-// (a mixed step 167 us, 800 TFLOP/s).  Over 8-bit rows the converting warps add 48 KB a tile to the same
-// traffic: 2700 cycles a tile, 2000 of them without any conversion, 505 TFLOP/s; fewer
-// instructions, rows fetched ahead and conversions by bit operations did not help.
+// themselves take 2048).  2048 new tokens behind 30720 cached ones, 32 heads over 8 of 128: 987 us, 1080
+// TFLOP/s (replayed from a graph, as the other times here; back to back from Python, under the power
+// cap, 1140 us).  Short units add 20000 cycles at the start of a CTA and 12000 a piece (a mixed step
+// 176 us, 760 TFLOP/s).  Over 8-bit rows the converting warps add 48 KB a tile to the same traffic: 2700
+// cycles a tile, 2000 of them without any conversion, 118 us and 493 TFLOP/s for a step of four
+// chunks; fewer instructions, rows fetched ahead and conversions by bit operations did not help.
+// Instructions count even where they do not run (the softmax loop is long, and what it and the other roles
+// fetch from L2 is waited for): the handling of keys without a block costs 1 to 2% of every call,
+// that of infinities in V up to 2.5% of a step of 8-bit chunks.
 #include <cuda.h>
 
 #include "chunk_plan.cuh"

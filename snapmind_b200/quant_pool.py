@@ -11,7 +11,8 @@ A row x of one token and head is held as ``c * 2^e``: e the smallest integer in
 [-100, 120] with ``max |x| <= 448 * 2^e``, c the e4m3 value nearest to ``x / 2^e`` (ties to
 even).  So a value is off by at most 2^-4 of itself (or by 2^(e - 10), for values below
 2^(e - 6)).  Infinities and NaN become NaN.  Queries, outputs and ``gather`` are in ``dtype``
-(bf16, f16 or f32).  The reference cache has no 8-bit form.
+(bf16, f16 or f32); attention takes the rows as they are held, also where ``dtype`` could not hold
+them.  The reference cache has no 8-bit form.
 """
 from __future__ import annotations
 
