@@ -583,7 +583,7 @@ SNAPMIND_API int snapmind_kv_gather_quant(const void *k_pool, const void *v_pool
  * table entry is no block (SNAPMIND_DEVERR_BLOCK_ID is set).  Rows of an e4m3 pool count as the
  * values c * 2^e that they stand for, of any exponent, in every kernel: those that an f16 call's
  * tensor-core kernel cannot hold make the CUDA-core kernel, launched behind it, do the
- * call over.  A sum of weights times V is f32 before it is divided: with n keys V should
+ * call over (so there out must not be q).  A sum of weights times V is f32 before it is divided: with n keys V should
  * stay below 2^119 / n (8-bit decodes have no such bound).
  * `workspace` holds snapmind_paged_gqa_chunk_workspace_bytes(head_dim) bytes on a
  * 256-byte boundary; its contents need no preparation and are not kept.  Calls

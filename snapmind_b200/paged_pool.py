@@ -27,6 +27,10 @@ from snapmind_b200.block_pool import BlockPool
 _FAR = 1 << 30  # no position is as far
 
 
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.untyped_storage().data_ptr() == b.untyped_storage().data_ptr()
+
+
 class PagedKVPool(BlockPool):
     quantised = False  # pool elements are the values themselves
 
@@ -204,6 +208,9 @@ class PagedKVPool(BlockPool):
             o_st = out.stride()
             if out.shape != q.shape or out.dtype != self.dtype or o_st[2] != 1:
                 raise ValueError("out must have q's shape and dtype, head dim contiguous")
+            if self.quantised and self.dtype == torch.float16 and _share(q, out):
+                q = q.clone()  # such a call may be done over, with the queries it began with
+                q_st = q.stride()
         _lib.require_same("attend", self.block_tables, q, out)
         if append is not None:
             self.append(layer, *append)

@@ -441,3 +441,27 @@ def test_decode_stores_rows_of_any_layout(cuda_device, cache):
             val = quantise64(x[b])[0] if cache == "e4m3" else x[b].double()
             hist[b] = torch.cat([hist[b], val.unsqueeze(1)], 1)
     check(out, q, [0, 1, 2], ks, vs, 40, 0, 2.0**-8)
+
+
+@pytest.mark.parametrize("single", [False, True])
+@pytest.mark.parametrize("cache,dtype,v_exp", [("same", "bf16", 0), ("e4m3", "bf16", 8), ("e4m3", "f16", -8), ("e4m3", "f16", 9)])
+def test_output_over_the_queries(cuda_device, cache, dtype, v_exp, single):
+    """out=q: the queries' rows become the outputs', also where a call is done over (V of exponent 9 in f16)."""
+    lens, d = [900, 130, 40], 64
+    pool, ks, vs = make_pool(DT[dtype], lens, 2, d, 16, 55, cache)
+    cu = [0, 1, 2, 3] if single else [0, 70, 200, 203]
+    g = torch.Generator(device="cuda").manual_seed(9)
+    if cache == "e4m3":
+        shape = pool.scales.shape[1:3] + (16,)
+        one = torch.zeros(shape, dtype=torch.bool, device="cuda")
+        one[int(pool.block_tables[0, 20]), 1, 7] = True
+        ks, vs = set_exponents(pool, lens, pick(g, (-9, -8), shape), torch.where(one, v_exp, -9))
+    q = torch.randn((cu[-1], 8, d), generator=g, device="cuda").to(DT[dtype])
+    out = q.clone()
+    if single:
+        got = pool.decode(0, out, out=out, window=0 if cache == "e4m3" else 1000)
+    else:
+        got = pool.attend_chunk(0, out, torch.tensor(cu, dtype=torch.int32, device="cuda"), out=out)
+    pool.check()
+    assert got is out
+    check(out, q, cu, ks, vs, 0, 0, HALF[DT[dtype]])
