@@ -465,3 +465,89 @@ def test_output_over_the_queries(cuda_device, cache, dtype, v_exp, single):
     pool.check()
     assert got is out
     check(out, q, cu, ks, vs, 0, 0, HALF[DT[dtype]])
+
+
+def test_a_captured_call_that_is_done_over_at_times(cuda_device):
+    """A captured f16 chunk over 8 bits, replayed over rows that f16 holds, over one that it does not, and back;
+    a second graph over the same pool in between."""
+    lens, new = [700, 90], [40, 90]
+    pool, _, _ = make_pool(torch.float16, lens, 2, 128, 16, 56, "e4m3")
+    g = torch.Generator(device="cuda").manual_seed(10)
+    shape = pool.scales.shape[1:3] + (16,)
+    exps = pick(g, (-9, -8), shape)
+    one = torch.zeros(shape, dtype=torch.bool, device="cuda")
+    one[int(pool.block_tables[0, 20]), 1, 7] = True
+    q = torch.randn((130, 8, 128), generator=g, device="cuda").half()
+    cu = [0, 40, 130]
+    cud = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    pool.attend_chunk(0, q, cud)
+    graphs = []
+    for window in (0, 500):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = pool.attend_chunk(0, q, cud, window=window)
+        graphs.append((graph, out, window))
+    for v_exp in (-9, 12, -9, 9, -9):
+        ks, vs = set_exponents(pool, lens, exps, torch.where(one, v_exp, -9))
+        for graph, out, window in graphs:
+            graph.replay()
+            check(out, q, cu, ks, vs, window, 0, HALF[torch.float16])
+    pool.check()
+
+
+@pytest.mark.parametrize("cache,dtype", [("same", "bf16"), ("e4m3", "bf16"), ("e4m3", "f16"), ("same", "f32")])
+def test_the_largest_batch(cuda_device, cache, dtype):
+    """8192 sequences; one more is refused."""
+    dtype, n = DT[dtype], 8192
+    rng = np.random.RandomState(3)
+    lens = rng.randint(0, 40, n)
+    pool, ks, vs = make_pool(dtype, lens.tolist(), 1, 128, 16, 57, cache)
+    new = np.minimum(lens, rng.randint(0, 4, n))
+    cu = np.concatenate([[0], np.cumsum(new)])
+    q = torch.randn((max(int(cu[-1]), n), 2, 128), device="cuda").to(dtype)
+    out = pool.attend_chunk(0, q[:int(cu[-1])], torch.tensor(cu, dtype=torch.int32, device="cuda"))
+    one = pool.decode(0, q[:n], window=25, sinks=2)
+    pool.check()
+    for b in [0, 1, n - 1, *rng.randint(0, n, 100).tolist()]:
+        a, e = int(cu[b]), int(cu[b + 1])
+        check(out[a:e], q[a:e], [0, e - a], ks[b:b + 1], vs[b:b + 1], 0, 0, HALF[dtype])
+        check(one[b:b + 1], q[b:b + 1], [0, 1], ks[b:b + 1], vs[b:b + 1], 25, 2, HALF[dtype])
+    more = type(pool)(1, 1, 128, 4, n + 1, 1, dtype=dtype)
+    with pytest.raises(ValueError, match="8192"):
+        more.decode(0, torch.zeros((n + 1, 2, 128), dtype=dtype, device="cuda"), window=25)
+
+
+@pytest.mark.parametrize("cache,d,single,generic", KERNELS)
+def test_a_million_tokens(cuda_device, cache, d, single, generic):
+    """One sequence past 2^20 tokens, the whole of it and a window with sinks: half of the keys have a V of 1, the
+    others 0, and a far stronger score, so that the sum over all of them is known."""
+    from snapmind_b200 import PagedKVPool, QuantizedKVPool
+
+    n, t = 2**20 + 777, 1 if single else 5
+    blocks = (n + 15) // 16
+    pool = (QuantizedKVPool if cache == "e4m3" else PagedKVPool)(1, 1, d, blocks, 1, blocks, dtype=torch.bfloat16)
+    pool.reserve(n, batch=1)
+    k = torch.zeros((1, 1, n, d), device="cuda", dtype=torch.bfloat16)
+    v = torch.zeros_like(k)
+    k[:, :, ::2, 3], v[:, :, 1::2] = 4.0, 1.0
+    pool.append(0, k, v)
+    q = torch.zeros((t, 4, d), device="cuda").bfloat16()
+    q[:, :, 3] = 4.0
+    scale = math.log(3) / 16  # even positions weigh 3, odd ones 1
+    cu = torch.tensor([0, t], dtype=torch.int32, device="cuda")
+    for window, sinks in ((0, 0), (2**19 + 1, 9)):
+        if single and cache == "same" and not window:
+            window = 2**30
+        if single:
+            out = pool.decode(0, q, scale=scale, window=window, sinks=sinks, force_generic=generic)
+        else:
+            out = pool.attend_chunk(0, q, cu, scale=scale, window=window, sinks=sinks, force_generic=generic)
+        for i in range(t):
+            pos = np.arange(n - t + i + 1)
+            pos = pos[(pos > n - t + i - window) | (pos < sinks)] if window else pos
+            odd, even = int((pos % 2).sum()), int((pos % 2 == 0).sum())
+            want = odd / (odd + 3 * even)
+            # the output's rounding, the weights' (all odd ones alike), the sums' and the scores' as in the other file
+            assert abs(float(out[i].double().mean()) - want) <= want * (2 * 2.0**-8 + 2.0**-12)
+            assert (out[i] == out[i, 0, 0]).all()
+    pool.check()
