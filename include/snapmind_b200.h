@@ -602,6 +602,99 @@ SNAPMIND_API int snapmind_paged_gqa_chunk(const void *q, int64_t q_stride_tok, i
                              int32_t num_blocks, int32_t window, int32_t sinks, int32_t flags, void *workspace,
                              int64_t workspace_bytes, int32_t *err_word, void *stream);
 
+/*
+ * snapmind_paged_gqa_chunk that also adds to every cached token the weight that the call's queries gave it:
+ *   mass[block][kv head][slot] += sum, over the call's queries i that see the token and the query heads that
+ *                                 read the kv head, of softmax(i)[token]
+ * for the layer of k_pool (mass NULL: only the attention).  Weights and sums are f32, taken from the scores anew
+ * once a row's softmax is known; the order of a sum depends on the sizes alone, so the same call gives the same
+ * bits.  A query that sees nothing adds nothing; one whose softmax is NaN makes the tokens that it sees NaN.
+ * q is read after out was written, so out must not be q.  The sequences must not share blocks, and calls that add
+ * to the same layer must not overlap on the GPU.  The workspace holds
+ * snapmind_paged_gqa_chunk_mass_workspace_bytes(...) bytes, on the terms of snapmind_paged_gqa_chunk's.  The reference returns its weights (snapmind/layers/attention/gqa.py:79-85) but
+ * keeps no sums of them.
+ */
+SNAPMIND_API int64_t snapmind_paged_gqa_chunk_mass_workspace_bytes(int32_t head_dim, int32_t total_q, int32_t n_q_heads);
+SNAPMIND_API int snapmind_paged_gqa_chunk_mass(const void *q, int64_t q_stride_tok, int64_t q_stride_head, int dtype,
+                             const void *k_pool, const void *v_pool, const void *scales, int pool_dtype,
+                             const int32_t *block_tables, int64_t table_stride_seq, int32_t table_width,
+                             const int32_t *seq_lens, const int32_t *cu_q, void *out, int64_t out_stride_tok,
+                             int64_t out_stride_head, float scale, int32_t batch, int32_t total_q,
+                             int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+                             int32_t num_blocks, int32_t window, int32_t sinks, int32_t flags, float *mass,
+                             void *workspace, int64_t workspace_bytes, int32_t *err_word, void *stream);
+
+/*
+ * Set to 0 the mass of the newest tokens of every sequence in all layers (after the reserve that
+ * made room for them): counts[b] of sequence b (device), or n_new each when counts is NULL.  Nothing happens while
+ * *err_word says that a reserve failed.
+ */
+SNAPMIND_API int snapmind_kv_clear_mass(float *mass, int64_t mass_layer_stride, const int32_t *block_tables,
+                             int64_t table_stride_seq, int32_t table_width, const int32_t *seq_lens,
+                             const int32_t *counts, int32_t n_new, int32_t batch, int32_t n_layers, int32_t n_heads,
+                             int32_t block_size, int32_t num_blocks, const int32_t *err_word, void *stream);
+
+/*
+ * Evict by accumulated weight.  Of every sequence with more than `budget` tokens each (layer, kv head) keeps the
+ * first `sinks`, the newest `recent` and those with the largest mass among the others (equal masses: the
+ * lowest index; NaN counts as the largest), `budget` in all; sinks + recent <= budget.  The kept rows of K, V
+ * (8-bit: and their scales) and their mass move to the front in their order; other slots stay as they were.
+ *   into NULL: in place.  The sequences (seqs: device ids, distinct; NULL: 0 .. n_seqs - 1) end with
+ *     min(length, budget) tokens and their last blocks go back to the free stack.
+ *   into (device ids, distinct, none of them in seqs): the sequences stay; what the targets held is replaced
+ *     by the kept tokens, their blocks grow or shrink (SNAPMIND_DEVERR_OUT_OF_BLOCKS and nothing happens
+ *     when the free stack has not enough).
+ * kept [n_layers][n_seqs][n_heads][budget] receives the kept indexes, ascending, -1 behind the last.
+ * pool_layer_stride and mass_layer_stride are in elements, scale_layer_stride in bytes.  Sequences must not share
+ * blocks.  The reference evicts the oldest tokens only (snapmind/kv_cache/paged.py evict).
+ */
+SNAPMIND_API int snapmind_kv_evict_by_mass(void *k_pool, void *v_pool, void *scales, int pool_dtype,
+                             int64_t pool_layer_stride, int64_t scale_layer_stride, float *mass,
+                             int64_t mass_layer_stride, int32_t *block_tables, int64_t table_stride_seq,
+                             int32_t table_width, int32_t *seq_lens, const int32_t *seqs, const int32_t *into,
+                             int32_t n_seqs, int32_t budget, int32_t recent, int32_t sinks, int32_t *kept,
+                             int32_t *free_stack, int32_t *free_top, int32_t n_layers, int32_t n_heads,
+                             int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t *err_word,
+                             void *stream);
+
+/*
+ * Norms of queries and keys for each head and their rotation, in one pass:
+ *   y = x / sqrt(mean(x^2) + eps) * norm   (norm NULL: y = x)
+ *   z = y * cos[p] + rotate_half(y) * sin[p] on the first rot_dim dims (snapmind/layers/positional/rope.py:47-61), z = y
+ *       behind them
+ * in f32, rounded once.  norm is [head_dim] in `dtype`, norm_stride_head elements between the heads' (0: one
+ * for all).  cos / sin tables: f32 [n_pos][rot_dim].  A position outside them sets SNAPMIND_DEVERR_POSITION,
+ * and the token is left out.
+ * snapmind_norm_rope_qk: q, k [batch][head][n_tok][head_dim] by element strides (dim contiguous) to q_out, k_out (which may be
+ *   q and k); position of token t of sequence b: positions[b * pos_stride_b + t], or t when NULL.
+ * snapmind_norm_rope_append: packed tokens q, k, v [token][head][head_dim]; q goes to q_out, the keys and values to
+ *   the pool slots that snapmind_kv_append_chunk gives them (cu_new NULL: token b is the newest of sequence b), in
+ *   the pool's type, 8-bit rows quantised in the same way from the f32 values.  Rows outside every sequence are rotated, not
+ *   stored.  positions: int64 [total_new].
+ * Extends RotaryPositionalEncoding.apply_to_qk followed by PagedKVCache.store (snapmind/kv_cache/paged.py:34-54); the
+ * reference has no norms of heads.
+ */
+SNAPMIND_API int snapmind_norm_rope_qk(const void *q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
+                             void *q_out, int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_t,
+                             int32_t n_q_heads, const void *k, int64_t k_stride_b, int64_t k_stride_h,
+                             int64_t k_stride_t, void *k_out, int64_t ko_stride_b, int64_t ko_stride_h,
+                             int64_t ko_stride_t, int32_t n_kv_heads, int dtype, const void *q_norm,
+                             int64_t q_norm_stride_h, const void *k_norm, int64_t k_norm_stride_h, float eps,
+                             int32_t batch, int32_t n_tok, int32_t head_dim, const float *cos_table,
+                             const float *sin_table, int32_t rot_dim, int64_t n_pos, const int64_t *positions,
+                             int64_t pos_stride_b, int32_t *err_word, void *stream);
+SNAPMIND_API int snapmind_norm_rope_append(const void *q, int64_t q_stride_tok, int64_t q_stride_head, void *q_out,
+                             int64_t qo_stride_tok, int64_t qo_stride_head, int32_t n_q_heads, const void *k,
+                             int64_t k_stride_tok, int64_t k_stride_head, const void *v, int64_t v_stride_tok,
+                             int64_t v_stride_head, int dtype, const void *q_norm, int64_t q_norm_stride_head,
+                             const void *k_norm, int64_t k_norm_stride_head, float eps, const float *cos_table,
+                             const float *sin_table, int32_t rot_dim, int64_t n_pos, const int64_t *positions,
+                             void *k_pool, void *v_pool, void *scales, int pool_dtype, const int32_t *block_tables,
+                             int64_t table_stride_seq, int32_t table_width, const int32_t *seq_lens,
+                             const int32_t *cu_new, int32_t batch, int32_t total_new, int32_t n_kv_heads,
+                             int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t *err_word,
+                             void *stream);
+
 #ifdef __cplusplus
 }
 #endif

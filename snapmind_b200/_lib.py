@@ -151,6 +151,32 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _i64, _i64, _int, _p, _p, _p, _int, _p, _i64, _i32, _p, _p, _p, _i64, _i64, _f32, _i32, _i32, _i32,
          _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p],
     ),
+    "snapmind_paged_gqa_chunk_mass_workspace_bytes": (_i64, [_i32, _i32, _i32]),
+    "snapmind_paged_gqa_chunk_mass": (
+        _int,
+        [_p, _i64, _i64, _int, _p, _p, _p, _int, _p, _i64, _i32, _p, _p, _p, _i64, _i64, _f32, _i32, _i32,
+         _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _p, _i64, _p, _p],
+    ),
+    "snapmind_kv_clear_mass": (
+        _int,
+        [_p, _i64, _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _p, _p],
+    ),
+    "snapmind_kv_evict_by_mass": (
+        _int,
+        [_p, _p, _p, _int, _i64, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _p,
+         _p, _i32, _i32, _i32, _i32, _i32, _p, _p],
+    ),
+    "snapmind_norm_rope_qk": (
+        _int,
+        [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32,
+         _int, _p, _i64, _p, _i64, _f32, _i32, _i32, _i32, _p, _p, _i32, _i64, _p, _i64, _p, _p],
+    ),
+    "snapmind_norm_rope_append": (
+        _int,
+        [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i64, _p, _i64, _i64, _int, _p, _i64, _p, _i64,
+         _f32, _p, _p, _i32, _i64, _p, _p, _p, _p, _int, _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _i32,
+         _i32, _i32, _p, _p],
+    ),
 }
 
 NOALLOC_DECODE_SCRATCH_BYTES = 16 << 20
@@ -243,6 +269,30 @@ def require_offsets(what: str, cu: torch.Tensor, like: torch.Tensor) -> None:
     if cu.dtype != torch.int32 or cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous():
         raise ValueError(f"{what}: offsets must be a contiguous int32 vector of batch + 1 entries")
     require_same(what, like, cu)
+
+
+def rope_args(what: str, q: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, q_norm, k_norm, n_q: int, n_kv: int,
+              eps: float) -> tuple[int, int, int]:
+    """Check the tables and norms of a norm-and-rotate call on ``q`` ``[..., D]``; returns the rotated dims and the strides
+    between the heads' norms of q and k."""
+    d = q.shape[-1]
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError(f"{what}: cos and sin must be f32 [n_pos, rotated dims] alike")
+    if not (cos.is_contiguous() and sin.is_contiguous()) or cos.shape[0] < 1 or cos.shape[1] % 2 or cos.shape[1] > d:
+        raise ValueError(f"{what}: cos and sin must be contiguous, an even number of dims, at most {d}")
+    if not eps >= 0.0:
+        raise ValueError(f"{what}: eps must not be negative")
+    strides = []
+    for w, heads in ((q_norm, n_q), (k_norm, n_kv)):
+        strides.append(0)
+        if w is None:
+            continue
+        if w.shape not in ((d,), (heads, d)) or w.dtype != q.dtype or w.stride(-1) != 1:
+            raise ValueError(f"{what}: norms must be [{d}] or [heads, {d}] in q's dtype, dims contiguous")
+        require_same(what, q, w)
+        if w.dim() == 2:
+            strides[-1] = w.stride(0)
+    return cos.shape[1], strides[0], strides[1]
 
 
 def raise_device_error(word: int, what: str) -> None:

@@ -77,6 +77,9 @@ class BlockPool:
             self.err.zero_()
             _lib.raise_device_error(word, type(self).__name__)
 
+    def _reserved(self, n_new: int, batch: int, counts: torch.Tensor | None = None) -> None:
+        """Launched behind every reserve: the first ``batch`` sequences grew by ``n_new`` tokens (``counts``: each its own)."""
+
     def reserve(self, n_new: int = 1, batch: int | None = None) -> None:
         """Grow the first ``batch`` sequences by ``n_new`` tokens (tables + lengths)."""
         batch = self.max_seqs if batch is None else batch
@@ -94,6 +97,7 @@ class BlockPool:
             self.err.data_ptr(), self._stream(),
         )  # fmt: skip
         _lib.check(status, f"{type(self).__name__}.reserve")
+        self._reserved(n_new, batch)
         self._host_lens[:batch] += n_new
         self._host_free -= need
 
@@ -122,6 +126,7 @@ class BlockPool:
                 self.err.data_ptr(), self._stream(),
             )  # fmt: skip
         _lib.check(status, f"{type(self).__name__}.reserve_each")
+        self._reserved(int(n.max()) if n.size else 0, len(n), counts)
         self._host_lens[:len(n)] += n
         self._host_free -= need
 
@@ -142,6 +147,7 @@ class BlockPool:
             self.err.data_ptr(), self._stream(),
         )  # fmt: skip
         _lib.check(status, f"{type(self).__name__}.reserve_device")
+        self._reserved(n_new, batch)
 
     def account_host(self, n_new: int, batch: int) -> None:
         """Advance the host mirrors as ``reserve(n_new, batch)`` would."""

@@ -12,7 +12,7 @@
 // tokens (32 heads over 4 of 64) take 55 us, 20 TFLOP/s of what is seen.  4 x 4 products from 8 reads, two CTAs of
 // 256 threads and loads a step ahead took 60 us (63000 wavefronts of shared memory in 92000 cycles), loads
 // element by element 92.  Larger rows need the threads: one CTA of 256, 4 x 4 products.
-#include "chunk_plan.cuh"
+#include "chunk_mass.cuh"
 #include "pairs.cuh"
 
 namespace snapmind {
@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(GenSmem<D4>::kThreads, GenSmem<D4>::kCtas) chu
         p.part_ml[slot * 2] = m[i];
         p.part_ml[slot * 2 + 1] = l[i];
       }
+      if (whole && tx == 0) write_stats(p, c.q_first + c.i0 + tok, head0 + g, m[i], l[i]);
 #pragma unroll
       for (int j = 0; j < kX; ++j) {
         const float4 y = make_float4(o[i][2 * j].x * f, o[i][2 * j].y * f, o[i][2 * j + 1].x * f, o[i][2 * j + 1].y * f);
@@ -424,6 +425,10 @@ __device__ __forceinline__ void merge_units(const ChunkParams& p) {
       float f = ml.x == -INFINITY ? ml.y : ex2(ml.x - ref), L = ml.y * f;
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      if (il == 0 && rl < n_rows) {
+        const int tok = p.by_gw.div(rl), g = rl - tok * p.gw;
+        if (g < heads) write_stats(p, first + i0 + tok, kvh * p.group + slice * p.gw + g, M, L);
+      }
       f *= L == 0.f ? 0.f : 1.f / L;  // a row that sees nothing: zeros
       if (p.means) f *= ml.y;
 #pragma unroll
@@ -497,6 +502,7 @@ __device__ __forceinline__ void merge_units(const ChunkParams& p) {
       }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
+    if (lane == 0) write_stats(p, first + i0 + p.by_gw.div(r), kvh * p.group + slice * p.gw + g, M, L);
     mul4(acc[0], inv);
     mul4(acc[1], inv);
     T* out = out_row(r, g);
@@ -589,20 +595,57 @@ int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st) {
 
 using namespace snapmind;
 
+static int64_t chunk_workspace_bytes(int32_t head_dim) { return partials_bytes(head_dim) + (max_ctas() * 4 + 255) / 256 * 256; }
+static int64_t stats_bytes(int32_t total_q, int32_t n_q_heads) { return ((int64_t)total_q * n_q_heads * 8 + 255) / 256 * 256; }
+
+// The attention of a call: the kernel that its shapes take, and the merge.
+static int launch_attention(ChunkParams& p, int dtype, int pool_dtype, int32_t flags, cudaStream_t st) {
+  const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
+  if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && decode_sinks_supported(p, dtype, pool_dtype)) {
+    const int rc = launch_decode_sinks(p, dtype, pool_dtype, st);
+    return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
+  }
+  if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && chunk_umma_supported(p, dtype, pool_dtype)) {
+    if (quant && dtype == SNAPMIND_DTYPE_F16) {
+      p.odd = reinterpret_cast<int32_t*>(static_cast<char*>(p.workspace) + partials_bytes(p.head_dim));
+      const int rc = launch_f16_over_e4m3(p, st);
+      if (rc != SNAPMIND_ERR_UNSUPPORTED) return rc;
+      p.odd = nullptr;
+    }
+    const int rc = launch_chunk_umma(p, dtype, pool_dtype, st);
+    if (rc != SNAPMIND_ERR_UNSUPPORTED) return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
+  }
+  int rc = plan_generic(p);
+  if (rc != SNAPMIND_OK) return rc;
+  switch (dtype) {
+    case SNAPMIND_DTYPE_F32: rc = quant ? launch_generic<float, uint8_t>(p, st) : launch_generic<float, float>(p, st); break;
+    case SNAPMIND_DTYPE_BF16:
+      rc = quant ? launch_generic<__nv_bfloat16, uint8_t>(p, st) : launch_generic<__nv_bfloat16, __nv_bfloat16>(p, st);
+      break;
+    default: rc = quant ? launch_generic<__half, uint8_t>(p, st) : launch_generic<__half, __half>(p, st); break;
+  }
+  return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
+}
+
 extern "C" {
 
 int64_t snapmind_paged_gqa_chunk_workspace_bytes(int32_t head_dim) {
-  if (head_dim <= 0 || head_dim > kGenMaxD) return 0;
-  return partials_bytes(head_dim) + (max_ctas() * 4 + 255) / 256 * 256;
+  return head_dim <= 0 || head_dim > kGenMaxD ? 0 : chunk_workspace_bytes(head_dim);
 }
 
-int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stride_head, int dtype, const void* k_pool,
+int64_t snapmind_paged_gqa_chunk_mass_workspace_bytes(int32_t head_dim, int32_t total_q, int32_t n_q_heads) {
+  if (head_dim <= 0 || head_dim > kGenMaxD || total_q < 0 || n_q_heads <= 0) return 0;
+  return chunk_workspace_bytes(head_dim) + stats_bytes(total_q, n_q_heads) + mass_workspace_bytes();
+}
+
+int snapmind_paged_gqa_chunk_mass(const void* q, int64_t q_stride_tok, int64_t q_stride_head, int dtype, const void* k_pool,
                              const void* v_pool, const void* scales, int pool_dtype, const int32_t* block_tables,
                              int64_t table_stride_seq, int32_t table_width, const int32_t* seq_lens,
                              const int32_t* cu_q, void* out, int64_t out_stride_tok, int64_t out_stride_head,
                              float scale, int32_t batch, int32_t total_q, int32_t n_q_heads, int32_t n_kv_heads,
                              int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t window, int32_t sinks,
-                             int32_t flags, void* workspace, int64_t workspace_bytes, int32_t* err_word, void* stream) {
+                             int32_t flags, float* mass, void* workspace, int64_t workspace_bytes, int32_t* err_word,
+                             void* stream) {
   SNAPMIND_CHECK_ARG(dtype_size(dtype) > 0, "paged_chunk: unknown dtype");
   SNAPMIND_CHECK_ARG(pool_dtype == dtype || pool_dtype == SNAPMIND_DTYPE_E4M3,
                      "paged_chunk: the pool holds the query's dtype or e4m3");
@@ -650,38 +693,32 @@ int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stri
   const int64_t room = (int64_t)table_width * block_size;
   p.max_len = room < (1 << 30) ? (int32_t)room : (1 << 30);
   p.err = err_word;
-  const int64_t need = snapmind_paged_gqa_chunk_workspace_bytes(head_dim);
+  const int64_t attention = chunk_workspace_bytes(head_dim);
+  const int64_t need = mass ? snapmind_paged_gqa_chunk_mass_workspace_bytes(head_dim, total_q, n_q_heads) : attention;
   SNAPMIND_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                      "paged_chunk: workspace needs %lld bytes on a 256-byte boundary, got %lld", (long long)need,
                      (long long)workspace_bytes);
   p.workspace = workspace;
   p.odd = nullptr;
+  char* more = static_cast<char*>(workspace) + attention;  // the rows' statistics, then what the pass over the weights needs
+  p.stats = mass ? reinterpret_cast<float2*>(more) : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
-  if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && decode_sinks_supported(p, dtype, pool_dtype)) {
-    const int rc = launch_decode_sinks(p, dtype, pool_dtype, st);
-    return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
-  }
-  if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && chunk_umma_supported(p, dtype, pool_dtype)) {
-    if (quant && dtype == SNAPMIND_DTYPE_F16) {
-      p.odd = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + partials_bytes(head_dim));
-      const int rc = launch_f16_over_e4m3(p, st);
-      if (rc != SNAPMIND_ERR_UNSUPPORTED) return rc;
-      p.odd = nullptr;
-    }
-    const int rc = launch_chunk_umma(p, dtype, pool_dtype, st);
-    if (rc != SNAPMIND_ERR_UNSUPPORTED) return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
-  }
-  int rc = plan_generic(p);
-  if (rc != SNAPMIND_OK) return rc;
-  switch (dtype) {
-    case SNAPMIND_DTYPE_F32: rc = quant ? launch_generic<float, uint8_t>(p, st) : launch_generic<float, float>(p, st); break;
-    case SNAPMIND_DTYPE_BF16:
-      rc = quant ? launch_generic<__nv_bfloat16, uint8_t>(p, st) : launch_generic<__nv_bfloat16, __nv_bfloat16>(p, st);
-      break;
-    default: rc = quant ? launch_generic<__half, uint8_t>(p, st) : launch_generic<__half, __half>(p, st); break;
-  }
-  return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
+  int rc = launch_attention(p, dtype, pool_dtype, flags, st);
+  if (rc != SNAPMIND_OK || !mass) return rc;
+  return launch_mass(p, dtype, pool_dtype, mass, more + stats_bytes(total_q, n_q_heads), st);
+}
+
+int snapmind_paged_gqa_chunk(const void* q, int64_t q_stride_tok, int64_t q_stride_head, int dtype, const void* k_pool,
+                             const void* v_pool, const void* scales, int pool_dtype, const int32_t* block_tables,
+                             int64_t table_stride_seq, int32_t table_width, const int32_t* seq_lens,
+                             const int32_t* cu_q, void* out, int64_t out_stride_tok, int64_t out_stride_head,
+                             float scale, int32_t batch, int32_t total_q, int32_t n_q_heads, int32_t n_kv_heads,
+                             int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t window, int32_t sinks,
+                             int32_t flags, void* workspace, int64_t workspace_bytes, int32_t* err_word, void* stream) {
+  return snapmind_paged_gqa_chunk_mass(q, q_stride_tok, q_stride_head, dtype, k_pool, v_pool, scales, pool_dtype, block_tables,
+                                       table_stride_seq, table_width, seq_lens, cu_q, out, out_stride_tok, out_stride_head,
+                                       scale, batch, total_q, n_q_heads, n_kv_heads, head_dim, block_size, num_blocks, window,
+                                       sinks, flags, nullptr, workspace, workspace_bytes, err_word, stream);
 }
 
 }  // extern "C"

@@ -772,6 +772,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         p.part_ml[slot * 2] = m;
         p.part_ml[slot * 2 + 1] = l;
       }
+      if (whole && mine) write_stats(p, c.q_first + c.i0 + tok, c.kvh * p.group + c.slice * p.gw + g, m, l);
       if (whole) {  // sees nothing: zeros
         const float inv = l == 0.f ? 0.f : 1.f / l;
         f *= inv;

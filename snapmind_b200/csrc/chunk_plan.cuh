@@ -51,6 +51,7 @@ struct ChunkParams {
   int32_t* odd;     // workspace: [n_odd] whether a CTA met rows that its kernel's types do not hold, or NULL
   int32_t n_odd;
   int32_t means;    // part_o holds a piece's weighted means of V (else its weighted sums)
+  float2* stats;    // [total_q][n_q_heads] reference (log2 units) and 1 / sum of every row's softmax, or NULL
   int32_t* err;
 };
 
@@ -146,27 +147,13 @@ __device__ __forceinline__ int cta_of(long long t, long long total, int n) {
   return (int)(x < (1ll << 32) && total < (1ll << 32) ? (long long)((uint32_t)x / (uint32_t)total) : x / total);
 }
 
-// The block's share of the line: fills S (total, t0, t1, first piece).  `tiles` is
-// scratch for batch ints.  Every thread of the block calls it; ends with a barrier.
-__device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* tiles) {
+// Where this CTA's share of a line begins and ends, with per_head units' worth of tiles[b] tiles for
+// every sequence: fills S (total, n, t0, t1 and, if the share holds a tile, b, u, rem).  Every thread of the block
+// calls it, with tiles[] visible; what warp 0 reads of S it may read at once, the others after a barrier.
+__device__ inline void line_share(const ChunkParams& p, PlanShared& S, const int32_t* tiles, int per_head) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
-  const int per_head = p.n_kv_heads * p.n_slices;
-  if (p.cu_q == nullptr) {
-    for (int b = tid; b < p.batch; b += blockDim.x) {
-      const int len = clamp_len(p, b);
-      check_len(p, len);
-      tiles[b] = key_tiles(p, len, 1, 0);
-    }
-  } else {
-    for (int b = warp; b < p.batch; b += nw) {
-      const int s = seq_tiles(p, b, lane);
-      if (lane == 0) tiles[b] = s;
-    }
-  }
-  __syncthreads();
-  // The tile line's length, and where this CTA's share begins.  Up to kWarpBatch sequences: every
-  // warp goes over them, 32 a step (no barrier, the last step finds the place); more: one run of
-  // sequences per thread and a scan over the block.
+  // Up to kWarpBatch sequences: every warp goes over them, 32 a step (no barrier, the last step finds the
+  // place); more: one run of sequences per thread and a scan over the block.
   constexpr int kWarpBatch = 256;
   long long t0, t1;
   if (p.batch <= kWarpBatch) {
@@ -246,7 +233,28 @@ __device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* 
     }
     __syncthreads();
   }
-  if (warp == 0 && t0 < t1) {
+}
+
+// The block's share of the line: fills S (total, t0, t1, first piece).  `tiles` is
+// scratch for batch ints.  Every thread of the block calls it; ends with a barrier.
+__device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* tiles) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  const int per_head = p.n_kv_heads * p.n_slices;
+  if (p.cu_q == nullptr) {
+    for (int b = tid; b < p.batch; b += blockDim.x) {
+      const int len = clamp_len(p, b);
+      check_len(p, len);
+      tiles[b] = key_tiles(p, len, 1, 0);
+    }
+  } else {
+    for (int b = warp; b < p.batch; b += nw) {
+      const int s = seq_tiles(p, b, lane);
+      if (lane == 0) tiles[b] = s;
+    }
+  }
+  __syncthreads();
+  line_share(p, S, tiles, per_head);
+  if (warp == 0 && S.t0 < S.t1) {
     Piece f;
     f.b = S.b;
     int hs = (int)__fdividef((float)S.rem, (float)S.u);  // off by one at most: hs is small
@@ -280,7 +288,7 @@ __device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* 
       }
       rem -= __shfl_sync(0xffffffffu, x, 31);
     }
-    f.tile1 = (int)min((long long)f.n_tiles, f.tile0 + (t1 - t0));
+    f.tile1 = (int)min((long long)f.n_tiles, f.tile0 + (S.t1 - S.t0));
     if (lane == 0) S.first = f;
   }
   __syncthreads();
@@ -421,6 +429,13 @@ __device__ inline void write_piece_info(const ChunkParams& p, const PlanShared& 
   h[6] = c.q_first;
   h[7] = c.n;
   h[0] = c.b;
+}
+
+// A finished row's softmax, for the kernel that adds its weights to their keys (chunk_mass.cu): the weight of
+// a key is 2^(score - x) y.  A row that sees nothing: 0, 0.
+__device__ __forceinline__ void write_stats(const ChunkParams& p, int64_t row, int head, float M, float L) {
+  if (p.stats != nullptr)
+    p.stats[row * p.n_q_heads + head] = make_float2(M == -INFINITY ? 0.f : M, L == 0.f ? 0.f : 1.f / L);
 }
 
 // 2^x by the hardware approximation (2 ulp); -inf -> 0.

@@ -87,6 +87,7 @@ template <> struct VecT<16> { using type = Vec16; };
 template <> struct VecT<8> { using type = Vec8; };
 template <> struct VecT<4> { using type = uint32_t; };
 template <> struct VecT<2> { using type = uint16_t; };
+template <> struct VecT<1> { using type = uint8_t; };
 
 // Largest power-of-two vector width (<= 16 bytes) dividing every given value.
 inline int vec_width(int64_t a, int64_t b = 0, int64_t c = 0, int64_t d = 0, int64_t e = 0) {

@@ -488,6 +488,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * half * half;
         }
         if (c.whole()) {
+          if (d == 0) write_stats(p, c.q_first, head0 + h, M, L);
           if constexpr (!kQuant)
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] *= inv;

@@ -1,0 +1,442 @@
+// Eviction from a paged cache by accumulated attention weight: per (layer, sequence, kv head) the first
+// `sinks` tokens, the newest `recent` and, of the others, those with the most weight stay (equal ones: the lowest
+// index), up to `budget`, and move to the front in their order.
+//
+//   select  the kept indexes of every (layer, sequence, head), and their weights to their new places;
+//   move    the kept rows of K and V (and 8-bit scales);
+//   tables  lengths, table rows and the free stack (before the others when the rows go to other sequences).
+//
+// In place is safe because the i-th kept token stands at index p_i >= i: rows move towards the front in
+// ascending order, a batch is read whole before it is written, and what a batch overwrites lies in front of all
+// that is still to be read.
+#include "common.cuh"
+
+namespace snapmind {
+namespace {
+
+struct EvictParams {
+  int32_t* tables;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t* seq_lens;
+  const int32_t* src;  // [n] sequence ids, NULL: 0 .. n - 1
+  const int32_t* dst;  // [n], NULL: in place
+  int32_t n, n_layers, n_heads, block_size, num_blocks, budget, recent, sinks;
+  FastDiv by_block, by_heads, by_units;  // by_units: n * n_heads
+  float* mass;
+  int64_t mass_layer;  // elements
+  int32_t* kept;       // [n_layers][n][n_heads][budget]
+  uint8_t* pool[2];
+  int64_t pool_layer;  // bytes
+  uint8_t* scales;
+  int64_t scale_layer;  // bytes
+  int32_t row_bytes;
+  int32_t slices, slice_bytes;  // a row's bytes are moved by `slices` CTAs
+  int32_t* free_stack;
+  int32_t* free_top;
+  int32_t* err;
+};
+
+__device__ __forceinline__ int src_id(const EvictParams& p, int i) { return p.src ? p.src[i] : i; }
+__device__ __forceinline__ int dst_id(const EvictParams& p, int i) { return p.dst ? p.dst[i] : src_id(p, i); }
+__device__ __forceinline__ int cached(const EvictParams& p, int seq) {
+  const int64_t room = (int64_t)p.table_width * p.block_size;
+  return (int)min((int64_t)max(0, p.seq_lens[seq]), room);
+}
+// Pool row of index j of the sequence whose table row is `table`, -1 (flagged): its entry is no block.
+__device__ __forceinline__ int64_t row_of(const EvictParams& p, const int32_t* table, int head, int j) {
+  const int k = p.by_block.div(j);
+  const int32_t phys = table[k];
+  if (phys < 0 || phys >= p.num_blocks) {
+    flag_error(p.err, SNAPMIND_DEVERR_BLOCK_ID);
+    return -1;
+  }
+  return ((int64_t)phys * p.n_heads + head) * p.block_size + (j - k * p.block_size);
+}
+
+// Order of weights as unsigned integers: -infinity lowest, infinity below NaN.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return (u & 0x7FFFFFFFu) > 0x7F800000u ? 0xFFFFFFFFu : u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int kSelectThreads = 512, kRadix = 11, kBins = 1 << kRadix;
+constexpr int kHeld = 8192;  // indexes whose order stays in shared memory
+
+struct SelectSmem {
+  uint32_t key[kHeld];
+  int32_t bins[kBins];
+  int32_t warp_sum[kSelectThreads / 32];
+  int32_t carry;
+  uint32_t prefix;  // of the lowest kept order
+  int32_t need;     // how many with exactly that order stay
+};
+
+__device__ __forceinline__ int block_scan(SelectSmem& S, int x, int* total) {  // exclusive
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  __syncthreads();
+  if (lane == 31) S.warp_sum[warp] = incl;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kSelectThreads / 32; ++w) {
+    if (w < warp) before += S.warp_sum[w];
+    all += S.warp_sum[w];
+  }
+  *total = all;
+  return before + incl - x;
+}
+
+__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
+  __shared__ SelectSmem S;
+  const int tid = threadIdx.x;
+  const int layer = blockIdx.x / (p.n * p.n_heads), u = blockIdx.x - layer * (p.n * p.n_heads);
+  const int i = u / p.n_heads, head = u - i * p.n_heads;
+  const int from = src_id(p, i), to = dst_id(p, i);
+  const int len = cached(p, from), keep = min(len, p.budget);
+  int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
+  float* mass = p.mass + layer * p.mass_layer;
+  const int32_t* table = p.tables + (int64_t)from * p.table_stride;
+  const int32_t* new_table = p.tables + (int64_t)to * p.table_stride;
+  const bool copies = p.dst != nullptr;
+  if (copies && p.seq_lens[to] != keep) return;  // it was not given its blocks
+  for (int x = keep + tid; x < p.budget; x += kSelectThreads) kept[x] = -1;
+  if (len <= p.budget) {
+    for (int x = tid; x < keep; x += kSelectThreads) {
+      kept[x] = x;
+      if (copies) {
+        const int64_t a = row_of(p, table, head, x), b = row_of(p, new_table, head, x);
+        if (a >= 0 && b >= 0) mass[b] = mass[a];
+      }
+    }
+    return;
+  }
+  // what stays in any case takes no part: [0, lo) and [hi, len)
+  const int lo = min(p.sinks, keep), hi = len - min(p.recent, keep - lo);
+  const auto weight = [&](int x) {
+    const int64_t row = row_of(p, table, head, x);
+    return row < 0 ? 0u : order_of(mass[row]);
+  };
+  for (int x = lo + tid; x < hi; x += kSelectThreads)
+    if (x - lo < kHeld) S.key[x - lo] = weight(x);
+  const auto key = [&](int x) { return x - lo < kHeld ? S.key[x - lo] : weight(x); };
+  int need = keep - lo - (len - hi);  // of [lo, hi)
+  uint32_t prefix = 0;
+  int shift = 32;
+  // the order of the need-th largest, 11, 11 and 10 bits at a time
+  for (int pass = 0; pass < 3 && need > 0; ++pass) {
+    const int bits = pass < 2 ? kRadix : 32 - 2 * kRadix;
+    const uint32_t above = shift == 32 ? 0u : prefix >> shift;
+    __syncthreads();
+    for (int x = tid; x < kBins; x += kSelectThreads) S.bins[x] = 0;
+    __syncthreads();
+    for (int x = lo + tid; x < hi; x += kSelectThreads) {
+      const uint32_t k = key(x);
+      if (shift == 32 || k >> shift == above) atomicAdd(&S.bins[(k >> (shift - bits)) & ((1u << bits) - 1)], 1);
+    }
+    __syncthreads();
+    // from the highest bin down: the bin where the count reaches `need`
+    constexpr int kPer = kBins / kSelectThreads;
+    int mine[kPer], sum = 0;
+#pragma unroll
+    for (int y = 0; y < kPer; ++y) {
+      const int bin = kBins - 1 - (tid * kPer + y);
+      mine[y] = S.bins[bin];
+      sum += mine[y];
+    }
+    int total, before = block_scan(S, sum, &total);
+#pragma unroll
+    for (int y = 0; y < kPer; ++y) {
+      if (before < need && before + mine[y] >= need) {
+        S.prefix = prefix | (uint32_t)(kBins - 1 - (tid * kPer + y)) << (shift - bits);
+        S.need = need - before;
+      }
+      before += mine[y];
+    }
+    __syncthreads();
+    prefix = S.prefix;
+    need = S.need;
+    shift -= bits;
+  }
+  const bool none = keep - lo - (len - hi) <= 0;
+  // in ascending order: what is above the border stays, of those on it the first `need`
+  int at = 0, equal = 0;
+  for (int base = 0; base < len; base += kSelectThreads) {
+    const int x = base + tid;
+    const bool sure = x < lo || (x >= hi && x < len);
+    const bool may = x >= lo && x < hi && !none;
+    const uint32_t k = may ? key(x) : 0u;
+    const bool on = may && k == prefix;
+    int here;
+    const int rank = block_scan(S, on, &here);
+    const bool stays = sure || (may && k > prefix) || (on && equal + rank < need);
+    equal += here;
+    float m = 0.f;
+    if (stays) {
+      const int64_t a = row_of(p, table, head, x);
+      if (a >= 0) m = mass[a];
+    }
+    int kept_here;
+    const int place = at + block_scan(S, stays, &kept_here);  // its barriers part the reads from the writes
+    if (stays) {
+      kept[place] = x;
+      const int64_t b = row_of(p, new_table, head, place);
+      if (b >= 0) mass[b] = m;
+    }
+    at += kept_here;
+  }
+}
+
+// Rows of the kept tokens of one (layer, sequence, head), slice_bytes of each K or V row.
+template <int W>
+__global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ EvictParams p) {
+  using V = typename VecT<W>::type;
+  constexpr int kDeep = 8;
+  const int unit = blockIdx.x, kv = blockIdx.y & 1, slice = blockIdx.y >> 1;
+  const int layer = unit / (p.n * p.n_heads), u = unit - layer * (p.n * p.n_heads);
+  const int i = u / p.n_heads, head = u - i * p.n_heads;
+  const int from = src_id(p, i), to = dst_id(p, i);
+  const int len = cached(p, from), keep = min(len, p.budget);
+  const bool copies = p.dst != nullptr;
+  if (copies ? p.seq_lens[to] != keep : len <= p.budget) return;
+  const int32_t* kept = p.kept + (int64_t)unit * p.budget;
+  const int32_t* table = p.tables + (int64_t)from * p.table_stride;
+  const int32_t* new_table = p.tables + (int64_t)to * p.table_stride;
+  uint8_t* pool = p.pool[kv] + layer * p.pool_layer + slice * p.slice_bytes;
+  uint8_t* scales = p.scales ? p.scales + layer * p.scale_layer : nullptr;
+  const int vecs = min(p.slice_bytes, p.row_bytes - slice * p.slice_bytes) / W;  // of a row
+  int first = 0;
+  if (!copies) {  // p_i - i never falls: the first that moves
+    int hi = keep;
+    while (first < hi) {
+      const int mid = (first + hi) >> 1;
+      if (kept[mid] > mid) hi = mid;
+      else first = mid + 1;
+    }
+  }
+  const int rows = blockDim.x / vecs;  // a pass
+  const int r = threadIdx.x / vecs, x = threadIdx.x - r * vecs;
+  const auto scale_at = [&](int64_t row) {
+    const int64_t block = row / p.block_size;
+    return (block * 2 + kv) * p.block_size + (row - block * p.block_size);
+  };
+  for (int base = first; base < keep; base += rows * kDeep) {
+    V v[kDeep];
+    uint8_t sc[kDeep];
+    int64_t b[kDeep];
+#pragma unroll
+    for (int y = 0; y < kDeep; ++y) {
+      const int k = base + y * rows + r;
+      b[y] = -1;
+      if (r < rows && k < keep) {
+        const int64_t a = row_of(p, table, head, kept[k]);
+        b[y] = a < 0 ? -1 : row_of(p, new_table, head, k);
+        if (b[y] >= 0) {
+          v[y] = *reinterpret_cast<const V*>(pool + a * p.row_bytes + x * W);
+          if (scales && slice == 0 && x == 0) sc[y] = scales[scale_at(a)];
+        }
+      }
+    }
+    if (!copies) __syncthreads();
+#pragma unroll
+    for (int y = 0; y < kDeep; ++y)
+      if (b[y] >= 0) {
+        *reinterpret_cast<V*>(pool + b[y] * p.row_bytes + x * W) = v[y];
+        if (scales && slice == 0 && x == 0) scales[scale_at(b[y])] = sc[y];
+      }
+  }
+}
+
+// Lengths, table rows and the free stack, by one block.  Sequence i of the call ends with
+// min(length of its source, budget) tokens.  Blocks are taken from the top of the stack in ascending order of
+// the call's sequences and come back in the reverse order, so that a pool that grows and evicts in turn gets the
+// same blocks again.
+constexpr int kTableThreads = 1024;
+__global__ void __launch_bounds__(kTableThreads) evict_tables_kernel(const __grid_constant__ EvictParams p) {
+  __shared__ int32_t s_pop[32], s_push[32];
+  __shared__ int32_t s_total[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int run = (p.n + kTableThreads - 1) / kTableThreads;
+  const int i0 = min(p.n, tid * run), i1 = min(p.n, i0 + run);
+  const auto blocks = [&](int len) { return p.by_block.div(len + p.block_size - 1); };
+  const auto ends = [&](int i) { return min(cached(p, src_id(p, i)), p.budget); };
+  int pop = 0, push = 0;
+  for (int i = i0; i < i1; ++i) {
+    const int d = blocks(ends(i)) - blocks(cached(p, dst_id(p, i)));
+    pop += max(d, 0);
+    push += max(-d, 0);
+  }
+  int a = pop, b = push;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) a += x, b += y;
+  }
+  if (lane == 31) s_pop[warp] = a, s_push[warp] = b;
+  __syncthreads();
+  if (tid == 0) {
+    int x = 0, y = 0;
+    for (int w = 0; w < kTableThreads / 32; ++w) {
+      const int px = s_pop[w], py = s_push[w];
+      s_pop[w] = x, s_push[w] = y;
+      x += px, y += py;
+    }
+    s_total[0] = x, s_total[1] = y;
+  }
+  __syncthreads();
+  const int top = *p.free_top, pops = s_total[0], pushes = s_total[1];
+  const int left = top - pops, end = left + pushes;
+  if (left < 0 || end > p.num_blocks) {  // nothing changes
+    if (tid == 0) flag_error(p.err, SNAPMIND_DEVERR_OUT_OF_BLOCKS);
+    return;
+  }
+  // every length is read before one is written: a source is no target of another sequence
+  int x = s_pop[warp] + a - pop, y = s_push[warp] + b - push;
+  // all that is popped is read before anything is pushed over it
+  for (int i = i0; i < i1; ++i) {
+    const int d = dst_id(p, i), old = blocks(cached(p, d)), now = blocks(ends(i));
+    int32_t* table = p.tables + (int64_t)d * p.table_stride;
+    for (int k = old; k < now; ++k) table[k] = p.free_stack[top - 1 - x++];
+  }
+  __syncthreads();
+  for (int i = i0; i < i1; ++i) {
+    const int d = dst_id(p, i), old = blocks(cached(p, d)), len = ends(i), now = blocks(len);
+    const int32_t* table = p.tables + (int64_t)d * p.table_stride;
+    for (int k = now; k < old; ++k) p.free_stack[end - 1 - y++] = table[k];
+  }
+  __syncthreads();
+  // in place a sequence's own length is its source's: after all reads of its own
+  for (int i = i0; i < i1; ++i) {
+    const int len = ends(i);
+    p.seq_lens[dst_id(p, i)] = len;
+  }
+  if (tid == 0) *p.free_top = end;
+}
+
+// Weights of the newest tokens of every sequence: 0, in all layers.  Not after a reserve that failed.
+struct ClearParams {
+  float* mass;
+  int64_t mass_layer;
+  const int32_t* tables;
+  int64_t table_stride;
+  int32_t table_width;
+  const int32_t* seq_lens;
+  const int32_t* counts;  // NULL: n_new each
+  int32_t n_new, batch, n_layers, n_heads, block_size, num_blocks;
+  const int32_t* err;
+};
+__global__ void __launch_bounds__(256) clear_mass_kernel(const __grid_constant__ ClearParams p) {
+  if (p.err != nullptr && (*p.err & (SNAPMIND_DEVERR_OUT_OF_BLOCKS | SNAPMIND_DEVERR_TABLE)) != 0) return;
+  const int per = p.n_layers * p.n_heads;
+  for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
+    const int len = p.seq_lens[b], n = min(p.counts ? p.counts[b] : p.n_new, len);
+    for (int64_t e = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; e < (int64_t)n * per; e += (int64_t)gridDim.x * blockDim.x) {
+      // (layer, head) outer, tokens inner: a block's slots lie side by side
+      const int lh = (int)(e / n), j = len - n + (int)(e - (int64_t)lh * n);
+      const int layer = lh / p.n_heads, head = lh - layer * p.n_heads, k = j / p.block_size;
+      if (k >= p.table_width) continue;
+      const int32_t phys = p.tables[(int64_t)b * p.table_stride + k];
+      if (phys < 0 || phys >= p.num_blocks) continue;
+      p.mass[layer * p.mass_layer + ((int64_t)phys * p.n_heads + head) * p.block_size + (j - k * p.block_size)] = 0.f;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace snapmind
+
+using namespace snapmind;
+
+extern "C" {
+
+int snapmind_kv_evict_by_mass(void* k_pool, void* v_pool, void* scales, int pool_dtype, int64_t pool_layer_stride,
+                              int64_t scale_layer_stride, float* mass, int64_t mass_layer_stride, int32_t* block_tables,
+                              int64_t table_stride_seq, int32_t table_width, int32_t* seq_lens, const int32_t* seqs,
+                              const int32_t* into, int32_t n_seqs, int32_t budget, int32_t recent, int32_t sinks,
+                              int32_t* kept, int32_t* free_stack, int32_t* free_top, int32_t n_layers, int32_t n_heads,
+                              int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t* err_word, void* stream) {
+  const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
+  SNAPMIND_CHECK_ARG(quant || dtype_size(pool_dtype) > 0, "kv_evict: unknown pool dtype");
+  SNAPMIND_CHECK_ARG(quant == (scales != nullptr), "kv_evict: scales go with an e4m3 pool, and only with one");
+  SNAPMIND_CHECK_ARG(n_seqs >= 0 && n_layers > 0 && n_heads > 0 && head_dim > 0 && block_size > 0 && num_blocks > 0 && table_width >= 0,
+                     "kv_evict: bad sizes");
+  SNAPMIND_CHECK_ARG(budget > 0 && recent >= 0 && sinks >= 0 && (int64_t)recent + sinks <= budget,
+                     "kv_evict: the newest %d and the first %d tokens do not fit a budget of %d", recent, sinks, budget);
+  SNAPMIND_CHECK_ARG((int64_t)table_width * block_size < (int64_t)1 << 31, "kv_evict: table rows of %d blocks are too long", table_width);
+  const int64_t units = (int64_t)n_layers * n_seqs * n_heads;
+  SNAPMIND_CHECK_ARG(units < (int64_t)1 << 31, "kv_evict: too many layers, sequences and heads for one call");
+  if (n_seqs == 0) return SNAPMIND_OK;
+  SNAPMIND_CHECK_ARG(k_pool && v_pool && mass && block_tables && seq_lens && kept && free_stack && free_top, "kv_evict: null pointer");
+  SNAPMIND_CHECK_ARG(into == nullptr || seqs != nullptr, "kv_evict: targets need the sequences named");
+  EvictParams p = {};
+  p.tables = block_tables;
+  p.table_stride = table_stride_seq;
+  p.table_width = table_width;
+  p.seq_lens = seq_lens;
+  p.src = seqs;
+  p.dst = into;
+  p.n = n_seqs;
+  p.n_layers = n_layers;
+  p.n_heads = n_heads;
+  p.block_size = block_size;
+  p.num_blocks = num_blocks;
+  p.budget = budget;
+  p.recent = recent;
+  p.sinks = sinks;
+  p.by_block = FastDiv(block_size);
+  p.mass = mass;
+  p.mass_layer = mass_layer_stride;
+  p.kept = kept;
+  p.pool[0] = static_cast<uint8_t*>(k_pool);
+  p.pool[1] = static_cast<uint8_t*>(v_pool);
+  const int esz = quant ? 1 : dtype_size(pool_dtype);
+  p.row_bytes = head_dim * esz;
+  p.pool_layer = pool_layer_stride * esz;
+  p.scales = static_cast<uint8_t*>(scales);
+  p.scale_layer = scale_layer_stride;
+  p.free_stack = free_stack;
+  p.free_top = free_top;
+  p.err = err_word;
+  p.slices = 1;
+  p.slice_bytes = p.row_bytes;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (into) evict_tables_kernel<<<1, kTableThreads, 0, st>>>(p);
+  evict_select_kernel<<<(uint32_t)units, kSelectThreads, 0, st>>>(p);
+  int w = vec_width(p.row_bytes, p.pool_layer, reinterpret_cast<intptr_t>(k_pool), reinterpret_cast<intptr_t>(v_pool));
+  SNAPMIND_CHECK_ARG(p.row_bytes / w <= 256, "kv_evict: rows of %d bytes are too long", p.row_bytes);
+  const dim3 grid((uint32_t)units, 2 * p.slices);
+  switch (w) {
+    case 16: evict_move_kernel<16><<<grid, 256, 0, st>>>(p); break;
+    case 8: evict_move_kernel<8><<<grid, 256, 0, st>>>(p); break;
+    case 4: evict_move_kernel<4><<<grid, 256, 0, st>>>(p); break;
+    case 2: evict_move_kernel<2><<<grid, 256, 0, st>>>(p); break;
+    default: evict_move_kernel<1><<<grid, 256, 0, st>>>(p);
+  }
+  if (!into) evict_tables_kernel<<<1, kTableThreads, 0, st>>>(p);
+  return cuda_status(cudaGetLastError(), "kv_evict launch");
+}
+
+int snapmind_kv_clear_mass(float* mass, int64_t mass_layer_stride, const int32_t* block_tables, int64_t table_stride_seq,
+                           int32_t table_width, const int32_t* seq_lens, const int32_t* counts, int32_t n_new, int32_t batch,
+                           int32_t n_layers, int32_t n_heads, int32_t block_size, int32_t num_blocks,
+                           const int32_t* err_word, void* stream) {
+  SNAPMIND_CHECK_ARG(batch >= 0 && n_new >= 0 && n_layers > 0 && n_heads > 0 && block_size > 0 && num_blocks > 0 && table_width >= 0,
+                     "kv_clear_mass: bad sizes");
+  if (batch == 0 || (counts == nullptr && n_new == 0)) return SNAPMIND_OK;
+  SNAPMIND_CHECK_ARG(mass && block_tables && seq_lens, "kv_clear_mass: null pointer");
+  const ClearParams p{mass, mass_layer_stride, block_tables, table_stride_seq, table_width, seq_lens, counts, n_new,
+                      batch, n_layers, n_heads, block_size, num_blocks, err_word};
+  const int64_t each = counts ? 4096 : (int64_t)n_new * n_layers * n_heads;
+  const int64_t blocks = (each + 255) / 256;
+  const dim3 grid((uint32_t)(blocks < 64 ? blocks : 64), (uint32_t)(batch < 1024 ? batch : 1024));
+  clear_mass_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return cuda_status(cudaGetLastError(), "kv_clear_mass launch");
+}
+
+}  // extern "C"

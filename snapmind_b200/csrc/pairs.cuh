@@ -55,4 +55,25 @@ __device__ __forceinline__ float e4m3_to_f(uint8_t c) { return __half2float(__ha
 // 2^(b - 127) of a scale byte in [27, 247] (a normal float's exponent field).
 __device__ __forceinline__ float scale_byte_to_f(uint32_t b) { return __uint_as_float(b << 23); }
 
+// e4m3 rows: the exponent of a row whose largest finite magnitude is a.
+__device__ __forceinline__ int row_exponent(float a) {
+  const uint32_t u = __float_as_uint(a);
+  const int k = (int)(u >> 23) - 127;
+  const int e = (u & 0x7FFFFFu) <= 0x600000u ? k - 8 : k - 7;  // a <= 1.75 2^(e + 8)
+  return min(max(e, -100), 120);
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a < INFINITY ? a : 0.f;  // false for NaN too
+}
+__device__ __forceinline__ float scaled(float x, float inv) {
+  return fabsf(x) < INFINITY ? x * inv : __uint_as_float(0x7FC00000u);
+}
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
 }  // namespace snapmind

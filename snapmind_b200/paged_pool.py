@@ -9,7 +9,10 @@ over one shared pool; this class is that extension, with all state on the GPU:
 * ``block_tables`` int32 ``[max_seqs][max_blocks_per_seq]``, ``seq_lens`` int32;
 * a device free stack (``free_stack``, ``free_top``) from which
   ``snapmind_kv_reserve`` grows tables deterministically (ascending sequence
-  order, blocks from the top of the stack).
+  order, blocks from the top of the stack);
+* with ``mass=True`` also ``mass``, f32 ``[layer][block][head][slot]``: the attention weight
+  that each cached token got from the calls with ``accumulate=True`` (zero when ``reserve``
+  makes room for it), by which ``evict`` thins the sequences.
 
 Block bookkeeping (tables, lengths, free stack, reserve/release) is in
 :class:`snapmind_b200.block_pool.BlockPool`.
@@ -45,6 +48,7 @@ class PagedKVPool(BlockPool):
         block_size: int = 16,
         dtype: torch.dtype = torch.bfloat16,
         device: torch.device | str | None = None,
+        mass: bool = False,
     ):
         super().__init__(num_blocks, max_seqs, max_blocks_per_seq, block_size, device)
         self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv_heads, head_dim
@@ -53,6 +57,10 @@ class PagedKVPool(BlockPool):
         self.layer_stride = num_blocks * n_kv_heads * block_size * head_dim
         self.scale_layer_stride = 0
         self._allocate((n_layers, num_blocks, n_kv_heads, block_size, head_dim))
+        # attention weight that every cached token got so far, of the layer and kv head, in the pool's own layout
+        self.mass = None
+        if mass:
+            self.mass = torch.zeros((n_layers, num_blocks, n_kv_heads, block_size), dtype=torch.float32, device=self.device)
         self._workspace = _lib.DecodeWorkspace(self.device)
         with self._on_device():
             self._chunk_ws = _lib.load().snapmind_paged_gqa_chunk_workspace_bytes(head_dim)
@@ -100,6 +108,60 @@ class PagedKVPool(BlockPool):
             self.err.data_ptr(), self._stream(),
         )  # fmt: skip
         _lib.check(status, "PagedKVPool.append")
+
+    def append_rope(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
+                    sin: torch.Tensor, positions: torch.Tensor, cu_new: torch.Tensor | None = None,
+                    q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+        """Norm, rotate and store new tokens in one pass: returns the rotated queries.
+
+        ``q`` ``[total, Hq, D]``, ``k``/``v`` ``[total, H, D]``, one dtype (any float dtype, ``out`` has it too).
+        Queries and keys are normalised per head, ``x / sqrt(mean x^2 + eps) * norm`` (``q_norm`` / ``k_norm``:
+        ``[D]``, or ``[heads, D]`` with weights for each head; ``None``: as they are), and rotated by the rows of ``cos`` /
+        ``sin`` (f32 ``[n_pos, R]``, rotate-half over the first R dims) at ``positions`` (int64 ``[total]``): the tokens'
+        own, which their indexes in a cache that evicts are not.  All in f32, rounded once.  K and V go where
+        ``append_packed`` puts them (``cu_new`` ``[B + 1]``), or without ``cu_new`` token b is the newest of
+        sequence b.  ``out`` may be ``q``.  A position outside the tables leaves its token out (``check()`` raises)."""
+        total, n_q, d = q.shape
+        want = (total, self.n_kv_heads, self.head_dim)
+        if d != self.head_dim or k.shape != want or v.shape != want:
+            raise ValueError(f"append_rope: expected q [total, heads, {self.head_dim}] and k, v {list(want)}, got "
+                             f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+        if k.dtype != q.dtype or v.dtype != q.dtype:
+            raise TypeError("append_rope: q, k and v differ in dtype")
+        if not 0 <= layer < self.n_layers:
+            raise ValueError(f"layer {layer} of a pool of {self.n_layers}")
+        if cu_new is not None:
+            _lib.require_offsets("append_rope", cu_new, self.block_tables)
+        batch = total if cu_new is None else cu_new.shape[0] - 1
+        if batch > self.max_seqs:
+            raise ValueError(f"append_rope: {batch} sequences, the pool holds {self.max_seqs}")
+        if positions.dtype != torch.int64 or positions.shape != (total,):
+            raise ValueError(f"append_rope: positions must be int64 [{total}]")
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+            raise ValueError("append_rope: out must have q's shape and dtype, head dim contiguous")
+        _lib.require_same("append_rope", self.block_tables, q, k, v, cos, sin, positions, out)
+        rot, q_st, k_st = _lib.rope_args("append_rope", q, cos, sin, q_norm, k_norm, n_q, self.n_kv_heads, eps)
+        q, k, v = (x if x.stride(2) == 1 else x.contiguous() for x in (q, k, v))
+        if total > 1 and not positions.is_contiguous():
+            positions = positions.contiguous()
+        step = layer * self.layer_stride * self.k.element_size()
+        with self._on_device():
+            status = _lib.load().snapmind_norm_rope_append(
+                q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), n_q,
+                k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _lib.dtype_code(q.dtype),
+                _lib.ptr(q_norm), q_st, _lib.ptr(k_norm), k_st, eps, cos.data_ptr(), sin.data_ptr(), rot, cos.shape[0],
+                positions.data_ptr(), self.k.data_ptr() + step, self.v.data_ptr() + step,
+                self.scales.data_ptr() + layer * self.scale_layer_stride if self.quantised else None, self._pool_code,
+                self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq, self.seq_lens.data_ptr(),
+                _lib.ptr(cu_new), batch, total, self.n_kv_heads, d, self.block_size, self.num_blocks, self.err.data_ptr(),
+                _lib.raw_stream(self._index),
+            )  # fmt: skip
+        if status:
+            _lib.check(status, f"{type(self).__name__}.append_rope")
+        return out
 
     def append_packed(self, layer: int | None, k_new: torch.Tensor, v_new: torch.Tensor,
                       cu_new: torch.Tensor) -> None:
@@ -149,10 +211,104 @@ class PagedKVPool(BlockPool):
         if status:
             _lib.check(status, f"{type(self).__name__}.append")
 
+    # -------------------------------------------------------------- eviction
+    def _reserved(self, n_new, batch, counts=None):
+        if self.mass is None or n_new == 0:
+            return
+        with self._on_device():
+            status = _lib.load().snapmind_kv_clear_mass(
+                self.mass.data_ptr(), self.mass.stride(0), self.block_tables.data_ptr(), self.max_blocks_per_seq,
+                self.max_blocks_per_seq, self.seq_lens.data_ptr(), _lib.ptr(counts), n_new, batch, self.n_layers,
+                self.n_kv_heads, self.block_size, self.num_blocks, self.err.data_ptr(), _lib.raw_stream(self._index),
+            )  # fmt: skip
+        _lib.check(status, f"{type(self).__name__}.reserve")
+
+    def set_state(self, tables, lens, free_stack) -> None:
+        super().set_state(tables, lens, free_stack)
+        if self.mass is not None:
+            self.mass.zero_()
+
+    def evict(self, budget: int, recent: int = 0, sinks: int = 0, batch: int | None = None, seqs=None,
+              into=None) -> torch.Tensor:
+        """Thin sequences to ``budget`` tokens by ``mass``: each layer and kv head keeps the first ``sinks``
+        tokens, the newest ``recent``, and of the others those with the largest accumulated weight (equal ones: the lowest
+        index; a NaN counts as the largest).  What stays moves to the front in its order, with its mass; a sequence of
+        at most ``budget`` tokens stays as it is.  The lengths of a sequence are those of all its layers and heads, so all
+        are thinned alike.  Keys keep the rotation they were stored with.
+
+        The first ``batch`` sequences, or those named in ``seqs`` (distinct), lose their last blocks to the free
+        stack.  With ``into`` (as many distinct sequences, none of them in ``seqs``) they stay whole, and what the
+        targets held is replaced by the thinned copies.  Sequences must not share blocks.
+
+        Returns the kept indexes, int32 ``[n_layers, n, n_kv_heads, budget]``, ascending, -1 behind the last."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("evict: a captured step takes evict_device, and the host's lengths by account_evict")
+        if seqs is not None and batch is not None:
+            raise ValueError("evict: batch or seqs, not both")
+        if into is not None and seqs is None:
+            raise ValueError("evict: into goes with seqs")
+        ids = list(range(self.max_seqs if batch is None else batch)) if seqs is None else [int(x) for x in seqs]
+        to = ids if into is None else [int(x) for x in into]
+        every = ids if into is None else ids + to
+        if len(to) != len(ids) or len(set(every)) != len(every) or any(not 0 <= x < self.max_seqs for x in every):
+            raise ValueError("evict: sequences must be distinct and inside the pool, and each have a target of its own")
+        if into is not None:
+            take = sum(max(0, self._blocks(min(int(self._host_lens[a]), budget)) - self._blocks(int(self._host_lens[b])))
+                       for a, b in zip(ids, to))
+            if take > self._host_free:
+                raise RuntimeError(_lib.OUT_OF_BLOCKS_MSG)
+        kept = self._evict(budget, recent, sinks, len(ids), None if seqs is None else self._ids(ids),
+                           None if into is None else self._ids(to))
+        self._account_evict(budget, ids, to)
+        return kept
+
+    def evict_device(self, budget: int, recent: int = 0, sinks: int = 0, batch: int | None = None) -> torch.Tensor:
+        """The device part of ``evict`` in place for the first ``batch`` sequences: launches that a CUDA graph can replay.
+        The caller accounts every replay with ``account_evict``."""
+        return self._evict(budget, recent, sinks, self.max_seqs if batch is None else batch, None, None)
+
+    def account_evict(self, budget: int, batch: int | None = None) -> None:
+        """Bring the host mirrors to what ``evict(budget, batch=batch)`` makes of them."""
+        ids = range(self.max_seqs if batch is None else batch)
+        self._account_evict(budget, ids, ids)
+
+    def _blocks(self, n: int) -> int:
+        return (n + self.block_size - 1) // self.block_size
+
+    def _ids(self, ids) -> torch.Tensor:
+        return torch.tensor(ids, dtype=torch.int32, device=self.device)
+
+    def _account_evict(self, budget, ids, to):
+        ends = [min(int(self._host_lens[a]), budget) for a in ids]
+        for b, n in zip(to, ends):
+            self._host_free += self._blocks(int(self._host_lens[b])) - self._blocks(n)
+            self._host_lens[b] = n
+
+    def _evict(self, budget, recent, sinks, n, ids, to):
+        if self.mass is None:
+            raise ValueError("evict needs a pool with mass=True")
+        if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
+            raise ValueError(f"evict: the newest {recent} and the first {sinks} tokens do not fit a budget of {budget}")
+        if not 0 <= n <= self.max_seqs:
+            raise ValueError(f"evict: {n} sequences, the pool holds {self.max_seqs}")
+        kept = torch.empty((self.n_layers, n, self.n_kv_heads, budget), dtype=torch.int32, device=self.device)
+        with self._on_device():
+            status = _lib.load().snapmind_kv_evict_by_mass(
+                self.k.data_ptr(), self.v.data_ptr(), self.scales.data_ptr() if self.quantised else None, self._pool_code,
+                self.layer_stride, self.scale_layer_stride, self.mass.data_ptr(), self.mass.stride(0),
+                self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq, self.seq_lens.data_ptr(),
+                _lib.ptr(ids), _lib.ptr(to), n, budget, recent, sinks, kept.data_ptr(), self.free_stack.data_ptr(),
+                self.free_top.data_ptr(), self.n_layers, self.n_kv_heads, self.head_dim, self.block_size, self.num_blocks,
+                self.err.data_ptr(), _lib.raw_stream(self._index),
+            )  # fmt: skip
+        if status:
+            _lib.check(status, f"{type(self).__name__}.evict")
+        return kept
+
     # ----------------------------------------------------------------- reads
     def attend_chunk(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor, out: torch.Tensor | None = None,
                      scale: float | None = None, window: int = 0, sinks: int = 0,
-                     force_generic: bool = False) -> torch.Tensor:
+                     force_generic: bool = False, accumulate: bool = False) -> torch.Tensor:
         """Causal attention of a ragged chunk of new tokens against layer ``layer``, in
         one launch: pieces of prompts, drafted tokens and single tokens together.
 
@@ -164,14 +320,18 @@ class PagedKVPool(BlockPool):
 
         A position that a query does not see never counts, whatever K and V hold there (a NaN in V
         of one of the chunk's tokens reaches the queries from it on).  ``force_generic`` takes the
-        CUDA-core kernel, all in f32."""
+        CUDA-core kernel, all in f32.
+
+        ``accumulate`` adds to ``mass[layer]`` the weight that each cached token gets from the chunk's queries, summed over
+        them and over the query heads that share its kv head (in f32, the same bits every time).  Such calls of one
+        layer must not overlap on the GPU, and the sequences must not share blocks."""
         _lib.require_offsets("attend_chunk", cu_q, self.block_tables)
         if cu_q.shape[0] - 1 > self.max_seqs:
             raise ValueError(f"attend_chunk: {cu_q.shape[0] - 1} sequences, the pool holds {self.max_seqs}")
         return self._attend(layer, q, cu_q, out, scale, window, sinks,
-                            _lib.DECODE_FORCE_GENERIC if force_generic else 0)
+                            _lib.DECODE_FORCE_GENERIC if force_generic else 0, accumulate=accumulate)
 
-    def _attend_tokens(self, layer, q, out, scale, batch, window, sinks, force_generic, append):
+    def _attend_tokens(self, layer, q, out, scale, batch, window, sinks, force_generic, append, accumulate=False):
         """One query per sequence for the first ``batch`` sequences, their newest token stored first if given."""
         rows = out
         if batch is not None:
@@ -183,10 +343,10 @@ class PagedKVPool(BlockPool):
             if append[0].shape != want or append[1].shape != want:
                 raise ValueError(f"append rows must be {list(want)}, got {tuple(append[0].shape)} and {tuple(append[1].shape)}")
         got = self._attend(layer, q, None, rows, scale, window, sinks,
-                           _lib.DECODE_FORCE_GENERIC if force_generic else 0, append)
+                           _lib.DECODE_FORCE_GENERIC if force_generic else 0, append, accumulate=accumulate)
         return got if out is None else out
 
-    def _attend(self, layer, q, cu, out, scale, window, sinks, flags, append=None, row=None):
+    def _attend(self, layer, q, cu, out, scale, window, sinks, flags, append=None, row=None, accumulate=False):
         """``row``: ``(table, length)`` pointers of the one sequence, in place of the pool's own tables and lengths."""
         total, n_q, d = q.shape
         if q.dtype != self.dtype:
@@ -197,6 +357,8 @@ class PagedKVPool(BlockPool):
             raise ValueError(f"layer {layer} of a pool of {self.n_layers}")
         if cu is None and total > self.max_seqs:
             raise ValueError(f"decode: {total} sequences, the pool holds {self.max_seqs}")
+        if accumulate and self.mass is None:
+            raise ValueError("accumulate needs a pool with mass=True")
         q_st = q.stride()
         if q_st[2] != 1:
             q = q.contiguous()
@@ -208,8 +370,8 @@ class PagedKVPool(BlockPool):
             o_st = out.stride()
             if out.shape != q.shape or out.dtype != self.dtype or o_st[2] != 1:
                 raise ValueError("out must have q's shape and dtype, head dim contiguous")
-            if self.quantised and self.dtype == torch.float16 and _share(q, out):
-                q = q.clone()  # such a call may be done over, with the queries it began with
+            if (accumulate or (self.quantised and self.dtype == torch.float16)) and _share(q, out):
+                q = q.clone()  # such a call may be done over, or takes the scores anew, with the queries it began with
                 q_st = q.stride()
         _lib.require_same("attend", self.block_tables, q, out)
         if append is not None:
@@ -219,19 +381,22 @@ class PagedKVPool(BlockPool):
         lib = _lib.load()
         # a workspace of its own for every call: calls on several streams, or in several
         # captured graphs, never share one
-        need = self._chunk_ws
+        need, mass = self._chunk_ws, None
+        if accumulate:
+            need = lib.snapmind_paged_gqa_chunk_mass_workspace_bytes(d, total, n_q)
+            mass = self.mass.data_ptr() + 4 * layer * self.num_blocks * self.n_kv_heads * self.block_size
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         step = layer * self.layer_stride * self.k.element_size()
         scales = self.scales.data_ptr() + layer * self.scale_layer_stride if self.quantised else None
         with self._on_device():
-            status = lib.snapmind_paged_gqa_chunk(
+            status = lib.snapmind_paged_gqa_chunk_mass(
                 q.data_ptr(), q_st[0], q_st[1], self._dcode, self.k.data_ptr() + step,
                 self.v.data_ptr() + step, scales, self._pool_code,
                 self.block_tables.data_ptr() if row is None else row[0],
                 self.max_blocks_per_seq, self.max_blocks_per_seq, self.seq_lens.data_ptr() if row is None else row[1],
                 None if cu is None else cu.data_ptr(), out.data_ptr(), o_st[0], o_st[1],
                 d ** -0.5 if scale is None else scale, total if cu is None else cu.shape[0] - 1, total, n_q,
-                self.n_kv_heads, d, self.block_size, self.num_blocks, window, sinks, flags, ws.data_ptr(), need,
+                self.n_kv_heads, d, self.block_size, self.num_blocks, window, sinks, flags, mass, ws.data_ptr(), need,
                 self.err.data_ptr(), _lib.raw_stream(self._index),
             )  # fmt: skip
         if status:
@@ -335,7 +500,7 @@ class PagedKVPool(BlockPool):
     def decode(self, layer: int, q: torch.Tensor, out: torch.Tensor | None = None, scale: float | None = None,
                batch: int | None = None, split_tokens: int = 0, force_generic: bool = False,
                max_seq_len: int | None = None, peers=None, append=None, window: int = 0,
-               sinks: int = 0) -> torch.Tensor | None:
+               sinks: int = 0, accumulate: bool = False) -> torch.Tensor | None:
         """Paged GQA decode attention of ``q`` ``[B, Hq, D]`` against layer ``layer``.
 
         With ``window`` > 0 a sequence attends to its last ``window`` tokens and its
@@ -347,11 +512,11 @@ class PagedKVPool(BlockPool):
         and returns None.  ``append=(k_new, v_new)`` (``[B, H, D]``, the pool's
         dtype) stores this step's token of every sequence (the last slot the
         latest ``reserve(1)`` gave it) in the same launch, in place of an
-        ``append`` call before the decode."""
-        if window or sinks:
+        ``append`` call before the decode.  ``accumulate`` as in ``attend_chunk``."""
+        if window or sinks or accumulate:
             if peers is not None:
-                raise ValueError("decode with a window has no peer form")
-            return self._attend_tokens(layer, q, out, scale, batch, window, sinks, force_generic, append)
+                raise ValueError("decode with a window, or that accumulates, has no peer form")
+            return self._attend_tokens(layer, q, out, scale, batch, window, sinks, force_generic, append, accumulate)
         batch = q.shape[0] if batch is None else batch
         n_q = q.shape[1]
         if peers is not None and append is not None:

@@ -2,7 +2,7 @@
 
 ``QuantizedKVPool`` is :class:`snapmind_b200.paged_pool.PagedKVPool` with half the bytes
 per token (of a 16-bit pool): the same block tables, reserve and release, ``append``,
-``append_packed``, ``gather``, ``decode`` and ``attend_chunk``.
+``append_packed``, ``append_rope``, ``gather``, ``decode``, ``attend_chunk`` and ``evict``.
 
 * ``k``, ``v``: ``torch.float8_e4m3fn`` ``[layer][block][head][slot][dim]``;
 * ``scales``: uint8 ``[layer][block][head][2][slot]`` (K, V): exponent + 127 of a row.
@@ -87,12 +87,12 @@ class QuantizedKVPool(PagedKVPool):
     def decode(self, layer: int, q: torch.Tensor, out: torch.Tensor | None = None, scale: float | None = None,
                batch: int | None = None, split_tokens: int = 0, force_generic: bool = False,
                max_seq_len: int | None = None, peers=None, append=None, window: int = 0,
-               sinks: int = 0) -> torch.Tensor:
+               sinks: int = 0, accumulate: bool = False) -> torch.Tensor:
         """``PagedKVPool.decode`` over the 8-bit rows (``split_tokens`` and ``max_seq_len``
         have no use: the kernel plans from the device lengths)."""
         if peers is not None:
             raise ValueError("QuantizedKVPool: decode has no peer form")
-        return self._attend_tokens(layer, q, out, scale, batch, window, sinks, force_generic, append)
+        return self._attend_tokens(layer, q, out, scale, batch, window, sinks, force_generic, append, accumulate)
 
     def decode_layers(self, *args, **kwargs):
         raise NotImplementedError("QuantizedKVPool: decode one layer at a time")
