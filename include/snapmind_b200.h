@@ -611,10 +611,12 @@ SNAPMIND_API int snapmind_paged_gqa_chunk(const void *q, int64_t q_stride_tok, i
  * bits.  A query that sees nothing adds nothing; one whose softmax is NaN makes the tokens that it sees NaN.
  * q is read after out was written, so out must not be q.  The sequences must not share blocks, and calls that add
  * to the same layer must not overlap on the GPU.  The workspace holds
- * snapmind_paged_gqa_chunk_mass_workspace_bytes(...) bytes, on the terms of snapmind_paged_gqa_chunk's.  The reference returns its weights (snapmind/layers/attention/gqa.py:79-85) but
+ * snapmind_paged_gqa_chunk_mass_workspace_bytes(...) bytes, on the terms of snapmind_paged_gqa_chunk's; `decodes` is
+ * 1 for a call without cu_q (whose scores are kept).  The reference returns its weights (snapmind/layers/attention/gqa.py:79-85) but
  * keeps no sums of them.
  */
-SNAPMIND_API int64_t snapmind_paged_gqa_chunk_mass_workspace_bytes(int32_t head_dim, int32_t total_q, int32_t n_q_heads);
+SNAPMIND_API int64_t snapmind_paged_gqa_chunk_mass_workspace_bytes(int32_t head_dim, int32_t total_q, int32_t n_q_heads,
+                             int32_t n_kv_heads, int32_t block_size, int32_t num_blocks, int32_t decodes);
 SNAPMIND_API int snapmind_paged_gqa_chunk_mass(const void *q, int64_t q_stride_tok, int64_t q_stride_head, int dtype,
                              const void *k_pool, const void *v_pool, const void *scales, int pool_dtype,
                              const int32_t *block_tables, int64_t table_stride_seq, int32_t table_width,

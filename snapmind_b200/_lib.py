@@ -151,7 +151,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _i64, _i64, _int, _p, _p, _p, _int, _p, _i64, _i32, _p, _p, _p, _i64, _i64, _f32, _i32, _i32, _i32,
          _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p],
     ),
-    "snapmind_paged_gqa_chunk_mass_workspace_bytes": (_i64, [_i32, _i32, _i32]),
+    "snapmind_paged_gqa_chunk_mass_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "snapmind_paged_gqa_chunk_mass": (
         _int,
         [_p, _i64, _i64, _int, _p, _p, _p, _int, _p, _i64, _i32, _p, _p, _p, _i64, _i64, _f32, _i32, _i32,

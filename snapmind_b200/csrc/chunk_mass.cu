@@ -204,6 +204,80 @@ int launch_generic(MassParams& mp, cudaStream_t st) {
   return go(mass_generic_kernel<T, KV, 4>, sizeof(MassSmem<4>), MassSmem<4>::kCtas, done[2]);
 }
 
+// Behind a decode that left its scores (decode_sinks.cu): the same CTAs on the same shares of the key line, a thread
+// a key.  HBM bound: 4 bytes a query head and 8 of mass for each key and kv head, against the 512 of a 16-bit row of
+// K and V that the decode read (scores taken from K anew would read half of those again).
+constexpr int kScoreThreads = 512, kScoreDeep = 2;
+template <int G>
+__global__ void __launch_bounds__(kScoreThreads, 2) mass_scores_kernel(const __grid_constant__ ChunkParams p, float* mass) {
+  extern __shared__ int32_t tiles[];
+  __shared__ PlanShared plan;
+  next_grid_may_launch();
+  // the lengths are older than the call's first kernel, which has begun: only what it left is waited for
+  plan_block(p, plan, tiles);
+  prior_grid_wait();
+  PieceWalk w;
+  for (bool on = w.start(plan); on; on = w.next(p)) {
+    const Piece& c = w.c;
+    const KeyRange kr = key_range(p, c.len, c.n, c.i0, c.i0 + 1);
+    const int group = G > 0 ? G : p.group;
+    const float2* stats = p.stats + (int64_t)c.q_first * p.n_q_heads + c.kvh * group;
+    float2 st[G > 0 ? G : 1];
+    if constexpr (G > 0) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) st[g] = stats[g];
+    }
+    const int32_t* table = p.tables + (int64_t)c.b * p.table_stride;
+    const int v1 = min(c.tile1 * p.key_tile, kr.v_len), q = kr.pos0;
+    for (int v0 = c.tile0 * p.key_tile + threadIdx.x; v0 < v1; v0 += kScoreThreads * kScoreDeep) {
+      int64_t row[kScoreDeep];
+      float m[kScoreDeep], s[kScoreDeep][G > 0 ? G : 1];
+#pragma unroll
+      for (int u = 0; u < kScoreDeep; ++u) {
+        const int v = v0 + u * kScoreThreads;
+        row[u] = -1;
+        if (v >= v1) continue;
+        const int pos = kr.position(v), j = p.by_block.div(pos);
+        const int32_t phys = table[j];
+        if (phys < 0 || phys >= p.num_blocks || (p.window > 0 && pos <= q - p.window && pos >= p.sinks)) continue;
+        row[u] = ((int64_t)phys * p.n_kv_heads + c.kvh) * p.block_size + (pos - j * p.block_size);
+        m[u] = mass[row[u]];
+        const float* from = p.scores + row[u] * group;
+        if constexpr (G == 2) *reinterpret_cast<float2*>(s[u]) = *reinterpret_cast<const float2*>(from);
+        if constexpr (G == 1) s[u][0] = *from;
+        if constexpr (G >= 4)
+#pragma unroll
+          for (int g = 0; g < G; g += 4) *reinterpret_cast<float4*>(&s[u][g]) = *reinterpret_cast<const float4*>(from + g);
+      }
+#pragma unroll
+      for (int u = 0; u < kScoreDeep; ++u) {
+        if (row[u] < 0) continue;
+        float sum = 0.f;
+        if constexpr (G > 0) {
+#pragma unroll
+          for (int g = 0; g < G; ++g) sum = fmaf(ex2(s[u][g] - st[g].x), st[g].y, sum);
+        } else {
+          for (int g = 0; g < group; ++g) sum = fmaf(ex2(p.scores[row[u] * group + g] - stats[g].x), stats[g].y, sum);
+        }
+        mass[row[u]] = m[u] + sum;
+      }
+    }
+  }
+}
+
+int launch_scores(const ChunkParams& p, float* mass, cudaStream_t st) {
+  const auto go = [&](auto kernel) {
+    return cuda_status(launch_dependent(kernel, dim3(p.n_ctas), kScoreThreads, (size_t)p.batch * 4, st, p, mass), "paged_chunk mass launch");
+  };
+  switch (p.group) {
+    case 1: return go(mass_scores_kernel<1>);
+    case 2: return go(mass_scores_kernel<2>);
+    case 4: return go(mass_scores_kernel<4>);
+    case 8: return go(mass_scores_kernel<8>);
+    default: return go(mass_scores_kernel<0>);
+  }
+}
+
 // Workspace: the attention's, then the rows' statistics, the cut units' pieces.
 constexpr int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 int64_t max_ctas() { return 4 * (int64_t)num_sms(); }
@@ -218,7 +292,8 @@ int launch_mass_merge(const MassParams& mp, cudaStream_t st) {
 }
 
 // After the attention kernels on the stream, which left p.stats.
-int launch_mass(const ChunkParams& p, int dtype, int pool_dtype, float* mass, void* workspace, cudaStream_t st) {
+int launch_mass(const ChunkParams& p, int dtype, int pool_dtype, int32_t flags, float* mass, void* workspace, cudaStream_t st) {
+  if (p.scores != nullptr) return launch_scores(p, mass, st);
   MassParams mp = {};
   mp.c = p;
   mp.mass = mass;

@@ -221,7 +221,7 @@ inline int mass_geometry(MassParams& mp, int rows, int key_tile, int n_ctas) {
 // chunk_mass.cu: the merge of cut units, behind a kernel of this plan; the whole pass behind the attention kernels
 // of a call, in a workspace of mass_workspace_bytes().
 int launch_mass_merge(const MassParams& mp, cudaStream_t st);
-int launch_mass(const ChunkParams& p, int dtype, int pool_dtype, float* mass, void* workspace, cudaStream_t st);
+int launch_mass(const ChunkParams& p, int dtype, int pool_dtype, int32_t flags, float* mass, void* workspace, cudaStream_t st);
 int64_t mass_workspace_bytes();
 
 // chunk_mass_umma.cu: whether the shapes fit, and the launch.

@@ -51,6 +51,7 @@ struct ChunkParams {
   int32_t* odd;     // workspace: [n_odd] whether a CTA met rows that its kernel's types do not hold, or NULL
   int32_t n_odd;
   int32_t means;    // part_o holds a piece's weighted means of V (else its weighted sums)
+  float* scores;    // [pool row][group] scores (log2 units) that a decode leaves for chunk_mass.cu, or NULL
   float2* stats;    // [total_q][n_q_heads] reference (log2 units) and 1 / sum of every row's softmax, or NULL
   int32_t* err;
 };
@@ -462,6 +463,8 @@ bool chunk_umma_supported(const ChunkParams& p, int dtype, int pool_dtype);
 int launch_chunk_umma(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st);
 bool decode_sinks_supported(const ChunkParams& p, int dtype, int pool_dtype);
 int launch_decode_sinks(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st);
+// Whether a call of such shapes may run on the decode kernel, which then leaves its scores.
+inline bool decode_keeps_scores(int head_dim, int group) { return head_dim == 128 && group <= 8; }
 
 // Sets a kernel's shared-memory attributes once per device (`done` is the instantiation's own).
 constexpr int kMaxDevices = 64;

@@ -60,6 +60,7 @@ struct Ctrl {
   float mr[kConsumers][kHeads];                          // R (16-bit caches: M)
   uint64_t full[N], empty[N];
   uint32_t have[N];  // parts of a stage's tile that were there to be copied
+  int32_t rows[N][kTile / 16];  // their pool rows (kScores)
   int32_t abort;
   PlanShared plan;
 };
@@ -111,7 +112,8 @@ __device__ __forceinline__ bool consumers_any(bool v) {
   return r != 0;
 }
 
-template <typename T, bool kQuant>
+// kScores: the scores of the tokens go to p.scores too, for the pass that adds their weights up.
+template <typename T, bool kQuant, bool kScores>
 __global__ void __launch_bounds__(kThreads, 2)
     decode_sinks_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, ChunkParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -162,6 +164,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint32_t bar = smem_u32(&S.full[st]);
         const uint32_t row_bytes = kQuant ? 128 : 2 * 128;
         if (kv == 0 && leader) S.have[st] = have;
+        if constexpr (kScores) {
+          const int y = at.row(j, lane & (at.parts - 1));
+          if (kv == 0 && lane < at.parts) S.rows[st][lane] = y;
+          __syncwarp();
+        }
         mbar_arrive_expect_tx_p(leader, bar, __popc(have) * (uint32_t)box * row_bytes);
         const uint32_t dst = smem_u32(ring + st * St::kBytes + (kv == 0 ? St::kK : St::kV));
         if constexpr (kQuant) {
@@ -318,6 +325,21 @@ __global__ void __launch_bounds__(kThreads, 2)
               uint32_t a[4];
               ldsm_x4(kb + (k >> 2) * St::kHalf + k_off[k & 3], a);
               mma16816<kMmaBf16>(sc, a, qf[k][0], qf[k][1]);
+            }
+          }
+          if constexpr (kScores) {
+            // a key's scores side by side: 16 bytes for four heads (rows past the last token, unseen ones: never read)
+            const int64_t row = S.rows[st][part] + 16 * warp - part * p.block_size;
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              float* to = p.scores + (row + g + 4 * i) * heads + 2 * tig;
+              const float a = sc[i] * q0, b = sc[i + 1] * q1;
+              if (heads % 2 == 0) {
+                if (2 * tig < heads) *reinterpret_cast<float2*>(to) = make_float2(a, b);
+              } else {
+                if (2 * tig < heads) to[0] = a;
+                if (2 * tig + 1 < heads) to[1] = b;
+              }
             }
           }
           // Scores less their references: xs for the sum, ys for the weights (16-bit caches: xs).  When a
@@ -519,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   next_grid_may_launch();
 }
 
-template <typename T, bool kQuant>
+template <typename T, bool kQuant, bool kScores>
 int launch(const ChunkParams& p, cudaStream_t st) {
   CUtensorMap k_map, v_map;
   const uint64_t rows = (uint64_t)p.num_blocks * p.n_kv_heads * p.block_size;
@@ -532,7 +554,7 @@ int launch(const ChunkParams& p, cudaStream_t st) {
     set_last_error("paged_chunk: tensor map encoding failed");
     return SNAPMIND_ERR_CUDA;
   }
-  auto kernel = decode_sinks_kernel<T, kQuant>;
+  auto kernel = decode_sinks_kernel<T, kQuant, kScores>;
   static bool done[kMaxDevices] = {};
   const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem_bytes<kQuant>(), done);
   if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
@@ -564,9 +586,12 @@ int launch_decode_sinks(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t 
   p.tokens = 1;
   p.means = pool_dtype == SNAPMIND_DTYPE_E4M3;
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
-  if (dtype == SNAPMIND_DTYPE_BF16)
-    return quant ? launch<__nv_bfloat16, true>(p, st) : launch<__nv_bfloat16, false>(p, st);
-  return quant ? launch<__half, true>(p, st) : launch<__half, false>(p, st);
+  const auto go = [&](auto t) -> int {
+    using T = decltype(t);
+    if (p.scores != nullptr) return quant ? launch<T, true, true>(p, st) : launch<T, false, true>(p, st);
+    return quant ? launch<T, true, false>(p, st) : launch<T, false, false>(p, st);
+  };
+  return dtype == SNAPMIND_DTYPE_BF16 ? go(__nv_bfloat16()) : go(__half());
 }
 
 }  // namespace snapmind

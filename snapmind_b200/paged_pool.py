@@ -383,7 +383,8 @@ class PagedKVPool(BlockPool):
         # captured graphs, never share one
         need, mass = self._chunk_ws, None
         if accumulate:
-            need = lib.snapmind_paged_gqa_chunk_mass_workspace_bytes(d, total, n_q)
+            need = lib.snapmind_paged_gqa_chunk_mass_workspace_bytes(d, total, n_q, self.n_kv_heads, self.block_size,
+                                                                     self.num_blocks, cu is None)
             mass = self.mass.data_ptr() + 4 * layer * self.num_blocks * self.n_kv_heads * self.block_size
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         step = layer * self.layer_stride * self.k.element_size()
