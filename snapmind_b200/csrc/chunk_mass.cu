@@ -300,6 +300,10 @@ int launch_mass(const ChunkParams& p, int dtype, int pool_dtype, int32_t flags, 
   mp.info = static_cast<int32_t*>(workspace);
   mp.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + info_bytes());
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
+  if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && chunk_umma_supported(p, dtype, pool_dtype)) {
+    const int rc = launch_mass_umma(mp, dtype, pool_dtype, st);
+    if (rc != SNAPMIND_ERR_UNSUPPORTED) return rc;
+  }
   switch (dtype) {
     case SNAPMIND_DTYPE_F32: return quant ? launch_generic<float, uint8_t>(mp, st) : launch_generic<float, float>(mp, st);
     case SNAPMIND_DTYPE_BF16:

@@ -224,8 +224,7 @@ int launch_mass_merge(const MassParams& mp, cudaStream_t st);
 int launch_mass(const ChunkParams& p, int dtype, int pool_dtype, int32_t flags, float* mass, void* workspace, cudaStream_t st);
 int64_t mass_workspace_bytes();
 
-// chunk_mass_umma.cu: whether the shapes fit, and the launch.
-bool mass_umma_supported(const ChunkParams& p, int dtype, int pool_dtype);
+// chunk_mass_umma.cu: for the shapes of chunk_umma_supported.
 int launch_mass_umma(MassParams& mp, int dtype, int pool_dtype, cudaStream_t st);
 
 }  // namespace snapmind
