@@ -647,14 +647,14 @@ SNAPMIND_API int snapmind_kv_clear_mass(float *mass, int64_t mass_layer_stride, 
  *     by the kept tokens, their blocks grow or shrink (SNAPMIND_DEVERR_OUT_OF_BLOCKS and nothing happens
  *     when the free stack has not enough).
  * kept [n_layers][n_seqs][n_heads][budget] receives the kept indexes, ascending, -1 behind the last.
- * pool_layer_stride and mass_layer_stride are in elements, scale_layer_stride in bytes.  Sequences must not share
- * blocks.  The reference evicts the oldest tokens only (snapmind/kv_cache/paged.py evict).
+ * pool_layer_stride and mass_layer_stride are in elements, scale_layer_stride in bytes.  max_len: the longest of the
+ * sequences, or 0 (it chooses the launch; longer ones are still right).  Sequences must not share blocks.  The reference evicts the oldest tokens only (snapmind/kv_cache/paged.py evict).
  */
 SNAPMIND_API int snapmind_kv_evict_by_mass(void *k_pool, void *v_pool, void *scales, int pool_dtype,
                              int64_t pool_layer_stride, int64_t scale_layer_stride, float *mass,
                              int64_t mass_layer_stride, int32_t *block_tables, int64_t table_stride_seq,
                              int32_t table_width, int32_t *seq_lens, const int32_t *seqs, const int32_t *into,
-                             int32_t n_seqs, int32_t budget, int32_t recent, int32_t sinks, int32_t *kept,
+                             int32_t n_seqs, int32_t budget, int32_t recent, int32_t sinks, int32_t max_len, int32_t *kept,
                              int32_t *free_stack, int32_t *free_top, int32_t n_layers, int32_t n_heads,
                              int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t *err_word,
                              void *stream);

@@ -163,7 +163,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "snapmind_kv_evict_by_mass": (
         _int,
-        [_p, _p, _p, _int, _i64, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _p,
+        [_p, _p, _p, _int, _i64, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _p, _p,
          _p, _i32, _i32, _i32, _i32, _i32, _p, _p],
     ),
     "snapmind_norm_rope_qk": (

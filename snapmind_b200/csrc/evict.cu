@@ -9,6 +9,8 @@
 // In place is safe because the i-th kept token stands at index p_i >= i: rows move towards the front in
 // ascending order, a batch is read whole before it is written, and what a batch overwrites lies in front of all
 // that is still to be read.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace snapmind {
@@ -22,7 +24,7 @@ struct EvictParams {
   const int32_t* src;  // [n] sequence ids, NULL: 0 .. n - 1
   const int32_t* dst;  // [n], NULL: in place
   int32_t n, n_layers, n_heads, block_size, num_blocks, budget, recent, sinks;
-  FastDiv by_block, by_heads, by_units;  // by_units: n * n_heads
+  FastDiv by_block;
   float* mass;
   int64_t mass_layer;  // elements
   int32_t* kept;       // [n_layers][n][n_heads][budget]
@@ -31,7 +33,7 @@ struct EvictParams {
   uint8_t* scales;
   int64_t scale_layer;  // bytes
   int32_t row_bytes;
-  int32_t slices, slice_bytes;  // a row's bytes are moved by `slices` CTAs
+  int32_t slices, slice_bytes;  // a row's bytes are moved by `slices` blocks
   int32_t* free_stack;
   int32_t* free_top;
   int32_t* err;
@@ -54,48 +56,34 @@ __device__ __forceinline__ int64_t row_of(const EvictParams& p, const int32_t* t
   return ((int64_t)phys * p.n_heads + head) * p.block_size + (j - k * p.block_size);
 }
 
-// Order of weights as unsigned integers: -infinity lowest, infinity below NaN.
+// Order of weights as unsigned integers: -infinity lowest, infinity below NaN, -0 with 0.
 __device__ __forceinline__ uint32_t order_of(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.f);
   return (u & 0x7FFFFFFFu) > 0x7F800000u ? 0xFFFFFFFFu : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelectThreads = 512, kRadix = 11, kBins = 1 << kRadix;
-constexpr int kHeld = 8192;  // indexes whose order stays in shared memory
+// Selection: a block per (layer, sequence, head).  The weights lie in shared memory (a chunk of them when there
+// are more), warp w holding run w of the chunk's indexes; the order of the last that stays is found 11 bits at a time
+// from histograms, and the kept indexes are counted per warp by ballots and written out in a second sweep.  What
+// bounds it is latency (a read of the table, one of the weights, a handful of barriers), so blocks are small
+// where sequences are short, several to an SM.
+constexpr int kRadix = 11, kBins = 1 << kRadix;
 
+template <int THREADS>
 struct SelectSmem {
-  uint32_t key[kHeld];
   int32_t bins[kBins];
-  int32_t warp_sum[kSelectThreads / 32];
-  int32_t carry;
+  int32_t above[THREADS / 32], equal[THREADS / 32];
   uint32_t prefix;  // of the lowest kept order
   int32_t need;     // how many with exactly that order stay
+  int32_t total;
 };
 
-__device__ __forceinline__ int block_scan(SelectSmem& S, int x, int* total) {  // exclusive
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = x;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
-  __syncthreads();
-  if (lane == 31) S.warp_sum[warp] = incl;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kSelectThreads / 32; ++w) {
-    if (w < warp) before += S.warp_sum[w];
-    all += S.warp_sum[w];
-  }
-  *total = all;
-  return before + incl - x;
-}
-
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ SelectSmem S;
-  const int tid = threadIdx.x;
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ EvictParams p, int chunk) {
+  extern __shared__ __align__(16) float held[];  // [chunk], a multiple of 4 * THREADS
+  __shared__ SelectSmem<THREADS> S;
+  constexpr int kWarps = THREADS / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int layer = blockIdx.x / (p.n * p.n_heads), u = blockIdx.x - layer * (p.n * p.n_heads);
   const int i = u / p.n_heads, head = u - i * p.n_heads;
   const int from = src_id(p, i), to = dst_id(p, i);
@@ -106,9 +94,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   const int32_t* new_table = p.tables + (int64_t)to * p.table_stride;
   const bool copies = p.dst != nullptr;
   if (copies && p.seq_lens[to] != keep) return;  // it was not given its blocks
-  for (int x = keep + tid; x < p.budget; x += kSelectThreads) kept[x] = -1;
+  for (int x = keep + tid; x < p.budget; x += THREADS) kept[x] = -1;
   if (len <= p.budget) {
-    for (int x = tid; x < keep; x += kSelectThreads) {
+    for (int x = tid; x < keep; x += THREADS) {
       kept[x] = x;
       if (copies) {
         const int64_t a = row_of(p, table, head, x), b = row_of(p, new_table, head, x);
@@ -119,38 +107,75 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   }
   // what stays in any case takes no part: [0, lo) and [hi, len)
   const int lo = min(p.sinks, keep), hi = len - min(p.recent, keep - lo);
-  const auto weight = [&](int x) {
-    const int64_t row = row_of(p, table, head, x);
-    return row < 0 ? 0u : order_of(mass[row]);
+  // weights [c0, c0 + chunk) into shared memory; an index without a block: -infinity
+  const auto load = [&](int c0) {
+    const int n = min(chunk, len - c0);
+    if ((p.block_size & 3) == 0) {
+      constexpr int kDeep = 4;
+      for (int x0 = 4 * tid; x0 < n; x0 += 4 * THREADS * kDeep) {
+        float4 v[kDeep];
+#pragma unroll
+        for (int y = 0; y < kDeep; ++y) {
+          const int x = x0 + y * 4 * THREADS;
+          v[y] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          if (x < n) {
+            const int64_t row = row_of(p, table, head, c0 + x);  // four slots of a block
+            if (row >= 0) v[y] = *reinterpret_cast<const float4*>(mass + row);
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < kDeep; ++y)
+          if (x0 + y * 4 * THREADS < n) *reinterpret_cast<float4*>(held + x0 + y * 4 * THREADS) = v[y];
+      }
+    } else {
+      for (int x = tid; x < n; x += THREADS) {
+        const int64_t row = row_of(p, table, head, c0 + x);
+        held[x] = row < 0 ? -INFINITY : mass[row];
+      }
+    }
   };
-  for (int x = lo + tid; x < hi; x += kSelectThreads)
-    if (x - lo < kHeld) S.key[x - lo] = weight(x);
-  const auto key = [&](int x) { return x - lo < kHeld ? S.key[x - lo] : weight(x); };
+  const bool one = len <= chunk;
+  if (one) load(0);
   int need = keep - lo - (len - hi);  // of [lo, hi)
+  const bool none = need <= 0;
   uint32_t prefix = 0;
   int shift = 32;
   // the order of the need-th largest, 11, 11 and 10 bits at a time
-  for (int pass = 0; pass < 3 && need > 0; ++pass) {
+  for (int pass = 0; pass < 3 && !none; ++pass) {
     const int bits = pass < 2 ? kRadix : 32 - 2 * kRadix;
-    const uint32_t above = shift == 32 ? 0u : prefix >> shift;
+    for (int x = tid; x < kBins; x += THREADS) S.bins[x] = 0;
     __syncthreads();
-    for (int x = tid; x < kBins; x += kSelectThreads) S.bins[x] = 0;
-    __syncthreads();
-    for (int x = lo + tid; x < hi; x += kSelectThreads) {
-      const uint32_t k = key(x);
-      if (shift == 32 || k >> shift == above) atomicAdd(&S.bins[(k >> (shift - bits)) & ((1u << bits) - 1)], 1);
+    for (int c0 = 0; c0 < len; c0 += chunk) {
+      if (!one) {
+        __syncthreads();
+        load(c0);
+        __syncthreads();
+      }
+      const int x1 = min(hi, c0 + chunk);
+      for (int x = max(lo, c0) + tid; x < x1; x += THREADS) {
+        const uint32_t k = order_of(held[x - c0]);
+        if (shift == 32 || k >> shift == prefix >> shift) atomicAdd(&S.bins[(k >> (shift - bits)) & ((1u << bits) - 1)], 1);
+      }
     }
     __syncthreads();
     // from the highest bin down: the bin where the count reaches `need`
-    constexpr int kPer = kBins / kSelectThreads;
+    constexpr int kPer = kBins / THREADS;
     int mine[kPer], sum = 0;
 #pragma unroll
     for (int y = 0; y < kPer; ++y) {
-      const int bin = kBins - 1 - (tid * kPer + y);
-      mine[y] = S.bins[bin];
+      mine[y] = S.bins[kBins - 1 - (tid * kPer + y)];
       sum += mine[y];
     }
-    int total, before = block_scan(S, sum, &total);
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) S.above[warp] = incl;
+    __syncthreads();
+    int before = incl - sum;
+    for (int w = 0; w < warp; ++w) before += S.above[w];
 #pragma unroll
     for (int y = 0; y < kPer; ++y) {
       if (before < need && before + mine[y] >= need) {
@@ -164,40 +189,77 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
     need = S.need;
     shift -= bits;
   }
-  const bool none = keep - lo - (len - hi) <= 0;
-  // in ascending order: what is above the border stays, of those on it the first `need`
+  // in ascending order: what is above the border stays, of those on it the first `need`.  A chunk is read whole
+  // before its kept weights are written, which is never past its own end.
   int at = 0, equal = 0;
-  for (int base = 0; base < len; base += kSelectThreads) {
-    const int x = base + tid;
-    const bool sure = x < lo || (x >= hi && x < len);
-    const bool may = x >= lo && x < hi && !none;
-    const uint32_t k = may ? key(x) : 0u;
-    const bool on = may && k == prefix;
-    int here;
-    const int rank = block_scan(S, on, &here);
-    const bool stays = sure || (may && k > prefix) || (on && equal + rank < need);
-    equal += here;
-    float m = 0.f;
-    if (stays) {
-      const int64_t a = row_of(p, table, head, x);
-      if (a >= 0) m = mass[a];
+  for (int c0 = 0; c0 < len; c0 += chunk) {
+    const int n = min(chunk, len - c0);
+    if (!one) {
+      __syncthreads();
+      load(c0);
     }
-    int kept_here;
-    const int place = at + block_scan(S, stays, &kept_here);  // its barriers part the reads from the writes
-    if (stays) {
-      kept[place] = x;
-      const int64_t b = row_of(p, new_table, head, place);
-      if (b >= 0) mass[b] = m;
+    __syncthreads();
+    const int run = (n + 32 * kWarps - 1) / (32 * kWarps) * 32, x0 = min(n, warp * run), x1 = min(n, x0 + run);
+    // bits of the lane's index: 1 it stays, 2 it is on the border
+    const auto sort = [&](int x) {
+      if (x >= x1) return 0;
+      const int j = c0 + x;
+      if (j < lo || j >= hi) return 1;
+      if (none) return 0;
+      const uint32_t k = order_of(held[x]);
+      return k > prefix ? 1 : k == prefix ? 2 : 0;
+    };
+    int above = 0, on = 0;
+    for (int x = x0; x < x1; x += 32) {
+      const int k = sort(x + lane);
+      above += __popc(__ballot_sync(0xffffffffu, k == 1));
+      on += __popc(__ballot_sync(0xffffffffu, k == 2));
     }
-    at += kept_here;
+    if (lane == 0) {
+      S.above[warp] = above;
+      S.equal[warp] = on;
+    }
+    __syncthreads();
+    int mine_at = at, mine_equal = equal, all_at = at, all_equal = equal;
+    for (int w = 0; w < kWarps; ++w) {
+      const int e = S.equal[w], k = S.above[w] + min(e, max(0, need - all_equal));
+      if (w < warp) {
+        mine_at += k;
+        mine_equal += e;
+      }
+      all_at += k;
+      all_equal += e;
+    }
+    for (int x = x0; x < x1; x += 32) {
+      const int k = sort(x + lane);
+      const uint32_t border = __ballot_sync(0xffffffffu, k == 2), below = (1u << lane) - 1u;
+      const bool stays = k == 1 || (k == 2 && mine_equal + __popc(border & below) < need);
+      const uint32_t those = __ballot_sync(0xffffffffu, stays);
+      if (stays) {
+        const int place = mine_at + __popc(those & below);
+        kept[place] = c0 + x + lane;
+        const int64_t b = row_of(p, new_table, head, place);
+        if (b >= 0) mass[b] = held[x + lane];
+      }
+      mine_at += __popc(those);
+      mine_equal += __popc(border);
+    }
+    at = all_at;
+    equal = all_equal;
   }
 }
 
-// Rows of the kept tokens of one (layer, sequence, head), slice_bytes of each K or V row.
-template <int W>
-__global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ EvictParams p) {
+// Rows of the kept tokens of one (layer, sequence, head): a block moves slice_bytes of each K or V row, TEAM lanes of
+// W bytes a row, 32 rows a warp and step.  A lane works out where one row comes from and goes to (and moves its
+// scale), and the teams fetch that by shuffles; the next step's indexes are read while this one's rows are on
+// their way.  Where there are few units, a row's columns go to several blocks, which never meet.
+constexpr int kMoveThreads = 256;
+template <int W, int TEAM>
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
   using V = typename VecT<W>::type;
-  constexpr int kDeep = 8;
+  constexpr int kTeams = 32 / TEAM, kDeep = TEAM;  // rows of a warp side by side, passes: 32 rows
+  constexpr int kHold = kDeep < 16 ? kDeep : 16;   // passes whose rows are held at once
+  constexpr int kRows = kHold * kTeams;            // of a warp and step
   const int unit = blockIdx.x, kv = blockIdx.y & 1, slice = blockIdx.y >> 1;
   const int layer = unit / (p.n * p.n_heads), u = unit - layer * (p.n * p.n_heads);
   const int i = u / p.n_heads, head = u - i * p.n_heads;
@@ -209,7 +271,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__
   const int32_t* table = p.tables + (int64_t)from * p.table_stride;
   const int32_t* new_table = p.tables + (int64_t)to * p.table_stride;
   uint8_t* pool = p.pool[kv] + layer * p.pool_layer + slice * p.slice_bytes;
-  uint8_t* scales = p.scales ? p.scales + layer * p.scale_layer : nullptr;
+  uint8_t* scales = p.scales && slice == 0 ? p.scales + layer * p.scale_layer : nullptr;
   const int vecs = min(p.slice_bytes, p.row_bytes - slice * p.slice_bytes) / W;  // of a row
   int first = 0;
   if (!copies) {  // p_i - i never falls: the first that moves
@@ -220,36 +282,41 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__
       else first = mid + 1;
     }
   }
-  const int rows = blockDim.x / vecs;  // a pass
-  const int r = threadIdx.x / vecs, x = threadIdx.x - r * vecs;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / TEAM, x = lane % TEAM;
+  constexpr int kWarps = kMoveThreads / 32, kStep = kWarps * kRows;
   const auto scale_at = [&](int64_t row) {
     const int64_t block = row / p.block_size;
     return (block * 2 + kv) * p.block_size + (row - block * p.block_size);
   };
-  for (int base = first; base < keep; base += rows * kDeep) {
-    V v[kDeep];
-    uint8_t sc[kDeep];
-    int64_t b[kDeep];
-#pragma unroll
-    for (int y = 0; y < kDeep; ++y) {
-      const int k = base + y * rows + r;
-      b[y] = -1;
-      if (r < rows && k < keep) {
-        const int64_t a = row_of(p, table, head, kept[k]);
-        b[y] = a < 0 ? -1 : row_of(p, new_table, head, k);
-        if (b[y] >= 0) {
-          v[y] = *reinterpret_cast<const V*>(pool + a * p.row_bytes + x * W);
-          if (scales && slice == 0 && x == 0) sc[y] = scales[scale_at(a)];
-        }
-      }
+  const auto index = [&](int base) {
+    const int k = base + warp * kRows + lane;
+    return lane < kRows && k < keep ? kept[k] : -1;
+  };
+  int next = index(first);
+  for (int base = first; base < keep; base += kStep) {
+    const int k = base + warp * kRows + lane;
+    int64_t a = -1, b = -1;
+    if (next >= 0) {
+      a = row_of(p, table, head, next);
+      b = row_of(p, new_table, head, k);
+      if (a < 0 || b < 0) a = b = -1;
     }
-    if (!copies) __syncthreads();
+    V v[kHold];
 #pragma unroll
-    for (int y = 0; y < kDeep; ++y)
-      if (b[y] >= 0) {
-        *reinterpret_cast<V*>(pool + b[y] * p.row_bytes + x * W) = v[y];
-        if (scales && slice == 0 && x == 0) scales[scale_at(b[y])] = sc[y];
-      }
+    for (int y = 0; y < kHold; ++y) {
+      const int64_t r = __shfl_sync(0xffffffffu, a, y * kTeams + sub);
+      if (r >= 0 && x < vecs) v[y] = *reinterpret_cast<const V*>(pool + r * p.row_bytes + x * W);
+    }
+    uint8_t sc = 0;
+    if (scales && a >= 0) sc = scales[scale_at(a)];
+    next = index(base + kStep);
+    if (!copies) __syncthreads();  // all of the step is read before any of it is written
+#pragma unroll
+    for (int y = 0; y < kHold; ++y) {
+      const int64_t r = __shfl_sync(0xffffffffu, b, y * kTeams + sub);
+      if (r >= 0 && x < vecs) *reinterpret_cast<V*>(pool + r * p.row_bytes + x * W) = v[y];
+    }
+    if (scales && b >= 0) scales[scale_at(b)] = sc;
   }
 }
 
@@ -359,8 +426,9 @@ int snapmind_kv_evict_by_mass(void* k_pool, void* v_pool, void* scales, int pool
                               int64_t scale_layer_stride, float* mass, int64_t mass_layer_stride, int32_t* block_tables,
                               int64_t table_stride_seq, int32_t table_width, int32_t* seq_lens, const int32_t* seqs,
                               const int32_t* into, int32_t n_seqs, int32_t budget, int32_t recent, int32_t sinks,
-                              int32_t* kept, int32_t* free_stack, int32_t* free_top, int32_t n_layers, int32_t n_heads,
-                              int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t* err_word, void* stream) {
+                              int32_t max_len, int32_t* kept, int32_t* free_stack, int32_t* free_top, int32_t n_layers,
+                              int32_t n_heads, int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t* err_word,
+                              void* stream) {
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
   SNAPMIND_CHECK_ARG(quant || dtype_size(pool_dtype) > 0, "kv_evict: unknown pool dtype");
   SNAPMIND_CHECK_ARG(quant == (scales != nullptr), "kv_evict: scales go with an e4m3 pool, and only with one");
@@ -403,20 +471,51 @@ int snapmind_kv_evict_by_mass(void* k_pool, void* v_pool, void* scales, int pool
   p.free_stack = free_stack;
   p.free_top = free_top;
   p.err = err_word;
-  p.slices = 1;
-  p.slice_bytes = p.row_bytes;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (into) evict_tables_kernel<<<1, kTableThreads, 0, st>>>(p);
-  evict_select_kernel<<<(uint32_t)units, kSelectThreads, 0, st>>>(p);
-  int w = vec_width(p.row_bytes, p.pool_layer, reinterpret_cast<intptr_t>(k_pool), reinterpret_cast<intptr_t>(v_pool));
-  SNAPMIND_CHECK_ARG(p.row_bytes / w <= 256, "kv_evict: rows of %d bytes are too long", p.row_bytes);
+  // Sequences of up to 4096 tokens: 256 threads (8 blocks an SM), up to 16384: 512, above: 1024, each with room for
+  // that many weights (above: 49152 at a time).
+  const int64_t room = (int64_t)table_width * block_size, longest = max_len > 0 && max_len < room ? max_len : room;
+  const auto select = [&](auto kernel, int threads, bool (&done)[64]) -> cudaError_t {
+    const int64_t step = 4 * (int64_t)threads;
+    const int chunk = (int)((longest < 49152 ? longest + step - 1 : (int64_t)49152) / step * step);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev >= 64 || !done[dev])) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 49152 * 4);
+      if (e == cudaSuccess && dev < 64) done[dev] = true;
+    }
+    if (e == cudaSuccess) kernel<<<(uint32_t)units, threads, chunk * 4, st>>>(p, chunk);
+    return e;
+  };
+  static bool done[3][64] = {};
+  const cudaError_t e = longest <= 4096 ? select(evict_select_kernel<256>, 256, done[0])
+                        : longest <= 16384 ? select(evict_select_kernel<512>, 512, done[1])
+                                           : select(evict_select_kernel<1024>, 1024, done[2]);
+  if (e != cudaSuccess) return cuda_status(e, "kv_evict select");
+  const int w = vec_width(p.row_bytes, p.pool_layer, reinterpret_cast<intptr_t>(k_pool), reinterpret_cast<intptr_t>(v_pool));
+  // a slice of up to 32 vectors a row; halves of it (128 bytes at least) while there are few blocks for the SMs
+  p.slice_bytes = p.row_bytes < 32 * w ? p.row_bytes : 32 * w;
+  while (p.slice_bytes % (2 * w) == 0 && p.slice_bytes >= 256 &&
+         units * 2 * ((p.row_bytes + p.slice_bytes - 1) / p.slice_bytes) < 4 * num_sms())
+    p.slice_bytes /= 2;
+  p.slices = (p.row_bytes + p.slice_bytes - 1) / p.slice_bytes;
+  SNAPMIND_CHECK_ARG(2 * (int64_t)p.slices <= 65535, "kv_evict: rows of %d bytes are too long", p.row_bytes);
   const dim3 grid((uint32_t)units, 2 * p.slices);
+  const auto move = [&](auto width) {
+    constexpr int W = decltype(width)::value;
+    const int vecs = p.slice_bytes / W;
+    if (vecs <= 4) evict_move_kernel<W, 4><<<grid, kMoveThreads, 0, st>>>(p);
+    else if (vecs <= 8) evict_move_kernel<W, 8><<<grid, kMoveThreads, 0, st>>>(p);
+    else if (vecs <= 16) evict_move_kernel<W, 16><<<grid, kMoveThreads, 0, st>>>(p);
+    else evict_move_kernel<W, 32><<<grid, kMoveThreads, 0, st>>>(p);
+  };
   switch (w) {
-    case 16: evict_move_kernel<16><<<grid, 256, 0, st>>>(p); break;
-    case 8: evict_move_kernel<8><<<grid, 256, 0, st>>>(p); break;
-    case 4: evict_move_kernel<4><<<grid, 256, 0, st>>>(p); break;
-    case 2: evict_move_kernel<2><<<grid, 256, 0, st>>>(p); break;
-    default: evict_move_kernel<1><<<grid, 256, 0, st>>>(p);
+    case 16: move(std::integral_constant<int, 16>()); break;
+    case 8: move(std::integral_constant<int, 8>()); break;
+    case 4: move(std::integral_constant<int, 4>()); break;
+    case 2: move(std::integral_constant<int, 2>()); break;
+    default: move(std::integral_constant<int, 1>());
   }
   if (!into) evict_tables_kernel<<<1, kTableThreads, 0, st>>>(p);
   return cuda_status(cudaGetLastError(), "kv_evict launch");

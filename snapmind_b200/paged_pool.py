@@ -21,6 +21,7 @@ from __future__ import annotations
 
 from collections.abc import MutableMapping
 
+import numpy as np
 import torch
 
 from snapmind_b200 import _lib
@@ -247,44 +248,40 @@ class PagedKVPool(BlockPool):
             raise ValueError("evict: batch or seqs, not both")
         if into is not None and seqs is None:
             raise ValueError("evict: into goes with seqs")
-        ids = list(range(self.max_seqs if batch is None else batch)) if seqs is None else [int(x) for x in seqs]
-        to = ids if into is None else [int(x) for x in into]
-        every = ids if into is None else ids + to
-        if len(to) != len(ids) or len(set(every)) != len(every) or any(not 0 <= x < self.max_seqs for x in every):
+        ids = np.arange(self.max_seqs if batch is None else batch) if seqs is None else np.asarray(seqs, dtype=np.int64).reshape(-1)
+        to = ids if into is None else np.asarray(into, dtype=np.int64).reshape(-1)
+        every = ids if into is None else np.concatenate([ids, to])
+        if len(to) != len(ids) or len(np.unique(every)) != len(every) or (every.size and not 0 <= every.min() <= every.max() < self.max_seqs):
             raise ValueError("evict: sequences must be distinct and inside the pool, and each have a target of its own")
-        if into is not None:
-            take = sum(max(0, self._blocks(min(int(self._host_lens[a]), budget)) - self._blocks(int(self._host_lens[b])))
-                       for a, b in zip(ids, to))
-            if take > self._host_free:
-                raise RuntimeError(_lib.OUT_OF_BLOCKS_MSG)
-        kept = self._evict(budget, recent, sinks, len(ids), None if seqs is None else self._ids(ids),
-                           None if into is None else self._ids(to))
-        self._account_evict(budget, ids, to)
+        if budget < 1:
+            raise ValueError(f"evict: a budget of {budget}")
+        lens = self._host_lens[ids]
+        ends, held = np.minimum(lens, budget), self._host_lens[to]
+        grow = (ends + self.block_size - 1) // self.block_size - (held + self.block_size - 1) // self.block_size
+        if into is not None and int(np.maximum(grow, 0).sum()) > self._host_free:
+            raise RuntimeError(_lib.OUT_OF_BLOCKS_MSG)
+        named = [None, None]
+        if seqs is not None:  # pinned, so that the copy waits for nothing
+            both = torch.from_numpy((ids if into is None else every).astype(np.int32)).pin_memory().to(self.device, non_blocking=True)
+            named = [both[:len(ids)], None if into is None else both[len(ids):]]
+        kept = self._evict(budget, recent, sinks, len(ids), *named, int(lens.max()) if lens.size else 1)
+        self._host_lens[to] = ends
+        self._host_free -= int(grow.sum())
         return kept
 
     def evict_device(self, budget: int, recent: int = 0, sinks: int = 0, batch: int | None = None) -> torch.Tensor:
         """The device part of ``evict`` in place for the first ``batch`` sequences: launches that a CUDA graph can replay.
         The caller accounts every replay with ``account_evict``."""
-        return self._evict(budget, recent, sinks, self.max_seqs if batch is None else batch, None, None)
+        return self._evict(budget, recent, sinks, self.max_seqs if batch is None else batch, None, None, 0)
 
     def account_evict(self, budget: int, batch: int | None = None) -> None:
         """Bring the host mirrors to what ``evict(budget, batch=batch)`` makes of them."""
-        ids = range(self.max_seqs if batch is None else batch)
-        self._account_evict(budget, ids, ids)
+        lens = self._host_lens[:self.max_seqs if batch is None else batch]
+        ends = np.minimum(lens, budget)
+        self._host_free += int(((lens + self.block_size - 1) // self.block_size - (ends + self.block_size - 1) // self.block_size).sum())
+        lens[:] = ends
 
-    def _blocks(self, n: int) -> int:
-        return (n + self.block_size - 1) // self.block_size
-
-    def _ids(self, ids) -> torch.Tensor:
-        return torch.tensor(ids, dtype=torch.int32, device=self.device)
-
-    def _account_evict(self, budget, ids, to):
-        ends = [min(int(self._host_lens[a]), budget) for a in ids]
-        for b, n in zip(to, ends):
-            self._host_free += self._blocks(int(self._host_lens[b])) - self._blocks(n)
-            self._host_lens[b] = n
-
-    def _evict(self, budget, recent, sinks, n, ids, to):
+    def _evict(self, budget, recent, sinks, n, ids, to, max_len):
         if self.mass is None:
             raise ValueError("evict needs a pool with mass=True")
         if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
@@ -297,7 +294,7 @@ class PagedKVPool(BlockPool):
                 self.k.data_ptr(), self.v.data_ptr(), self.scales.data_ptr() if self.quantised else None, self._pool_code,
                 self.layer_stride, self.scale_layer_stride, self.mass.data_ptr(), self.mass.stride(0),
                 self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq, self.seq_lens.data_ptr(),
-                _lib.ptr(ids), _lib.ptr(to), n, budget, recent, sinks, kept.data_ptr(), self.free_stack.data_ptr(),
+                _lib.ptr(ids), _lib.ptr(to), n, budget, recent, sinks, max_len, kept.data_ptr(), self.free_stack.data_ptr(),
                 self.free_top.data_ptr(), self.n_layers, self.n_kv_heads, self.head_dim, self.block_size, self.num_blocks,
                 self.err.data_ptr(), _lib.raw_stream(self._index),
             )  # fmt: skip

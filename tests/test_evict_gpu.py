@@ -188,6 +188,8 @@ def weights(shape, g, kind):
         x = torch.where((r > 0.1) & (r < 0.2), -x, x)
         x = torch.where(r > 0.98, torch.full_like(x, float("-inf")), x)
         x = torch.where((r > 0.2) & (r < 0.3), x * 1e-42, x)
+        x = torch.where((r > 0.3) & (r < 0.32), torch.zeros_like(x), x)
+        x = torch.where((r > 0.32) & (r < 0.34), -torch.zeros_like(x), x)
     return x
 
 
