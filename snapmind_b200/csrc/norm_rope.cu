@@ -10,8 +10,7 @@
 // as the append kernel does), or the keys to a plain tensor.  All arithmetic is f32, rounded once on the way out.
 //
 // HBM bound: a row is read once and written once.  A team of lanes holds a row, eight elements a lane, so a
-// sum of squares is a few shuffles and the rotation's partner is one lane away; a CTA takes a token, and a lane keeps
-// the token's cosines and sines for all the rows that it does.
+// sum of squares is a few shuffles and the rotation's partner is one lane away.
 #include "pairs.cuh"
 
 namespace snapmind {
@@ -86,104 +85,212 @@ __device__ __forceinline__ int64_t token_position(const NormRopeParams& p, int b
   return -1;
 }
 
+// A lane's eight elements of a row: four from d0 and four from d1, as they lie in memory and as pairs of f32.
+template <typename T> struct Four { using type = uint2; };
+template <> struct Four<float> { using type = uint4; };
+template <typename T> struct Raw { typename Four<T>::type w[2]; };
 template <typename T>
-__device__ __forceinline__ void load8(const T* x, float* f) {
-  uint4 w[sizeof(T) / 2];
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(x)[i];
-  const T* e = reinterpret_cast<const T*>(w);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = Conv<T>::to_f(e[i]);
+__device__ __forceinline__ Raw<T> load_raw(const T* x, int d0, int d1) {
+  using V = typename Four<T>::type;
+  return Raw<T>{{*reinterpret_cast<const V*>(x + d0), *reinterpret_cast<const V*>(x + d1)}};
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* x, const float* f) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(x)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(x)[1] = make_float4(f[4], f[5], f[6], f[7]);
-  } else {
-    *reinterpret_cast<uint4*>(x) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-  }
+__device__ __forceinline__ void spread8(const Raw<T>& r, float2* f) {
+  const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = make_float2(Conv<T>::to_f(e[2 * i]), Conv<T>::to_f(e[2 * i + 1]));
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* x, float2 a, float2 b) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(x) = make_float4(a.x, a.y, b.x, b.y);
+  else *reinterpret_cast<uint2*>(x) = make_uint2(pack2<T>(a.x, a.y), pack2<T>(b.x, b.y));
 }
 
-// One CTA per token; TEAM lanes per row, of which head_dim / 8 hold eight elements each.
+// A CTA takes a run of items (token, kHeads heads) of one of q, k and v; TEAM lanes hold a row, head_dim / 8 of them eight
+// elements each: a lane of the rotated part four and the four that they turn with, so nothing is exchanged but the
+// sum of squares, and a token's cosines and sines serve kHeads rows.  Where tokens come from and go to (positions,
+// sequences, lengths, table entries: reads that wait for one another) is worked out for all of a CTA's tokens at
+// once, and the next item's rows, cosines and sines are on their way while one is computed.  What bounds it beside HBM
+// is the number of instructions: 8200 tokens of 48 heads of 128 (bf16) took 70 us with 219 a row and warp (64-bit
+// addresses, partners by shuffles), 79 with 178 and cosines that a row waited for, 41 us (4.6 TB/s) with 115.
+struct Rows32 { int32_t seq, head, tok, out_seq, out_head, out_tok; };  // RowSet's strides where they fit
+struct Split {
+  Rows32 at[3];        // q, k, v
+  int32_t q, k;        // CTAs of q, of k (v's come last)
+  int32_t items;       // of a CTA
+  FastDiv by_groups[2], by_tok;  // groups of kHeads heads: of q, of k and v
+  int32_t groups[2];
+};
+constexpr int kMostItems = 512, kHeads = 4;
+
 template <typename T, typename KV, int TEAM>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
+__global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const __grid_constant__ NormRopeParams p, const __grid_constant__ Split split) {
   constexpr int kTeams = kThreads / TEAM;
   constexpr bool kQuant = std::is_same<KV, uint8_t>::value;
+  constexpr uint32_t kAll = 0xffffffffu;
+  __shared__ int32_t at_turn[kMostItems + 2];  // of the CTA's tokens: the first of its cosines, -1: no such position
+  __shared__ int64_t at_row[kMostItems + 2];   // pool row of head 0, -1: none
+  __shared__ int64_t at_scale[kQuant ? kMostItems + 2 : 1];  // its K scale
   const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
-  const int b = p.n_seq == 1 ? 0 : blockIdx.x / p.n_tok, t = blockIdx.x - b * p.n_tok;
-  const bool stores = p.v.in != nullptr;
   const bool mine = 8 * lane < p.head_dim, turns = 8 * lane < p.rot;
-  const int d = mine ? 8 * lane : 0;
-  // the lane that holds the rotation's partner, and its sign
-  const int half = p.rot / 16, other = !turns ? lane : lane < half ? lane + half : lane - half;
-  const float sign = lane < half ? -1.f : 1.f;
-  const int64_t pos = token_position(p, b, t);
-  if (pos < 0) return;
-  const int64_t slot = stores ? token_slot(p, t) : -1;
-  float c[8], s[8];
+  const int d0 = !mine ? 0 : turns ? 4 * lane : 8 * lane, d1 = !mine ? 4 : turns ? p.rot / 2 + d0 : d0 + 4;
+  const int cta = blockIdx.x, kind = cta < split.q ? 0 : cta < split.q + split.k ? 1 : 2;
+  const RowSet& set = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
+  const Rows32& by = split.at[kind];
+  const FastDiv& by_groups = split.by_groups[kind > 0];
+  const int n_groups = split.groups[kind > 0], all = p.n_seq * p.n_tok * n_groups;
+  const int e0 = (cta - (kind == 0 ? 0 : kind == 1 ? split.q : split.q + split.k)) * split.items, e1 = min(all, e0 + split.items);
+  const int token0 = by_groups.div(e0), tokens = by_groups.div(e1 - 1) - token0 + 1;
+  const bool stores = kind > 0 && p.v.in != nullptr;
+  const T* in = static_cast<const T*>(set.in);
+  const auto sequence = [&](int token) { return p.n_seq == 1 ? 0 : split.by_tok.div(token); };
+  struct Item { Raw<T> row[kHeads]; };
+  const auto fetch = [&](Item& r, int e) {
+    r = Item{};
+    if (e >= e1 || !mine) return;
+    const int token = by_groups.div(e), head = (e - token * n_groups) * kHeads, b = sequence(token);
+    const T* from = in + (b * by.seq + head * by.head + (token - b * p.n_tok) * by.tok);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
-  if (turns) {
-    load8(p.cos_t + pos * p.rot + d, c);
-    load8(p.sin_t + pos * p.rot + d, s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] *= sign;
+    for (int h = 0; h < kHeads; ++h)
+      if (head + h < set.heads) r.row[h] = load_raw(from + h * by.head, d0, d1);
+  };
+  Raw<float> c_next = {}, s_next = {};
+  const auto fetch_turn = [&](int e) {
+    if (kind == 2 || !turns || e >= e1) return;
+    const int turn = at_turn[by_groups.div(e) - token0];
+    if (turn < 0) return;
+    c_next = load_raw(p.cos_t + turn, d0, d1);
+    s_next = load_raw(p.sin_t + turn, d0, d1);
+  };
+  Item next;
+  fetch(next, e0 + team);
+  for (int i = threadIdx.x; i < tokens; i += kThreads) {
+    const int token = token0 + i, b = sequence(token), t = token - b * p.n_tok;
+    const int64_t pos = token_position(p, b, t);
+    at_turn[i] = pos < 0 ? -1 : (int)pos * p.rot;
+    const int64_t row = stores && pos >= 0 ? token_slot(p, t) : -1;
+    at_row[i] = row;
+    if (kQuant && row >= 0) at_scale[i] = scale_byte_at(p, row, 0);
   }
-  const int rows = p.q.heads + p.k.heads + (stores ? p.v.heads : 0);
+  // a row's largest magnitude, by its team; infinities become NaN, as they are stored, and NaN do not count
+  const auto magnitude = [&](float2* x) {
+    const auto largest = [&] {
+      float a = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) a = fmaxf(a, fmaxf(fabsf(x[k].x), fabsf(x[k].y)));
+#pragma unroll
+      for (int o = TEAM / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(kAll, a, o));
+      return a;
+    };
+    float a = largest();
+    if (__any_sync(kAll, a == INFINITY)) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[k].x = fabsf(x[k].x) < INFINITY ? x[k].x : __uint_as_float(0x7FC00000u);
+        x[k].y = fabsf(x[k].y) < INFINITY ? x[k].y : __uint_as_float(0x7FC00000u);
+      }
+      a = largest();
+    }
+    return a;
+  };
+  // a row into the pool: of token token0 + i, head h
+  const auto put = [&](int i, int64_t row0, int h, const float2* x, float a) {
+    KV* to = static_cast<KV*>(p.pool[kind > 1]) + (row0 + h * p.block_size) * p.head_dim;
+    if constexpr (kQuant) {
+      const int x2 = row_exponent(a);
+      const float inv = __uint_as_float((uint32_t)(127 - x2) << 23);
+      const auto codes = [&](float2 y, float2 z) {
+        y = mul2(y, inv), z = mul2(z, inv);
+        return codes4(y.x, y.y, z.x, z.y);
+      };
+      *reinterpret_cast<uint32_t*>(to + d0) = codes(x[0], x[1]);
+      *reinterpret_cast<uint32_t*>(to + d1) = codes(x[2], x[3]);
+      if (lane == 0) p.scales[at_scale[i] + (2 * h + kind - 1) * p.block_size] = (uint8_t)(x2 + 127);
+    } else {
+      store4(to + d0, x[0], x[1]);
+      store4(to + d1, x[2], x[3]);
+    }
+  };
+  if (kind == 2) {  // values: as they are, in the pool's type
+    __syncthreads();
+    for (int base = e0; base < e1; base += kTeams) {
+      const int e = min(base + team, e1 - 1), i = by_groups.div(e) - token0, head0 = (e - (token0 + i) * n_groups) * kHeads;
+      const int64_t row0 = at_row[i];
+      const bool there = base + team < e1 && row0 >= 0 && mine;
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+        const bool on = there && head0 + h < set.heads;
+        if constexpr (std::is_same<T, KV>::value) {
+          if (on) {
+            T* to = static_cast<T*>(p.pool[1]) + (row0 + (head0 + h) * p.block_size) * p.head_dim;
+            *reinterpret_cast<typename Four<T>::type*>(to + d0) = next.row[h].w[0];
+            *reinterpret_cast<typename Four<T>::type*>(to + d1) = next.row[h].w[1];
+          }
+        } else {
+          float2 x[4];
+          spread8(next.row[h], x);
+          const float a = kQuant ? magnitude(x) : 0.f;
+          if (on) put(i, row0, head0 + h, x, a);
+        }
+      }
+      fetch(next, base + kTeams + team);
+    }
+    return;
+  }
+  const T* norm = static_cast<const T*>(kind == 0 ? p.q_norm : p.k_norm);
+  const int norm_head = (int)(kind == 0 ? p.q_norm_head : p.k_norm_head);
+  float2 w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = make_float2(1.f, 1.f);
+  if (norm != nullptr && norm_head == 0) spread8(load_raw(norm, d0, d1), w);
   const float inv_d = 1.f / p.head_dim;
-  for (int r0 = 0; r0 < rows; r0 += kTeams) {
-    const int r = r0 + team;  // a warp's teams run together: shuffles inside
-    const int kind = r < p.q.heads ? 0 : r < p.q.heads + p.k.heads ? 1 : 2;
-    const int h = kind == 0 ? r : kind == 1 ? r - p.q.heads : r - p.q.heads - p.k.heads;
-    const RowSet& set = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
-    float x[8];
+  __syncthreads();
+  fetch_turn(e0 + team);
+  for (int base = e0; base < e1; base += kTeams) {
+    const Item now = next;
+    float2 c[4], s[4];
+    spread8(c_next, c);
+    spread8(s_next, s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (r < rows && mine) load8(static_cast<const T*>(set.in) + b * set.seq + h * set.head + t * set.tok + d, x);
-    // the teams of a warp may hold rows of different kinds: every shuffle is taken by all lanes
-    float sum = 0.f;
+    for (int k = 0; k < 2; ++k) s[k] = make_float2(-s[k].x, -s[k].y);
+    fetch(next, base + kTeams + team);
+    fetch_turn(base + kTeams + team);
+    const int e = min(base + team, e1 - 1), token = by_groups.div(e), i = token - token0, head0 = (e - token * n_groups) * kHeads;
+    const int64_t row0 = at_row[i];
+    const bool there = base + team < e1 && at_turn[i] >= 0 && mine && (!stores || row0 >= 0);
+    const int b = sequence(token);
+    T* to_out = static_cast<T*>(set.out) + (b * by.out_seq + head0 * by.out_head + (token - b * p.n_tok) * by.out_tok);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+    for (int h = 0; h < kHeads; ++h) {
+      const bool on = there && head0 + h < set.heads;
+      float2 x[4];
+      spread8(now.row[h], x);
+      if (norm != nullptr) {
+        float2 sq = times(x[0], x[0]);
 #pragma unroll
-    for (int o = TEAM / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const void* norm = kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr;
-    if (norm != nullptr && r < rows) {
-      float w[8];
-      load8(static_cast<const T*>(norm) + h * (kind == 0 ? p.q_norm_head : p.k_norm_head) + d, w);
-      const float f = 1.f / sqrtf(fmaf(sum, inv_d, p.eps));
+        for (int k = 1; k < 4; ++k) sq = fma2(x[k], x[k], sq);
+        float sum = sq.x + sq.y;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * f * w[i];
-    }
-    __syncwarp();
-    float y[8];
+        for (int o = TEAM / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+        const float f = rsqrtf(fmaf(sum, inv_d, p.eps));
+        if (norm_head != 0 && on) spread8(load_raw(norm + (head0 + h) * norm_head, d0, d1), w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], other, TEAM);
-    if (kind < 2) {
+        for (int k = 0; k < 4; ++k) x[k] = times(mul2(x[k], f), w[k]);
+      }
+      if (turns) {  // x[0 .. 1] turn with x[2 .. 3]
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = fmaf(y[i], s[i], x[i] * c[i]);
-    }
-    float a = 0.f;
-    if (kQuant) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a = fmaxf(a, finite_abs(x[i]));
-#pragma unroll
-      for (int o = TEAM / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-    }
-    if (r >= rows || !mine) continue;
-    if (kind == 0 || !stores) {
-      store8(static_cast<T*>(set.out) + b * set.out_seq + h * set.out_head + t * set.out_tok + d, x);
-    } else if (slot >= 0) {
-      const int64_t row = slot + (int64_t)h * p.block_size;
-      KV* to = static_cast<KV*>(p.pool[kind - 1]) + row * p.head_dim + d;
-      if constexpr (kQuant) {
-        const int e = row_exponent(a);
-        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-        *reinterpret_cast<uint2*>(to) = make_uint2(codes4(scaled(x[0], inv), scaled(x[1], inv), scaled(x[2], inv), scaled(x[3], inv)),
-                                                   codes4(scaled(x[4], inv), scaled(x[5], inv), scaled(x[6], inv), scaled(x[7], inv)));
-        if (lane == 0) p.scales[scale_byte_at(p, row, kind - 1)] = (uint8_t)(e + 127);
-      } else {
-        store8(to, x);
+        for (int k = 0; k < 2; ++k) {
+          const float2 y0 = x[k], y1 = x[k + 2];
+          x[k] = fma2(y1, s[k], times(y0, c[k]));
+          x[k + 2] = fma2(y0, s[k + 2], times(y1, c[k + 2]));
+        }
+      }
+      if (stores) {
+        const float a = kQuant ? magnitude(x) : 0.f;
+        if (on) put(i, row0, head0 + h, x, a);
+      } else if (on) {
+        store4(to_out + h * by.out_head + d0, x[0], x[1]);
+        store4(to_out + h * by.out_head + d1, x[2], x[3]);
       }
     }
   }
@@ -243,7 +350,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_any_kernel(const __grid_co
         for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
         const int e = row_exponent(a);
         const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-        each([&](int d, float z) { to[d] = (uint8_t)codes4(scaled(z, inv), 0.f, 0.f, 0.f); });
+        each([&](int d, float z) { to[d] = (uint8_t)codes2(scaled(z, inv), 0.f); });
         if (lane == 0) p.scales[scale_byte_at(p, row, kind - 1)] = (uint8_t)(e + 127);
       } else {
         each([&](int d, float z) { to[d] = Conv<KV>::from_f(z); });
@@ -252,27 +359,53 @@ __global__ void __launch_bounds__(kThreads) norm_rope_any_kernel(const __grid_co
   }
 }
 
-bool vectors_fit(const NormRopeParams& p, int esz, int pool_esz) {
-  if (p.head_dim % 8 || p.head_dim > 256 || p.rot % 16) return false;
-  const auto a16 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
-  const int v = 16 / esz;
-  for (const RowSet* s : {&p.q, &p.k, &p.v}) {
-    if (!a16(s->in) || !a16(s->out)) return false;
-    if (s->seq % v || s->head % v || s->tok % v || s->out_seq % v || s->out_head % v || s->out_tok % v) return false;
+// Whether the rows are whole pieces of four elements, and their offsets fit 32 bits.
+bool pieces_fit(const NormRopeParams& p, int esz, int pool_esz, Split& split) {
+  if (p.head_dim % 8 || p.head_dim > 256 || p.rot % 8) return false;
+  const auto aligned = [](const void* x, int to) { return (reinterpret_cast<uintptr_t>(x) & (to - 1)) == 0; };
+  const RowSet* sets[3] = {&p.q, &p.k, &p.v};
+  for (int i = 0; i < 3; ++i) {
+    const RowSet& s = *sets[i];
+    if (!aligned(s.in, 4 * esz) || !aligned(s.out, 4 * esz)) return false;
+    const auto fit = [&](int64_t seq, int64_t head, int64_t tok) {
+      if (seq < 0 || head < 0 || tok < 0 || seq % 4 || head % 4 || tok % 4) return false;
+      const auto reach = [](int64_t stride, int64_t n) { return n <= 1 ? 0.0 : (double)stride * (double)(n - 1); };
+      return reach(seq, p.n_seq) + reach(head, s.heads) + reach(tok, p.n_tok) + p.head_dim < 2147483648.0;
+    };
+    if (!fit(s.seq, s.head, s.tok) || !fit(s.out_seq, s.out_head, s.out_tok)) return false;
+    const auto of = [](int64_t stride, int n) { return n <= 1 ? 0 : (int32_t)stride; };
+    split.at[i] = Rows32{of(s.seq, p.n_seq), of(s.head, s.heads), of(s.tok, p.n_tok), of(s.out_seq, p.n_seq), of(s.out_head, s.heads), of(s.out_tok, p.n_tok)};
   }
-  if (!a16(p.q_norm) || !a16(p.k_norm) || p.q_norm_head % v || p.k_norm_head % v) return false;
-  if (!a16(p.cos_t) || !a16(p.sin_t)) return false;
-  return a16(p.pool[0]) && a16(p.pool[1]) && (p.head_dim * pool_esz) % 8 == 0;
+  for (int64_t head : {p.q_norm_head, p.k_norm_head})
+    if (head < 0 || head % 4 || head > 1 << 20) return false;
+  if (!aligned(p.q_norm, 4 * esz) || !aligned(p.k_norm, 4 * esz) || !aligned(p.cos_t, 16) || !aligned(p.sin_t, 16)) return false;
+  if (p.n_pos * p.rot >= (int64_t)1 << 31) return false;
+  return aligned(p.pool[0], 4 * pool_esz) && aligned(p.pool[1], 4 * pool_esz);
 }
 
 template <typename T, typename KV>
 int launch(const NormRopeParams& p, cudaStream_t st) {
   const int64_t tokens = (int64_t)p.n_seq * p.n_tok;
-  if (vectors_fit(p, sizeof(T), sizeof(KV))) {
+  Split split = {};
+  if (pieces_fit(p, sizeof(T), sizeof(KV), split)) {
     const int lanes = p.head_dim / 8;
-    if (lanes <= 8) norm_rope_kernel<T, KV, 8><<<(uint32_t)tokens, kThreads, 0, st>>>(p);
-    else if (lanes <= 16) norm_rope_kernel<T, KV, 16><<<(uint32_t)tokens, kThreads, 0, st>>>(p);
-    else norm_rope_kernel<T, KV, 32><<<(uint32_t)tokens, kThreads, 0, st>>>(p);
+    // items of a CTA: one wave of two CTAs an SM, an item for every team at least
+    for (int i = 0; i < 2; ++i) {
+      split.groups[i] = ((i ? p.k.heads : p.q.heads) + kHeads - 1) / kHeads;
+      split.by_groups[i] = FastDiv(split.groups[i] > 0 ? split.groups[i] : 1);
+    }
+    const int64_t all = tokens * (split.groups[0] + split.groups[1] * (p.v.in ? 2 : 1)), slots = 2 * (int64_t)num_sms() - 2;
+    const int teams = kThreads / (lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32);
+    int64_t items = ((all + slots - 1) / slots + teams - 1) / teams * teams;
+    items = items < kMostItems ? items : kMostItems;
+    split.items = (int32_t)items;
+    split.q = (int32_t)((tokens * split.groups[0] + items - 1) / items);
+    split.k = (int32_t)((tokens * split.groups[1] + items - 1) / items);
+    split.by_tok = FastDiv(p.n_tok);
+    const uint32_t grid = split.q + split.k + (p.v.in ? split.k : 0);
+    if (lanes <= 8) norm_rope_kernel<T, KV, 8><<<grid, kThreads, 0, st>>>(p, split);
+    else if (lanes <= 16) norm_rope_kernel<T, KV, 16><<<grid, kThreads, 0, st>>>(p, split);
+    else norm_rope_kernel<T, KV, 32><<<grid, kThreads, 0, st>>>(p, split);
   } else {
     norm_rope_any_kernel<T, KV><<<(uint32_t)tokens, kThreads, 0, st>>>(p);
   }
@@ -300,7 +433,7 @@ int launch_any(const NormRopeParams& p, int dtype, int pool_dtype, cudaStream_t 
 int check_common(const NormRopeParams& p, int dtype, int64_t tokens) {
   SNAPMIND_CHECK_ARG(dtype_size(dtype) > 0, "norm_rope: unknown dtype");
   SNAPMIND_CHECK_ARG(p.n_seq >= 0 && p.n_tok >= 0 && p.q.heads >= 0 && p.k.heads > 0 && p.head_dim > 0 && p.n_pos > 0 &&
-                         tokens < (int64_t)1 << 31,
+                         tokens * (p.q.heads > p.k.heads ? p.q.heads : p.k.heads) < (int64_t)1 << 30,
                      "norm_rope: bad sizes");
   SNAPMIND_CHECK_ARG(p.rot >= 0 && p.rot <= p.head_dim && p.rot % 2 == 0, "norm_rope: %d rotated dims of %d (even, at most head_dim)",
                      p.rot, p.head_dim);

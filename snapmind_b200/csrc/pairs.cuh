@@ -26,6 +26,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
+__device__ __forceinline__ float2 times(float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 __device__ __forceinline__ float2 mul2(float2 a, float b) {
   float2 r;
   asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %4}; mul.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
@@ -70,10 +77,7 @@ __device__ __forceinline__ float finite_abs(float x) {
 __device__ __forceinline__ float scaled(float x, float inv) {
   return fabsf(x) < INFINITY ? x * inv : __uint_as_float(0x7FC00000u);
 }
-__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
+__device__ __forceinline__ uint32_t codes2(float a, float b) { return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) { return codes2(a, b) | (codes2(c, d) << 16); }
 
 }  // namespace snapmind
