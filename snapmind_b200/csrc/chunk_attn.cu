@@ -596,7 +596,7 @@ int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st) {
 using namespace snapmind;
 
 static int64_t chunk_workspace_bytes(int32_t head_dim) { return partials_bytes(head_dim) + (max_ctas() * 4 + 255) / 256 * 256; }
-static int64_t stats_bytes(int32_t total_q, int32_t n_q_heads) { return ((int64_t)total_q * n_q_heads * 8 + 255) / 256 * 256; }
+static int64_t stats_bytes(int32_t total_q, int32_t n_q_heads) { return ((int64_t)total_q * n_q_heads * 4 + 255) / 256 * 256; }
 
 // The attention of a call: the kernel that its shapes take, and the merge.
 static int launch_attention(ChunkParams& p, int dtype, int pool_dtype, int32_t flags, cudaStream_t st) {
@@ -711,7 +711,7 @@ int snapmind_paged_gqa_chunk_mass(const void* q, int64_t q_stride_tok, int64_t q
   p.odd = nullptr;
   char* more = static_cast<char*>(workspace) + attention;  // the rows' statistics, then what the pass over the weights needs
   char* pass = more + stats_bytes(total_q, n_q_heads);
-  p.stats = mass ? reinterpret_cast<float2*>(more) : nullptr;
+  p.stats = mass ? reinterpret_cast<float*>(more) : nullptr;
   if (mass && cu_q == nullptr && decode_keeps_scores(head_dim, p.group)) p.scores = reinterpret_cast<float*>(pass + mass_workspace_bytes());
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = launch_attention(p, dtype, pool_dtype, flags, st);

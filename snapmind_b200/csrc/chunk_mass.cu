@@ -18,7 +18,7 @@ struct MassSmem {
   static constexpr int kCtas = D4 == 1 ? 4 : D4 == 2 ? 2 : 1;
   float q[kRows * P];
   float k[kKeys * P];
-  float2 stats[kRows];
+  float x[kRows];
   int32_t qpos[kRows];
   int64_t row[kKeys];
   int32_t pos[kKeys];
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, MassSmem<D4>::kCtas) mass_generic_ke
       if (tid < kRows) {
         int tok, g;
         const bool there = query(tid, &tok, &g);
-        S.stats[tid] = there ? p.stats[(int64_t)(c.q_first + tok) * p.n_q_heads + head0 + g] : make_float2(0.f, 0.f);
+        S.x[tid] = there ? *row_stats(p, c.kvh, c.q_first + tok, slice * p.gw + g) : -INFINITY;
         S.qpos[tid] = there ? w.kr.pos0 + tok : INT32_MIN / 2;
       }
       load_rows<T, D4>(S.q, hd, q_vec,
@@ -145,11 +145,11 @@ __global__ void __launch_bounds__(kThreads, MassSmem<D4>::kCtas) mass_generic_ke
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 st = S.stats[ty + 16 * i];
+        const float x = S.x[ty + 16 * i];
         const int q = S.qpos[ty + 16 * i];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float weight = ex2(fmaf(s2[i][j].x + s2[i][j].y, c2, -st.x)) * st.y;
+          const float weight = ex2(fmaf(s2[i][j].x + s2[i][j].y, c2, x));
           if (sees(p, q, S.pos[tx + 16 * j])) acc[j] += weight;
         }
       }
@@ -221,8 +221,8 @@ __global__ void __launch_bounds__(kScoreThreads, 2) mass_scores_kernel(const __g
     const Piece& c = w.c;
     const KeyRange kr = key_range(p, c.len, c.n, c.i0, c.i0 + 1);
     const int group = G > 0 ? G : p.group;
-    const float2* stats = p.stats + (int64_t)c.q_first * p.n_q_heads + c.kvh * group;
-    float2 st[G > 0 ? G : 1];
+    const float* stats = row_stats(p, c.kvh, c.q_first, 0);
+    float st[G > 0 ? G : 1];
     if constexpr (G > 0) {
 #pragma unroll
       for (int g = 0; g < G; ++g) st[g] = stats[g];
@@ -255,9 +255,9 @@ __global__ void __launch_bounds__(kScoreThreads, 2) mass_scores_kernel(const __g
         float sum = 0.f;
         if constexpr (G > 0) {
 #pragma unroll
-          for (int g = 0; g < G; ++g) sum = fmaf(ex2(s[u][g] - st[g].x), st[g].y, sum);
+          for (int g = 0; g < G; ++g) sum += ex2(s[u][g] + st[g]);
         } else {
-          for (int g = 0; g < group; ++g) sum = fmaf(ex2(p.scores[row[u] * group + g] - stats[g].x), stats[g].y, sum);
+          for (int g = 0; g < group; ++g) sum += ex2(p.scores[row[u] * group + g] + stats[g]);
         }
         mass[row[u]] = m[u] + sum;
       }

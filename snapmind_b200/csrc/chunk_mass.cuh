@@ -1,9 +1,9 @@
 // Work plan of the kernels that add the weights of a call's softmax to their keys (chunk_mass.cu,
 // chunk_mass_umma.cu).
 //
-//   mass[key] += sum over the call's rows i that see it of 2^(score(i, key) - x_i) y_i
+//   mass[key] += sum over the call's rows i that see it of 2^(score(i, key) + x_i)
 //
-// with x_i, y_i the reference and 1 / sum that the attention kernels left (ChunkParams::stats).  A weight is
+// with x_i = -log2 of the row's sum, as the attention kernels left it (ChunkParams::stats).  A weight is
 // known only when its row's whole softmax is, so it takes a second pass over the scores, but not over V.
 //
 // The roles of chunk_plan.cuh are turned round: a unit is one (sequence, kv head, tile of key_tile keys),
@@ -200,6 +200,11 @@ __device__ __forceinline__ int64_t mass_row(const ChunkParams& p, const KeyRange
     return -1;
   }
   return ((int64_t)phys * p.n_kv_heads + kvh) * p.block_size + (*pos - j * p.block_size);
+}
+
+// x_i of row (token, head g of the kv head's group).
+__device__ __forceinline__ const float* row_stats(const ChunkParams& p, int kvh, int64_t token, int g) {
+  return p.stats + (kvh * (int64_t)p.total_q + token) * p.group + g;
 }
 
 // Whether a query at position q sees position pos.

@@ -12,9 +12,15 @@
 //                   go to the key's factor c)
 //   warp 9          stages Q by TMA
 //   warp 10         issues the MMAs
-//   warp 11         the rows' x_i
+//   warp 11         stages the rows' x_i
 // Rows of the last step that are no queries, and keys that a row does not see, are left out by intervals: the
 // rows that see a key are one run of them.
+// What bounds it is the exponentials: a step of 256 keys x 128 rows has 2048 cycles of them (an SM does 16 a cycle) and
+// took 2900, the rest being what a warp waits for between its chunks (without them it took 1250, 1024 of them
+// products).  2048 new tokens behind 30720 cached ones, 32 heads over 8 of 128: about 640 us behind the attention's 990;
+// 16 x 5 tokens over 1 to 8 thousand: 44 us, of which K takes 21 to read.  Tried and no better: four warps a key tile more
+// (1% here, 7 us more for the small case), a part of the exponentials by a polynomial on the FMA units (with
+// those 6%, without 3% worse), four stages of Q.
 #include <cuda.h>
 
 #include "chunk_mass.cuh"
@@ -37,12 +43,12 @@ template <int D> struct Shape {
 };
 
 struct Ctrl {
-  uint64_t k_full[2], k_empty[2], q_full[2], q_empty[2], x_full[2], x_empty[2];
+  uint64_t k_full[2], k_empty[2], q_full[4], q_empty[4], x_full[4], x_empty[4];
   uint64_t s_full[2][2], s_free[2][2];  // [key tile][buffer]
   uint64_t done;                        // every MMA has completed
   uint32_t tmem_base;
   int32_t abort;
-  alignas(16) float x[2][kRowsStep];  // -x_i of a step's rows
+  alignas(16) float x[4][kRowsStep];  // x_i of a step's rows
   MassShared plan;
 };
 
@@ -51,8 +57,8 @@ static_assert(smem_bytes<128>() <= 232448, "shared memory budget");
 static_assert(Shape<64>::kQRing >= kMaxChunkBatch * 4, "plan scratch in the K stages");
 
 template <bool kQuant> struct Roles {
-  static constexpr int kThreads = kQuant ? 512 : 384;
-  static constexpr int kLoadK = 8, kLoadQ = 9, kMma = 10, kStats = 11, kConvert = 12;
+  static constexpr int kLoadK = 8, kLoadQ = kLoadK + 1, kMma = kLoadK + 2, kStats = kLoadK + 3, kConvert = kLoadK + 4;
+  static constexpr int kThreads = (kConvert + (kQuant ? 4 : 0)) * 32;
 };
 
 __device__ __forceinline__ uint32_t low_bits(int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; }
@@ -90,13 +96,17 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&C.k_full[i]), kQuant ? 128 : 1);
       mbar_init(smem_u32(&C.k_empty[i]), 1);
-      mbar_init(smem_u32(&C.q_full[i]), 1);
-      mbar_init(smem_u32(&C.q_empty[i]), 1);
-      mbar_init(smem_u32(&C.x_full[i]), 32);
-      mbar_init(smem_u32(&C.x_empty[i]), 256);
+      mbar_init(smem_u32(&C.q_full[2 * i]), 1);
+      mbar_init(smem_u32(&C.q_empty[2 * i]), 1);
+      mbar_init(smem_u32(&C.q_full[2 * i + 1]), 1);
+      mbar_init(smem_u32(&C.q_empty[2 * i + 1]), 1);
+      for (int k = 2 * i; k < 2 * i + 2; ++k) {
+        mbar_init(smem_u32(&C.x_full[k]), 2 * 32);
+        mbar_init(smem_u32(&C.x_empty[k]), 8);
+      }
       for (int t = 0; t < 2; ++t) {
         mbar_init(smem_u32(&C.s_full[t][i]), 1);
-        mbar_init(smem_u32(&C.s_free[t][i]), 128);
+        mbar_init(smem_u32(&C.s_free[t][i]), 4);
       }
     }
     mbar_init(smem_u32(&C.done), 1);
@@ -121,7 +131,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
 
   MassWalk w;
   bool on = w.start(p, C.plan), ok = true;
-  if (warp >= 8) {
+  if (warp >= Ro::kLoadK) {
     if (warp == Ro::kLoadK) {
       // ------------------------------------------------------------------ K copies
       if constexpr (!kQuant) {
@@ -137,35 +147,32 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
           TileRows at(tiles, w.kr, c, lane);
           const int b = w.c.b, kvh = w.c.kvh;
           for (int next = w.c.tile; on && w.c.b == b && w.c.kvh == kvh && w.c.tile == next; on = w.next(mp), ++unit, ++next) {
-            const int st = unit & 1;
-            ok = __all_sync(0xffffffffu, role_wait(C.abort, smem_u32(&C.k_empty[st]), ((unit >> 1) & 1) ^ 1));
+            const int st = unit % Sh::kK;
+            ok = __all_sync(0xffffffffu, role_wait(C.abort, smem_u32(&C.k_empty[st]), ((unit / Sh::kK) & 1) ^ 1));
             if (!ok) break;
             const uint32_t bar = smem_u32(&C.k_full[st]);
-            // both tiles' bytes are announced before either is copied
+            // both tiles' bytes are announced before either is copied (a batch of the table walk holds both)
             at.advance(2 * w.c.tile);
-            const uint32_t have0 = at.have(2 * w.c.tile);
-            int y0[16];
+            const uint32_t have = __popc(at.have(2 * w.c.tile)) + __popc(at.have(2 * w.c.tile + 1));
+            mbar_arrive_expect_tx_p(leader, bar, have * (uint32_t)at.box * (2 * D));
+#pragma unroll 1
+            for (int tile = 0; tile < 2; ++tile) {
+              const uint32_t to = smem_u32(base + (st * 2 + tile) * Sh::kTileBytes);
+#pragma unroll 1
+              for (int x0 = 0; x0 < at.parts; x0 += 8) {
+                int y[8];  // all rows first: a shuffle between two copies costs more than the copies
 #pragma unroll
-            for (int x = 0; x < 16; ++x) y0[x] = at.row(2 * w.c.tile, x & (at.parts - 1));
-            at.advance(2 * w.c.tile + 1);
-            const uint32_t have1 = at.have(2 * w.c.tile + 1);
-            mbar_arrive_expect_tx_p(leader, bar, (__popc(have0) + __popc(have1)) * (uint32_t)at.box * (2 * D));
-            const uint32_t to = smem_u32(base + st * 2 * Sh::kTileBytes);
+                for (int x = 0; x < 8; ++x) y[x] = at.row(2 * w.c.tile + tile, (x0 + x) & (at.parts - 1));
 #pragma unroll
-            for (int x = 0; x < 16; ++x)
-              tma_load_4d_p(x < at.parts && y0[x] >= 0 ? leader : 0u, to + x * at.box * (D * 2), &k_map, 0, 0, 0, y0[x] >> 3, bar);
-            int y1[16];
-#pragma unroll
-            for (int x = 0; x < 16; ++x) y1[x] = at.row(2 * w.c.tile + 1, x & (at.parts - 1));
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-              tma_load_4d_p(x < at.parts && y1[x] >= 0 ? leader : 0u, to + Sh::kTileBytes + x * at.box * (D * 2), &k_map, 0, 0, 0,
-                            y1[x] >> 3, bar);
+                for (int x = 0; x < 8; ++x)
+                  tma_load_4d_p(x0 + x < at.parts && y[x] >= 0 ? leader : 0u, to + (x0 + x) * at.box * (D * 2), &k_map, 0, 0, 0, y[x] >> 3, bar);
+              }
+            }
           }
         }
         if (!ok && lane == 0) give_up(C, p.err);
-        for (uint32_t i = unit > 2 ? unit - 2 : 0; i < unit; ++i)  // every copy issued has landed (bounded)
-          mbar_wait(smem_u32(&C.k_full[i & 1]), (i >> 1) & 1);
+        for (uint32_t i = unit > Sh::kK ? unit - Sh::kK : 0; i < unit; ++i)  // every copy issued has landed (bounded)
+          mbar_wait(smem_u32(&C.k_full[i % Sh::kK]), (i / Sh::kK) & 1);
       }
     } else if (warp == Ro::kLoadQ) {
       // ------------------------------------------------------------------ Q copies
@@ -200,13 +207,13 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         return ok;
       };
       for (; on && ok; on = w.next(mp), ++unit) {
-        if (!wait(&C.k_full[unit & 1], (unit >> 1) & 1)) break;
+        if (!wait(&C.k_full[unit % Sh::kK], (unit / Sh::kK) & 1)) break;
         for (int s = w.c.s0; s < w.c.s1 && ok; ++s, ++q) {
           const int st = q % Sh::kQ, buf = q & 1;
           if (!wait(&C.q_full[st], (q / Sh::kQ) & 1)) break;
           for (int t = 0; t < 2; ++t) {
             if (!wait(&C.s_free[t][buf], ((q >> 1) & 1) ^ 1)) break;
-            const uint64_t kd = k_desc + ((unit & 1) * 2 + t) * (Sh::kTileBytes >> 4), qd = q_desc + st * (Sh::kTileBytes >> 4);
+            const uint64_t kd = k_desc + ((unit % Sh::kK) * 2 + t) * (Sh::kTileBytes >> 4), qd = q_desc + st * (Sh::kTileBytes >> 4);
 #pragma unroll
             for (int kb = 0; kb < D / 64; ++kb)
 #pragma unroll
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
           }
           if (ok) umma_commit_p(leader, smem_u32(&C.q_empty[st]));
         }
-        if (ok) umma_commit_p(leader, smem_u32(&C.k_empty[unit & 1]));
+        if (ok) umma_commit_p(leader, smem_u32(&C.k_empty[unit % Sh::kK]));
       }
       if (!ok && lane == 0) give_up(C, p.err);
       // MMAs in flight end (bounded) before TMEM and shared memory go
@@ -229,21 +236,22 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       for (; on && ok; on = w.next(mp)) {
         for (int s = w.c.s0; s < w.c.s1; ++s, ++q) {
           const Step at(p, w.c, s);
-          float x[4];
+          const uint32_t bar = smem_u32(&C.x_full[q & 3]);
+          ok = __all_sync(0xffffffffu, role_wait(C.abort, smem_u32(&C.x_empty[q & 3]), ((q >> 2) & 1) ^ 1));
+          if (!ok) break;
+          // a step's rows lie side by side; they are copied, so that no step waits for the last one's
+          const float* from = row_stats(p, w.c.kvh, w.c.q_first + at.i0, at.head0 - w.c.kvh * p.group);
+          float* to = C.x[q & 3];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = lane + 32 * i, tok = p.by_gw.div(r), g = r - tok * p.gw;
-            x[i] = -INFINITY;
-            if (r < at.valid) {
-              const float2 st = p.stats[(int64_t)(w.c.q_first + at.i0 + tok) * p.n_q_heads + at.head0 + g];
-              x[i] = st.y == 0.f ? -INFINITY : log2f(st.y) - st.x;
-            }
+            const int r = lane + 32 * i;
+            if (r < at.valid)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to + r)), "l"(from + r) : "memory");
+            else
+              to[r] = -INFINITY;
           }
-          ok = __all_sync(0xffffffffu, role_wait(C.abort, smem_u32(&C.x_empty[q & 1]), ((q >> 1) & 1) ^ 1));
-          if (!ok) break;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) C.x[q & 1][lane + 32 * i] = x[i];
-          mbar_arrive(smem_u32(&C.x_full[q & 1]));
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+          mbar_arrive(bar);
         }
       }
       if (!ok && lane == 0) give_up(C, p.err);
@@ -252,8 +260,8 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
       const int ct = tid - Ro::kConvert * 32;
       uint32_t unit = 0;
       for (; on && ok; on = w.next(mp), ++unit) {
-        const int st = unit & 1;
-        ok = __all_sync(0xffffffffu, role_wait(C.abort, smem_u32(&C.k_empty[st]), ((unit >> 1) & 1) ^ 1));
+        const int st = unit % Sh::kK;
+        ok = __all_sync(0xffffffffu, role_wait(C.abort, smem_u32(&C.k_empty[st]), ((unit / Sh::kK) & 1) ^ 1));
         if (!ok) break;
         // D / 16 threads share a row, 16 codes each
         constexpr int kLanes = D / 16, kPass = 128 / kLanes;
@@ -289,13 +297,16 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
   } else {
     // ------------------------------------------------------------------ weights: thread = key
     const int t = warp >> 2, key = tid & 127;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t from0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * 2 * kRowsStep;
     const float c2 = p.scale * kLog2e;
     uint32_t q = 0;
-    for (; on && ok; on = w.next(mp)) {
-      const MassPiece& c = w.c;
-      int pos = 0;
-      const int64_t row = mass_row(p, w.kr, c.b, c.kvh, c.tile, t * kTile + key, &pos);
+    // the pool row of the thread's key is looked up a unit ahead
+    int pos_next = 0;
+    int64_t row_next = on ? mass_row(p, w.kr, w.c.b, w.c.kvh, w.c.tile, t * kTile + key, &pos_next) : -1;
+    while (on && ok) {
+      const MassPiece c = w.c;
+      const int pos = pos_next, pos0 = w.kr.pos0;
+      const int64_t row = row_next;
       float f = c2, old = 0.f;
       if (row >= 0) {
         if constexpr (kQuant) {
@@ -304,59 +315,90 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         }
         if (c.whole()) old = mp.mass[row];
       }
+      on = w.next(mp);
+      if (on) row_next = mass_row(p, w.kr, w.c.b, w.c.kvh, w.c.tile, t * kTile + key, &pos_next);
+      // steps whose rows all see all of the warp's keys: first tokens from `from_i0` to `to_i0` (keys that are none do
+      // not matter, nor do rows past the last token of a step: their x is -infinity)
+      const int far = 1 << 30;
+      const int from_i0 = __reduce_max_sync(0xffffffffu, row >= 0 ? pos - pos0 : -far);
+      const int to_i0 = min(c.n - p.tokens, __reduce_min_sync(0xffffffffu, row >= 0 && p.window > 0 && pos >= p.sinks
+                                                                               ? (int)min((long long)pos + p.window - p.tokens - pos0, (long long)far)
+                                                                               : far));
+      int i0 = c.r0 * p.tokens + (p.n_slices == 1 ? c.s0 * p.tokens : 0);
       float sum = 0.f;
-      for (int s = c.s0; s < c.s1; ++s, ++q) {
-        const Step at(p, c, s);
-        // the rows that see the key: tokens [pos - qpos0, pos + window - qpos0) of the step's
-        const int qpos0 = w.kr.pos0 + at.i0;
-        int lo = 0, hi = 0;
-        if (row >= 0) {
-          lo = min(max(pos - qpos0, 0), kRowsStep) * p.gw;
-          hi = at.valid;
-          if (p.window > 0 && pos >= p.sinks)
-            hi = min(hi, (int)min(max((long long)pos + p.window - qpos0, 0ll), (long long)kRowsStep) * p.gw);
-        }
-        const bool any = __any_sync(0xffffffffu, lo < hi), all = __all_sync(0xffffffffu, lo == 0 && hi == kRowsStep);
-        ok = role_wait(C.abort, smem_u32(&C.x_full[q & 1]), (q >> 1) & 1) &&
+      for (int s = c.s0; s < c.s1; ++s, ++q, i0 += p.tokens) {
+        ok = role_wait(C.abort, smem_u32(&C.x_full[q & 3]), (q >> 2) & 1) &&
              role_wait(C.abort, smem_u32(&C.s_full[t][q & 1]), (q >> 1) & 1);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        if (any) {
-          const uint32_t from = tmem + lanes + (t * 2 + (q & 1)) * kRowsStep;
-          const float* xs = C.x[q & 1];
-          float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          const auto add32 = [&](int x0, uint32_t see, auto whole) {
-            float v[32];
-            tmem_ld32(from + x0, v);
-            tmem_wait_ld();
+        const uint32_t from = from0 + (q & 1) * kRowsStep;
+        const float* xs = C.x[q & 3];
+        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        if (i0 >= from_i0 && i0 <= to_i0 && p.n_slices == 1) {
+          float v[2][32];
+          tmem_ld32(from, v[0]);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float2 x = *reinterpret_cast<const float2*>(xs + x0 + i);
-              float2 a = fma2(make_float2(v[i], v[i + 1]), make_float2(f, f), x);
-              if constexpr (!decltype(whole)::value) {
+          for (int k = 0; k < kRowsStep / 32; ++k) {
+            float* u = v[k & 1];
+            tmem_wait_ld32(u);
+            if (k + 1 < kRowsStep / 32) {
+              tmem_ld32(from + 32 * (k + 1), v[(k + 1) & 1]);
+            } else {  // all scores have been read
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(&C.s_free[t][q & 1]));
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(xs + 32 * k + i);
+              float2 a = fma2(make_float2(u[i], u[i + 1]), make_float2(f, f), make_float2(x.x, x.y));
+              float2 b = fma2(make_float2(u[i + 2], u[i + 3]), make_float2(f, f), make_float2(x.z, x.w));
+              a = make_float2(ex2(a.x), ex2(a.y));
+              b = make_float2(ex2(b.x), ex2(b.y));
+              acc[0] = add2(acc[0], a);
+              acc[1] = add2(acc[1], b);
+            }
+          }
+        } else {
+          const Step at(p, c, s);
+          // the rows that see the key: tokens [pos - qpos0, pos + window - qpos0) of the step's
+          const int qpos0 = pos0 + at.i0;
+          int lo = 0, hi = 0;
+          if (row >= 0) {
+            lo = min(max(pos - qpos0, 0), kRowsStep) * p.gw;
+            hi = at.valid;
+            if (p.window > 0 && pos >= p.sinks)
+              hi = min(hi, (int)min(max((long long)pos + p.window - qpos0, 0ll), (long long)kRowsStep) * p.gw);
+          }
+          if (__any_sync(0xffffffffu, lo < hi)) {
+#pragma unroll 1
+            for (int x0 = 0; x0 < at.valid; x0 += 32) {
+              float v[32];
+              tmem_ld32(from + x0, v);
+              const uint32_t see = low_bits(hi - x0) & ~low_bits(lo - x0);
+              tmem_wait_ld32(v);
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const float2 x = *reinterpret_cast<const float2*>(xs + x0 + i);
+                float2 a = fma2(make_float2(v[i], v[i + 1]), make_float2(f, f), x);
                 if (!(see >> i & 1)) a.x = -INFINITY;
                 if (!(see >> (i + 1) & 1)) a.y = -INFINITY;
+                a.x = ex2(a.x);
+                a.y = ex2(a.y);
+                acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], a);
               }
-              a.x = ex2(a.x);
-              a.y = ex2(a.y);
-              acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], a);
             }
-          };
-          if (all) {
-#pragma unroll 1
-            for (int x0 = 0; x0 < kRowsStep; x0 += 32) add32(x0, ~0u, std::true_type());
-          } else {
-#pragma unroll 1
-            for (int x0 = 0; x0 < at.valid; x0 += 32) add32(x0, low_bits(hi - x0) & ~low_bits(lo - x0), std::false_type());
           }
-          sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&C.s_free[t][q & 1]));
         }
-        tc_fence_before();
-        mbar_arrive(smem_u32(&C.s_free[t][q & 1]));
-        mbar_arrive(smem_u32(&C.x_empty[q & 1]));
+        sum += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&C.x_empty[q & 3]));
       }
       if (!ok) break;
       if (!c.whole()) mp.part[mass_slot(c) * kUnit + t * kTile + key] = sum;

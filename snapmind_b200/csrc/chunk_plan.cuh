@@ -52,7 +52,7 @@ struct ChunkParams {
   int32_t n_odd;
   int32_t means;    // part_o holds a piece's weighted means of V (else its weighted sums)
   float* scores;    // [pool row][group] scores (log2 units) that a decode leaves for chunk_mass.cu, or NULL
-  float2* stats;    // [total_q][n_q_heads] reference (log2 units) and 1 / sum of every row's softmax, or NULL
+  float* stats;     // [n_kv_heads][total_q][group] -log2 of every row's softmax sum (of 2^score), or NULL
   int32_t* err;
 };
 
@@ -432,11 +432,12 @@ __device__ inline void write_piece_info(const ChunkParams& p, const PlanShared& 
   h[0] = c.b;
 }
 
-// A finished row's softmax, for the kernel that adds its weights to their keys (chunk_mass.cu): the weight of
-// a key is 2^(score - x) y.  A row that sees nothing: 0, 0.
+// A finished row's softmax (M, sum of 2^(score - M)), for the kernels that add its weights to their keys (chunk_mass.cu):
+// the weight of a key is 2^(score + x).  A row that sees nothing: -infinity.
 __device__ __forceinline__ void write_stats(const ChunkParams& p, int64_t row, int head, float M, float L) {
-  if (p.stats != nullptr)
-    p.stats[row * p.n_q_heads + head] = make_float2(M == -INFINITY ? 0.f : M, L == 0.f ? 0.f : 1.f / L);
+  if (p.stats == nullptr) return;
+  const int kvh = head / p.group;
+  p.stats[(kvh * (int64_t)p.total_q + row) * p.group + (head - kvh * p.group)] = L == 0.f ? -INFINITY : -((M == -INFINITY ? 0.f : M) + log2f(L));
 }
 
 // 2^x by the hardware approximation (2 ulp); -inf -> 0.
