@@ -27,6 +27,11 @@ with its own ``apply_to_qk``.  The projections and the output projection stay
 torch, as in the reference.  Without a cache (``kv_cache=None``) the layer
 attends causally over its own ``T`` tokens through a transient one-layer pool.
 
+With ``qk_norm_eps`` the layer has ``q_norm`` and ``k_norm`` (``nn.RMSNorm`` over a head's dims, which the reference
+layer has not): queries and keys are normalised per head before they turn, in the same kernel, and over a
+``PagedKVPool`` stored by it too (``append_rope``).  Over a pool with ``mass=True`` every query's weights are
+accumulated for ``PagedKVPool.evict``.
+
 Differences a caller can see: the attention weights are not materialised (the
 second output is ``None``); ``mask`` must be ``None`` or the causal mask of
 snapmind/layers/attention/sdpa.py ``create_causal_mask`` (what the reference
@@ -85,6 +90,7 @@ class PagedGroupedQueryAttention(_AttentionBase):
         bias: bool = False,
         pe: nn.Module | None = None,
         head_dim: int | None = None,
+        qk_norm_eps: float | None = None,
     ):
         super().__init__()
         if head_dim is None:
@@ -101,6 +107,9 @@ class PagedGroupedQueryAttention(_AttentionBase):
         self.k_proj = nn.Linear(d_model, self.n_kv_heads * self.head_dim, bias=bias)
         self.v_proj = nn.Linear(d_model, self.n_kv_heads * self.head_dim, bias=bias)
         self.out_proj = nn.Linear(n_heads * self.head_dim, d_model, bias=bias)
+        self.q_norm = self.k_norm = None
+        if qk_norm_eps is not None:
+            self.q_norm, self.k_norm = (nn.RMSNorm(self.head_dim, eps=qk_norm_eps) for _ in range(2))
 
     def _split_heads(self, x: torch.Tensor, n_heads: int) -> torch.Tensor:
         batch, seq_len, _ = x.shape
@@ -122,17 +131,45 @@ class PagedGroupedQueryAttention(_AttentionBase):
             sin = sin.float().contiguous()
         return cos, sin
 
+    def _positions(self, position_ids, batch: int, n_tok: int, device):
+        """(positions or None, elements between two sequences' lists)."""
+        if position_ids is None:
+            return None, 0
+        pos, stride = position_ids.reshape(-1), 0
+        if pos.numel() == batch * n_tok and batch > 1:
+            stride = n_tok  # one position list per sequence
+        elif pos.numel() != n_tok:
+            raise ValueError(f"gqa_paged: {pos.numel()} positions for {batch} x {n_tok} tokens")
+        return pos.to(device=device, dtype=torch.int64).contiguous(), stride
+
+    def _place(self, q, k, position_ids, err: torch.Tensor):
+        """Norm (with ``qk_norm_eps``) and rotate fresh projections ``[B, heads, T, D]``: by one kernel, in place, where
+        ``pe`` has the tables that it takes, else by the modules."""
+        tables = self._rope_tables(q) if self.pe is not None else None
+        if tables is not None:
+            (self._rope if self.q_norm is None else self._norm_rope)(q, k, position_ids, tables, err)
+            return q, k
+        if self.q_norm is not None:
+            q, k = self.q_norm(q), self.k_norm(k)
+        return (q, k) if self.pe is None else self.pe.apply_to_qk(q, k, position_ids)
+
+    def _norm_rope(self, q, k, position_ids, tables, err: torch.Tensor) -> None:
+        cos, sin = tables
+        pos, pos_stride = self._positions(position_ids, q.shape[0], q.shape[2], q.device)
+        rot, _, _ = _lib.rope_args("gqa_paged", q, cos, sin, self.q_norm.weight, self.k_norm.weight, self.n_heads,
+                                   self.n_kv_heads, self.q_norm.eps)
+        qk = [(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2)) for x in (q, k)]
+        status = _lib.load().snapmind_norm_rope_qk(
+            *qk[0], *qk[0], q.shape[1], *qk[1], *qk[1], k.shape[1], _lib.dtype_code(q.dtype), self.q_norm.weight.data_ptr(), 0,
+            self.k_norm.weight.data_ptr(), 0, self.q_norm.eps, q.shape[0], q.shape[2], self.head_dim, cos.data_ptr(),
+            sin.data_ptr(), rot, cos.shape[0], _lib.ptr(pos), pos_stride, err.data_ptr(), _lib.stream_handle(q.device),
+        )  # fmt: skip
+        _lib.check(status, "gqa_paged norm and rope")
+
     def _rope(self, q, k, position_ids, tables, err: torch.Tensor) -> None:
         cos, sin = tables
-        batch, n_tok = q.shape[0], q.shape[2]
-        pos, pos_stride = None, 0
-        if position_ids is not None:
-            pos = position_ids.reshape(-1)
-            if pos.numel() == batch * n_tok and batch > 1:
-                pos_stride = n_tok  # one position list per sequence
-            elif pos.numel() != n_tok:
-                raise ValueError(f"gqa_paged: {pos.numel()} positions for {batch} x {n_tok} tokens")
-            pos = pos.to(device=q.device, dtype=torch.int64).contiguous()
+        n_tok = q.shape[2]
+        pos, pos_stride = self._positions(position_ids, q.shape[0], n_tok, q.device)
         status = _lib.load().snapmind_rope_qk(
             q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), q.shape[1],
             k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), k.shape[1],
@@ -175,12 +212,7 @@ class PagedGroupedQueryAttention(_AttentionBase):
                 f"gqa_paged: cache holds {cache.n_heads} heads x {cache.head_dim}, "
                 f"layer needs {self.n_kv_heads} x {self.head_dim}"
             )
-        if self.pe is not None:
-            tables = self._rope_tables(q)
-            if tables is not None:
-                self._rope(q, k, position_ids, tables, cache._err)  # in place on the fresh projections
-            else:
-                q, k = self.pe.apply_to_qk(q, k, position_ids)
+        q, k = self._place(q, k, position_ids, cache._err)  # in place on the fresh projections
         if cache.device_steps_active:  # one token at the device counters (a captured decode step)
             if n_new != 1 or mask is not None:
                 raise ValueError("gqa_paged: device steps take one token and no mask")
@@ -216,25 +248,43 @@ class PagedGroupedQueryAttention(_AttentionBase):
         q = self._split_heads(self.q_proj(x), self.n_heads)
         k = self._split_heads(self.k_proj(x), self.n_kv_heads)
         v = self._split_heads(self.v_proj(x), self.n_kv_heads)
-        if self.pe is not None:
-            tables = self._rope_tables(q)
-            if tables is not None:
-                self._rope(q, k, position_ids, tables, pool.err)
-            else:
-                q, k = self.pe.apply_to_qk(q, k, position_ids)
-        qd = q if q.dtype == pool.dtype else q.to(pool.dtype)
         if n_new == 1:
             if mask is not None:
                 raise ValueError("gqa_paged: a decode step takes no mask")
-            pool.append(layer, k[:, :, 0], v[:, :, 0])
-            out = pool.decode(layer, qd[:, :, 0], max_seq_len=view.capacity)
-            out = out.to(x.dtype).reshape(batch, 1, self.n_heads * self.head_dim)
         else:
             if view.stored and mask is None:
                 raise ValueError("gqa_paged: pool views take multi-token steps as causal prefill only")
             if mask is not None and not _is_causal_mask(mask, n_new, n_new):
                 raise ValueError("gqa_paged supports no mask or the causal mask only")
-            pool.append(layer, k, v)
+        # a pool with mass: the weights of every query count towards evictions
+        weighs = pool.mass is not None
+        cu = None
+        if n_new > 1 and (weighs or self.q_norm is not None):
+            cu = torch.arange(0, (batch + 1) * n_new, n_new, dtype=torch.int32, device=x.device)
+        tables = self._rope_tables(q) if self.pe is not None and self.q_norm is not None else None
+        if tables is not None:  # norm, rotation and store in one pass
+            pos, stride = self._positions(position_ids, batch, n_new, x.device)
+            if pos is None:
+                pos = torch.arange(n_new, device=x.device)
+            pos = pos if stride or batch == 1 else pos.repeat(batch)
+            rows = [t.transpose(1, 2).reshape(batch * n_new, -1, self.head_dim) for t in (q, k, v)]
+            rows[0] = pool.append_rope(layer, *rows, *tables, pos, cu_new=cu, q_norm=self.q_norm.weight.detach(),
+                                       k_norm=self.k_norm.weight.detach(), eps=self.q_norm.eps)
+            q = rows[0].view(batch, n_new, self.n_heads, self.head_dim).transpose(1, 2)
+        else:
+            q, k = self._place(q, k, position_ids, pool.err)
+            if n_new == 1:
+                pool.append(layer, k[:, :, 0], v[:, :, 0])
+            else:
+                pool.append(layer, k, v)
+        qd = q if q.dtype == pool.dtype else q.to(pool.dtype)
+        if n_new == 1:
+            out = pool.decode(layer, qd[:, :, 0], max_seq_len=view.capacity, accumulate=weighs)
+            out = out.to(x.dtype).reshape(batch, 1, self.n_heads * self.head_dim)
+        elif weighs:
+            out = pool.attend_chunk(layer, qd.transpose(1, 2).reshape(batch * n_new, self.n_heads, self.head_dim), cu, accumulate=True)
+            out = out.to(x.dtype).reshape(batch, n_new, self.n_heads * self.head_dim)
+        else:
             out = torch.empty((batch, self.n_heads, n_new, self.head_dim), dtype=pool.dtype, device=x.device)
             lens = pool.host_lens
             for b in range(batch):
@@ -259,12 +309,7 @@ class PagedGroupedQueryAttention(_AttentionBase):
         v = self._split_heads(self.v_proj(x), self.n_kv_heads)
         if cache.n_heads != self.n_kv_heads or cache.head_dim != self.head_dim:
             raise ValueError("gqa_paged: cache heads / head_dim do not match the layer")
-        if self.pe is not None:
-            tables = self._rope_tables(q)
-            if tables is not None:
-                self._rope(q, k, position_ids, tables, cache._err)
-            else:
-                q, k = self.pe.apply_to_qk(q, k, position_ids)
+        q, k = self._place(q, k, position_ids, cache._err)
         w, n_new, n_old = cache.window_size, x.shape[1], cache.num_tokens(layer)
         if mask is not None:
             if n_old:

@@ -23,7 +23,10 @@ The generated ids equal an eager run's; the cache ends in the same state.
 one sequence): B prompts of one length are prefilled into a ``PagedKVPool``,
 then every decode step grows all B sequences on the device
 (``snapmind_kv_reserve``), appends their K/V rows and runs one batched paged
-decode per layer — captured once and replayed, like ``GraphDecoder``.
+decode per layer — captured once and replayed, like ``GraphDecoder``.  With a ``budget`` (over a
+pool with ``mass=True``) the sequences stay bounded: whenever they hold ``slack`` tokens more, the
+ones with the least accumulated attention weight are evicted between two replays
+(``PagedKVPool.evict``); positions run on.
 """
 from __future__ import annotations
 
@@ -115,8 +118,14 @@ class GraphDecoder:
 
 
 class BatchedGraphDecoder:
-    def __init__(self, model: torch.nn.Module, pool: PagedKVPool, batch: int, use_graph: bool = True):
+    def __init__(self, model: torch.nn.Module, pool: PagedKVPool, batch: int, use_graph: bool = True,
+                 budget: int | None = None, slack: int = 64, recent: int = 0, sinks: int = 0):
+        """``budget``: tokens that a sequence is thinned to once it holds ``budget + slack`` (its prompt right away);
+        ``recent`` and ``sinks`` of them are the newest and the first, whatever they weigh."""
+        if budget is not None and (pool.mass is None or slack < 1):
+            raise ValueError("BatchedGraphDecoder: a budget needs a pool with mass=True and a slack of at least 1")
         self.model, self.pool, self.batch, self.use_graph = model, pool, batch, use_graph
+        self.budget, self.slack, self.recent, self.sinks = budget, slack, recent, sinks
         self.views = pool.layer_views(batch)
         self._graph: torch.cuda.CUDAGraph | None = None
         self._steps_left = 0
@@ -133,13 +142,20 @@ class BatchedGraphDecoder:
         logits = self.model(prompts.to(dev), kv_cache=self.views)[:, -1]
         self.tok = logits.argmax(-1).reshape(b, 1).clone()
         self.pos = torch.full((b,), t, dtype=torch.long, device=dev)
+        if self.budget is not None:
+            self._evict()
+
+    def _evict(self) -> None:
+        self.pool.evict(self.budget, recent=self.recent, sinks=self.sinks, batch=self.batch)
 
     @torch.no_grad()
     def begin(self, n_steps: int) -> None:
         pool, b = self.pool, self.batch
-        if pool.blocks_needed(n_steps, b) > pool._host_free:
+        # tokens that a sequence grows by before it is thinned again
+        grows = n_steps if self.budget is None else min(n_steps, max(0, self.budget + self.slack - int(pool.host_lens[:b].min())))
+        if pool.blocks_needed(grows, b) > pool._host_free:
             raise RuntimeError("PagedKVCache: out of blocks")
-        cap = int(pool.host_lens[:b].max()) + n_steps
+        cap = int(pool.host_lens[:b].max()) + grows
         if (cap + pool.block_size - 1) // pool.block_size > pool.max_blocks_per_seq:
             raise ValueError("BatchedGraphDecoder: sequences would outgrow their block table rows")
         for view in self.views.values():
@@ -148,6 +164,7 @@ class BatchedGraphDecoder:
         self.ids[0] = self.tok.reshape(b)
         self.idx = torch.ones((1,), dtype=torch.long, device=pool.device)
         self._steps_total = self._steps_left = n_steps
+        self._unaccounted = 0  # steps that the pool's host mirrors do not know of
         self._graph = None
 
     def _step(self) -> None:
@@ -179,6 +196,14 @@ class BatchedGraphDecoder:
             else:
                 self._step()
             self._steps_left -= 1
+            self._unaccounted += 1
+            if self.budget is not None and int(self.pool.host_lens[:self.batch].max()) + self._unaccounted >= self.budget + self.slack:
+                self._account()
+                self._evict()
+
+    def _account(self) -> None:
+        self.pool.account_host(self._unaccounted, self.batch)
+        self._unaccounted = 0
 
     @torch.no_grad()
     def finish(self) -> list[list[int]]:
@@ -186,7 +211,7 @@ class BatchedGraphDecoder:
         if self._steps_left:
             raise RuntimeError(f"BatchedGraphDecoder: {self._steps_left} decode steps not run")
         self._graph = None
-        self.pool.account_host(self._steps_total, self.batch)
+        self._account()
         for view in self.views.values():
             view.capacity = None
         self.pool.check()
