@@ -275,24 +275,24 @@ def rope_args(what: str, q: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
               eps: float) -> tuple[int, int, int]:
     """Check the tables and norms of a norm-and-rotate call on ``q`` ``[..., D]``; returns the rotated dims and the strides
     between the heads' norms of q and k."""
-    d = q.shape[-1]
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    d, dtype, c = q.shape[-1], q.dtype, cos.shape
+    if len(c) != 2 or c != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError(f"{what}: cos and sin must be f32 [n_pos, rotated dims] alike")
-    if not (cos.is_contiguous() and sin.is_contiguous()) or cos.shape[0] < 1 or cos.shape[1] % 2 or cos.shape[1] > d:
+    if not (cos.is_contiguous() and sin.is_contiguous()) or c[0] < 1 or c[1] % 2 or c[1] > d:
         raise ValueError(f"{what}: cos and sin must be contiguous, an even number of dims, at most {d}")
     if not eps >= 0.0:
         raise ValueError(f"{what}: eps must not be negative")
-    strides = []
-    for w, heads in ((q_norm, n_q), (k_norm, n_kv)):
-        strides.append(0)
+    strides = [0, 0]
+    for i, w in enumerate((q_norm, k_norm)):
         if w is None:
             continue
-        if w.shape not in ((d,), (heads, d)) or w.dtype != q.dtype or w.stride(-1) != 1:
+        st, shape = w.stride(), w.shape
+        if shape != (d,) and shape != ((n_kv if i else n_q), d) or w.dtype != dtype or st[-1] != 1:
             raise ValueError(f"{what}: norms must be [{d}] or [heads, {d}] in q's dtype, dims contiguous")
         require_same(what, q, w)
-        if w.dim() == 2:
-            strides[-1] = w.stride(0)
-    return cos.shape[1], strides[0], strides[1]
+        if len(st) == 2:
+            strides[i] = st[0]
+    return c[1], strides[0], strides[1]
 
 
 def raise_device_error(word: int, what: str) -> None:

@@ -63,11 +63,13 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 
 // Selection: a block per (layer, sequence, head).  The weights lie in shared memory (a chunk of them when there
-// are more), warp w holding run w of the chunk's indexes; the order of the last that stays is found 11 bits at a time
-// from histograms, and the kept indexes are counted per warp by ballots and written out in a second sweep.  What
+// are more), warp w holding run w of the chunk's indexes; the order of the last that stays is found from a histogram
+// of the highest 11 bits, counted as the weights come in, and then among the few of its bin (or 11 bits at a time, if
+// they are not few), and the kept indexes are counted per warp by ballots and written out in a second sweep.  What
 // bounds it is latency (a read of the table, one of the weights, a handful of barriers), so blocks are small
 // where sequences are short, several to an SM.
 constexpr int kRadix = 11, kBins = 1 << kRadix;
+constexpr int kFew = 256;  // that many are listed and compared with one another (800 took 25 us more than another histogram)
 
 template <int THREADS>
 struct SelectSmem {
@@ -75,7 +77,8 @@ struct SelectSmem {
   int32_t above[THREADS / 32], equal[THREADS / 32];
   uint32_t prefix;  // of the lowest kept order
   int32_t need;     // how many with exactly that order stay
-  int32_t total;
+  int32_t there;    // indexes in the prefix's bin
+  int32_t listed;
 };
 
 template <int THREADS>
@@ -107,7 +110,13 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
   }
   // what stays in any case takes no part: [0, lo) and [hi, len)
   const int lo = min(p.sinks, keep), hi = len - min(p.recent, keep - lo);
-  // weights [c0, c0 + chunk) into shared memory; an index without a block: -infinity
+  const bool one = len <= chunk;
+  int need = keep - lo - (len - hi);  // of [lo, hi)
+  const bool none = need <= 0;
+  const auto count = [&](int x, float m) {  // the first histogram: the highest bits
+    if (x >= lo && x < hi) atomicAdd(&S.bins[order_of(m) >> (32 - kRadix)], 1);
+  };
+  // weights [c0, c0 + chunk) into shared memory (an index without a block: -infinity), counted on the way if all fit
   const auto load = [&](int c0) {
     const int n = min(chunk, len - c0);
     if ((p.block_size & 3) == 0) {
@@ -125,27 +134,33 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
         }
 #pragma unroll
         for (int y = 0; y < kDeep; ++y)
-          if (x0 + y * 4 * THREADS < n) *reinterpret_cast<float4*>(held + x0 + y * 4 * THREADS) = v[y];
+          if (x0 + y * 4 * THREADS < n) {
+            const int x = x0 + y * 4 * THREADS;
+            *reinterpret_cast<float4*>(held + x) = v[y];
+            if (one && !none) count(x, v[y].x), count(x + 1, v[y].y), count(x + 2, v[y].z), count(x + 3, v[y].w);
+          }
       }
     } else {
       for (int x = tid; x < n; x += THREADS) {
         const int64_t row = row_of(p, table, head, c0 + x);
         held[x] = row < 0 ? -INFINITY : mass[row];
+        if (one && !none) count(x, held[x]);
       }
     }
   };
-  const bool one = len <= chunk;
+  for (int x = tid; x < kBins; x += THREADS) S.bins[x] = 0;
+  __syncthreads();
   if (one) load(0);
-  int need = keep - lo - (len - hi);  // of [lo, hi)
-  const bool none = need <= 0;
   uint32_t prefix = 0;
   int shift = 32;
   // the order of the need-th largest, 11, 11 and 10 bits at a time
   for (int pass = 0; pass < 3 && !none; ++pass) {
     const int bits = pass < 2 ? kRadix : 32 - 2 * kRadix;
-    for (int x = tid; x < kBins; x += THREADS) S.bins[x] = 0;
-    __syncthreads();
-    for (int c0 = 0; c0 < len; c0 += chunk) {
+    if (pass > 0) {
+      for (int x = tid; x < kBins; x += THREADS) S.bins[x] = 0;
+      __syncthreads();
+    }
+    for (int c0 = 0; c0 < len && !(one && pass == 0); c0 += chunk) {
       if (!one) {
         __syncthreads();
         load(c0);
@@ -181,6 +196,8 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
       if (before < need && before + mine[y] >= need) {
         S.prefix = prefix | (uint32_t)(kBins - 1 - (tid * kPer + y)) << (shift - bits);
         S.need = need - before;
+        S.there = mine[y];
+        S.listed = 0;
       }
       before += mine[y];
     }
@@ -188,6 +205,33 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     prefix = S.prefix;
     need = S.need;
     shift -= bits;
+    const int there = S.there;
+    if (one && shift > 0 && there <= kFew) {
+      // listed where the bins were, which all have read; each counts those above it
+      uint32_t* list = reinterpret_cast<uint32_t*>(S.bins);
+      for (int x = lo + tid; x < hi; x += THREADS) {
+        const uint32_t k = order_of(held[x]);
+        if (k >> shift == prefix >> shift) list[atomicAdd(&S.listed, 1)] = k;
+      }
+      __syncthreads();
+      if (tid < there) {
+        const uint32_t k = list[tid];
+        int above = 0, same = 0;
+        for (int j = 0; j < there; ++j) {
+          const uint32_t other = list[j];
+          above += other > k;
+          same += other == k;
+        }
+        if (above < need && above + same >= need) {  // (its equals write the same)
+          S.prefix = k;
+          S.need = need - above;
+        }
+      }
+      __syncthreads();
+      prefix = S.prefix;
+      need = S.need;
+      break;
+    }
   }
   // in ascending order: what is above the border stays, of those on it the first `need`.  A chunk is read whole
   // before its kept weights are written, which is never past its own end.
@@ -473,7 +517,7 @@ int snapmind_kv_evict_by_mass(void* k_pool, void* v_pool, void* scales, int pool
   p.err = err_word;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (into) evict_tables_kernel<<<1, kTableThreads, 0, st>>>(p);
-  // Sequences of up to 4096 tokens: 256 threads (8 blocks an SM), up to 16384: 512, above: 1024, each with room for
+  // Sequences of up to 4096 tokens: 256 threads (4 blocks an SM), up to 16384: 512, above: 1024, each with room for
   // that many weights (above: 49152 at a time).
   const int64_t room = (int64_t)table_width * block_size, longest = max_len > 0 && max_len < room ? max_len : room;
   const auto select = [&](auto kernel, int threads, bool (&done)[64]) -> cudaError_t {
@@ -483,6 +527,8 @@ int snapmind_kv_evict_by_mass(void* k_pool, void* v_pool, void* scales, int pool
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev >= 64 || !done[dev])) {
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 49152 * 4);
+      if (e == cudaSuccess)  // room for the blocks that are meant to share an SM
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
       if (e == cudaSuccess && dev < 64) done[dev] = true;
     }
     if (e == cudaSuccess) kernel<<<(uint32_t)units, threads, chunk * 4, st>>>(p, chunk);

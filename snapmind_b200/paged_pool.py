@@ -128,36 +128,45 @@ class PagedKVPool(BlockPool):
         if d != self.head_dim or k.shape != want or v.shape != want:
             raise ValueError(f"append_rope: expected q [total, heads, {self.head_dim}] and k, v {list(want)}, got "
                              f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
-        if k.dtype != q.dtype or v.dtype != q.dtype:
+        dtype = q.dtype
+        if k.dtype != dtype or v.dtype != dtype:
             raise TypeError("append_rope: q, k and v differ in dtype")
         if not 0 <= layer < self.n_layers:
             raise ValueError(f"layer {layer} of a pool of {self.n_layers}")
+        batch, cu = total, None
         if cu_new is not None:
             _lib.require_offsets("append_rope", cu_new, self.block_tables)
-        batch = total if cu_new is None else cu_new.shape[0] - 1
+            batch, cu = cu_new.shape[0] - 1, cu_new.data_ptr()
         if batch > self.max_seqs:
             raise ValueError(f"append_rope: {batch} sequences, the pool holds {self.max_seqs}")
         if positions.dtype != torch.int64 or positions.shape != (total,):
             raise ValueError(f"append_rope: positions must be int64 [{total}]")
+        q_st, k_st, v_st = q.stride(), k.stride(), v.stride()
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
-            raise ValueError("append_rope: out must have q's shape and dtype, head dim contiguous")
+            o_st = out.stride()
+        else:
+            o_st = out.stride()
+            if out.shape != q.shape or out.dtype != dtype or o_st[2] != 1:
+                raise ValueError("append_rope: out must have q's shape and dtype, head dim contiguous")
         _lib.require_same("append_rope", self.block_tables, q, k, v, cos, sin, positions, out)
-        rot, q_st, k_st = _lib.rope_args("append_rope", q, cos, sin, q_norm, k_norm, n_q, self.n_kv_heads, eps)
-        q, k, v = (x if x.stride(2) == 1 else x.contiguous() for x in (q, k, v))
-        if total > 1 and not positions.is_contiguous():
+        rot, qn_st, kn_st = _lib.rope_args("append_rope", q, cos, sin, q_norm, k_norm, n_q, self.n_kv_heads, eps)
+        if q_st[2] != 1 or k_st[2] != 1 or v_st[2] != 1:
+            q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+            q_st, k_st, v_st = q.stride(), k.stride(), v.stride()
+        if total > 1 and positions.stride(0) != 1:
             positions = positions.contiguous()
         step = layer * self.layer_stride * self.k.element_size()
+        tables = self.block_tables.data_ptr()
         with self._on_device():
             status = _lib.load().snapmind_norm_rope_append(
-                q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), n_q,
-                k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _lib.dtype_code(q.dtype),
-                _lib.ptr(q_norm), q_st, _lib.ptr(k_norm), k_st, eps, cos.data_ptr(), sin.data_ptr(), rot, cos.shape[0],
+                q.data_ptr(), q_st[0], q_st[1], out.data_ptr(), o_st[0], o_st[1], n_q,
+                k.data_ptr(), k_st[0], k_st[1], v.data_ptr(), v_st[0], v_st[1], _lib.dtype_code(dtype),
+                _lib.ptr(q_norm), qn_st, _lib.ptr(k_norm), kn_st, eps, cos.data_ptr(), sin.data_ptr(), rot, cos.shape[0],
                 positions.data_ptr(), self.k.data_ptr() + step, self.v.data_ptr() + step,
                 self.scales.data_ptr() + layer * self.scale_layer_stride if self.quantised else None, self._pool_code,
-                self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq, self.seq_lens.data_ptr(),
-                _lib.ptr(cu_new), batch, total, self.n_kv_heads, d, self.block_size, self.num_blocks, self.err.data_ptr(),
+                tables, self.max_blocks_per_seq, self.max_blocks_per_seq, self.seq_lens.data_ptr(),
+                cu, batch, total, self.n_kv_heads, d, self.block_size, self.num_blocks, self.err.data_ptr(),
                 _lib.raw_stream(self._index),
             )  # fmt: skip
         if status:
