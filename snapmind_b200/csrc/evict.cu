@@ -69,11 +69,12 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 // bounds it is latency (a read of the table, one of the weights, a handful of barriers), so blocks are small
 // where sequences are short, several to an SM.
 constexpr int kRadix = 11, kBins = 1 << kRadix;
+static_assert(2 * 49152 / 32 <= kBins + 1024, "bits of a chunk");
 constexpr int kFew = 256;  // that many are listed and compared with one another (800 took 25 us more than another histogram)
 
 template <int THREADS>
 struct SelectSmem {
-  int32_t bins[kBins];
+  int32_t bins[kBins + 1024];  // later two words of bits for every 32 indexes of a chunk
   int32_t above[THREADS / 32], equal[THREADS / 32];
   uint32_t prefix;  // of the lowest kept order
   int32_t need;     // how many with exactly that order stay
@@ -190,7 +191,12 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     if (lane == 31) S.above[warp] = incl;
     __syncthreads();
     int before = incl - sum;
-    for (int w = 0; w < warp; ++w) before += S.above[w];
+    {
+      int x = lane < warp ? S.above[lane] : 0;  // 32 warps at most
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      before += x;
+    }
 #pragma unroll
     for (int y = 0; y < kPer; ++y) {
       if (before < need && before + mine[y] >= need) {
@@ -243,21 +249,23 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
       load(c0);
     }
     __syncthreads();
-    const int run = (n + 32 * kWarps - 1) / (32 * kWarps) * 32, x0 = min(n, warp * run), x1 = min(n, x0 + run);
-    // bits of the lane's index: 1 it stays, 2 it is on the border
-    const auto sort = [&](int x) {
-      if (x >= x1) return 0;
-      const int j = c0 + x;
-      if (j < lo || j >= hi) return 1;
-      if (none) return 0;
-      const uint32_t k = order_of(held[x]);
-      return k > prefix ? 1 : k == prefix ? 2 : 0;
-    };
+    const int run = (n + 32 * kWarps - 1) / (32 * kWarps) * 32, x0 = min(n, warp * run), x1 = min(n, x0 + run);  // x0 of a run with an index is a multiple of 32
+    // 32 indexes' bits: those that stay, those on the border
+    uint2* bits = reinterpret_cast<uint2*>(S.bins);
     int above = 0, on = 0;
     for (int x = x0; x < x1; x += 32) {
-      const int k = sort(x + lane);
-      above += __popc(__ballot_sync(0xffffffffu, k == 1));
-      on += __popc(__ballot_sync(0xffffffffu, k == 2));
+      const int j = c0 + x + lane;
+      bool sure = j < lo || j >= hi, border = false;
+      if (!sure && !none) {
+        const uint32_t k = order_of(held[min(x + lane, x1 - 1)]);
+        sure = k > prefix;
+        border = k == prefix;
+      }
+      const bool there = x + lane < x1;
+      const uint32_t a = __ballot_sync(0xffffffffu, there && sure), e = __ballot_sync(0xffffffffu, there && border);
+      if (lane == 0) bits[x >> 5] = make_uint2(a, e);
+      above += __popc(a);
+      on += __popc(e);
     }
     if (lane == 0) {
       S.above[warp] = above;
@@ -274,11 +282,11 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
       all_at += k;
       all_equal += e;
     }
+    const uint32_t below = (1u << lane) - 1u;
     for (int x = x0; x < x1; x += 32) {
-      const int k = sort(x + lane);
-      const uint32_t border = __ballot_sync(0xffffffffu, k == 2), below = (1u << lane) - 1u;
-      const bool stays = k == 1 || (k == 2 && mine_equal + __popc(border & below) < need);
-      const uint32_t those = __ballot_sync(0xffffffffu, stays);
+      const uint2 m = bits[x >> 5];
+      const bool stays = (m.x >> lane & 1) || ((m.y >> lane & 1) && mine_equal + __popc(m.y & below) < need);
+      const uint32_t those = m.y == 0 ? m.x : __ballot_sync(0xffffffffu, stays);
       if (stays) {
         const int place = mine_at + __popc(those & below);
         kept[place] = c0 + x + lane;
@@ -286,7 +294,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
         if (b >= 0) mass[b] = held[x + lane];
       }
       mine_at += __popc(those);
-      mine_equal += __popc(border);
+      mine_equal += __popc(m.y);
     }
     at = all_at;
     equal = all_equal;
