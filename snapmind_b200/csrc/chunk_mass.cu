@@ -204,10 +204,13 @@ int launch_generic(MassParams& mp, cudaStream_t st) {
   return go(mass_generic_kernel<T, KV, 4>, sizeof(MassSmem<4>), MassSmem<4>::kCtas, done[2]);
 }
 
-// Behind a decode that left its scores (decode_sinks.cu): the same CTAs on the same shares of the key line, a thread
-// a key.  HBM bound: 4 bytes a query head and 8 of mass for each key and kv head, against the 512 of a 16-bit row of
-// K and V that the decode read (scores taken from K anew would read half of those again).
-constexpr int kScoreThreads = 512, kScoreDeep = 2;
+// Behind a decode that left its scores (decode_sinks.cu): the same CTAs on the same shares of the key line, four keys of
+// a block a thread.  HBM bound: 4 bytes a query head and 8 of mass for each key and kv head, against the 512 of a
+// 16-bit row of K and V that the decode read (scores taken from K anew would read half of those again).  A thread a key
+// took 31 us beside the 440 of a decode of 128 sequences of 1 to 8 thousand tokens (32 heads over 8 of 128), this 25.  Tried and
+// dropped: the merge of the output beside this kernel instead of before it, every warp putting a cut unit's sums
+// together for itself (one sequence of 32768: 48 us, 43 without).
+constexpr int kScoreThreads = 512;
 template <int G>
 __global__ void __launch_bounds__(kScoreThreads, 2) mass_scores_kernel(const __grid_constant__ ChunkParams p, float* mass) {
   extern __shared__ int32_t tiles[];
@@ -229,38 +232,37 @@ __global__ void __launch_bounds__(kScoreThreads, 2) mass_scores_kernel(const __g
     }
     const int32_t* table = p.tables + (int64_t)c.b * p.table_stride;
     const int v1 = min(c.tile1 * p.key_tile, kr.v_len), q = kr.pos0;
-    for (int v0 = c.tile0 * p.key_tile + threadIdx.x; v0 < v1; v0 += kScoreThreads * kScoreDeep) {
-      int64_t row[kScoreDeep];
-      float m[kScoreDeep], s[kScoreDeep][G > 0 ? G : 1];
+    for (int v = c.tile0 * p.key_tile + 4 * threadIdx.x; v < v1; v += 4 * kScoreThreads) {
+      const int pos = kr.position(v), j = p.by_block.div(pos);  // blocks are a multiple of 16 tokens: four in one
+      const int32_t phys = table[j];
+      if (phys < 0 || phys >= p.num_blocks) continue;
+      const int64_t row = ((int64_t)phys * p.n_kv_heads + c.kvh) * p.block_size + (pos - j * p.block_size);
+      float4* at = reinterpret_cast<float4*>(mass + row);
+      const float* from = p.scores + row * group;
+      float4 m = *at;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (G > 0) {
+        float s[4 * G];
 #pragma unroll
-      for (int u = 0; u < kScoreDeep; ++u) {
-        const int v = v0 + u * kScoreThreads;
-        row[u] = -1;
-        if (v >= v1) continue;
-        const int pos = kr.position(v), j = p.by_block.div(pos);
-        const int32_t phys = table[j];
-        if (phys < 0 || phys >= p.num_blocks || (p.window > 0 && pos <= q - p.window && pos >= p.sinks)) continue;
-        row[u] = ((int64_t)phys * p.n_kv_heads + c.kvh) * p.block_size + (pos - j * p.block_size);
-        m[u] = mass[row[u]];
-        const float* from = p.scores + row[u] * group;
-        if constexpr (G == 2) *reinterpret_cast<float2*>(s[u]) = *reinterpret_cast<const float2*>(from);
-        if constexpr (G == 1) s[u][0] = *from;
-        if constexpr (G >= 4)
+        for (int i = 0; i < G; ++i) *reinterpret_cast<float4*>(&s[4 * i]) = reinterpret_cast<const float4*>(from)[i];
 #pragma unroll
-          for (int g = 0; g < G; g += 4) *reinterpret_cast<float4*>(&s[u][g]) = *reinterpret_cast<const float4*>(from + g);
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int g = 0; g < G; ++g) sum[i] += ex2(s[i * G + g] + st[g]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          for (int g = 0; g < group; ++g) sum[i] += ex2(from[i * group + g] + stats[g]);
       }
-#pragma unroll
-      for (int u = 0; u < kScoreDeep; ++u) {
-        if (row[u] < 0) continue;
-        float sum = 0.f;
-        if constexpr (G > 0) {
-#pragma unroll
-          for (int g = 0; g < G; ++g) sum += ex2(s[u][g] + st[g]);
-        } else {
-          for (int g = 0; g < group; ++g) sum += ex2(p.scores[row[u] * group + g] + stats[g]);
-        }
-        mass[row[u]] = m[u] + sum;
+      m = make_float4(m.x + sum[0], m.y + sum[1], m.z + sum[2], m.w + sum[3]);
+      if (v + 4 <= v1 && (p.window <= 0 || pos > q - p.window || pos + 3 < p.sinks)) {
+        *at = m;
+        continue;
       }
+      const float y[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v + i < v1 && sees(p, q, pos + i)) mass[row + i] = y[i];
     }
   }
 }
