@@ -701,6 +701,11 @@ int snapmind_paged_gqa_chunk_mass(const void* q, int64_t q_stride_tok, int64_t q
   const int64_t room = (int64_t)table_width * block_size;
   p.max_len = room < (1 << 30) ? (int32_t)room : (1 << 30);
   p.err = err_word;
+  if (mass) {  // the pass over the weights counts its steps in 32 bits: refused before anything is launched
+    const int gw = p.group < kRows ? p.group : kRows, tokens = kRows / gw, slices = (p.group + gw - 1) / gw;
+    SNAPMIND_CHECK_ARG(((int64_t)total_q / tokens + batch) * slices * (p.max_len / kKeys + 2) < (int64_t)1 << 31,
+                       "paged_chunk: %d new tokens over tables of %d positions are too many for one call", total_q, p.max_len);
+  }
   const int64_t attention = chunk_workspace_bytes(head_dim);
   const int64_t need = mass ? snapmind_paged_gqa_chunk_mass_workspace_bytes(head_dim, total_q, n_q_heads, n_kv_heads, block_size,
                                                                             num_blocks, cu_q == nullptr)

@@ -43,7 +43,7 @@ template <int D> struct Shape {
 };
 
 struct Ctrl {
-  uint64_t k_full[2], k_empty[2], q_full[4], q_empty[4], x_full[4], x_empty[4];
+  uint64_t k_full[2], k_empty[2], q_full[2], q_empty[2], x_full[4], x_empty[4];
   uint64_t s_full[2][2], s_free[2][2];  // [key tile][buffer]
   uint64_t done;                        // every MMA has completed
   uint32_t tmem_base;
@@ -96,10 +96,8 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&C.k_full[i]), kQuant ? 128 : 1);
       mbar_init(smem_u32(&C.k_empty[i]), 1);
-      mbar_init(smem_u32(&C.q_full[2 * i]), 1);
-      mbar_init(smem_u32(&C.q_empty[2 * i]), 1);
-      mbar_init(smem_u32(&C.q_full[2 * i + 1]), 1);
-      mbar_init(smem_u32(&C.q_empty[2 * i + 1]), 1);
+      mbar_init(smem_u32(&C.q_full[i]), 1);
+      mbar_init(smem_u32(&C.q_empty[i]), 1);
       for (int k = 2 * i; k < 2 * i + 2; ++k) {
         mbar_init(smem_u32(&C.x_full[k]), 2 * 32);
         mbar_init(smem_u32(&C.x_empty[k]), 8);
@@ -255,6 +253,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         }
       }
       if (!ok && lane == 0) give_up(C, p.err);
+      asm volatile("cp.async.wait_all;" ::: "memory");  // no copy outlives the block
     } else if (kQuant && warp >= Ro::kConvert) {
       // ------------------------------------------------------------------ e4m3 codes -> 16-bit K tiles
       const int ct = tid - Ro::kConvert * 32;

@@ -2,6 +2,7 @@
 import ctypes
 
 import pytest
+import torch
 
 import snapmind_b200._lib as lib
 
@@ -93,3 +94,20 @@ def test_append_rope_refusals(kw, word):
 
 def test_append_rope_of_nothing():
     assert rope(batch=0, total=0) == lib.OK
+
+
+def chunk_mass(total=8, width=4, mass=256, dtype=0, x=X):
+    return lib.load().snapmind_paged_gqa_chunk_mass(x, 512, 64, dtype, x, x, None, dtype, x, width, width, x, x, x, 512, 64, 1.0, 1,
+                                                    total, 8, 1, 64, 16, 4, 0, 0, 0, ctypes.c_void_p(mass), x, 1 << 60, None, None)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up pointers")
+@pytest.mark.parametrize("kw,word", [
+    (dict(total=1 << 22, width=1 << 22), "too many"),
+    (dict(total=1 << 30, width=1 << 16), "too many"),
+    (dict(mass=260), "16-byte"),
+])
+def test_accumulate_refusals(kw, word):
+    """All before the attention of the call is launched."""
+    assert chunk_mass(**kw) == lib.ERR_BAD_ARGUMENT
+    assert word in lib.last_error()
