@@ -2,7 +2,8 @@
 // CUDA-core pass over the scores (any head_dim up to 256, any block size and type) and the merge of cut units.
 //
 // The CUDA-core pass: 64 query rows x 64 keys a step, thread (ty, tx) holding rows ty + 16 i and keys tx + 16 j,
-// all in f32; the keys stay in shared memory while the rows go by.
+// all in f32; the keys stay in shared memory while the rows go by.  FMA and shared-memory issue bound it: 4 prompts
+// of 256 f32 tokens (32 heads over 4 of 64) take 56 us of attention and 40 for the weights.
 #include "chunk_mass.cuh"
 #include "pairs.cuh"
 

@@ -66,8 +66,10 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 // are more), warp w holding run w of the chunk's indexes; the order of the last that stays is found from a histogram
 // of the highest 11 bits, counted as the weights come in, and then among the few of its bin (or 11 bits at a time, if
 // they are not few), and the kept indexes are counted per warp by ballots and written out in a second sweep.  What
-// bounds it is latency (a read of the table, one of the weights, a handful of barriers), so blocks are small
-// where sequences are short, several to an SM.
+// bounds it is instructions (64% of the issue slots: the sweeps, and orders made of weights), with a read of the
+// table, one of the weights and a handful of barriers for latency, so blocks are small where sequences are short,
+// several to an SM: 1024 units of 2112 tokens 26 us, 1024 of 1 to 8 thousand 67, 128 of 32768 47.  Tried and dropped:
+// histogram additions put together by the lanes of a bin (128 units: 77 us, 54 without), fewer registers (76 us, 70).
 constexpr int kRadix = 11, kBins = 1 << kRadix;
 static_assert(2 * 49152 / 32 <= kBins + 1024, "bits of a chunk");
 constexpr int kFew = 256;  // that many are listed and compared with one another (800 took 25 us more than another histogram)
@@ -304,7 +306,9 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
 // Rows of the kept tokens of one (layer, sequence, head): a block moves slice_bytes of each K or V row, TEAM lanes of
 // W bytes a row, 32 rows a warp and step.  A lane works out where one row comes from and goes to (and moves its
 // scale), and the teams fetch that by shuffles; the next step's indexes are read while this one's rows are on
-// their way.  Where there are few units, a row's columns go to several blocks, which never meet.
+// their way.  Where there are few units, a row's columns go to several blocks, which never meet.  HBM bound: 16 layers
+// of 4096 rows of 256 bytes for each of 8 heads, K and V, take 105 us (5.1 TB/s; 227 with a row's place worked out by every
+// lane of it), 8-bit rows of 1024 units 94 (5.6 TB/s).
 constexpr int kMoveThreads = 256;
 template <int W, int TEAM>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
