@@ -383,7 +383,8 @@ __device__ __forceinline__ void mul4(float4& a, float f) {
   a.w *= f;
 }
 
-template <typename T>
+// kStats: the rows' softmax sums go to p.stats.
+template <typename T, bool kStats>
 __device__ __forceinline__ void merge_units(const ChunkParams& p) {
   const int cta = blockIdx.x + 1;
   if (cta >= p.n_ctas) return;
@@ -425,7 +426,7 @@ __device__ __forceinline__ void merge_units(const ChunkParams& p) {
       float f = ml.x == -INFINITY ? ml.y : ex2(ml.x - ref), L = ml.y * f;
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-      if (il == 0 && rl < n_rows) {
+      if (kStats && il == 0 && rl < n_rows) {
         const int tok = p.by_gw.div(rl), g = rl - tok * p.gw;
         if (g < heads) write_stats(p, first + i0 + tok, kvh * p.group + slice * p.gw + g, M, L);
       }
@@ -502,7 +503,7 @@ __device__ __forceinline__ void merge_units(const ChunkParams& p) {
       }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    if (lane == 0) write_stats(p, first + i0 + p.by_gw.div(r), kvh * p.group + slice * p.gw + g, M, L);
+    if (kStats && lane == 0) write_stats(p, first + i0 + p.by_gw.div(r), kvh * p.group + slice * p.gw + g, M, L);
     mul4(acc[0], inv);
     mul4(acc[1], inv);
     T* out = out_row(r, g);
@@ -511,20 +512,20 @@ __device__ __forceinline__ void merge_units(const ChunkParams& p) {
   }
 }
 
-template <typename T>
+template <typename T, bool kStats>
 __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkParams p) {
   next_grid_may_launch();  // every block of this grid has started by then
   prior_grid_wait();
-  merge_units<T>(p);
+  merge_units<T, kStats>(p);
 }
 // After a call that may have been done over: `again` merges the units of that.
-template <typename T>
+template <typename T, bool kStats>
 __global__ void __launch_bounds__(32 * kMergeWarps)
     chunk_merge_either_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ ChunkParams again) {
   next_grid_may_launch();
   prior_grid_wait();
-  if (any_odd(again)) merge_units<T>(again);
-  else merge_units<T>(p);
+  if (any_odd(again)) merge_units<T, kStats>(again);
+  else merge_units<T, kStats>(p);
 }
 
 dim3 merge_grid(const ChunkParams& p) {
@@ -562,8 +563,8 @@ int launch_f16_over_e4m3(ChunkParams& p, cudaStream_t st) {
   rc = launch_generic<__half, uint8_t>(again, st);
   if (rc != SNAPMIND_OK) return rc;
   const dim3 a = merge_grid(p), b = merge_grid(again);
-  return cuda_status(launch_dependent(chunk_merge_either_kernel<__half>, dim3(a.x > b.x ? a.x : b.x, a.y > b.y ? a.y : b.y),
-                                      32 * kMergeWarps, 0, st, p, again),
+  const auto kernel = p.stats ? chunk_merge_either_kernel<__half, true> : chunk_merge_either_kernel<__half, false>;
+  return cuda_status(launch_dependent(kernel, dim3(a.x > b.x ? a.x : b.x, a.y > b.y ? a.y : b.y), 32 * kMergeWarps, 0, st, p, again),
                      "paged_chunk merge");
 }
 
@@ -585,9 +586,9 @@ int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st) {
     return cuda_status(launch_dependent(kernel, merge_grid(p), 32 * kMergeWarps, 0, st, p), "paged_chunk merge");
   };
   switch (dtype) {
-    case SNAPMIND_DTYPE_F32: return go(chunk_merge_kernel<float>);
-    case SNAPMIND_DTYPE_BF16: return go(chunk_merge_kernel<__nv_bfloat16>);
-    default: return go(chunk_merge_kernel<__half>);
+    case SNAPMIND_DTYPE_F32: return p.stats ? go(chunk_merge_kernel<float, true>) : go(chunk_merge_kernel<float, false>);
+    case SNAPMIND_DTYPE_BF16: return p.stats ? go(chunk_merge_kernel<__nv_bfloat16, true>) : go(chunk_merge_kernel<__nv_bfloat16, false>);
+    default: return p.stats ? go(chunk_merge_kernel<__half, true>) : go(chunk_merge_kernel<__half, false>);
   }
 }
 
