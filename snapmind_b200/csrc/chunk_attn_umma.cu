@@ -279,6 +279,9 @@ __device__ __forceinline__ bool odd_row(int kv, const uint4& codes, const uint4&
   return (top & 0x80008000u) != 0;
 }
 
+// Out of line: instructions that most calls do not need.
+__device__ __noinline__ void stats_of(const ChunkParams& p, int row, int head, float m, float l) { write_stats(p, row, head, m, l); }
+
 // The third warpgroup (e4m3: and the fourth) gives up registers that the softmax threads, with a row
 // of 128 scores each, need: 3 x 128 threads are launched with 168 each, 4 x 128 with 128.
 template <bool kQuant> struct Roles {
@@ -772,7 +775,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         p.part_ml[slot * 2] = m;
         p.part_ml[slot * 2 + 1] = l;
       }
-      if (whole && mine) write_stats(p, c.q_first + c.i0 + tok, c.kvh * p.group + c.slice * p.gw + g, m, l);
+      if (p.stats != nullptr && whole && mine) stats_of(p, c.q_first + c.i0 + tok, c.kvh * p.group + c.slice * p.gw + g, m, l);
       if (whole) {  // sees nothing: zeros
         const float inv = l == 0.f ? 0.f : 1.f / l;
         f *= inv;
