@@ -79,8 +79,13 @@ struct Step {
   }
 };
 
-// tiles: mp.c for tiles of 128 keys.
-template <typename T, int D, bool kQuant>
+// tiles: mp.c for tiles of 128 keys.  kFull: no row of a step is left without a query (the heads divide 128), or its score
+// does not matter: such a row is zeros of Q, and a key that holds an infinity would give it NaN, which an x of
+// -infinity does not take out (an e4m3 row holds none, and with a NaN it is NaN for whoever sees it).  A NaN score of a row
+// with a query goes with an x of NaN, so NaN scores may become numbers: one maximum each for the later half of the rows.  It
+// costs calls of 3 heads a kv head 1% (2048 new of 32768: 1261 us, 1244 without); a branch on the row's number cost
+// them 8%, and in the kernel of full steps 4%.
+template <typename T, int D, bool kQuant, bool kFull>
 __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     mass_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                      const __grid_constant__ MassParams mp, const __grid_constant__ ChunkParams tiles) {
@@ -314,10 +319,12 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         }
         if (c.whole()) old = mp.mass[row];
       }
+      // of a row without a query (kFull): f low is finite; a query's score below it weighs nothing, or its x is NaN
+      const float low = -3e38f / fmaxf(1.f, fabsf(f));
       on = w.next(mp);
       if (on) row_next = mass_row(p, w.kr, w.c.b, w.c.kvh, w.c.tile, t * kTile + key, &pos_next);
       // steps whose rows all see all of the warp's keys: first tokens from `from_i0` to `to_i0` (keys that are none do
-      // not matter, nor do rows past the last token of a step: their x is -infinity)
+      // not matter)
       const int far = 1 << 30;
       const int from_i0 = __reduce_max_sync(0xffffffffu, row >= 0 ? pos - pos0 : -far);
       const int to_i0 = min(c.n - p.tokens, __reduce_min_sync(0xffffffffu, row >= 0 && p.window > 0 && pos >= p.sinks
@@ -349,6 +356,10 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(smem_u32(&C.s_free[t][q & 1]));
+            }
+            if (!kFull && k >= kRowsStep / 64) {  // (more than half of a step's rows have queries)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) u[i] = fmaxf(u[i], low);
             }
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
@@ -427,10 +438,8 @@ bool q_step_map(CUtensorMap* map, bool bf16, const ChunkParams& p, int D) {
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D, bool kQuant>
-int launch(MassParams& mp, cudaStream_t st) {
-  const int rc = mass_geometry(mp, kRowsStep, kUnit, num_sms());
-  if (rc != SNAPMIND_OK) return rc;
+template <typename T, int D, bool kQuant, bool kFull>
+int launch_geometry(MassParams& mp, cudaStream_t st) {
   ChunkParams tiles = mp.c;
   tiles.key_tile = kTile;
   tiles.by_tile = FastDiv(kTile);
@@ -440,13 +449,22 @@ int launch(MassParams& mp, cudaStream_t st) {
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   if ((!kQuant && !tensor_map_row_groups(&k_map, bf16, mp.c.k_pool, rows, D, box / 8)) || !q_step_map(&q_map, bf16, mp.c, D))
     return SNAPMIND_ERR_UNSUPPORTED;  // the caller takes the CUDA-core kernel
-  auto kernel = mass_umma_kernel<T, D, kQuant>;
+  auto kernel = mass_umma_kernel<T, D, kQuant, kFull>;
   static bool done[kMaxDevices] = {};
   const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem_bytes<D>(), done);
   if (e != cudaSuccess) return cuda_status(e, "paged_chunk mass smem attribute");
   const int status = cuda_status(launch_dependent(kernel, dim3(mp.c.n_ctas), Roles<kQuant>::kThreads, smem_bytes<D>(), st, q_map, k_map, mp, tiles),
                                  "paged_chunk mass launch");
   return status != SNAPMIND_OK ? status : launch_mass_merge(mp, st);
+}
+
+template <typename T, int D, bool kQuant>
+int launch(MassParams& mp, cudaStream_t st) {
+  const int rc = mass_geometry(mp, kRowsStep, kUnit, num_sms());
+  if (rc != SNAPMIND_OK) return rc;
+  if constexpr (!kQuant)
+    if (mp.c.tokens * mp.c.gw < kRowsStep) return launch_geometry<T, D, kQuant, false>(mp, st);
+  return launch_geometry<T, D, kQuant, true>(mp, st);
 }
 
 }  // namespace
