@@ -519,6 +519,15 @@ SNAPMIND_API int snapmind_kv_reserve_each(int32_t *block_tables, int64_t table_s
                              int32_t *err_word, void *stream);
 
 /*
+ * Either of the two (n_each NULL: n_new tokens each) that also writes this call's own error bits to *status (device), 0 when
+ * the sequences grew: the error word keeps what other calls set.
+ */
+SNAPMIND_API int snapmind_kv_reserve_status(int32_t *block_tables, int64_t table_stride_seq, int32_t table_width,
+                             int32_t *seq_lens, const int32_t *n_each, int32_t n_new, int32_t batch,
+                             int32_t block_size, int32_t *free_stack, int32_t *free_top, int32_t num_blocks,
+                             int32_t *err_word, int32_t *status, void *stream);
+
+/*
  * Append chunks of new K/V rows, of one length for every sequence or ragged,
  * to a pool of f32 / bf16 / f16 elements or to an 8-bit pool
  * (pool_dtype SNAPMIND_DTYPE_E4M3).
@@ -628,13 +637,13 @@ SNAPMIND_API int snapmind_paged_gqa_chunk_mass(const void *q, int64_t q_stride_t
 
 /*
  * Set to 0 the mass of the newest tokens of every sequence in all layers (after the reserve that
- * made room for them): counts[b] of sequence b (device), or n_new each when counts is NULL.  Nothing happens while
- * *err_word says that a reserve failed.
+ * made room for them): counts[b] of sequence b (device), or n_new each when counts is NULL.  Nothing happens if *status, as
+ * snapmind_kv_reserve_status wrote it, says that the reserve failed (status NULL: it did not).
  */
 SNAPMIND_API int snapmind_kv_clear_mass(float *mass, int64_t mass_layer_stride, const int32_t *block_tables,
                              int64_t table_stride_seq, int32_t table_width, const int32_t *seq_lens,
                              const int32_t *counts, int32_t n_new, int32_t batch, int32_t n_layers, int32_t n_heads,
-                             int32_t block_size, int32_t num_blocks, const int32_t *err_word, void *stream);
+                             int32_t block_size, int32_t num_blocks, const int32_t *status, void *stream);
 
 /*
  * Evict by accumulated weight.  Of every sequence with more than `budget` tokens each (layer, kv head) keeps the

@@ -134,6 +134,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _i64, _i64, _p, _p, _int, _p, _i64, _i32, _p, _p, _i64, _i64, _f32, _i32, _i32, _i32,
          _i32, _i32, _i32, _i32, _i32, _i32, _p, _p],
     ),
+    "snapmind_kv_reserve_status": (_int, [_p, _i64, _i32, _p, _p, _i32, _i32, _i32, _p, _p, _i32, _p, _p, _p]),
     "snapmind_kv_reserve_each": (_int, [_p, _i64, _i32, _p, _p, _i32, _i32, _p, _p, _i32, _p, _p]),
     "snapmind_kv_append_chunk": (
         _int,

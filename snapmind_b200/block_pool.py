@@ -35,6 +35,7 @@ class BlockPool:
         self.free_stack = torch.arange(num_blocks - 1, -1, -1, dtype=torch.int32, device=self.device)
         self.free_top = torch.tensor([num_blocks], dtype=torch.int32, device=self.device)
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._reserve_status = None  # error bits of the last reserve alone, for pools that act on them (``_reserved``)
         self._host_lens = np.zeros(max_seqs, dtype=np.int64)
         self._host_free = num_blocks
 
@@ -80,6 +81,17 @@ class BlockPool:
     def _reserved(self, n_new: int, batch: int, counts: torch.Tensor | None = None) -> None:
         """Launched behind every reserve: the first ``batch`` sequences grew by ``n_new`` tokens (``counts``: each its own)."""
 
+    def _grow(self, what: str, n_new: int, batch: int, counts: torch.Tensor | None = None) -> None:
+        with self._on_device():
+            status = _lib.load().snapmind_kv_reserve_status(
+                self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq,
+                self.seq_lens.data_ptr(), _lib.ptr(counts), n_new, batch, self.block_size,
+                self.free_stack.data_ptr(), self.free_top.data_ptr(), self.num_blocks,
+                self.err.data_ptr(), _lib.ptr(self._reserve_status), _lib.raw_stream(self._index),
+            )  # fmt: skip
+        _lib.check(status, f"{type(self).__name__}.{what}")
+        self._reserved(n_new, batch, counts)
+
     def reserve(self, n_new: int = 1, batch: int | None = None) -> None:
         """Grow the first ``batch`` sequences by ``n_new`` tokens (tables + lengths)."""
         batch = self.max_seqs if batch is None else batch
@@ -90,14 +102,7 @@ class BlockPool:
             raise RuntimeError(_lib.OUT_OF_BLOCKS_MSG)
         if batch and int(((lens + n_new + bs - 1) // bs).max()) > self.max_blocks_per_seq:
             raise ValueError("sequence would outgrow its block table row")
-        status = _lib.load().snapmind_kv_reserve(
-            self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq,
-            self.seq_lens.data_ptr(), batch, n_new, bs,
-            self.free_stack.data_ptr(), self.free_top.data_ptr(), self.num_blocks,
-            self.err.data_ptr(), self._stream(),
-        )  # fmt: skip
-        _lib.check(status, f"{type(self).__name__}.reserve")
-        self._reserved(n_new, batch)
+        self._grow("reserve", n_new, batch)
         self._host_lens[:batch] += n_new
         self._host_free -= need
 
@@ -118,15 +123,7 @@ class BlockPool:
         if len(n) and int(want.max()) > self.max_blocks_per_seq:
             raise ValueError("sequence would outgrow its block table row")
         counts = torch.from_numpy(n.astype(np.int32)).to(self.device)
-        with self._on_device():
-            status = _lib.load().snapmind_kv_reserve_each(
-                self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq,
-                self.seq_lens.data_ptr(), counts.data_ptr(), len(n), bs,
-                self.free_stack.data_ptr(), self.free_top.data_ptr(), self.num_blocks,
-                self.err.data_ptr(), self._stream(),
-            )  # fmt: skip
-        _lib.check(status, f"{type(self).__name__}.reserve_each")
-        self._reserved(int(n.max()) if n.size else 0, len(n), counts)
+        self._grow("reserve_each", int(n.max()) if n.size else 0, len(n), counts)
         self._host_lens[:len(n)] += n
         self._host_free -= need
 
@@ -140,14 +137,7 @@ class BlockPool:
         """The device part of ``reserve`` only (no host mirrors, no checks): a
         launch that a CUDA graph can replay.  The caller checks the capacity
         for all replays up front and accounts them with ``account_host``."""
-        status = _lib.load().snapmind_kv_reserve(
-            self.block_tables.data_ptr(), self.max_blocks_per_seq, self.max_blocks_per_seq,
-            self.seq_lens.data_ptr(), batch, n_new, self.block_size,
-            self.free_stack.data_ptr(), self.free_top.data_ptr(), self.num_blocks,
-            self.err.data_ptr(), self._stream(),
-        )  # fmt: skip
-        _lib.check(status, f"{type(self).__name__}.reserve_device")
-        self._reserved(n_new, batch)
+        self._grow("reserve_device", n_new, batch)
 
     def account_host(self, n_new: int, batch: int) -> None:
         """Advance the host mirrors as ``reserve(n_new, batch)`` would."""

@@ -442,7 +442,8 @@ __global__ void __launch_bounds__(kTableThreads) evict_tables_kernel(const __gri
   if (tid == 0) *p.free_top = end;
 }
 
-// Weights of the newest tokens of every sequence: 0, in all layers.  Not after a reserve that failed.
+// Weights of the newest tokens of every sequence: 0, in all layers.  Not after a reserve that failed: those of older tokens
+// would go.
 struct ClearParams {
   float* mass;
   int64_t mass_layer;
@@ -452,10 +453,10 @@ struct ClearParams {
   const int32_t* seq_lens;
   const int32_t* counts;  // NULL: n_new each
   int32_t n_new, batch, n_layers, n_heads, block_size, num_blocks;
-  const int32_t* err;
+  const int32_t* status;  // of the reserve
 };
 __global__ void __launch_bounds__(256) clear_mass_kernel(const __grid_constant__ ClearParams p) {
-  if (p.err != nullptr && (*p.err & (SNAPMIND_DEVERR_OUT_OF_BLOCKS | SNAPMIND_DEVERR_TABLE)) != 0) return;
+  if (p.status != nullptr && (*p.status & (SNAPMIND_DEVERR_OUT_OF_BLOCKS | SNAPMIND_DEVERR_TABLE)) != 0) return;
   const int per = p.n_layers * p.n_heads;
   for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
     const int len = p.seq_lens[b], n = min(p.counts ? p.counts[b] : p.n_new, len);
@@ -582,13 +583,13 @@ int snapmind_kv_evict_by_mass(void* k_pool, void* v_pool, void* scales, int pool
 int snapmind_kv_clear_mass(float* mass, int64_t mass_layer_stride, const int32_t* block_tables, int64_t table_stride_seq,
                            int32_t table_width, const int32_t* seq_lens, const int32_t* counts, int32_t n_new, int32_t batch,
                            int32_t n_layers, int32_t n_heads, int32_t block_size, int32_t num_blocks,
-                           const int32_t* err_word, void* stream) {
+                           const int32_t* status, void* stream) {
   SNAPMIND_CHECK_ARG(batch >= 0 && n_new >= 0 && n_layers > 0 && n_heads > 0 && block_size > 0 && num_blocks > 0 && table_width >= 0,
                      "kv_clear_mass: bad sizes");
   if (batch == 0 || (counts == nullptr && n_new == 0)) return SNAPMIND_OK;
   SNAPMIND_CHECK_ARG(mass && block_tables && seq_lens, "kv_clear_mass: null pointer");
   const ClearParams p{mass, mass_layer_stride, block_tables, table_stride_seq, table_width, seq_lens, counts, n_new,
-                      batch, n_layers, n_heads, block_size, num_blocks, err_word};
+                      batch, n_layers, n_heads, block_size, num_blocks, status};
   const int64_t each = counts ? 4096 : (int64_t)n_new * n_layers * n_heads;
   const int64_t blocks = (each + 255) / 256;
   const dim3 grid((uint32_t)(blocks < 64 ? blocks : 64), (uint32_t)(batch < 1024 ? batch : 1024));

@@ -333,6 +333,7 @@ struct ReserveParams {
   int32_t num_blocks;
   int32_t* err;
   const int32_t* n_each = nullptr;  // reserve: new tokens of every sequence (NULL: n_new each)
+  int32_t* status = nullptr;        // reserve: this call's own error bits (NULL: not wanted)
 };
 
 // Exclusive block-wide scan of one int per thread; returns the prefix and
@@ -392,6 +393,7 @@ __global__ void __launch_bounds__(1024) kv_reserve_kernel(ReserveParams p) {
   const int top = *p.free_top;
   if (threadIdx.x == 0 && s_need > (unsigned long long)max(top, 0)) s_bad |= SNAPMIND_DEVERR_OUT_OF_BLOCKS;
   __syncthreads();
+  if (threadIdx.x == 0 && p.status != nullptr) *p.status = s_bad;
   if (s_bad) {
     if (threadIdx.x == 0) flag_error(p.err, s_bad);
     return;
@@ -666,32 +668,37 @@ int snapmind_kv_copy_slots(void* k_pool, void* v_pool, int dtype, const int32_t*
   SNAPMIND_LAUNCH_CHECK("kv_copy_slots launch");
 }
 
+static int reserve(const ReserveParams& p, const char* name, void* stream) {
+  SNAPMIND_CHECK_ARG(p.batch >= 0 && p.n_new >= 0 && p.block_size > 0 && p.table_width >= 0, "%s: bad sizes", name);
+  if (p.batch == 0) return SNAPMIND_OK;
+  SNAPMIND_CHECK_ARG(p.tables && p.seq_lens && p.free_stack && p.free_top, "%s: null pointer", name);
+  kv_reserve_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return cuda_status(cudaGetLastError(), "kv_reserve launch");
+}
+
 int snapmind_kv_reserve(int32_t* block_tables, int64_t table_stride_seq, int32_t table_width,
                         int32_t* seq_lens, int32_t batch, int32_t n_new, int32_t block_size,
                         int32_t* free_stack, int32_t* free_top, int32_t num_blocks,
                         int32_t* err_word, void* stream) {
-  SNAPMIND_CHECK_ARG(batch >= 0 && n_new >= 0 && block_size > 0 && table_width >= 0,
-                     "kv_reserve: bad sizes");
-  if (batch == 0) return SNAPMIND_OK;
-  SNAPMIND_CHECK_ARG(block_tables && seq_lens && free_stack && free_top,
-                     "kv_reserve: null pointer");
-  ReserveParams p{block_tables, table_stride_seq, table_width, seq_lens, nullptr, batch, n_new,
-                  block_size, free_stack, free_top, num_blocks, err_word};
-  kv_reserve_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  SNAPMIND_LAUNCH_CHECK("kv_reserve launch");
+  return reserve(ReserveParams{block_tables, table_stride_seq, table_width, seq_lens, nullptr, batch, n_new,
+                               block_size, free_stack, free_top, num_blocks, err_word}, "kv_reserve", stream);
 }
 
 int snapmind_kv_reserve_each(int32_t* block_tables, int64_t table_stride_seq, int32_t table_width,
                              int32_t* seq_lens, const int32_t* n_new, int32_t batch, int32_t block_size,
                              int32_t* free_stack, int32_t* free_top, int32_t num_blocks, int32_t* err_word,
                              void* stream) {
-  SNAPMIND_CHECK_ARG(batch >= 0 && block_size > 0 && table_width >= 0, "kv_reserve_each: bad sizes");
-  if (batch == 0) return SNAPMIND_OK;
-  SNAPMIND_CHECK_ARG(block_tables && seq_lens && n_new && free_stack && free_top, "kv_reserve_each: null pointer");
-  ReserveParams p{block_tables, table_stride_seq, table_width, seq_lens, nullptr, batch, 0,
-                  block_size, free_stack, free_top, num_blocks, err_word, n_new};
-  kv_reserve_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  SNAPMIND_LAUNCH_CHECK("kv_reserve_each launch");
+  SNAPMIND_CHECK_ARG(n_new != nullptr || batch <= 0, "kv_reserve_each: null pointer");
+  return reserve(ReserveParams{block_tables, table_stride_seq, table_width, seq_lens, nullptr, batch, 0,
+                               block_size, free_stack, free_top, num_blocks, err_word, n_new}, "kv_reserve_each", stream);
+}
+
+int snapmind_kv_reserve_status(int32_t* block_tables, int64_t table_stride_seq, int32_t table_width,
+                               int32_t* seq_lens, const int32_t* n_each, int32_t n_new, int32_t batch,
+                               int32_t block_size, int32_t* free_stack, int32_t* free_top, int32_t num_blocks,
+                               int32_t* err_word, int32_t* status, void* stream) {
+  return reserve(ReserveParams{block_tables, table_stride_seq, table_width, seq_lens, nullptr, batch, n_new,
+                               block_size, free_stack, free_top, num_blocks, err_word, n_each, status}, "kv_reserve_status", stream);
 }
 
 int snapmind_kv_release(int32_t* block_tables, int64_t table_stride_seq, int32_t table_width,

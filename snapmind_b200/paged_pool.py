@@ -62,6 +62,7 @@ class PagedKVPool(BlockPool):
         self.mass = None
         if mass:
             self.mass = torch.zeros((n_layers, num_blocks, n_kv_heads, block_size), dtype=torch.float32, device=self.device)
+            self._reserve_status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._workspace = _lib.DecodeWorkspace(self.device)
         with self._on_device():
             self._chunk_ws = _lib.load().snapmind_paged_gqa_chunk_workspace_bytes(head_dim)
@@ -229,7 +230,7 @@ class PagedKVPool(BlockPool):
             status = _lib.load().snapmind_kv_clear_mass(
                 self.mass.data_ptr(), self.mass.stride(0), self.block_tables.data_ptr(), self.max_blocks_per_seq,
                 self.max_blocks_per_seq, self.seq_lens.data_ptr(), _lib.ptr(counts), n_new, batch, self.n_layers,
-                self.n_kv_heads, self.block_size, self.num_blocks, self.err.data_ptr(), _lib.raw_stream(self._index),
+                self.n_kv_heads, self.block_size, self.num_blocks, _lib.ptr(self._reserve_status), _lib.raw_stream(self._index),
             )  # fmt: skip
         _lib.check(status, f"{type(self).__name__}.reserve")
 

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import snapmind_b200._lib as lib
 from test_chunk_gpu import DT, make_pool
 from test_evict_gpu import U, dense, reference_mass
 
@@ -46,3 +47,41 @@ def test_keys_that_an_infinity_masks(dtype, group, d, new, generic):
         pool.attend_chunk(0, q, torch.tensor([0, t], dtype=torch.int32, device="cuda"), accumulate=True, force_generic=generic)
     got, sees = dense(pool, pool.mass[0], 0, n), n - t + t // 3 + 1
     assert torch.isnan(got[0, :sees]).all() and not torch.isnan(got[0, sees:]).any() and not torch.isnan(got[1]).any()
+
+
+def test_new_tokens_after_an_error():
+    """What an error word says of other calls does not keep a reserve's new tokens from weighing nothing; a reserve that
+    failed leaves all weights as they are."""
+    from snapmind_b200 import PagedKVPool
+
+    for word in (lib.DEVERR_TABLE, lib.DEVERR_OUT_OF_BLOCKS, lib.DEVERR_TABLE | lib.DEVERR_BLOCK_ID):
+        for how in ("reserve", "each", "device"):
+            pool = PagedKVPool(2, 3, 64, 16, max_seqs=2, max_blocks_per_seq=8, mass=True)
+            pool.reserve(20)
+            pool.mass.fill_(7.0)
+            pool.err.fill_(word)
+            if how == "reserve":
+                pool.reserve(5)
+            elif how == "each":
+                pool.reserve_each([5, 5])
+            else:
+                pool.reserve_device(5, 2)
+            for layer in range(2):
+                for b in range(2):
+                    m = dense(pool, pool.mass[layer], b, 25)
+                    assert (m[:, 20:] == 0).all() and (m[:, :20] == 7).all(), (word, how)
+            assert int((pool.mass == 0).sum()) == 2 * 3 * 2 * 5
+            assert int(pool.err.item()) == word
+    # a reserve on the device that fails, one that succeeds behind it, without a check between them
+    pool = PagedKVPool(1, 2, 64, 4, max_seqs=2, max_blocks_per_seq=8, mass=True)
+    pool.reserve(20)
+    pool.mass.fill_(7.0)
+    pool.reserve_device(30, 2)
+    assert (pool.mass == 7).all() and pool.seq_lens.tolist() == [20, 20]
+    pool.reserve_device(12, 2)
+    pool.account_host(12, 2)
+    for b in range(2):
+        m = dense(pool, pool.mass[0], b, 32)
+        assert (m[:, 20:] == 0).all() and (m[:, :20] == 7).all()
+    with pytest.raises(RuntimeError, match="out of blocks"):
+        pool.check()
