@@ -655,7 +655,8 @@ SNAPMIND_API int snapmind_kv_clear_mass(float *mass, int64_t mass_layer_stride, 
  *   into (device ids, distinct, none of them in seqs): the sequences stay; what the targets held is replaced
  *     by the kept tokens, their blocks grow or shrink (SNAPMIND_DEVERR_OUT_OF_BLOCKS and nothing happens
  *     when the free stack has not enough).
- * kept [n_layers][n_seqs][n_heads][budget] receives the kept indexes, ascending, -1 behind the last.
+ * kept [n_layers][n_seqs][n_heads][budget] receives the kept indexes, ascending, -1 behind the last (and nothing but -1 when
+ * the blocks did not suffice).
  * pool_layer_stride and mass_layer_stride are in elements, scale_layer_stride in bytes.  max_len: the longest of the
  * sequences, or 0 (it chooses the launch; longer ones are still right).  Sequences must not share blocks.  The reference evicts the oldest tokens only (snapmind/kv_cache/paged.py evict).
  */

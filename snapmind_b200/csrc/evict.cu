@@ -56,6 +56,11 @@ __device__ __forceinline__ int64_t row_of(const EvictParams& p, const int32_t* t
   return ((int64_t)phys * p.n_heads + head) * p.block_size + (j - k * p.block_size);
 }
 
+// What tells the kernels of a call with targets that it was refused (their lengths do not: a target may have had its own
+// before): the first kept index of a sequence's first layer and head is -1.  There evict_tables_kernel leaves it, and
+// what selection writes in the end says the same: 0 or more, or -1 where a sequence keeps nothing.
+__device__ __forceinline__ int32_t* mark_of(const EvictParams& p, int i) { return p.kept + (int64_t)i * p.n_heads * p.budget; }
+
 // Order of weights as unsigned integers: -infinity lowest, infinity below NaN, -0 with 0.
 __device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
@@ -92,15 +97,15 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int layer = blockIdx.x / (p.n * p.n_heads), u = blockIdx.x - layer * (p.n * p.n_heads);
   const int i = u / p.n_heads, head = u - i * p.n_heads;
+  int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
+  const bool copies = p.dst != nullptr, refused = copies && *mark_of(p, i) < 0;
   const int from = src_id(p, i), to = dst_id(p, i);
   const int len = cached(p, from), keep = min(len, p.budget);
-  int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
   float* mass = p.mass + layer * p.mass_layer;
   const int32_t* table = p.tables + (int64_t)from * p.table_stride;
   const int32_t* new_table = p.tables + (int64_t)to * p.table_stride;
-  const bool copies = p.dst != nullptr;
-  if (copies && p.seq_lens[to] != keep) return;  // it was not given its blocks
-  for (int x = keep + tid; x < p.budget; x += THREADS) kept[x] = -1;
+  for (int x = (refused ? 0 : keep) + tid; x < p.budget; x += THREADS) kept[x] = -1;
+  if (refused) return;
   if (len <= p.budget) {
     for (int x = tid; x < keep; x += THREADS) {
       kept[x] = x;
@@ -322,8 +327,8 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
   const int from = src_id(p, i), to = dst_id(p, i);
   const int len = cached(p, from), keep = min(len, p.budget);
   const bool copies = p.dst != nullptr;
-  if (copies ? p.seq_lens[to] != keep : len <= p.budget) return;
   const int32_t* kept = p.kept + (int64_t)unit * p.budget;
+  if (copies ? *mark_of(p, i) < 0 : len <= p.budget) return;
   const int32_t* table = p.tables + (int64_t)from * p.table_stride;
   const int32_t* new_table = p.tables + (int64_t)to * p.table_stride;
   uint8_t* pool = p.pool[kv] + layer * p.pool_layer + slice * p.slice_bytes;
@@ -415,7 +420,10 @@ __global__ void __launch_bounds__(kTableThreads) evict_tables_kernel(const __gri
   __syncthreads();
   const int top = *p.free_top, pops = s_total[0], pushes = s_total[1];
   const int left = top - pops, end = left + pushes;
-  if (left < 0 || end > p.num_blocks) {  // nothing changes
+  const bool refused = left < 0 || end > p.num_blocks;
+  if (p.dst != nullptr)  // (in place the other kernels have run already)
+    for (int i = i0; i < i1; ++i) *mark_of(p, i) = refused ? -1 : 0;
+  if (refused) {  // nothing changes
     if (tid == 0) flag_error(p.err, SNAPMIND_DEVERR_OUT_OF_BLOCKS);
     return;
   }

@@ -49,6 +49,45 @@ def test_keys_that_an_infinity_masks(dtype, group, d, new, generic):
     assert torch.isnan(got[0, :sees]).all() and not torch.isnan(got[0, sees:]).any() and not torch.isnan(got[1]).any()
 
 
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_copies_without_blocks(cache):
+    """A call whose targets find too few blocks on the device changes nothing, a target that holds as many tokens as it would
+    end with among them, and names no kept token."""
+    from snapmind_b200 import PagedKVPool, QuantizedKVPool
+
+    cls = QuantizedKVPool if cache == "e4m3" else PagedKVPool
+    pool = cls(2, 2, 64, 24, max_seqs=4, max_blocks_per_seq=8, dtype=torch.bfloat16, mass=True)
+    pool.reserve_each([100, 90, 32, 0])
+    g = torch.Generator(device="cuda").manual_seed(1)
+    state = [pool.k, pool.v, pool.mass, pool.block_tables, pool.seq_lens, pool.free_stack, pool.free_top]
+    for x in state[:2] + ([pool.scales] if cache == "e4m3" else []):
+        x.view(torch.uint8).copy_(torch.randint(0, 256, x.view(torch.uint8).shape, generator=g, device="cuda", dtype=torch.int32).to(torch.uint8))
+    if cache == "e4m3":
+        state.append(pool.scales)
+    pool.mass.copy_(torch.rand(pool.mass.shape, generator=g, device="cuda"))
+    top = int(pool.free_top)
+    pool.free_top.fill_(1)  # the host's count does not know: sequence 3 would need two
+    held = [x.view(torch.uint8).clone() for x in state]
+    kept = pool.evict(32, recent=3, seqs=[0, 1], into=[2, 3])
+    for x, y in zip(state, held):
+        assert torch.equal(x.view(torch.uint8), y)
+    assert (kept == -1).all()
+    with pytest.raises(RuntimeError, match="out of blocks"):
+        pool.check()
+    # with the blocks there, the same call is what it says
+    pool.free_top.fill_(top)
+    kept = pool.evict(32, recent=3, seqs=[0, 1], into=[2, 3])
+    pool.check()
+    assert pool.seq_lens.tolist() == [100, 90, 32, 32] and int(pool.free_top) == top - 2 and (kept >= 0).all()
+    for layer in range(2):
+        for b in range(2):
+            i = kept[layer, b].long()
+            for x in (pool.k, pool.v):
+                a = dense(pool, x[layer].view(torch.uint8), b, 100 - 10 * b)
+                z = dense(pool, x[layer].view(torch.uint8), 2 + b, 32)
+                assert torch.equal(z, torch.gather(a, 1, i.unsqueeze(-1).expand(-1, -1, a.shape[-1])))
+
+
 def test_new_tokens_after_an_error():
     """What an error word says of other calls does not keep a reserve's new tokens from weighing nothing; a reserve that
     failed leaves all weights as they are."""
