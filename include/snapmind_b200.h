@@ -657,7 +657,8 @@ SNAPMIND_API int snapmind_kv_clear_mass(float *mass, int64_t mass_layer_stride, 
  *     when the free stack has not enough).
  * kept [n_layers][n_seqs][n_heads][budget] receives the kept indexes, ascending, -1 behind the last (and nothing but -1 when
  * the blocks did not suffice).
- * pool_layer_stride and mass_layer_stride are in elements, scale_layer_stride in bytes.  max_len: the longest of the
+ * pool_layer_stride and mass_layer_stride are in elements, scale_layer_stride in bytes; where block_size is a multiple of 4 each
+ * layer of mass stands on a 16-byte boundary.  max_len: the longest of the
  * sequences, or 0 (it chooses the launch; longer ones are still right).  Sequences must not share blocks.  The reference evicts the oldest tokens only (snapmind/kv_cache/paged.py evict).
  */
 SNAPMIND_API int snapmind_kv_evict_by_mass(void *k_pool, void *v_pool, void *scales, int pool_dtype,

@@ -507,6 +507,9 @@ int snapmind_kv_evict_by_mass(void* k_pool, void* v_pool, void* scales, int pool
   if (n_seqs == 0) return SNAPMIND_OK;
   SNAPMIND_CHECK_ARG(k_pool && v_pool && mass && block_tables && seq_lens && kept && free_stack && free_top, "kv_evict: null pointer");
   SNAPMIND_CHECK_ARG(into == nullptr || seqs != nullptr, "kv_evict: targets need the sequences named");
+  // weights are read four at a time where a block's are a multiple of four
+  SNAPMIND_CHECK_ARG(block_size % 4 != 0 || ((reinterpret_cast<uintptr_t>(mass) & 15) == 0 && mass_layer_stride % 4 == 0),
+                     "kv_evict: with blocks of %d tokens each layer of mass must stand on a 16-byte boundary", block_size);
   EvictParams p = {};
   p.tables = block_tables;
   p.table_stride = table_stride_seq;
