@@ -615,7 +615,7 @@ SNAPMIND_API int snapmind_paged_gqa_chunk(const void *q, int64_t q_stride_tok, i
  * snapmind_paged_gqa_chunk that also adds to every cached token the weight that the call's queries gave it:
  *   mass[block][kv head][slot] += sum, over the call's queries i that see the token and the query heads that
  *                                 read the kv head, of softmax(i)[token]
- * for the layer of k_pool (16-byte boundary; mass NULL: only the attention).  Weights and sums are f32, taken from the scores anew
+ * for the layer of k_pool (16-byte boundary where block_size is a multiple of 4; mass NULL: only the attention).  Weights and sums are f32, taken from the scores anew
  * once a row's softmax is known; the order of a sum depends on the sizes alone, so the same call gives the same
  * bits.  A query that sees nothing adds nothing; one whose softmax is NaN makes the tokens that it sees NaN.
  * q is read after out was written, so out must not be q.  The sequences must not share blocks, and calls that add

@@ -670,7 +670,10 @@ int snapmind_paged_gqa_chunk_mass(const void* q, int64_t q_stride_tok, int64_t q
   SNAPMIND_CHECK_ARG(cu_q != nullptr || total_q == batch, "paged_chunk: without cu_q there is one query per sequence");
   if (batch == 0 || total_q == 0) return SNAPMIND_OK;
   SNAPMIND_CHECK_ARG(q && k_pool && v_pool && block_tables && seq_lens && out, "paged_chunk: null pointer");
-  SNAPMIND_CHECK_ARG((reinterpret_cast<uintptr_t>(mass) & 15) == 0, "paged_chunk: mass must stand on a 16-byte boundary");
+  // weights are read four at a time only where a block's are a multiple of four; a later layer of smaller blocks
+  // may stand on any float
+  SNAPMIND_CHECK_ARG((reinterpret_cast<uintptr_t>(mass) & (block_size % 4 == 0 ? 15 : 3)) == 0,
+                     "paged_chunk: mass must stand on a 16-byte boundary (with blocks of %d tokens)", block_size);
   ChunkParams p = {};
   // the stride of an axis of one is never used: give it the dense value, whatever the caller's is
   if (total_q == 1) q_stride_tok = out_stride_tok = (int64_t)n_q_heads * head_dim;

@@ -1,10 +1,13 @@
 """The bounded cache where its calls could go wrong.  Tolerances of accumulated weights are those of test_evict_gpu.py."""
+from types import SimpleNamespace
+
+import numpy as np
 import pytest
 import torch
 
 import snapmind_b200._lib as lib
 from test_chunk_gpu import DT, make_pool
-from test_evict_gpu import U, dense, reference_mass
+from test_evict_gpu import U, check_mass, dense, reference_mass
 
 pytestmark = pytest.mark.gpu
 
@@ -86,6 +89,50 @@ def test_copies_without_blocks(cache):
                 a = dense(pool, x[layer].view(torch.uint8), b, 100 - 10 * b)
                 z = dense(pool, x[layer].view(torch.uint8), 2 + b, 32)
                 assert torch.equal(z, torch.gather(a, 1, i.unsqueeze(-1).expand(-1, -1, a.shape[-1])))
+
+
+@pytest.mark.parametrize("dtype,cache,hq,hkv,d,bs,lens,new", [
+    # layers of a number of weights that is no multiple of 4
+    ("f32", "same", 2, 1, 40, 2, [30, 33], [5, 33]),
+    ("bf16", "same", 3, 1, 128, 5, [31, 12], [7, 2]),
+    ("bf16", "same", 3, 3, 64, 10, [31, 12], [7, 12]),
+    ("f16", "e4m3", 2, 1, 64, 3, [31, 12], [7, 2]),
+    ("f32", "same", 2, 1, 40, 2, [30, 33], None),
+    ("bf16", "same", 3, 1, 128, 5, [31, 12], None),
+    # what the kernels for larger blocks take
+    ("bf16", "same", 32, 8, 128, 16, [700, 129], [130, 1]),
+    ("bf16", "e4m3", 8, 2, 64, 32, [700, 129], [130, 1]),
+    ("bf16", "same", 32, 8, 128, 16, [700, 129], None),
+    ("f16", "e4m3", 8, 2, 128, 32, [700, 129], None),
+])
+def test_weights_of_a_later_layer(dtype, cache, hq, hkv, d, bs, lens, new):
+    pool, ks, _ = make_pool(DT[dtype], lens, hkv, d, bs, 11, cache, layers=3)
+    assert (pool.num_blocks * hkv * bs % 4 != 0) == (bs < 16)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    pool.mass = torch.rand((3, pool.num_blocks, hkv, bs), generator=g, device="cuda")
+    before = pool.mass.clone()
+    counts = new or [1] * len(lens)
+    q = torch.randn((sum(counts), hq, d), generator=g, device="cuda").to(DT[dtype])
+    if new is None:
+        pool.decode(2, q, accumulate=True)
+    else:
+        pool.attend_chunk(2, q, torch.tensor([0, *np.cumsum(new)], dtype=torch.int32, device="cuda"), accumulate=True)
+    pool.check()
+    assert torch.equal(pool.mass[:2], before[:2])
+    last = SimpleNamespace(mass=pool.mass[2:], block_size=bs, block_tables=pool.block_tables)
+    check_mass(last, before[2:], ks, q, counts, 0, 0, d ** -0.5)
+    # another layer's weights first: layer 1 on its own
+    pool.mass.copy_(before)
+    pool.k[1].view(torch.uint8).copy_(pool.k[2].view(torch.uint8))
+    pool.v[1].view(torch.uint8).copy_(pool.v[2].view(torch.uint8))
+    if cache == "e4m3":
+        pool.scales[1].copy_(pool.scales[2])
+    if new is None:
+        pool.decode(1, q, accumulate=True)
+    else:
+        pool.attend_chunk(1, q, torch.tensor([0, *np.cumsum(new)], dtype=torch.int32, device="cuda"), accumulate=True)
+    assert torch.equal(pool.mass[0], before[0]) and torch.equal(pool.mass[2], before[2])
+    check_mass(SimpleNamespace(mass=pool.mass[1:2], block_size=bs, block_tables=pool.block_tables), before[1:2], ks, q, counts, 0, 0, d ** -0.5)
 
 
 def test_new_tokens_after_an_error():
