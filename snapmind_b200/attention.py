@@ -142,15 +142,23 @@ class PagedGroupedQueryAttention(_AttentionBase):
             raise ValueError(f"gqa_paged: {pos.numel()} positions for {batch} x {n_tok} tokens")
         return pos.to(device=device, dtype=torch.int64).contiguous(), stride
 
+    def _norms_fit(self, q) -> bool:
+        """Whether the norms are what the kernels take: the rows' type (not f32 norms over bf16 rows, nor projections under
+        autocast) and device."""
+        return all(m.weight.dtype == q.dtype and m.weight.device == q.device for m in (self.q_norm, self.k_norm))
+
     def _place(self, q, k, position_ids, err: torch.Tensor):
         """Norm (with ``qk_norm_eps``) and rotate fresh projections ``[B, heads, T, D]``: by one kernel, in place, where
-        ``pe`` has the tables that it takes, else by the modules."""
+        ``pe`` has the tables that it takes, else by the modules (rounded to the rows' type, whatever the norms')."""
         tables = self._rope_tables(q) if self.pe is not None else None
-        if tables is not None:
-            (self._rope if self.q_norm is None else self._norm_rope)(q, k, position_ids, tables, err)
-            return q, k
         if self.q_norm is not None:
-            q, k = self.q_norm(q), self.k_norm(k)
+            if tables is not None and self._norms_fit(q):
+                self._norm_rope(q, k, position_ids, tables, err)
+                return q, k
+            q, k = self.q_norm(q).to(q.dtype), self.k_norm(k).to(k.dtype)
+        if tables is not None:
+            self._rope(q, k, position_ids, tables, err)
+            return q, k
         return (q, k) if self.pe is None else self.pe.apply_to_qk(q, k, position_ids)
 
     def _norm_rope(self, q, k, position_ids, tables, err: torch.Tensor) -> None:
@@ -261,7 +269,8 @@ class PagedGroupedQueryAttention(_AttentionBase):
         cu = None
         if n_new > 1 and (weighs or self.q_norm is not None):
             cu = torch.arange(0, (batch + 1) * n_new, n_new, dtype=torch.int32, device=x.device)
-        tables = self._rope_tables(q) if self.pe is not None and self.q_norm is not None else None
+        fused = self.pe is not None and self.q_norm is not None and self._norms_fit(q)
+        tables = self._rope_tables(q) if fused else None
         if tables is not None:  # norm, rotation and store in one pass
             pos, stride = self._positions(position_ids, batch, n_new, x.device)
             if pos is None:

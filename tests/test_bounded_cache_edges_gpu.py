@@ -4,8 +4,11 @@ from types import SimpleNamespace
 import numpy as np
 import pytest
 import torch
+import torch.nn as nn
 
 import snapmind_b200._lib as lib
+from llama_harness import Rope
+from test_budget_gpu import normed_attention, reference_layer
 from test_chunk_gpu import DT, make_pool
 from test_evict_gpu import U, check_mass, dense, reference_mass
 
@@ -171,3 +174,67 @@ def test_new_tokens_after_an_error():
         assert (m[:, 20:] == 0).all() and (m[:, :20] == 7).all()
     with pytest.raises(RuntimeError, match="out of blocks"):
         pool.check()
+
+
+class Normed(nn.Module):
+    """A projection whose heads are normalised by a module and brought back to the projection's type."""
+
+    def __init__(self, proj, norm, heads):
+        super().__init__()
+        self.proj, self.norm, self.heads = proj, norm, heads
+
+    def forward(self, x):
+        y = self.proj(x)
+        z = self.norm(y.view(*y.shape[:-1], self.heads, -1).transpose(1, 2)).to(y.dtype)
+        return z.transpose(1, 2).reshape(y.shape)
+
+
+@pytest.mark.parametrize("where", ["pool", "weighing pool", "cache", "none"])
+@pytest.mark.parametrize("rows,norms,auto", [
+    (torch.bfloat16, torch.float32, False), (torch.float32, torch.bfloat16, False), (torch.float32, torch.float32, True),
+    (torch.float16, torch.bfloat16, False),
+])
+@torch.no_grad()
+def test_norms_of_another_type(rows, norms, auto, where):
+    """Norms kept in another type than the projections' rows (or projections under autocast) are the modules' own, rounded to
+    the rows' type: the bits of a layer without norms whose projections end with them."""
+    from snapmind_b200 import PagedGroupedQueryAttention, PagedKVCache, PagedKVPool
+
+    torch.manual_seed(2)
+    rope = Rope(64, 128, 10000.0).cuda()
+    layer = normed_attention(d_model=256, n_heads=8, n_kv_heads=2, pe=rope, head_dim=64).cuda()
+    for m in (layer.q_norm, layer.k_norm):  # weights that every type holds
+        m.weight.copy_(1 + torch.randint(-8, 9, (64,)) / 32)
+    for m in (layer.q_proj, layer.k_proj, layer.v_proj, layer.out_proj):
+        m.to(rows)
+    layer.q_norm.to(norms), layer.k_norm.to(norms)
+    plain = PagedGroupedQueryAttention(d_model=256, n_heads=8, n_kv_heads=2, pe=rope, head_dim=64).cuda()
+    plain.q_proj, plain.k_proj = Normed(layer.q_proj, layer.q_norm, 8), Normed(layer.k_proj, layer.k_norm, 2)
+    plain.v_proj, plain.out_proj = layer.v_proj, layer.out_proj
+    x = torch.randn(1 if where in ("cache", "none") else 3, 40, 256, device="cuda").to(rows)
+    held = torch.bfloat16 if auto else rows
+    mask = torch.triu(torch.full((33, 33), -torch.inf), 1).cuda()
+    got = []
+    for m in (layer, plain):
+        with torch.autocast("cuda", torch.bfloat16, enabled=auto):
+            if where == "none":
+                got.append(m(x[:, :33], mask=mask)[0])
+                continue
+            if where == "cache":
+                view = PagedKVCache(64, 1, 2, 64, dtype=held, device="cuda").layer_dicts()[0]
+            else:
+                pool = PagedKVPool(1, 2, 64, 24, 3, 8, dtype=held, mass=where != "pool")
+                view = pool.layer_views(3)[0]
+                pool.reserve(33)
+            out = [m(x[:, :33], kv_cache=view, mask=mask)[0]]
+            for t in range(33, 40):
+                if where != "cache":
+                    pool.reserve(1)
+                out.append(m(x[:, t:t + 1], kv_cache=view, position_ids=torch.full((len(x),), t, device="cuda"))[0])
+            got.append(torch.cat(out, 1))
+            if where != "cache":
+                pool.check()
+    assert torch.equal(*got)
+    if rows == torch.float32 and not auto:  # and the formulas, as test_plugin_over_a_pool has them
+        want = reference_layer(layer, x[:, :got[0].shape[1]], rope)
+        assert (got[0].double() - want).abs().max() <= 2.0**-12 * want.abs().max()
