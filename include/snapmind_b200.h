@@ -620,8 +620,10 @@ SNAPMIND_API int snapmind_paged_gqa_chunk(const void *q, int64_t q_stride_tok, i
  * bits.  A query that sees nothing adds nothing; one whose softmax is NaN makes the tokens that it sees NaN.
  * q is read after out was written, so out must not be q.  The sequences must not share blocks, and calls that add
  * to the same layer must not overlap on the GPU.  The workspace holds
- * snapmind_paged_gqa_chunk_mass_workspace_bytes(...) bytes, on the terms of snapmind_paged_gqa_chunk's; `decodes` is
- * 1 for a call without cu_q (whose scores are kept).  The reference returns its weights (snapmind/layers/attention/gqa.py:79-85) but
+ * snapmind_paged_gqa_chunk_mass_workspace_bytes(...) bytes, on the terms of snapmind_paged_gqa_chunk's.  `decodes` 1 adds
+ * room for the scores of a call without cu_q (16-bit queries, head_dim 128, at most 8 query heads a kv head, blocks of 16, 32 or a
+ * multiple of 64 tokens), with num_blocks the pool's or batch * table_width, whichever is less; without that room the
+ * call reads K once more.  The reference returns its weights (snapmind/layers/attention/gqa.py:79-85) but
  * keeps no sums of them.
  */
 SNAPMIND_API int64_t snapmind_paged_gqa_chunk_mass_workspace_bytes(int32_t head_dim, int32_t total_q, int32_t n_q_heads,

@@ -597,15 +597,13 @@ int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st) {
 using namespace snapmind;
 
 static int64_t chunk_workspace_bytes(int32_t head_dim) { return partials_bytes(head_dim) + (max_ctas() * 4 + 255) / 256 * 256; }
+static int64_t scores_bytes(int64_t blocks, int32_t block_size, int32_t n_q_heads) { return blocks * block_size * n_q_heads * 4; }
 static int64_t stats_bytes(int32_t total_q, int32_t n_q_heads) { return ((int64_t)total_q * n_q_heads * 4 + 255) / 256 * 256; }
 
 // The attention of a call: the kernel that its shapes take, and the merge.
 static int launch_attention(ChunkParams& p, int dtype, int pool_dtype, int32_t flags, cudaStream_t st) {
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
-  float* scores = p.scores;  // there is room for them
-  p.scores = nullptr;
   if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && decode_sinks_supported(p, dtype, pool_dtype)) {
-    p.scores = scores;
     const int rc = launch_decode_sinks(p, dtype, pool_dtype, st);
     return rc != SNAPMIND_OK ? rc : launch_chunk_merge(p, dtype, st);
   }
@@ -642,7 +640,7 @@ int64_t snapmind_paged_gqa_chunk_mass_workspace_bytes(int32_t head_dim, int32_t 
                                                       int32_t decodes) {
   if (head_dim <= 0 || head_dim > kGenMaxD || total_q < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || block_size <= 0 || num_blocks <= 0)
     return 0;
-  const int64_t scores = decodes && decode_keeps_scores(head_dim, n_q_heads / n_kv_heads) ? (int64_t)num_blocks * block_size * n_q_heads * 4 : 0;
+  const int64_t scores = decodes && decode_keeps_scores(head_dim, n_q_heads / n_kv_heads) ? scores_bytes(num_blocks, block_size, n_q_heads) : 0;
   return chunk_workspace_bytes(head_dim) + stats_bytes(total_q, n_q_heads) + mass_workspace_bytes() + scores;
 }
 
@@ -712,7 +710,7 @@ int snapmind_paged_gqa_chunk_mass(const void* q, int64_t q_stride_tok, int64_t q
   }
   const int64_t attention = chunk_workspace_bytes(head_dim);
   const int64_t need = mass ? snapmind_paged_gqa_chunk_mass_workspace_bytes(head_dim, total_q, n_q_heads, n_kv_heads, block_size,
-                                                                            num_blocks, cu_q == nullptr)
+                                                                            num_blocks, 0)
                             : attention;
   SNAPMIND_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                      "paged_chunk: workspace needs %lld bytes on a 256-byte boundary, got %lld", (long long)need,
@@ -722,7 +720,14 @@ int snapmind_paged_gqa_chunk_mass(const void* q, int64_t q_stride_tok, int64_t q
   char* more = static_cast<char*>(workspace) + attention;  // the rows' statistics, then what the pass over the weights needs
   char* pass = more + stats_bytes(total_q, n_q_heads);
   p.stats = mass ? reinterpret_cast<float*>(more) : nullptr;
-  if (mass && cu_q == nullptr && decode_keeps_scores(head_dim, p.group)) p.scores = reinterpret_cast<float*>(pass + mass_workspace_bytes());
+  if (mass && !(flags & SNAPMIND_DECODE_FORCE_GENERIC) && decode_sinks_supported(p, dtype, pool_dtype)) {
+    // a decode keeps its scores where there is room for them, by sequence or by block, whichever is less
+    const int64_t rows = (int64_t)batch * table_width;
+    if (workspace_bytes >= need + scores_bytes(rows < num_blocks ? rows : num_blocks, block_size, n_q_heads)) {
+      p.scores = reinterpret_cast<float*>(pass + mass_workspace_bytes());
+      p.scores_room = rows < num_blocks ? (int32_t)room : 0;
+    }
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = launch_attention(p, dtype, pool_dtype, flags, st);
   if (rc != SNAPMIND_OK || !mass) return rc;

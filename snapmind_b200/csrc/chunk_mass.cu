@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) mass_scores_kernel(const __g
       if (phys < 0 || phys >= p.num_blocks) continue;
       const int64_t row = ((int64_t)phys * p.n_kv_heads + c.kvh) * p.block_size + (pos - j * p.block_size);
       float4* at = reinterpret_cast<float4*>(mass + row);
-      const float* from = p.scores + row * group;
+      const float* from = p.scores + (p.scores_room > 0 ? (int64_t)(c.b * p.n_kv_heads + c.kvh) * p.scores_room + v : row) * group;
       float4 m = *at;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
       if constexpr (G > 0) {

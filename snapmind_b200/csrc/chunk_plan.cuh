@@ -51,7 +51,8 @@ struct ChunkParams {
   int32_t* odd;     // workspace: [n_odd] whether a CTA met rows that its kernel's types do not hold, or NULL
   int32_t n_odd;
   int32_t means;    // part_o holds a piece's weighted means of V (else its weighted sums)
-  float* scores;    // [pool row][group] scores (log2 units) that a decode leaves for chunk_mass.cu, or NULL
+  float* scores;    // [score row][group] scores (log2 units) that a decode leaves for chunk_mass.cu, or NULL
+  int32_t scores_room;  // score row of a key: (sequence * kv heads + kv head) * scores_room + its place on the virtual axis; 0: its pool row
   float* stats;     // [n_kv_heads][total_q][group] -log2 of every row's softmax sum (of 2^score), or NULL
   int32_t* err;
 };
@@ -464,7 +465,7 @@ bool chunk_umma_supported(const ChunkParams& p, int dtype, int pool_dtype);
 int launch_chunk_umma(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st);
 bool decode_sinks_supported(const ChunkParams& p, int dtype, int pool_dtype);
 int launch_decode_sinks(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st);
-// Whether a call of such shapes may run on the decode kernel, which then leaves its scores.
+// Whether a call of such shapes may run on the decode kernel, which then leaves its scores (where there is room for them).
 inline bool decode_keeps_scores(int head_dim, int group) { return head_dim == 128 && group <= 8; }
 
 // Sets a kernel's shared-memory attributes once per device (`done` is the instantiation's own).

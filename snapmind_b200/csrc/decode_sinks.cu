@@ -60,7 +60,7 @@ struct Ctrl {
   float mr[kConsumers][kHeads];                          // R (16-bit caches: M)
   uint64_t full[N], empty[N];
   uint32_t have[N];  // parts of a stage's tile that were there to be copied
-  int32_t rows[N][kTile / 16];  // their pool rows (kScores)
+  int32_t rows[N][kTile / 16];  // their score rows (kScores)
   int32_t abort;
   PlanShared plan;
 };
@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (kv == 0 && leader) S.have[st] = have;
         if constexpr (kScores) {
           const int y = at.row(j, lane & (at.parts - 1));
-          if (kv == 0 && lane < at.parts) S.rows[st][lane] = y;
+          if (kv == 0 && lane < at.parts)
+            S.rows[st][lane] = p.scores_room > 0 ? (c.b * p.n_kv_heads + c.kvh) * p.scores_room + j * kTile + lane * box : y;
           __syncwarp();
         }
         mbar_arrive_expect_tx_p(leader, bar, __popc(have) * (uint32_t)box * row_bytes);

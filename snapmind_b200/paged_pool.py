@@ -390,8 +390,10 @@ class PagedKVPool(BlockPool):
         # captured graphs, never share one
         need, mass = self._chunk_ws, None
         if accumulate:
+            # a decode on the tensor cores keeps its scores: room for what its sequences, or the pool, can hold
+            keeps = cu is None and self.dtype != torch.float32 and not flags and (self.block_size in (16, 32) or self.block_size % 64 == 0)
             need = lib.snapmind_paged_gqa_chunk_mass_workspace_bytes(d, total, n_q, self.n_kv_heads, self.block_size,
-                                                                     self.num_blocks, cu is None)
+                                                                     min(self.num_blocks, max(1, total * self.max_blocks_per_seq)), keeps)
             mass = self.mass.data_ptr() + 4 * layer * self.num_blocks * self.n_kv_heads * self.block_size
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         step = layer * self.layer_stride * self.k.element_size()

@@ -238,3 +238,53 @@ def test_norms_of_another_type(rows, norms, auto, where):
     if rows == torch.float32 and not auto:  # and the formulas, as test_plugin_over_a_pool has them
         want = reference_layer(layer, x[:, :got[0].shape[1]], rope)
         assert (got[0].double() - want).abs().max() <= 2.0**-12 * want.abs().max()
+
+
+@pytest.mark.parametrize("dtype,cache,hq,seqs,bs,few", [
+    ("bf16", "same", 32, 4, 16, True), ("f16", "e4m3", 32, 4, 16, True), ("f32", "same", 32, 4, 16, True), ("bf16", "same", 32, 4, 8, True),
+    ("bf16", "same", 32, 64, 16, False),
+])
+def test_workspace_of_a_decode(dtype, cache, hq, seqs, bs, few):
+    """A decode that accumulates takes no more room than its own sequences' table rows, or the pool, have tokens for, and none
+    for scores that it does not keep."""
+    from snapmind_b200 import PagedKVPool, QuantizedKVPool
+
+    nb, width, d, batch = 40960 // bs * 4, 2048 // bs, 128, 2 if few else seqs
+    pool = (QuantizedKVPool if cache == "e4m3" else PagedKVPool)(1, 8, d, nb if few else seqs * 8, max_seqs=seqs, max_blocks_per_seq=width, block_size=bs,
+                                                               dtype=DT[dtype], mass=True)
+    pool.reserve(100)
+    q = torch.randn((batch, hq, d), device="cuda").to(DT[dtype])
+    pool.decode(0, q, accumulate=True)
+    size = lib.load().snapmind_paged_gqa_chunk_mass_workspace_bytes
+    base = size(d, batch, hq, 8, bs, pool.num_blocks, 0)
+    scores = min(batch * width, pool.num_blocks) * bs * hq * 4 if DT[dtype] != torch.float32 and bs == 16 else 0
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    pool.decode(0, q, accumulate=True)
+    assert torch.cuda.max_memory_allocated() - held <= base + scores + (4 << 20)  # outputs, and what the allocator does not split off
+    pool.check()
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dtype,cache,hq,hkv,bs,window,sinks", [
+    ("bf16", "same", 32, 8, 16, 0, 0), ("f16", "e4m3", 8, 2, 32, 0, 0), ("bf16", "same", 5, 5, 64, 300, 20), ("bf16", "e4m3", 14, 2, 128, 200, 130),
+])
+def test_scores_by_sequence_and_by_block(dtype, cache, hq, hkv, bs, window, sinks, wide):
+    """Decodes of a few of a pool's sequences, and of all that a pool with long table rows holds."""
+    lens = [900, 1, 401, 64, 777]
+    pool, ks, _ = make_pool(DT[dtype], lens, hkv, 128, bs, 13, cache, spare=0 if wide else 400)
+    batch = 5 if wide else 2
+    assert (batch * pool.max_blocks_per_seq > pool.num_blocks) == wide
+    g = torch.Generator(device="cuda").manual_seed(4)
+    pool.mass = torch.rand((1, pool.num_blocks, hkv, bs), generator=g, device="cuda")
+    before = pool.mass.clone()
+    q = torch.randn((batch, hq, 128), generator=g, device="cuda").to(DT[dtype])
+    pool.decode(0, q, accumulate=True, window=window, sinks=sinks)
+    pool.check()
+    check_mass(pool, before, ks[:batch], q, [1] * batch, window, sinks, 128 ** -0.5)
+    first = pool.mass.clone()
+    pool.mass.copy_(before)
+    pool.decode(0, q, accumulate=True, window=window, sinks=sinks)
+    assert torch.equal(pool.mass, first)
