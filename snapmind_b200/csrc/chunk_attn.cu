@@ -80,7 +80,8 @@ __device__ __forceinline__ bool out_vec(const ChunkParams& p) {
 }
 
 // p.odd: a second go at a call of the tcgen05 kernel, which only some CTA's odd rows make necessary.
-template <typename T, typename KV, int D4>
+// kStats: the rows' softmax sums go to p.stats (a branch on that pointer cost the f32 prompts 1.7%).
+template <typename T, typename KV, int D4, bool kStats>
 __global__ void __launch_bounds__(GenSmem<D4>::kThreads, GenSmem<D4>::kCtas) chunk_generic_kernel(ChunkParams p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   using Smem = GenSmem<D4>;
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(GenSmem<D4>::kThreads, GenSmem<D4>::kCtas) chu
         p.part_ml[slot * 2] = m[i];
         p.part_ml[slot * 2 + 1] = l[i];
       }
-      if (whole && tx == 0) write_stats(p, c.q_first + c.i0 + tok, head0 + g, m[i], l[i]);
+      if (kStats && whole && tx == 0) write_stats(p, c.q_first + c.i0 + tok, head0 + g, m[i], l[i]);
 #pragma unroll
       for (int j = 0; j < kX; ++j) {
         const float4 y = make_float4(o[i][2 * j].x * f, o[i][2 * j].y * f, o[i][2 * j + 1].x * f, o[i][2 * j + 1].y * f);
@@ -533,7 +534,7 @@ dim3 merge_grid(const ChunkParams& p) {
   return dim3(p.n_ctas - 1, (used + kMergeWarps * kMergeRows - 1) / (kMergeWarps * kMergeRows));
 }
 
-template <typename T, typename KV>
+template <typename T, typename KV, bool kStats>
 int launch_generic(const ChunkParams& p, cudaStream_t st) {
   const auto go = [&](auto kernel, int threads, size_t smem, bool (&done)[kMaxDevices]) -> int {
     const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem, done);
@@ -543,9 +544,13 @@ int launch_generic(const ChunkParams& p, cudaStream_t st) {
   static bool done[3][kMaxDevices] = {};
   static_assert(sizeof(GenSmem<4>) <= 232448, "shared memory budget");
   static_assert(sizeof(GenSmem<1>().q) + sizeof(GenSmem<1>().k) >= kMaxChunkBatch * 4, "plan scratch");
-  if (p.head_dim <= 64) return go(chunk_generic_kernel<T, KV, 1>, GenSmem<1>::kThreads, sizeof(GenSmem<1>), done[0]);
-  if (p.head_dim <= 128) return go(chunk_generic_kernel<T, KV, 2>, GenSmem<2>::kThreads, sizeof(GenSmem<2>), done[1]);
-  return go(chunk_generic_kernel<T, KV, 4>, GenSmem<4>::kThreads, sizeof(GenSmem<4>), done[2]);
+  if (p.head_dim <= 64) return go(chunk_generic_kernel<T, KV, 1, kStats>, GenSmem<1>::kThreads, sizeof(GenSmem<1>), done[0]);
+  if (p.head_dim <= 128) return go(chunk_generic_kernel<T, KV, 2, kStats>, GenSmem<2>::kThreads, sizeof(GenSmem<2>), done[1]);
+  return go(chunk_generic_kernel<T, KV, 4, kStats>, GenSmem<4>::kThreads, sizeof(GenSmem<4>), done[2]);
+}
+template <typename T, typename KV>
+int launch_generic(const ChunkParams& p, cudaStream_t st) {
+  return p.stats ? launch_generic<T, KV, true>(p, st) : launch_generic<T, KV, false>(p, st);
 }
 
 int plan_generic(ChunkParams& p) {
