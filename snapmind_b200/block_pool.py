@@ -29,7 +29,8 @@ class BlockPool:
         self.num_blocks, self.max_seqs, self.block_size = num_blocks, max_seqs, block_size
         self.max_blocks_per_seq = max_blocks_per_seq
         self.block_tables = torch.zeros((max_seqs, max_blocks_per_seq), dtype=torch.int32, device=self.device)
-        self._index = self.block_tables.device.index
+        self._device = self.block_tables.device  # with its index
+        self._index = self._device.index
         self.seq_lens = torch.zeros(max_seqs, dtype=torch.int32, device=self.device)
         # free_stack[top-1] is popped first; initially block 0, then 1, ...
         self.free_stack = torch.arange(num_blocks - 1, -1, -1, dtype=torch.int32, device=self.device)
@@ -44,7 +45,7 @@ class BlockPool:
 
     def _on_device(self):
         """Context in which the pool's device is the current one (kernels launch on its stream)."""
-        return _NOTHING if torch.cuda.current_device() == self._index else torch.cuda.device(self._index)
+        return _NOTHING if torch._C._cuda_getDevice() == self._index else torch.cuda.device(self._index)
 
     @property
     def host_lens(self) -> np.ndarray:

@@ -80,8 +80,9 @@ __device__ inline void mass_plan(const MassParams& mp, MassShared& S, int32_t* t
     if (lane == 0) tiles[b] = s * p.n_slices;
   }
   __syncthreads();
-  line_share(p, S.line, tiles, p.n_kv_heads);
-  if (warp == 0 && S.line.t0 < S.line.t1) {
+  long long t0, t1;
+  line_share(p, S.line, tiles, p.n_kv_heads, t0, t1);
+  if (warp == 0 && t0 < t1) {
     MassPiece f;
     f.b = S.line.b;
     f.kvh = (int)(S.line.rem / S.line.u);
@@ -111,7 +112,7 @@ __device__ inline void mass_plan(const MassParams& mp, MassShared& S, int32_t* t
       }
       rem -= __shfl_sync(0xffffffffu, x, 31);
     }
-    f.s1 = (int)min((long long)f.steps, f.s0 + (S.line.t1 - S.line.t0));
+    f.s1 = (int)min((long long)f.steps, f.s0 + (t1 - t0));
     if (lane == 0) S.first = f;
   }
   __syncthreads();

@@ -151,13 +151,14 @@ __device__ __forceinline__ int cta_of(long long t, long long total, int n) {
 
 // Where this CTA's share of a line begins and ends, with per_head units' worth of tiles[b] tiles for
 // every sequence: fills S (total, n, t0, t1 and, if the share holds a tile, b, u, rem).  Every thread of the block
-// calls it, with tiles[] visible; what warp 0 reads of S it may read at once, the others after a barrier.
-__device__ inline void line_share(const ChunkParams& p, PlanShared& S, const int32_t* tiles, int per_head) {
+// calls it, with tiles[] visible; what warp 0 reads of S it may read at once, the others after a barrier.  t0 and t1 also
+// in registers.
+__device__ __forceinline__ void line_share(const ChunkParams& p, PlanShared& S, const int32_t* tiles, int per_head, long long& t0,
+                                           long long& t1) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
   // Up to kWarpBatch sequences: every warp goes over them, 32 a step (no barrier, the last step finds the
   // place); more: one run of sequences per thread and a scan over the block.
   constexpr int kWarpBatch = 256;
-  long long t0, t1;
   if (p.batch <= kWarpBatch) {
     int sum = 0;
     for (int b = lane; b < p.batch; b += 32) sum += tiles[b];
@@ -255,8 +256,9 @@ __device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* 
     }
   }
   __syncthreads();
-  line_share(p, S, tiles, per_head);
-  if (warp == 0 && S.t0 < S.t1) {
+  long long t0, t1;
+  line_share(p, S, tiles, per_head, t0, t1);
+  if (warp == 0 && t0 < t1) {
     Piece f;
     f.b = S.b;
     int hs = (int)__fdividef((float)S.rem, (float)S.u);  // off by one at most: hs is small
@@ -290,7 +292,7 @@ __device__ inline void plan_block(const ChunkParams& p, PlanShared& S, int32_t* 
       }
       rem -= __shfl_sync(0xffffffffu, x, 31);
     }
-    f.tile1 = (int)min((long long)f.n_tiles, f.tile0 + (S.t1 - S.t0));
+    f.tile1 = (int)min((long long)f.n_tiles, f.tile0 + (t1 - t0));
     if (lane == 0) S.first = f;
   }
   __syncthreads();
@@ -436,7 +438,6 @@ __device__ inline void write_piece_info(const ChunkParams& p, const PlanShared& 
 // A finished row's softmax (M, sum of 2^(score - M)), for the kernels that add its weights to their keys (chunk_mass.cu):
 // the weight of a key is 2^(score + x).  A row that sees nothing: -infinity.
 __device__ __forceinline__ void write_stats(const ChunkParams& p, int64_t row, int head, float M, float L) {
-  if (p.stats == nullptr) return;
   const int kvh = head / p.group;
   p.stats[(kvh * (int64_t)p.total_q + row) * p.group + (head - kvh * p.group)] = L == 0.f ? -INFINITY : -((M == -INFINITY ? 0.f : M) + log2f(L));
 }

@@ -112,8 +112,8 @@ __device__ __forceinline__ bool consumers_any(bool v) {
   return r != 0;
 }
 
-// kScores: the scores of the tokens go to p.scores too, for the pass that adds their weights up (128 sequences of 1 to 8
-// thousand tokens: 3% more bytes than the decode without).
+// kScores: the rows' softmax sums go to p.stats, and the scores of the tokens to p.scores where there is room for them, for
+// the pass that adds their weights up (128 sequences of 1 to 8 thousand tokens: 3% more bytes than the decode without).
 template <typename T, bool kQuant, bool kScores>
 __global__ void __launch_bounds__(kThreads, 2)
     decode_sinks_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, ChunkParams p) {
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               mma16816<kMmaBf16>(sc, a, qf[k][0], qf[k][1]);
             }
           }
-          if constexpr (kScores) {
+          if (kScores && p.scores != nullptr) {
             // a key's scores side by side: 16 bytes for four heads (rows past the last token, unseen ones: never read)
             const int64_t row = S.rows[st][part] + 16 * warp - part * p.block_size;
 #pragma unroll
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * half * half;
         }
         if (c.whole()) {
-          if (d == 0) write_stats(p, c.q_first, head0 + h, M, L);
+          if (kScores && d == 0) write_stats(p, c.q_first, head0 + h, M, L);
           if constexpr (!kQuant)
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] *= inv;
@@ -603,7 +603,7 @@ int launch_decode_sinks(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t 
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
   const auto go = [&](auto t) -> int {
     using T = decltype(t);
-    if (p.scores != nullptr) return quant ? launch<T, true, true>(p, st) : launch<T, false, true>(p, st);
+    if (p.stats != nullptr) return quant ? launch<T, true, true>(p, st) : launch<T, false, true>(p, st);
     return quant ? launch<T, true, false>(p, st) : launch<T, false, false>(p, st);
   };
   return dtype == SNAPMIND_DTYPE_BF16 ? go(__nv_bfloat16()) : go(__half());

@@ -380,7 +380,8 @@ class PagedKVPool(BlockPool):
             if (accumulate or (self.quantised and self.dtype == torch.float16)) and _share(q, out):
                 q = q.clone()  # such a call may be done over, or takes the scores anew, with the queries it began with
                 q_st = q.stride()
-        _lib.require_same("attend", self.block_tables, q, out)
+        if q.device != self._device or out.device != self._device:
+            _lib.require_same("attend", self.block_tables, q, out)
         if append is not None:
             self.append(layer, *append)
         if not (-1 <= window <= _FAR and -1 <= sinks <= _FAR):  # the C entry takes 32 bits
@@ -395,7 +396,7 @@ class PagedKVPool(BlockPool):
             need = lib.snapmind_paged_gqa_chunk_mass_workspace_bytes(d, total, n_q, self.n_kv_heads, self.block_size,
                                                                      min(self.num_blocks, max(1, total * self.max_blocks_per_seq)), keeps)
             mass = self.mass.data_ptr() + 4 * layer * self.num_blocks * self.n_kv_heads * self.block_size
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = torch.empty(need, dtype=torch.uint8, device=self._device)
         step = layer * self.layer_stride * self.k.element_size()
         scales = self.scales.data_ptr() + layer * self.scale_layer_stride if self.quantised else None
         with self._on_device():

@@ -288,3 +288,28 @@ def test_scores_by_sequence_and_by_block(dtype, cache, hq, hkv, bs, window, sink
     pool.mass.copy_(before)
     pool.decode(0, q, accumulate=True, window=window, sinks=sinks)
     assert torch.equal(pool.mass, first)
+
+
+@pytest.mark.parametrize("dtype,cache", [("bf16", "same"), ("f16", "e4m3")])
+def test_a_decode_without_room_for_scores(dtype, cache):
+    """The C entry with the workspace of a call that keeps none: the same output, and the weights from K."""
+    lens = [900, 1, 401]
+    pool, ks, _ = make_pool(DT[dtype], lens, 2, 128, 16, 19, cache)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    pool.mass = torch.rand((1, pool.num_blocks, 2, 16), generator=g, device="cuda")
+    before = pool.mass.clone()
+    q = torch.randn((3, 8, 128), generator=g, device="cuda").to(DT[dtype])
+    want = pool.decode(0, q, accumulate=True)
+    pool.mass.copy_(before)
+    need = lib.load().snapmind_paged_gqa_chunk_mass_workspace_bytes(128, 3, 8, 2, 16, pool.num_blocks, 0)
+    ws, out, width = torch.empty(need, dtype=torch.uint8, device="cuda"), torch.empty_like(q), pool.max_blocks_per_seq
+    args = (q.data_ptr(), 8 * 128, 128, lib.dtype_code(q.dtype), pool.k.data_ptr(), pool.v.data_ptr(),
+            pool.scales.data_ptr() if cache == "e4m3" else None, lib.DTYPE_E4M3 if cache == "e4m3" else lib.dtype_code(q.dtype),
+            pool.block_tables.data_ptr(), width, width, pool.seq_lens.data_ptr(), None, out.data_ptr(), 8 * 128, 128, 128 ** -0.5, 3, 3, 8, 2,
+            128, 16, pool.num_blocks, 0, 0, 0, pool.mass.data_ptr(), ws.data_ptr())
+    call = lib.load().snapmind_paged_gqa_chunk_mass
+    assert call(*args, need, pool.err.data_ptr(), lib.stream_handle(torch.device("cuda"))) == lib.OK
+    pool.check()
+    assert torch.equal(out, want)
+    check_mass(pool, before, ks, q, [1] * 3, 0, 0, 128 ** -0.5)
+    assert call(*args, need - 1, pool.err.data_ptr(), lib.stream_handle(torch.device("cuda"))) == lib.ERR_BAD_ARGUMENT
