@@ -290,6 +290,28 @@ def test_scores_by_sequence_and_by_block(dtype, cache, hq, hkv, bs, window, sink
     assert torch.equal(pool.mass, first)
 
 
+@pytest.mark.parametrize("dtype,cache,hq,hkv,d,bs,decode", [
+    ("bf16", "same", 8, 2, 128, 16, True), ("bf16", "e4m3", 8, 2, 128, 16, True), ("bf16", "same", 8, 2, 128, 16, False),
+    ("f16", "e4m3", 6, 2, 64, 16, False), ("f32", "same", 4, 2, 64, 16, False), ("f32", "same", 4, 2, 64, 16, True),
+])
+def test_many_sequences(dtype, cache, hq, hkv, d, bs, decode):
+    """More sequences than a warp goes over when it plans."""
+    rng = np.random.RandomState(5)
+    lens = [int(x) for x in rng.randint(0, 200, 400)]
+    new = [1] * 400 if decode else [int(min(n, rng.randint(0, 9))) for n in lens]
+    pool, ks, _ = make_pool(DT[dtype], lens, hkv, d, bs, 17, cache)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    pool.mass = torch.rand((1, pool.num_blocks, hkv, bs), generator=g, device="cuda")
+    before = pool.mass.clone()
+    q = torch.randn((sum(new), hq, d), generator=g, device="cuda").to(DT[dtype])
+    if decode:
+        pool.decode(0, q, accumulate=True)
+    else:
+        pool.attend_chunk(0, q, torch.tensor([0, *np.cumsum(new)], dtype=torch.int32, device="cuda"), accumulate=True)
+    pool.check()
+    check_mass(pool, before, ks, q, new, 0, 0, d ** -0.5)
+
+
 @pytest.mark.parametrize("dtype,cache", [("bf16", "same"), ("f16", "e4m3")])
 def test_a_decode_without_room_for_scores(dtype, cache):
     """The C entry with the workspace of a call that keeps none: the same output, and the weights from K."""
