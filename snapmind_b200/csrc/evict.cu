@@ -542,7 +542,9 @@ int snapmind_kv_evict_by_mass(void* k_pool, void* v_pool, void* scales, int pool
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (into) evict_tables_kernel<<<1, kTableThreads, 0, st>>>(p);
   // Sequences of up to 4096 tokens: 256 threads (4 blocks an SM), up to 16384: 512, above: 1024, each with room for
-  // that many weights (above: 49152 at a time).
+  // that many weights (above: 49152 at a time).  Calls that keep 256 rows of 16 bytes, us with 256 / 512 / 1024 threads: 1024 units
+  // of 4096 tokens 66 / 76 / 104, of 8192 90 / 97 / 128 (16 units: 39 / 35 / 35), 512 units of 16384 109 / 87 / 104, 256
+  // units of 17000 66 / 55 / 64, of 32768 158 / 100 / 85.
   const int64_t room = (int64_t)table_width * block_size, longest = max_len > 0 && max_len < room ? max_len : room;
   const auto select = [&](auto kernel, int threads, bool (&done)[64]) -> cudaError_t {
     const int64_t step = 4 * (int64_t)threads;

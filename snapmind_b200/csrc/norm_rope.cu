@@ -110,9 +110,11 @@ __device__ __forceinline__ void store4(T* x, float2 a, float2 b) {
 // elements each: a lane of the rotated part four and the four that they turn with, so nothing is exchanged but the
 // sum of squares, and a token's cosines and sines serve kHeads rows.  Where tokens come from and go to (positions,
 // sequences, lengths, table entries: reads that wait for one another) is worked out for all of a CTA's tokens at
-// once, and the next item's rows, cosines and sines are on their way while one is computed.  What bounds it beside HBM
-// is the number of instructions: 8200 tokens of 48 heads of 128 (bf16) took 70 us with 219 a row and warp (64-bit
-// addresses, partners by shuffles), 79 with 178 and cosines that a row waited for, 41 us (4.6 TB/s) with 115.
+// once, and the next item's rows, cosines and sines are on their way while one is computed.  Fewer instructions
+// made it fast: 8200 tokens of 48 heads of 128 (bf16) took 70 us with 219 a row and warp (64-bit
+// addresses, partners by shuffles), 79 with 178 and cosines that a row waited for, 41 us (4.6 TB/s) with 115.  Now
+// neither they (56% of the issue slots; into 8-bit rows 53%) nor HBM (41%; 25%) are full, at 16 warps an SM and one item
+// ahead.
 struct Rows32 { int32_t seq, head, tok, out_seq, out_head, out_tok; };  // RowSet's strides where they fit
 struct Split {
   Rows32 at[3];        // q, k, v
