@@ -82,7 +82,7 @@ __device__ __forceinline__ bool out_vec(const ChunkParams& p) {
 // p.odd: a second go at a call of the tcgen05 kernel, which only some CTA's odd rows make necessary.
 // kStats: the rows' softmax sums go to p.stats (a branch on that pointer cost the f32 prompts 1.7%).
 template <typename T, typename KV, int D4, bool kStats>
-__global__ void __launch_bounds__(GenSmem<D4>::kThreads, GenSmem<D4>::kCtas) chunk_generic_kernel(ChunkParams p) {
+__global__ void __launch_bounds__(GenSmem<D4>::kThreads, GenSmem<D4>::kCtas) chunk_generic_kernel(CallParams<kStats> p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   using Smem = GenSmem<D4>;
   constexpr int P = Smem::P, PS = Smem::PS, D = Smem::D, kTx = Smem::kTx, kJ = Smem::kJ, kX = Smem::kX;
@@ -336,7 +336,8 @@ __global__ void __launch_bounds__(GenSmem<D4>::kThreads, GenSmem<D4>::kCtas) chu
         p.part_ml[slot * 2] = m[i];
         p.part_ml[slot * 2 + 1] = l[i];
       }
-      if (kStats && whole && tx == 0) write_stats(p, c.q_first + c.i0 + tok, head0 + g, m[i], l[i]);
+      if constexpr (kStats)
+        if (whole && tx == 0) write_stats(p, c.q_first + c.i0 + tok, head0 + g, m[i], l[i]);
 #pragma unroll
       for (int j = 0; j < kX; ++j) {
         const float4 y = make_float4(o[i][2 * j].x * f, o[i][2 * j].y * f, o[i][2 * j + 1].x * f, o[i][2 * j + 1].y * f);
@@ -386,7 +387,7 @@ __device__ __forceinline__ void mul4(float4& a, float f) {
 
 // kStats: the rows' softmax sums go to p.stats.
 template <typename T, bool kStats>
-__device__ __forceinline__ void merge_units(const ChunkParams& p) {
+__device__ __forceinline__ void merge_units(const CallParams<kStats>& p) {
   const int cta = blockIdx.x + 1;
   if (cta >= p.n_ctas) return;
   const int4 h0 = *reinterpret_cast<const int4*>(p.heads + (int64_t)cta * kPieceInts);
@@ -427,9 +428,9 @@ __device__ __forceinline__ void merge_units(const ChunkParams& p) {
       float f = ml.x == -INFINITY ? ml.y : ex2(ml.x - ref), L = ml.y * f;
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-      if (kStats && il == 0 && rl < n_rows) {
+      if constexpr (kStats) {
         const int tok = p.by_gw.div(rl), g = rl - tok * p.gw;
-        if (g < heads) write_stats(p, first + i0 + tok, kvh * p.group + slice * p.gw + g, M, L);
+        if (il == 0 && rl < n_rows && g < heads) write_stats(p, first + i0 + tok, kvh * p.group + slice * p.gw + g, M, L);
       }
       f *= L == 0.f ? 0.f : 1.f / L;  // a row that sees nothing: zeros
       if (p.means) f *= ml.y;
@@ -504,7 +505,8 @@ __device__ __forceinline__ void merge_units(const ChunkParams& p) {
       }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    if (kStats && lane == 0) write_stats(p, first + i0 + p.by_gw.div(r), kvh * p.group + slice * p.gw + g, M, L);
+    if constexpr (kStats)
+      if (lane == 0) write_stats(p, first + i0 + p.by_gw.div(r), kvh * p.group + slice * p.gw + g, M, L);
     mul4(acc[0], inv);
     mul4(acc[1], inv);
     T* out = out_row(r, g);
@@ -514,7 +516,7 @@ __device__ __forceinline__ void merge_units(const ChunkParams& p) {
 }
 
 template <typename T, bool kStats>
-__global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkParams p) {
+__global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(CallParams<kStats> p) {
   next_grid_may_launch();  // every block of this grid has started by then
   prior_grid_wait();
   merge_units<T, kStats>(p);
@@ -522,7 +524,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) chunk_merge_kernel(ChunkPara
 // After a call that may have been done over: `again` merges the units of that.
 template <typename T, bool kStats>
 __global__ void __launch_bounds__(32 * kMergeWarps)
-    chunk_merge_either_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ ChunkParams again) {
+    chunk_merge_either_kernel(const __grid_constant__ CallParams<kStats> p, const __grid_constant__ CallParams<kStats> again) {
   next_grid_may_launch();
   prior_grid_wait();
   if (any_odd(again)) merge_units<T, kStats>(again);
@@ -535,7 +537,7 @@ dim3 merge_grid(const ChunkParams& p) {
 }
 
 template <typename T, typename KV, bool kStats>
-int launch_generic(const ChunkParams& p, cudaStream_t st) {
+int launch_generic(const WeighedParams& p, cudaStream_t st) {
   const auto go = [&](auto kernel, int threads, size_t smem, bool (&done)[kMaxDevices]) -> int {
     const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem, done);
     if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
@@ -549,7 +551,7 @@ int launch_generic(const ChunkParams& p, cudaStream_t st) {
   return go(chunk_generic_kernel<T, KV, 4, kStats>, GenSmem<4>::kThreads, sizeof(GenSmem<4>), done[2]);
 }
 template <typename T, typename KV>
-int launch_generic(const ChunkParams& p, cudaStream_t st) {
+int launch_generic(const WeighedParams& p, cudaStream_t st) {
   return p.stats ? launch_generic<T, KV, true>(p, st) : launch_generic<T, KV, false>(p, st);
 }
 
@@ -559,8 +561,8 @@ int plan_generic(ChunkParams& p) {
 
 // The tcgen05 kernel, then the CUDA-core kernel over the same call, which returns at once unless a
 // CTA of the first met rows that f16 does not hold, then one merge for both.
-int launch_f16_over_e4m3(ChunkParams& p, cudaStream_t st) {
-  ChunkParams again = p;
+int launch_f16_over_e4m3(WeighedParams& p, cudaStream_t st) {
+  WeighedParams again = p;
   int rc = plan_generic(again);
   if (rc == SNAPMIND_OK) rc = launch_chunk_umma(p, SNAPMIND_DTYPE_F16, SNAPMIND_DTYPE_E4M3, st);
   if (rc != SNAPMIND_OK) return rc;
@@ -568,9 +570,11 @@ int launch_f16_over_e4m3(ChunkParams& p, cudaStream_t st) {
   rc = launch_generic<__half, uint8_t>(again, st);
   if (rc != SNAPMIND_OK) return rc;
   const dim3 a = merge_grid(p), b = merge_grid(again);
-  const auto kernel = p.stats ? chunk_merge_either_kernel<__half, true> : chunk_merge_either_kernel<__half, false>;
-  return cuda_status(launch_dependent(kernel, dim3(a.x > b.x ? a.x : b.x, a.y > b.y ? a.y : b.y), 32 * kMergeWarps, 0, st, p, again),
-                     "paged_chunk merge");
+  const auto go = [&](auto kernel) {
+    return cuda_status(launch_dependent(kernel, dim3(a.x > b.x ? a.x : b.x, a.y > b.y ? a.y : b.y), 32 * kMergeWarps, 0, st, p, again),
+                       "paged_chunk merge");
+  };
+  return p.stats ? go(chunk_merge_either_kernel<__half, true>) : go(chunk_merge_either_kernel<__half, false>);
 }
 
 // The largest workspace of the kernels: one CTA per SM with units of 256 rows, or three with 64.
@@ -585,7 +589,7 @@ int64_t partials_bytes(int head_dim) {
 
 }  // namespace
 
-int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st) {
+int launch_chunk_merge(const WeighedParams& p, int dtype, cudaStream_t st) {
   if (p.n_ctas < 2) return SNAPMIND_OK;
   const auto go = [&](auto kernel) {
     return cuda_status(launch_dependent(kernel, merge_grid(p), 32 * kMergeWarps, 0, st, p), "paged_chunk merge");
@@ -606,7 +610,7 @@ static int64_t scores_bytes(int64_t blocks, int32_t block_size, int32_t n_q_head
 static int64_t stats_bytes(int32_t total_q, int32_t n_q_heads) { return ((int64_t)total_q * n_q_heads * 4 + 255) / 256 * 256; }
 
 // The attention of a call: the kernel that its shapes take, and the merge.
-static int launch_attention(ChunkParams& p, int dtype, int pool_dtype, int32_t flags, cudaStream_t st) {
+static int launch_attention(WeighedParams& p, int dtype, int pool_dtype, int32_t flags, cudaStream_t st) {
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
   if (!(flags & SNAPMIND_DECODE_FORCE_GENERIC) && decode_sinks_supported(p, dtype, pool_dtype)) {
     const int rc = launch_decode_sinks(p, dtype, pool_dtype, st);
@@ -677,7 +681,7 @@ int snapmind_paged_gqa_chunk_mass(const void* q, int64_t q_stride_tok, int64_t q
   // may stand on any float
   SNAPMIND_CHECK_ARG((reinterpret_cast<uintptr_t>(mass) & (block_size % 4 == 0 ? 15 : 3)) == 0,
                      "paged_chunk: mass must stand on a 16-byte boundary (with blocks of %d tokens)", block_size);
-  ChunkParams p = {};
+  WeighedParams p = {};
   // the stride of an axis of one is never used: give it the dense value, whatever the caller's is
   if (total_q == 1) q_stride_tok = out_stride_tok = (int64_t)n_q_heads * head_dim;
   if (n_q_heads == 1) q_stride_head = out_stride_head = head_dim;

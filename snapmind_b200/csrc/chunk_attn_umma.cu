@@ -279,9 +279,6 @@ __device__ __forceinline__ bool odd_row(int kv, const uint4& codes, const uint4&
   return (top & 0x80008000u) != 0;
 }
 
-// Out of line: instructions that most calls do not need.
-__device__ __noinline__ void stats_of(const ChunkParams& p, int row, int head, float m, float l) { write_stats(p, row, head, m, l); }
-
 // The third warpgroup (e4m3: and the fourth) gives up registers that the softmax threads, with a row
 // of 128 scores each, need: 3 x 128 threads are launched with 168 each, 4 x 128 with 128.
 template <bool kQuant> struct Roles {
@@ -293,10 +290,11 @@ template <bool kQuant> struct Roles {
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
-template <typename T, int D, bool kQuant>
+// kStats: the rows' softmax sums go to p.stats.
+template <typename T, int D, bool kQuant, bool kStats>
 __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
     chunk_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                      const __grid_constant__ CUtensorMap v_map, const __grid_constant__ ChunkParams p) {
+                      const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CallParams<kStats> p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using Sh = Shape<D, kQuant>;
@@ -778,7 +776,8 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
         p.part_ml[slot * 2] = m;
         p.part_ml[slot * 2 + 1] = l;
       }
-      if (p.stats != nullptr && whole && mine) stats_of(p, c.q_first + c.i0 + tok, c.kvh * p.group + c.slice * p.gw + g, m, l);
+      if constexpr (kStats)
+        if (whole && mine) write_stats(p, c.q_first + c.i0 + tok, c.kvh * p.group + c.slice * p.gw + g, m, l);
       if (whole) {  // sees nothing: zeros
         const float inv = l == 0.f ? 0.f : 1.f / l;
         f *= inv;
@@ -846,8 +845,8 @@ bool q_tiles_map(CUtensorMap* map, bool bf16, const ChunkParams& p, int D) {
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D, bool kQuant>
-int launch(const ChunkParams& p, cudaStream_t st) {
+template <typename T, int D, bool kQuant, bool kStats>
+int launch(const WeighedParams& p, cudaStream_t st) {
   CUtensorMap q_map, k_map, v_map;
   const uint64_t rows = (uint64_t)p.num_blocks * p.n_kv_heads * p.block_size;
   const uint32_t box = p.block_size < kKeys ? p.block_size : kKeys;
@@ -856,7 +855,7 @@ int launch(const ChunkParams& p, cudaStream_t st) {
                              : tensor_map_row_groups(&k_map, bf16, p.k_pool, rows, D, box / 8) &&
                                    tensor_map_row_groups(&v_map, bf16, p.v_pool, rows, D, box / 8);
   if (!mapped || !q_tiles_map(&q_map, bf16, p, D)) return SNAPMIND_ERR_UNSUPPORTED;  // the caller takes the CUDA-core kernel
-  auto kernel = chunk_umma_kernel<T, D, kQuant>;
+  auto kernel = chunk_umma_kernel<T, D, kQuant, kStats>;
   static bool done[kMaxDevices] = {};
   const cudaError_t e = kernel_attributes(reinterpret_cast<const void*>(kernel), smem_bytes<D, kQuant>(), done);
   if (e != cudaSuccess) return cuda_status(e, "paged_chunk smem attribute");
@@ -883,14 +882,18 @@ bool chunk_umma_supported(const ChunkParams& p, int dtype, int pool_dtype) {
   return encode_tiled() != nullptr;
 }
 
-int launch_chunk_umma(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st) {
+int launch_chunk_umma(WeighedParams& p, int dtype, int pool_dtype, cudaStream_t st) {
   const int rc = plan_geometry(p, 2 * kTileM, kTileM, kKeys, num_sms());
   if (rc != SNAPMIND_OK) return rc;
   const bool quant = pool_dtype == SNAPMIND_DTYPE_E4M3;
   const auto go = [&](auto t) -> int {
     using T = decltype(t);
-    if (p.head_dim == 64) return quant ? launch<T, 64, true>(p, st) : launch<T, 64, false>(p, st);
-    return quant ? launch<T, 128, true>(p, st) : launch<T, 128, false>(p, st);
+    const auto of = [&](auto stats) -> int {
+      constexpr bool kStats = decltype(stats)::value;
+      if (p.head_dim == 64) return quant ? launch<T, 64, true, kStats>(p, st) : launch<T, 64, false, kStats>(p, st);
+      return quant ? launch<T, 128, true, kStats>(p, st) : launch<T, 128, false, kStats>(p, st);
+    };
+    return p.stats != nullptr ? of(std::true_type()) : of(std::false_type());
   };
   return dtype == SNAPMIND_DTYPE_BF16 ? go(__nv_bfloat16()) : go(__half());
 }

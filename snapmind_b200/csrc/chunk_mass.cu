@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kThreads, MassSmem<D4>::kCtas) mass_generic_ke
   using Smem = MassSmem<D4>;
   constexpr int P = Smem::P, D = Smem::D;
   constexpr bool kQuant = std::is_same<KV, uint8_t>::value;
-  const ChunkParams& p = mp.c;
+  const WeighedParams& p = mp.c;
   Smem& S = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   next_grid_may_launch();
@@ -213,7 +213,7 @@ int launch_generic(MassParams& mp, cudaStream_t st) {
 // together for itself (one sequence of 32768: 48 us, 43 without).
 constexpr int kScoreThreads = 512;
 template <int G>
-__global__ void __launch_bounds__(kScoreThreads, 2) mass_scores_kernel(const __grid_constant__ ChunkParams p, float* mass) {
+__global__ void __launch_bounds__(kScoreThreads, 2) mass_scores_kernel(const __grid_constant__ WeighedParams p, float* mass) {
   extern __shared__ int32_t tiles[];
   __shared__ PlanShared plan;
   next_grid_may_launch();
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) mass_scores_kernel(const __g
   }
 }
 
-int launch_scores(const ChunkParams& p, float* mass, cudaStream_t st) {
+int launch_scores(const WeighedParams& p, float* mass, cudaStream_t st) {
   const auto go = [&](auto kernel) {
     return cuda_status(launch_dependent(kernel, dim3(p.n_ctas), kScoreThreads, (size_t)p.batch * 4, st, p, mass), "paged_chunk mass launch");
   };
@@ -295,7 +295,7 @@ int launch_mass_merge(const MassParams& mp, cudaStream_t st) {
 }
 
 // After the attention kernels on the stream, which left p.stats.
-int launch_mass(const ChunkParams& p, int dtype, int pool_dtype, int32_t flags, float* mass, void* workspace, cudaStream_t st) {
+int launch_mass(const WeighedParams& p, int dtype, int pool_dtype, int32_t flags, float* mass, void* workspace, cudaStream_t st) {
   if (p.scores != nullptr) return launch_scores(p, mass, st);
   MassParams mp = {};
   mp.c = p;

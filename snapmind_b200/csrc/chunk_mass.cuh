@@ -3,7 +3,7 @@
 //
 //   mass[key] += sum over the call's rows i that see it of 2^(score(i, key) + x_i)
 //
-// with x_i = -log2 of the row's sum, as the attention kernels left it (ChunkParams::stats).  A weight is
+// with x_i = -log2 of the row's sum, as the attention kernels left it (WeighedParams::stats).  A weight is
 // known only when its row's whole softmax is, so it takes a second pass over the scores, but not over V.
 //
 // The roles of chunk_plan.cuh are turned round: a unit is one (sequence, kv head, tile of key_tile keys),
@@ -18,7 +18,7 @@
 namespace snapmind {
 
 struct MassParams {
-  ChunkParams c;      // gw, n_slices, tokens, rows, key_tile, n_ctas: this kernel's own
+  WeighedParams c;    // gw, n_slices, tokens, rows, key_tile, n_ctas: this kernel's own
   FastDiv by_tokens;  // by c.tokens
   float* mass;        // [block][kv head][slot] of the layer
   int32_t* info;      // workspace: [n_ctas][kMassInts]
@@ -204,7 +204,7 @@ __device__ __forceinline__ int64_t mass_row(const ChunkParams& p, const KeyRange
 }
 
 // x_i of row (token, head g of the kv head's group).
-__device__ __forceinline__ const float* row_stats(const ChunkParams& p, int kvh, int64_t token, int g) {
+__device__ __forceinline__ const float* row_stats(const WeighedParams& p, int kvh, int64_t token, int g) {
   return p.stats + (kvh * (int64_t)p.total_q + token) * p.group + g;
 }
 
@@ -227,7 +227,7 @@ inline int mass_geometry(MassParams& mp, int rows, int key_tile, int n_ctas) {
 // chunk_mass.cu: the merge of cut units, behind a kernel of this plan; the whole pass behind the attention kernels
 // of a call, in a workspace of mass_workspace_bytes().
 int launch_mass_merge(const MassParams& mp, cudaStream_t st);
-int launch_mass(const ChunkParams& p, int dtype, int pool_dtype, int32_t flags, float* mass, void* workspace, cudaStream_t st);
+int launch_mass(const WeighedParams& p, int dtype, int pool_dtype, int32_t flags, float* mass, void* workspace, cudaStream_t st);
 int64_t mass_workspace_bytes();
 
 // chunk_mass_umma.cu: for the shapes of chunk_umma_supported.

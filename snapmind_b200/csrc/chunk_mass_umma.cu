@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(Roles<kQuant>::kThreads, 1)
   using Sh = Shape<D>;
   using Ro = Roles<kQuant>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  const ChunkParams& p = mp.c;
+  const WeighedParams& p = mp.c;
   Ctrl& C = *reinterpret_cast<Ctrl*>(base + Sh::kCtrl);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {

@@ -18,6 +18,8 @@
 // position(v) = v + (v >= v_sink ? shift : 0), so nothing between is read.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace snapmind {
@@ -51,11 +53,17 @@ struct ChunkParams {
   int32_t* odd;     // workspace: [n_odd] whether a CTA met rows that its kernel's types do not hold, or NULL
   int32_t n_odd;
   int32_t means;    // part_o holds a piece's weighted means of V (else its weighted sums)
-  float* scores;    // [score row][group] scores (log2 units) that a decode leaves for chunk_mass.cu, or NULL
-  int32_t scores_room;  // score row of a key: (sequence * kv heads + kv head) * scores_room + its place on the virtual axis; 0: its pool row
-  float* stats;     // [n_kv_heads][total_q][group] -log2 of every row's softmax sum (of 2^score), or NULL
   int32_t* err;
 };
+
+// A call, with what the attention leaves for the pass that adds its weights up (chunk_mass.cu).  The kernels of other calls take
+// ChunkParams alone: 24 bytes more of parameters made the two launches of a call 0.6 us slower on the host.
+struct WeighedParams : ChunkParams {
+  float* stats;         // [n_kv_heads][total_q][group] -log2 of every row's softmax sum (of 2^score), or NULL: no weights
+  float* scores;        // [score row][group] scores (log2 units) that a decode leaves, or NULL
+  int32_t scores_room;  // score row of a key: (sequence * kv heads + kv head) * scores_room + its place on the virtual axis; 0: its pool row
+};
+template <bool kStats> using CallParams = typename std::conditional<kStats, WeighedParams, ChunkParams>::type;
 
 constexpr int kPieceInts = 8;   // b, kv head, slice, first token, first and last piece's CTA, first query row, new tokens
 constexpr int kMaxChunkBatch = 8192;
@@ -437,7 +445,7 @@ __device__ inline void write_piece_info(const ChunkParams& p, const PlanShared& 
 
 // A finished row's softmax (M, sum of 2^(score - M)), for the kernels that add its weights to their keys (chunk_mass.cu):
 // the weight of a key is 2^(score + x).  A row that sees nothing: -infinity.
-__device__ __forceinline__ void write_stats(const ChunkParams& p, int64_t row, int head, float M, float L) {
+__device__ __forceinline__ void write_stats(const WeighedParams& p, int64_t row, int head, float M, float L) {
   const int kvh = head / p.group;
   p.stats[(kvh * (int64_t)p.total_q + row) * p.group + (head - kvh * p.group)] = L == 0.f ? -INFINITY : -((M == -INFINITY ? 0.f : M) + log2f(L));
 }
@@ -458,14 +466,14 @@ __device__ __forceinline__ bool any_odd(const ChunkParams& p) {
 }
 
 // chunk_attn.cu: merges the cut units, after the attention kernel on the stream.
-int launch_chunk_merge(const ChunkParams& p, int dtype, cudaStream_t st);
+int launch_chunk_merge(const WeighedParams& p, int dtype, cudaStream_t st);
 
 // chunk_attn_umma.cu (tcgen05) and decode_sinks.cu (one token per sequence): whether the
 // shapes fit, the unit geometry and CTA count they want, and the launch.
 bool chunk_umma_supported(const ChunkParams& p, int dtype, int pool_dtype);
-int launch_chunk_umma(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st);
+int launch_chunk_umma(WeighedParams& p, int dtype, int pool_dtype, cudaStream_t st);
 bool decode_sinks_supported(const ChunkParams& p, int dtype, int pool_dtype);
-int launch_decode_sinks(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st);
+int launch_decode_sinks(WeighedParams& p, int dtype, int pool_dtype, cudaStream_t st);
 // Whether a call of such shapes may run on the decode kernel, which then leaves its scores (where there is room for them).
 inline bool decode_keeps_scores(int head_dim, int group) { return head_dim == 128 && group <= 8; }
 

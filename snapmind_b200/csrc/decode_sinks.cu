@@ -116,7 +116,7 @@ __device__ __forceinline__ bool consumers_any(bool v) {
 // the pass that adds their weights up (128 sequences of 1 to 8 thousand tokens: 3% more bytes than the decode without).
 template <typename T, bool kQuant, bool kScores>
 __global__ void __launch_bounds__(kThreads, 2)
-    decode_sinks_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, ChunkParams p) {
+    decode_sinks_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, CallParams<kScores> p) {
   extern __shared__ uint8_t smem_raw[];
   using St = Stage<kQuant>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -331,18 +331,20 @@ __global__ void __launch_bounds__(kThreads, 2)
               mma16816<kMmaBf16>(sc, a, qf[k][0], qf[k][1]);
             }
           }
-          if (kScores && p.scores != nullptr) {
-            // a key's scores side by side: 16 bytes for four heads (rows past the last token, unseen ones: never read)
-            const int64_t row = S.rows[st][part] + 16 * warp - part * p.block_size;
+          if constexpr (kScores) {
+            if (p.scores != nullptr) {
+              // a key's scores side by side: 16 bytes for four heads (rows past the last token, unseen ones: never read)
+              const int64_t row = S.rows[st][part] + 16 * warp - part * p.block_size;
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-              float* to = p.scores + (row + g + 4 * i) * heads + 2 * tig;
-              const float a = sc[i] * q0, b = sc[i + 1] * q1;
-              if (heads % 2 == 0) {
-                if (2 * tig < heads) *reinterpret_cast<float2*>(to) = make_float2(a, b);
-              } else {
-                if (2 * tig < heads) to[0] = a;
-                if (2 * tig + 1 < heads) to[1] = b;
+              for (int i = 0; i < 4; i += 2) {
+                float* to = p.scores + (row + g + 4 * i) * heads + 2 * tig;
+                const float a = sc[i] * q0, b = sc[i + 1] * q1;
+                if (heads % 2 == 0) {
+                  if (2 * tig < heads) *reinterpret_cast<float2*>(to) = make_float2(a, b);
+                } else {
+                  if (2 * tig < heads) to[0] = a;
+                  if (2 * tig + 1 < heads) to[1] = b;
+                }
               }
             }
           }
@@ -527,7 +529,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * half * half;
         }
         if (c.whole()) {
-          if (kScores && d == 0) write_stats(p, c.q_first, head0 + h, M, L);
+          if constexpr (kScores)
+            if (d == 0) write_stats(p, c.q_first, head0 + h, M, L);
           if constexpr (!kQuant)
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] *= inv;
@@ -559,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 template <typename T, bool kQuant, bool kScores>
-int launch(const ChunkParams& p, cudaStream_t st) {
+int launch(const WeighedParams& p, cudaStream_t st) {
   CUtensorMap k_map, v_map;
   const uint64_t rows = (uint64_t)p.num_blocks * p.n_kv_heads * p.block_size;
   const uint32_t box = p.block_size < kTile ? p.block_size : kTile;
@@ -597,7 +600,7 @@ bool decode_sinks_supported(const ChunkParams& p, int dtype, int pool_dtype) {
   return encode_tiled() != nullptr;
 }
 
-int launch_decode_sinks(ChunkParams& p, int dtype, int pool_dtype, cudaStream_t st) {
+int launch_decode_sinks(WeighedParams& p, int dtype, int pool_dtype, cudaStream_t st) {
   const int rc = plan_geometry(p, kHeads, kHeads, kTile, 2 * num_sms());
   if (rc != SNAPMIND_OK) return rc;
   p.tokens = 1;
